@@ -163,6 +163,68 @@ int h24_int8_quantize(const float *w, int64_t rows, int64_t cols, int8_t *q, uin
 int h24_int8_dequant(const int8_t *q, const uint16_t *mu16, int64_t rows, int64_t cols,
                      uint16_t *out16, void *stream);
 
+/* ---- the INT8 head path: norm, product, sampling ---------------------------
+ * From a model's last hidden state to its next token without materialising
+ * the INT8 head (PackedInt8Linear, pollux.py:535-558; the sampling settings of
+ * generate.py:143-329).  No counterpart in the reference's code, which
+ * materialises the head and calls torch. */
+
+/* Activations in 8 bits: residual addition, RMS norm and per-row INT8, in one
+ * pass.  s = x + residual in fp32, v = s * gain, i = 1/sqrt(mean(s^2) + eps),
+ * mu = max(max|v| * i, 1e-8), q = clamp(rint(v * i / mu * 127), -128, 127),
+ * scale = mu / 127 (fp32): q * scale is the normed row.  residual_out (may be
+ * NULL) receives s rounded to x's type; the norm is taken of the unrounded s.
+ * x, residual (may be NULL) and residual_out have element type `dtype`
+ * (H24_DTYPE_*); row r of x starts at r * x_stride elements, of residual at
+ * r * residual_stride; q, scale and residual_out are contiguous.  gain: cols
+ * elements of `dtype` or of H24_DTYPE_F32 (gain_dtype).  residual_out may be
+ * x or residual itself where that is contiguous.  A NaN in a row makes its
+ * scale NaN and every q 0. */
+int h24_add_rms_norm_int8(const void *x, const void *residual, const void *gain, int gain_dtype,
+                          int64_t rows, int64_t cols, int64_t x_stride, int64_t residual_stride,
+                          int dtype, float eps, int8_t *q, float *scale, void *residual_out,
+                          void *stream);
+
+/* The quantisation alone: mu = max(max|x|, 1e-8), q and scale as above. */
+int h24_rows_int8_quantize(const void *x, int64_t rows, int64_t cols, int64_t x_stride, int dtype,
+                           int8_t *q, float *scale, void *stream);
+
+/* out = q * scale[row], rounded to `dtype`; all contiguous. */
+int h24_rows_int8_dequant(const int8_t *q, const float *scale, int64_t rows, int64_t cols, int dtype,
+                          void *out, void *stream);
+
+/* y[t][o] = (sum_k q[t][k] * w[o][k]) * scale[t] * fp16(mu16[o] / 127) + bias[o]
+ * for tokens t and out_features o: the product of quantised rows with an INT8
+ * layer (w and mu16 as h24_int8_quantize writes them, the weight scale as
+ * h24_int8_dequant reads it).  The sum is exact in int32, the scaling fp32, y
+ * (contiguous, element type out_dtype) rounded once.  Row t of q starts at
+ * t * q_stride bytes; bias: out_features fp32 or NULL.  in_features is at
+ * most 131,000 (the sum cannot overflow). */
+int h24_int8_linear(const int8_t *q, const float *scale, int64_t tokens, int64_t q_stride,
+                    const int8_t *w, const uint16_t *mu16, int64_t out_features, int64_t in_features,
+                    const float *bias, int out_dtype, void *y, void *stream);
+
+/* One token a row of logits (`rows` x `vocab`, element type `dtype`, row r at
+ * r * stride elements) from the uniform number u[r] in [0, 1).
+ *   z_i = (l_i - max l) * fp32(1 / T), w_i = rint(exp(z_i) * 2^40) (64 bits);
+ *   in the order of z descending, ties by index: the first top_k (0 or less:
+ *   all); of these, those whose mass before them is below ceil(top_p * their
+ *   mass) (at least the first; top_p >= 1: all); of these, w_i >=
+ *   ceil(min_p * 2^40);
+ *   tokens[r] = the first index at which the running mass of what is left, in
+ *   the order of the indices, exceeds floor(u * mass).
+ * Every sum is exact, so the token does not depend on how the work is split.
+ * T <= 0 (or NaN) takes the largest logit, lowest index.  A NaN logit is never
+ * chosen; a row without a logit above -inf gives -1.  logprobs (may be NULL)
+ * receives z - log(sum of all w / 2^40) of the token: its log-probability
+ * under the temperature before the three cuts.  Each setting is an array of
+ * one value a row, or NULL and the scalar beside it.  vocab is at most 2^22. */
+int h24_sample_tokens(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t stride,
+                      const float *u, const float *temperature, float temperature_all,
+                      const int32_t *top_k, int32_t top_k_all, const float *top_p, float top_p_all,
+                      const float *min_p, float min_p_all, int64_t *tokens, float *logprobs,
+                      void *stream);
+
 /* ---- nearest codeword (castor._leech_nn_kernel / castor_quantize_leech,
  *      castor.py:386-560; pack._quantize_h24_layer search, pack.py:166-177) --
  * x: n atoms of 24 fp32 values (16-byte aligned), out_idx: n int32 indices.

@@ -29,6 +29,7 @@ KERNEL_SCREEN, KERNEL_RESCORE, KERNEL_PREP = 0, 1, 2
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I = ctypes.c_int
+_F = ctypes.c_float
 SIGNATURES = {
     "h24_last_error": (ctypes.c_char_p, []),
     "h24_version": (ctypes.c_char_p, []),
@@ -46,6 +47,11 @@ SIGNATURES = {
     "h24_project_layers": (_I, [_P, _I, _P]),
     "h24_int8_quantize": (_I, [_P, _I64, _I64, _P, _P, _P]),
     "h24_int8_dequant": (_I, [_P, _P, _I64, _I64, _P, _P]),
+    "h24_add_rms_norm_int8": (_I, [_P, _P, _P, _I, _I64, _I64, _I64, _I64, _I, _F, _P, _P, _P, _P]),
+    "h24_rows_int8_quantize": (_I, [_P, _I64, _I64, _I64, _I, _P, _P, _P]),
+    "h24_rows_int8_dequant": (_I, [_P, _P, _I64, _I64, _I, _P, _P]),
+    "h24_int8_linear": (_I, [_P, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _I, _P, _P]),
+    "h24_sample_tokens": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _F, _P, _I, _P, _F, _P, _F, _P, _P, _P]),
     "h24_quantize": (_I, [_P, _I64, _I, _P, _P]),
     "h24_quantize_layer": (_I, [_P, _I64, _I64, _P, _P, _P]),
     "h24_quantize_layer_host": (_I, [_P, _I64, _I64, _P, _P, _P]),
@@ -102,6 +108,8 @@ _lock = threading.Lock()
 def load() -> ctypes.CDLL:
     """Load libh24.so (raises if it has not been built)."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not os.path.exists(LIB_PATH):

@@ -71,6 +71,9 @@ def _stream(dev: torch.device) -> int:
 def _call(dev: torch.device, name: str, *args) -> None:
     """Call libh24 with ``dev``'s context current (the library runs on the
     current device and the caller's current torch stream)."""
+    if dev.index == torch.cuda.current_device():  # entering the device's context costs microseconds
+        N.call(name, *args)
+        return
     with torch.cuda.device(dev):
         N.call(name, *args)
 

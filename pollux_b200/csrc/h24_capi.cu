@@ -510,6 +510,77 @@ int h24_int8_dequant(const int8_t *q, const uint16_t *mu16, int64_t rows, int64_
   return launch_int8_dequant(q, mu16, rows, cols, out16, as_stream(stream));
 }
 
+static bool known_dtype(int dtype) {
+  return dtype == H24_DTYPE_F32 || dtype == H24_DTYPE_F16 || dtype == H24_DTYPE_BF16;
+}
+
+int h24_add_rms_norm_int8(const void *x, const void *residual, const void *gain, int gain_dtype, int64_t rows,
+                          int64_t cols, int64_t x_stride, int64_t residual_stride, int dtype, float eps, int8_t *q,
+                          float *scale, void *residual_out, void *stream) {
+  if (rows < 0 || cols < 0) return fail(H24_ERR_INVALID, "add_rms_norm_int8: negative size");
+  if (!known_dtype(dtype)) return fail(H24_ERR_INVALID, "add_rms_norm_int8: unknown dtype");
+  if (gain_dtype != dtype && gain_dtype != H24_DTYPE_F32)
+    return fail(H24_ERR_INVALID, "add_rms_norm_int8: gain must have x's dtype or fp32");
+  if (!(eps >= 0.f)) return fail(H24_ERR_INVALID, "add_rms_norm_int8: eps must not be negative");
+  if (rows == 0 || cols == 0) return H24_OK;
+  if (!x || !gain || !q || !scale) return fail(H24_ERR_INVALID, "add_rms_norm_int8: null pointer");
+  if (x_stride < 0 || (residual && residual_stride < 0))
+    return fail(H24_ERR_INVALID, "add_rms_norm_int8: negative stride");
+  return launch_rows_int8(x, residual, gain, gain_dtype, rows, cols, x_stride, residual_stride, dtype, eps, q, scale,
+                          residual_out, as_stream(stream));
+}
+
+int h24_rows_int8_quantize(const void *x, int64_t rows, int64_t cols, int64_t x_stride, int dtype, int8_t *q,
+                           float *scale, void *stream) {
+  if (rows < 0 || cols < 0) return fail(H24_ERR_INVALID, "rows_int8_quantize: negative size");
+  if (!known_dtype(dtype)) return fail(H24_ERR_INVALID, "rows_int8_quantize: unknown dtype");
+  if (rows == 0 || cols == 0) return H24_OK;
+  if (!x || !q || !scale) return fail(H24_ERR_INVALID, "rows_int8_quantize: null pointer");
+  if (x_stride < 0) return fail(H24_ERR_INVALID, "rows_int8_quantize: negative stride");
+  return launch_rows_int8(x, nullptr, nullptr, dtype, rows, cols, x_stride, 0, dtype, 0.f, q, scale, nullptr,
+                          as_stream(stream));
+}
+
+int h24_rows_int8_dequant(const int8_t *q, const float *scale, int64_t rows, int64_t cols, int dtype, void *out,
+                          void *stream) {
+  if (rows < 0 || cols < 0) return fail(H24_ERR_INVALID, "rows_int8_dequant: negative size");
+  if (!known_dtype(dtype)) return fail(H24_ERR_INVALID, "rows_int8_dequant: unknown dtype");
+  if (rows == 0 || cols == 0) return H24_OK;
+  if (!q || !scale || !out) return fail(H24_ERR_INVALID, "rows_int8_dequant: null pointer");
+  return launch_rows_dequant(q, scale, rows, cols, dtype, out, as_stream(stream));
+}
+
+int h24_int8_linear(const int8_t *q, const float *scale, int64_t tokens, int64_t q_stride, const int8_t *w,
+                    const uint16_t *mu16, int64_t out_features, int64_t in_features, const float *bias,
+                    int out_dtype, void *y, void *stream) {
+  if (tokens < 0 || out_features < 0 || in_features < 0) return fail(H24_ERR_INVALID, "int8_linear: negative size");
+  // 131,000 * 128 * 128 < 2^31: the int32 sum cannot overflow.
+  if (in_features > 131000) return fail(H24_ERR_INVALID, "int8_linear: in_features above 131000");
+  if (out_features > INT32_MAX || tokens > INT32_MAX) return fail(H24_ERR_INVALID, "int8_linear: size above 2^31 - 1");
+  if (!known_dtype(out_dtype)) return fail(H24_ERR_INVALID, "int8_linear: unknown dtype");
+  if (q_stride < 0) return fail(H24_ERR_INVALID, "int8_linear: negative stride");
+  if (tokens == 0 || out_features == 0) return H24_OK;
+  if (!scale || !mu16 || !y || (in_features > 0 && (!q || !w)))
+    return fail(H24_ERR_INVALID, "int8_linear: null pointer");
+  H24_TABLES_OR_FAIL(T);
+  return launch_int8_linear(T, q, scale, tokens, q_stride, w, mu16, out_features, in_features, bias, out_dtype, y,
+                            as_stream(stream));
+}
+
+int h24_sample_tokens(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t stride, const float *u,
+                      const float *temperature, float temperature_all, const int32_t *top_k, int32_t top_k_all,
+                      const float *top_p, float top_p_all, const float *min_p, float min_p_all, int64_t *tokens,
+                      float *logprobs, void *stream) {
+  if (rows < 0 || vocab < 0 || stride < 0) return fail(H24_ERR_INVALID, "sample_tokens: negative size");
+  if (!known_dtype(dtype)) return fail(H24_ERR_INVALID, "sample_tokens: unknown dtype");
+  if (vocab > (1 << 22)) return fail(H24_ERR_INVALID, "sample_tokens: vocab above 2^22");
+  if (rows == 0) return H24_OK;
+  if (vocab == 0) return fail(H24_ERR_INVALID, "sample_tokens: empty vocabulary");
+  if (!logits || !u || !tokens) return fail(H24_ERR_INVALID, "sample_tokens: null pointer");
+  return launch_sample(logits, dtype, rows, vocab, stride, u, temperature, temperature_all, top_k, top_k_all, top_p,
+                       top_p_all, min_p, min_p_all, tokens, logprobs, as_stream(stream));
+}
+
 int h24_quantize(const float *x, int64_t n, int rule, int32_t *out_idx, void *stream) {
   H24_TABLES_OR_FAIL(T);
   if (n < 0) return fail(H24_ERR_INVALID, "quantize: negative atom count");

@@ -202,6 +202,19 @@ int launch_int8_quantize(const float *w, int64_t rows, int64_t cols, int8_t *q, 
                          cudaStream_t s);
 int launch_int8_dequant(const int8_t *q, const uint16_t *mu16, int64_t rows, int64_t cols,
                         uint16_t *out, cudaStream_t s);
+// Activations in 8 bits (h24_int8_rows.cu).  gain null: quantisation alone.
+int launch_rows_int8(const void *x, const void *residual, const void *gain, int gain_dtype, int64_t rows,
+                     int64_t cols, int64_t x_stride, int64_t residual_stride, int dtype, float eps, int8_t *q,
+                     float *scale, void *residual_out, cudaStream_t s);
+int launch_rows_dequant(const int8_t *q, const float *scale, int64_t rows, int64_t cols, int dtype, void *out,
+                        cudaStream_t s);
+int launch_int8_linear(const Tables *t, const int8_t *q, const float *scale, int64_t tokens, int64_t q_stride,
+                       const int8_t *w, const uint16_t *mu16, int64_t out, int64_t in, const float *bias,
+                       int out_dtype, void *y, cudaStream_t s);
+int launch_sample(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t stride, const float *u,
+                  const float *temperature, float temperature1, const int32_t *top_k, int32_t top_k1,
+                  const float *top_p, float top_p1, const float *min_p, float min_p1, int64_t *tokens,
+                  float *logprobs, cudaStream_t s);
 // Row scales of `rows` rows of n elements at w (fp32 or bf16), which are rows
 // first_row.. of a 16-byte aligned matrix of matrix_rows rows, in the
 // reference's arithmetic (h24_rowrms.cu): sigma32 = sqrt(mean(w^2) + 1e-8),

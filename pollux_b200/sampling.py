@@ -1,0 +1,78 @@
+"""Token sampling on libh24: temperature, top-k, top-p and min-p (the settings
+of generate.py:143-329, with min-p) from given uniform numbers.
+
+Probabilities are 64-bit fixed-point weights, so every sum is exact and a row's
+token depends only on its logits, its settings and its number -- not on the
+batch it is in or on how the GPU splits the row.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _native as N
+from .castor import _call, _stream, _work_device
+from .int8 import _code, _rows
+
+MAX_VOCAB = 1 << 22
+
+
+def _setting(v, rows: int, dtype: torch.dtype, dev: torch.device, name: str):
+    """(tensor kept alive, pointer or None, scalar) of one sampling setting."""
+    if not isinstance(v, torch.Tensor):
+        return None, None, v
+    if v.numel() != rows:
+        raise ValueError(f"{name} must be a number or hold one value for each of the {rows} rows, got {tuple(v.shape)}")
+    if v.device != dev or v.dtype != dtype:
+        v = v.to(device=dev, dtype=dtype)
+    v = v.reshape(-1).contiguous()
+    return v, v.data_ptr(), 0
+
+
+def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: float | torch.Tensor = 1.0,
+                  top_k: int | torch.Tensor = 0, top_p: float | torch.Tensor = 1.0,
+                  min_p: float | torch.Tensor = 0.0, return_logprob: bool = False):
+    """One token for each row of ``logits`` [..., vocab] from uniform numbers
+    ``u`` [...] in [0, 1).
+
+    Tokens are ordered by scaled logit, ties by index.  Kept are the first
+    ``top_k`` (0: all); of these the shortest run from the top that reaches
+    ``top_p`` of their mass (1: all); of these the ones with at least ``min_p``
+    of the most probable token's probability.  The token is where the running
+    mass of what is kept, in the order of the vocabulary, passes ``u`` of it.
+    ``temperature`` 0 takes the largest logit.  Each setting is a number or a
+    tensor with one value a row.
+
+    NaN logits are never chosen; a row with no logit above -inf gives -1.
+    Returns int64 tokens of the leading shape, with ``return_logprob`` also the
+    fp32 log-probabilities of the tokens at that temperature before the cuts
+    (-inf for a row that gives -1)."""
+    if logits.dim() < 1:
+        raise ValueError("logits must have at least one dimension")
+    code = _code(logits.dtype, "logits")
+    lead, vocab = logits.shape[:-1], logits.shape[-1]
+    if not 0 < vocab <= MAX_VOCAB:
+        raise ValueError(f"the vocabulary must hold 1 to {MAX_VOCAB} tokens, got {vocab}")
+    for name, v, ok in (("temperature", temperature, lambda v: v >= 0), ("top_k", top_k, lambda v: v >= 0),
+                        ("top_p", top_p, lambda v: 0 <= v <= 1), ("min_p", min_p, lambda v: 0 <= v <= 1)):
+        if not isinstance(v, torch.Tensor) and not ok(v):
+            raise ValueError(f"{name} out of range: {v}")
+    dev = _work_device(logits)
+    rows = logits.numel() // vocab
+    if u.numel() != rows:
+        raise ValueError(f"u must hold one number for each of the {rows} rows, got {tuple(u.shape)}")
+    tokens = torch.empty(lead, dtype=torch.int64, device=dev)
+    logprob = torch.empty(lead, dtype=torch.float32, device=dev) if return_logprob else None
+    if rows:
+        lr = _rows(logits, dev)
+        us, up, _ = _setting(u, rows, torch.float32, dev, "u")
+        ts, tp, t1 = _setting(temperature, rows, torch.float32, dev, "temperature")
+        ks, kp, k1 = _setting(top_k, rows, torch.int32, dev, "top_k")
+        ps, pp, p1 = _setting(top_p, rows, torch.float32, dev, "top_p")
+        ms, mp, m1 = _setting(min_p, rows, torch.float32, dev, "min_p")
+        _call(dev, "h24_sample_tokens", lr.data_ptr(), code, rows, vocab, lr.stride(0), up, tp, t1, kp,
+              min(int(k1), vocab), pp, p1, mp, m1, tokens.data_ptr(),
+              None if logprob is None else logprob.data_ptr(), _stream(dev))
+    if logits.device != dev:
+        tokens = tokens.to(logits.device)
+        logprob = None if logprob is None else logprob.to(logits.device)
+    return (tokens, logprob) if return_logprob else tokens
