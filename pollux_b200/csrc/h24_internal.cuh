@@ -125,6 +125,9 @@ int cuda_fail(cudaError_t e, const char *what);
     if (_e != cudaSuccess) return ::h24::cuda_fail(_e, #expr); \
   } while (0)
 
+#ifdef __CUDACC__
+__host__ __device__
+#endif
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Programmatic dependent launch.  A kernel launched by launch_pdl calls

@@ -14,6 +14,15 @@
 // largest probability is the smallest weight kept; with at most 2^22 tokens a
 // row's mass stays below 2^62.
 //
+// sample_cluster_kernel reads a row once.  A cluster of 1 to 8 CTAs holds it in
+// shared memory, a slice each; a histogram of |z| in 2,048 steps of 1/72 (below
+// |z| = 28.4 a weight rounds to 0) gives for each step a count and, where top-p
+// asks, a mass; the CTAs add the histograms through distributed shared memory,
+// a share of the steps each, and the step in which a cut falls is known.  Are
+// there at most 1,024 tokens up to it, they go to the first CTA, which sorts
+// them and finishes; else the tokens of that one step settle the cut and the
+// CTAs add and walk what is kept, in place.
+//
 // "z descending, index ascending" is one 64-bit key: |z|'s bits above the
 // index (z <= 0, so |z| ascending is z descending, and the bits of
 // non-negative floats ascend with them).  A selection is then a cut on that
@@ -22,6 +31,8 @@
 
 namespace h24 {
 namespace {
+
+using u64 = unsigned long long;
 
 constexpr float kOne = 1099511627776.0f;  // 2^40
 constexpr int kSampleThreads = 1024;
@@ -54,46 +65,51 @@ __device__ __forceinline__ float logit_at(const void *row, int64_t i) {
 
 // |z| of a logit.
 __device__ __forceinline__ float dist(float l, float m, float inv_t) {
-  return l == m ? 0.f : fabsf(__fmul_rn(__fsub_rn(l, m), inv_t));
+  const float d = fabsf(__fmul_rn(__fsub_rn(l, m), inv_t));
+  return l == m ? 0.f : (d == d ? d : INFINITY);  // NaN: a masked logit at an infinite temperature
 }
 
-__device__ __forceinline__ unsigned long long weight(float d) {
-  return static_cast<unsigned long long>(__float2ll_rn(expf(-d) * kOne));
+__device__ __forceinline__ u64 weight(float d) {
+  return static_cast<u64>(__float2ll_rn(expf(-d) * kOne));
 }
 
-__device__ __forceinline__ unsigned long long order_key(float d, int64_t i) {
-  return (static_cast<unsigned long long>(__float_as_uint(d)) << 32) | static_cast<unsigned long long>(i);
+constexpr int kIndexBits = 22;
+__device__ __forceinline__ u64 order_key(float d, int64_t i) {
+  return (static_cast<u64>(__float_as_uint(d)) << kIndexBits) | static_cast<u64>(i);
 }
+__device__ __forceinline__ float key_dist(u64 key) { return __uint_as_float(static_cast<uint32_t>(key >> kIndexBits)); }
+__device__ __forceinline__ uint32_t key_index(u64 key) { return static_cast<uint32_t>(key) & ((1u << kIndexBits) - 1); }
 
 // What step 2 and 3 ask for, in the arithmetic the header states.
-__device__ __forceinline__ unsigned long long mass_limit(float p, unsigned long long mk) {
+__device__ __forceinline__ u64 mass_limit(float p, u64 mk) {
   const double x = ceil(static_cast<double>(p) * static_cast<double>(mk));
-  return x > 1.0 ? static_cast<unsigned long long>(x) : 1ull;
+  return x > 1.0 ? static_cast<u64>(x) : 1ull;
 }
-__device__ __forceinline__ unsigned long long weight_floor(float min_p) {
+__device__ __forceinline__ u64 weight_floor(float min_p) {
   const double x = ceil(fmin(fmax(static_cast<double>(min_p), 0.0), 1.0) * static_cast<double>(kOne));
-  return x > 1.0 ? static_cast<unsigned long long>(x) : 1ull;  // weight 0 is never chosen
+  return x > 1.0 ? static_cast<u64>(x) : 1ull;  // weight 0 is never chosen
 }
-__device__ __forceinline__ unsigned long long draw_target(float u, unsigned long long mass) {
+__device__ __forceinline__ u64 draw_target(float u, u64 mass) {
   const double x = floor((u > 0.f ? static_cast<double>(u) : 0.0) * static_cast<double>(mass));
-  return x >= static_cast<double>(mass - 1) ? mass - 1 : static_cast<unsigned long long>(x);
+  return x >= static_cast<double>(mass - 1) ? mass - 1 : static_cast<u64>(x);
 }
 
-__device__ unsigned long long block_sum(unsigned long long v, unsigned long long *red) {
+__device__ u64 block_sum(u64 v, u64 *red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
-  unsigned long long r = 0;
+  u64 r = 0;
   for (int w = 0; w < kSampleThreads / 32; ++w) r += red[w];
   __syncthreads();
   return r;
 }
 
-// A block per row; every step reads the row again.
+// A block per row; every step reads the row again.  For vocabularies whose row
+// does not fit the shared memory of a cluster.
 template <int DT>
 __global__ void __launch_bounds__(kSampleThreads) sample_rows_kernel(const SampleArgs a) {
-  __shared__ unsigned long long hist[256], red[32], sh_digit, sh_left;
+  __shared__ u64 hist[256], red[32], sh_digit, sh_left;
   __shared__ float redf[32];
   const int t = threadIdx.x;
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
@@ -119,29 +135,29 @@ __global__ void __launch_bounds__(kSampleThreads) sample_rows_kernel(const Sampl
       }
       continue;
     }
-    unsigned long long sum = 0;
+    u64 sum = 0;
     for (int64_t i = t; i < a.vocab; i += kSampleThreads) sum += weight(dist(logit_at<DT>(row, i), m, inv_t));
-    const unsigned long long total = block_sum(sum, red);
+    const u64 total = block_sum(sum, red);
 
     // The key of the last element kept: the first at which the count (by_mass
     // false) or the mass of the order up to and with it reaches `want`, among
     // keys <= cut.
-    unsigned long long cut = ~0ull;
-    auto select = [&](bool by_mass, unsigned long long want) {
-      unsigned long long prefix = 0, left = want;
+    u64 cut = ~0ull;
+    auto select = [&](bool by_mass, u64 want) {
+      u64 prefix = 0, left = want;
       for (int shift = 56; shift >= 0; shift -= 8) {
         for (int i = t; i < 256; i += kSampleThreads) hist[i] = 0;
         __syncthreads();
         for (int64_t i = t; i < a.vocab; i += kSampleThreads) {
           const float d = dist(logit_at<DT>(row, i), m, inv_t);
-          const unsigned long long key = order_key(d, i);
+          const u64 key = order_key(d, i);
           if (key <= cut && (shift == 56 || (key >> (shift + 8)) == prefix))
             atomicAdd(&hist[(key >> shift) & 255], by_mass ? weight(d) : 1ull);
         }
         __syncthreads();
         if (t == 0) {
           int b = 0;
-          unsigned long long l = left;
+          u64 l = left;
           while (b < 255 && hist[b] < l) l -= hist[b++];
           sh_digit = b;
           sh_left = l;
@@ -153,9 +169,9 @@ __global__ void __launch_bounds__(kSampleThreads) sample_rows_kernel(const Sampl
       }
       cut = prefix;
     };
-    unsigned long long mk = total;
+    u64 mk = total;
     if (k > 0 && k < a.vocab) {
-      select(false, static_cast<unsigned long long>(k));
+      select(false, static_cast<u64>(k));
       sum = 0;
       for (int64_t i = t; i < a.vocab; i += kSampleThreads) {
         const float d = dist(logit_at<DT>(row, i), m, inv_t);
@@ -164,29 +180,29 @@ __global__ void __launch_bounds__(kSampleThreads) sample_rows_kernel(const Sampl
       mk = block_sum(sum, red);
     }
     if (p < 1.f) select(true, mass_limit(p, mk));
-    const unsigned long long least = weight_floor(min_p);
-    auto kept = [&](int64_t i) -> unsigned long long {
+    const u64 least = weight_floor(min_p);
+    auto kept = [&](int64_t i) -> u64 {
       const float d = dist(logit_at<DT>(row, i), m, inv_t);
-      const unsigned long long w = weight(d);
+      const u64 w = weight(d);
       return order_key(d, i) <= cut && w >= least ? w : 0ull;
     };
     sum = 0;
     for (int64_t i = t; i < a.vocab; i += kSampleThreads) sum += kept(i);
-    const unsigned long long target = draw_target(a.u[r], block_sum(sum, red));
+    const u64 target = draw_target(a.u[r], block_sum(sum, red));
     // The running mass, a block's width of indices at a time.
-    unsigned long long base = 0;
+    u64 base = 0;
     for (int64_t i0 = 0; i0 < a.vocab; i0 += kSampleThreads) {
       const int64_t i = i0 + t;
-      const unsigned long long w = i < a.vocab ? kept(i) : 0ull;
-      unsigned long long run = w;
+      const u64 w = i < a.vocab ? kept(i) : 0ull;
+      u64 run = w;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long up = __shfl_up_sync(0xffffffffu, run, o);
+        const u64 up = __shfl_up_sync(0xffffffffu, run, o);
         if ((t & 31) >= o) run += up;
       }
       if ((t & 31) == 31) red[t >> 5] = run;
       __syncthreads();
-      unsigned long long before = base, all = base;
+      u64 before = base, all = base;
       for (int j = 0; j < kSampleThreads / 32; ++j) {
         if (j < (t >> 5)) before += red[j];
         all += red[j];
@@ -206,6 +222,621 @@ __global__ void __launch_bounds__(kSampleThreads) sample_rows_kernel(const Sampl
   }
 }
 
+
+// ---------------------------------------------------------------------------
+// distributed shared memory of the cluster
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t su32(const void *p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ uint32_t peer(const void *p, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(su32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ uint32_t peer_ld(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void peer_st(uint32_t addr, u64 v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t peer_add(uint32_t addr, uint32_t v) {
+  uint32_t r;
+  asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(r) : "r"(addr), "r"(v) : "memory");
+  return r;
+}
+
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kBins = 2048;
+constexpr float kBinsPerNat = 72.0f;  // 2048 / 72 = 28.44: exp(-28.42) * 2^40 = 1/2
+constexpr int kList = 1024;
+constexpr int kMaxCluster = 8;
+
+struct Cut {  // where a cut falls: the step, what is before it and in it
+  u64 bin, count_before, mass_before, count, mass;
+};
+
+struct SampleShared {
+  uint32_t count[kBins], lo[kBins], hi[kBins];
+  u64 list[kList];
+  u64 slot[kMaxCluster];                          // one value of each CTA
+  u64 slice_count[kMaxCluster], slice_mass[kMaxCluster];
+  u64 total[kMaxCluster], first[kMaxCluster], kept[kMaxCluster];
+  Cut cut;
+  u64 scan_c[kWarps], scan_m[kWarps];
+  u64 red[kWarps];
+  u64 pick;
+  uint32_t list_n;
+};
+
+__device__ __forceinline__ void cluster_sync(int c) {
+  if (c == 1) {
+    __syncthreads();
+  } else {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+}
+
+__device__ __forceinline__ u64 warp_sum(u64 v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ u64 warp_scan(u64 v, int lane) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 up = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += up;
+  }
+  return v;
+}
+__device__ u64 sum_block(u64 v, u64 *red) {
+  v = warp_sum(v);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  u64 r = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) r += red[w];
+  __syncthreads();
+  return r;
+}
+
+// The elements of one 16-byte vector of a slice, NaN as -inf.
+template <int DT>
+struct Vec {
+  static constexpr int kN = DT == H24_DTYPE_F32 ? 4 : 8;
+  float v[kN];
+  __device__ __forceinline__ explicit Vec(uint4 raw) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (DT == H24_DTYPE_F32) {
+        v[i] = __uint_as_float(w[i]);
+      } else if (DT == H24_DTYPE_F16) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+      } else {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kN; ++i) v[i] = v[i] == v[i] ? v[i] : -INFINITY;
+  }
+};
+
+__device__ __forceinline__ int bin_of(float d) { return static_cast<int>(d * kBinsPerNat); }  // d below 28.44
+
+// Sorts the first n (a power of two) keys of the list, ascending.
+__device__ void sort_list(u64 *list, int n) {
+  for (int k = 2; k <= n; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      for (int i = threadIdx.x; i < n / 2; i += kThreads) {
+        const int a = ((i & ~(j - 1)) << 1) | (i & (j - 1)), b = a | j;
+        const u64 x = list[a], y = list[b];
+        if ((x > y) == ((a & k) == 0)) list[a] = y, list[b] = x;
+      }
+      __syncthreads();
+    }
+}
+
+struct RowSettings {
+  int64_t k;
+  float inv_t, p, u;
+  u64 least;
+};
+
+template <int DT>
+__global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleArgs a, int nc, int slice) {
+  using V = Vec<DT>;
+  constexpr int kVN = V::kN, kSize = DT == H24_DTYPE_F32 ? 4 : 2;
+  extern __shared__ __align__(16) uint8_t sample_raw[];
+  SampleShared &S = *reinterpret_cast<SampleShared *>(sample_raw);
+  uint4 *data = reinterpret_cast<uint4 *>(sample_raw + (sizeof(SampleShared) + 15) / 16 * 16);
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int rank = static_cast<int>(blockIdx.x) % nc;
+  const int64_t r = blockIdx.x / nc;
+  const int begin = rank * slice;
+  const int n = static_cast<int>(max(int64_t(0), min(static_cast<int64_t>(slice), a.vocab - begin)));
+  const int nvec = (n + kVN - 1) / kVN;
+
+  if (t == 0) S.list_n = 0;
+  for (int i = t; i < 3 * kBins / 4; i += kThreads) reinterpret_cast<uint4 *>(S.count)[i] = make_uint4(0, 0, 0, 0);
+  __syncwarp();
+  if (nc > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  pdl_enter();
+  RowSettings R;
+  {
+    float temp = a.temperature ? a.temperature[r] : a.temperature1;
+    R.k = a.top_k ? a.top_k[r] : a.top_k1;
+    R.p = a.top_p ? a.top_p[r] : a.top_p1;
+    R.least = weight_floor(a.min_p ? a.min_p[r] : a.min_p1);
+    R.u = a.u[r];
+    if (!(temp > 0.f)) temp = 1.f, R.k = 1;
+    if (R.k <= 0 || R.k > a.vocab) R.k = a.vocab;
+    R.inv_t = __fdiv_rn(1.0f, temp);
+  }
+
+  // ---- the slice into shared memory, and the row's largest logit ----
+  const uint8_t *src = static_cast<const uint8_t *>(a.logits) + (r * a.stride + begin) * kSize;
+  float mx = -INFINITY;
+  const int nfull = aligned16(src) ? n / kVN : 0;  // vectors that can be loaded whole
+  for (int i = t; i < nfull; i += kThreads) {
+    const uint4 raw = __ldcs(reinterpret_cast<const uint4 *>(src) + i);
+    data[i] = raw;
+    const V v(raw);
+#pragma unroll
+    for (int j = 0; j < kVN; ++j) mx = fmaxf(mx, v.v[j]);
+  }
+  {  // the rest by the element, padded with -inf to a whole vector
+    for (int i = nfull * kVN + t; i < nvec * kVN; i += kThreads) {
+      if (DT == H24_DTYPE_F32)
+        reinterpret_cast<float *>(data)[i] = i < n ? reinterpret_cast<const float *>(src)[i] : -INFINITY;
+      else
+        reinterpret_cast<uint16_t *>(data)[i] = i < n ? reinterpret_cast<const uint16_t *>(src)[i]
+                                                     : static_cast<uint16_t>(DT == H24_DTYPE_F16 ? 0xFC00 : 0xFF80);
+      if (i < n) mx = fmaxf(mx, logit_at<DT>(src, i));
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  if (lane == 0) S.red[warp] = __float_as_uint(mx);
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, __uint_as_float(static_cast<uint32_t>(S.red[w])));
+  if (nc > 1) {
+    // Every CTA of the cluster has started: its shared memory may be written.
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (t < nc) peer_st(peer(&S.slot[rank], t), __float_as_uint(mx));
+    cluster_sync(nc);
+    for (int c = 0; c < nc; ++c) mx = fmaxf(mx, __uint_as_float(static_cast<uint32_t>(S.slot[c])));
+  }
+  __syncthreads();  // S.red
+  const float m = mx;
+  if (m == -INFINITY) {  // nothing to choose from (the same for the whole cluster)
+    if (rank == 0 && t == 0) {
+      a.tokens[r] = -1;
+      if (a.logprobs) a.logprobs[r] = -INFINITY;
+    }
+    return;
+  }
+
+  // ---- total mass, first index of the maximum, histogram ----
+  const bool cut_k = R.k > 1 && R.k < a.vocab, cut_p = R.k > 1 && R.p < 1.f;
+  u64 sum = 0;
+  uint32_t first = 0xFFFFFFFFu;
+  for (int i = t; i < nvec; i += kThreads) {
+    const V v(data[i]);
+#pragma unroll
+    for (int j = 0; j < kVN; ++j) {
+      const float d = dist(v.v[j], m, R.inv_t);
+      const u64 w = weight(d);
+      if (w == 0) continue;
+      sum += w;
+      if (v.v[j] == m) first = min(first, static_cast<uint32_t>(begin + i * kVN + j));
+      if (cut_k || cut_p) {
+        const int b = bin_of(d);
+        atomicAdd(&S.count[b], 1u);
+        if (cut_p) {
+          const uint32_t wl = static_cast<uint32_t>(w), old = atomicAdd(&S.lo[b], wl);
+          const uint32_t wh = static_cast<uint32_t>(w >> 32) + (old + wl < old ? 1u : 0u);
+          if (wh) atomicAdd(&S.hi[b], wh);
+        }
+      }
+    }
+  }
+  sum = sum_block(sum, S.red);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+  if (lane == 0) S.red[warp] = first;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) first = min(first, static_cast<uint32_t>(S.red[w]));
+  if (t < nc) {
+    peer_st(peer(&S.total[rank], t), sum);
+    peer_st(peer(&S.first[rank], t), first);
+  }
+  cluster_sync(nc);
+  u64 total = 0;
+  for (int c = 0; c < nc; ++c) {
+    total += S.total[c];
+    first = min(first, static_cast<uint32_t>(S.first[c]));
+  }
+  auto answer = [&](uint32_t index, float d) {
+    a.tokens[r] = index;
+    if (a.logprobs)
+      a.logprobs[r] = -d - logf(static_cast<float>(static_cast<double>(total) / static_cast<double>(kOne)));
+  };
+  if (R.k == 1) {
+    if (rank == 0 && t == 0) answer(first, 0.f);
+    return;
+  }
+
+  // This CTA's share of the steps, added over the cluster: `per` steps a
+  // thread, with the count and mass before them (of the whole row).
+  const int share = kBins / nc, per = (share + kThreads - 1) / kThreads;
+  uint32_t bc[4];
+  u64 bm[4], pre_c = 0, pre_m = 0;
+  auto gather_bins = [&](bool masses) {
+    u64 c = 0, q = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      bc[j] = 0;
+      bm[j] = 0;
+      const int b = t * per + j;
+      if (j < per && b < share) {
+        for (int x = 0; x < nc; ++x) {
+          bc[j] += peer_ld(peer(&S.count[rank * share + b], x));
+          if (masses)
+            bm[j] += peer_ld(peer(&S.lo[rank * share + b], x)) +
+                     (static_cast<u64>(peer_ld(peer(&S.hi[rank * share + b], x))) << 32);
+        }
+      }
+      c += bc[j];
+      q += bm[j];
+    }
+    const u64 ic = warp_scan(c, lane), im = warp_scan(q, lane);
+    if (lane == 31) S.scan_c[warp] = ic, S.scan_m[warp] = im;
+    __syncthreads();
+    pre_c = ic - c;
+    pre_m = im - q;
+    u64 all_c = 0, all_m = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) pre_c += S.scan_c[w], pre_m += S.scan_m[w];
+      all_c += S.scan_c[w];
+      all_m += S.scan_m[w];
+    }
+    if (t < nc) {
+      peer_st(peer(&S.slice_count[rank], t), all_c);
+      peer_st(peer(&S.slice_mass[rank], t), all_m);
+    }
+    cluster_sync(nc);
+    for (int x = 0; x < rank; ++x) pre_c += S.slice_count[x], pre_m += S.slice_mass[x];
+  };
+  // The step at which the running count (or mass) reaches `want`, told to all.
+  auto find = [&](bool by_mass, u64 want) -> Cut {
+    u64 c = pre_c, q = pre_m;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const u64 before = by_mass ? q : c, in = by_mass ? bm[j] : bc[j];
+      if (before < want && want <= before + in) {
+        for (int x = 0; x < nc; ++x) {
+          const uint32_t to = peer(&S.cut, x);
+          peer_st(to, static_cast<u64>(rank * share + t * per + j));
+          peer_st(to + 8, c);
+          peer_st(to + 16, q);
+          peer_st(to + 24, bc[j]);
+          peer_st(to + 32, bm[j]);
+        }
+      }
+      c += bc[j];
+      q += bm[j];
+    }
+    cluster_sync(nc);
+    return S.cut;
+  };
+  // Keys that satisfy `wanted` go to the first CTA's list; their number (in
+  // the first CTA) is S.list_n.
+  auto collect = [&](auto wanted) {
+    const uint32_t counter = peer(&S.list_n, 0), list0 = peer(&S.list[0], 0);
+    for (int i0 = 0; i0 < nvec; i0 += kThreads) {
+      const int i = i0 + t;
+      const V v(i < nvec ? data[i] : make_uint4(0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu));  // NaN
+#pragma unroll
+      for (int j = 0; j < kVN; ++j) {
+        const float d = dist(v.v[j], m, R.inv_t);
+        const u64 key = order_key(d, begin + i * kVN + j);
+        const bool yes = d < 28.44f && wanted(d, key);
+        const uint32_t ballot = __ballot_sync(0xffffffffu, yes);
+        if (ballot == 0) continue;
+        const int lead = __ffs(ballot) - 1;
+        uint32_t at = 0;
+        if (lane == lead) at = peer_add(counter, __popc(ballot));
+        at = __shfl_sync(0xffffffffu, at, lead) + __popc(ballot & ((1u << lane) - 1));
+        if (yes && at < kList) peer_st(list0 + at * 8, key);
+      }
+    }
+  };
+  auto sorted = [&]() -> int {  // the first CTA's list, sorted; its length
+    const int len = static_cast<int>(min(S.list_n, static_cast<uint32_t>(kList)));
+    int pow2 = 2;
+    while (pow2 < len) pow2 <<= 1;
+    for (int i = len + t; i < pow2; i += kThreads) S.list[i] = ~0ull;
+    __syncthreads();
+    sort_list(S.list, pow2);
+    return len;
+  };
+  // Exclusive running sum, over the list in its order, of f(i) for entries 2t and 2t + 1.
+  auto list_scan = [&](u64 x0, u64 x1, u64 &b0, u64 &b1, u64 &all) {
+    const u64 inc = warp_scan(x0 + x1, lane);
+    if (lane == 31) S.red[warp] = inc;
+    __syncthreads();
+    b0 = inc - x0 - x1;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) b0 += S.red[w];
+      all += S.red[w];
+    }
+    b1 = b0 + x0;
+    __syncthreads();
+  };
+  // First CTA, list path: all three cuts and the choice, from the list.
+  auto finish_list = [&](u64 keep_n, bool by_p, u64 mk_known) {
+    const int len = sorted();
+    const int i0 = 2 * t, i1 = 2 * t + 1;
+    const u64 k0 = i0 < len ? S.list[i0] : ~0ull, k1 = i1 < len ? S.list[i1] : ~0ull;
+    u64 w0 = i0 < len && static_cast<u64>(i0) < keep_n ? weight(key_dist(k0)) : 0;
+    u64 w1 = i1 < len && static_cast<u64>(i1) < keep_n ? weight(key_dist(k1)) : 0;
+    u64 b0, b1, all;
+    list_scan(w0, w1, b0, b1, all);
+    if (by_p) {
+      const u64 limit = mass_limit(R.p, mk_known ? mk_known : all);
+      if (b0 >= limit) w0 = 0;
+      if (b1 >= limit) w1 = 0;
+    }
+    if (w0 < R.least) w0 = 0;
+    if (w1 < R.least) w1 = 0;
+    const u64 target = draw_target(R.u, sum_block(w0 + w1, S.red));
+    // What is kept, by index: index above |z|'s bits.
+    auto flip = [](u64 key) { return (static_cast<u64>(key_index(key)) << 32) | (key >> kIndexBits); };
+    int pow2 = 2;
+    while (pow2 < len) pow2 <<= 1;
+    if (i0 < pow2) S.list[i0] = w0 ? flip(k0) : ~0ull;
+    if (i1 < pow2) S.list[i1] = w1 ? flip(k1) : ~0ull;
+    __syncthreads();
+    sort_list(S.list, pow2);
+    const u64 f0 = i0 < pow2 ? S.list[i0] : ~0ull, f1 = i1 < pow2 ? S.list[i1] : ~0ull;
+    w0 = f0 != ~0ull ? weight(__uint_as_float(static_cast<uint32_t>(f0))) : 0;
+    w1 = f1 != ~0ull ? weight(__uint_as_float(static_cast<uint32_t>(f1))) : 0;
+    list_scan(w0, w1, b0, b1, all);
+    if (w0 && b0 <= target && target < b0 + w0)
+      answer(static_cast<uint32_t>(f0 >> 32), __uint_as_float(static_cast<uint32_t>(f0)));
+    if (w1 && b1 <= target && target < b1 + w1)
+      answer(static_cast<uint32_t>(f1 >> 32), __uint_as_float(static_cast<uint32_t>(f1)));
+  };
+  // The key of the last token a cut keeps, when it falls into step c.bin:
+  // the first at which the count (mass) reaches `want`; `mass` gets what is
+  // kept in all.  Steps with more tokens than the list are halved 2^11-fold by
+  // key until they fit.
+  auto settle = [&](Cut c, bool by_mass, u64 want, u64 limit_key, bool masses, u64 *mass) -> u64 {
+    const int bin = static_cast<int>(c.bin);
+    u64 lo = order_key(fmaxf(static_cast<float>(bin - 1), 0.f) / kBinsPerNat, 0);
+    u64 width = order_key(static_cast<float>(bin + 2) / kBinsPerNat, 0) - lo;
+    auto in_reach = [&](float d, u64 key) {
+      return bin_of(d) == bin && key <= limit_key && key >= lo && key - lo < width;
+    };
+    while (c.count > kList) {
+      int shift = 0;
+      while ((width >> shift) > static_cast<u64>(kBins)) ++shift;
+      cluster_sync(nc);  // every CTA has read its peers' histograms
+      for (int i = t; i < 3 * kBins / 4; i += kThreads) reinterpret_cast<uint4 *>(S.count)[i] = make_uint4(0, 0, 0, 0);
+      __syncthreads();
+      for (int i = t; i < nvec; i += kThreads) {
+        const V v(data[i]);
+#pragma unroll
+        for (int j = 0; j < kVN; ++j) {
+          const float d = dist(v.v[j], m, R.inv_t);
+          const u64 key = order_key(d, begin + i * kVN + j);
+          if (!(d < 28.44f) || !in_reach(d, key)) continue;
+          const u64 w = weight(d);
+          const int b = static_cast<int>(min((key - lo) >> shift, static_cast<u64>(kBins - 1)));
+          if (w == 0) continue;
+          atomicAdd(&S.count[b], 1u);
+          if (masses) {
+            const uint32_t wl = static_cast<uint32_t>(w), old = atomicAdd(&S.lo[b], wl);
+            const uint32_t wh = static_cast<uint32_t>(w >> 32) + (old + wl < old ? 1u : 0u);
+            if (wh) atomicAdd(&S.hi[b], wh);
+          }
+        }
+      }
+      const u64 cb = c.count_before, mb = c.mass_before;
+      cluster_sync(nc);
+      gather_bins(masses);
+      c = find(by_mass, want - (by_mass ? mb : cb));
+      c.count_before += cb;
+      c.mass_before += mb;
+      lo += c.bin << shift;
+      width = u64(1) << shift;
+    }
+    if (t == 0 && rank == 0) S.list_n = 0;
+    cluster_sync(nc);
+    collect([&](float d, u64 key) { return in_reach(d, key) && weight(d) != 0; });
+    cluster_sync(nc);
+    if (rank == 0) {
+      const int len = sorted();
+      const u64 k0 = 2 * t < len ? S.list[2 * t] : ~0ull, k1 = 2 * t + 1 < len ? S.list[2 * t + 1] : ~0ull;
+      const u64 w0 = 2 * t < len ? weight(key_dist(k0)) : 0, w1 = 2 * t + 1 < len ? weight(key_dist(k1)) : 0;
+      u64 b0, b1, all;
+      list_scan(w0, w1, b0, b1, all);
+      const u64 left = want - (by_mass ? c.mass_before : c.count_before);  // at least 1
+      auto tell = [&](u64 key, u64 through) {
+        for (int x = 0; x < nc; ++x) {
+          peer_st(peer(&S.pick, x), key);
+          peer_st(peer(&S.slot[0], x), c.mass_before + through);
+        }
+      };
+      if (by_mass ? (w0 && b0 < left && left <= b0 + w0) : static_cast<u64>(2 * t + 1) == left) tell(k0, b0 + w0);
+      if (by_mass ? (w1 && b1 < left && left <= b1 + w1) : static_cast<u64>(2 * t + 2) == left) tell(k1, b1 + w1);
+    }
+    cluster_sync(nc);
+    *mass = S.slot[0];
+    return S.pick;
+  };
+
+  u64 cut = ~0ull;
+  if (cut_k || cut_p) {
+    gather_bins(cut_p);
+    u64 found = 0;
+    for (int x = 0; x < nc; ++x) found += S.slice_count[x];
+    u64 mk = total;
+    const u64 c0 = pre_c, m0 = pre_m;
+    uint32_t bc0[4];
+    u64 bm0[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bc0[j] = bc[j], bm0[j] = bm[j];
+    if (cut_k && static_cast<u64>(R.k) < found) {
+      const Cut c = find(false, static_cast<u64>(R.k));
+      if (c.count_before + c.count <= kList) {
+        collect([&](float d, u64) { return bin_of(d) <= static_cast<int>(c.bin) && weight(d) != 0; });
+        cluster_sync(nc);
+        if (rank == 0) finish_list(static_cast<u64>(R.k), cut_p, 0);
+        return;
+      }
+      cut = settle(c, false, static_cast<u64>(R.k), ~0ull, cut_p, &mk);
+    }
+    if (cut_p) {
+      const u64 limit = mass_limit(R.p, mk);
+      pre_c = c0;
+      pre_m = m0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) bc[j] = bc0[j], bm[j] = bm0[j];
+      cluster_sync(nc);  // S.cut has been read by all
+      const Cut c = find(true, limit);
+      if (c.count_before + c.count <= kList) {
+        if (t == 0 && rank == 0) S.list_n = 0;
+        cluster_sync(nc);
+        collect([&](float d, u64 key) { return bin_of(d) <= static_cast<int>(c.bin) && key <= cut && weight(d) != 0; });
+        cluster_sync(nc);
+        if (rank == 0) finish_list(~0ull, true, mk);
+        return;
+      }
+      u64 unused;
+      cut = settle(c, true, limit, cut, true, &unused);
+    }
+  }
+
+  // ---- what is kept, in place: its mass a warp, and the walk ----
+  const int v0 = static_cast<int>(static_cast<int64_t>(nvec) * warp / kWarps);
+  const int v1 = static_cast<int>(static_cast<int64_t>(nvec) * (warp + 1) / kWarps);
+  auto kept = [&](float l, int index, float *dd) -> u64 {
+    const float d = dist(l, m, R.inv_t);
+    const u64 w = weight(d);
+    *dd = d;
+    return w >= R.least && order_key(d, index) <= cut ? w : 0;
+  };
+  u64 mine = 0;
+  float d;
+  for (int i = v0 + lane; i < v1; i += 32) {
+    const V v(data[i]);
+#pragma unroll
+    for (int j = 0; j < kVN; ++j) mine += kept(v.v[j], begin + i * kVN + j, &d);
+  }
+  mine = warp_sum(mine);
+  __syncthreads();
+  if (lane == 0) S.red[warp] = mine;
+  __syncthreads();
+  u64 before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += S.red[w];
+    all += S.red[w];
+  }
+  if (t < nc) peer_st(peer(&S.kept[rank], t), all);
+  cluster_sync(nc);
+  u64 mass = 0;
+  for (int c = 0; c < nc; ++c) {
+    if (c < rank) before += S.kept[c];
+    mass += S.kept[c];
+  }
+  const u64 target = draw_target(R.u, mass);
+  if (before <= target && target < before + mine) {  // one warp of the cluster
+    for (int i0 = v0; i0 < v1; i0 += 32) {
+      const int i = i0 + lane;
+      u64 own = 0;
+      if (i < v1) {
+        const V v(data[i]);
+#pragma unroll
+        for (int j = 0; j < kVN; ++j) own += kept(v.v[j], begin + i * kVN + j, &d);
+      }
+      const u64 inc = warp_scan(own, lane), start = before + inc - own;
+      if (i < v1 && start <= target && target < start + own) {
+        const V v(data[i]);
+        u64 at = start;
+#pragma unroll
+        for (int j = 0; j < kVN; ++j) {
+          const u64 w = kept(v.v[j], begin + i * kVN + j, &d);
+          if (w && at <= target && target < at + w) answer(begin + i * kVN + j, d);
+          at += w;
+        }
+      }
+      before += __shfl_sync(0xffffffffu, inc, 31);
+      if (before > target) break;
+    }
+  }
+}
+
+
+constexpr int kSampleSmemMax = 227 * 1024;
+
+// Shared memory of a CTA whose slice holds `slice` logits of `size` bytes.
+size_t sample_smem(int64_t slice, int size) {
+  return (sizeof(SampleShared) + 15) / 16 * 16 + static_cast<size_t>(slice * size + 15) / 16 * 16;
+}
+
+template <int DT>
+int launch_sample_typed(const SampleArgs &a, cudaStream_t s) {
+  const int size = DT == H24_DTYPE_F32 ? 4 : 2;
+  int nc = 1;
+  int64_t slice = 0;
+  for (;; nc *= 2) {
+    slice = ((a.vocab + nc - 1) / nc + 15) / 16 * 16;
+    const bool fits = sample_smem(slice, size) <= kSampleSmemMax;
+    if (fits && (nc == kMaxCluster || a.rows * nc >= 296 || slice <= 2048)) break;
+    if (nc == kMaxCluster) break;
+  }
+  if (sample_smem(slice, size) > kSampleSmemMax || a.rows * nc > INT32_MAX) {
+    sample_rows_kernel<DT><<<wave_grid(a.rows, 2), kSampleThreads, 0, s>>>(a);
+    H24_CUDA_TRY(cudaGetLastError());
+    count_launches(1);
+    return H24_OK;
+  }
+  const auto kernel = sample_cluster_kernel<DT>;
+  H24_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleSmemMax));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.rows * nc));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = sample_smem(slice, size);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(nc);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  H24_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, nc, static_cast<int>(slice)));
+  count_launches(1);
+  return H24_OK;
+}
+
 }  // namespace
 
 int launch_sample(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t stride, const float *u,
@@ -214,15 +845,11 @@ int launch_sample(const void *logits, int dtype, int64_t rows, int64_t vocab, in
                   float *logprobs, cudaStream_t s) {
   const SampleArgs a{logits, rows, vocab, stride, u, temperature, top_k, top_p, min_p, temperature1, top_p1, min_p1,
                      top_k1, tokens, logprobs};
-  const int grid = wave_grid(rows, 2);
   switch (dtype) {
-    case H24_DTYPE_F32: sample_rows_kernel<H24_DTYPE_F32><<<grid, kSampleThreads, 0, s>>>(a); break;
-    case H24_DTYPE_F16: sample_rows_kernel<H24_DTYPE_F16><<<grid, kSampleThreads, 0, s>>>(a); break;
-    default: sample_rows_kernel<H24_DTYPE_BF16><<<grid, kSampleThreads, 0, s>>>(a); break;
+    case H24_DTYPE_F32: return launch_sample_typed<H24_DTYPE_F32>(a, s);
+    case H24_DTYPE_F16: return launch_sample_typed<H24_DTYPE_F16>(a, s);
+    default: return launch_sample_typed<H24_DTYPE_BF16>(a, s);
   }
-  H24_CUDA_TRY(cudaGetLastError());
-  count_launches(1);
-  return H24_OK;
 }
 
 }  // namespace h24
