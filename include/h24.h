@@ -189,7 +189,8 @@ int h24_add_rms_norm_int8(const void *x, const void *residual, const void *gain,
 int h24_rows_int8_quantize(const void *x, int64_t rows, int64_t cols, int64_t x_stride, int dtype,
                            int8_t *q, float *scale, void *stream);
 
-/* out = q * scale[row], rounded to `dtype`; all contiguous. */
+/* out = q * scale[row], rounded to `dtype`; all contiguous, q and out 16-byte
+ * aligned. */
 int h24_rows_int8_dequant(const int8_t *q, const float *scale, int64_t rows, int64_t cols, int dtype,
                           void *out, void *stream);
 

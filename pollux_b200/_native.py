@@ -7,6 +7,8 @@ Signatures carry plain device pointers, sizes and a CUDA stream handle.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import threading
 
@@ -124,6 +126,31 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+_torch_calls = None
+_TORCH_ENTRIES = ("h24_add_rms_norm_int8", "h24_rows_int8_quantize", "h24_rows_int8_dequant", "h24_int8_linear",
+                  "h24_sample_tokens")
+
+
+def torch_calls():
+    """The module _h24_torch, which makes the decoding-step calls of libh24
+    straight from torch tensors (raises if it has not been built)."""
+    global _torch_calls
+    if _torch_calls is None:
+        import torch  # noqa: F401  (the module's symbols are torch's)
+        lib = load()
+        with _lock:
+            if _torch_calls is None:
+                path = os.path.join(_HERE, "_lib", "_h24_torch.so")
+                if not os.path.exists(path):
+                    raise H24Error(f"_h24_torch.so not found at {path}; build it with `python -m pollux_b200.build`")
+                loader = importlib.machinery.ExtensionFileLoader("_h24_torch", path)
+                mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("_h24_torch", loader))
+                loader.exec_module(mod)
+                mod.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in _TORCH_ENTRIES))
+                _torch_calls = mod
+    return _torch_calls
+
+
 def check(rc: int, what: str) -> None:
     """Turn a status code into the exception the reference would raise."""
     if rc == H24_OK:
@@ -137,4 +164,6 @@ def check(rc: int, what: str) -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(load(), name)(*args), name)
+    rc = getattr(_lib or load(), name)(*args)
+    if rc != H24_OK:
+        check(rc, name)

@@ -65,7 +65,7 @@ def _work_device(t: torch.Tensor) -> torch.device:
 
 
 def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(dev.index)  # the handle without a Stream object
 
 
 def _call(dev: torch.device, name: str, *args) -> None:

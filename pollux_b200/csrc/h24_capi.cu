@@ -526,6 +526,7 @@ int h24_add_rms_norm_int8(const void *x, const void *residual, const void *gain,
   if (!x || !gain || !q || !scale) return fail(H24_ERR_INVALID, "add_rms_norm_int8: null pointer");
   if (x_stride < 0 || (residual && residual_stride < 0))
     return fail(H24_ERR_INVALID, "add_rms_norm_int8: negative stride");
+  if (rows > INT32_MAX) return fail(H24_ERR_INVALID, "add_rms_norm_int8: more than 2^31 - 1 rows");
   return launch_rows_int8(x, residual, gain, gain_dtype, rows, cols, x_stride, residual_stride, dtype, eps, q, scale,
                           residual_out, as_stream(stream));
 }
@@ -537,6 +538,7 @@ int h24_rows_int8_quantize(const void *x, int64_t rows, int64_t cols, int64_t x_
   if (rows == 0 || cols == 0) return H24_OK;
   if (!x || !q || !scale) return fail(H24_ERR_INVALID, "rows_int8_quantize: null pointer");
   if (x_stride < 0) return fail(H24_ERR_INVALID, "rows_int8_quantize: negative stride");
+  if (rows > INT32_MAX) return fail(H24_ERR_INVALID, "rows_int8_quantize: more than 2^31 - 1 rows");
   return launch_rows_int8(x, nullptr, nullptr, dtype, rows, cols, x_stride, 0, dtype, 0.f, q, scale, nullptr,
                           as_stream(stream));
 }
@@ -547,6 +549,7 @@ int h24_rows_int8_dequant(const int8_t *q, const float *scale, int64_t rows, int
   if (!known_dtype(dtype)) return fail(H24_ERR_INVALID, "rows_int8_dequant: unknown dtype");
   if (rows == 0 || cols == 0) return H24_OK;
   if (!q || !scale || !out) return fail(H24_ERR_INVALID, "rows_int8_dequant: null pointer");
+  if (!aligned16(q) || !aligned16(out)) return fail(H24_ERR_INVALID, "rows_int8_dequant: q and out must be 16-byte aligned");
   return launch_rows_dequant(q, scale, rows, cols, dtype, out, as_stream(stream));
 }
 

@@ -416,9 +416,8 @@ int split_smem(int n, int stages) { return 1024 + kHeadBytes + stages * (kABytes
 
 template <bool kTma, typename Out>
 int launch_split(const CUtensorMap &wmap, const CUtensorMap &qmap, const LinArgs &a, int smem, cudaStream_t s) {
-  const auto kernel = int8_linear_split_kernel<kTma, Out>;
-  H24_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax));
-  H24_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+  constexpr auto kernel = int8_linear_split_kernel<kTma, Out>;
+  H24_CUDA_TRY(allow_smem<kernel>(kSmemMax));
   const int64_t tiles = (static_cast<int64_t>(a.out) + kM - 1) / kM * a.tok_tiles;
   if (tiles * a.split > INT32_MAX) return fail(H24_ERR_INVALID, "int8_linear: too many tiles");
   cudaLaunchConfig_t cfg = {};

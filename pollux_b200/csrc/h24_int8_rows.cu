@@ -5,35 +5,40 @@
 //   v_c    = s_c * g_c,  m = max_c |v_c|                fp32
 //   i      = 1 / sqrt(mean_c(s_c^2) + eps)              fp32
 //   mu     = max(m * i, fp32(1e-8)),  scale = mu / 127  fp32
-//   q_c    = clamp(rint(v_c * (i * 127 / mu)), -128, 127)
+//   q_c    = rint(v_c * (i * 127 / mu))                 within [-127, 127]
 // Quantisation alone takes v = x and i = 1.  A NaN in a row (or an infinite
 // element under the norm) makes its scale NaN and every q 0, as the row
 // quantiser of the weights does.  The norm is taken of the unrounded sum.
 #include "h24_internal.cuh"
+#include <cstdlib>
+#define NVWANT (std::getenv("NV") ? atoi(std::getenv("NV")) : 1)
 
 namespace h24 {
 namespace {
 
 constexpr float kRowEps = 1e-8f;  // smallest mu, as for the weights (pack.py:124-136)
-constexpr int kRowThreads = 256;
+constexpr int kDeqThreads = 256;
 
 template <int DT>
 struct Elem;
 template <>
 struct Elem<H24_DTYPE_F32> {
   using T = float;
+  static constexpr int kVec = 4;
   static __device__ __forceinline__ float up(float v) { return v; }
   static __device__ __forceinline__ float down(float v) { return v; }
 };
 template <>
 struct Elem<H24_DTYPE_F16> {
   using T = __half;
+  static constexpr int kVec = 8;
   static __device__ __forceinline__ float up(__half v) { return __half2float(v); }
   static __device__ __forceinline__ __half down(float v) { return __float2half_rn(v); }
 };
 template <>
 struct Elem<H24_DTYPE_BF16> {
   using T = __nv_bfloat16;
+  static constexpr int kVec = 8;
   static __device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
   static __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
 };
@@ -56,79 +61,308 @@ struct RowArgs {
   void *residual_out;
 };
 
-// rint(v * k) as int8; NaN gives 0.
-__device__ __forceinline__ int8_t quant_act(float v, float k) {
-  const float t = v * k;
-  return t != t ? int8_t(0) : static_cast<int8_t>(static_cast<int>(fminf(fmaxf(rintf(t), -128.0f), 127.0f)));
+// rint(v * k), |v * k| below 2^22, in the low byte: adding 1.5 * 2^23 leaves the
+// integer, rounded to nearest even, in the low bits of the sum.  One fused
+// multiply-add an element, where a rounding and a conversion instruction each
+// run at an eighth of its rate.
+__device__ __forceinline__ uint32_t quant_act(float v, float k) {
+  return __float_as_uint(fmaf(v, k, 12582912.0f));
 }
 
-// One block per row, two passes over it.
-template <int DT, bool kNorm>
-__global__ void __launch_bounds__(kRowThreads) rows_int8_kernel(const RowArgs a) {
-  using E = Elem<DT>;
-  using T = typename E::T;
-  __shared__ float red[2][kRowThreads / 32];
-  pdl_enter();
-  const int t = threadIdx.x;
-  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    const T *x = static_cast<const T *>(a.x) + r * a.x_stride;
-    const T *res = a.residual ? static_cast<const T *>(a.residual) + r * a.residual_stride : nullptr;
-    auto gain = [&](int64_t c) {
-      return a.gain_f32 ? static_cast<const float *>(a.gain)[c] : E::up(static_cast<const T *>(a.gain)[c]);
-    };
-    float ss = 0.f, m = 0.f;
-    for (int64_t c = t; c < a.cols; c += kRowThreads) {
-      float s = E::up(x[c]);
-      if (kNorm) {
-        if (res) s += E::up(res[c]);
-        ss = fmaf(s, s, ss);
-        m = nan_max(m, fabsf(s * gain(c)));
-      } else {
-        m = nan_max(m, fabsf(s));
-      }
-    }
+// The value of one row's partial (sum of squares, largest magnitude) over a
+// block of `warps` warps.
+__device__ __forceinline__ void reduce_row(float &ss, float &m, float (*red)[32], int warps) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      m = nan_max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    }
-    if ((t & 31) == 0) red[0][t >> 5] = ss, red[1][t >> 5] = m;
-    __syncthreads();
-    ss = 0.f, m = 0.f;
-    for (int w = 0; w < kRowThreads / 32; ++w) ss += red[0][w], m = nan_max(m, red[1][w]);
-    __syncthreads();
-    const float inv = kNorm ? 1.0f / sqrtf(ss / static_cast<float>(a.cols) + a.eps) : 1.0f;
-    float mu = m * inv;
-    mu = mu != mu ? mu : fmaxf(mu, kRowEps);
-    const float k = inv * (127.0f / mu);
-    for (int64_t c = t; c < a.cols; c += kRowThreads) {
-      float s = E::up(x[c]);
-      if (kNorm) {
-        if (res) s += E::up(res[c]);
-        if (a.residual_out) static_cast<T *>(a.residual_out)[r * a.cols + c] = E::down(s);
-        s *= gain(c);
-      }
-      a.q[r * a.cols + c] = quant_act(s, k);
-    }
-    if (t == 0) a.scale[r] = mu / 127.0f;
+  for (int o = 16; o > 0; o >>= 1) {
+    ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    m = nan_max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  }
+  if (warps == 1) return;
+  const int t = threadIdx.x;
+  if ((t & 31) == 0) red[0][t >> 5] = ss, red[1][t >> 5] = m;
+  __syncthreads();
+  ss = 0.f;
+  m = 0.f;
+  for (int w = 0; w < warps; ++w) ss += red[0][w], m = nan_max(m, red[1][w]);
+}
+
+// mu / 127 and the factor that takes v to q, from a row's sums.  |v * factor|
+// is at most 127 (1 + 2^-21), which rounds to 127: q needs no clamp.  A row
+// whose mu is not finite has every q 0: `dead`.
+template <bool kNorm>
+__device__ __forceinline__ float row_factor(const RowArgs &a, float ss, float m, float *scale, bool *dead) {
+  const float inv = kNorm ? 1.0f / sqrtf(ss / static_cast<float>(a.cols) + a.eps) : 1.0f;
+  float mu = m * inv;
+  mu = mu != mu ? mu : fmaxf(mu, kRowEps);
+  *scale = mu / 127.0f;
+  *dead = !(mu <= 3.402823466e38f);
+  return inv * (127.0f / mu);
+}
+
+// `live` (at most kVec) consecutive elements as fp32, zeros after them; kVec
+// elements are 16 bytes.  kAligned: whole and 16-byte aligned, one load.
+template <int DT, bool kAligned>
+__device__ __forceinline__ void load_vec(const typename Elem<DT>::T *p, int live, float (&v)[Elem<DT>::kVec]) {
+  using E = Elem<DT>;
+  if (kAligned) {
+    alignas(16) typename E::T x[E::kVec];
+    *reinterpret_cast<uint4 *>(x) = *reinterpret_cast<const uint4 *>(p);
+#pragma unroll
+    for (int j = 0; j < E::kVec; ++j) v[j] = E::up(x[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < E::kVec; ++j) v[j] = j < live ? E::up(p[j]) : 0.f;
   }
 }
 
-template <int DT>
-__global__ void __launch_bounds__(kRowThreads) rows_dequant_kernel(const int8_t *__restrict__ q,
-                                                                   const float *__restrict__ scale, int64_t rows,
-                                                                   int64_t cols, void *out) {
+// A block of blockDim.x threads per row; thread t holds the 16-byte groups t,
+// t + blockDim.x, ... (at most NV) of its row in registers, so the row is read
+// once.  Rows that are not 16-byte aligned, or end inside a group, are read
+// and written by the element in the same groups: a row's result does not
+// depend on where it lies.
+template <int DT, bool kAligned, int NV, bool kNorm>
+__global__ void __launch_bounds__(1024) rows_int8_kernel(const RowArgs a) {
   using E = Elem<DT>;
+  using T = typename E::T;
+  constexpr int VEC = E::kVec;
+  __shared__ float red[2][32];
   pdl_enter();
-  const int64_t total = rows * cols, stride = static_cast<int64_t>(gridDim.x) * kRowThreads;
-  for (int64_t i = blockIdx.x * static_cast<int64_t>(kRowThreads) + threadIdx.x; i < total; i += stride)
-    static_cast<typename E::T *>(out)[i] = E::down(static_cast<float>(q[i]) * scale[i / cols]);
+  const int t = threadIdx.x, nt = blockDim.x;
+  const int cols = static_cast<int>(a.cols);
+  const int64_t r = blockIdx.x;
+  const T *x = static_cast<const T *>(a.x) + r * a.x_stride;
+  float v[NV][VEC];
+  float ss = 0.f, m = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int at = (t + i * nt) * VEC;
+    if (at < cols) load_vec<DT, kAligned>(x + at, cols - at, v[i]);
+  }
+  if (kNorm && a.residual) {
+    const T *res = static_cast<const T *>(a.residual) + r * a.residual_stride;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int at = (t + i * nt) * VEC;
+      if (at < cols) {
+        float s[VEC];
+        load_vec<DT, kAligned>(res + at, cols - at, s);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[i][j] += s[j];
+      }
+    }
+  }
+  if (kNorm && a.residual_out) {
+    T *sum_out = static_cast<T *>(a.residual_out) + r * a.cols;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int at = (t + i * nt) * VEC;
+      if (at < cols) {
+        alignas(16) T o[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) o[j] = E::down(v[i][j]);
+        if (kAligned) {
+          *reinterpret_cast<uint4 *>(sum_out + at) = *reinterpret_cast<const uint4 *>(o);
+        } else {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            if (at + j < cols) sum_out[at + j] = o[j];
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int at = (t + i * nt) * VEC;
+    if (at < cols) {
+      if (kNorm) {
+        float g[VEC];
+        if (DT != H24_DTYPE_F32 && a.gain_f32) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            g[j] = kAligned || at + j < cols ? __ldg(static_cast<const float *>(a.gain) + at + j) : 0.f;
+        } else {
+          load_vec<DT, kAligned>(static_cast<const T *>(a.gain) + at, cols - at, g);
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          ss = fmaf(v[i][j], v[i][j], ss);
+          v[i][j] *= g[j];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) m = nan_max(m, fabsf(v[i][j]));
+    }
+  }
+  reduce_row(ss, m, red, nt >> 5);
+  float scale;
+  bool dead;
+  const float k = row_factor<kNorm>(a, ss, m, &scale, &dead);
+  int8_t *q = a.q + r * a.cols;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int at = (t + i * nt) * VEC;
+    if (at < cols) {
+      if (kAligned) {
+        uint32_t w[VEC / 4];
+#pragma unroll
+        for (int j = 0; j < VEC; j += 4)
+          w[j / 4] = dead ? 0u
+                          : __byte_perm(__byte_perm(quant_act(v[i][j], k), quant_act(v[i][j + 1], k), 0x0040),
+                                        __byte_perm(quant_act(v[i][j + 2], k), quant_act(v[i][j + 3], k), 0x0040),
+                                        0x5410);
+        if constexpr (VEC == 8)
+          *reinterpret_cast<uint2 *>(q + at) = make_uint2(w[0], w[1]);
+        else
+          *reinterpret_cast<uint32_t *>(q + at) = w[0];
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (at + j < cols) q[at + j] = dead ? int8_t(0) : static_cast<int8_t>(quant_act(v[i][j], k));
+      }
+    }
+  }
+  if (t == 0) a.scale[r] = scale;
+}
+
+constexpr int kLongThreads = 512;
+
+// Rows too long for the registers of a block: two passes over the row.
+template <int DT, bool kNorm>
+__global__ void __launch_bounds__(kLongThreads) rows_int8_long_kernel(const RowArgs a) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  __shared__ float red[2][32];
+  pdl_enter();
+  const int t = threadIdx.x;
+  const int64_t r = blockIdx.x;
+  const T *x = static_cast<const T *>(a.x) + r * a.x_stride;
+  const T *res = a.residual ? static_cast<const T *>(a.residual) + r * a.residual_stride : nullptr;
+  auto gain = [&](int64_t c) {
+    return a.gain_f32 ? static_cast<const float *>(a.gain)[c] : E::up(static_cast<const T *>(a.gain)[c]);
+  };
+  float ss = 0.f, m = 0.f;
+  for (int64_t c = t; c < a.cols; c += kLongThreads) {
+    float s = E::up(x[c]);
+    if (kNorm) {
+      if (res) s += E::up(res[c]);
+      ss = fmaf(s, s, ss);
+      m = nan_max(m, fabsf(s * gain(c)));
+    } else {
+      m = nan_max(m, fabsf(s));
+    }
+  }
+  reduce_row(ss, m, red, kLongThreads / 32);
+  float scale;
+  bool dead;
+  const float k = row_factor<kNorm>(a, ss, m, &scale, &dead);
+  for (int64_t c = t; c < a.cols; c += kLongThreads) {
+    float s = E::up(x[c]);
+    if (kNorm) {
+      if (res) s += E::up(res[c]);
+      if (a.residual_out) static_cast<T *>(a.residual_out)[r * a.cols + c] = E::down(s);
+      s *= gain(c);
+    }
+    a.q[r * a.cols + c] = dead ? int8_t(0) : static_cast<int8_t>(quant_act(s, k));
+  }
+  if (t == 0) a.scale[r] = scale;
+}
+
+constexpr int kDeqUnroll = 4;
+
+// Groups of 16 output bytes of the flat array, kDeqUnroll in flight a thread
+// (a warp's store covers whole sectors: two groups a thread side by side wrote
+// half sectors and ran at 4.5 TB/s).  kInRow: cols is a multiple of a group, so
+// its elements share a row.
+template <int DT, bool kInRow>
+__global__ void __launch_bounds__(kDeqThreads) rows_dequant_kernel(const int8_t *__restrict__ q,
+                                                                   const float *__restrict__ scale, int64_t total,
+                                                                   int64_t cols, typename Elem<DT>::T *out) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  constexpr int VEC = E::kVec;
+  pdl_enter();
+  const int64_t nvec = total / VEC, step = static_cast<int64_t>(gridDim.x) * kDeqThreads * kDeqUnroll;
+  const bool narrow = total <= 0xFFFFFFFFll;
+  for (int64_t i0 = blockIdx.x * static_cast<int64_t>(kDeqThreads) * kDeqUnroll + threadIdx.x; i0 < nvec; i0 += step) {
+    uint32_t raw[kDeqUnroll][VEC / 4];
+    float s[kDeqUnroll];
+    int64_t row[kDeqUnroll];
+#pragma unroll
+    for (int u = 0; u < kDeqUnroll; ++u) {
+      const int64_t i = i0 + u * kDeqThreads;
+      if (i >= nvec) continue;
+      if constexpr (VEC == 8) {
+        const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(q) + i);
+        raw[u][0] = w.x;
+        raw[u][1] = w.y;
+      } else {
+        raw[u][0] = __ldcs(reinterpret_cast<const uint32_t *>(q) + i);
+      }
+      row[u] = narrow ? static_cast<uint32_t>(i * VEC) / static_cast<uint32_t>(cols) : i * VEC / cols;
+      s[u] = __ldg(scale + row[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kDeqUnroll; ++u) {
+      const int64_t i = i0 + u * kDeqThreads;
+      if (i >= nvec) continue;
+      int64_t left = (row[u] + 1) * cols - i * VEC;  // elements of the row from here
+      alignas(16) T o[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        if (!kInRow && left-- == 0) {
+          s[u] = __ldg(scale + ++row[u]);
+          left = cols - 1;
+        }
+        const int8_t b = static_cast<int8_t>(raw[u][j / 4] >> (8 * (j % 4)));
+        o[j] = E::down(static_cast<float>(b) * s[u]);
+      }
+      __stcs(reinterpret_cast<uint4 *>(out) + i, *reinterpret_cast<const uint4 *>(o));
+    }
+  }
+  if (blockIdx.x == 0 && threadIdx.x < total % VEC) {
+    const int64_t i = nvec * VEC + threadIdx.x;
+    out[i] = E::down(static_cast<float>(q[i]) * scale[i / cols]);
+  }
+}
+
+template <int DT, bool kNorm, int NV>
+int launch_rows_nv(const RowArgs &a, bool aligned, int threads, cudaStream_t s) {
+  const auto kernel = aligned ? rows_int8_kernel<DT, true, NV, kNorm> : rows_int8_kernel<DT, false, NV, kNorm>;
+  H24_CUDA_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(a.rows)), dim3(threads), s, a));
+  count_launches(1);
+  return H24_OK;
 }
 
 template <int DT, bool kNorm>
 int launch_rows(const RowArgs &a, cudaStream_t s) {
-  const int grid = wave_grid(a.rows, blocks_per_sm(rows_int8_kernel<DT, kNorm>, kRowThreads, 0));
-  H24_CUDA_TRY(launch_pdl(rows_int8_kernel<DT, kNorm>, dim3(grid), dim3(kRowThreads), s, a));
+  constexpr int kVec = Elem<DT>::kVec;
+  const bool aligned = a.cols % kVec == 0 && a.x_stride % kVec == 0 && a.residual_stride % kVec == 0 &&
+                       aligned16(a.x) && aligned16(a.residual) && aligned16(a.residual_out) && aligned16(a.gain) &&
+                       (reinterpret_cast<uintptr_t>(a.q) & 7) == 0;
+  const int64_t nvec = (a.cols + kVec - 1) / kVec;
+  int want = NVWANT;
+  for (int nv = want; nv <= 8; nv *= 2) {
+    const int64_t threads = ((nvec + nv - 1) / nv + 31) / 32 * 32;
+    if (threads > (nv < 8 ? 512 : 1024)) continue;
+    switch (nv) {
+      case 1: return launch_rows_nv<DT, kNorm, 1>(a, aligned, static_cast<int>(threads), s);
+      case 2: return launch_rows_nv<DT, kNorm, 2>(a, aligned, static_cast<int>(threads), s);
+      case 4: return launch_rows_nv<DT, kNorm, 4>(a, aligned, static_cast<int>(threads), s);
+      default: return launch_rows_nv<DT, kNorm, 8>(a, aligned, static_cast<int>(threads), s);
+    }
+  }
+  H24_CUDA_TRY(launch_pdl(rows_int8_long_kernel<DT, kNorm>, dim3(static_cast<unsigned>(a.rows)), dim3(kLongThreads), s, a));
+  count_launches(1);
+  return H24_OK;
+}
+
+template <int DT>
+int launch_dequant_rows(const int8_t *q, const float *scale, int64_t total, int64_t cols, void *out, cudaStream_t s) {
+  constexpr int kPerBlock = Elem<DT>::kVec * kDeqThreads * kDeqUnroll;
+  const int grid = wave_grid((total + kPerBlock - 1) / kPerBlock, 8);
+  const auto kernel = cols % Elem<DT>::kVec == 0 ? rows_dequant_kernel<DT, true> : rows_dequant_kernel<DT, false>;
+  H24_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(kDeqThreads), s, q, scale, total, cols,
+                          static_cast<typename Elem<DT>::T *>(out)));
   count_launches(1);
   return H24_OK;
 }
@@ -150,13 +384,12 @@ int launch_rows_int8(const void *x, const void *residual, const void *gain, int 
 
 int launch_rows_dequant(const int8_t *q, const float *scale, int64_t rows, int64_t cols, int dtype, void *out,
                         cudaStream_t s) {
-  const int grid = wave_grid((rows * cols + kRowThreads - 1) / kRowThreads, 8);
-  const auto kernel = dtype == H24_DTYPE_F32   ? rows_dequant_kernel<H24_DTYPE_F32>
-                      : dtype == H24_DTYPE_F16 ? rows_dequant_kernel<H24_DTYPE_F16>
-                                               : rows_dequant_kernel<H24_DTYPE_BF16>;
-  H24_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(kRowThreads), s, q, scale, rows, cols, out));
-  count_launches(1);
-  return H24_OK;
+  const int64_t total = rows * cols;
+  switch (dtype) {
+    case H24_DTYPE_F32: return launch_dequant_rows<H24_DTYPE_F32>(q, scale, total, cols, out, s);
+    case H24_DTYPE_F16: return launch_dequant_rows<H24_DTYPE_F16>(q, scale, total, cols, out, s);
+    default: return launch_dequant_rows<H24_DTYPE_BF16>(q, scale, total, cols, out, s);
+  }
 }
 
 }  // namespace h24

@@ -816,8 +816,8 @@ int launch_sample_typed(const SampleArgs &a, cudaStream_t s) {
     count_launches(1);
     return H24_OK;
   }
-  const auto kernel = sample_cluster_kernel<DT>;
-  H24_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSampleSmemMax));
+  constexpr auto kernel = sample_cluster_kernel<DT>;
+  H24_CUDA_TRY(allow_smem<kernel>(kSampleSmemMax));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.rows * nc));
   cfg.blockDim = dim3(kThreads);

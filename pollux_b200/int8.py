@@ -21,7 +21,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _native as N
-from .castor import _call, _stream, _work_device
+from .castor import _aligned, _call, _stream, _work_device
 
 _DTYPES = {torch.float32: N.DTYPE_F32, torch.float16: N.DTYPE_F16, torch.bfloat16: N.DTYPE_BF16}
 MAX_IN_FEATURES = 131_000  # above this an int32 sum of int8 products could overflow
@@ -41,7 +41,7 @@ def _rows(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
         t = t.to(dev)
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
-    if t.stride(1) != 1 and t.shape[1] > 1 or t.stride(0) < 0:
+    if t.stride(1) != 1 and t.shape[1] > 1:
         t = t.contiguous()
     return t
 
@@ -51,7 +51,7 @@ def _vector(t: torch.Tensor, n: int, dtype: torch.dtype | None, dev: torch.devic
         raise ValueError(f"{what} must hold {n} values, got {tuple(t.shape)}")
     if t.device != dev or (dtype is not None and t.dtype != dtype):
         t = t.to(device=dev, dtype=dtype)
-    return t.reshape(-1).contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _check_rows(t: torch.Tensor, what: str) -> None:
@@ -68,6 +68,9 @@ def add_rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Ten
     ``summed = x + residual`` in x's dtype, the next layer's residual (None
     without ``residual``).  Sums, statistics and the norm are fp32, taken of the
     unrounded sum.  A row with a NaN gets a NaN scale and zeros."""
+    got = (N._torch_calls or N.torch_calls()).add_rms_norm_int8(x, weight, residual, eps)
+    if got is not None:
+        return got
     _check_rows(x, "x")
     code = _code(x.dtype, "x")
     if eps < 0:
@@ -83,9 +86,9 @@ def add_rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Ten
     # The kernel reads gains of x's dtype or fp32; another 16-bit type widens exactly.
     w = _vector(weight, cols, None if weight.dtype in (x.dtype, torch.float32) else torch.float32, dev, "weight")
     rows = xr.shape[0]
-    q = torch.empty(x.shape, dtype=torch.int8, device=dev)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-    summed = None if rr is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+    q = xr.new_empty(x.shape, dtype=torch.int8)
+    scale = xr.new_empty(x.shape[:-1], dtype=torch.float32)
+    summed = None if rr is None else xr.new_empty(x.shape)
     if rows and cols:
         _call(dev, "h24_add_rms_norm_int8", xr.data_ptr(), None if rr is None else rr.data_ptr(), w.data_ptr(),
               code if w.dtype == x.dtype else N.DTYPE_F32, rows, cols, xr.stride(0),
@@ -100,13 +103,16 @@ def add_rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Ten
 def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Per-row int8 of ``x`` over its last dimension: ``(q, scale)`` with
     ``q * scale`` within half a scale of x."""
+    got = (N._torch_calls or N.torch_calls()).quantize_rows_int8(x)
+    if got is not None:
+        return got
     _check_rows(x, "x")
     code = _code(x.dtype, "x")
     dev = _work_device(x)
     xr = _rows(x, dev)
     rows, cols = xr.shape
-    q = torch.empty(x.shape, dtype=torch.int8, device=dev)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    q = xr.new_empty(x.shape, dtype=torch.int8)
+    scale = xr.new_empty(x.shape[:-1], dtype=torch.float32)
     if rows and cols:
         _call(dev, "h24_rows_int8_quantize", xr.data_ptr(), rows, cols, xr.stride(0), code, q.data_ptr(),
               scale.data_ptr(), _stream(dev))
@@ -115,6 +121,9 @@ def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 def dequantize_rows_int8(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``q * scale`` per row, rounded once to ``dtype``."""
+    got = (N._torch_calls or N.torch_calls()).dequantize_rows_int8(q, scale, dtype)
+    if got is not None:
+        return got
     _check_rows(q, "q")
     if q.dtype != torch.int8:
         raise TypeError(f"q must be int8, got {q.dtype}")
@@ -122,9 +131,9 @@ def dequantize_rows_int8(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtyp
     dev = _work_device(q)
     cols = q.shape[-1]
     rows = q.numel() // cols if cols else 0
-    out = torch.empty(q.shape, dtype=dtype, device=dev)
+    qr = _aligned(q if q.device == dev else q.to(dev))
+    out = qr.new_empty(q.shape, dtype=dtype)
     if rows and cols:
-        qr = (q if q.device == dev else q.to(dev)).contiguous()
         s = _vector(scale, rows, torch.float32, dev, "scale")
         _call(dev, "h24_rows_int8_dequant", qr.data_ptr(), s.data_ptr(), rows, cols, code, out.data_ptr(),
               _stream(dev))
@@ -138,6 +147,9 @@ def int8_linear(q: torch.Tensor, scale: torch.Tensor, weight_int8: torch.Tensor,
     ``mu_rows`` [out] (``W = weight_int8 * fp16(mu / 127)``, as
     ``PackedInt8Linear``).  The sum is exact in int32; the scaling and the bias
     are fp32; the result is rounded once to ``out_dtype``."""
+    got = (N._torch_calls or N.torch_calls()).int8_linear(q, scale, weight_int8, mu_rows, bias, out_dtype)
+    if got is not None:
+        return got
     _check_rows(q, "q")
     if q.dtype != torch.int8 or weight_int8.dtype != torch.int8:
         raise TypeError(f"q and weight_int8 must be int8, got {q.dtype} and {weight_int8.dtype}")
@@ -155,12 +167,13 @@ def int8_linear(q: torch.Tensor, scale: torch.Tensor, weight_int8: torch.Tensor,
     dev = _work_device(q)
     qr = _rows(q, dev)
     w = weight_int8 if weight_int8.device == dev else weight_int8.to(dev)
-    w = w.contiguous()
+    if not w.is_contiguous():
+        w = w.contiguous()
     tokens = qr.shape[0] if in_f else scale.numel()
     s = _vector(scale, tokens, torch.float32, dev, "scale")
     mu = _vector(mu_rows, out_f, None, dev, "mu_rows")
     b = None if bias is None else _vector(bias, out_f, torch.float32, dev, "bias")
-    y = torch.empty(q.shape[:-1] + (out_f,), dtype=out_dtype, device=dev)
+    y = qr.new_empty(q.shape[:-1] + (out_f,), dtype=out_dtype)
     if tokens and out_f:
         _call(dev, "h24_int8_linear", qr.data_ptr(), s.data_ptr(), tokens, qr.stride(0), w.data_ptr(), mu.data_ptr(),
               out_f, in_f, None if b is None else b.data_ptr(), code, y.data_ptr(), _stream(dev))

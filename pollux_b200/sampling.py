@@ -14,6 +14,7 @@ from .castor import _call, _stream, _work_device
 from .int8 import _code, _rows
 
 MAX_VOCAB = 1 << 22
+_INF = float("inf")
 
 
 def _setting(v, rows: int, dtype: torch.dtype, dev: torch.device, name: str):
@@ -24,7 +25,8 @@ def _setting(v, rows: int, dtype: torch.dtype, dev: torch.device, name: str):
         raise ValueError(f"{name} must be a number or hold one value for each of the {rows} rows, got {tuple(v.shape)}")
     if v.device != dev or v.dtype != dtype:
         v = v.to(device=dev, dtype=dtype)
-    v = v.reshape(-1).contiguous()
+    if not v.is_contiguous():
+        v = v.contiguous()
     return v, v.data_ptr(), 0
 
 
@@ -46,31 +48,34 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: float | to
     Returns int64 tokens of the leading shape, with ``return_logprob`` also the
     fp32 log-probabilities of the tokens at that temperature before the cuts
     (-inf for a row that gives -1)."""
+    got = (N._torch_calls or N.torch_calls()).sample_tokens(logits, u, temperature, top_k, top_p, min_p, return_logprob)
+    if got is not None:
+        return got
     if logits.dim() < 1:
         raise ValueError("logits must have at least one dimension")
     code = _code(logits.dtype, "logits")
     lead, vocab = logits.shape[:-1], logits.shape[-1]
     if not 0 < vocab <= MAX_VOCAB:
         raise ValueError(f"the vocabulary must hold 1 to {MAX_VOCAB} tokens, got {vocab}")
-    for name, v, ok in (("temperature", temperature, lambda v: v >= 0), ("top_k", top_k, lambda v: v >= 0),
-                        ("top_p", top_p, lambda v: 0 <= v <= 1), ("min_p", min_p, lambda v: 0 <= v <= 1)):
-        if not isinstance(v, torch.Tensor) and not ok(v):
+    rows = logits.numel() // vocab
+    for name, v, most in (("temperature", temperature, _INF), ("top_k", top_k, _INF), ("top_p", top_p, 1.0),
+                          ("min_p", min_p, 1.0)):
+        if not isinstance(v, torch.Tensor) and not 0 <= v <= most:
             raise ValueError(f"{name} out of range: {v}")
     dev = _work_device(logits)
-    rows = logits.numel() // vocab
     if u.numel() != rows:
         raise ValueError(f"u must hold one number for each of the {rows} rows, got {tuple(u.shape)}")
-    tokens = torch.empty(lead, dtype=torch.int64, device=dev)
-    logprob = torch.empty(lead, dtype=torch.float32, device=dev) if return_logprob else None
+    ts, tp, t1 = _setting(temperature, rows, torch.float32, dev, "temperature")
+    ks, kp, k1 = _setting(top_k, rows, torch.int32, dev, "top_k")
+    ps, pp, p1 = _setting(top_p, rows, torch.float32, dev, "top_p")
+    ms, mp, m1 = _setting(min_p, rows, torch.float32, dev, "min_p")
+    us, up, _ = _setting(u, rows, torch.float32, dev, "u")
+    lr = _rows(logits, dev)
+    tokens = lr.new_empty(lead, dtype=torch.int64)
+    logprob = lr.new_empty(lead, dtype=torch.float32) if return_logprob else None
     if rows:
-        lr = _rows(logits, dev)
-        us, up, _ = _setting(u, rows, torch.float32, dev, "u")
-        ts, tp, t1 = _setting(temperature, rows, torch.float32, dev, "temperature")
-        ks, kp, k1 = _setting(top_k, rows, torch.int32, dev, "top_k")
-        ps, pp, p1 = _setting(top_p, rows, torch.float32, dev, "top_p")
-        ms, mp, m1 = _setting(min_p, rows, torch.float32, dev, "min_p")
         _call(dev, "h24_sample_tokens", lr.data_ptr(), code, rows, vocab, lr.stride(0), up, tp, t1, kp,
-              min(int(k1), vocab), pp, p1, mp, m1, tokens.data_ptr(),
+              vocab if k1 > vocab else int(k1), pp, p1, mp, m1, tokens.data_ptr(),
               None if logprob is None else logprob.data_ptr(), _stream(dev))
     if logits.device != dev:
         tokens = tokens.to(logits.device)
