@@ -10,8 +10,6 @@
 // element under the norm) makes its scale NaN and every q 0, as the row
 // quantiser of the weights does.  The norm is taken of the unrounded sum.
 #include "h24_internal.cuh"
-#include <cstdlib>
-#define NVWANT (std::getenv("NV") ? atoi(std::getenv("NV")) : 1)
 
 namespace h24 {
 namespace {
@@ -99,64 +97,77 @@ __device__ __forceinline__ float row_factor(const RowArgs &a, float ss, float m,
   return inv * (127.0f / mu);
 }
 
-// `live` (at most kVec) consecutive elements as fp32, zeros after them; kVec
-// elements are 16 bytes.  kAligned: whole and 16-byte aligned, one load.
-template <int DT, bool kAligned>
-__device__ __forceinline__ void load_vec(const typename Elem<DT>::T *p, int live, float (&v)[Elem<DT>::kVec]) {
+// The elements of a 16-byte group as fp32.
+template <int DT>
+__device__ __forceinline__ void widen(uint4 raw, float (&v)[Elem<DT>::kVec]) {
   using E = Elem<DT>;
-  if (kAligned) {
-    alignas(16) typename E::T x[E::kVec];
-    *reinterpret_cast<uint4 *>(x) = *reinterpret_cast<const uint4 *>(p);
+  alignas(16) typename E::T x[E::kVec];
+  *reinterpret_cast<uint4 *>(x) = raw;
 #pragma unroll
-    for (int j = 0; j < E::kVec; ++j) v[j] = E::up(x[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < E::kVec; ++j) v[j] = j < live ? E::up(p[j]) : 0.f;
-  }
+  for (int j = 0; j < E::kVec; ++j) v[j] = E::up(x[j]);
 }
 
-// A block of blockDim.x threads per row; thread t holds the 16-byte groups t,
-// t + blockDim.x, ... (at most NV) of its row in registers, so the row is read
-// once.  Rows that are not 16-byte aligned, or end inside a group, are read
-// and written by the element in the same groups: a row's result does not
-// depend on where it lies.
+// Thread t of a block holds the 16-byte groups t, t + blockDim.x, ... (at most
+// NV) of its row in registers, so the row is read once.  A block walks rows r, r + gridDim.x, ..., and asks for
+// the next row before it reduces the present one.  Rows that are not 16-byte
+// aligned, or end inside a group, are read and written by the element in the
+// same groups: a row's result does not depend on where it lies.
 template <int DT, bool kAligned, int NV, bool kNorm>
-__global__ void __launch_bounds__(1024) rows_int8_kernel(const RowArgs a) {
+__global__ void __launch_bounds__(NV < 8 ? 512 : 1024) rows_int8_kernel(const RowArgs a) {
   using E = Elem<DT>;
   using T = typename E::T;
   constexpr int VEC = E::kVec;
-  __shared__ float red[2][32];
+  __shared__ float red[2][2][32];
   pdl_enter();
   const int t = threadIdx.x, nt = blockDim.x;
   const int cols = static_cast<int>(a.cols);
-  const int64_t r = blockIdx.x;
-  const T *x = static_cast<const T *>(a.x) + r * a.x_stride;
-  float v[NV][VEC];
-  float ss = 0.f, m = 0.f;
+  const bool has_res = kNorm && a.residual != nullptr;
+  uint4 raw[NV], raw_res[NV];
+  auto ask = [&](int64_t r) {
+    if (!kAligned || r >= a.rows) return;
+    const uint4 *x = reinterpret_cast<const uint4 *>(static_cast<const T *>(a.x) + r * a.x_stride);
+    const uint4 *res = reinterpret_cast<const uint4 *>(static_cast<const T *>(a.residual) + r * a.residual_stride);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int at = (t + i * nt) * VEC;
-    if (at < cols) load_vec<DT, kAligned>(x + at, cols - at, v[i]);
-  }
-  if (kNorm && a.residual) {
-    const T *res = static_cast<const T *>(a.residual) + r * a.residual_stride;
+    for (int i = 0; i < NV; ++i)
+      if ((t + i * nt) * VEC < cols) {
+        raw[i] = x[t + i * nt];
+        if (has_res) raw_res[i] = res[t + i * nt];
+      }
+  };
+  ask(blockIdx.x);
+  int turn = 0;
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x, turn ^= 1) {
+    float v[NV][VEC];
+    float ss = 0.f, m = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int at = (t + i * nt) * VEC;
-      if (at < cols) {
-        float s[VEC];
-        load_vec<DT, kAligned>(res + at, cols - at, s);
+      if (at >= cols) continue;
+      if (kAligned) {
+        widen<DT>(raw[i], v[i]);
+        if (has_res) {
+          float s[VEC];
+          widen<DT>(raw_res[i], s);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[i][j] += s[j];
+          for (int j = 0; j < VEC; ++j) v[i][j] += s[j];
+        }
+      } else {
+        const T *x = static_cast<const T *>(a.x) + r * a.x_stride + at;
+        const T *res = static_cast<const T *>(a.residual) + r * a.residual_stride + at;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          v[i][j] = at + j < cols ? E::up(x[j]) : 0.f;
+          if (has_res && at + j < cols) v[i][j] += E::up(res[j]);
+        }
       }
     }
-  }
-  if (kNorm && a.residual_out) {
+    ask(r + gridDim.x);
     T *sum_out = static_cast<T *>(a.residual_out) + r * a.cols;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int at = (t + i * nt) * VEC;
-      if (at < cols) {
+      if (at >= cols) continue;
+      if (kNorm && a.residual_out) {
         alignas(16) T o[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) o[j] = E::down(v[i][j]);
@@ -168,20 +179,17 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(const RowArgs a) {
             if (at + j < cols) sum_out[at + j] = o[j];
         }
       }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int at = (t + i * nt) * VEC;
-    if (at < cols) {
       if (kNorm) {
         float g[VEC];
         if (DT != H24_DTYPE_F32 && a.gain_f32) {
 #pragma unroll
           for (int j = 0; j < VEC; ++j)
             g[j] = kAligned || at + j < cols ? __ldg(static_cast<const float *>(a.gain) + at + j) : 0.f;
+        } else if (kAligned) {
+          widen<DT>(__ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.gain) + at)), g);
         } else {
-          load_vec<DT, kAligned>(static_cast<const T *>(a.gain) + at, cols - at, g);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) g[j] = at + j < cols ? E::up(static_cast<const T *>(a.gain)[at + j]) : 0.f;
         }
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
@@ -192,16 +200,15 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(const RowArgs a) {
 #pragma unroll
       for (int j = 0; j < VEC; ++j) m = nan_max(m, fabsf(v[i][j]));
     }
-  }
-  reduce_row(ss, m, red, nt >> 5);
-  float scale;
-  bool dead;
-  const float k = row_factor<kNorm>(a, ss, m, &scale, &dead);
-  int8_t *q = a.q + r * a.cols;
+    reduce_row(ss, m, red[turn], nt >> 5);
+    float scale;
+    bool dead;
+    const float k = row_factor<kNorm>(a, ss, m, &scale, &dead);
+    int8_t *q = a.q + r * a.cols;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int at = (t + i * nt) * VEC;
-    if (at < cols) {
+    for (int i = 0; i < NV; ++i) {
+      const int at = (t + i * nt) * VEC;
+      if (at >= cols) continue;
       if (kAligned) {
         uint32_t w[VEC / 4];
 #pragma unroll
@@ -220,8 +227,8 @@ __global__ void __launch_bounds__(1024) rows_int8_kernel(const RowArgs a) {
           if (at + j < cols) q[at + j] = dead ? int8_t(0) : static_cast<int8_t>(quant_act(v[i][j], k));
       }
     }
+    if (t == 0) a.scale[r] = scale;
   }
-  if (t == 0) a.scale[r] = scale;
 }
 
 constexpr int kLongThreads = 512;
@@ -328,7 +335,8 @@ __global__ void __launch_bounds__(kDeqThreads) rows_dequant_kernel(const int8_t 
 template <int DT, bool kNorm, int NV>
 int launch_rows_nv(const RowArgs &a, bool aligned, int threads, cudaStream_t s) {
   const auto kernel = aligned ? rows_int8_kernel<DT, true, NV, kNorm> : rows_int8_kernel<DT, false, NV, kNorm>;
-  H24_CUDA_TRY(launch_pdl(kernel, dim3(static_cast<unsigned>(a.rows)), dim3(threads), s, a));
+  const int grid = wave_grid(a.rows, blocks_per_sm(kernel, threads, 0));
+  H24_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(threads), s, a));
   count_launches(1);
   return H24_OK;
 }
@@ -340,12 +348,14 @@ int launch_rows(const RowArgs &a, cudaStream_t s) {
                        aligned16(a.x) && aligned16(a.residual) && aligned16(a.residual_out) && aligned16(a.gain) &&
                        (reinterpret_cast<uintptr_t>(a.q) & 7) == 0;
   const int64_t nvec = (a.cols + kVec - 1) / kVec;
-  int want = NVWANT;
-  for (int nv = want; nv <= 8; nv *= 2) {
+  // Two groups a thread, more where a row needs over 512 threads.  One group
+  // runs [1,1920] bf16 in 1.82 us instead of 2.08 but [4096,1920] in 13.3
+  // instead of 10.5.  The number of rows has no say, so that a row's sum is
+  // the same in every batch.
+  for (int nv = 2; nv <= 8; nv *= 2) {
     const int64_t threads = ((nvec + nv - 1) / nv + 31) / 32 * 32;
     if (threads > (nv < 8 ? 512 : 1024)) continue;
     switch (nv) {
-      case 1: return launch_rows_nv<DT, kNorm, 1>(a, aligned, static_cast<int>(threads), s);
       case 2: return launch_rows_nv<DT, kNorm, 2>(a, aligned, static_cast<int>(threads), s);
       case 4: return launch_rows_nv<DT, kNorm, 4>(a, aligned, static_cast<int>(threads), s);
       default: return launch_rows_nv<DT, kNorm, 8>(a, aligned, static_cast<int>(threads), s);
