@@ -15,12 +15,14 @@
 // row's mass stays below 2^62.
 //
 // sample_cluster_kernel reads a row once.  A cluster of 1 to 8 CTAs holds it in
-// shared memory, a slice each; a histogram of |z| in 2,048 steps of 1/72 (below
-// |z| = 28.4 a weight rounds to 0) gives for each step a count and, where top-p
-// asks, a mass; the CTAs add the histograms through distributed shared memory,
-// a share of the steps each, and the step in which a cut falls is known.  Are
-// there at most 1,024 tokens up to it, they go to the first CTA, which sorts
-// them and finishes; else the tokens of that one step settle the cut and the
+// shared memory, a slice each.  A cut is found from a histogram of |z| in steps
+// of 1/72 (beyond |z| = 28.4 a weight rounds to 0), which the CTAs add through
+// distributed shared memory, a share of the steps each.  For top-k only each
+// thread's largest logit is counted: the step that holds the k-th of those
+// bounds the k-th token, and what lies up to it (k and a few more) goes to the
+// first CTA, which makes all three cuts and the choice.  For top-p alone every
+// step gets a count and a mass; a few tokens up to the cut go the same way, and
+// otherwise the tokens of the one step in which the cut falls settle it and the
 // CTAs add and walk what is kept, in place.
 //
 // "z descending, index ascending" is one 64-bit key: |z|'s bits above the
@@ -69,8 +71,15 @@ __device__ __forceinline__ float dist(float l, float m, float inv_t) {
   return l == m ? 0.f : (d == d ? d : INFINITY);  // NaN: a masked logit at an infinite temperature
 }
 
+// rint(exp(-d) * 2^40) without a 64-bit conversion: from 2^23 on a float is an
+// integer, its mantissa shifted; below, adding 2^23 leaves the nearest (even)
+// integer in the low bits.
 __device__ __forceinline__ u64 weight(float d) {
-  return static_cast<u64>(__float2ll_rn(expf(-d) * kOne));
+  const float f = expf(-d) * kOne;
+  const uint32_t bits = __float_as_uint(f);
+  const int shift = static_cast<int>(bits >> 23) - 150;
+  const uint32_t small = __float_as_uint(f + 8388608.0f) - 0x4B000000u;
+  return shift >= 0 ? static_cast<u64>((bits & 0x7FFFFFu) | 0x800000u) << shift : small;
 }
 
 constexpr int kIndexBits = 22;
@@ -234,9 +243,12 @@ __device__ __forceinline__ uint32_t peer(const void *p, int rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(su32(p)), "r"(rank));
   return r;
 }
-__device__ __forceinline__ uint32_t peer_ld(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ uint4 peer_ld4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
 __device__ __forceinline__ void peer_st(uint32_t addr, u64 v) {
@@ -250,8 +262,10 @@ __device__ __forceinline__ uint32_t peer_add(uint32_t addr, uint32_t v) {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBins = 2048;
-constexpr float kBinsPerNat = 72.0f;  // 2048 / 72 = 28.44: exp(-28.42) * 2^40 = 1/2
+// Steps of |z|: 2,046 up to 28.45, where exp(-|z|) * 2^40 is below 1/2.
+constexpr float kBinsPerNat = 71.9f, kFar = 28.45f;
 constexpr int kList = 1024;
+constexpr int kFew = 128;  // lists up to this long are ranked by counting
 constexpr int kMaxCluster = 8;
 
 struct Cut {  // where a cut falls: the step, what is before it and in it
@@ -261,14 +275,16 @@ struct Cut {  // where a cut falls: the step, what is before it and in it
 struct SampleShared {
   uint32_t count[kBins], lo[kBins], hi[kBins];
   u64 list[kList];
-  u64 slot[kMaxCluster];                          // one value of each CTA
+  u64 few[2][kFew];
+  u64 slot[kMaxCluster];  // one value of each CTA
   u64 slice_count[kMaxCluster], slice_mass[kMaxCluster];
   u64 total[kMaxCluster], first[kMaxCluster], kept[kMaxCluster];
   Cut cut;
   u64 scan_c[kWarps], scan_m[kWarps];
+  u64 warp_total[kWarps], warp_kept[kWarps];
   u64 red[kWarps];
   u64 pick;
-  uint32_t list_n;
+  uint32_t list_n, local_n;
 };
 
 __device__ __forceinline__ void cluster_sync(int c) {
@@ -329,10 +345,13 @@ struct Vec {
   }
 };
 
-__device__ __forceinline__ int bin_of(float d) { return static_cast<int>(d * kBinsPerNat); }  // d below 28.44
+// The step of a |z| below kFar: the nearest one (an addition, no conversion).
+__device__ __forceinline__ int bin_of(float d) {
+  return static_cast<int>(__float_as_uint(fmaf(d, kBinsPerNat, 8388608.0f)) - 0x4B000000u);
+}
 
 // Sorts the first n (a power of two) keys of the list, ascending.
-__device__ void sort_list(u64 *list, int n) {
+__device__ __noinline__ void sort_list(u64 *list, int n) {
   for (int k = 2; k <= n; k <<= 1)
     for (int j = k >> 1; j > 0; j >>= 1) {
       for (int i = threadIdx.x; i < n / 2; i += kThreads) {
@@ -351,7 +370,7 @@ struct RowSettings {
 };
 
 template <int DT>
-__global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleArgs a, int nc, int slice) {
+__global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const SampleArgs a, int nc, int slice) {
   using V = Vec<DT>;
   constexpr int kVN = V::kN, kSize = DT == H24_DTYPE_F32 ? 4 : 2;
   extern __shared__ __align__(16) uint8_t sample_raw[];
@@ -363,9 +382,15 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
   const int begin = rank * slice;
   const int n = static_cast<int>(max(int64_t(0), min(static_cast<int64_t>(slice), a.vocab - begin)));
   const int nvec = (n + kVN - 1) / kVN;
+  // A warp's part of the slice, in the order of the indices.
+  const int v0 = static_cast<int>(static_cast<int64_t>(nvec) * warp / kWarps);
+  const int v1 = static_cast<int>(static_cast<int64_t>(nvec) * (warp + 1) / kWarps);
 
-  if (t == 0) S.list_n = 0;
-  for (int i = t; i < 3 * kBins / 4; i += kThreads) reinterpret_cast<uint4 *>(S.count)[i] = make_uint4(0, 0, 0, 0);
+  auto clear_steps = [&]() {
+    for (int i = t; i < 3 * kBins / 4; i += kThreads) reinterpret_cast<uint4 *>(S.count)[i] = make_uint4(0, 0, 0, 0);
+  };
+  if (t == 0) S.list_n = 0, S.local_n = 0;
+  clear_steps();
   __syncwarp();
   if (nc > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   pdl_enter();
@@ -381,27 +406,28 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
     R.inv_t = __fdiv_rn(1.0f, temp);
   }
 
-  // ---- the slice into shared memory, and the row's largest logit ----
+  // ---- the slice into shared memory; each thread's and the row's largest logit ----
   const uint8_t *src = static_cast<const uint8_t *>(a.logits) + (r * a.stride + begin) * kSize;
-  float mx = -INFINITY;
+  float mine_max = -INFINITY;
   const int nfull = aligned16(src) ? n / kVN : 0;  // vectors that can be loaded whole
+#pragma unroll 4
   for (int i = t; i < nfull; i += kThreads) {
     const uint4 raw = __ldcs(reinterpret_cast<const uint4 *>(src) + i);
     data[i] = raw;
     const V v(raw);
 #pragma unroll
-    for (int j = 0; j < kVN; ++j) mx = fmaxf(mx, v.v[j]);
+    for (int j = 0; j < kVN; ++j) mine_max = fmaxf(mine_max, v.v[j]);
   }
-  {  // the rest by the element, padded with -inf to a whole vector
-    for (int i = nfull * kVN + t; i < nvec * kVN; i += kThreads) {
-      if (DT == H24_DTYPE_F32)
-        reinterpret_cast<float *>(data)[i] = i < n ? reinterpret_cast<const float *>(src)[i] : -INFINITY;
-      else
-        reinterpret_cast<uint16_t *>(data)[i] = i < n ? reinterpret_cast<const uint16_t *>(src)[i]
-                                                     : static_cast<uint16_t>(DT == H24_DTYPE_F16 ? 0xFC00 : 0xFF80);
-      if (i < n) mx = fmaxf(mx, logit_at<DT>(src, i));
-    }
+  // The rest by the element, padded with -inf to a whole vector.
+  for (int i = nfull * kVN + t; i < nvec * kVN; i += kThreads) {
+    if (DT == H24_DTYPE_F32)
+      reinterpret_cast<float *>(data)[i] = i < n ? reinterpret_cast<const float *>(src)[i] : -INFINITY;
+    else
+      reinterpret_cast<uint16_t *>(data)[i] = i < n ? reinterpret_cast<const uint16_t *>(src)[i]
+                                                   : static_cast<uint16_t>(DT == H24_DTYPE_F16 ? 0xFC00 : 0xFF80);
+    if (i < n) mine_max = fmaxf(mine_max, logit_at<DT>(src, i));
   }
+  float mx = mine_max;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   if (lane == 0) S.red[warp] = __float_as_uint(mx);
@@ -415,7 +441,6 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
     cluster_sync(nc);
     for (int c = 0; c < nc; ++c) mx = fmaxf(mx, __uint_as_float(static_cast<uint32_t>(S.slot[c])));
   }
-  __syncthreads();  // S.red
   const float m = mx;
   if (m == -INFINITY) {  // nothing to choose from (the same for the whole cluster)
     if (rank == 0 && t == 0) {
@@ -425,81 +450,111 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
     return;
   }
 
-  // ---- total mass, first index of the maximum, histogram ----
-  const bool cut_k = R.k > 1 && R.k < a.vocab, cut_p = R.k > 1 && R.p < 1.f;
-  u64 sum = 0;
-  uint32_t first = 0xFFFFFFFFu;
-  for (int i = t; i < nvec; i += kThreads) {
-    const V v(data[i]);
+  // ---- one pass: total mass, what min-p leaves of it, the largest logit's
+  // first index, and the steps that a cut at p looks at ----
+  const bool greedy = R.k == 1, cut_k = !greedy && R.k < a.vocab, cut_p = !greedy && R.p < 1.f;
+  auto count_step = [&](int b, u64 w, bool masses) {
+    atomicAdd(&S.count[b], 1u);
+    if (masses) {
+      const uint32_t wl = static_cast<uint32_t>(w), old = atomicAdd(&S.lo[b], wl);
+      const uint32_t wh = static_cast<uint32_t>(w >> 32) + (old + wl < old ? 1u : 0u);
+      if (wh) atomicAdd(&S.hi[b], wh);
+    }
+  };
+  // Without top-k, tokens beyond |z| = ln(4 V / (1 - p)) hold less than (1 - p)
+  // of the mass together, so the cut at p falls before them.
+  const bool steps_of_all = cut_p && !cut_k;
+  const float far = steps_of_all ? fminf(kFar, logf(4.0f * static_cast<float>(a.vocab) / (1.0f - R.p)) + 0.01f) : 0.f;
+  if (a.logprobs || !cut_k) {
+    u64 total = 0, kept = 0;
+    uint32_t first = 0xFFFFFFFFu;
+    for (int i = v0 + lane; i < v1; i += 32) {
+      const V v(data[i]);
 #pragma unroll
-    for (int j = 0; j < kVN; ++j) {
-      const float d = dist(v.v[j], m, R.inv_t);
-      const u64 w = weight(d);
-      if (w == 0) continue;
-      sum += w;
-      if (v.v[j] == m) first = min(first, static_cast<uint32_t>(begin + i * kVN + j));
-      if (cut_k || cut_p) {
-        const int b = bin_of(d);
-        atomicAdd(&S.count[b], 1u);
-        if (cut_p) {
-          const uint32_t wl = static_cast<uint32_t>(w), old = atomicAdd(&S.lo[b], wl);
-          const uint32_t wh = static_cast<uint32_t>(w >> 32) + (old + wl < old ? 1u : 0u);
-          if (wh) atomicAdd(&S.hi[b], wh);
-        }
+      for (int j = 0; j < kVN; ++j) {
+        const float d = dist(v.v[j], m, R.inv_t);
+        const u64 w = weight(d);
+        total += w;
+        if (w >= R.least) kept += w;
+        if (greedy && v.v[j] == m) first = min(first, static_cast<uint32_t>(begin + i * kVN + j));
+        if (steps_of_all && d < far) count_step(bin_of(d), w, true);
       }
     }
+    total = warp_sum(total);
+    kept = warp_sum(kept);
+    first = __reduce_min_sync(0xffffffffu, first);
+    if (lane == 0) {
+      S.warp_total[warp] = total;
+      S.warp_kept[warp] = kept;
+      S.scan_c[warp] = first;
+    }
+  } else if (lane == 0) {
+    S.warp_total[warp] = 0;
   }
-  sum = sum_block(sum, S.red);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
-  if (lane == 0) S.red[warp] = first;
+  // The k-th largest of the threads' largest logits is at most the k-th
+  // largest logit: the steps of those alone give a bound on the cut at k.
+  if (cut_k) {
+    const float d = dist(mine_max, m, R.inv_t);
+    if (d < kFar && weight(d)) atomicAdd(&S.count[bin_of(d)], 1u);
+  }
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) first = min(first, static_cast<uint32_t>(S.red[w]));
   if (t < nc) {
-    peer_st(peer(&S.total[rank], t), sum);
-    peer_st(peer(&S.first[rank], t), first);
+    u64 tot = 0, kep = 0, fir = ~0ull;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      tot += S.warp_total[w];
+      kep += S.warp_kept[w];
+      fir = min(fir, S.scan_c[w]);
+    }
+    peer_st(peer(&S.total[rank], t), tot);
+    peer_st(peer(&S.kept[rank], t), kep);
+    peer_st(peer(&S.first[rank], t), fir);
   }
   cluster_sync(nc);
   u64 total = 0;
-  for (int c = 0; c < nc; ++c) {
-    total += S.total[c];
-    first = min(first, static_cast<uint32_t>(S.first[c]));
-  }
+  for (int c = 0; c < nc; ++c) total += S.total[c];
   auto answer = [&](uint32_t index, float d) {
     a.tokens[r] = index;
     if (a.logprobs)
       a.logprobs[r] = -d - logf(static_cast<float>(static_cast<double>(total) / static_cast<double>(kOne)));
   };
-  if (R.k == 1) {
-    if (rank == 0 && t == 0) answer(first, 0.f);
+  if (greedy) {
+    if (rank == 0 && t == 0) {
+      u64 first = ~0ull;
+      for (int c = 0; c < nc; ++c) first = min(first, S.first[c]);
+      answer(static_cast<uint32_t>(first), 0.f);
+    }
     return;
   }
 
-  // This CTA's share of the steps, added over the cluster: `per` steps a
-  // thread, with the count and mass before them (of the whole row).
-  const int share = kBins / nc, per = (share + kThreads - 1) / kThreads;
+  // This CTA's share of the steps, added over the cluster: four steps for each
+  // group of nc lanes, one CTA's counts a lane, with the count and mass before
+  // them (of the whole row).
+  const int share = kBins / nc, my_bin = rank * share + t / nc * 4;
   uint32_t bc[4];
   u64 bm[4], pre_c = 0, pre_m = 0;
   auto gather_bins = [&](bool masses) {
-    u64 c = 0, q = 0;
+    const int x = t & (nc - 1);
+    const uint4 c4 = peer_ld4(peer(&S.count[my_bin], x));
+    bc[0] = c4.x, bc[1] = c4.y, bc[2] = c4.z, bc[3] = c4.w;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      bc[j] = 0;
-      bm[j] = 0;
-      const int b = t * per + j;
-      if (j < per && b < share) {
-        for (int x = 0; x < nc; ++x) {
-          bc[j] += peer_ld(peer(&S.count[rank * share + b], x));
-          if (masses)
-            bm[j] += peer_ld(peer(&S.lo[rank * share + b], x)) +
-                     (static_cast<u64>(peer_ld(peer(&S.hi[rank * share + b], x))) << 32);
-        }
-      }
-      c += bc[j];
-      q += bm[j];
+    for (int j = 0; j < 4; ++j) bm[j] = 0;
+    if (masses) {
+      const uint4 l4 = peer_ld4(peer(&S.lo[my_bin], x)), h4 = peer_ld4(peer(&S.hi[my_bin], x));
+      bm[0] = l4.x | static_cast<u64>(h4.x) << 32;
+      bm[1] = l4.y | static_cast<u64>(h4.y) << 32;
+      bm[2] = l4.z | static_cast<u64>(h4.z) << 32;
+      bm[3] = l4.w | static_cast<u64>(h4.w) << 32;
     }
-    const u64 ic = warp_scan(c, lane), im = warp_scan(q, lane);
+    for (int o = 1; o < nc; o <<= 1) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        bc[j] += __shfl_xor_sync(0xffffffffu, bc[j], o);
+        if (masses) bm[j] += __shfl_xor_sync(0xffffffffu, bm[j], o);
+      }
+    }
+    const u64 c = static_cast<u64>(bc[0]) + bc[1] + bc[2] + bc[3], q = bm[0] + bm[1] + bm[2] + bm[3];
+    const u64 ic = warp_scan(x == 0 ? c : 0, lane), im = masses ? warp_scan(x == 0 ? q : 0, lane) : 0;
     if (lane == 31) S.scan_c[warp] = ic, S.scan_m[warp] = im;
     __syncthreads();
     pre_c = ic - c;
@@ -516,62 +571,72 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
       peer_st(peer(&S.slice_mass[rank], t), all_m);
     }
     cluster_sync(nc);
-    for (int x = 0; x < rank; ++x) pre_c += S.slice_count[x], pre_m += S.slice_mass[x];
+    for (int y = 0; y < rank; ++y) pre_c += S.slice_count[y], pre_m += S.slice_mass[y];
+  };
+  auto counted = [&]() -> u64 {
+    u64 c = 0;
+    for (int y = 0; y < nc; ++y) c += S.slice_count[y];
+    return c;
   };
   // The step at which the running count (or mass) reaches `want`, told to all.
   auto find = [&](bool by_mass, u64 want) -> Cut {
-    u64 c = pre_c, q = pre_m;
+    if ((t & (nc - 1)) == 0) {
+      u64 c = pre_c, q = pre_m;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const u64 before = by_mass ? q : c, in = by_mass ? bm[j] : bc[j];
-      if (before < want && want <= before + in) {
-        for (int x = 0; x < nc; ++x) {
-          const uint32_t to = peer(&S.cut, x);
-          peer_st(to, static_cast<u64>(rank * share + t * per + j));
-          peer_st(to + 8, c);
-          peer_st(to + 16, q);
-          peer_st(to + 24, bc[j]);
-          peer_st(to + 32, bm[j]);
+      for (int j = 0; j < 4; ++j) {
+        const u64 before = by_mass ? q : c, in = by_mass ? bm[j] : bc[j];
+        if (before < want && want <= before + in) {
+          for (int x = 0; x < nc; ++x) {
+            const uint32_t to = peer(&S.cut, x);
+            peer_st(to, static_cast<u64>(my_bin + j));
+            peer_st(to + 8, c);
+            peer_st(to + 16, q);
+            peer_st(to + 24, bc[j]);
+            peer_st(to + 32, bm[j]);
+          }
         }
+        c += bc[j];
+        q += bm[j];
       }
-      c += bc[j];
-      q += bm[j];
     }
     cluster_sync(nc);
     return S.cut;
   };
-  // Keys that satisfy `wanted` go to the first CTA's list; their number (in
-  // the first CTA) is S.list_n.
-  auto collect = [&](auto wanted) {
+  // Keys that satisfy `wanted` go to the first CTA's list (as many as fit);
+  // returns their number in the cluster.  Starts and ends with the cluster in
+  // step; S.list_n and S.local_n are zero at the start.
+  auto collect = [&](auto wanted) -> u64 {
     const uint32_t counter = peer(&S.list_n, 0), list0 = peer(&S.list[0], 0);
-    for (int i0 = 0; i0 < nvec; i0 += kThreads) {
-      const int i = i0 + t;
-      const V v(i < nvec ? data[i] : make_uint4(0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu, 0xFFFFFFFFu));  // NaN
+    for (int i = v0 + lane; i < v1; i += 32) {
+      const V v(data[i]);
 #pragma unroll
       for (int j = 0; j < kVN; ++j) {
         const float d = dist(v.v[j], m, R.inv_t);
-        const u64 key = order_key(d, begin + i * kVN + j);
-        const bool yes = d < 28.44f && wanted(d, key);
-        const uint32_t ballot = __ballot_sync(0xffffffffu, yes);
-        if (ballot == 0) continue;
-        const int lead = __ffs(ballot) - 1;
-        uint32_t at = 0;
-        if (lane == lead) at = peer_add(counter, __popc(ballot));
-        at = __shfl_sync(0xffffffffu, at, lead) + __popc(ballot & ((1u << lane) - 1));
-        if (yes && at < kList) peer_st(list0 + at * 8, key);
+        if (d < kFar) {
+          const u64 key = order_key(d, begin + i * kVN + j);
+          if (wanted(d, key) && weight(d)) {
+            atomicAdd(&S.local_n, 1u);
+            const uint32_t at = peer_add(counter, 1u);
+            if (at < kList) peer_st(list0 + at * 8, key);
+          }
+        }
       }
     }
+    __syncthreads();
+    if (t < nc) peer_st(peer(&S.slot[rank], t), S.local_n);
+    cluster_sync(nc);
+    u64 all = 0;
+    for (int c = 0; c < nc; ++c) all += S.slot[c];
+    return all;
   };
-  auto sorted = [&]() -> int {  // the first CTA's list, sorted; its length
-    const int len = static_cast<int>(min(S.list_n, static_cast<uint32_t>(kList)));
+  auto sort_by_key = [&](int len) {
     int pow2 = 2;
     while (pow2 < len) pow2 <<= 1;
     for (int i = len + t; i < pow2; i += kThreads) S.list[i] = ~0ull;
     __syncthreads();
     sort_list(S.list, pow2);
-    return len;
   };
-  // Exclusive running sum, over the list in its order, of f(i) for entries 2t and 2t + 1.
+  // Exclusive running sum over the list of the values of entries 2t and 2t + 1.
   auto list_scan = [&](u64 x0, u64 x1, u64 &b0, u64 &b1, u64 &all) {
     const u64 inc = warp_scan(x0 + x1, lane);
     if (lane == 31) S.red[warp] = inc;
@@ -586,9 +651,70 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
     b1 = b0 + x0;
     __syncthreads();
   };
-  // First CTA, list path: all three cuts and the choice, from the list.
-  auto finish_list = [&](u64 keep_n, bool by_p, u64 mk_known) {
-    const int len = sorted();
+  // For lists of at most kFew keys: four threads an entry (entry t / 4) count
+  // the keys before it and add their weights, `total_w` those of all.
+  constexpr int kPer = kThreads / kFew;
+  auto rank_few = [&](int len, u64 key, u64 *before_w, u64 *total_w) -> int {
+    int before = 0;
+    u64 w = 0, all = 0;
+    for (int i = t % kPer; i < len; i += kPer) {
+      const bool less = S.list[i] < key;
+      const u64 wi = S.few[0][i];
+      before += less;
+      w += less ? wi : 0;
+      all += wi;
+    }
+#pragma unroll
+    for (int o = 1; o < kPer; o <<= 1) {
+      before += __shfl_xor_sync(0xffffffffu, before, o);
+      w += __shfl_xor_sync(0xffffffffu, w, o);
+      all += __shfl_xor_sync(0xffffffffu, all, o);
+    }
+    *before_w = w;
+    *total_w = all;
+    return before;
+  };
+  // First CTA, list path: all three cuts and the choice, from the list (which
+  // holds at least every token that step 1 keeps, or step 2 where mk is known).
+  auto finish_list = [&](int len, u64 keep_n, bool by_p, u64 mk) {
+    if (len <= kFew) {
+      for (int i = t; i < len; i += kThreads) S.few[0][i] = weight(key_dist(S.list[i]));
+      __syncthreads();
+      const int e = t / kPer;
+      const u64 key = e < len ? S.list[e] : ~0ull;
+      u64 before, all, w = e < len ? S.few[0][e] : 0;
+      const int place = rank_few(len, key, &before, &all);
+      if (static_cast<u64>(place) >= keep_n) w = 0;
+      if (by_p) {
+        if (!mk) {  // the mass of the first keep_n
+          if (static_cast<u64>(place) == min(keep_n, static_cast<u64>(len)) - 1 && t % kPer == 0 && e < len)
+            S.pick = before + S.few[0][e];
+          __syncthreads();
+          mk = S.pick;
+        }
+        if (before >= mass_limit(R.p, mk)) w = 0;
+      }
+      if (w < R.least) w = 0;
+      if (t % kPer == 0 && e < len) S.few[1][e] = w;
+      __syncthreads();
+      // The running mass in the order of the indices.
+      u64 run = 0, mass = 0;
+      const uint32_t index = key_index(key);
+      for (int i = t % kPer; i < len; i += kPer) {
+        const u64 wi = S.few[1][i];
+        mass += wi;
+        run += key_index(S.list[i]) < index ? wi : 0;
+      }
+#pragma unroll
+      for (int o = 1; o < kPer; o <<= 1) {
+        run += __shfl_xor_sync(0xffffffffu, run, o);
+        mass += __shfl_xor_sync(0xffffffffu, mass, o);
+      }
+      const u64 target = draw_target(R.u, mass);
+      if (t % kPer == 0 && w && run <= target && target < run + w) answer(index, key_dist(key));
+      return;
+    }
+    sort_by_key(len);
     const int i0 = 2 * t, i1 = 2 * t + 1;
     const u64 k0 = i0 < len ? S.list[i0] : ~0ull, k1 = i1 < len ? S.list[i1] : ~0ull;
     u64 w0 = i0 < len && static_cast<u64>(i0) < keep_n ? weight(key_dist(k0)) : 0;
@@ -596,7 +722,7 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
     u64 b0, b1, all;
     list_scan(w0, w1, b0, b1, all);
     if (by_p) {
-      const u64 limit = mass_limit(R.p, mk_known ? mk_known : all);
+      const u64 limit = mass_limit(R.p, mk ? mk : all);
       if (b0 >= limit) w0 = 0;
       if (b1 >= limit) w1 = 0;
     }
@@ -620,39 +746,32 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
     if (w1 && b1 <= target && target < b1 + w1)
       answer(static_cast<uint32_t>(f1 >> 32), __uint_as_float(static_cast<uint32_t>(f1)));
   };
-  // The key of the last token a cut keeps, when it falls into step c.bin:
-  // the first at which the count (mass) reaches `want`; `mass` gets what is
-  // kept in all.  Steps with more tokens than the list are halved 2^11-fold by
-  // key until they fit.
+  // The key of the last token a cut keeps, when it falls into step c.bin: the
+  // first at which the count (mass) reaches `want`; `mass` gets what is kept in
+  // all.  Steps with more tokens than the list are divided 2^11-fold by key
+  // until they fit.
   auto settle = [&](Cut c, bool by_mass, u64 want, u64 limit_key, bool masses, u64 *mass) -> u64 {
     const int bin = static_cast<int>(c.bin);
-    u64 lo = order_key(fmaxf(static_cast<float>(bin - 1), 0.f) / kBinsPerNat, 0);
+    u64 lo = order_key(fmaxf(static_cast<float>(bin - 2), 0.f) / kBinsPerNat, 0);
     u64 width = order_key(static_cast<float>(bin + 2) / kBinsPerNat, 0) - lo;
     auto in_reach = [&](float d, u64 key) {
       return bin_of(d) == bin && key <= limit_key && key >= lo && key - lo < width;
     };
     while (c.count > kList) {
       int shift = 0;
-      while ((width >> shift) > static_cast<u64>(kBins)) ++shift;
-      cluster_sync(nc);  // every CTA has read its peers' histograms
-      for (int i = t; i < 3 * kBins / 4; i += kThreads) reinterpret_cast<uint4 *>(S.count)[i] = make_uint4(0, 0, 0, 0);
+      while ((width >> shift) > static_cast<u64>(kBins - 1)) ++shift;
+      cluster_sync(nc);  // every CTA has read its peers' steps
+      clear_steps();
       __syncthreads();
-      for (int i = t; i < nvec; i += kThreads) {
+      for (int i = v0 + lane; i < v1; i += 32) {
         const V v(data[i]);
 #pragma unroll
         for (int j = 0; j < kVN; ++j) {
           const float d = dist(v.v[j], m, R.inv_t);
           const u64 key = order_key(d, begin + i * kVN + j);
-          if (!(d < 28.44f) || !in_reach(d, key)) continue;
+          if (!(d < kFar) || !in_reach(d, key)) continue;
           const u64 w = weight(d);
-          const int b = static_cast<int>(min((key - lo) >> shift, static_cast<u64>(kBins - 1)));
-          if (w == 0) continue;
-          atomicAdd(&S.count[b], 1u);
-          if (masses) {
-            const uint32_t wl = static_cast<uint32_t>(w), old = atomicAdd(&S.lo[b], wl);
-            const uint32_t wh = static_cast<uint32_t>(w >> 32) + (old + wl < old ? 1u : 0u);
-            if (wh) atomicAdd(&S.hi[b], wh);
-          }
+          if (w) count_step(static_cast<int>((key - lo) >> shift), w, masses);
         }
       }
       const u64 cb = c.count_before, mb = c.mass_before;
@@ -664,50 +783,86 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
       lo += c.bin << shift;
       width = u64(1) << shift;
     }
-    if (t == 0 && rank == 0) S.list_n = 0;
+    if (t == 0) S.list_n = 0, S.local_n = 0;
     cluster_sync(nc);
-    collect([&](float d, u64 key) { return in_reach(d, key) && weight(d) != 0; });
-    cluster_sync(nc);
+    const int len = static_cast<int>(min(collect(in_reach), static_cast<u64>(kList)));
     if (rank == 0) {
-      const int len = sorted();
-      const u64 k0 = 2 * t < len ? S.list[2 * t] : ~0ull, k1 = 2 * t + 1 < len ? S.list[2 * t + 1] : ~0ull;
-      const u64 w0 = 2 * t < len ? weight(key_dist(k0)) : 0, w1 = 2 * t + 1 < len ? weight(key_dist(k1)) : 0;
-      u64 b0, b1, all;
-      list_scan(w0, w1, b0, b1, all);
       const u64 left = want - (by_mass ? c.mass_before : c.count_before);  // at least 1
       auto tell = [&](u64 key, u64 through) {
         for (int x = 0; x < nc; ++x) {
           peer_st(peer(&S.pick, x), key);
-          peer_st(peer(&S.slot[0], x), c.mass_before + through);
+          peer_st(peer(&S.cut.mass, x), c.mass_before + through);
         }
       };
-      if (by_mass ? (w0 && b0 < left && left <= b0 + w0) : static_cast<u64>(2 * t + 1) == left) tell(k0, b0 + w0);
-      if (by_mass ? (w1 && b1 < left && left <= b1 + w1) : static_cast<u64>(2 * t + 2) == left) tell(k1, b1 + w1);
+      if (len <= kFew) {
+        for (int i = t; i < len; i += kThreads) S.few[0][i] = weight(key_dist(S.list[i]));
+        __syncthreads();
+        const int e = t / kPer;
+        const u64 key = e < len ? S.list[e] : ~0ull, w = e < len ? S.few[0][e] : 0;
+        u64 before, all;
+        const int place = rank_few(len, key, &before, &all);
+        if (t % kPer == 0 && e < len &&
+            (by_mass ? before < left && left <= before + w : static_cast<u64>(place + 1) == left))
+          tell(key, before + w);
+      } else {
+        sort_by_key(len);
+        const u64 k0 = 2 * t < len ? S.list[2 * t] : ~0ull, k1 = 2 * t + 1 < len ? S.list[2 * t + 1] : ~0ull;
+        const u64 w0 = 2 * t < len ? weight(key_dist(k0)) : 0, w1 = 2 * t + 1 < len ? weight(key_dist(k1)) : 0;
+        u64 b0, b1, all;
+        list_scan(w0, w1, b0, b1, all);
+        if (by_mass ? (w0 && b0 < left && left <= b0 + w0) : static_cast<u64>(2 * t + 1) == left) tell(k0, b0 + w0);
+        if (by_mass ? (w1 && b1 < left && left <= b1 + w1) : static_cast<u64>(2 * t + 2) == left) tell(k1, b1 + w1);
+      }
     }
     cluster_sync(nc);
-    *mass = S.slot[0];
+    *mass = S.cut.mass;
     return S.pick;
   };
 
   u64 cut = ~0ull;
+  if (cut_k) {
+    // From the threads' largest logits: a step at or beyond the one where the cut falls.
+    gather_bins(false);
+    if (counted() >= static_cast<u64>(R.k)) {
+      const int last = static_cast<int>(find(false, static_cast<u64>(R.k)).bin);
+      const u64 len = collect([&](float d, u64) { return bin_of(d) <= last; });
+      if (len <= kList) {
+        if (rank == 0) finish_list(static_cast<int>(len), static_cast<u64>(R.k), cut_p, 0);
+        return;
+      }
+    }
+    // Too many, or k above the number of threads: the steps of all tokens.
+    cluster_sync(nc);
+    clear_steps();
+    if (t == 0) S.list_n = 0, S.local_n = 0;
+    __syncthreads();
+    u64 all = 0;
+    for (int i = v0 + lane; i < v1; i += 32) {
+      const V v(data[i]);
+#pragma unroll
+      for (int j = 0; j < kVN; ++j) {
+        const float d = dist(v.v[j], m, R.inv_t);
+        const u64 w = weight(d);
+        all += w;
+        if (w) count_step(bin_of(d), w, cut_p);
+      }
+    }
+    all = sum_block(all, S.red);
+    if (t < nc) peer_st(peer(&S.total[rank], t), all);
+    cluster_sync(nc);
+    total = 0;
+    for (int c = 0; c < nc; ++c) total += S.total[c];
+  }
   if (cut_k || cut_p) {
     gather_bins(cut_p);
-    u64 found = 0;
-    for (int x = 0; x < nc; ++x) found += S.slice_count[x];
     u64 mk = total;
     const u64 c0 = pre_c, m0 = pre_m;
     uint32_t bc0[4];
     u64 bm0[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) bc0[j] = bc[j], bm0[j] = bm[j];
-    if (cut_k && static_cast<u64>(R.k) < found) {
+    if (cut_k && static_cast<u64>(R.k) < counted()) {
       const Cut c = find(false, static_cast<u64>(R.k));
-      if (c.count_before + c.count <= kList) {
-        collect([&](float d, u64) { return bin_of(d) <= static_cast<int>(c.bin) && weight(d) != 0; });
-        cluster_sync(nc);
-        if (rank == 0) finish_list(static_cast<u64>(R.k), cut_p, 0);
-        return;
-      }
       cut = settle(c, false, static_cast<u64>(R.k), ~0ull, cut_p, &mk);
     }
     if (cut_p) {
@@ -718,12 +873,11 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
       for (int j = 0; j < 4; ++j) bc[j] = bc0[j], bm[j] = bm0[j];
       cluster_sync(nc);  // S.cut has been read by all
       const Cut c = find(true, limit);
-      if (c.count_before + c.count <= kList) {
-        if (t == 0 && rank == 0) S.list_n = 0;
+      if (c.count_before + c.count <= kFew) {  // longer lists cost more than the passes below
+        if (t == 0) S.list_n = 0, S.local_n = 0;
         cluster_sync(nc);
-        collect([&](float d, u64 key) { return bin_of(d) <= static_cast<int>(c.bin) && key <= cut && weight(d) != 0; });
-        cluster_sync(nc);
-        if (rank == 0) finish_list(~0ull, true, mk);
+        const u64 len = collect([&](float d, u64 key) { return bin_of(d) <= static_cast<int>(c.bin) && key <= cut; });
+        if (rank == 0) finish_list(static_cast<int>(min(len, static_cast<u64>(kList))), ~0ull, true, mk);
         return;
       }
       u64 unused;
@@ -732,40 +886,38 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
   }
 
   // ---- what is kept, in place: its mass a warp, and the walk ----
-  const int v0 = static_cast<int>(static_cast<int64_t>(nvec) * warp / kWarps);
-  const int v1 = static_cast<int>(static_cast<int64_t>(nvec) * (warp + 1) / kWarps);
   auto kept = [&](float l, int index, float *dd) -> u64 {
     const float d = dist(l, m, R.inv_t);
     const u64 w = weight(d);
     *dd = d;
     return w >= R.least && order_key(d, index) <= cut ? w : 0;
   };
-  u64 mine = 0;
   float d;
-  for (int i = v0 + lane; i < v1; i += 32) {
-    const V v(data[i]);
+  if (cut_k || cut_p) {
+    u64 mine = 0;
+    for (int i = v0 + lane; i < v1; i += 32) {
+      const V v(data[i]);
 #pragma unroll
-    for (int j = 0; j < kVN; ++j) mine += kept(v.v[j], begin + i * kVN + j, &d);
+      for (int j = 0; j < kVN; ++j) mine += kept(v.v[j], begin + i * kVN + j, &d);
+    }
+    mine = warp_sum(mine);
+    if (lane == 0) S.warp_kept[warp] = mine;
+    __syncthreads();
+    if (t < nc) {
+      u64 all = 0;
+      for (int w = 0; w < kWarps; ++w) all += S.warp_kept[w];
+      peer_st(peer(&S.kept[rank], t), all);
+    }
+    cluster_sync(nc);
   }
-  mine = warp_sum(mine);
-  __syncthreads();
-  if (lane == 0) S.red[warp] = mine;
-  __syncthreads();
-  u64 before = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += S.red[w];
-    all += S.red[w];
-  }
-  if (t < nc) peer_st(peer(&S.kept[rank], t), all);
-  cluster_sync(nc);
-  u64 mass = 0;
+  u64 before = 0, mass = 0;
+  for (int w = 0; w < warp; ++w) before += S.warp_kept[w];
   for (int c = 0; c < nc; ++c) {
     if (c < rank) before += S.kept[c];
     mass += S.kept[c];
   }
   const u64 target = draw_target(R.u, mass);
-  if (before <= target && target < before + mine) {  // one warp of the cluster
+  if (before <= target && target < before + S.warp_kept[warp]) {  // one warp of the cluster
     for (int i0 = v0; i0 < v1; i0 += 32) {
       const int i = i0 + lane;
       u64 own = 0;
@@ -774,10 +926,14 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
 #pragma unroll
         for (int j = 0; j < kVN; ++j) own += kept(v.v[j], begin + i * kVN + j, &d);
       }
-      const u64 inc = warp_scan(own, lane), start = before + inc - own;
-      if (i < v1 && start <= target && target < start + own) {
+      const u64 all = warp_sum(own);
+      if (before + all <= target) {
+        before += all;
+        continue;
+      }
+      u64 at = before + warp_scan(own, lane) - own;
+      if (i < v1 && at <= target && target < at + own) {
         const V v(data[i]);
-        u64 at = start;
 #pragma unroll
         for (int j = 0; j < kVN; ++j) {
           const u64 w = kept(v.v[j], begin + i * kVN + j, &d);
@@ -785,12 +941,10 @@ __global__ void __launch_bounds__(kThreads) sample_cluster_kernel(const SampleAr
           at += w;
         }
       }
-      before += __shfl_sync(0xffffffffu, inc, 31);
-      if (before > target) break;
+      break;
     }
   }
 }
-
 
 constexpr int kSampleSmemMax = 227 * 1024;
 
@@ -802,13 +956,14 @@ size_t sample_smem(int64_t slice, int size) {
 template <int DT>
 int launch_sample_typed(const SampleArgs &a, cudaStream_t s) {
   const int size = DT == H24_DTYPE_F32 ? 4 : 2;
+  // The fewest CTAs a row with which two CTAs fit an SM and two an SM are
+  // there, as long as a CTA's slice has 2,048 logits.
   int nc = 1;
   int64_t slice = 0;
   for (;; nc *= 2) {
     slice = ((a.vocab + nc - 1) / nc + 15) / 16 * 16;
-    const bool fits = sample_smem(slice, size) <= kSampleSmemMax;
-    if (fits && (nc == kMaxCluster || a.rows * nc >= 296 || slice <= 2048)) break;
-    if (nc == kMaxCluster) break;
+    if (nc == kMaxCluster || slice <= 2048) break;
+    if (sample_smem(slice, size) <= kSampleSmemMax / 2 - 1024 && a.rows * nc >= 296) break;
   }
   if (sample_smem(slice, size) > kSampleSmemMax || a.rows * nc > INT32_MAX) {
     sample_rows_kernel<DT><<<wave_grid(a.rows, 2), kSampleThreads, 0, s>>>(a);
