@@ -30,6 +30,8 @@
 // non-negative floats ascend with them).  A selection is then a cut on that
 // key, found by histograms of its digits.
 #include "h24_internal.cuh"
+#include <cstdlib>
+#define MANYROWS (std::getenv("MANY") ? atoi(std::getenv("MANY")) : 148)
 
 namespace h24 {
 namespace {
@@ -37,7 +39,7 @@ namespace {
 using u64 = unsigned long long;
 
 constexpr float kOne = 1099511627776.0f;  // 2^40
-constexpr int kSampleThreads = 1024;
+constexpr float kLargest = 3.402823466e38f;
 
 struct SampleArgs {
   const void *logits;
@@ -53,34 +55,26 @@ struct SampleArgs {
   float *logprobs;
 };
 
-template <int DT>
-__device__ __forceinline__ float logit_at(const void *row, int64_t i) {
-  float v;
-  if (DT == H24_DTYPE_F32)
-    v = __ldg(static_cast<const float *>(row) + i);
-  else if (DT == H24_DTYPE_F16)
-    v = __half2float(static_cast<const __half *>(row)[i]);
-  else
-    v = __bfloat162float(static_cast<const __nv_bfloat16 *>(row)[i]);
-  return v == v ? v : -INFINITY;  // NaN: never chosen
-}
+// |z| of a logit; m is finite and inv_t within fp32's normal range.  l = m
+// gives 0, -inf gives inf, NaN gives NaN (which no comparison lets pass), and
+// +inf, which counts as the largest number, gives -inf: see near().
+__device__ __forceinline__ float dist(float l, float m, float inv_t) { return __fmul_rn(__fsub_rn(m, l), inv_t); }
+__device__ __forceinline__ float near(float d) { return fmaxf(d, 0.f); }  // of a d that has passed a comparison
 
-// |z| of a logit.
-__device__ __forceinline__ float dist(float l, float m, float inv_t) {
-  const float d = fabsf(__fmul_rn(__fsub_rn(l, m), inv_t));
-  return l == m ? 0.f : (d == d ? d : INFINITY);  // NaN: a masked logit at an infinite temperature
+// A weight from f = exp(-d) * 2^40.  Below 2^32 (|z| above 5.5, nearly every
+// token) one conversion; from there the float is an integer, its mantissa
+// shifted.  (A 64-bit conversion, or integer steps for both ranges, cost more
+// issue slots.)
+__device__ __forceinline__ float scaled(float d) { return expf(-d) * kOne; }
+__device__ __forceinline__ u64 to_weight(float f) {
+  u64 w = __float2uint_rn(f);
+  if (f >= 4294967040.0f) {
+    const uint32_t bits = __float_as_uint(fminf(f, kOne));
+    w = static_cast<u64>((bits & 0x7FFFFFu) | 0x800000u) << ((bits >> 23) - 150);
+  }
+  return w;
 }
-
-// rint(exp(-d) * 2^40) without a 64-bit conversion: from 2^23 on a float is an
-// integer, its mantissa shifted; below, adding 2^23 leaves the nearest (even)
-// integer in the low bits.
-__device__ __forceinline__ u64 weight(float d) {
-  const float f = expf(-d) * kOne;
-  const uint32_t bits = __float_as_uint(f);
-  const int shift = static_cast<int>(bits >> 23) - 150;
-  const uint32_t small = __float_as_uint(f + 8388608.0f) - 0x4B000000u;
-  return shift >= 0 ? static_cast<u64>((bits & 0x7FFFFFu) | 0x800000u) << shift : small;
-}
+__device__ __forceinline__ u64 weight(float d) { return to_weight(scaled(d)); }
 
 constexpr int kIndexBits = 22;
 __device__ __forceinline__ u64 order_key(float d, int64_t i) {
@@ -103,135 +97,6 @@ __device__ __forceinline__ u64 draw_target(float u, u64 mass) {
   return x >= static_cast<double>(mass - 1) ? mass - 1 : static_cast<u64>(x);
 }
 
-__device__ u64 block_sum(u64 v, u64 *red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  u64 r = 0;
-  for (int w = 0; w < kSampleThreads / 32; ++w) r += red[w];
-  __syncthreads();
-  return r;
-}
-
-// A block per row; every step reads the row again.  For vocabularies whose row
-// does not fit the shared memory of a cluster.
-template <int DT>
-__global__ void __launch_bounds__(kSampleThreads) sample_rows_kernel(const SampleArgs a) {
-  __shared__ u64 hist[256], red[32], sh_digit, sh_left;
-  __shared__ float redf[32];
-  const int t = threadIdx.x;
-  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    const uint8_t *row = static_cast<const uint8_t *>(a.logits) + r * a.stride * (DT == H24_DTYPE_F32 ? 4 : 2);
-    float temp = a.temperature ? a.temperature[r] : a.temperature1;
-    int64_t k = a.top_k ? a.top_k[r] : a.top_k1;
-    const float p = a.top_p ? a.top_p[r] : a.top_p1;
-    const float min_p = a.min_p ? a.min_p[r] : a.min_p1;
-    if (!(temp > 0.f)) temp = 1.f, k = 1;
-    const float inv_t = __fdiv_rn(1.0f, temp);
-    float m = -INFINITY;
-    for (int64_t i = t; i < a.vocab; i += kSampleThreads) m = fmaxf(m, logit_at<DT>(row, i));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((t & 31) == 0) redf[t >> 5] = m;
-    __syncthreads();
-    for (int w = 0; w < kSampleThreads / 32; ++w) m = fmaxf(m, redf[w]);
-    __syncthreads();
-    if (m == -INFINITY) {  // nothing to choose from
-      if (t == 0) {
-        a.tokens[r] = -1;
-        if (a.logprobs) a.logprobs[r] = -INFINITY;
-      }
-      continue;
-    }
-    u64 sum = 0;
-    for (int64_t i = t; i < a.vocab; i += kSampleThreads) sum += weight(dist(logit_at<DT>(row, i), m, inv_t));
-    const u64 total = block_sum(sum, red);
-
-    // The key of the last element kept: the first at which the count (by_mass
-    // false) or the mass of the order up to and with it reaches `want`, among
-    // keys <= cut.
-    u64 cut = ~0ull;
-    auto select = [&](bool by_mass, u64 want) {
-      u64 prefix = 0, left = want;
-      for (int shift = 56; shift >= 0; shift -= 8) {
-        for (int i = t; i < 256; i += kSampleThreads) hist[i] = 0;
-        __syncthreads();
-        for (int64_t i = t; i < a.vocab; i += kSampleThreads) {
-          const float d = dist(logit_at<DT>(row, i), m, inv_t);
-          const u64 key = order_key(d, i);
-          if (key <= cut && (shift == 56 || (key >> (shift + 8)) == prefix))
-            atomicAdd(&hist[(key >> shift) & 255], by_mass ? weight(d) : 1ull);
-        }
-        __syncthreads();
-        if (t == 0) {
-          int b = 0;
-          u64 l = left;
-          while (b < 255 && hist[b] < l) l -= hist[b++];
-          sh_digit = b;
-          sh_left = l;
-        }
-        __syncthreads();
-        prefix = (prefix << 8) | sh_digit;
-        left = sh_left;
-        __syncthreads();
-      }
-      cut = prefix;
-    };
-    u64 mk = total;
-    if (k > 0 && k < a.vocab) {
-      select(false, static_cast<u64>(k));
-      sum = 0;
-      for (int64_t i = t; i < a.vocab; i += kSampleThreads) {
-        const float d = dist(logit_at<DT>(row, i), m, inv_t);
-        if (order_key(d, i) <= cut) sum += weight(d);
-      }
-      mk = block_sum(sum, red);
-    }
-    if (p < 1.f) select(true, mass_limit(p, mk));
-    const u64 least = weight_floor(min_p);
-    auto kept = [&](int64_t i) -> u64 {
-      const float d = dist(logit_at<DT>(row, i), m, inv_t);
-      const u64 w = weight(d);
-      return order_key(d, i) <= cut && w >= least ? w : 0ull;
-    };
-    sum = 0;
-    for (int64_t i = t; i < a.vocab; i += kSampleThreads) sum += kept(i);
-    const u64 target = draw_target(a.u[r], block_sum(sum, red));
-    // The running mass, a block's width of indices at a time.
-    u64 base = 0;
-    for (int64_t i0 = 0; i0 < a.vocab; i0 += kSampleThreads) {
-      const int64_t i = i0 + t;
-      const u64 w = i < a.vocab ? kept(i) : 0ull;
-      u64 run = w;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const u64 up = __shfl_up_sync(0xffffffffu, run, o);
-        if ((t & 31) >= o) run += up;
-      }
-      if ((t & 31) == 31) red[t >> 5] = run;
-      __syncthreads();
-      u64 before = base, all = base;
-      for (int j = 0; j < kSampleThreads / 32; ++j) {
-        if (j < (t >> 5)) before += red[j];
-        all += red[j];
-      }
-      run += before;
-      if (w && run > target && run - w <= target) {
-        a.tokens[r] = i;
-        if (a.logprobs)
-          a.logprobs[r] = -dist(logit_at<DT>(row, i), m, inv_t) -
-                          logf(static_cast<float>(static_cast<double>(total) / static_cast<double>(kOne)));
-      }
-      base = all;
-      __syncthreads();
-      if (base > target) break;
-    }
-    __syncthreads();
-  }
-}
-
-
 // ---------------------------------------------------------------------------
 // distributed shared memory of the cluster
 // ---------------------------------------------------------------------------
@@ -253,6 +118,9 @@ __device__ __forceinline__ uint4 peer_ld4(uint32_t addr) {
 }
 __device__ __forceinline__ void peer_st(uint32_t addr, u64 v) {
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
+}
+__device__ __forceinline__ void peer_add64(uint32_t addr, u64 v) {
+  asm volatile("red.shared::cluster.add.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
 __device__ __forceinline__ uint32_t peer_add(uint32_t addr, uint32_t v) {
   uint32_t r;
@@ -280,12 +148,15 @@ struct SampleShared {
   u64 slice_count[kMaxCluster], slice_mass[kMaxCluster];
   u64 total[kMaxCluster], first[kMaxCluster], kept[kMaxCluster];
   Cut cut;
-  u64 scan_c[kWarps], scan_m[kWarps];
+  u64 scan_m[kWarps];
+  uint32_t step_c[kWarps], warp_first[kWarps];
   u64 warp_total[kWarps], warp_kept[kWarps];
   u64 red[kWarps];
   u64 pick;
-  uint32_t list_n, local_n;
+  uint32_t list_n, local_n, base;
 };
+
+static_assert(kList * 8 <= kBins * 4, "a CTA's own list lies over one word of the steps");
 
 __device__ __forceinline__ void cluster_sync(int c) {
   if (c == 1) {
@@ -301,10 +172,11 @@ __device__ __forceinline__ u64 warp_sum(u64 v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-__device__ __forceinline__ u64 warp_scan(u64 v, int lane) {  // inclusive
+template <typename T>
+__device__ __forceinline__ T warp_scan(T v, int lane) {  // inclusive
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const u64 up = __shfl_up_sync(0xffffffffu, v, o);
+    const T up = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += up;
   }
   return v;
@@ -320,7 +192,7 @@ __device__ u64 sum_block(u64 v, u64 *red) {
   return r;
 }
 
-// The elements of one 16-byte vector of a slice, NaN as -inf.
+// The elements of one 16-byte vector of a slice.
 template <int DT>
 struct Vec {
   static constexpr int kN = DT == H24_DTYPE_F32 ? 4 : 8;
@@ -340,8 +212,6 @@ struct Vec {
         v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
       }
     }
-#pragma unroll
-    for (int i = 0; i < kN; ++i) v[i] = v[i] == v[i] ? v[i] : -INFINITY;
   }
 };
 
@@ -369,8 +239,8 @@ struct RowSettings {
   u64 least;
 };
 
-template <int DT>
-__global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const SampleArgs a, int nc, int slice) {
+template <int DT, bool kHeld>
+__global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel(const SampleArgs a, int nc, int slice) {
   using V = Vec<DT>;
   constexpr int kVN = V::kN, kSize = DT == H24_DTYPE_F32 ? 4 : 2;
   extern __shared__ __align__(16) uint8_t sample_raw[];
@@ -403,29 +273,46 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
     R.u = a.u[r];
     if (!(temp > 0.f)) temp = 1.f, R.k = 1;
     if (R.k <= 0 || R.k > a.vocab) R.k = a.vocab;
-    R.inv_t = __fdiv_rn(1.0f, temp);
+    R.inv_t = fminf(fmaxf(__fdiv_rn(1.0f, temp), 1.17549435e-38f), kLargest);
   }
 
-  // ---- the slice into shared memory; each thread's and the row's largest logit ----
+  // ---- the slice into shared memory (kHeld; else it is read again in each
+  // pass, from L2); each thread's and the row's largest logit ----
   const uint8_t *src = static_cast<const uint8_t *>(a.logits) + (r * a.stride + begin) * kSize;
   float mine_max = -INFINITY;
   const int nfull = aligned16(src) ? n / kVN : 0;  // vectors that can be loaded whole
+  // Vector i by the element, -inf past the slice's end.
+  auto pieces = [&](int i) -> uint4 {
+    alignas(16) uint8_t raw[16];
+#pragma unroll
+    for (int j = 0; j < kVN; ++j) {
+      const int e = i * kVN + j;
+      if (DT == H24_DTYPE_F32)
+        reinterpret_cast<float *>(raw)[j] = e < n ? reinterpret_cast<const float *>(src)[e] : -INFINITY;
+      else
+        reinterpret_cast<uint16_t *>(raw)[j] = e < n ? reinterpret_cast<const uint16_t *>(src)[e]
+                                                    : static_cast<uint16_t>(DT == H24_DTYPE_F16 ? 0xFC00 : 0xFF80);
+    }
+    return *reinterpret_cast<const uint4 *>(raw);
+  };
+  auto at = [&](int i) -> V {
+    if (kHeld) return V(data[i]);
+    return V(i < nfull ? __ldcg(reinterpret_cast<const uint4 *>(src) + i) : pieces(i));
+  };
 #pragma unroll 4
   for (int i = t; i < nfull; i += kThreads) {
-    const uint4 raw = __ldcs(reinterpret_cast<const uint4 *>(src) + i);
-    data[i] = raw;
+    const uint4 raw = kHeld ? __ldcs(reinterpret_cast<const uint4 *>(src) + i) : __ldcg(reinterpret_cast<const uint4 *>(src) + i);
+    if (kHeld) data[i] = raw;
     const V v(raw);
 #pragma unroll
     for (int j = 0; j < kVN; ++j) mine_max = fmaxf(mine_max, v.v[j]);
   }
-  // The rest by the element, padded with -inf to a whole vector.
-  for (int i = nfull * kVN + t; i < nvec * kVN; i += kThreads) {
-    if (DT == H24_DTYPE_F32)
-      reinterpret_cast<float *>(data)[i] = i < n ? reinterpret_cast<const float *>(src)[i] : -INFINITY;
-    else
-      reinterpret_cast<uint16_t *>(data)[i] = i < n ? reinterpret_cast<const uint16_t *>(src)[i]
-                                                   : static_cast<uint16_t>(DT == H24_DTYPE_F16 ? 0xFC00 : 0xFF80);
-    if (i < n) mine_max = fmaxf(mine_max, logit_at<DT>(src, i));
+  for (int i = nfull + t; i < nvec; i += kThreads) {
+    const uint4 raw = pieces(i);
+    if (kHeld) data[i] = raw;
+    const V v(raw);
+#pragma unroll
+    for (int j = 0; j < kVN; ++j) mine_max = fmaxf(mine_max, v.v[j]);
   }
   float mx = mine_max;
 #pragma unroll
@@ -441,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
     cluster_sync(nc);
     for (int c = 0; c < nc; ++c) mx = fmaxf(mx, __uint_as_float(static_cast<uint32_t>(S.slot[c])));
   }
-  const float m = mx;
+  const float m = fminf(mx, kLargest);
   if (m == -INFINITY) {  // nothing to choose from (the same for the whole cluster)
     if (rank == 0 && t == 0) {
       a.tokens[r] = -1;
@@ -465,28 +352,59 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
   // of the mass together, so the cut at p falls before them.
   const bool steps_of_all = cut_p && !cut_k;
   const float far = steps_of_all ? fminf(kFar, logf(4.0f * static_cast<float>(a.vocab) / (1.0f - R.p)) + 0.01f) : 0.f;
+  const bool floor_counts = !greedy && !cut_k && !cut_p && R.least > 1;  // what min-p leaves is not the total
   if (a.logprobs || !cut_k) {
     u64 total = 0, kept = 0;
     uint32_t first = 0xFFFFFFFFu;
-    for (int i = v0 + lane; i < v1; i += 32) {
-      const V v(data[i]);
+    // Four or eight weights that are all below 2^29 (nearly always) add up in 32 bits.
+    auto pass = [&](auto each) {
+      for (int i = v0 + lane; i < v1; i += 32) {
+        const V v = at(i);
+        float d[kVN], f[kVN], top = 0.f;
 #pragma unroll
-      for (int j = 0; j < kVN; ++j) {
-        const float d = dist(v.v[j], m, R.inv_t);
-        const u64 w = weight(d);
-        total += w;
-        if (w >= R.least) kept += w;
-        if (greedy && v.v[j] == m) first = min(first, static_cast<uint32_t>(begin + i * kVN + j));
-        if (steps_of_all && d < far) count_step(bin_of(d), w, true);
+        for (int j = 0; j < kVN; ++j) {
+          d[j] = dist(v.v[j], m, R.inv_t);
+          f[j] = scaled(d[j]);
+          top = fmaxf(top, f[j]);
+        }
+        if (top < 536870912.0f) {
+          uint32_t sum = 0;
+#pragma unroll
+          for (int j = 0; j < kVN; ++j) {
+            const uint32_t w = __float2uint_rn(f[j]);
+            sum += w;
+            each(i, j, v.v[j], d[j], w);
+          }
+          total += sum;
+        } else {
+#pragma unroll
+          for (int j = 0; j < kVN; ++j) {
+            const u64 w = to_weight(f[j]);
+            total += w;
+            each(i, j, v.v[j], d[j], w);
+          }
+        }
       }
-    }
+    };
+    if (steps_of_all)
+      pass([&](int, int, float, float d, u64 w) {
+        if (d < far) count_step(bin_of(near(d)), w, true);
+      });
+    else if (greedy)
+      pass([&](int i, int j, float l, float, u64) {
+        if (l >= m) first = min(first, static_cast<uint32_t>(begin + i * kVN + j));
+      });
+    else if (floor_counts)
+      pass([&](int, int, float, float, u64 w) { kept += w >= R.least ? w : 0; });
+    else
+      pass([](int, int, float, float, u64) {});
     total = warp_sum(total);
-    kept = warp_sum(kept);
-    first = __reduce_min_sync(0xffffffffu, first);
+    kept = floor_counts ? warp_sum(kept) : total;
+    if (greedy) first = __reduce_min_sync(0xffffffffu, first);
     if (lane == 0) {
       S.warp_total[warp] = total;
       S.warp_kept[warp] = kept;
-      S.scan_c[warp] = first;
+      S.warp_first[warp] = first;
     }
   } else if (lane == 0) {
     S.warp_total[warp] = 0;
@@ -494,21 +412,19 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
   // The k-th largest of the threads' largest logits is at most the k-th
   // largest logit: the steps of those alone give a bound on the cut at k.
   if (cut_k) {
-    const float d = dist(mine_max, m, R.inv_t);
+    const float d = near(dist(mine_max, m, R.inv_t));
     if (d < kFar && weight(d)) atomicAdd(&S.count[bin_of(d)], 1u);
   }
   __syncthreads();
-  if (t < nc) {
-    u64 tot = 0, kep = 0, fir = ~0ull;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      tot += S.warp_total[w];
-      kep += S.warp_kept[w];
-      fir = min(fir, S.scan_c[w]);
+  if (warp == 0) {
+    const u64 tot = warp_sum(lane < kWarps ? S.warp_total[lane] : 0);
+    const u64 kep = floor_counts ? warp_sum(lane < kWarps ? S.warp_kept[lane] : 0) : tot;
+    const uint32_t fir = greedy ? __reduce_min_sync(0xffffffffu, lane < kWarps ? S.warp_first[lane] : 0xFFFFFFFFu) : 0;
+    if (lane < nc) {
+      peer_st(peer(&S.total[rank], lane), tot);
+      peer_st(peer(&S.kept[rank], lane), kep);
+      if (greedy) peer_st(peer(&S.first[rank], lane), fir);
     }
-    peer_st(peer(&S.total[rank], t), tot);
-    peer_st(peer(&S.kept[rank], t), kep);
-    peer_st(peer(&S.first[rank], t), fir);
   }
   cluster_sync(nc);
   u64 total = 0;
@@ -532,7 +448,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
   // them (of the whole row).
   const int share = kBins / nc, my_bin = rank * share + t / nc * 4;
   uint32_t bc[4];
-  u64 bm[4], pre_c = 0, pre_m = 0;
+  uint32_t pre_c = 0;
+  u64 bm[4], pre_m = 0;
   auto gather_bins = [&](bool masses) {
     const int x = t & (nc - 1);
     const uint4 c4 = peer_ld4(peer(&S.count[my_bin], x));
@@ -553,18 +470,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
         if (masses) bm[j] += __shfl_xor_sync(0xffffffffu, bm[j], o);
       }
     }
-    const u64 c = static_cast<u64>(bc[0]) + bc[1] + bc[2] + bc[3], q = bm[0] + bm[1] + bm[2] + bm[3];
-    const u64 ic = warp_scan(x == 0 ? c : 0, lane), im = masses ? warp_scan(x == 0 ? q : 0, lane) : 0;
-    if (lane == 31) S.scan_c[warp] = ic, S.scan_m[warp] = im;
+    const uint32_t c = bc[0] + bc[1] + bc[2] + bc[3];
+    const u64 q = bm[0] + bm[1] + bm[2] + bm[3];
+    const uint32_t ic = warp_scan(x == 0 ? c : 0u, lane);
+    const u64 im = masses ? warp_scan(x == 0 ? q : u64(0), lane) : 0;
+    if (lane == 31) S.step_c[warp] = ic, S.scan_m[warp] = im;
     __syncthreads();
     pre_c = ic - c;
     pre_m = im - q;
-    u64 all_c = 0, all_m = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) pre_c += S.scan_c[w], pre_m += S.scan_m[w];
-      all_c += S.scan_c[w];
-      all_m += S.scan_m[w];
+    // Warps before this one, and all of them.
+    const uint32_t wc = lane < kWarps ? S.step_c[lane] : 0u;
+    pre_c += __reduce_add_sync(0xffffffffu, lane < warp ? wc : 0u);
+    const uint32_t all_c = __reduce_add_sync(0xffffffffu, wc);
+    u64 all_m = 0;
+    if (masses) {
+      const u64 wm = lane < kWarps ? S.scan_m[lane] : 0;
+      pre_m += warp_sum(lane < warp ? wm : 0);
+      all_m = warp_sum(wm);
     }
     if (t < nc) {
       peer_st(peer(&S.slice_count[rank], t), all_c);
@@ -602,33 +524,51 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
     cluster_sync(nc);
     return S.cut;
   };
-  // Keys that satisfy `wanted` go to the first CTA's list (as many as fit);
-  // returns their number in the cluster.  Starts and ends with the cluster in
-  // step; S.list_n and S.local_n are zero at the start.
-  auto collect = [&](auto wanted) -> u64 {
-    const uint32_t counter = peer(&S.list_n, 0), list0 = peer(&S.list[0], 0);
+  // Of the tokens of steps up to `last`: keys that satisfy `wanted` go to the first CTA's list (as many as fit);
+  // returns their number in the cluster.  Of those that satisfy `sure` before
+  // it, what min-p leaves is added up a warp.  Starts and ends with the cluster
+  // in step; S.list_n and S.local_n are zero at the start.
+  auto collect = [&](int last, auto sure, auto wanted) -> u64 {
+    const float bound = fminf(static_cast<float>(last + 1) / kBinsPerNat, kFar);  // a step ends half a step before
+    // First a list of this CTA's own, over the steps' masses (read by now).
+    u64 *own = nc == 1 ? S.list : reinterpret_cast<u64 *>(S.lo);
+    u64 mine = 0;
     for (int i = v0 + lane; i < v1; i += 32) {
-      const V v(data[i]);
+      const V v = at(i);
 #pragma unroll
       for (int j = 0; j < kVN; ++j) {
-        const float d = dist(v.v[j], m, R.inv_t);
-        if (d < kFar) {
+        float d = dist(v.v[j], m, R.inv_t);
+        if (d < bound) {
+          d = near(d);
           const u64 key = order_key(d, begin + i * kVN + j);
-          if (wanted(d, key) && weight(d)) {
-            atomicAdd(&S.local_n, 1u);
-            const uint32_t at = peer_add(counter, 1u);
-            if (at < kList) peer_st(list0 + at * 8, key);
+          if (bin_of(d) > last) continue;
+          if (sure(d, key)) {
+            const u64 w = weight(d);
+            mine += w >= R.least ? w : 0;
+          } else if (wanted(d, key) && weight(d)) {
+            const uint32_t place = atomicAdd(&S.local_n, 1u);
+            if (place < kList) own[place] = key;
           }
         }
       }
     }
+    mine = warp_sum(mine);
+    if (lane == 0) S.warp_kept[warp] = mine;
     __syncthreads();
-    if (t < nc) peer_st(peer(&S.slot[rank], t), S.local_n);
+    const uint32_t here = S.local_n;
+    if (nc == 1) return here;
+    if (t < nc) peer_st(peer(&S.slot[rank], t), here);
+    if (t == 0) S.base = peer_add(peer(&S.list_n, 0), here);
+    __syncthreads();
+    const uint32_t to = peer(&S.list[0], 0), base = S.base;
+    for (uint32_t i = t; i < min(here, static_cast<uint32_t>(kList)); i += kThreads)
+      if (base + i < kList) peer_st(to + (base + i) * 8, own[i]);
     cluster_sync(nc);
     u64 all = 0;
     for (int c = 0; c < nc; ++c) all += S.slot[c];
     return all;
   };
+  const auto none = [](float, u64) { return false; };
   auto sort_by_key = [&](int len) {
     int pow2 = 2;
     while (pow2 < len) pow2 <<= 1;
@@ -748,7 +688,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
   };
   // The key of the last token a cut keeps, when it falls into step c.bin: the
   // first at which the count (mass) reaches `want`; `mass` gets what is kept in
-  // all.  Steps with more tokens than the list are divided 2^11-fold by key
+  // all, S.warp_kept what min-p leaves of it in each warp's part.  Steps with more tokens than the list are divided 2^11-fold by key
   // until they fit.
   auto settle = [&](Cut c, bool by_mass, u64 want, u64 limit_key, bool masses, u64 *mass) -> u64 {
     const int bin = static_cast<int>(c.bin);
@@ -764,12 +704,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
       clear_steps();
       __syncthreads();
       for (int i = v0 + lane; i < v1; i += 32) {
-        const V v(data[i]);
+        const V v = at(i);
 #pragma unroll
         for (int j = 0; j < kVN; ++j) {
-          const float d = dist(v.v[j], m, R.inv_t);
+          float d = dist(v.v[j], m, R.inv_t);
+          if (!(d < kFar)) continue;
+          d = near(d);
           const u64 key = order_key(d, begin + i * kVN + j);
-          if (!(d < kFar) || !in_reach(d, key)) continue;
+          if (!in_reach(d, key)) continue;
           const u64 w = weight(d);
           if (w) count_step(static_cast<int>((key - lo) >> shift), w, masses);
         }
@@ -785,7 +727,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
     }
     if (t == 0) S.list_n = 0, S.local_n = 0;
     cluster_sync(nc);
-    const int len = static_cast<int>(min(collect(in_reach), static_cast<u64>(kList)));
+    const auto before_reach = [&](float d, u64 key) {
+      const int b = bin_of(d);
+      return b < bin || (b == bin && key < lo);
+    };
+    const int len = static_cast<int>(min(collect(bin, before_reach, in_reach), static_cast<u64>(kList)));
     if (rank == 0) {
       const u64 left = want - (by_mass ? c.mass_before : c.count_before);  // at least 1
       auto tell = [&](u64 key, u64 through) {
@@ -793,6 +739,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
           peer_st(peer(&S.pick, x), key);
           peer_st(peer(&S.cut.mass, x), c.mass_before + through);
         }
+      };
+      // A kept token of the list joins the sum of the warp that holds it.
+      auto keep = [&](u64 key, u64 w) {
+        if (w < R.least) return;
+        const int index = static_cast<int>(key_index(key)), cta = index / slice;
+        const int its = static_cast<int>(min(static_cast<int64_t>(slice), a.vocab - static_cast<int64_t>(cta) * slice));
+        const int vecs = (its + kVN - 1) / kVN, vec = (index - cta * slice) / kVN;
+        int w16 = static_cast<int>(static_cast<int64_t>(vec) * kWarps / vecs);
+        while (static_cast<int>(static_cast<int64_t>(vecs) * (w16 + 1) / kWarps) <= vec) ++w16;
+        peer_add64(peer(&S.warp_kept[w16], cta), w);
       };
       if (len <= kFew) {
         for (int i = t; i < len; i += kThreads) S.few[0][i] = weight(key_dist(S.list[i]));
@@ -804,6 +760,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
         if (t % kPer == 0 && e < len &&
             (by_mass ? before < left && left <= before + w : static_cast<u64>(place + 1) == left))
           tell(key, before + w);
+        if (t % kPer == 0 && e < len && (by_mass ? before < left : static_cast<u64>(place) < left)) keep(key, w);
       } else {
         sort_by_key(len);
         const u64 k0 = 2 * t < len ? S.list[2 * t] : ~0ull, k1 = 2 * t + 1 < len ? S.list[2 * t + 1] : ~0ull;
@@ -812,6 +769,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
         list_scan(w0, w1, b0, b1, all);
         if (by_mass ? (w0 && b0 < left && left <= b0 + w0) : static_cast<u64>(2 * t + 1) == left) tell(k0, b0 + w0);
         if (by_mass ? (w1 && b1 < left && left <= b1 + w1) : static_cast<u64>(2 * t + 2) == left) tell(k1, b1 + w1);
+        if (w0 && (by_mass ? b0 < left : static_cast<u64>(2 * t) < left)) keep(k0, w0);
+        if (w1 && (by_mass ? b1 < left : static_cast<u64>(2 * t + 1) < left)) keep(k1, w1);
       }
     }
     cluster_sync(nc);
@@ -825,7 +784,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
     gather_bins(false);
     if (counted() >= static_cast<u64>(R.k)) {
       const int last = static_cast<int>(find(false, static_cast<u64>(R.k)).bin);
-      const u64 len = collect([&](float d, u64) { return bin_of(d) <= last; });
+      const u64 len = collect(last, none, [](float, u64) { return true; });
       if (len <= kList) {
         if (rank == 0) finish_list(static_cast<int>(len), static_cast<u64>(R.k), cut_p, 0);
         return;
@@ -838,13 +797,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
     __syncthreads();
     u64 all = 0;
     for (int i = v0 + lane; i < v1; i += 32) {
-      const V v(data[i]);
+      const V v = at(i);
 #pragma unroll
       for (int j = 0; j < kVN; ++j) {
         const float d = dist(v.v[j], m, R.inv_t);
         const u64 w = weight(d);
         all += w;
-        if (w) count_step(bin_of(d), w, cut_p);
+        if (w) count_step(bin_of(near(d)), w, cut_p);
       }
     }
     all = sum_block(all, S.red);
@@ -856,7 +815,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
   if (cut_k || cut_p) {
     gather_bins(cut_p);
     u64 mk = total;
-    const u64 c0 = pre_c, m0 = pre_m;
+    const uint32_t c0 = pre_c;
+    const u64 m0 = pre_m;
     uint32_t bc0[4];
     u64 bm0[4];
 #pragma unroll
@@ -876,7 +836,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
       if (c.count_before + c.count <= kFew) {  // longer lists cost more than the passes below
         if (t == 0) S.list_n = 0, S.local_n = 0;
         cluster_sync(nc);
-        const u64 len = collect([&](float d, u64 key) { return bin_of(d) <= static_cast<int>(c.bin) && key <= cut; });
+        const u64 len = collect(static_cast<int>(c.bin), none, [&](float, u64 key) { return key <= cut; });
         if (rank == 0) finish_list(static_cast<int>(min(len, static_cast<u64>(kList))), ~0ull, true, mk);
         return;
       }
@@ -888,21 +848,24 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
   // ---- what is kept, in place: its mass a warp, and the walk ----
   auto kept = [&](float l, int index, float *dd) -> u64 {
     const float d = dist(l, m, R.inv_t);
-    const u64 w = weight(d);
-    *dd = d;
-    return w >= R.least && order_key(d, index) <= cut ? w : 0;
+    const u64 w = weight(d);  // 0 of a NaN
+    *dd = near(d);
+    return w >= R.least && order_key(near(d), index) <= cut ? w : 0;
   };
   float d;
   if (cut_k || cut_p) {
-    u64 mine = 0;
-    for (int i = v0 + lane; i < v1; i += 32) {
-      const V v(data[i]);
+    // (k may have had nothing to cut, and then there was no pass for it.)
+    if (cut == ~0ull) {
+      u64 mine = 0;
+      for (int i = v0 + lane; i < v1; i += 32) {
+        const V v = at(i);
 #pragma unroll
-      for (int j = 0; j < kVN; ++j) mine += kept(v.v[j], begin + i * kVN + j, &d);
+        for (int j = 0; j < kVN; ++j) mine += kept(v.v[j], begin + i * kVN + j, &d);
+      }
+      mine = warp_sum(mine);
+      if (lane == 0) S.warp_kept[warp] = mine;
+      __syncthreads();
     }
-    mine = warp_sum(mine);
-    if (lane == 0) S.warp_kept[warp] = mine;
-    __syncthreads();
     if (t < nc) {
       u64 all = 0;
       for (int w = 0; w < kWarps; ++w) all += S.warp_kept[w];
@@ -922,7 +885,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
       const int i = i0 + lane;
       u64 own = 0;
       if (i < v1) {
-        const V v(data[i]);
+        const V v = at(i);
 #pragma unroll
         for (int j = 0; j < kVN; ++j) own += kept(v.v[j], begin + i * kVN + j, &d);
       }
@@ -931,14 +894,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_cluster_kernel(const Sampl
         before += all;
         continue;
       }
-      u64 at = before + warp_scan(own, lane) - own;
-      if (i < v1 && at <= target && target < at + own) {
-        const V v(data[i]);
+      u64 here = before + warp_scan(own, lane) - own;
+      if (i < v1 && here <= target && target < here + own) {
+        const V v = at(i);
 #pragma unroll
         for (int j = 0; j < kVN; ++j) {
           const u64 w = kept(v.v[j], begin + i * kVN + j, &d);
-          if (w && at <= target && target < at + w) answer(begin + i * kVN + j, d);
-          at += w;
+          if (w && here <= target && target < here + w) answer(begin + i * kVN + j, d);
+          here += w;
         }
       }
       break;
@@ -953,30 +916,14 @@ size_t sample_smem(int64_t slice, int size) {
   return (sizeof(SampleShared) + 15) / 16 * 16 + static_cast<size_t>(slice * size + 15) / 16 * 16;
 }
 
-template <int DT>
-int launch_sample_typed(const SampleArgs &a, cudaStream_t s) {
-  const int size = DT == H24_DTYPE_F32 ? 4 : 2;
-  // The fewest CTAs a row with which two CTAs fit an SM and two an SM are
-  // there, as long as a CTA's slice has 2,048 logits.
-  int nc = 1;
-  int64_t slice = 0;
-  for (;; nc *= 2) {
-    slice = ((a.vocab + nc - 1) / nc + 15) / 16 * 16;
-    if (nc == kMaxCluster || slice <= 2048) break;
-    if (sample_smem(slice, size) <= kSampleSmemMax / 2 - 1024 && a.rows * nc >= 296) break;
-  }
-  if (sample_smem(slice, size) > kSampleSmemMax || a.rows * nc > INT32_MAX) {
-    sample_rows_kernel<DT><<<wave_grid(a.rows, 2), kSampleThreads, 0, s>>>(a);
-    H24_CUDA_TRY(cudaGetLastError());
-    count_launches(1);
-    return H24_OK;
-  }
-  constexpr auto kernel = sample_cluster_kernel<DT>;
+template <int DT, bool kHeld>
+int launch_cluster(const SampleArgs &a, int nc, int64_t slice, size_t smem, cudaStream_t s) {
+  constexpr auto kernel = sample_cluster_kernel<DT, kHeld>;
   H24_CUDA_TRY(allow_smem<kernel>(kSampleSmemMax));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.rows * nc));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = sample_smem(slice, size);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -986,10 +933,26 @@ int launch_sample_typed(const SampleArgs &a, cudaStream_t s) {
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = nc > 1 ? 2 : 1;
   H24_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, nc, static_cast<int>(slice)));
   count_launches(1);
   return H24_OK;
+}
+
+template <int DT>
+int launch_sample_typed(const SampleArgs &a, cudaStream_t s) {
+  const int size = DT == H24_DTYPE_F32 ? 4 : 2;
+  if (a.rows > INT32_MAX / kMaxCluster) return fail(H24_ERR_INVALID, "sample_tokens: too many rows");
+  // The most CTAs a row that are there at once, one an SM, with slices of at
+  // least 1,024 logits; a row that does not fit them, or rows enough for the
+  // SMs by themselves, run a CTA a row that reads it from L2.
+  int nc = kMaxCluster;
+  while (nc > 1 && (a.rows * nc > 148 || a.vocab < 1024 * nc)) nc /= 2;
+  if (const char *e = std::getenv("NC")) nc = atoi(e);
+  const int64_t slice = ((a.vocab + nc - 1) / nc + 15) / 16 * 16;
+  if (a.rows >= MANYROWS || sample_smem(slice, size) > kSampleSmemMax)
+    return launch_cluster<DT, false>(a, 1, a.vocab, sample_smem(0, size), s);
+  return launch_cluster<DT, true>(a, nc, slice, sample_smem(slice, size), s);
 }
 
 }  // namespace
