@@ -135,6 +135,7 @@ constexpr float kBinsPerNat = 71.9f, kFar = 28.45f;
 constexpr int kList = 1024;
 constexpr int kFew = 128;  // lists up to this long are ranked by counting
 constexpr int kMaxCluster = 8;
+constexpr int kRing = 6;
 
 struct Cut {  // where a cut falls: the step, what is before it and in it
   u64 bin, count_before, mass_before, count, mass;
@@ -295,24 +296,66 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
     }
     return *reinterpret_cast<const uint4 *>(raw);
   };
-  auto at = [&](int i) -> V {
-    if (kHeld) return V(data[i]);
-    return V(i < nfull ? __ldcg(reinterpret_cast<const uint4 *>(src) + i) : pieces(i));
+  auto raw_at = [&](int i) -> uint4 {
+    if (kHeld) return data[i];
+    return i < nfull ? __ldcg(reinterpret_cast<const uint4 *>(src) + i) : pieces(i);
   };
+  auto at = [&](int i) -> V { return V(raw_at(i)); };
+  // Every vector of this warp's part, a lane each: f(vector, its number, live);
+  // the lanes stay together, past the end with no vector and live false.  What
+  // is not held comes from global memory through a ring of kRing copies a lane,
+  // so that many are on their way without a register each.
+  uint4 *ring = data + warp * kRing * 32 + lane;
+  auto each_vector = [&](auto f) {
+    if (kHeld) {
+      for (int i0 = v0; i0 < v1; i0 += 32) {
+        const int i = i0 + lane;
+        f(V(data[min(i, v1 - 1)]), i, i < v1);
+      }
+      return;
+    }
+    const int whole = min(v1, nfull);
+    auto ask = [&](int i, int slot) {
+      if (i < whole)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(su32(ring + slot * 32)),
+                     "l"(reinterpret_cast<const uint4 *>(src) + i)
+                     : "memory");
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (int k = 0; k < kRing; ++k) ask(v0 + 32 * k + lane, k);
+    int slot = 0;
+    for (int i0 = v0; i0 < v1; i0 += 32) {
+      const int i = i0 + lane;
+      asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
+      const V v(i < whole ? ring[slot * 32] : pieces(i));  // past the slice's end all -inf
+      ask(i + 32 * kRing, slot);
+      if (++slot == kRing) slot = 0;
+      f(v, i, i < v1);
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+  };
+  if (kHeld) {
 #pragma unroll 4
-  for (int i = t; i < nfull; i += kThreads) {
-    const uint4 raw = kHeld ? __ldcs(reinterpret_cast<const uint4 *>(src) + i) : __ldcg(reinterpret_cast<const uint4 *>(src) + i);
-    if (kHeld) data[i] = raw;
-    const V v(raw);
+    for (int i = t; i < nfull; i += kThreads) {
+      const uint4 raw = __ldcs(reinterpret_cast<const uint4 *>(src) + i);
+      data[i] = raw;
+      const V v(raw);
 #pragma unroll
-    for (int j = 0; j < kVN; ++j) mine_max = fmaxf(mine_max, v.v[j]);
-  }
-  for (int i = nfull + t; i < nvec; i += kThreads) {
-    const uint4 raw = pieces(i);
-    if (kHeld) data[i] = raw;
-    const V v(raw);
+      for (int j = 0; j < kVN; ++j) mine_max = fmaxf(mine_max, v.v[j]);
+    }
+    for (int i = nfull + t; i < nvec; i += kThreads) {
+      const uint4 raw = pieces(i);
+      data[i] = raw;
+      const V v(raw);
 #pragma unroll
-    for (int j = 0; j < kVN; ++j) mine_max = fmaxf(mine_max, v.v[j]);
+      for (int j = 0; j < kVN; ++j) mine_max = fmaxf(mine_max, v.v[j]);
+    }
+  } else {
+    each_vector([&](const V &v, int, bool live) {
+#pragma unroll
+      for (int j = 0; j < kVN; ++j)
+        if (live) mine_max = fmaxf(mine_max, v.v[j]);
+    });
   }
   float mx = mine_max;
 #pragma unroll
@@ -337,111 +380,15 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
     return;
   }
 
-  // ---- one pass: total mass, what min-p leaves of it, the largest logit's
-  // first index, and the steps that a cut at p looks at ----
   const bool greedy = R.k == 1, cut_k = !greedy && R.k < a.vocab, cut_p = !greedy && R.p < 1.f;
-  auto count_step = [&](int b, u64 w, bool masses) {
-    atomicAdd(&S.count[b], 1u);
+  auto count_step = [&](int b, u64 w, bool counts, bool masses) {
+    if (counts) atomicAdd(&S.count[b], 1u);
     if (masses) {
       const uint32_t wl = static_cast<uint32_t>(w), old = atomicAdd(&S.lo[b], wl);
       const uint32_t wh = static_cast<uint32_t>(w >> 32) + (old + wl < old ? 1u : 0u);
       if (wh) atomicAdd(&S.hi[b], wh);
     }
   };
-  // Without top-k, tokens beyond |z| = ln(4 V / (1 - p)) hold less than (1 - p)
-  // of the mass together, so the cut at p falls before them.
-  const bool steps_of_all = cut_p && !cut_k;
-  const float far = steps_of_all ? fminf(kFar, logf(4.0f * static_cast<float>(a.vocab) / (1.0f - R.p)) + 0.01f) : 0.f;
-  const bool floor_counts = !greedy && !cut_k && !cut_p && R.least > 1;  // what min-p leaves is not the total
-  if (a.logprobs || !cut_k) {
-    u64 total = 0, kept = 0;
-    uint32_t first = 0xFFFFFFFFu;
-    // Four or eight weights that are all below 2^29 (nearly always) add up in 32 bits.
-    auto pass = [&](auto each) {
-      for (int i = v0 + lane; i < v1; i += 32) {
-        const V v = at(i);
-        float d[kVN], f[kVN], top = 0.f;
-#pragma unroll
-        for (int j = 0; j < kVN; ++j) {
-          d[j] = dist(v.v[j], m, R.inv_t);
-          f[j] = scaled(d[j]);
-          top = fmaxf(top, f[j]);
-        }
-        if (top < 536870912.0f) {
-          uint32_t sum = 0;
-#pragma unroll
-          for (int j = 0; j < kVN; ++j) {
-            const uint32_t w = __float2uint_rn(f[j]);
-            sum += w;
-            each(i, j, v.v[j], d[j], w);
-          }
-          total += sum;
-        } else {
-#pragma unroll
-          for (int j = 0; j < kVN; ++j) {
-            const u64 w = to_weight(f[j]);
-            total += w;
-            each(i, j, v.v[j], d[j], w);
-          }
-        }
-      }
-    };
-    if (steps_of_all)
-      pass([&](int, int, float, float d, u64 w) {
-        if (d < far) count_step(bin_of(near(d)), w, true);
-      });
-    else if (greedy)
-      pass([&](int i, int j, float l, float, u64) {
-        if (l >= m) first = min(first, static_cast<uint32_t>(begin + i * kVN + j));
-      });
-    else if (floor_counts)
-      pass([&](int, int, float, float, u64 w) { kept += w >= R.least ? w : 0; });
-    else
-      pass([](int, int, float, float, u64) {});
-    total = warp_sum(total);
-    kept = floor_counts ? warp_sum(kept) : total;
-    if (greedy) first = __reduce_min_sync(0xffffffffu, first);
-    if (lane == 0) {
-      S.warp_total[warp] = total;
-      S.warp_kept[warp] = kept;
-      S.warp_first[warp] = first;
-    }
-  } else if (lane == 0) {
-    S.warp_total[warp] = 0;
-  }
-  // The k-th largest of the threads' largest logits is at most the k-th
-  // largest logit: the steps of those alone give a bound on the cut at k.
-  if (cut_k) {
-    const float d = near(dist(mine_max, m, R.inv_t));
-    if (d < kFar && weight(d)) atomicAdd(&S.count[bin_of(d)], 1u);
-  }
-  __syncthreads();
-  if (warp == 0) {
-    const u64 tot = warp_sum(lane < kWarps ? S.warp_total[lane] : 0);
-    const u64 kep = floor_counts ? warp_sum(lane < kWarps ? S.warp_kept[lane] : 0) : tot;
-    const uint32_t fir = greedy ? __reduce_min_sync(0xffffffffu, lane < kWarps ? S.warp_first[lane] : 0xFFFFFFFFu) : 0;
-    if (lane < nc) {
-      peer_st(peer(&S.total[rank], lane), tot);
-      peer_st(peer(&S.kept[rank], lane), kep);
-      if (greedy) peer_st(peer(&S.first[rank], lane), fir);
-    }
-  }
-  cluster_sync(nc);
-  u64 total = 0;
-  for (int c = 0; c < nc; ++c) total += S.total[c];
-  auto answer = [&](uint32_t index, float d) {
-    a.tokens[r] = index;
-    if (a.logprobs)
-      a.logprobs[r] = -d - logf(static_cast<float>(static_cast<double>(total) / static_cast<double>(kOne)));
-  };
-  if (greedy) {
-    if (rank == 0 && t == 0) {
-      u64 first = ~0ull;
-      for (int c = 0; c < nc; ++c) first = min(first, S.first[c]);
-      answer(static_cast<uint32_t>(first), 0.f);
-    }
-    return;
-  }
 
   // This CTA's share of the steps, added over the cluster: four steps for each
   // group of nc lanes, one CTA's counts a lane, with the count and mass before
@@ -524,41 +471,15 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
     cluster_sync(nc);
     return S.cut;
   };
-  // Of the tokens of steps up to `last`: keys that satisfy `wanted` go to the first CTA's list (as many as fit);
-  // returns their number in the cluster.  Of those that satisfy `sure` before
-  // it, what min-p leaves is added up a warp.  Starts and ends with the cluster
-  // in step; S.list_n and S.local_n are zero at the start.
-  auto collect = [&](int last, auto sure, auto wanted) -> u64 {
-    const float bound = fminf(static_cast<float>(last + 1) / kBinsPerNat, kFar);  // a step ends half a step before
-    // First a list of this CTA's own, over the steps' masses (read by now).
-    u64 *own = nc == 1 ? S.list : reinterpret_cast<u64 *>(S.lo);
-    u64 mine = 0;
-    for (int i = v0 + lane; i < v1; i += 32) {
-      const V v = at(i);
-#pragma unroll
-      for (int j = 0; j < kVN; ++j) {
-        float d = dist(v.v[j], m, R.inv_t);
-        if (d < bound) {
-          d = near(d);
-          const u64 key = order_key(d, begin + i * kVN + j);
-          if (bin_of(d) > last) continue;
-          if (sure(d, key)) {
-            const u64 w = weight(d);
-            mine += w >= R.least ? w : 0;
-          } else if (wanted(d, key) && weight(d)) {
-            const uint32_t place = atomicAdd(&S.local_n, 1u);
-            if (place < kList) own[place] = key;
-          }
-        }
-      }
-    }
-    mine = warp_sum(mine);
-    if (lane == 0) S.warp_kept[warp] = mine;
+  // Sends this CTA's own list (S.local_n keys) to the first CTA's, as many as
+  // fit; returns the number in the cluster.  The cluster is in step after it.
+  u64 *own = nc == 1 ? S.list : reinterpret_cast<u64 *>(S.lo);  // over the steps' masses, read by then
+  auto ship = [&]() -> u64 {
     __syncthreads();
     const uint32_t here = S.local_n;
     if (nc == 1) return here;
     if (t < nc) peer_st(peer(&S.slot[rank], t), here);
-    if (t == 0) S.base = peer_add(peer(&S.list_n, 0), here);
+    if (t == 0 && here) S.base = peer_add(peer(&S.list_n, 0), here);
     __syncthreads();
     const uint32_t to = peer(&S.list[0], 0), base = S.base;
     for (uint32_t i = t; i < min(here, static_cast<uint32_t>(kList)); i += kThreads)
@@ -568,7 +489,214 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
     for (int c = 0; c < nc; ++c) all += S.slot[c];
     return all;
   };
+  auto list_key = [&](u64 key) {
+    const uint32_t place = atomicAdd(&S.local_n, 1u);
+    if (place < kList) own[place] = key;
+  };
+  // Of the tokens of steps up to `last`: keys that satisfy `wanted` go to the
+  // own list, and of those that satisfy `sure` before it, what min-p leaves is
+  // added up a warp.  A warp queues what lies within the bound and works on 32
+  // at a time: one lane in twenty would otherwise hold up the rest.
+  auto collect = [&](int last, auto sure, auto wanted) {
+    const float bound = fminf(static_cast<float>(last + 1) / kBinsPerNat, kFar);  // a step ends half a step before
+    u64 *queue = reinterpret_cast<u64 *>(S.hi) + warp * 64;
+    u64 mine = 0;
+    int queued = 0;
+    auto work = [&](bool any) {
+      if (any) {
+        const u64 key = queue[lane];
+        const float d = key_dist(key), f = scaled(d);
+        if (bin_of(d) <= last) {
+          const u64 w = to_weight(f);
+          if (sure(d, key))
+            mine += w >= R.least ? w : 0;
+          else if (w && wanted(d, key))
+            list_key(key);
+        }
+      }
+    };
+    each_vector([&](const V &v, int i, bool live) {
+#pragma unroll
+      for (int j = 0; j < kVN; ++j) {
+        const float d = dist(v.v[j], m, R.inv_t);
+        const bool in = d < bound && live;
+        const uint32_t votes = __ballot_sync(0xffffffffu, in);
+        if (votes == 0) continue;
+        if (in) queue[queued + __popc(votes & ((1u << lane) - 1))] = order_key(near(d), begin + i * kVN + j);
+        queued += __popc(votes);
+        if (queued >= 32) {
+          __syncwarp();
+          work(true);
+          queued -= 32;
+          const u64 over = queue[32 + lane];
+          __syncwarp();
+          if (lane < queued) queue[lane] = over;
+        }
+      }
+    });
+    __syncwarp();
+    work(lane < queued);
+    mine = warp_sum(mine);
+    if (lane == 0) S.warp_kept[warp] = mine;
+  };
+
   const auto none = [](float, u64) { return false; };
+
+  // The k-th largest of the threads' largest logits is at most the k-th
+  // largest logit: the steps of those alone give one at or beyond that in which
+  // the cut at k falls.
+  int k_last = -1;
+  if (cut_k) {
+    const float d = near(dist(fminf(mine_max, kLargest), m, R.inv_t));
+    if (d < kFar && weight(d)) atomicAdd(&S.count[bin_of(d)], 1u);
+    cluster_sync(nc);
+    gather_bins(false);
+    if (counted() >= static_cast<u64>(R.k)) k_last = static_cast<int>(find(false, static_cast<u64>(R.k)).bin);
+  }
+
+  // ---- one pass: total mass, what min-p leaves of it, the largest logit's
+  // first index, and the steps that a cut at p looks at ----
+  // Without top-k: tokens beyond |z| = ln(1.25 V / ((1 - p) L)) hold less than
+  // (1 - p) of a mass of at least L, so the cut at p falls before them and their
+  // steps need no mass.  L: the threads' largest logits of this CTA (CTAs may
+  // differ in what they leave out; the cut falls before all of it).
+  const bool steps_of_all = cut_p && !cut_k;
+  float far = 0.f;
+  if (steps_of_all) {
+    float some = mine_max > -INFINITY ? expf(-near(dist(fminf(mine_max, kLargest), m, R.inv_t))) : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) some += __shfl_xor_sync(0xffffffffu, some, o);
+    if (lane == 0) S.warp_first[warp] = __float_as_uint(some);
+    __syncthreads();
+    some = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) some += __uint_as_float(S.warp_first[w]);
+    __syncthreads();
+    far = logf(1.25f * static_cast<float>(a.vocab) / ((1.0f - R.p) * fmaxf(some, 1.0f))) + 0.01f;
+    if (far > 26.f) far = kFar;  // beyond, the weights' rounding counts
+  }
+  const bool floor_counts = !greedy && !cut_k && !cut_p && R.least > 1;  // what min-p leaves is not the total
+  if (a.logprobs || !cut_k) {
+    u64 total = 0, kept = 0;
+    uint32_t first = 0xFFFFFFFFu;
+    // A vector of weights below 2^32 takes one conversion each.  (With a bound of
+    // 2^29, which lets four add up in 32 bits, half of the warps had a lane above it.)
+    auto pass = [&](auto few, auto each) {
+      each_vector([&](const V &v, int i, bool live) {
+        float d[kVN], f[kVN], top = 0.f;
+#pragma unroll
+        for (int j = 0; j < kVN; ++j) {
+          d[j] = live ? dist(v.v[j], m, R.inv_t) : INFINITY;
+          f[j] = scaled(d[j]);
+          top = fmaxf(top, f[j]);
+        }
+        if (top < 4294967040.0f) {
+          uint32_t w[kVN];
+#pragma unroll
+          for (int j = 0; j < kVN; ++j) {
+            w[j] = __float2uint_rn(f[j]);
+            total += w[j];
+          }
+          few(i, v.v, d, w);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kVN; ++j) {
+            const u64 w = to_weight(f[j]);
+            total += w;
+            each(i, j, v.v[j], d[j], w);
+          }
+        }
+      });
+    };
+    // `each` for a vector of small weights too.
+    auto same = [&](auto each) {
+      return [each](int i, const float(&l)[kVN], const float(&d)[kVN], const uint32_t(&w)[kVN]) {
+#pragma unroll
+        for (int j = 0; j < kVN; ++j) each(i, j, l[j], d[j], w[j]);
+      };
+    };
+    if (k_last >= 0) {
+      const float bound = fminf(static_cast<float>(k_last + 1) / kBinsPerNat, kFar);
+      auto each = [&](int i, int j, float, float d, u64 w) {
+        if (d < bound && w && bin_of(near(d)) <= k_last) list_key(order_key(near(d), begin + i * kVN + j));
+      };
+      pass(same(each), each);
+    } else if (steps_of_all) {
+      // Small weights have no high word but a carry: the sums of a vector are
+      // asked for together and looked at after.
+      pass(
+          [&](int, const float(&)[kVN], const float(&d)[kVN], const uint32_t(&w)[kVN]) {
+            uint32_t old[kVN];
+            bool carry = false;
+#pragma unroll
+            for (int j = 0; j < kVN; ++j) old[j] = d[j] < far ? atomicAdd(&S.lo[bin_of(d[j])], w[j]) : 0u;
+#pragma unroll
+            for (int j = 0; j < kVN; ++j) carry |= d[j] < far && old[j] + w[j] < old[j];
+            if (carry) {
+#pragma unroll
+              for (int j = 0; j < kVN; ++j)
+                if (d[j] < far && old[j] + w[j] < old[j]) atomicAdd(&S.hi[bin_of(d[j])], 1u);
+            }
+          },
+          [&](int, int, float, float d, u64 w) {
+            if (d < far) count_step(bin_of(near(d)), w, false, true);
+          });
+    } else if (greedy) {
+      auto each = [&](int i, int j, float l, float, u64) {
+        if (l >= m && i < v1) first = min(first, static_cast<uint32_t>(begin + i * kVN + j));
+      };
+      pass(same(each), each);
+    } else if (floor_counts) {
+      auto each = [&](int, int, float, float, u64 w) { kept += w >= R.least ? w : 0; };
+      pass(same(each), each);
+    } else {
+      pass([](int, const float(&)[kVN], const float(&)[kVN], const uint32_t(&)[kVN]) {},
+           [](int, int, float, float, u64) {});
+    }
+    total = warp_sum(total);
+    kept = floor_counts ? warp_sum(kept) : total;
+    if (greedy) first = __reduce_min_sync(0xffffffffu, first);
+    if (lane == 0) {
+      S.warp_total[warp] = total;
+      S.warp_kept[warp] = kept;
+      S.warp_first[warp] = first;
+    }
+  } else {
+    if (lane == 0) S.warp_total[warp] = 0;
+    if (k_last >= 0) collect(k_last, none, [](float, u64) { return true; });
+  }
+  __syncthreads();
+  if (warp == 0) {
+    const u64 tot = warp_sum(lane < kWarps ? S.warp_total[lane] : 0);
+    const u64 kep = floor_counts ? warp_sum(lane < kWarps ? S.warp_kept[lane] : 0) : tot;
+    const uint32_t fir = greedy ? __reduce_min_sync(0xffffffffu, lane < kWarps ? S.warp_first[lane] : 0xFFFFFFFFu) : 0;
+    if (lane < nc) {
+      peer_st(peer(&S.total[rank], lane), tot);
+      peer_st(peer(&S.kept[rank], lane), kep);
+      if (greedy) peer_st(peer(&S.first[rank], lane), fir);
+    }
+  }
+  u64 listed = 0;
+  if (k_last >= 0)
+    listed = ship();
+  else
+    cluster_sync(nc);
+  u64 total = 0;
+  for (int c = 0; c < nc; ++c) total += S.total[c];
+  auto answer = [&](uint32_t index, float d) {
+    a.tokens[r] = index;
+    if (a.logprobs)
+      a.logprobs[r] = -d - logf(static_cast<float>(static_cast<double>(total) / static_cast<double>(kOne)));
+  };
+  if (greedy) {
+    if (rank == 0 && t == 0) {
+      u64 first = ~0ull;
+      for (int c = 0; c < nc; ++c) first = min(first, S.first[c]);
+      answer(static_cast<uint32_t>(first), 0.f);
+    }
+    return;
+  }
+
   auto sort_by_key = [&](int len) {
     int pow2 = 2;
     while (pow2 < len) pow2 <<= 1;
@@ -614,9 +742,9 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
     *total_w = all;
     return before;
   };
-  // First CTA, list path: all three cuts and the choice, from the list (which
-  // holds at least every token that step 1 keeps, or step 2 where mk is known).
-  auto finish_list = [&](int len, u64 keep_n, bool by_p, u64 mk) {
+  // First CTA: all three cuts and the choice, from the list (which holds at
+  // least every token that step 1 keeps).
+  auto finish_list = [&](int len, u64 keep_n, bool by_p) {
     if (len <= kFew) {
       for (int i = t; i < len; i += kThreads) S.few[0][i] = weight(key_dist(S.list[i]));
       __syncthreads();
@@ -626,13 +754,11 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
       const int place = rank_few(len, key, &before, &all);
       if (static_cast<u64>(place) >= keep_n) w = 0;
       if (by_p) {
-        if (!mk) {  // the mass of the first keep_n
-          if (static_cast<u64>(place) == min(keep_n, static_cast<u64>(len)) - 1 && t % kPer == 0 && e < len)
-            S.pick = before + S.few[0][e];
-          __syncthreads();
-          mk = S.pick;
-        }
-        if (before >= mass_limit(R.p, mk)) w = 0;
+        // The mass of the first keep_n.
+        if (static_cast<u64>(place) == min(keep_n, static_cast<u64>(len)) - 1 && t % kPer == 0 && e < len)
+          S.pick = before + S.few[0][e];
+        __syncthreads();
+        if (before >= mass_limit(R.p, S.pick)) w = 0;
       }
       if (w < R.least) w = 0;
       if (t % kPer == 0 && e < len) S.few[1][e] = w;
@@ -662,7 +788,7 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
     u64 b0, b1, all;
     list_scan(w0, w1, b0, b1, all);
     if (by_p) {
-      const u64 limit = mass_limit(R.p, mk ? mk : all);
+      const u64 limit = mass_limit(R.p, all);
       if (b0 >= limit) w0 = 0;
       if (b1 >= limit) w1 = 0;
     }
@@ -697,10 +823,23 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
     auto in_reach = [&](float d, u64 key) {
       return bin_of(d) == bin && key <= limit_key && key >= lo && key - lo < width;
     };
-    while (c.count > kList) {
+    int len;
+    for (;;) {
+      if (t == 0) S.list_n = 0, S.local_n = 0;
+      cluster_sync(nc);
+      collect(
+          bin,
+          [&](float d, u64 key) {
+            const int b = bin_of(d);
+            return b < bin || (b == bin && key < lo);
+          },
+          in_reach);
+      const u64 found = ship();
+      len = static_cast<int>(found);
+      if (found <= kList) break;
       int shift = 0;
       while ((width >> shift) > static_cast<u64>(kBins - 1)) ++shift;
-      cluster_sync(nc);  // every CTA has read its peers' steps
+      cluster_sync(nc);
       clear_steps();
       __syncthreads();
       for (int i = v0 + lane; i < v1; i += 32) {
@@ -713,7 +852,7 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
           const u64 key = order_key(d, begin + i * kVN + j);
           if (!in_reach(d, key)) continue;
           const u64 w = weight(d);
-          if (w) count_step(static_cast<int>((key - lo) >> shift), w, masses);
+          if (w) count_step(static_cast<int>((key - lo) >> shift), w, !by_mass, masses);
         }
       }
       const u64 cb = c.count_before, mb = c.mass_before;
@@ -725,13 +864,6 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
       lo += c.bin << shift;
       width = u64(1) << shift;
     }
-    if (t == 0) S.list_n = 0, S.local_n = 0;
-    cluster_sync(nc);
-    const auto before_reach = [&](float d, u64 key) {
-      const int b = bin_of(d);
-      return b < bin || (b == bin && key < lo);
-    };
-    const int len = static_cast<int>(min(collect(bin, before_reach, in_reach), static_cast<u64>(kList)));
     if (rank == 0) {
       const u64 left = want - (by_mass ? c.mass_before : c.count_before);  // at least 1
       auto tell = [&](u64 key, u64 through) {
@@ -780,15 +912,9 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
 
   u64 cut = ~0ull;
   if (cut_k) {
-    // From the threads' largest logits: a step at or beyond the one where the cut falls.
-    gather_bins(false);
-    if (counted() >= static_cast<u64>(R.k)) {
-      const int last = static_cast<int>(find(false, static_cast<u64>(R.k)).bin);
-      const u64 len = collect(last, none, [](float, u64) { return true; });
-      if (len <= kList) {
-        if (rank == 0) finish_list(static_cast<int>(len), static_cast<u64>(R.k), cut_p, 0);
-        return;
-      }
+    if (k_last >= 0 && listed <= kList) {
+      if (rank == 0) finish_list(static_cast<int>(listed), static_cast<u64>(R.k), cut_p);
+      return;
     }
     // Too many, or k above the number of threads: the steps of all tokens.
     cluster_sync(nc);
@@ -803,7 +929,7 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
         const float d = dist(v.v[j], m, R.inv_t);
         const u64 w = weight(d);
         all += w;
-        if (w) count_step(bin_of(near(d)), w, cut_p);
+        if (w) count_step(bin_of(near(d)), w, true, cut_p);
       }
     }
     all = sum_block(all, S.red);
@@ -833,13 +959,6 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
       for (int j = 0; j < 4; ++j) bc[j] = bc0[j], bm[j] = bm0[j];
       cluster_sync(nc);  // S.cut has been read by all
       const Cut c = find(true, limit);
-      if (c.count_before + c.count <= kFew) {  // longer lists cost more than the passes below
-        if (t == 0) S.list_n = 0, S.local_n = 0;
-        cluster_sync(nc);
-        const u64 len = collect(static_cast<int>(c.bin), none, [&](float, u64 key) { return key <= cut; });
-        if (rank == 0) finish_list(static_cast<int>(min(len, static_cast<u64>(kList))), ~0ull, true, mk);
-        return;
-      }
       u64 unused;
       cut = settle(c, true, limit, cut, true, &unused);
     }
@@ -951,7 +1070,7 @@ int launch_sample_typed(const SampleArgs &a, cudaStream_t s) {
   if (const char *e = std::getenv("NC")) nc = atoi(e);
   const int64_t slice = ((a.vocab + nc - 1) / nc + 15) / 16 * 16;
   if (a.rows >= MANYROWS || sample_smem(slice, size) > kSampleSmemMax)
-    return launch_cluster<DT, false>(a, 1, a.vocab, sample_smem(0, size), s);
+    return launch_cluster<DT, false>(a, 1, a.vocab, sample_smem(kWarps * kRing * 32 * 16 / size, size), s);
   return launch_cluster<DT, true>(a, nc, slice, sample_smem(slice, size), s);
 }
 
