@@ -53,6 +53,7 @@ struct SampleArgs {
   int32_t top_k1;
   int64_t *tokens;
   float *logprobs;
+  bool sorted;  // rows in the order of costly_first()
 };
 
 // |z| of a logit; m is finite and inv_t within fp32's normal range.  l = m
@@ -135,7 +136,8 @@ constexpr float kBinsPerNat = 71.9f, kFar = 28.45f;
 constexpr int kList = 1024;
 constexpr int kFew = 128;  // lists up to this long are ranked by counting
 constexpr int kMaxCluster = 8;
-constexpr int kRing = 6;
+constexpr int kRing = 4;   // vectors on their way a lane
+constexpr int kQueue = 6;  // tokens a lane keeps until a warp works on them together
 
 struct Cut {  // where a cut falls: the step, what is before it and in it
   u64 bin, count_before, mass_before, count, mass;
@@ -145,6 +147,7 @@ struct SampleShared {
   uint32_t count[kBins], lo[kBins], hi[kBins];
   u64 list[kList];
   u64 few[2][kFew];
+  uint2 queue[kWarps][kQueue][32];
   u64 slot[kMaxCluster];  // one value of each CTA
   u64 slice_count[kMaxCluster], slice_mass[kMaxCluster];
   u64 total[kMaxCluster], first[kMaxCluster], kept[kMaxCluster];
@@ -234,6 +237,40 @@ __device__ __noinline__ void sort_list(u64 *list, int n) {
     }
 }
 
+// The row that a CTA of its own takes, when rows with different settings are
+// more than fit at once: those with a cut at p alone first (three passes), then
+// those with a cut at k, then the rest, so that no long row starts last.
+__device__ int64_t costly_first(const SampleArgs &a) {
+  auto kind = [&](int64_t r) {
+    const float t = a.temperature ? a.temperature[r] : a.temperature1, p = a.top_p ? a.top_p[r] : a.top_p1;
+    const int64_t k = t > 0.f ? (a.top_k ? a.top_k[r] : a.top_k1) : 1;
+    return k == 1 ? 2 : k > 0 && k < a.vocab ? 1 : p < 1.f ? 0 : 2;
+  };
+  __shared__ int64_t row;
+  const int64_t want = blockIdx.x;
+  int64_t before = 0;  // rows of the kinds, and of the rows, before
+  for (int c = 0; c < 3; ++c)
+    for (int64_t r0 = 0; r0 < a.rows; r0 += kThreads) {
+      const int64_t r = r0 + threadIdx.x;
+      const bool is = r < a.rows && kind(r) == c;
+      const int here = __syncthreads_count(is);
+      if (want < before + here) {
+        // The (want - before)-th of these: counted by warps, then by lanes.
+        __shared__ int warps[kWarps];
+        const uint32_t votes = __ballot_sync(0xffffffffu, is);
+        if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = __popc(votes);
+        __syncthreads();
+        int64_t at = before;
+        for (int w = 0; w < static_cast<int>(threadIdx.x >> 5); ++w) at += warps[w];
+        if (is && at + __popc(votes & ((1u << (threadIdx.x & 31)) - 1)) == want) row = r;
+        __syncthreads();
+        return row;
+      }
+      before += here;
+    }
+  return want;  // not reached: every row is of a kind
+}
+
 struct RowSettings {
   int64_t k;
   float inv_t, p, u;
@@ -249,7 +286,6 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
   uint4 *data = reinterpret_cast<uint4 *>(sample_raw + (sizeof(SampleShared) + 15) / 16 * 16);
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int rank = static_cast<int>(blockIdx.x) % nc;
-  const int64_t r = blockIdx.x / nc;
   const int begin = rank * slice;
   const int n = static_cast<int>(max(int64_t(0), min(static_cast<int64_t>(slice), a.vocab - begin)));
   const int nvec = (n + kVN - 1) / kVN;
@@ -265,6 +301,7 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
   __syncwarp();
   if (nc > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   pdl_enter();
+  const int64_t r = a.sorted ? costly_first(a) : blockIdx.x / nc;
   RowSettings R;
   {
     float temp = a.temperature ? a.temperature[r] : a.temperature1;
@@ -380,7 +417,8 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
     return;
   }
 
-  const bool greedy = R.k == 1, cut_k = !greedy && R.k < a.vocab, cut_p = !greedy && R.p < 1.f;
+  const bool greedy = R.k == 1, cut_k = !greedy && R.k < a.vocab;
+  bool cut_p = !greedy && R.p < 1.f;
   auto count_step = [&](int b, u64 w, bool counts, bool masses) {
     if (counts) atomicAdd(&S.count[b], 1u);
     if (masses) {
@@ -495,49 +533,47 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
   };
   // Of the tokens of steps up to `last`: keys that satisfy `wanted` go to the
   // own list, and of those that satisfy `sure` before it, what min-p leaves is
-  // added up a warp.  A warp queues what lies within the bound and works on 32
-  // at a time: one lane in twenty would otherwise hold up the rest.
+  // added up a warp.  Each lane keeps what lies within the bound until one has
+  // no room for four more: a token in a hundred would otherwise hold up its
+  // warp each time, and a vote on every token costs more than its weight.
   auto collect = [&](int last, auto sure, auto wanted) {
     const float bound = fminf(static_cast<float>(last + 1) / kBinsPerNat, kFar);  // a step ends half a step before
-    u64 *queue = reinterpret_cast<u64 *>(S.hi) + warp * 64;
-    u64 mine = 0;
-    int queued = 0;
-    auto work = [&](bool any) {
-      if (any) {
-        const u64 key = queue[lane];
-        const float d = key_dist(key), f = scaled(d);
-        if (bin_of(d) <= last) {
-          const u64 w = to_weight(f);
-          if (sure(d, key))
-            mine += w >= R.least ? w : 0;
-          else if (w && wanted(d, key))
-            list_key(key);
-        }
+    uint2 *mine = &S.queue[warp][0][lane];
+    u64 sum = 0;
+    int have = 0;
+    auto flush = [&]() {
+      const int rounds = __reduce_max_sync(0xffffffffu, have);
+      for (int q = 0; q < rounds; ++q) {
+        if (q >= have) continue;
+        const uint2 e = mine[q * 32];
+        const float d = __uint_as_float(e.y);
+        if (bin_of(d) > last) continue;
+        const u64 w = weight(d), key = order_key(d, e.x);
+        if (sure(d, key))
+          sum += w >= R.least ? w : 0;
+        else if (w && wanted(d, key))
+          list_key(key);
       }
+      have = 0;
+      __syncwarp();
     };
     each_vector([&](const V &v, int i, bool live) {
 #pragma unroll
-      for (int j = 0; j < kVN; ++j) {
-        const float d = dist(v.v[j], m, R.inv_t);
-        const bool in = d < bound && live;
-        const uint32_t votes = __ballot_sync(0xffffffffu, in);
-        if (votes == 0) continue;
-        if (in) queue[queued + __popc(votes & ((1u << lane) - 1))] = order_key(near(d), begin + i * kVN + j);
-        queued += __popc(votes);
-        if (queued >= 32) {
-          __syncwarp();
-          work(true);
-          queued -= 32;
-          const u64 over = queue[32 + lane];
-          __syncwarp();
-          if (lane < queued) queue[lane] = over;
+      for (int g = 0; g < kVN; g += 4) {
+#pragma unroll
+        for (int j = g; j < g + 4; ++j) {
+          const float d = dist(v.v[j], m, R.inv_t);
+          if (d < bound && live) {
+            mine[have * 32] = make_uint2(begin + i * kVN + j, __float_as_uint(near(d)));
+            ++have;
+          }
         }
+        if (__any_sync(0xffffffffu, have > kQueue - 4)) flush();
       }
     });
-    __syncwarp();
-    work(lane < queued);
-    mine = warp_sum(mine);
-    if (lane == 0) S.warp_kept[warp] = mine;
+    flush();
+    sum = warp_sum(sum);
+    if (lane == 0) S.warp_kept[warp] = sum;
   };
 
   const auto none = [](float, u64) { return false; };
@@ -554,15 +590,52 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
     if (counted() >= static_cast<u64>(R.k)) k_last = static_cast<int>(find(false, static_cast<u64>(R.k)).bin);
   }
 
-  // ---- one pass: total mass, what min-p leaves of it, the largest logit's
-  // first index, and the steps that a cut at p looks at ----
-  // Without top-k: tokens beyond |z| = ln(1.25 V / ((1 - p) L)) hold less than
-  // (1 - p) of a mass of at least L, so the cut at p falls before them and their
-  // steps need no mass.  L: the threads' largest logits of this CTA (CTAs may
-  // differ in what they leave out; the cut falls before all of it).
-  const bool steps_of_all = cut_p && !cut_k;
-  float far = 0.f;
-  if (steps_of_all) {
+  // ---- one pass: total mass, and what the settings ask for beside it ----
+  // f(|z|s, weights) of every vector of this warp's part; `few` where all of
+  // its weights are below 2^32, one conversion each, else `each` for each.
+  // (With a bound of 2^29, which lets four add up in 32 bits, half of the
+  // warps had a lane above it.)
+  auto pass = [&](auto few, auto each) -> u64 {
+    u64 sum = 0;
+    each_vector([&](const V &v, int i, bool live) {
+      float d[kVN], f[kVN], top = 0.f;
+#pragma unroll
+      for (int j = 0; j < kVN; ++j) {
+        d[j] = live ? dist(v.v[j], m, R.inv_t) : INFINITY;
+        f[j] = scaled(d[j]);
+        top = fmaxf(top, f[j]);
+      }
+      if (top < 4294967040.0f) {
+        uint32_t w[kVN];
+#pragma unroll
+        for (int j = 0; j < kVN; ++j) {
+          w[j] = __float2uint_rn(f[j]);
+          sum += w[j];
+        }
+        few(i, v.v, d, w);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVN; ++j) {
+          const u64 w = to_weight(f[j]);
+          sum += w;
+          each(i, j, v.v[j], d[j], w);
+        }
+      }
+    });
+    return warp_sum(sum);
+  };
+  // `each` for a vector of small weights too.
+  auto same = [&](auto each) {
+    return [each](int i, const float(&l)[kVN], const float(&d)[kVN], const uint32_t(&w)[kVN]) {
+#pragma unroll
+      for (int j = 0; j < kVN; ++j) each(i, j, l[j], d[j], w[j]);
+    };
+  };
+  // The masses of the steps that the cut at p may fall in.  Tokens beyond |z| =
+  // ln(1.25 V / ((1 - p) L)) hold less than (1 - p) of a mass of at least L, so
+  // the cut falls before them.  L: the threads' largest logits of this CTA
+  // (CTAs may differ in what they leave out; the cut falls before all of it).
+  auto pass_steps = [&]() -> u64 {
     float some = mine_max > -INFINITY ? expf(-near(dist(fminf(mine_max, kLargest), m, R.inv_t))) : 0.f;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) some += __shfl_xor_sync(0xffffffffu, some, o);
@@ -571,95 +644,71 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
     some = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) some += __uint_as_float(S.warp_first[w]);
-    __syncthreads();
-    far = logf(1.25f * static_cast<float>(a.vocab) / ((1.0f - R.p) * fmaxf(some, 1.0f))) + 0.01f;
+    float far = logf(1.25f * static_cast<float>(a.vocab) / ((1.0f - R.p) * fmaxf(some, 1.0f))) + 0.01f;
     if (far > 26.f) far = kFar;  // beyond, the weights' rounding counts
-  }
-  const bool floor_counts = !greedy && !cut_k && !cut_p && R.least > 1;  // what min-p leaves is not the total
+    // Small weights have no high word but a carry: the sums of a vector are
+    // asked for together and looked at after.
+    return pass(
+        [&](int, const float(&)[kVN], const float(&d)[kVN], const uint32_t(&w)[kVN]) {
+          uint32_t old[kVN];
+          bool carry = false;
+#pragma unroll
+          for (int j = 0; j < kVN; ++j) old[j] = d[j] < far ? atomicAdd(&S.lo[bin_of(d[j])], w[j]) : 0u;
+#pragma unroll
+          for (int j = 0; j < kVN; ++j) carry |= d[j] < far && old[j] + w[j] < old[j];
+          if (carry) {
+#pragma unroll
+            for (int j = 0; j < kVN; ++j)
+              if (d[j] < far && old[j] + w[j] < old[j]) atomicAdd(&S.hi[bin_of(d[j])], 1u);
+          }
+        },
+        [&](int, int, float, float d, u64 w) {
+          if (d < far) count_step(bin_of(near(d)), w, false, true);
+        });
+  };
+  // What min-p leaves may lie before the cut at p as a whole, and then p cuts
+  // nothing of it: its mass is looked at first.
+  const bool steps_of_all = cut_p && !cut_k;
+  const bool floor_counts = !greedy && !cut_k && R.least > 1;
   if (a.logprobs || !cut_k) {
-    u64 total = 0, kept = 0;
+    u64 sum = 0, kept = 0;
     uint32_t first = 0xFFFFFFFFu;
-    // A vector of weights below 2^32 takes one conversion each.  (With a bound of
-    // 2^29, which lets four add up in 32 bits, half of the warps had a lane above it.)
-    auto pass = [&](auto few, auto each) {
-      each_vector([&](const V &v, int i, bool live) {
-        float d[kVN], f[kVN], top = 0.f;
-#pragma unroll
-        for (int j = 0; j < kVN; ++j) {
-          d[j] = live ? dist(v.v[j], m, R.inv_t) : INFINITY;
-          f[j] = scaled(d[j]);
-          top = fmaxf(top, f[j]);
-        }
-        if (top < 4294967040.0f) {
-          uint32_t w[kVN];
-#pragma unroll
-          for (int j = 0; j < kVN; ++j) {
-            w[j] = __float2uint_rn(f[j]);
-            total += w[j];
-          }
-          few(i, v.v, d, w);
-        } else {
-#pragma unroll
-          for (int j = 0; j < kVN; ++j) {
-            const u64 w = to_weight(f[j]);
-            total += w;
-            each(i, j, v.v[j], d[j], w);
-          }
-        }
-      });
-    };
-    // `each` for a vector of small weights too.
-    auto same = [&](auto each) {
-      return [each](int i, const float(&l)[kVN], const float(&d)[kVN], const uint32_t(&w)[kVN]) {
-#pragma unroll
-        for (int j = 0; j < kVN; ++j) each(i, j, l[j], d[j], w[j]);
-      };
-    };
     if (k_last >= 0) {
       const float bound = fminf(static_cast<float>(k_last + 1) / kBinsPerNat, kFar);
       auto each = [&](int i, int j, float, float d, u64 w) {
         if (d < bound && w && bin_of(near(d)) <= k_last) list_key(order_key(near(d), begin + i * kVN + j));
       };
-      pass(same(each), each);
-    } else if (steps_of_all) {
-      // Small weights have no high word but a carry: the sums of a vector are
-      // asked for together and looked at after.
-      pass(
-          [&](int, const float(&)[kVN], const float(&d)[kVN], const uint32_t(&w)[kVN]) {
-            uint32_t old[kVN];
-            bool carry = false;
+      sum = pass(
+          [&](int i, const float(&l)[kVN], const float(&d)[kVN], const uint32_t(&w)[kVN]) {
+            float least = d[0];
 #pragma unroll
-            for (int j = 0; j < kVN; ++j) old[j] = d[j] < far ? atomicAdd(&S.lo[bin_of(d[j])], w[j]) : 0u;
+            for (int j = 1; j < kVN; ++j) least = fminf(least, d[j]);
+            if (least < bound) {  // rare: one test a vector
 #pragma unroll
-            for (int j = 0; j < kVN; ++j) carry |= d[j] < far && old[j] + w[j] < old[j];
-            if (carry) {
-#pragma unroll
-              for (int j = 0; j < kVN; ++j)
-                if (d[j] < far && old[j] + w[j] < old[j]) atomicAdd(&S.hi[bin_of(d[j])], 1u);
+              for (int j = 0; j < kVN; ++j) each(i, j, l[j], d[j], w[j]);
             }
           },
-          [&](int, int, float, float d, u64 w) {
-            if (d < far) count_step(bin_of(near(d)), w, false, true);
-          });
+          each);
     } else if (greedy) {
       auto each = [&](int i, int j, float l, float, u64) {
         if (l >= m && i < v1) first = min(first, static_cast<uint32_t>(begin + i * kVN + j));
       };
-      pass(same(each), each);
+      sum = pass(same(each), each);
+      first = __reduce_min_sync(0xffffffffu, first);
     } else if (floor_counts) {
       auto each = [&](int, int, float, float, u64 w) { kept += w >= R.least ? w : 0; };
-      pass(same(each), each);
+      sum = pass(same(each), each);
+    } else if (steps_of_all) {
+      sum = pass_steps();
     } else {
-      pass([](int, const float(&)[kVN], const float(&)[kVN], const uint32_t(&)[kVN]) {},
-           [](int, int, float, float, u64) {});
+      sum = pass([](int, const float(&)[kVN], const float(&)[kVN], const uint32_t(&)[kVN]) {},
+                 [](int, int, float, float, u64) {});
     }
-    total = warp_sum(total);
-    kept = floor_counts ? warp_sum(kept) : total;
-    if (greedy) first = __reduce_min_sync(0xffffffffu, first);
+    kept = floor_counts ? warp_sum(kept) : sum;
     if (lane == 0) {
-      S.warp_total[warp] = total;
+      S.warp_total[warp] = sum;
       S.warp_kept[warp] = kept;
-      S.warp_first[warp] = first;
+      if (greedy) S.warp_first[warp] = first;
     }
   } else {
     if (lane == 0) S.warp_total[warp] = 0;
@@ -683,6 +732,16 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
     cluster_sync(nc);
   u64 total = 0;
   for (int c = 0; c < nc; ++c) total += S.total[c];
+  if (steps_of_all && floor_counts) {
+    u64 kept = 0;
+    for (int c = 0; c < nc; ++c) kept += S.kept[c];
+    if (kept <= mass_limit(R.p, total)) {
+      cut_p = false;
+    } else {
+      pass_steps();
+      cluster_sync(nc);
+    }
+  }
   auto answer = [&](uint32_t index, float d) {
     a.tokens[r] = index;
     if (a.logprobs)
@@ -1028,7 +1087,7 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
   }
 }
 
-constexpr int kSampleSmemMax = 227 * 1024;
+constexpr int kSampleSmemMax = 226 * 1024;  // (and a little static)
 
 // Shared memory of a CTA whose slice holds `slice` logits of `size` bytes.
 size_t sample_smem(int64_t slice, int size) {
@@ -1070,7 +1129,11 @@ int launch_sample_typed(const SampleArgs &a, cudaStream_t s) {
   if (const char *e = std::getenv("NC")) nc = atoi(e);
   const int64_t slice = ((a.vocab + nc - 1) / nc + 15) / 16 * 16;
   if (a.rows >= MANYROWS || sample_smem(slice, size) > kSampleSmemMax)
-    return launch_cluster<DT, false>(a, 1, a.vocab, sample_smem(kWarps * kRing * 32 * 16 / size, size), s);
+  {
+    SampleArgs b = a;
+    b.sorted = a.rows > 296 && a.rows <= 8192 && (a.top_k || a.top_p || a.temperature) && !std::getenv("NOSORT");
+    return launch_cluster<DT, false>(b, 1, a.vocab, sample_smem(kWarps * kRing * 32 * 16 / size, size), s);
+  }
   return launch_cluster<DT, true>(a, nc, slice, sample_smem(slice, size), s);
 }
 
@@ -1081,7 +1144,7 @@ int launch_sample(const void *logits, int dtype, int64_t rows, int64_t vocab, in
                   const float *top_p, float top_p1, const float *min_p, float min_p1, int64_t *tokens,
                   float *logprobs, cudaStream_t s) {
   const SampleArgs a{logits, rows, vocab, stride, u, temperature, top_k, top_p, min_p, temperature1, top_p1, min_p1,
-                     top_k1, tokens, logprobs};
+                     top_k1, tokens, logprobs, false};
   switch (dtype) {
     case H24_DTYPE_F32: return launch_sample_typed<H24_DTYPE_F32>(a, s);
     case H24_DTYPE_F16: return launch_sample_typed<H24_DTYPE_F16>(a, s);
