@@ -14,24 +14,30 @@
 // largest probability is the smallest weight kept; with at most 2^22 tokens a
 // row's mass stays below 2^62.
 //
-// sample_cluster_kernel reads a row once.  A cluster of 1 to 8 CTAs holds it in
-// shared memory, a slice each.  A cut is found from a histogram of |z| in steps
-// of 1/72 (beyond |z| = 28.4 a weight rounds to 0), which the CTAs add through
-// distributed shared memory, a share of the steps each.  For top-k only each
-// thread's largest logit is counted: the step that holds the k-th of those
-// bounds the k-th token, and what lies up to it (k and a few more) goes to the
-// first CTA, which makes all three cuts and the choice.  For top-p alone every
-// step gets a count and a mass; a few tokens up to the cut go the same way, and
-// otherwise the tokens of the one step in which the cut falls settle it and the
-// CTAs add and walk what is kept, in place.
+// A row is held by a cluster of 1 to 8 CTAs, a slice each in shared memory, or,
+// where there are rows enough for the SMs, read by one CTA from L2 in each pass.
+// A cut is found from a histogram of |z| in steps of 1/72 (beyond |z| = 28.4 a
+// weight rounds to 0), which the CTAs add through distributed shared memory, a
+// share of the steps each.
+//   top-k: only each thread's largest logit is counted.  The k-th largest of
+//     those bounds the k-th token, so the tokens of the steps up to its own (k
+//     and a few more) are listed in the pass that adds the weights; the first
+//     CTA ranks the list and makes all three cuts and the choice.
+//   top-p alone: the steps get masses in the pass that adds the weights, which
+//     gives the step in which the cut falls.  A second pass adds what lies
+//     before that step and lists its tokens; the first CTA finds the last one
+//     kept, and the warp in whose part the target falls walks it.
+//   neither, or a min-p that leaves less than p: the walk alone.
+// What bounds it, measured on a B200: one row, the chain of a dozen barriers
+// and exchanges ([1,50688] fp32, k = 50, p = 0.9: 10.9 us; no cut: 7.2); many
+// rows, instruction issue and the second read from L2 ([512,50688] fp32: no
+// cut 67 us, k = 50 59, p = 0.9 142, for 15.9 us of HBM traffic).
 //
 // "z descending, index ascending" is one 64-bit key: |z|'s bits above the
 // index (z <= 0, so |z| ascending is z descending, and the bits of
 // non-negative floats ascend with them).  A selection is then a cut on that
 // key, found by histograms of its digits.
 #include "h24_internal.cuh"
-#include <cstdlib>
-#define MANYROWS (std::getenv("MANY") ? atoi(std::getenv("MANY")) : 148)
 
 namespace h24 {
 namespace {
@@ -136,7 +142,6 @@ constexpr float kBinsPerNat = 71.9f, kFar = 28.45f;
 constexpr int kList = 1024;
 constexpr int kFew = 128;  // lists up to this long are ranked by counting
 constexpr int kMaxCluster = 8;
-constexpr int kRing = 4;   // vectors on their way a lane
 constexpr int kQueue = 6;  // tokens a lane keeps until a warp works on them together
 
 struct Cut {  // where a cut falls: the step, what is before it and in it
@@ -271,6 +276,10 @@ __device__ int64_t costly_first(const SampleArgs &a) {
   return want;  // not reached: every row is of a kind
 }
 
+struct Always {  // a condition that the compiler knows
+  constexpr operator bool() const { return true; }
+};
+
 struct RowSettings {
   int64_t k;
   float inv_t, p, u;
@@ -339,37 +348,25 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
   };
   auto at = [&](int i) -> V { return V(raw_at(i)); };
   // Every vector of this warp's part, a lane each: f(vector, its number, live);
-  // the lanes stay together, past the end with no vector and live false.  What
-  // is not held comes from global memory through a ring of kRing copies a lane,
-  // so that many are on their way without a register each.
-  uint4 *ring = data + warp * kRing * 32 + lane;
+  // the lanes stay together, past the end with live false.  What is not held
+  // is loaded kAhead vectors at a time.
   auto each_vector = [&](auto f) {
-    if (kHeld) {
-      for (int i0 = v0; i0 < v1; i0 += 32) {
-        const int i = i0 + lane;
-        f(V(data[min(i, v1 - 1)]), i, i < v1);
+    int i0 = v0;
+    if constexpr (!kHeld) {
+      constexpr int kAhead = 16 / kVN;
+      const int whole = min(v1, nfull);
+      for (; i0 + 32 * kAhead <= whole; i0 += 32 * kAhead) {
+        uint4 raw[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) raw[u] = __ldcg(reinterpret_cast<const uint4 *>(src) + i0 + 32 * u + lane);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) f(V(raw[u]), i0 + 32 * u + lane, Always{});
       }
-      return;
     }
-    const int whole = min(v1, nfull);
-    auto ask = [&](int i, int slot) {
-      if (i < whole)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(su32(ring + slot * 32)),
-                     "l"(reinterpret_cast<const uint4 *>(src) + i)
-                     : "memory");
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    for (int k = 0; k < kRing; ++k) ask(v0 + 32 * k + lane, k);
-    int slot = 0;
-    for (int i0 = v0; i0 < v1; i0 += 32) {
+    for (; i0 < v1; i0 += 32) {
       const int i = i0 + lane;
-      asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
-      const V v(i < whole ? ring[slot * 32] : pieces(i));  // past the slice's end all -inf
-      ask(i + 32 * kRing, slot);
-      if (++slot == kRing) slot = 0;
-      f(v, i, i < v1);
+      f(V(raw_at(min(i, v1 - 1))), i, i < v1);
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
   };
   if (kHeld) {
 #pragma unroll 4
@@ -388,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
       for (int j = 0; j < kVN; ++j) mine_max = fmaxf(mine_max, v.v[j]);
     }
   } else {
-    each_vector([&](const V &v, int, bool live) {
+    each_vector([&](const V &v, int, auto live) {
 #pragma unroll
       for (int j = 0; j < kVN; ++j)
         if (live) mine_max = fmaxf(mine_max, v.v[j]);
@@ -557,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
       have = 0;
       __syncwarp();
     };
-    each_vector([&](const V &v, int i, bool live) {
+    each_vector([&](const V &v, int i, auto live) {
 #pragma unroll
       for (int g = 0; g < kVN; g += 4) {
 #pragma unroll
@@ -597,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
   // warps had a lane above it.)
   auto pass = [&](auto few, auto each) -> u64 {
     u64 sum = 0;
-    each_vector([&](const V &v, int i, bool live) {
+    each_vector([&](const V &v, int i, auto live) {
       float d[kVN], f[kVN], top = 0.f;
 #pragma unroll
       for (int j = 0; j < kVN; ++j) {
@@ -636,16 +633,19 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
   // the cut falls before them.  L: the threads' largest logits of this CTA
   // (CTAs may differ in what they leave out; the cut falls before all of it).
   auto pass_steps = [&]() -> u64 {
-    float some = mine_max > -INFINITY ? expf(-near(dist(fminf(mine_max, kLargest), m, R.inv_t))) : 0.f;
+    float far = kFar;
+    if (!kHeld) {  // (a slice that is held has too few tokens for this to pay)
+      float some = mine_max > -INFINITY ? expf(-near(dist(fminf(mine_max, kLargest), m, R.inv_t))) : 0.f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) some += __shfl_xor_sync(0xffffffffu, some, o);
-    if (lane == 0) S.warp_first[warp] = __float_as_uint(some);
-    __syncthreads();
-    some = 0.f;
+      for (int o = 16; o > 0; o >>= 1) some += __shfl_xor_sync(0xffffffffu, some, o);
+      if (lane == 0) S.warp_first[warp] = __float_as_uint(some);
+      __syncthreads();
+      some = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) some += __uint_as_float(S.warp_first[w]);
-    float far = logf(1.25f * static_cast<float>(a.vocab) / ((1.0f - R.p) * fmaxf(some, 1.0f))) + 0.01f;
-    if (far > 26.f) far = kFar;  // beyond, the weights' rounding counts
+      for (int w = 0; w < kWarps; ++w) some += __uint_as_float(S.warp_first[w]);
+      far = logf(1.25f * static_cast<float>(a.vocab) / ((1.0f - R.p) * fmaxf(some, 1.0f))) + 0.01f;
+      if (far > 26.f) far = kFar;  // beyond, the weights' rounding counts
+    }
     // Small weights have no high word but a carry: the sums of a vector are
     // asked for together and looked at after.
     return pass(
@@ -1121,18 +1121,20 @@ template <int DT>
 int launch_sample_typed(const SampleArgs &a, cudaStream_t s) {
   const int size = DT == H24_DTYPE_F32 ? 4 : 2;
   if (a.rows > INT32_MAX / kMaxCluster) return fail(H24_ERR_INVALID, "sample_tokens: too many rows");
-  // The most CTAs a row that are there at once, one an SM, with slices of at
-  // least 1,024 logits; a row that does not fit them, or rows enough for the
-  // SMs by themselves, run a CTA a row that reads it from L2.
+  // Clusters where a CTA each fits an SM: the most CTAs a row that are there at
+  // once, with slices of at least 1,024 logits.  Rows enough for the SMs by
+  // themselves, or too long for a cluster, run a CTA a row that reads it from
+  // L2 in each pass ([512,50688] fp32, p = 0.9: 142 us, in clusters of four 275;
+  // [64,50688] bf16, p = 0.95: 60 us, in clusters of two 36; [1,50688] fp32,
+  // k = 50: 15.6 us, in a cluster of eight 10.9).
   int nc = kMaxCluster;
   while (nc > 1 && (a.rows * nc > 148 || a.vocab < 1024 * nc)) nc /= 2;
-  if (const char *e = std::getenv("NC")) nc = atoi(e);
   const int64_t slice = ((a.vocab + nc - 1) / nc + 15) / 16 * 16;
-  if (a.rows >= MANYROWS || sample_smem(slice, size) > kSampleSmemMax)
-  {
+  if (a.rows >= 148 || sample_smem(slice, size) > kSampleSmemMax) {
     SampleArgs b = a;
-    b.sorted = a.rows > 296 && a.rows <= 8192 && (a.top_k || a.top_p || a.temperature) && !std::getenv("NOSORT");
-    return launch_cluster<DT, false>(b, 1, a.vocab, sample_smem(kWarps * kRing * 32 * 16 / size, size), s);
+    // Two CTAs an SM are there at once.  (Up to 8,192 rows: every CTA counts the settings of all.)
+    b.sorted = a.rows > 296 && a.rows <= 8192 && (a.top_k || a.top_p || a.temperature);
+    return launch_cluster<DT, false>(b, 1, a.vocab, sample_smem(0, size), s);
   }
   return launch_cluster<DT, true>(a, nc, slice, sample_smem(slice, size), s);
 }
