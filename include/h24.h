@@ -216,7 +216,7 @@ int h24_int8_linear(const int8_t *q, const float *scale, int64_t tokens, int64_t
  *   the order of the indices, exceeds floor(u * mass).
  * Every sum is exact, so the token does not depend on how the work is split.
  * T <= 0 (or NaN) takes the largest logit, lowest index.  A NaN logit is never
- * chosen; a row without a logit above -inf gives -1.  logprobs (may be NULL)
+ * chosen, +inf counts as the largest fp32 number; a row without a logit above -inf gives -1.  logprobs (may be NULL)
  * receives z - log(sum of all w / 2^40) of the token: its log-probability
  * under the temperature before the three cuts.  Each setting is an array of
  * one value a row, or NULL and the scalar beside it.  vocab is at most 2^22. */

@@ -10,8 +10,10 @@ Modules:
   pack           -- pack._quantize_h24_layer and pack._quantize_int8 mirrors
   packed_linear  -- PackedH24Linear / PackedInt8* / materialize mirrors, batched materialize
   plx            -- .plx container reader / writer
+  int8           -- INT8 head path: residual + RMS norm to int8 rows, int8 product
+  sampling       -- temperature, top-k, top-p and min-p from given numbers
   shard          -- row sharding across ranks, optional all-gather of packed bytes
-  build          -- nvcc build recipe of libh24.so
+  build          -- build recipe of libh24.so and of its torch module
 """
 from __future__ import annotations
 

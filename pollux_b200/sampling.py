@@ -44,7 +44,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: float | to
     ``temperature`` 0 takes the largest logit.  Each setting is a number or a
     tensor with one value a row.
 
-    NaN logits are never chosen; a row with no logit above -inf gives -1.
+    NaN logits are never chosen, +inf counts as the largest fp32 number; a row
+    with no logit above -inf gives -1.
     Returns int64 tokens of the leading shape, with ``return_logprob`` also the
     fp32 log-probabilities of the tokens at that temperature before the cuts
     (-inf for a row that gives -1)."""
