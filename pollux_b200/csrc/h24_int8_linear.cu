@@ -91,9 +91,6 @@ __device__ __forceinline__ bool bar_wait(uint64_t *bar, uint32_t parity, volatil
   return bar_try(bar, parity) || bar_wait_slow(bar, parity, abort, err, heed);
 }
 
-__device__ __forceinline__ void bar_arrive(uint64_t *bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(su32(bar)) : "memory");
-}
 __device__ __forceinline__ void bar_expect(uint64_t *bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(su32(bar)), "r"(bytes) : "memory");
 }
@@ -179,48 +176,72 @@ __device__ __forceinline__ void put4(Half *y, const float (&v)[4]) {
   *reinterpret_cast<uint2 *>(y) = *reinterpret_cast<const uint2 *>(h);
 }
 
-// 16 bytes at `p`, any alignment, from the 4-byte words around it; words not
-// wholly inside [lo, hi) are read by the byte, and bytes from p + valid on
+// The 16 bytes at `a` (16-byte aligned); those outside [lo, hi) are not read
+// and come back as zeros.
+__device__ __forceinline__ uint4 load16_within(const int8_t *a, const int8_t *lo, const int8_t *hi) {
+  if (a >= lo && a + 16 <= hi) return __ldg(reinterpret_cast<const uint4 *>(a));
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll  // the sixteen loads in flight together
+  for (int j = 0; j < 16; ++j)
+    if (a + j >= lo && a + j < hi) w[j / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(__ldg(a + j))) << (8 * (j & 3));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// 16 bytes at offset `off` (0-15) of two aligned blocks; bytes from `valid` on
 // come back as zeros.
-__device__ __forceinline__ uint4 load16_any(const int8_t *p, int valid, const int8_t *lo, const int8_t *hi) {
-  const uint32_t sh = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 3u);
-  const int8_t *a = p - sh;
-  uint32_t w[5];
+__device__ __forceinline__ uint4 join16(uint4 x, uint4 y, uint32_t off, int valid) {
+  const uint32_t v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+  uint32_t h[6], w[5], r[4];  // words off / 8 * 2 on, then off / 4 on
 #pragma unroll
-  for (int i = 0; i < 5; ++i) {
-    const int8_t *x = a + 4 * i;
-    w[i] = 0;
-    if (i == 4 && sh == 0) break;
-    if (x >= lo && x + 4 <= hi) {
-      w[i] = __ldg(reinterpret_cast<const uint32_t *>(x));
-    } else {
+  for (int i = 0; i < 6; ++i) h[i] = (off & 8) ? v[i + 2] : v[i];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (x + j >= lo && x + j < hi)
-          w[i] |= static_cast<uint32_t>(static_cast<uint8_t>(__ldg(x + j))) << (8 * j);
-    }
-  }
-  uint32_t r[4];
+  for (int i = 0; i < 5; ++i) w[i] = (off & 4) ? h[i + 1] : h[i];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    r[i] = __funnelshift_r(w[i], w[i + 1], 8 * sh);
+    r[i] = __funnelshift_r(w[i], w[i + 1], 8 * (off & 3));
     const int left = valid - 4 * i;
     if (left < 4) r[i] &= left <= 0 ? 0u : (0xFFFFFFFFu >> (8 * (4 - left)));
   }
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-// Rows [row0, row0 + rows) x k [k0, k0 + 128) of a byte matrix into a swizzled
-// tile, by the 128 threads of the filling warps; outside it zeros.
-__device__ __forceinline__ void fill_tile(uint8_t *tile, int rows, const int8_t *base, int64_t stride, int row0,
-                                          int nrows, int k0, int in, int t) {
-  const int8_t *hi = base + static_cast<int64_t>(nrows - 1) * stride + in;
-  for (int i = t; i < rows * 8; i += 128) {
-    const int r = i >> 3, c = i & 7, k = k0 + 16 * c;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (row0 + r < nrows && k < in)
-      v = load16_any(base + static_cast<int64_t>(row0 + r) * stride + k, in - k, base, hi);
-    *reinterpret_cast<uint4 *>(tile + r * 128 + ((c ^ (r & 7)) << 4)) = v;
+__device__ __forceinline__ uint32_t offset16(const int8_t *p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 15u);
+}
+
+// 16 bytes at `p`, any alignment, from the two aligned blocks around it (a
+// warp's neighbours share them in L1); bytes from p + valid on come back as zeros.
+__device__ __forceinline__ uint4 load16_any(const int8_t *p, int valid, const int8_t *lo, const int8_t *hi) {
+  const uint32_t off = offset16(p);
+  return join16(load16_within(p - off, lo, hi), off ? load16_within(p - off + 16, lo, hi) : make_uint4(0, 0, 0, 0), off,
+                valid);
+}
+
+// Rows of a byte matrix at any pitch and alignment, copied to rows of `pitch`
+// bytes (a multiple of 16), zeros past their end: what TMA can read.  Where a
+// layer or its input is not 16-byte aligned, the copy and the tiles over it
+// (2 more bytes of traffic a byte) take [4096,1919] x [7680,1919] from 1,106 us
+// with tiles filled by hand to REPACK_BIG, and [20,1921] x [7680,1921] from 61 to
+// REPACK_SMALL.
+struct RepackArgs {
+  const int8_t *src;
+  int64_t stride;
+  int8_t *dst;
+  int64_t rows;
+};
+constexpr int kRepackThreads = 256;
+__global__ void __launch_bounds__(kRepackThreads) repack_rows_kernel(const RepackArgs a0, const RepackArgs a1, int cols,
+                                                                     int chunks) {
+  pdl_enter();
+  const int64_t total0 = a0.rows * chunks, total = total0 + a1.rows * chunks;
+  for (int64_t i = blockIdx.x * static_cast<int64_t>(kRepackThreads) + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * kRepackThreads) {
+    const RepackArgs &a = i < total0 ? a0 : a1;
+    const int64_t at = i < total0 ? i : i - total0;
+    const int64_t r = at <= 0xFFFFFFFFll ? static_cast<uint32_t>(at) / static_cast<uint32_t>(chunks) : at / chunks;
+    const int c = static_cast<int>(at - r * chunks) * 16;
+    const int8_t *hi = a.src + (a.rows - 1) * a.stride + cols;
+    reinterpret_cast<uint4 *>(a.dst)[at] = load16_any(a.src + r * a.stride + c, cols - c, a.src, hi);
   }
 }
 
@@ -332,9 +353,8 @@ constexpr int kSplitThreads = 192;  // warp 0 loads, warp 1 issues MMAs, warps 2
 // One CTA per 128 x n tile and k slice.  The `split` CTAs of a cluster take a
 // slice of the tile's k each; their int32 partial tiles meet in distributed
 // shared memory, where CTA r finishes every split-th part of the tokens (the
-// sum is an integer, so the order does not matter).  kTma: operands arrive by
-// TMA (16-byte aligned rows); otherwise warps 2-5 place them by hand.
-template <bool kTma, typename Out>
+// sum is an integer, so the order does not matter).
+template <typename Out>
 __global__ void __launch_bounds__(kSplitThreads) int8_linear_split_kernel(const __grid_constant__ CUtensorMap wmap,
                                                                           const __grid_constant__ CUtensorMap qmap,
                                                                           const __grid_constant__ LinArgs a) {
@@ -353,14 +373,14 @@ __global__ void __launch_bounds__(kSplitThreads) int8_linear_split_kernel(const 
 
   if (t == 0) {
     for (int s = 0; s < a.stages; ++s) {
-      bar_init(&H.full[s], kTma ? 1 : 128);
+      bar_init(&H.full[s], 1);
       bar_init(&H.empty[s], 1);
     }
     bar_init(&H.done, 1);
     H.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    if (kTma) {
+    if (a.in > 0) {
       asm volatile("prefetch.tensormap [%0];" ::"l"(&wmap) : "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(&qmap) : "memory");
     }
@@ -378,7 +398,7 @@ __global__ void __launch_bounds__(kSplitThreads) int8_linear_split_kernel(const 
   pdl_enter();
 
   if (warp == 0) {
-    if (kTma && lane == 0) {
+    if (lane == 0) {
       int s = 0;
       uint32_t ph = 0;
       int issued = 0;
@@ -410,20 +430,6 @@ __global__ void __launch_bounds__(kSplitThreads) int8_linear_split_kernel(const 
     }
     mma_commit(&H.done);
   } else {
-    const int ft = t - 64;
-    if (!kTma) {
-      int s = 0;
-      uint32_t ph = 0;
-      for (int i = 0; i < nkb; ++i) {
-        if (!bar_wait(&H.empty[s], ph ^ 1, abort, a.err)) break;
-        uint8_t *st = stages + static_cast<size_t>(s) * stage_bytes;
-        fill_tile(st, kM, a.w, a.in, o0, a.out, (kb0 + i) * kKB, a.in, ft);
-        fill_tile(st + kABytes, a.n, a.q, a.q_stride, t0, a.tokens, (kb0 + i) * kKB, a.in, ft);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        bar_arrive(&H.full[s]);
-        if (++s == a.stages) s = 0, ph ^= 1;
-      }
-    }
     // The warp's number from lane 0: the compiler then keeps what follows from
     // it, the column addresses above all, in uniform registers.
     const int quarter = __shfl_sync(0xffffffffu, warp, 0) & 3, row = quarter * 32 + lane;  // TMEM lanes
@@ -493,7 +499,7 @@ constexpr int kVecThreads = 256;
 template <int T, int R, bool kAhead, bool kAligned, typename Out>
 __global__ void __launch_bounds__(kVecThreads) int8_linear_vec_kernel(const LinArgs a) {
   constexpr int kVecChunk = T > 4 ? 4096 : 8192;  // k per pass: the tokens' rows of a pass lie in shared memory
-  constexpr int U = kAligned ? 4 : 1;             // 16-byte loads of each row in flight
+  constexpr int U = 4;                            // 16-byte loads of each row in flight
   __shared__ __align__(16) uint8_t xs[T][kVecChunk];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int64_t o0 = (static_cast<int64_t>(blockIdx.x) * (kVecThreads / 32) + warp) * R;
@@ -506,9 +512,52 @@ __global__ void __launch_bounds__(kVecThreads) int8_linear_vec_kernel(const LinA
       for (int k = lane * 128; k < a.in; k += 32 * 128)
         asm volatile("prefetch.global.L2 [%0];" ::"l"(a.w + (o0 + r) * a.in + k));
   pdl_enter();
+  // The blocks around these rows lie inside the matrix.
+  const bool inner = live == R && o0 * a.in >= 16 && (o0 + R) * a.in + 32 <= static_cast<int64_t>(a.out) * a.in;
+  // Lane k * R + r finishes row r, token k; what it needs is asked for first.
+  const int fr = lane % R, fk = lane / R;
+  const bool finishes = fr < live && fk < T && fk < a.tokens;
+  const float sc = finishes ? __ldg(a.scale + fk) : 0.f, ws = finishes ? weight_scale(a.mu16, o0 + fr) : 0.f;
+  const float b = finishes && a.bias ? __ldg(a.bias + o0 + fr) : 0.f;
+  uint4 w[R][U], next[kAligned ? 1 : R][kAligned ? 1 : U];
+  // Vectors v0 + 32 u + lane of the rows, of the kn bytes from k0.  `settle`
+  // makes them from their two blocks where the rows are off the boundary.
+  auto ask = [&](int k0, int kn, int v0) {
+    const int vecs = (kn + 15) / 16;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int v = v0 + 32 * u + lane;
+        const int8_t *p = a.w + (o0 + r) * a.in + k0 + 16 * v;
+        if constexpr (kAligned) {
+          w[r][u] = v < vecs && r < live ? __ldcs(reinterpret_cast<const uint4 *>(p)) : make_uint4(0, 0, 0, 0);
+        } else if (inner) {
+          p -= 16 * max(v - (vecs - 1), 0);
+          const uint4 *block = reinterpret_cast<const uint4 *>(p - offset16(p));
+          w[r][u] = __ldg(block);
+          next[r][u] = __ldg(block + 1);
+        } else {
+          w[r][u] = v < vecs && r < live ? load16_any(p, kn - 16 * v, a.w, wend) : make_uint4(0, 0, 0, 0);
+        }
+      }
+  };
+  auto settle = [&](int k0, int kn, int v0) {
+    if constexpr (!kAligned) {
+      if (inner) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            w[r][u] = join16(w[r][u], next[r][u], offset16(a.w + (o0 + r) * a.in + k0),
+                             kn - 16 * (v0 + 32 * u + lane));
+      }
+    }
+  };
   int acc[R][T] = {};
   for (int k0 = 0; k0 < a.in; k0 += kVecChunk) {
     const int kn = min(kVecChunk, a.in - k0), vecs = (kn + 15) / 16;
+    ask(k0, kn, 0);  // on their way while the tokens are placed
     if (k0) __syncthreads();
     const int8_t *qend = a.q + (a.tokens - 1) * a.q_stride + a.in;
     for (int i = t; i < T * vecs; i += kVecThreads) {
@@ -522,18 +571,8 @@ __global__ void __launch_bounds__(kVecThreads) int8_linear_vec_kernel(const LinA
     }
     __syncthreads();
     for (int v0 = 0; v0 < vecs; v0 += 32 * U) {
-      uint4 w[R][U];
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int v = v0 + 32 * u + lane;
-          w[r][u] = make_uint4(0, 0, 0, 0);
-          if (v < vecs && r < live) {
-            const int8_t *p = a.w + (o0 + r) * a.in + k0 + 16 * v;
-            w[r][u] = kAligned ? __ldcs(reinterpret_cast<const uint4 *>(p)) : load16_any(p, kn - 16 * v, a.w, wend);
-          }
-        }
+      if (v0) ask(k0, kn, v0);
+      settle(k0, kn, v0);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int v = v0 + 32 * u + lane;
@@ -552,7 +591,6 @@ __global__ void __launch_bounds__(kVecThreads) int8_linear_vec_kernel(const LinA
       }
     }
   }
-  // Lane r * T + k finishes row r, token k.
   int mine = 0;
 #pragma unroll
   for (int r = 0; r < R; ++r)
@@ -561,35 +599,33 @@ __global__ void __launch_bounds__(kVecThreads) int8_linear_vec_kernel(const LinA
       const int sum = __reduce_add_sync(0xffffffffu, acc[r][k]);
       if (lane == k * R + r) mine = sum;
     }
-  const int r = lane % R, k = lane / R;
-  if (r < live && k < T && k < a.tokens) {
-    const int64_t o = o0 + r;
-    put(static_cast<Out *>(a.y) + k * static_cast<int64_t>(a.out) + o,
-        finish(mine, __ldg(a.scale + k), weight_scale(a.mu16, o), a.bias ? __ldg(a.bias + o) : 0.f));
-  }
+  if (finishes)
+    put(static_cast<Out *>(a.y) + fk * static_cast<int64_t>(a.out) + o0 + fr, finish(mine, sc, ws, b));
 }
 
-template <int T, int R, bool kAhead, typename Out>
-int launch_vec(const LinArgs &a, bool aligned, cudaStream_t s) {
+template <int T, int R, bool kAhead, bool kAligned, typename Out>
+int launch_vec(const LinArgs &a, cudaStream_t s) {
   const int64_t per_block = static_cast<int64_t>(kVecThreads / 32) * R;
   const unsigned grid = static_cast<unsigned>((a.out + per_block - 1) / per_block);
-  const auto kernel = aligned ? int8_linear_vec_kernel<T, R, kAhead, true, Out> : int8_linear_vec_kernel<T, R, kAhead, false, Out>;
-  H24_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(kVecThreads), s, a));
+  H24_CUDA_TRY(launch_pdl(int8_linear_vec_kernel<T, R, kAhead, kAligned, Out>, dim3(grid), dim3(kVecThreads), s, a));
   count_launches(1);
   return H24_OK;
 }
 
 template <int T, typename Out>
 int launch_vec_rows(const LinArgs &a, bool aligned, cudaStream_t s) {
+  // Off the boundary two blocks are held for each vector: one row a warp.
+  if (!aligned)
+    return a.out >= 148 * 8 * 8 ? launch_vec<T, 1, true, false, Out>(a, s) : launch_vec<T, 1, false, false, Out>(a, s);
   // Rows a warp, so that the warps of the layer fill the GPU; the L2 requests
   // ahead of the previous kernel's end only where the grid is many waves.
   // One token, us, 1 / 2 / 4 rows with and (without) the requests:
   // 50688 x 1920: 16.0 (17.6) / 15.0 (18.0) / 17.4 (18.1);
   // 7680 x 1920: 4.7 (4.3) / 3.8 (3.8) / 3.7 (3.5); 1920 x 7680: 5.7 (4.5) / 5.6 (5.9) / 6.4 (6.0).
   const int R = a.out >= 148 * 8 * 8 ? 2 : a.out >= 148 * 8 * 4 ? 4 : 1;
-  if (R == 4) return launch_vec<T, 4, false, Out>(a, aligned, s);
-  if (R == 2) return launch_vec<T, 2, true, Out>(a, aligned, s);
-  return launch_vec<T, 1, false, Out>(a, aligned, s);
+  if (R == 4) return launch_vec<T, 4, false, true, Out>(a, s);
+  if (R == 2) return launch_vec<T, 2, true, true, Out>(a, s);
+  return launch_vec<T, 1, false, true, Out>(a, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -846,7 +882,7 @@ double pair_us(int64_t tokens, int64_t out, int64_t kblocks, int n, double hbm_u
   return 4.5 + (us > hbm_us ? us : hbm_us);
 }
 
-Plan make_plan(int64_t tokens, int64_t out, int64_t in, int out_size, bool aligned) {
+Plan make_plan(int64_t tokens, int64_t out, int64_t in, int out_size) {
   // Up to four tokens without tiles; three and four only where the weights are
   // few (dp4a's work grows with the tokens): [4,1920] x [7680,1920] 4.8 us
   // against 5.5 in tiles, x [50688,1920] 22 against 18.
@@ -862,12 +898,11 @@ Plan make_plan(int64_t tokens, int64_t out, int64_t in, int out_size, bool align
       if (us < best_us) best_us = us, best = {kSplit, n, split};
     }
   }
-  if (aligned)
-    for (int n = 32; n <= 256; n += 32) {
-      if (n > 32 && tokens <= n - 32) break;
-      const double us = pair_us(tokens, out, kblocks, n, hbm_us);
-      if (us < best_us) best_us = us, best = {kPair, n, 1};
-    }
+  for (int n = 32; n <= 256; n += 32) {
+    if (n > 32 && tokens <= n - 32) break;
+    const double us = pair_us(tokens, out, kblocks, n, hbm_us);
+    if (us < best_us) best_us = us, best = {kPair, n, 1};
+  }
   return best;
 }
 
@@ -905,9 +940,9 @@ constexpr int kSmemPerSm = 228 * 1024, kSmemMax = 227 * 1024;
 // Shared memory of a split-kernel CTA with `stages` stages.
 int split_smem(int n, int stages) { return 1024 + kHeadBytes + stages * (kABytes + n * kKB); }
 
-template <bool kTma, typename Out>
+template <typename Out>
 int launch_split(const CUtensorMap &wmap, const CUtensorMap &qmap, const LinArgs &a, int smem, cudaStream_t s) {
-  constexpr auto kernel = int8_linear_split_kernel<kTma, Out>;
+  constexpr auto kernel = int8_linear_split_kernel<Out>;
   H24_CUDA_TRY(allow_smem<kernel>(kSmemMax));
   const int64_t tiles = (static_cast<int64_t>(a.out) + kM - 1) / kM * a.tok_tiles;
   if (tiles * a.split > INT32_MAX) return fail(H24_ERR_INVALID, "int8_linear: too many tiles");
@@ -966,7 +1001,7 @@ int launch_typed(const Plan &plan, bool aligned, const CUtensorMap &wmap, const 
     return launch_vec_rows<4, Out>(a, aligned, s);
   }
   if (plan.kind == kPair) return launch_pair<Out>(wmap, qmap, a, s);
-  return aligned ? launch_split<true, Out>(wmap, qmap, a, smem, s) : launch_split<false, Out>(wmap, qmap, a, smem, s);
+  return launch_split<Out>(wmap, qmap, a, smem, s);
 }
 
 }  // namespace
@@ -987,8 +1022,28 @@ int launch_int8_linear(const Tables *T, const int8_t *q, const float *scale, int
   a.out = static_cast<int>(out);
   a.in = static_cast<int>(in);
   a.y_vec = aligned16(y);
-  const bool aligned = in > 0 && in % 16 == 0 && q_stride % 16 == 0 && q_stride >= in && aligned16(q) && aligned16(w);
-  const Plan plan = make_plan(tokens, out, in, out_dtype == H24_DTYPE_F32 ? 4 : 2, aligned);
+  const bool w_aligned = in % 16 == 0 && aligned16(w);
+  const bool q_aligned = in % 16 == 0 && q_stride % 16 == 0 && q_stride >= in && aligned16(q);
+  const Plan plan = make_plan(tokens, out, in, out_dtype == H24_DTYPE_F32 ? 4 : 2);
+  int8_t *copy = nullptr;
+  int64_t w_stride = in;
+  if (plan.kind != kVec && in > 0 && !(w_aligned && q_aligned)) {
+    const int64_t pitch = (in + 15) / 16 * 16, w_rows = w_aligned ? 0 : out, q_rows = q_aligned ? 0 : tokens;
+    H24_CUDA_TRY(cudaMallocFromPoolAsync(reinterpret_cast<void **>(&copy), static_cast<size_t>((w_rows + q_rows) * pitch),
+                                         T->pool, s));
+    const RepackArgs rw{w, in, copy, w_rows}, rq{q, q_stride, copy + w_rows * pitch, q_rows};
+    const int chunks = static_cast<int>(pitch / 16);
+    const int64_t blocks = ((w_rows + q_rows) * chunks + kRepackThreads - 1) / kRepackThreads;
+    const cudaError_t e = launch_pdl(repack_rows_kernel, dim3(wave_grid(blocks, 8)), dim3(kRepackThreads), s, rw, rq,
+                                     static_cast<int>(in), chunks);
+    if (e != cudaSuccess) {
+      cudaFreeAsync(copy, s);
+      return cuda_fail(e, "int8_linear: repack launch");
+    }
+    count_launches(1);
+    if (w_rows) w = rw.dst, w_stride = pitch;
+    if (q_rows) q = rq.dst, q_stride = pitch;
+  }
   a.n = plan.n;
   a.split = plan.split;
   CUtensorMap wmap{}, qmap{};
@@ -1019,14 +1074,24 @@ int launch_int8_linear(const Tables *T, const int8_t *q, const float *scale, int
     const int share = static_cast<int>(static_cast<int64_t>(kSmemPerSm) * a.tmem_cols / 512);
     smem = smem < part ? part : smem;
     smem = smem < share ? share : smem;
-    if (aligned && (!make_map(&wmap, w, out, in, in, kM) || !make_map(&qmap, q, tokens, in, q_stride, rows)))
+    // (An empty sum loads nothing and needs no maps.)
+    if (in > 0 && (!make_map(&wmap, w, out, w_stride, w_stride, kM) ||
+                   !make_map(&qmap, q, tokens, w_stride, q_stride, rows))) {
+      if (copy) cudaFreeAsync(copy, s);
       return fail(H24_ERR_CUDA, "int8_linear: cuTensorMapEncodeTiled failed");
+    }
   }
+  int rc;
   switch (out_dtype) {
-    case H24_DTYPE_F32: return launch_typed<float>(plan, aligned, wmap, qmap, a, smem, s);
-    case H24_DTYPE_F16: return launch_typed<__half>(plan, aligned, wmap, qmap, a, smem, s);
-    default: return launch_typed<__nv_bfloat16>(plan, aligned, wmap, qmap, a, smem, s);
+    case H24_DTYPE_F32: rc = launch_typed<float>(plan, w_aligned && q_aligned, wmap, qmap, a, smem, s); break;
+    case H24_DTYPE_F16: rc = launch_typed<__half>(plan, w_aligned && q_aligned, wmap, qmap, a, smem, s); break;
+    default: rc = launch_typed<__nv_bfloat16>(plan, w_aligned && q_aligned, wmap, qmap, a, smem, s); break;
   }
+  if (copy) {
+    const cudaError_t e = cudaFreeAsync(copy, s);
+    if (rc == H24_OK && e != cudaSuccess) rc = cuda_fail(e, "cudaFreeAsync");
+  }
+  return rc;
 }
 
 }  // namespace h24
