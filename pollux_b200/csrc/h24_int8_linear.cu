@@ -221,8 +221,7 @@ __device__ __forceinline__ uint4 load16_any(const int8_t *p, int valid, const in
 // bytes (a multiple of 16), zeros past their end: what TMA can read.  Where a
 // layer or its input is not 16-byte aligned, the copy and the tiles over it
 // (2 more bytes of traffic a byte) take [4096,1919] x [7680,1919] from 1,106 us
-// with tiles filled by hand to REPACK_BIG, and [20,1921] x [7680,1921] from 61 to
-// REPACK_SMALL.
+// with tiles filled by hand to 57, and [20,1921] x [7680,1921] from 61 to 14.
 struct RepackArgs {
   const int8_t *src;
   int64_t stride;
@@ -502,111 +501,125 @@ __global__ void __launch_bounds__(kVecThreads) int8_linear_vec_kernel(const LinA
   constexpr int U = 4;                            // 16-byte loads of each row in flight
   __shared__ __align__(16) uint8_t xs[T][kVecChunk];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const int64_t o0 = (static_cast<int64_t>(blockIdx.x) * (kVecThreads / 32) + warp) * R;
-  const int live = static_cast<int>(min(static_cast<int64_t>(R), a.out - o0));  // rows of this warp, maybe none
+  constexpr int kRows = kVecThreads / 32 * R;  // of a block
   const int8_t *wend = a.w + static_cast<int64_t>(a.out) * a.in;
   // Towards L2 while the kernel before this one ends (L2 holds whatever that
   // one may still write, so the loads after it see it).
-  if (kAhead)
-    for (int r = 0; r < live; ++r)
+  if (kAhead) {
+    const int64_t o0 = (static_cast<int64_t>(blockIdx.x) * (kVecThreads / 32) + warp) * R;
+    for (int r = 0; r < R && o0 + r < a.out; ++r)
       for (int k = lane * 128; k < a.in; k += 32 * 128)
         asm volatile("prefetch.global.L2 [%0];" ::"l"(a.w + (o0 + r) * a.in + k));
+  }
   pdl_enter();
-  // The blocks around these rows lie inside the matrix.
-  const bool inner = live == R && o0 * a.in >= 16 && (o0 + R) * a.in + 32 <= static_cast<int64_t>(a.out) * a.in;
-  // Lane k * R + r finishes row r, token k; what it needs is asked for first.
-  const int fr = lane % R, fk = lane / R;
-  const bool finishes = fr < live && fk < T && fk < a.tokens;
-  const float sc = finishes ? __ldg(a.scale + fk) : 0.f, ws = finishes ? weight_scale(a.mu16, o0 + fr) : 0.f;
-  const float b = finishes && a.bias ? __ldg(a.bias + o0 + fr) : 0.f;
-  uint4 w[R][U], next[kAligned ? 1 : R][kAligned ? 1 : U];
-  // Vectors v0 + 32 u + lane of the rows, of the kn bytes from k0.  `settle`
-  // makes them from their two blocks where the rows are off the boundary.
-  auto ask = [&](int k0, int kn, int v0) {
-    const int vecs = (kn + 15) / 16;
+  bool placed = false;  // the tokens are in shared memory, all of them
+  for (int64_t group = blockIdx.x; group * kRows < a.out; group += gridDim.x) {
+    const int64_t o0 = (group * (kVecThreads / 32) + warp) * R;
+    const int live = static_cast<int>(min(static_cast<int64_t>(R), a.out - o0));  // rows of this warp, maybe none
+    // The blocks around these rows lie inside the matrix.
+    const bool inner = live == R && o0 * a.in >= 16 && (o0 + R) * a.in + 32 <= static_cast<int64_t>(a.out) * a.in;
+    // Lane k * R + r finishes row r, token k; what it needs is asked for first.
+    const int fr = lane % R, fk = lane / R;
+    const bool finishes = fr < live && fk < T && fk < a.tokens;
+    const float sc = finishes ? __ldg(a.scale + fk) : 0.f, ws = finishes ? weight_scale(a.mu16, o0 + fr) : 0.f;
+    const float b = finishes && a.bias ? __ldg(a.bias + o0 + fr) : 0.f;
+    uint4 w[R][U], next[kAligned ? 1 : R][kAligned ? 1 : U];
+    // Vectors v0 + 32 u + lane of the rows, of the kn bytes from k0.  `settle`
+    // makes them from their two blocks where the rows are off the boundary.
+    auto ask = [&](int k0, int kn, int v0) {
+      const int vecs = (kn + 15) / 16;
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+      for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int v = v0 + 32 * u + lane;
-        const int8_t *p = a.w + (o0 + r) * a.in + k0 + 16 * v;
-        if constexpr (kAligned) {
-          w[r][u] = v < vecs && r < live ? __ldcs(reinterpret_cast<const uint4 *>(p)) : make_uint4(0, 0, 0, 0);
-        } else if (inner) {
-          p -= 16 * max(v - (vecs - 1), 0);
-          const uint4 *block = reinterpret_cast<const uint4 *>(p - offset16(p));
-          w[r][u] = __ldg(block);
-          next[r][u] = __ldg(block + 1);
-        } else {
-          w[r][u] = v < vecs && r < live ? load16_any(p, kn - 16 * v, a.w, wend) : make_uint4(0, 0, 0, 0);
+        for (int u = 0; u < U; ++u) {
+          const int v = v0 + 32 * u + lane;
+          const int8_t *p = a.w + (o0 + r) * a.in + k0 + 16 * v;
+          if constexpr (kAligned) {
+            w[r][u] = v < vecs && r < live ? __ldcs(reinterpret_cast<const uint4 *>(p)) : make_uint4(0, 0, 0, 0);
+          } else if (inner) {
+            p -= 16 * max(v - (vecs - 1), 0);
+            const uint4 *block = reinterpret_cast<const uint4 *>(p - offset16(p));
+            w[r][u] = __ldg(block);
+            next[r][u] = __ldg(block + 1);
+          } else {
+            w[r][u] = v < vecs && r < live ? load16_any(p, kn - 16 * v, a.w, wend) : make_uint4(0, 0, 0, 0);
+          }
+        }
+    };
+    auto settle = [&](int k0, int kn, int v0) {
+      if constexpr (!kAligned) {
+        if (inner) {
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+              w[r][u] = join16(w[r][u], next[r][u], offset16(a.w + (o0 + r) * a.in + k0),
+                               kn - 16 * (v0 + 32 * u + lane));
         }
       }
-  };
-  auto settle = [&](int k0, int kn, int v0) {
-    if constexpr (!kAligned) {
-      if (inner) {
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-          for (int u = 0; u < U; ++u)
-            w[r][u] = join16(w[r][u], next[r][u], offset16(a.w + (o0 + r) * a.in + k0),
-                             kn - 16 * (v0 + 32 * u + lane));
+    };
+    int acc[R][T] = {};
+    for (int k0 = 0; k0 < a.in; k0 += kVecChunk) {
+      const int kn = min(kVecChunk, a.in - k0), vecs = (kn + 15) / 16;
+      ask(k0, kn, 0);  // on their way while the tokens are placed
+      if (!placed) {
+        if (k0 || group != blockIdx.x) __syncthreads();
+        const int8_t *qend = a.q + (a.tokens - 1) * a.q_stride + a.in;
+        for (int i = t; i < T * vecs; i += kVecThreads) {
+          const int tok = i / vecs, v = i - tok * vecs;
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (tok < a.tokens) {
+            const int8_t *p = a.q + tok * a.q_stride + k0 + 16 * v;
+            x = kAligned ? __ldg(reinterpret_cast<const uint4 *>(p)) : load16_any(p, kn - 16 * v, a.q, qend);
+          }
+          *reinterpret_cast<uint4 *>(&xs[tok][16 * v]) = x;
+        }
+        __syncthreads();
+        placed = a.in <= kVecChunk;
       }
-    }
-  };
-  int acc[R][T] = {};
-  for (int k0 = 0; k0 < a.in; k0 += kVecChunk) {
-    const int kn = min(kVecChunk, a.in - k0), vecs = (kn + 15) / 16;
-    ask(k0, kn, 0);  // on their way while the tokens are placed
-    if (k0) __syncthreads();
-    const int8_t *qend = a.q + (a.tokens - 1) * a.q_stride + a.in;
-    for (int i = t; i < T * vecs; i += kVecThreads) {
-      const int tok = i / vecs, v = i - tok * vecs;
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (tok < a.tokens) {
-        const int8_t *p = a.q + tok * a.q_stride + k0 + 16 * v;
-        x = kAligned ? __ldg(reinterpret_cast<const uint4 *>(p)) : load16_any(p, kn - 16 * v, a.q, qend);
-      }
-      *reinterpret_cast<uint4 *>(&xs[tok][16 * v]) = x;
-    }
-    __syncthreads();
-    for (int v0 = 0; v0 < vecs; v0 += 32 * U) {
-      if (v0) ask(k0, kn, v0);
-      settle(k0, kn, v0);
+      for (int v0 = 0; v0 < vecs; v0 += 32 * U) {
+        if (v0) ask(k0, kn, v0);
+        settle(k0, kn, v0);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int v = v0 + 32 * u + lane;
-        if (v >= vecs) break;
+        for (int u = 0; u < U; ++u) {
+          const int v = v0 + 32 * u + lane;
+          if (v >= vecs) break;
 #pragma unroll
-        for (int k = 0; k < T; ++k) {
-          const int4 x = *reinterpret_cast<const int4 *>(&xs[k][16 * v]);
+          for (int k = 0; k < T; ++k) {
+            const int4 x = *reinterpret_cast<const int4 *>(&xs[k][16 * v]);
 #pragma unroll
-          for (int r = 0; r < R; ++r) {
-            acc[r][k] = __dp4a(static_cast<int>(w[r][u].x), x.x, acc[r][k]);
-            acc[r][k] = __dp4a(static_cast<int>(w[r][u].y), x.y, acc[r][k]);
-            acc[r][k] = __dp4a(static_cast<int>(w[r][u].z), x.z, acc[r][k]);
-            acc[r][k] = __dp4a(static_cast<int>(w[r][u].w), x.w, acc[r][k]);
+            for (int r = 0; r < R; ++r) {
+              acc[r][k] = __dp4a(static_cast<int>(w[r][u].x), x.x, acc[r][k]);
+              acc[r][k] = __dp4a(static_cast<int>(w[r][u].y), x.y, acc[r][k]);
+              acc[r][k] = __dp4a(static_cast<int>(w[r][u].z), x.z, acc[r][k]);
+              acc[r][k] = __dp4a(static_cast<int>(w[r][u].w), x.w, acc[r][k]);
+            }
           }
         }
       }
     }
+    int mine = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int k = 0; k < T; ++k) {
+        const int sum = __reduce_add_sync(0xffffffffu, acc[r][k]);
+        if (lane == k * R + r) mine = sum;
+      }
+    if (finishes)
+      put(static_cast<Out *>(a.y) + fk * static_cast<int64_t>(a.out) + o0 + fr, finish(mine, sc, ws, b));
   }
-  int mine = 0;
-#pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int k = 0; k < T; ++k) {
-      const int sum = __reduce_add_sync(0xffffffffu, acc[r][k]);
-      if (lane == k * R + r) mine = sum;
-    }
-  if (finishes)
-    put(static_cast<Out *>(a.y) + fk * static_cast<int64_t>(a.out) + o0 + fr, finish(mine, sc, ws, b));
 }
 
 template <int T, int R, bool kAhead, bool kAligned, typename Out>
 int launch_vec(const LinArgs &a, cudaStream_t s) {
   const int64_t per_block = static_cast<int64_t>(kVecThreads / 32) * R;
-  const unsigned grid = static_cast<unsigned>((a.out + per_block - 1) / per_block);
+  const int64_t groups = (a.out + per_block - 1) / per_block;
+  // Off the boundary placing the tokens costs as much as eight rows: the blocks
+  // of one wave place them once each.  ([1,1919] x [50688,1919]: 39 us, 49 with a
+  // block for each eight rows.)
+  const auto kernel = int8_linear_vec_kernel<T, R, kAhead, kAligned, Out>;
+  const int grid = kAligned ? static_cast<int>(groups) : wave_grid(groups, blocks_per_sm(kernel, kVecThreads, 0));
   H24_CUDA_TRY(launch_pdl(int8_linear_vec_kernel<T, R, kAhead, kAligned, Out>, dim3(grid), dim3(kVecThreads), s, a));
   count_launches(1);
   return H24_OK;
