@@ -7,6 +7,16 @@
 // The weights are the M operand (128 output features a tile, one TMEM lane
 // each) and the tokens the N operand, so one token costs 16 columns of a tile
 // and not 128 rows, and a warp's 32 lanes store 32 neighbouring outputs.
+//
+// Three kernels, chosen by make_plan from an estimate of bytes and latency:
+//   one to four tokens: dp4a over the weight rows, bound by their bytes
+//     ([1,1920] x [50688,1920] 15.0-16.1 us: 0.93-0.99 of the measured HBM rate);
+//   a few to a few hundred: tiles of 128 x n, the k split over a cluster where
+//     tiles are few; bound by a launch's chain of latencies (5.4 us for [32,1920]
+//     x [7680,1920], 2.3 of them bytes) and by the fill of shared memory;
+//   many: pairs of SMs on 256 x n tiles, bound by L2: at 2.6-2.7 PTOP/s the pairs
+//     fetch 10-11 TB/s through it, what it gave in every run ([4096,1920] x
+//     [7680,1920] bf16 46.8 us, [1024,1920] x [50688,1920] fp32 88.7).
 #include <cuda.h>  // CUtensorMap and its enums; the entry point is looked up at run time
 
 #include "h24_internal.cuh"
@@ -497,8 +507,8 @@ constexpr int kVecThreads = 256;
 // TMEM.
 template <int T, int R, bool kAhead, bool kAligned, typename Out>
 __global__ void __launch_bounds__(kVecThreads) int8_linear_vec_kernel(const LinArgs a) {
-  constexpr int kVecChunk = T > 4 ? 4096 : 8192;  // k per pass: the tokens' rows of a pass lie in shared memory
-  constexpr int U = 4;                            // 16-byte loads of each row in flight
+  constexpr int kVecChunk = 8192;  // k per pass: the tokens' rows of a pass lie in shared memory
+  constexpr int U = 4;             // 16-byte loads of each row in flight
   __shared__ __align__(16) uint8_t xs[T][kVecChunk];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   constexpr int kRows = kVecThreads / 32 * R;  // of a block
@@ -618,9 +628,9 @@ int launch_vec(const LinArgs &a, cudaStream_t s) {
   // Off the boundary placing the tokens costs as much as eight rows: the blocks
   // of one wave place them once each.  ([1,1919] x [50688,1919]: 39 us, 49 with a
   // block for each eight rows.)
-  const auto kernel = int8_linear_vec_kernel<T, R, kAhead, kAligned, Out>;
-  const int grid = kAligned ? static_cast<int>(groups) : wave_grid(groups, blocks_per_sm(kernel, kVecThreads, 0));
-  H24_CUDA_TRY(launch_pdl(int8_linear_vec_kernel<T, R, kAhead, kAligned, Out>, dim3(grid), dim3(kVecThreads), s, a));
+  constexpr auto kernel = int8_linear_vec_kernel<T, R, kAhead, kAligned, Out>;
+  const int grid = kAligned ? static_cast<int>(groups) : wave_grid(groups, blocks_per_sm_once<kernel>(kVecThreads));
+  H24_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(kVecThreads), s, a));
   count_launches(1);
   return H24_OK;
 }

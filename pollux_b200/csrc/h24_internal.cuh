@@ -182,6 +182,18 @@ int blocks_per_sm(K kernel, int threads, size_t dyn_smem) {
   return per;
 }
 
+// blocks_per_sm without dynamic shared memory, asked of the driver once per
+// kernel and block size (a question costs a short launch as much as a third of
+// its time).
+template <auto kernel>
+int blocks_per_sm_once(int threads) {
+  static std::atomic<int> known[33];  // by warps
+  std::atomic<int> &k = known[threads / 32];
+  int per = k.load(std::memory_order_relaxed);
+  if (per == 0) k.store(per = blocks_per_sm(kernel, threads, 0), std::memory_order_relaxed);
+  return per;
+}
+
 // Grid of at most one resident wave (SMs x `per_sm` blocks), fewer when the
 // work needs fewer blocks: a grid-stride kernel then finishes in one wave
 // instead of leaving a partial second one.
