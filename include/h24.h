@@ -200,7 +200,10 @@ int h24_rows_int8_dequant(const int8_t *q, const float *scale, int64_t rows, int
  * h24_int8_dequant reads it).  The sum is exact in int32, the scaling fp32, y
  * (contiguous, element type out_dtype) rounded once.  Row t of q starts at
  * t * q_stride bytes; bias: out_features fp32 or NULL.  in_features is at
- * most 131,000 (the sum cannot overflow). */
+ * most 131,000 (the sum cannot overflow).  With five tokens or more, rows that
+ * are not 16-byte aligned are copied to a stream-ordered workspace from the
+ * library's device memory pool, freed on the same stream.  h24_check reports
+ * a bounded wait that ran out. */
 int h24_int8_linear(const int8_t *q, const float *scale, int64_t tokens, int64_t q_stride,
                     const int8_t *w, const uint16_t *mu16, int64_t out_features, int64_t in_features,
                     const float *bias, int out_dtype, void *y, void *stream);
@@ -368,7 +371,8 @@ int64_t h24_launch_count(void);
 
 /* Synchronise `stream` and report a device-side failure of earlier quantize
  * calls on the current device: H24_ERR_TIMEOUT if a bounded wait inside the
- * screening kernel ran out (the word is then cleared), else H24_OK. */
+ * screening kernel, the LUT GEMV or the int8 product ran out (the word is then
+ * cleared), else H24_OK. */
 int h24_check(void *stream);
 
 

@@ -20,9 +20,11 @@ _INF = float("inf")
 def _setting(v, rows: int, dtype: torch.dtype, dev: torch.device, name: str):
     """(tensor kept alive, pointer or None, scalar) of one sampling setting."""
     if not isinstance(v, torch.Tensor):
-        return None, None, v
+        return None, None, float(v)
     if v.numel() != rows:
         raise ValueError(f"{name} must be a number or hold one value for each of the {rows} rows, got {tuple(v.shape)}")
+    if dtype == torch.int32 and v.dtype == torch.int64:
+        v = v.clamp(0, MAX_VOCAB)  # what the vocabulary holds, and no more than 32 bits
     if v.device != dev or v.dtype != dtype:
         v = v.to(device=dev, dtype=dtype)
     if not v.is_contiguous():

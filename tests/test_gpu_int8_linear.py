@@ -149,3 +149,42 @@ def test_head_without_materialize(m):
     assert ((y.double() - want).abs() <= bound + want.abs() * 2.0 ** -8 + 1e-6).all()
     lin.materialize()
     assert torch.equal(lin(x), torch.nn.functional.linear(x, lin.weight.to(x.dtype)))
+
+
+def test_offsets_beyond_32_bits(m):
+    """An output of 2.5e9 elements, and input rows 1.5e9 bytes apart."""
+    q, scale, w, mu, b = _inputs(50000, 50688, 32, 6)
+    scale = scale / 100
+    y = m.int8_linear(q, scale, w, mu, b, torch.bfloat16)
+    for rows in (slice(0, 3), slice(24990, 24994), slice(49997, 50000)):
+        _check(y[rows], q[rows], scale[rows], w, mu, b)
+    del y
+    base = torch.empty(4_500_000_100, device="cuda", dtype=torch.int8)
+    for tokens in (3, 4):
+        for k in (96, 93):
+            v = base.as_strided((tokens, k), (1_500_000_000, 1))[:3]
+            v.copy_(q[:3].repeat(1, 3)[:, :k])
+            w2, s2 = w[:300].repeat(1, 3)[:, :k].contiguous(), scale[:3]
+            assert torch.equal(m.int8_linear(v, s2, w2, mu[:300]), m.int8_linear(v.contiguous(), s2, w2, mu[:300]))
+    del base
+    base = torch.empty(4_500_000_100, device="cuda", dtype=torch.int8)
+    v = base.as_strided((6, 96), (800_000_000, 1))
+    v.copy_(q[:6].repeat(1, 3))
+    w2 = w[:300].repeat(1, 3)
+    assert torch.equal(m.int8_linear(v, scale[:6], w2, mu[:300]), m.int8_linear(v.contiguous(), scale[:6], w2, mu[:300]))
+
+
+@pytest.mark.parametrize("tokens,in_f", [(1, 1920), (3, 333), (40, 480), (40, 333), (700, 1001)])
+def test_in_a_graph(m, tokens, in_f):
+    """Every path, the copy of unaligned rows among them, captured and replayed on new inputs in place."""
+    q, scale, w, mu, b = _inputs(tokens, 1000, in_f, 21)
+    m.int8_linear(q, scale, w, mu, b)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = m.int8_linear(q, scale, w, mu, b)
+    for seed in (1, 2):
+        for dst, src in zip((q, scale, w, mu, b), _inputs(tokens, 1000, in_f, seed)):
+            dst.copy_(src)
+        graph.replay()
+        _check(y, q, scale, w, mu, b)

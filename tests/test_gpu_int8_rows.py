@@ -156,3 +156,17 @@ def test_more_rows_than_a_grid(m):
     q, scale, _ = m.add_rms_norm_int8(x, w)
     s = x.double()
     _check(q, scale, s, 1 / torch.sqrt((s * s).mean(-1) + 1e-6), 24)
+
+
+def test_offsets_beyond_32_bits(m):
+    """Rows 1.2e9 elements apart: element offsets pass 2^31, byte offsets 2^32."""
+    base = torch.empty(2_400_000_200, device="cuda", dtype=torch.bfloat16)
+    for cols in (96, 93):
+        x = base.as_strided((3, cols), (1_200_000_000, 1))
+        x.copy_(torch.randn(3, cols, device="cuda"))
+        w = torch.randn(cols, device="cuda").to(torch.bfloat16)
+        r = torch.randn(3, cols, device="cuda").to(torch.bfloat16)
+        for args in ((x, w, r), (r, w, x)):
+            got = m.add_rms_norm_int8(*args)
+            want = m.add_rms_norm_int8(*(a.contiguous() for a in args))
+            assert all(torch.equal(a, b) for a, b in zip(got, want))

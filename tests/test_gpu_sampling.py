@@ -213,3 +213,41 @@ def test_another_stream(m):
         got = [m.sample_tokens(logits, u, top_p=0.9) for _ in range(5)]
     torch.cuda.synchronize()
     assert all(torch.equal(g, want) for g in got)
+
+
+def test_offsets_beyond_32_bits(m):
+    base = torch.empty(2_400_060_000, device="cuda", dtype=torch.bfloat16)
+    logits = base.as_strided((3, 50688), (1_200_000_000, 1))
+    src, u = _logits(3, 50688, 61, torch.bfloat16)
+    logits.copy_(src)
+    for kw in (dict(), dict(top_k=40, top_p=0.9), dict(top_p=0.9)):
+        assert torch.equal(m.sample_tokens(logits, u, **kw), m.sample_tokens(src, u, **kw))
+
+
+def test_kinds_of_settings(m):
+    """64-bit counts, numpy numbers, ints for floats, and settings on the host."""
+    logits, u = _logits(4, 700, 62)
+    want = m.sample_tokens(logits, u, temperature=1.0, top_k=30, top_p=1.0, min_p=0.0)
+    assert torch.equal(m.sample_tokens(logits, u, temperature=1, top_k=30.0, top_p=1, min_p=0), want)
+    assert torch.equal(m.sample_tokens(logits, u, temperature=np.float32(1), top_k=np.int64(30), top_p=np.float64(1)), want)
+    assert torch.equal(m.sample_tokens(logits, u.cpu().double(), top_k=torch.full((4,), 30)), want)
+    assert torch.equal(m.sample_tokens(logits, u, top_k=torch.full((4,), 2 ** 40 + 30, device="cuda")), m.sample_tokens(logits, u))
+    assert torch.equal(m.sample_tokens(logits, u, top_k=10 ** 12), m.sample_tokens(logits, u))
+    with pytest.raises(ValueError, match="top_p"):
+        m.sample_tokens(logits, u, top_p=torch.ones(3, device="cuda"))
+    with pytest.raises(ValueError, match="u must"):
+        m.sample_tokens(logits, u[:3])
+
+
+@pytest.mark.parametrize("rows", [3, 400])
+def test_many_equal_tokens_at_a_cut(m, rows):
+    """More tokens of one value than the sorted list holds, at the cut of k and of p."""
+    vocab = 30000
+    logits = torch.zeros(rows, vocab, device="cuda")
+    logits[:, ::7] = 1.0
+    logits[:, 5] = 4.0
+    u = torch.linspace(0, 0.999, rows, device="cuda")
+    for kw in (dict(top_k=3000), dict(top_k=9000), dict(top_p=0.3), dict(top_p=0.7), dict(top_k=9000, top_p=0.5)):
+        tok = m.sample_tokens(logits, u, **kw)
+        pick = torch.arange(0, rows, max(1, rows // 3))
+        assert torch.equal(_check(m, logits[pick], u[pick], **kw), tok[pick])
