@@ -198,9 +198,14 @@ int blocks_per_sm_once(int threads) {
 // work needs fewer blocks: a grid-stride kernel then finishes in one wave
 // instead of leaving a partial second one.
 inline int wave_grid(int64_t want_blocks, int per_sm) {
-  int dev = 0, sms = 148;
+  static std::atomic<int> known[64];  // SMs of a device, asked once
+  int dev = 0;
   cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  int sms = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (sms == 0) {
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) sms = 148;
+    if (dev < 64) known[dev].store(sms, std::memory_order_relaxed);
+  }
   const int64_t cap = static_cast<int64_t>(sms) * per_sm;
   return static_cast<int>(want_blocks < 1 ? 1 : (want_blocks < cap ? want_blocks : cap));
 }
