@@ -873,8 +873,8 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
   };
   // The key of the last token a cut keeps, when it falls into step c.bin: the
   // first at which the count (mass) reaches `want`; `mass` gets what is kept in
-  // all, S.warp_kept what min-p leaves of it in each warp's part.  Steps with more tokens than the list are divided 2^11-fold by key
-  // until they fit.
+  // all, S.warp_kept what min-p leaves of it in each warp's part.  Steps with
+  // more tokens than the list are divided 2^11-fold by key until they fit.
   auto settle = [&](Cut c, bool by_mass, u64 want, u64 limit_key, bool masses, u64 *mass) -> u64 {
     const int bin = static_cast<int>(c.bin);
     u64 lo = order_key(fmaxf(static_cast<float>(bin - 2), 0.f) / kBinsPerNat, 0);
@@ -1051,39 +1051,51 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
     }
     cluster_sync(nc);
   }
-  u64 before = 0, mass = 0;
-  for (int w = 0; w < warp; ++w) before += S.warp_kept[w];
+  u64 base = 0, mass = 0;  // what is kept before this CTA, and in all
   for (int c = 0; c < nc; ++c) {
-    if (c < rank) before += S.kept[c];
+    if (c < rank) base += S.kept[c];
     mass += S.kept[c];
   }
   const u64 target = draw_target(R.u, mass);
-  if (before <= target && target < before + S.warp_kept[warp]) {  // one warp of the cluster
-    for (int i0 = v0; i0 < v1; i0 += 32) {
-      const int i = i0 + lane;
-      u64 own = 0;
-      if (i < v1) {
-        const V v = at(i);
+  if (target < base || target >= base + S.kept[rank]) return;  // (the same for the whole CTA)
+  // The warp's part in which the target falls, walked by all warps, a vector a
+  // thread and round.  (By its own warp, 25 reads from L2 one after the other
+  // took as long as the pass before.)
+  int part = 0;
+  for (; part < kWarps - 1; ++part) {
+    if (target < base + S.warp_kept[part]) break;
+    base += S.warp_kept[part];
+  }
+  const int p1 = static_cast<int>(static_cast<int64_t>(nvec) * (part + 1) / kWarps);
+  for (int p0 = static_cast<int>(static_cast<int64_t>(nvec) * part / kWarps); p0 < p1; p0 += kThreads) {
+    const int i = p0 + t;
+    u64 own = 0;
+    if (i < p1) {
+      const V v = at(i);
 #pragma unroll
-        for (int j = 0; j < kVN; ++j) own += kept(v.v[j], begin + i * kVN + j, &d);
-      }
-      const u64 all = warp_sum(own);
-      if (before + all <= target) {
-        before += all;
-        continue;
-      }
-      u64 here = before + warp_scan(own, lane) - own;
-      if (i < v1 && here <= target && target < here + own) {
-        const V v = at(i);
-#pragma unroll
-        for (int j = 0; j < kVN; ++j) {
-          const u64 w = kept(v.v[j], begin + i * kVN + j, &d);
-          if (w && here <= target && target < here + w) answer(begin + i * kVN + j, d);
-          here += w;
-        }
-      }
-      break;
+      for (int j = 0; j < kVN; ++j) own += kept(v.v[j], begin + i * kVN + j, &d);
     }
+    const u64 through = warp_scan(own, lane);
+    __syncthreads();  // S.red
+    if (lane == 31) S.red[warp] = through;
+    __syncthreads();
+    u64 here = base + through - own;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const u64 all = S.red[w];
+      if (w < warp) here += all;
+      base += all;
+    }
+    if (own && here <= target && target < here + own) {
+      const V v = at(i);
+#pragma unroll
+      for (int j = 0; j < kVN; ++j) {
+        const u64 w = kept(v.v[j], begin + i * kVN + j, &d);
+        if (w && here <= target && target < here + w) answer(begin + i * kVN + j, d);
+        here += w;
+      }
+    }
+    if (base > target) break;
   }
 }
 
