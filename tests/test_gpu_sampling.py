@@ -251,3 +251,16 @@ def test_many_equal_tokens_at_a_cut(m, rows):
         tok = m.sample_tokens(logits, u, **kw)
         pick = torch.arange(0, rows, max(1, rows // 3))
         assert torch.equal(_check(m, logits[pick], u[pick], **kw), tok[pick])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("spread", [0.5, 2.0, 6.0])
+def test_cut_at_p_does_not_depend_on_the_batch(m, spread, dtype):
+    """From flat rows, whose nucleus is most of the vocabulary, to peaked ones, alone and in batches of every kind."""
+    logits, u = _logits(600, 9001, 71, dtype, spread)
+    for kw in (dict(top_p=0.5), dict(top_p=0.9), dict(top_p=0.95), dict(top_p=0.97, temperature=0.7), dict(top_p=0.9, min_p=0.001)):
+        want = m.sample_tokens(logits, u, **kw)
+        for n in (1, 7, 40, 100, 160):
+            assert torch.equal(m.sample_tokens(logits[:n], u[:n], **kw), want[:n])
+        pick = torch.tensor([0, 299, 599], device="cuda")
+        assert torch.equal(_check(m, logits[pick], u[pick], **kw), want[pick])
