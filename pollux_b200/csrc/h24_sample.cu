@@ -29,9 +29,11 @@
 //     kept, and the warp in whose part the target falls walks it.
 //   neither, or a min-p that leaves less than p: the walk alone.
 // What bounds it, measured on a B200: one row, the chain of a dozen barriers
-// and exchanges ([1,50688] fp32, k = 50, p = 0.9: 10.9 us; no cut: 7.2); many
-// rows, instruction issue and the second read from L2 ([512,50688] fp32: no
-// cut 67 us, k = 50 59, p = 0.9 142, for 15.9 us of HBM traffic).
+// and exchanges ([1,50688] fp32, k = 50, p = 0.9: 10.9 us; no cut: 7.3); many
+// rows, instruction issue and the second and third read from L2 ([512,50688]
+// fp32: no cut 51 us, k = 50 58, p = 0.9 127, for 15.9 us of HBM traffic).  For
+// a cut at p, a list bounded by the threads' maxima as for k was tried: half of
+// the rows' cuts lie behind 700 tokens, and 2,200 cost what the steps cost.
 //
 // "z descending, index ascending" is one 64-bit key: |z|'s bits above the
 // index (z <= 0, so |z| ascending is z descending, and the bits of
@@ -1136,7 +1138,7 @@ int launch_sample_typed(const SampleArgs &a, cudaStream_t s) {
   // Clusters where a CTA each fits an SM: the most CTAs a row that are there at
   // once, with slices of at least 1,024 logits.  Rows enough for the SMs by
   // themselves, or too long for a cluster, run a CTA a row that reads it from
-  // L2 in each pass ([512,50688] fp32, p = 0.9: 142 us, in clusters of four 275;
+  // L2 in each pass ([512,50688] fp32, p = 0.9: 127 us, in clusters of four 275;
   // [64,50688] bf16, p = 0.95: 60 us, in clusters of two 36; [1,50688] fp32,
   // k = 50: 15.6 us, in a cluster of eight 10.9).
   int nc = kMaxCluster;
