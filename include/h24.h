@@ -213,7 +213,7 @@ int h24_int8_linear(const int8_t *q, const float *scale, int64_t tokens, int64_t
  *   z_i = (l_i - max l) * fp32(1 / T), w_i = rint(exp(z_i) * 2^40) (64 bits);
  *   in the order of z descending, ties by index: the first top_k (0 or less:
  *   all); of these, those whose mass before them is below ceil(top_p * their
- *   mass) (at least the first; top_p >= 1: all); of these, w_i >=
+ *   mass) (at least the first; top_p >= 1 or NaN: all); of these, w_i >=
  *   ceil(min_p * 2^40);
  *   tokens[r] = the first index at which the running mass of what is left, in
  *   the order of the indices, exceeds floor(u * mass).

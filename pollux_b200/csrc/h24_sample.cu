@@ -318,6 +318,7 @@ __global__ void __launch_bounds__(kThreads, kHeld ? 1 : 2) sample_cluster_kernel
     float temp = a.temperature ? a.temperature[r] : a.temperature1;
     R.k = a.top_k ? a.top_k[r] : a.top_k1;
     R.p = a.top_p ? a.top_p[r] : a.top_p1;
+    if (R.p < 0.f) R.p = 0.f;  // the first token alone
     R.least = weight_floor(a.min_p ? a.min_p[r] : a.min_p1);
     R.u = a.u[r];
     if (!(temp > 0.f)) temp = 1.f, R.k = 1;

@@ -264,3 +264,27 @@ def test_cut_at_p_does_not_depend_on_the_batch(m, spread, dtype):
             assert torch.equal(m.sample_tokens(logits[:n], u[:n], **kw), want[:n])
         pick = torch.tensor([0, 299, 599], device="cuda")
         assert torch.equal(_check(m, logits[pick], u[pick], **kw), want[pick])
+
+
+@pytest.mark.parametrize("rows", [4, 300])
+def test_settings_out_of_range_in_tensors(m, rows):
+    """What a number would be refused for has a meaning in a tensor, which is
+    not looked at on the host: below 0 as 0, above 1 and NaN as no cut."""
+    logits, u = _logits(rows, 4001, 81)
+    def one(v):
+        return torch.full((rows,), v, device="cuda")
+    plain = m.sample_tokens(logits, u)
+    best = logits.argmax(-1)
+    assert torch.equal(m.sample_tokens(logits, u, top_p=one(-5.0)), best)
+    assert torch.equal(m.sample_tokens(logits, u, top_p=one(float("-inf"))), best)
+    assert torch.equal(m.sample_tokens(logits, u, top_p=one(7.0)), plain)
+    assert torch.equal(m.sample_tokens(logits, u, top_p=one(float("nan"))), plain)
+    assert torch.equal(m.sample_tokens(logits, u, min_p=one(-1.0)), plain)
+    assert torch.equal(m.sample_tokens(logits, u, min_p=one(9.0)), best)
+    assert torch.equal(m.sample_tokens(logits, u, min_p=one(float("nan"))), plain)
+    assert torch.equal(m.sample_tokens(logits, u, top_k=one(-3)), plain)
+    assert torch.equal(m.sample_tokens(logits, u, temperature=one(-2.0)), best)
+    assert torch.equal(m.sample_tokens(logits, u, temperature=one(float("nan"))), best)
+    spread = m.sample_tokens(logits, u, temperature=one(float("inf")))
+    flat = m.sample_tokens(torch.zeros_like(logits), u)
+    assert torch.equal(spread, flat)
