@@ -273,11 +273,11 @@ __device__ __forceinline__ void tmem_wait32(int (&r)[32]) {
 #undef H24_I8
 #undef H24_O8
 
-// (The scales come by shuffle, loaded before: a load inside each column's test
-// put its latency between every two stores, 11.5 us a 256 x 256 tile.)
 // 32 columns of this warp's lanes to the outputs of `left` (at least 1) tokens
 // at `col` (of the first feature of the warp; the same for all lanes), lane
-// l's feature at col + l.  Lane j holds token j's scale.
+// l's feature at col + l.  Lane j holds token j's scale, loaded before: a load
+// inside each column's test put its latency between every two stores (11.5 us
+// a 256 x 256 tile).
 template <typename Out>
 __device__ __forceinline__ void store32(const int (&r)[32], float scales, int left, float ws, float b, Out *col,
                                         int64_t pitch, uint32_t lane, bool live) {
@@ -921,7 +921,7 @@ Plan make_plan(int64_t tokens, int64_t out, int64_t in, int out_size) {
       if (us < best_us) best_us = us, best = {kSplit, n, split};
     }
   }
-  for (int n = 32; n <= 256; n += 32) {
+  for (int n = 32; n <= 256 && in > 0; n += 32) {  // (an empty sum has no MMA to fill a pair's accumulators)
     if (n > 32 && tokens <= n - 32) break;
     const double us = pair_us(tokens, out, kblocks, n, hbm_us);
     if (us < best_us) best_us = us, best = {kPair, n, 1};

@@ -188,3 +188,14 @@ def test_in_a_graph(m, tokens, in_f):
             dst.copy_(src)
         graph.replay()
         _check(y, q, scale, w, mu, b)
+
+
+@pytest.mark.parametrize("tokens", [1, 5, 300, 3000])
+def test_empty_sum(m, tokens):
+    """in_features 0 in every size that would take another path: the bias, or zeros, after a call that left sums in TMEM."""
+    full = _inputs(tokens, 50688, 128, 3)
+    m.int8_linear(*full, torch.bfloat16)
+    q, scale, w, mu, b = full
+    y = m.int8_linear(q[:, :0], scale, w[:, :0], mu, b, torch.bfloat16)
+    assert torch.equal(y, b.to(torch.bfloat16).expand(tokens, 50688))
+    assert (m.int8_linear(q[:, :0], scale, w[:, :0], mu, None, torch.float16) == 0).all()
