@@ -178,8 +178,10 @@ int h24_int8_dequant(const int8_t *q, const uint16_t *mu16, int64_t rows, int64_
  * (H24_DTYPE_*); row r of x starts at r * x_stride elements, of residual at
  * r * residual_stride; q, scale and residual_out are contiguous.  gain: cols
  * elements of `dtype` or of H24_DTYPE_F32 (gain_dtype).  residual_out may be
- * x or residual itself where that is contiguous.  A NaN in a row makes its
- * scale NaN and every q 0. */
+ * x or residual itself where that is contiguous.  A NaN or an infinite s makes
+ * the row's scale NaN and every q 0; a finite row whose squares pass fp32's
+ * range is normed as any other (with a 16-bit residual_out over x or residual:
+ * from the rounded sum). */
 int h24_add_rms_norm_int8(const void *x, const void *residual, const void *gain, int gain_dtype,
                           int64_t rows, int64_t cols, int64_t x_stride, int64_t residual_stride,
                           int dtype, float eps, int8_t *q, float *scale, void *residual_out,

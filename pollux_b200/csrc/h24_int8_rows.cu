@@ -8,7 +8,9 @@
 //   q_c    = rint(v_c * (i * 127 / mu))                 within [-127, 127]
 // Quantisation alone takes v = x and i = 1.  A NaN in a row (or an infinite
 // element under the norm) makes its scale NaN and every q 0, as the row
-// quantiser of the weights does.  The norm is taken of the unrounded sum.
+// quantiser of the weights does.  The norm is taken of the unrounded sum.  Where
+// the sum of squares passes fp32's range (an element above 1.8e19), it is taken
+// again of s * 2^-80: see wide_factor.
 //
 // Bound by HBM where there are rows: 7 bytes an element in bf16 (x, r, r', q).
 // On a B200 [4096,1920] bf16 takes 10.5 us (5.3 TB/s, 0.80 of the measured
@@ -21,6 +23,7 @@ namespace h24 {
 namespace {
 
 constexpr float kRowEps = 1e-8f;  // smallest mu, as for the weights (pack.py:124-136)
+constexpr float kSmall = 8.271806125530277e-25f;  // 2^-80
 constexpr int kDeqThreads = 256;
 
 template <int DT>
@@ -92,16 +95,29 @@ __device__ __forceinline__ void reduce_row(float &ss, float &m, float (*red)[32]
 
 // mu / 127 and the factor that takes v to q, from a row's sums.  |v * factor|
 // is at most 127 (1 + 2^-21), which rounds to 127: q needs no clamp.  A row
-// whose mu is not finite has every q 0: `dead`.
+// whose mu is not finite has every q 0: `dead`.  A sum of squares that is not
+// finite makes mu NaN (ss - ss; it is 0 of any other).
 template <bool kNorm>
 __device__ __forceinline__ float row_factor(const RowArgs &a, float ss, float m, float *scale, bool *dead) {
   const float inv = kNorm ? 1.0f / sqrtf(ss / static_cast<float>(a.cols) + a.eps) : 1.0f;
-  float mu = m * inv;
+  float mu = kNorm ? fmaf(m, inv, ss - ss) : m;
   mu = mu != mu ? mu : fmaxf(mu, kRowEps);
   *scale = mu / 127.0f;
   *dead = !(mu <= 3.402823466e38f);
   return inv * (127.0f / mu);
 }
+
+// The same for a finite row whose squares pass fp32's range, from big, the sum of
+// (s * 2^-80)^2.  That cannot overflow, and what underflows in it is below a
+// rounding of such a sum.  inv is i * 2^80, since i itself may be too small a
+// number; q takes v to 127 v / m, without i, unless mu is at its floor.
+__device__ __forceinline__ float wide_factor(const RowArgs &a, float big, float m, float *scale) {
+  const float inv = 1.0f / sqrtf(big / static_cast<float>(a.cols) + a.eps * kSmall * kSmall);
+  const float mu = fmaxf(m * kSmall * inv, kRowEps);
+  *scale = mu / 127.0f;
+  return mu > kRowEps ? 127.0f / m : inv * (127.0f / kRowEps) * kSmall;
+}
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
 
 // The elements of a 16-byte group as fp32.
 template <int DT>
@@ -113,13 +129,49 @@ __device__ __forceinline__ void widen(uint4 raw, float (&v)[Elem<DT>::kVec]) {
   for (int j = 0; j < E::kVec; ++j) v[j] = E::up(x[j]);
 }
 
+// The block's finite rows among those that rows_int8_kernel gave a NaN scale,
+// read again by the element.  Where the sum was written over x or the residual,
+// it stands for them, in 16 bits rounded.
+template <int DT>
+__device__ __noinline__ void wide_rows(const RowArgs &a, float (*red)[32]) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  const bool over = a.residual_out && (a.residual_out == a.x || a.residual_out == a.residual);
+  auto sum_at = [&](int64_t r, int64_t c) {
+    if (over) return E::up(static_cast<const T *>(a.residual_out)[r * a.cols + c]);
+    const float s = E::up(static_cast<const T *>(a.x)[r * a.x_stride + c]);
+    return a.residual ? s + E::up(static_cast<const T *>(a.residual)[r * a.residual_stride + c]) : s;
+  };
+  auto gain = [&](int64_t c) {
+    return a.gain_f32 ? static_cast<const float *>(a.gain)[c] : E::up(static_cast<const T *>(a.gain)[c]);
+  };
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const float marked = a.scale[r];
+    if (marked == marked) continue;
+    float big = 0.f, m = 0.f;
+    for (int64_t c = threadIdx.x; c < a.cols; c += blockDim.x) {
+      const float s = sum_at(r, c);
+      big = fmaf(s * kSmall, s * kSmall, big);
+      m = nan_max(m, fabsf(s * gain(c)));
+    }
+    __syncthreads();  // all have read the mark, and what red held
+    reduce_row(big, m, red, blockDim.x >> 5);
+    if (!finite(big) || !finite(m)) continue;  // (the same for the whole block)
+    float scale;
+    const float k = wide_factor(a, big, m, &scale);
+    for (int64_t c = threadIdx.x; c < a.cols; c += blockDim.x)
+      a.q[r * a.cols + c] = static_cast<int8_t>(quant_act(sum_at(r, c) * gain(c), k));
+    if (threadIdx.x == 0) a.scale[r] = scale;
+  }
+}
+
 // Thread t of a block holds the 16-byte groups t, t + blockDim.x, ... (at most
 // NV) of its row in registers, so the row is read once.  A block walks rows r, r + gridDim.x, ..., and asks for
 // the next row before it reduces the present one.  Rows that are not 16-byte
 // aligned, or end inside a group, are read and written by the element in the
 // same groups: a row's result does not depend on where it lies.
 template <int DT, bool kAligned, int NV, bool kNorm>
-__global__ void __launch_bounds__(NV < 8 ? 512 : 1024) rows_int8_kernel(const RowArgs a) {
+__global__ void __launch_bounds__(NV < 8 ? 512 : 1024) rows_int8_kernel(const __grid_constant__ RowArgs a) {
   using E = Elem<DT>;
   using T = typename E::T;
   constexpr int VEC = E::kVec;
@@ -235,6 +287,17 @@ __global__ void __launch_bounds__(NV < 8 ? 512 : 1024) rows_int8_kernel(const Ro
     }
     if (t == 0) a.scale[r] = scale;
   }
+  // Rows that look like NaN are looked at here, outside the loop: a test and a
+  // second sum inside it took [4096,7680] bf16 from 36.6 us to 44 and more (this:
+  // 37.1).  The squares of fp16 cannot overflow.
+  if (kNorm && DT != H24_DTYPE_F16) {
+    bool marked = false;
+    __syncthreads();
+    for (int64_t r = blockIdx.x + static_cast<int64_t>(t) * gridDim.x; r < a.rows;
+         r += static_cast<int64_t>(nt) * gridDim.x)
+      marked |= a.scale[r] != a.scale[r];
+    if (__syncthreads_or(marked)) wide_rows<DT>(a, red[0]);
+  }
 }
 
 constexpr int kLongThreads = 512;
@@ -267,7 +330,20 @@ __global__ void __launch_bounds__(kLongThreads) rows_int8_long_kernel(const RowA
   reduce_row(ss, m, red, kLongThreads / 32);
   float scale;
   bool dead;
-  const float k = row_factor<kNorm>(a, ss, m, &scale, &dead);
+  float k = row_factor<kNorm>(a, ss, m, &scale, &dead);
+  if (kNorm && !finite(ss) && finite(m)) {  // (the same for the whole block)
+    float big = 0.f, unused = 0.f;
+    for (int64_t c = t; c < a.cols; c += kLongThreads) {
+      const float s = (E::up(x[c]) + (res ? E::up(res[c]) : 0.f)) * kSmall;
+      big = fmaf(s, s, big);
+    }
+    __syncthreads();  // red has been read
+    reduce_row(big, unused, red, kLongThreads / 32);
+    if (finite(big)) {
+      k = wide_factor(a, big, m, &scale);
+      dead = false;
+    }
+  }
   for (int64_t c = t; c < a.cols; c += kLongThreads) {
     float s = E::up(x[c]);
     if (kNorm) {
