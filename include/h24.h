@@ -181,7 +181,7 @@ int h24_int8_dequant(const int8_t *q, const uint16_t *mu16, int64_t rows, int64_
  * x or residual itself where that is contiguous.  A NaN or an infinite s makes
  * the row's scale NaN and every q 0; a finite row whose squares pass fp32's
  * range is normed as any other (with a 16-bit residual_out over x or residual:
- * from the rounded sum). */
+ * from the rounded sum).  With cols 0 every scale is that of a row of zeros. */
 int h24_add_rms_norm_int8(const void *x, const void *residual, const void *gain, int gain_dtype,
                           int64_t rows, int64_t cols, int64_t x_stride, int64_t residual_stride,
                           int dtype, float eps, int8_t *q, float *scale, void *residual_out,

@@ -522,8 +522,8 @@ int h24_add_rms_norm_int8(const void *x, const void *residual, const void *gain,
   if (gain_dtype != dtype && gain_dtype != H24_DTYPE_F32)
     return fail(H24_ERR_INVALID, "add_rms_norm_int8: gain must have x's dtype or fp32");
   if (!(eps >= 0.f)) return fail(H24_ERR_INVALID, "add_rms_norm_int8: eps must not be negative");
-  if (rows == 0 || cols == 0) return H24_OK;
-  if (!x || !gain || !q || !scale) return fail(H24_ERR_INVALID, "add_rms_norm_int8: null pointer");
+  if (rows == 0) return H24_OK;
+  if (!scale || (cols > 0 && (!x || !gain || !q))) return fail(H24_ERR_INVALID, "add_rms_norm_int8: null pointer");
   if (x_stride < 0 || (residual && residual_stride < 0))
     return fail(H24_ERR_INVALID, "add_rms_norm_int8: negative stride");
   if (rows > INT32_MAX) return fail(H24_ERR_INVALID, "add_rms_norm_int8: more than 2^31 - 1 rows");
@@ -535,8 +535,8 @@ int h24_rows_int8_quantize(const void *x, int64_t rows, int64_t cols, int64_t x_
                            float *scale, void *stream) {
   if (rows < 0 || cols < 0) return fail(H24_ERR_INVALID, "rows_int8_quantize: negative size");
   if (!known_dtype(dtype)) return fail(H24_ERR_INVALID, "rows_int8_quantize: unknown dtype");
-  if (rows == 0 || cols == 0) return H24_OK;
-  if (!x || !q || !scale) return fail(H24_ERR_INVALID, "rows_int8_quantize: null pointer");
+  if (rows == 0) return H24_OK;
+  if (!scale || (cols > 0 && (!x || !q))) return fail(H24_ERR_INVALID, "rows_int8_quantize: null pointer");
   if (x_stride < 0) return fail(H24_ERR_INVALID, "rows_int8_quantize: negative stride");
   if (rows > INT32_MAX) return fail(H24_ERR_INVALID, "rows_int8_quantize: more than 2^31 - 1 rows");
   return launch_rows_int8(x, nullptr, nullptr, dtype, rows, cols, x_stride, 0, dtype, 0.f, q, scale, nullptr,

@@ -440,7 +440,7 @@ int launch_rows(const RowArgs &a, cudaStream_t s) {
   // instead of 10.5.  The number of rows has no say, so that a row's sum is
   // the same in every batch.
   for (int nv = 2; nv <= 8; nv *= 2) {
-    const int64_t threads = ((nvec + nv - 1) / nv + 31) / 32 * 32;
+    const int64_t threads = nvec == 0 ? 32 : ((nvec + nv - 1) / nv + 31) / 32 * 32;
     if (threads > (nv < 8 ? 512 : 1024)) continue;
     switch (nv) {
       case 2: return launch_rows_nv<DT, kNorm, 2>(a, aligned, static_cast<int>(threads), s);
@@ -471,7 +471,7 @@ int launch_rows_int8(const void *x, const void *residual, const void *gain, int 
                      float *scale, void *residual_out, cudaStream_t s) {
   const RowArgs a{x, residual, gain, rows, cols, x_stride, residual_stride, eps,
                   gain_dtype == H24_DTYPE_F32, q, scale, residual_out};
-  const bool norm = gain != nullptr;
+  const bool norm = gain != nullptr && cols > 0;  // (rows without elements: the scale of zeros)
   switch (dtype) {
     case H24_DTYPE_F32: return norm ? launch_rows<H24_DTYPE_F32, true>(a, s) : launch_rows<H24_DTYPE_F32, false>(a, s);
     case H24_DTYPE_F16: return norm ? launch_rows<H24_DTYPE_F16, true>(a, s) : launch_rows<H24_DTYPE_F16, false>(a, s);

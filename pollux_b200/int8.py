@@ -89,7 +89,7 @@ def add_rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Ten
     q = xr.new_empty(x.shape, dtype=torch.int8)
     scale = xr.new_empty(x.shape[:-1], dtype=torch.float32)
     summed = None if rr is None else xr.new_empty(x.shape)
-    if rows and cols:
+    if rows:
         _call(dev, "h24_add_rms_norm_int8", xr.data_ptr(), None if rr is None else rr.data_ptr(), w.data_ptr(),
               code if w.dtype == x.dtype else N.DTYPE_F32, rows, cols, xr.stride(0),
               0 if rr is None else rr.stride(0), code, eps, q.data_ptr(), scale.data_ptr(),
@@ -113,7 +113,7 @@ def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     rows, cols = xr.shape
     q = xr.new_empty(x.shape, dtype=torch.int8)
     scale = xr.new_empty(x.shape[:-1], dtype=torch.float32)
-    if rows and cols:
+    if rows:
         _call(dev, "h24_rows_int8_quantize", xr.data_ptr(), rows, cols, xr.stride(0), code, q.data_ptr(),
               scale.data_ptr(), _stream(dev))
     return (q, scale) if x.device == dev else (q.to(x.device), scale.to(x.device))
