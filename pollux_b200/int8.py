@@ -16,6 +16,8 @@ gradient.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
@@ -40,7 +42,7 @@ def _rows(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
     if t.device != dev:
         t = t.to(dev)
     if t.dim() != 2:
-        t = t.reshape(-1, t.shape[-1])
+        t = t.reshape(math.prod(t.shape[:-1]), t.shape[-1])  # (-1 has no answer where the last is 0)
     if t.stride(1) != 1 and t.shape[1] > 1:
         t = t.contiguous()
     return t
@@ -169,7 +171,7 @@ def int8_linear(q: torch.Tensor, scale: torch.Tensor, weight_int8: torch.Tensor,
     w = weight_int8 if weight_int8.device == dev else weight_int8.to(dev)
     if not w.is_contiguous():
         w = w.contiguous()
-    tokens = qr.shape[0] if in_f else scale.numel()
+    tokens = qr.shape[0]
     s = _vector(scale, tokens, torch.float32, dev, "scale")
     mu = _vector(mu_rows, out_f, None, dev, "mu_rows")
     b = None if bias is None else _vector(bias, out_f, torch.float32, dev, "bias")
