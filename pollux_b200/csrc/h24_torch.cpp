@@ -12,6 +12,7 @@
 #include <Python.h>
 
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -30,11 +31,15 @@ struct {
   decltype(&h24_sample_tokens) sample;
 } g_h24;
 
-// The tensor behind `o` if it is a contiguous CUDA tensor of device `dev`.
+// The tensor behind `o` if it is a contiguous CUDA tensor of device `dev` of
+// which no gradient is asked.
 const at::Tensor *plain(PyObject *o, int dev) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor &t = THPVariable_Unpack(o);
-  return t.is_cuda() && t.get_device() == dev && t.layout() == at::kStrided && t.is_contiguous() ? &t : nullptr;
+  return t.is_cuda() && t.get_device() == dev && t.layout() == at::kStrided && t.is_contiguous() &&
+                 !(t.requires_grad() && c10::GradMode::is_enabled())
+             ? &t
+             : nullptr;
 }
 
 int code_of(at::ScalarType t) {

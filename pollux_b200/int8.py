@@ -11,8 +11,9 @@ and fp16 row scales that the ``.plx`` container holds for ``tok_emb`` and
 ``enable_int8_forward`` makes the not-yet-materialised ``PackedInt8Linear``
 layers of a model (the reference's included) run this way: the head is read as
 1 byte a weight where ``materialize`` + ``F.linear`` (pollux.py:545-558) read 2.
-All of it is for inference: the weights are buffers and nothing records a
-gradient.
+All of it is for inference: the weights are buffers and nothing has a gradient.
+Where an input requires one, the outputs do too, and a backward pass that reaches
+them raises NotImplementedError.
 """
 from __future__ import annotations
 
@@ -48,6 +49,24 @@ def _rows(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
     return t
 
 
+class _NoGradient(torch.autograd.Function):
+    """A call whose outputs stand in the graph, so that a gradient that is asked of it raises and is not lost."""
+
+    @staticmethod
+    def forward(ctx, fn, *args):
+        ctx.name = fn.__name__
+        return fn(*args)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise NotImplementedError(f"{ctx.name} is for inference and has no gradient; call it under torch.no_grad() "
+                                  "or on detached tensors")
+
+
+def _tracked(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 def _vector(t: torch.Tensor, n: int, dtype: torch.dtype | None, dev: torch.device, what: str) -> torch.Tensor:
     if t.numel() != n:
         raise ValueError(f"{what} must hold {n} values, got {tuple(t.shape)}")
@@ -73,6 +92,8 @@ def add_rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Ten
     got = (N._torch_calls or N.torch_calls()).add_rms_norm_int8(x, weight, residual, eps)
     if got is not None:
         return got
+    if _tracked(x, weight, residual):
+        return _NoGradient.apply(add_rms_norm_int8, x, weight, residual, eps)
     _check_rows(x, "x")
     code = _code(x.dtype, "x")
     if eps < 0:
@@ -108,6 +129,8 @@ def quantize_rows_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     got = (N._torch_calls or N.torch_calls()).quantize_rows_int8(x)
     if got is not None:
         return got
+    if _tracked(x):
+        return _NoGradient.apply(quantize_rows_int8, x)
     _check_rows(x, "x")
     code = _code(x.dtype, "x")
     dev = _work_device(x)
@@ -126,6 +149,8 @@ def dequantize_rows_int8(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtyp
     got = (N._torch_calls or N.torch_calls()).dequantize_rows_int8(q, scale, dtype)
     if got is not None:
         return got
+    if _tracked(scale):
+        return _NoGradient.apply(dequantize_rows_int8, q, scale, dtype)
     _check_rows(q, "q")
     if q.dtype != torch.int8:
         raise TypeError(f"q must be int8, got {q.dtype}")
@@ -152,6 +177,8 @@ def int8_linear(q: torch.Tensor, scale: torch.Tensor, weight_int8: torch.Tensor,
     got = (N._torch_calls or N.torch_calls()).int8_linear(q, scale, weight_int8, mu_rows, bias, out_dtype)
     if got is not None:
         return got
+    if _tracked(scale, mu_rows, bias):
+        return _NoGradient.apply(int8_linear, q, scale, weight_int8, mu_rows, bias, out_dtype)
     _check_rows(q, "q")
     if q.dtype != torch.int8 or weight_int8.dtype != torch.int8:
         raise TypeError(f"q and weight_int8 must be int8, got {q.dtype} and {weight_int8.dtype}")

@@ -11,7 +11,7 @@ import torch
 
 from . import _native as N
 from .castor import _call, _stream, _work_device
-from .int8 import _code, _rows
+from .int8 import _NoGradient, _code, _rows, _tracked
 
 MAX_VOCAB = 1 << 22
 _INF = float("inf")
@@ -50,10 +50,12 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: float | to
     with no logit above -inf gives -1.
     Returns int64 tokens of the leading shape, with ``return_logprob`` also the
     fp32 log-probabilities of the tokens at that temperature before the cuts
-    (-inf for a row that gives -1)."""
+    (-inf for a row that gives -1); no gradient goes through them."""
     got = (N._torch_calls or N.torch_calls()).sample_tokens(logits, u, temperature, top_k, top_p, min_p, return_logprob)
     if got is not None:
         return got
+    if return_logprob and _tracked(logits):
+        return _NoGradient.apply(sample_tokens, logits, u, temperature, top_k, top_p, min_p, return_logprob)
     if logits.dim() < 1:
         raise ValueError("logits must have at least one dimension")
     code = _code(logits.dtype, "logits")
