@@ -42,6 +42,28 @@ const at::Tensor *plain(PyObject *o, int dev) {
              : nullptr;
 }
 
+// Whether `t` has a value for each row of `x`, in their order: x's leading
+// dimensions up to ones, or one of the two a flat list.  (As _holds_rows in
+// int8.py, which answers for what is refused here.)
+bool holds_rows(const at::Tensor &t, const at::Tensor &x) {
+  const at::IntArrayRef own = t.sizes(), want = x.sizes().slice(0, x.dim() - 1);
+  int64_t n = 1;
+  for (const int64_t d : want) n *= d;
+  if (t.numel() != n) return false;
+  if (own.equals(want)) return true;
+  size_t i = 0, j = 0, n_own = 0, n_want = 0;
+  for (const int64_t d : own) n_own += d != 1;
+  for (const int64_t d : want) n_want += d != 1;
+  if (n_own <= 1 || n_want <= 1) return true;
+  if (n_own != n_want) return false;
+  for (;; ++i, ++j) {
+    while (i < own.size() && own[i] == 1) ++i;
+    while (j < want.size() && want[j] == 1) ++j;
+    if (i == own.size()) return true;
+    if (own[i] != want[j]) return false;
+  }
+}
+
 int code_of(at::ScalarType t) {
   return t == at::kFloat ? H24_DTYPE_F32 : t == at::kHalf ? H24_DTYPE_F16 : t == at::kBFloat16 ? H24_DTYPE_BF16 : -1;
 }
@@ -149,7 +171,7 @@ PyObject *dequantize_rows_int8(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const at::Tensor *s = q ? plain(a[1], dev) : nullptr;
     at::ScalarType type;
     if (!s || q->dim() < 1 || q->numel() == 0 || q->scalar_type() != at::kChar || s->scalar_type() != at::kFloat ||
-        s->numel() * q->size(-1) != q->numel() || !dtype_of(a[2], &type))
+        !holds_rows(*s, *q) || !dtype_of(a[2], &type))
       Py_RETURN_NONE;
     const at::Tensor out = fresh(q->sizes(), type, dev);
     if (g_h24.dequant(static_cast<const int8_t *>(q->const_data_ptr()), static_cast<const float *>(s->const_data_ptr()),
@@ -175,7 +197,7 @@ PyObject *int8_linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
         mu->scalar_type() != at::kHalf || !dtype_of(a[5], &type))
       Py_RETURN_NONE;
     const int64_t in = w->size(1), out = w->size(0), tokens = s->numel();
-    if (q->size(-1) != in || tokens * in != q->numel() || mu->numel() != out ||
+    if (q->size(-1) != in || !holds_rows(*s, *q) || mu->numel() != out ||
         (b && (b->scalar_type() != at::kFloat || b->numel() != out)))
       Py_RETURN_NONE;
     at::DimVector sizes(q->sizes());
@@ -192,12 +214,12 @@ PyObject *int8_linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
 }
 
 // A sampling setting: a number in [0, most] or one value a row.
-bool setting(PyObject *o, int dev, int64_t rows, at::ScalarType type, double most, const void **p, double *v) {
+bool setting(PyObject *o, int dev, const at::Tensor &logits, at::ScalarType type, double most, const void **p, double *v) {
   *p = nullptr;
   *v = 0;
   if (number(o, v)) return *v >= 0 && *v <= most;
   const at::Tensor *t = plain(o, dev);
-  if (!t || t->scalar_type() != type || t->numel() != rows) return false;
+  if (!t || t->scalar_type() != type || !holds_rows(*t, logits)) return false;
   *p = t->const_data_ptr();
   return true;
 }
@@ -214,9 +236,9 @@ PyObject *sample_tokens(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const double inf = std::numeric_limits<double>::infinity();
     const void *tp, *kp, *pp, *mp;
     double t, k, p, m;
-    if (u->numel() != rows || !setting(a[2], dev, rows, at::kFloat, inf, &tp, &t) ||
-        !setting(a[3], dev, rows, at::kInt, inf, &kp, &k) || !setting(a[4], dev, rows, at::kFloat, 1.0, &pp, &p) ||
-        !setting(a[5], dev, rows, at::kFloat, 1.0, &mp, &m))
+    if (!holds_rows(*u, *l) || !setting(a[2], dev, *l, at::kFloat, inf, &tp, &t) ||
+        !setting(a[3], dev, *l, at::kInt, inf, &kp, &k) || !setting(a[4], dev, *l, at::kFloat, 1.0, &pp, &p) ||
+        !setting(a[5], dev, *l, at::kFloat, 1.0, &mp, &m))
       Py_RETURN_NONE;
     const int want = PyObject_IsTrue(a[6]);
     const at::Tensor tokens = fresh(l->sizes().slice(0, l->dim() - 1), at::kLong, dev);

@@ -75,6 +75,20 @@ def _vector(t: torch.Tensor, n: int, dtype: torch.dtype | None, dev: torch.devic
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _holds_rows(t: torch.Tensor, lead) -> bool:
+    """Whether ``t`` has a value for each row of leading dimensions ``lead``, in their order: the same dimensions
+    up to ones, or one of the two a flat list."""
+    if t.numel() != math.prod(lead):
+        return False
+    own, want = [n for n in t.shape if n != 1], [n for n in lead if n != 1]
+    return own == want or len(own) <= 1 or len(want) <= 1 or t.numel() == 0
+
+
+def _check_scale(scale: torch.Tensor, q: torch.Tensor) -> None:
+    if not _holds_rows(scale, q.shape[:-1]):
+        raise ValueError(f"scale must hold one value for each row of q, {tuple(q.shape[:-1])}, got {tuple(scale.shape)}")
+
+
 def _check_rows(t: torch.Tensor, what: str) -> None:
     if t.dim() < 1:
         raise ValueError(f"{what} must have at least one dimension")
@@ -155,6 +169,7 @@ def dequantize_rows_int8(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtyp
     if q.dtype != torch.int8:
         raise TypeError(f"q must be int8, got {q.dtype}")
     code = _code(dtype, "dtype")
+    _check_scale(scale, q)
     dev = _work_device(q)
     cols = q.shape[-1]
     rows = q.numel() // cols if cols else 0
@@ -170,7 +185,7 @@ def dequantize_rows_int8(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtyp
 def int8_linear(q: torch.Tensor, scale: torch.Tensor, weight_int8: torch.Tensor, mu_rows: torch.Tensor,
                 bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """``(q * scale) @ W.T + bias`` for int8 rows ``q`` [..., in] with fp32
-    ``scale`` [...], and the INT8 layer ``weight_int8`` [out, in] with fp16
+    ``scale`` [...] (or as a flat list), and the INT8 layer ``weight_int8`` [out, in] with fp16
     ``mu_rows`` [out] (``W = weight_int8 * fp16(mu / 127)``, as
     ``PackedInt8Linear``).  The sum is exact in int32; the scaling and the bias
     are fp32; the result is rounded once to ``out_dtype``."""
@@ -193,6 +208,7 @@ def int8_linear(q: torch.Tensor, scale: torch.Tensor, weight_int8: torch.Tensor,
     if in_f > MAX_IN_FEATURES:
         raise ValueError(f"in_features must be at most {MAX_IN_FEATURES}, got {in_f}")
     code = _code(out_dtype, "out_dtype")
+    _check_scale(scale, q)
     dev = _work_device(q)
     qr = _rows(q, dev)
     w = weight_int8 if weight_int8.device == dev else weight_int8.to(dev)

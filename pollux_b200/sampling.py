@@ -11,18 +11,16 @@ import torch
 
 from . import _native as N
 from .castor import _call, _stream, _work_device
-from .int8 import _NoGradient, _code, _rows, _tracked
+from .int8 import _NoGradient, _code, _holds_rows, _rows, _tracked
 
 MAX_VOCAB = 1 << 22
 _INF = float("inf")
 
 
-def _setting(v, rows: int, dtype: torch.dtype, dev: torch.device, name: str):
+def _setting(v, dtype: torch.dtype, dev: torch.device):
     """(tensor kept alive, pointer or None, scalar) of one sampling setting."""
     if not isinstance(v, torch.Tensor):
         return None, None, float(v)
-    if v.numel() != rows:
-        raise ValueError(f"{name} must be a number or hold one value for each of the {rows} rows, got {tuple(v.shape)}")
     if dtype == torch.int32 and v.dtype == torch.int64:
         v = v.clamp(0, MAX_VOCAB)  # what the vocabulary holds, and no more than 32 bits
     if v.device != dev or v.dtype != dtype:
@@ -44,7 +42,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: float | to
     of the most probable token's probability.  The token is where the running
     mass of what is kept, in the order of the vocabulary, passes ``u`` of it.
     ``temperature`` 0 takes the largest logit.  Each setting is a number or a
-    tensor with one value a row.
+    tensor with one value a row, of the leading shape or a flat list.
 
     NaN logits are never chosen, +inf counts as the largest fp32 number; a row
     with no logit above -inf gives -1.
@@ -65,16 +63,20 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: float | to
     rows = logits.numel() // vocab
     for name, v, most in (("temperature", temperature, _INF), ("top_k", top_k, _INF), ("top_p", top_p, 1.0),
                           ("min_p", min_p, 1.0)):
-        if not isinstance(v, torch.Tensor) and not 0 <= v <= most:
+        if isinstance(v, torch.Tensor):
+            if not _holds_rows(v, lead):
+                raise ValueError(f"{name} must be a number or hold one value for each row, {tuple(lead)}, "
+                                 f"got {tuple(v.shape)}")
+        elif not 0 <= v <= most:
             raise ValueError(f"{name} out of range: {v}")
+    if not _holds_rows(u, lead):
+        raise ValueError(f"u must hold one number for each row, {tuple(lead)}, got {tuple(u.shape)}")
     dev = _work_device(logits)
-    if u.numel() != rows:
-        raise ValueError(f"u must hold one number for each of the {rows} rows, got {tuple(u.shape)}")
-    ts, tp, t1 = _setting(temperature, rows, torch.float32, dev, "temperature")
-    ks, kp, k1 = _setting(top_k, rows, torch.int32, dev, "top_k")
-    ps, pp, p1 = _setting(top_p, rows, torch.float32, dev, "top_p")
-    ms, mp, m1 = _setting(min_p, rows, torch.float32, dev, "min_p")
-    us, up, _ = _setting(u, rows, torch.float32, dev, "u")
+    ts, tp, t1 = _setting(temperature, torch.float32, dev)
+    ks, kp, k1 = _setting(top_k, torch.int32, dev)
+    ps, pp, p1 = _setting(top_p, torch.float32, dev)
+    ms, mp, m1 = _setting(min_p, torch.float32, dev)
+    us, up, _ = _setting(u, torch.float32, dev)
     lr = _rows(logits, dev)
     tokens = lr.new_empty(lead, dtype=torch.int64)
     logprob = lr.new_empty(lead, dtype=torch.float32) if return_logprob else None
