@@ -270,13 +270,27 @@ const HostTables &host_tables() {
   return H;
 }
 
+// While this stands, what this thread allocates and copies on streams of its own
+// does not end a graph capture that is under way.
+struct OutsideCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
+// The copies run on a stream of their own: the legacy default stream would wait
+// for, and end, a capture.
 int build_device_tables(int dev, Tables *T) {
   const HostTables &H = host_tables();
   if (!H.ok) return fail(H24_ERR_STATE, "codebook construction failed: " + H.err);
+  const OutsideCapture outside;
+  H24_CUDA_TRY(cudaStreamCreateWithFlags(&T->copy_stream, cudaStreamNonBlocking));
+  H24_CUDA_TRY(cudaStreamCreateWithFlags(&T->d2h_stream, cudaStreamNonBlocking));
+  const cudaStream_t s = T->copy_stream;
   void *p = nullptr;
-  const auto upload = [&p](const void *src, size_t bytes) -> int {
+  const auto upload = [&p, s](const void *src, size_t bytes) -> int {
     H24_CUDA_TRY(cudaMalloc(&p, bytes));
-    H24_CUDA_TRY(cudaMemcpy(p, src, bytes, cudaMemcpyHostToDevice));
+    H24_CUDA_TRY(cudaMemcpyAsync(p, src, bytes, cudaMemcpyHostToDevice, s));
     return H24_OK;
   };
   int rc = upload(H.golay.data(), H.golay.size() * sizeof(uint16_t));
@@ -292,15 +306,12 @@ int build_device_tables(int dev, Tables *T) {
   T->idx1 = static_cast<const int32_t *>(p);
   if ((rc = upload(H.oct_by_triple.data(), H.oct_by_triple.size() * 4)) != H24_OK) return rc;
   T->oct_by_triple = static_cast<const uint2 *>(p);
-  H24_CUDA_TRY(cudaMalloc(&p, H.raw.size()));
-  H24_CUDA_TRY(cudaMemcpy(p, H.raw.data(), H.raw.size(), cudaMemcpyHostToDevice));
+  if ((rc = upload(H.raw.data(), H.raw.size())) != H24_OK) return rc;
   T->cb_raw = static_cast<const int8_t *>(p);
-  H24_CUDA_TRY(cudaMalloc(&p, H.nib.size() * sizeof(uint32_t)));
-  H24_CUDA_TRY(
-      cudaMemcpy(p, H.nib.data(), H.nib.size() * sizeof(uint32_t), cudaMemcpyHostToDevice));
+  if ((rc = upload(H.nib.data(), H.nib.size() * sizeof(uint32_t))) != H24_OK) return rc;
   T->cb_nib = static_cast<const uint32_t *>(p);
   H24_CUDA_TRY(cudaMalloc(&p, 3 * sizeof(int64_t) + 16));
-  H24_CUDA_TRY(cudaMemset(p, 0, 3 * sizeof(int64_t) + 16));
+  H24_CUDA_TRY(cudaMemsetAsync(p, 0, 3 * sizeof(int64_t) + 16, s));
   T->stats = static_cast<int64_t *>(p);
   T->err = reinterpret_cast<int *>(static_cast<char *>(p) + 3 * sizeof(int64_t));
   cudaMemPoolProps props = {};
@@ -311,8 +322,7 @@ int build_device_tables(int dev, Tables *T) {
   H24_CUDA_TRY(cudaMemPoolCreate(&T->pool, &props));
   uint64_t keep = ~uint64_t(0);
   H24_CUDA_TRY(cudaMemPoolSetAttribute(T->pool, cudaMemPoolAttrReleaseThreshold, &keep));
-  H24_CUDA_TRY(cudaStreamCreateWithFlags(&T->copy_stream, cudaStreamNonBlocking));
-  H24_CUDA_TRY(cudaStreamCreateWithFlags(&T->d2h_stream, cudaStreamNonBlocking));
+  H24_CUDA_TRY(cudaStreamSynchronize(s));
   std::memcpy(T->fingerprint, H.fingerprint, sizeof(T->fingerprint));
   T->device = dev;
   return H24_OK;
