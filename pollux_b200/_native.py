@@ -10,7 +10,9 @@ import ctypes
 import importlib.machinery
 import importlib.util
 import os
+import sysconfig
 import threading
+import warnings
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # H24_LIBRARY selects another build of the same library (e.g. a tuning variant).
@@ -131,18 +133,35 @@ _TORCH_ENTRIES = ("h24_add_rms_norm_int8", "h24_rows_int8_quantize", "h24_rows_i
                   "h24_sample_tokens")
 
 
+def torch_module_path() -> str:
+    """Where the module _h24_torch lies.  It is bound to one torch and one
+    interpreter, so their versions are in its name and no other finds it."""
+    import torch
+    return os.path.join(_HERE, "_lib", f"_h24_torch.{torch.__version__}.{sysconfig.get_config_var('SOABI')}.so")
+
+
+class _GeneralPath:
+    """In place of the module where it has not been built: every call is left to the general path."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
 def torch_calls():
     """The module _h24_torch, which makes the decoding-step calls of libh24
-    straight from torch tensors (raises if it has not been built)."""
+    straight from torch tensors.  Without it they take the general path, which
+    makes the same calls of libh24 at some ten microseconds more."""
     global _torch_calls
     if _torch_calls is None:
-        import torch  # noqa: F401  (the module's symbols are torch's)
+        path = torch_module_path()  # (imports torch, whose symbols the module takes)
         lib = load()
         with _lock:
             if _torch_calls is None:
-                path = os.path.join(_HERE, "_lib", "_h24_torch.so")
                 if not os.path.exists(path):
-                    raise H24Error(f"_h24_torch.so not found at {path}; build it with `python -m pollux_b200.build`")
+                    warnings.warn(f"{os.path.basename(path)} has not been built: the INT8 head path's calls take "
+                                  "longer on the host; build it with `python -m pollux_b200.build`", RuntimeWarning)
+                    _torch_calls = _GeneralPath()
+                    return _torch_calls
                 loader = importlib.machinery.ExtensionFileLoader("_h24_torch", path)
                 mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("_h24_torch", loader))
                 loader.exec_module(mod)
