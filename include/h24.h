@@ -202,13 +202,19 @@ int h24_rows_int8_dequant(const int8_t *q, const float *scale, int64_t rows, int
  * h24_int8_dequant reads it).  The sum is exact in int32, the scaling fp32, y
  * (contiguous, element type out_dtype) rounded once.  Row t of q starts at
  * t * q_stride bytes; bias: out_features fp32 or NULL.  in_features is at
- * most 131,000 (the sum cannot overflow).  With five tokens or more, rows that
- * are not 16-byte aligned are copied to a stream-ordered workspace from the
- * library's device memory pool, freed on the same stream.  h24_check reports
- * a bounded wait that ran out. */
+ * most 131,000 (the sum cannot overflow).  With five tokens or more (three, where
+ * the layer has more than 24 Mi weights), rows that are not 16-byte aligned are
+ * copied to a stream-ordered workspace from the library's device memory pool,
+ * freed on the same stream.  h24_check reports a bounded wait that ran out. */
 int h24_int8_linear(const int8_t *q, const float *scale, int64_t tokens, int64_t q_stride,
                     const int8_t *w, const uint16_t *mu16, int64_t out_features, int64_t in_features,
                     const float *bias, int out_dtype, void *y, void *stream);
+
+/* The way h24_int8_linear takes for these sizes (needs no device): plan[0] is the
+ * kernel (0: weight rows by dp4a, 1: tiles of one CTA, 2: tiles of pairs of
+ * CTAs), plan[1] the tokens of a tile, plan[2] the CTAs that share a tile's sum. */
+int h24_int8_linear_plan(int64_t tokens, int64_t out_features, int64_t in_features, int out_dtype,
+                         int32_t plan[3]);
 
 /* One token a row of logits (`rows` x `vocab`, element type `dtype`, row r at
  * r * stride elements) from the uniform number u[r] in [0, 1).

@@ -55,6 +55,7 @@ SIGNATURES = {
     "h24_rows_int8_quantize": (_I, [_P, _I64, _I64, _I64, _I, _P, _P, _P]),
     "h24_rows_int8_dequant": (_I, [_P, _P, _I64, _I64, _I, _P, _P]),
     "h24_int8_linear": (_I, [_P, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _I, _P, _P]),
+    "h24_int8_linear_plan": (_I, [_I64, _I64, _I64, _I, _P]),
     "h24_sample_tokens": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _F, _P, _I, _P, _F, _P, _F, _P, _P, _P]),
     "h24_quantize": (_I, [_P, _I64, _I, _P, _P]),
     "h24_quantize_layer": (_I, [_P, _I64, _I64, _P, _P, _P]),

@@ -563,6 +563,17 @@ int h24_rows_int8_dequant(const int8_t *q, const float *scale, int64_t rows, int
   return launch_rows_dequant(q, scale, rows, cols, dtype, out, as_stream(stream));
 }
 
+int h24_int8_linear_plan(int64_t tokens, int64_t out_features, int64_t in_features, int out_dtype, int32_t plan[3]) {
+  if (tokens < 1 || out_features < 1 || in_features < 0) return fail(H24_ERR_INVALID, "int8_linear_plan: no tokens or features");
+  if (in_features > 131000) return fail(H24_ERR_INVALID, "int8_linear_plan: in_features above 131000");
+  if (out_features > INT32_MAX || tokens > INT32_MAX)
+    return fail(H24_ERR_INVALID, "int8_linear_plan: size above 2^31 - 1");
+  if (!known_dtype(out_dtype)) return fail(H24_ERR_INVALID, "int8_linear_plan: unknown dtype");
+  if (!plan) return fail(H24_ERR_INVALID, "int8_linear_plan: null pointer");
+  int8_linear_plan(tokens, out_features, in_features, out_dtype, plan);
+  return H24_OK;
+}
+
 int h24_int8_linear(const int8_t *q, const float *scale, int64_t tokens, int64_t q_stride, const int8_t *w,
                     const uint16_t *mu16, int64_t out_features, int64_t in_features, const float *bias,
                     int out_dtype, void *y, void *stream) {

@@ -1029,6 +1029,13 @@ int launch_typed(const Plan &plan, bool aligned, const CUtensorMap &wmap, const 
 
 }  // namespace
 
+void int8_linear_plan(int64_t tokens, int64_t out, int64_t in, int out_dtype, int32_t plan[3]) {
+  const Plan p = make_plan(tokens, out, in, out_dtype == H24_DTYPE_F32 ? 4 : 2);
+  plan[0] = p.kind;
+  plan[1] = p.n;
+  plan[2] = p.split;
+}
+
 int launch_int8_linear(const Tables *T, const int8_t *q, const float *scale, int64_t tokens, int64_t q_stride,
                        const int8_t *w, const uint16_t *mu16, int64_t out, int64_t in, const float *bias,
                        int out_dtype, void *y, cudaStream_t s) {

@@ -244,6 +244,7 @@ int launch_rows_int8(const void *x, const void *residual, const void *gain, int 
                      float *scale, void *residual_out, cudaStream_t s);
 int launch_rows_dequant(const int8_t *q, const float *scale, int64_t rows, int64_t cols, int dtype, void *out,
                         cudaStream_t s);
+void int8_linear_plan(int64_t tokens, int64_t out, int64_t in, int out_dtype, int32_t plan[3]);
 int launch_int8_linear(const Tables *t, const int8_t *q, const float *scale, int64_t tokens, int64_t q_stride,
                        const int8_t *w, const uint16_t *mu16, int64_t out, int64_t in, const float *bias,
                        int out_dtype, void *y, cudaStream_t s);
