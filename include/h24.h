@@ -179,7 +179,8 @@ int h24_int8_dequant(const int8_t *q, const uint16_t *mu16, int64_t rows, int64_
  * r * residual_stride; q, scale and residual_out are contiguous.  gain: cols
  * elements of `dtype` or of H24_DTYPE_F32 (gain_dtype).  residual_out may be
  * x or residual itself where that is contiguous.  A NaN or an infinite s makes
- * the row's scale NaN and every q 0; a finite row whose squares pass fp32's
+ * the row's scale NaN and every q 0, a product s * gain beyond fp32 a scale that
+ * is not finite and every q 0; a finite row whose squares pass fp32's
  * range is normed as any other (with a 16-bit residual_out over x or residual:
  * from the rounded sum).  With cols 0 every scale is that of a row of zeros. */
 int h24_add_rms_norm_int8(const void *x, const void *residual, const void *gain, int gain_dtype,
@@ -187,7 +188,8 @@ int h24_add_rms_norm_int8(const void *x, const void *residual, const void *gain,
                           int dtype, float eps, int8_t *q, float *scale, void *residual_out,
                           void *stream);
 
-/* The quantisation alone: mu = max(max|x|, 1e-8), q and scale as above. */
+/* The quantisation alone: mu = max(max|x|, 1e-8), q and scale as above (an
+ * infinite x: an infinite scale, every q 0). */
 int h24_rows_int8_quantize(const void *x, int64_t rows, int64_t cols, int64_t x_stride, int dtype,
                            int8_t *q, float *scale, void *stream);
 

@@ -9,7 +9,8 @@
 // and not 128 rows, and a warp's 32 lanes store 32 neighbouring outputs.
 //
 // Three kernels, chosen by make_plan from an estimate of bytes and latency:
-//   one to four tokens: dp4a over the weight rows, bound by their bytes
+//   one or two tokens (four, where the layer is small): dp4a over the weight
+//     rows, bound by their bytes
 //     ([1,1920] x [50688,1920] 15.0-16.1 us: 0.93-0.99 of the measured HBM rate);
 //   a few to a few hundred: tiles of 128 x n, the k split over a cluster where
 //     tiles are few; bound by a launch's chain of latencies (5.4 us for [32,1920]
@@ -906,6 +907,10 @@ double pair_us(int64_t tokens, int64_t out, int64_t kblocks, int n, double hbm_u
 }
 
 Plan make_plan(int64_t tokens, int64_t out, int64_t in, int out_size) {
+  // (Whether rows lie on 16 bytes has no say here, although the copy that the
+  // tiles then need costs two more bytes a byte: [3,3473] x [19944,3473] takes
+  // 48 us through it, [3,1919] x [50688,1919] 68, and one token on such rows 37.
+  // The limits below were measured on aligned rows.)
   // Up to four tokens without tiles; three and four only where the weights are
   // few (dp4a's work grows with the tokens): [4,1920] x [7680,1920] 4.8 us
   // against 5.5 in tiles, x [50688,1920] 22 against 18.

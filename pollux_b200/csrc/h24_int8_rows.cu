@@ -13,10 +13,14 @@
 // again of s * 2^-80: see wide_factor.
 //
 // Bound by HBM where there are rows: 7 bytes an element in bf16 (x, r, r', q).
-// On a B200 [4096,1920] bf16 takes 10.5 us (5.3 TB/s, 0.80 of the measured
-// copy rate), [4096,7680] 36.5 (6.0 TB/s, 0.92), [4096,1920] fp32 16.5 (6.2,
-// 0.95); one row 2.1 us, a launch's latency.  The way back: 4.9 us for
-// [4096,1920] to bf16, its int8 rows still in L2.
+// On a B200, a call among others: [4096,1920] bf16 10.1 us (5.5 TB/s, 0.83 of
+// the measured copy rate), [4096,7680] 37.1 (5.9, 0.91; fp16 44.0), [4096,1920]
+// fp32 15.8 (6.5, 0.99); one row 2.1 us, a launch's latency.  Rows off 16 bytes
+// are read and written by the element, which costs a sector each time:
+// [4096,1919] bf16 38.9 us, [2028,841] 11.3.  Rows of 16,385 to 65,536 elements
+// of 16 bits do not fit the registers (see the kernel): [512,32768] bf16 92 us
+// for 117 MB, [512,65536] 182 for 235.  The way back: 4.9 us for [4096,1920] to
+// bf16, its int8 rows still in L2.
 #include "h24_internal.cuh"
 
 namespace h24 {
@@ -166,8 +170,11 @@ __device__ __noinline__ void wide_rows(const RowArgs &a, float (*red)[32]) {
 }
 
 // Thread t of a block holds the 16-byte groups t, t + blockDim.x, ... (at most
-// NV) of its row in registers, so the row is read once.  A block walks rows r, r + gridDim.x, ..., and asks for
-// the next row before it reduces the present one.  Rows that are not 16-byte
+// NV) of its row in registers, so the row is read once.  (For NV = 8 the 1,024
+// threads' registers are too few, and part of the row goes through local memory:
+// ptxas reports 1.6 KB of spill stores a thread in bf16, 0.6 in fp32.)  A block
+// walks rows r, r + gridDim.x, ..., and asks for the next row before it reduces
+// the present one.  Rows that are not 16-byte
 // aligned, or end inside a group, are read and written by the element in the
 // same groups: a row's result does not depend on where it lies.
 template <int DT, bool kAligned, int NV, bool kNorm>

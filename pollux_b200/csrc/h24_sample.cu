@@ -31,7 +31,9 @@
 // What bounds it, measured on a B200: one row, the chain of a dozen barriers
 // and exchanges ([1,50688] fp32, k = 50, p = 0.9: 10.9 us; no cut: 7.3); many
 // rows, instruction issue and the second and third read from L2 ([512,50688]
-// fp32: no cut 51 us, k = 50 58, p = 0.9 127, for 15.9 us of HBM traffic).  For
+// fp32: no cut 51 us, k = 50 43-58, p = 0.9 122-127, for 15.9 us of HBM traffic;
+// fp16 and bf16, p = 0.9: 134; rows off 16 bytes, which every pass reads by the
+// element: [512,50257] fp32 73, 65 and 143).  For
 // a cut at p, a list bounded by the threads' maxima as for k was tried: half of
 // the rows' cuts lie behind 700 tokens, and 2,200 cost what the steps cost.
 //
@@ -1136,12 +1138,16 @@ template <int DT>
 int launch_sample_typed(const SampleArgs &a, cudaStream_t s) {
   const int size = DT == H24_DTYPE_F32 ? 4 : 2;
   if (a.rows > INT32_MAX / kMaxCluster) return fail(H24_ERR_INVALID, "sample_tokens: too many rows");
-  // Clusters where a CTA each fits an SM: the most CTAs a row that are there at
-  // once, with slices of at least 1,024 logits.  Rows enough for the SMs by
+  // Clusters where the rows' CTAs are no more than the SMs, with slices of at least
+  // 1,024 logits.  (What fits at once is less: 15 clusters of eight and 36 of four,
+  // so 16 to 18 rows, and 37, take a second wave: [15,50688] fp32, p = 0.9: 21 us,
+  // [16,50688] 39, [19,50688] 23.)  Rows enough for the SMs by
   // themselves, or too long for a cluster, run a CTA a row that reads it from
   // L2 in each pass ([512,50688] fp32, p = 0.9: 127 us, in clusters of four 275;
   // [64,50688] bf16, p = 0.95: 60 us, in clusters of two 36; [1,50688] fp32,
-  // k = 50: 15.6 us, in a cluster of eight 10.9).
+  // k = 50: 15.6 us, in a cluster of eight 10.9).  A slice of fp32 logits fits up
+  // to 42,700 of them: [74,50688] fp32, p = 0.9, in clusters of two 30 us, [75,50688]
+  // by a CTA a row 46, [147,50688] 52; [64,131072] 75; one row of 600,001 254.
   int nc = kMaxCluster;
   while (nc > 1 && (a.rows * nc > 148 || a.vocab < 1024 * nc)) nc /= 2;
   const int64_t slice = ((a.vocab + nc - 1) / nc + 15) / 16 * 16;
