@@ -239,6 +239,47 @@ int h24_sample_tokens(const void *logits, int dtype, int64_t rows, int64_t vocab
                       const float *min_p, float min_p_all, int64_t *tokens, float *logprobs,
                       void *stream);
 
+/* ---- the training head path ------------------------------------------------
+ * Loss of a model's head and its gradients, with the logits never in memory
+ * (F.linear + F.cross_entropy of a [vocab, d] head in torch; no counterpart in
+ * the reference's code). */
+#define H24_REDUCE_NONE 0
+#define H24_REDUCE_MEAN 1
+#define H24_REDUCE_SUM 2
+
+/* loss[t] = log(sum_v exp(z[t][v])) - z[t][target[t]], z = x W^T: the product
+ * exact, sums and loss fp32.  x: `tokens` rows of in_features elements, row t
+ * at t * x_stride elements; w: `vocab` rows at w_stride; both of one `dtype`,
+ * H24_DTYPE_F16 or H24_DTYPE_BF16.  A token whose target is ignore_index has
+ * loss 0 and what its row of x holds does not matter; a target outside
+ * [0, vocab) makes the loss NaN, and the gradients.  loss: `tokens` fp32
+ * (H24_REDUCE_NONE) or one, the sum or the mean over the tokens that are not
+ * ignored (NaN where there is none).  state: 3 * tokens + 1 int32 for the
+ * backward pass.  Up to 2^24 in_features.  Scratch (a copy of the rows of x, 16
+ * bytes a token for each 256 of the vocabulary, and a copy of w where its rows
+ * are not on 16 bytes) comes from the library's pool and is freed on the
+ * stream.  h24_check reports a bounded wait that ran out. */
+int h24_linear_ce_forward(const void *x, int64_t tokens, int64_t x_stride, const void *w, int64_t vocab,
+                          int64_t w_stride, int64_t in_features, int dtype, const int64_t *target,
+                          int64_t ignore_index, int reduction, float *loss, int32_t *state, void *stream);
+
+/* dx[t] = g_t sum_v d[t][v] w[v] and dw[v] = sum_t g_t d[t][v] x[t], with
+ * d = softmax(z) - onehot(target) rounded to `dtype` (in fp16 held times 2^15),
+ * sums in fp32, each result rounded once.  x, w and the sizes are those of the
+ * forward call that wrote `state`, and unchanged.  dloss: the loss's gradient,
+ * one a token at t * dloss_stride (H24_REDUCE_NONE; for dw, x is first
+ * multiplied with g_t / max|g| and rounded) or one.  dx (tokens x in_features)
+ * and dw (vocab x in_features) are contiguous and of `dtype`; either may be
+ * NULL.  The logits are computed again, for a piece of the vocabulary at a
+ * time; scratch as above, and 2 * 96 MiB at most for the pieces (more where 256
+ * columns of all tokens are more) and 4 bytes for each element of dx and slice
+ * of its sum. */
+int h24_linear_ce_backward(const void *x, int64_t tokens, int64_t x_stride, const void *w, int64_t vocab,
+                           int64_t w_stride, int64_t in_features, int dtype, int reduction,
+                           const float *dloss, int64_t dloss_stride, const int32_t *state, void *dx,
+                           void *dw, void *stream);
+
+
 /* ---- nearest codeword (castor._leech_nn_kernel / castor_quantize_leech,
  *      castor.py:386-560; pack._quantize_h24_layer search, pack.py:166-177) --
  * x: n atoms of 24 fp32 values (16-byte aligned), out_idx: n int32 indices.

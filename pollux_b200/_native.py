@@ -26,6 +26,7 @@ H24_ERR_TIMEOUT = 4
 H24_ERR_STATE = 5
 RULE_TRAIN = 0
 RULE_PACK = 1
+REDUCE_NONE, REDUCE_MEAN, REDUCE_SUM = 0, 1, 2
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 KERNEL_SCREEN, KERNEL_RESCORE, KERNEL_PREP = 0, 1, 2
 
@@ -57,6 +58,8 @@ SIGNATURES = {
     "h24_int8_linear": (_I, [_P, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _I, _P, _P]),
     "h24_int8_linear_plan": (_I, [_I64, _I64, _I64, _I, _P]),
     "h24_sample_tokens": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _F, _P, _I, _P, _F, _P, _F, _P, _P, _P]),
+    "h24_linear_ce_forward": (_I, [_P, _I64, _I64, _P, _I64, _I64, _I64, _I, _P, _I64, _I, _P, _P, _P]),
+    "h24_linear_ce_backward": (_I, [_P, _I64, _I64, _P, _I64, _I64, _I64, _I, _I, _P, _I64, _P, _P, _P, _P]),
     "h24_quantize": (_I, [_P, _I64, _I, _P, _P]),
     "h24_quantize_layer": (_I, [_P, _I64, _I64, _P, _P, _P]),
     "h24_quantize_layer_host": (_I, [_P, _I64, _I64, _P, _P, _P]),

@@ -605,6 +605,59 @@ int h24_sample_tokens(const void *logits, int dtype, int64_t rows, int64_t vocab
                        top_p_all, min_p, min_p_all, tokens, logprobs, as_stream(stream));
 }
 
+static int check_ce(const char *what, const void *x, int64_t tokens, int64_t x_stride, const void *w, int64_t vocab,
+                    int64_t w_stride, int64_t in_features, int dtype, int reduction) {
+  const std::string name = what;
+  if (tokens < 0 || x_stride < 0 || w_stride < 0) return fail(H24_ERR_INVALID, name + ": negative size or stride");
+  if (vocab < 1 || in_features < 1) return fail(H24_ERR_INVALID, name + ": empty vocabulary or in_features");
+  if (in_features > (1 << 24)) return fail(H24_ERR_INVALID, name + ": in_features above 2^24");
+  if (tokens > INT32_MAX - 1024 || vocab > INT32_MAX - 1024 || ((tokens + 255) / 256) * ((vocab + 63) / 64) > (1 << 30))
+    return fail(H24_ERR_INVALID, name + ": too many tokens or too large a vocabulary");
+  if (dtype != H24_DTYPE_F16 && dtype != H24_DTYPE_BF16) return fail(H24_ERR_INVALID, name + ": dtype must be fp16 or bf16");
+  if (reduction != H24_REDUCE_NONE && reduction != H24_REDUCE_MEAN && reduction != H24_REDUCE_SUM)
+    return fail(H24_ERR_INVALID, name + ": unknown reduction");
+  if (tokens > 0 && (!x || !w)) return fail(H24_ERR_INVALID, name + ": null pointer");
+  if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 1) != 0)
+    return fail(H24_ERR_INVALID, name + ": unaligned elements");
+  return H24_OK;
+}
+
+int h24_linear_ce_forward(const void *x, int64_t tokens, int64_t x_stride, const void *w, int64_t vocab,
+                          int64_t w_stride, int64_t in_features, int dtype, const int64_t *target,
+                          int64_t ignore_index, int reduction, float *loss, int32_t *state, void *stream) {
+  const int rc = check_ce("linear_ce_forward", x, tokens, x_stride, w, vocab, w_stride, in_features, dtype, reduction);
+  if (rc != H24_OK) return rc;
+  if (tokens == 0) {
+    if (reduction == H24_REDUCE_NONE) return H24_OK;
+    if (!loss) return fail(H24_ERR_INVALID, "linear_ce_forward: null pointer");
+    // The sum over no token is 0, the mean NaN (all bits set).
+    H24_CUDA_TRY(cudaMemsetAsync(loss, reduction == H24_REDUCE_SUM ? 0 : 0xFF, sizeof(float), as_stream(stream)));
+    return H24_OK;
+  }
+  if (!target || !loss || !state) return fail(H24_ERR_INVALID, "linear_ce_forward: null pointer");
+  H24_TABLES_OR_FAIL(T);
+  return launch_ce_forward(T, {x, tokens, x_stride, w, vocab, w_stride, in_features, dtype, reduction}, target,
+                           ignore_index, loss, state, as_stream(stream));
+}
+
+int h24_linear_ce_backward(const void *x, int64_t tokens, int64_t x_stride, const void *w, int64_t vocab,
+                           int64_t w_stride, int64_t in_features, int dtype, int reduction,
+                           const float *dloss, int64_t dloss_stride, const int32_t *state, void *dx,
+                           void *dw, void *stream) {
+  const int rc = check_ce("linear_ce_backward", x, tokens, x_stride, w, vocab, w_stride, in_features, dtype, reduction);
+  if (rc != H24_OK) return rc;
+  if (dloss_stride < 0) return fail(H24_ERR_INVALID, "linear_ce_backward: negative size or stride");
+  if (!dx && !dw) return H24_OK;
+  if (tokens == 0) {
+    if (dw) H24_CUDA_TRY(cudaMemsetAsync(dw, 0, static_cast<size_t>(vocab * in_features * 2), as_stream(stream)));
+    return H24_OK;
+  }
+  if (!dloss || !state) return fail(H24_ERR_INVALID, "linear_ce_backward: null pointer");
+  H24_TABLES_OR_FAIL(T);
+  return launch_ce_backward(T, {x, tokens, x_stride, w, vocab, w_stride, in_features, dtype, reduction}, dloss,
+                            dloss_stride, state, dx, dw, as_stream(stream));
+}
+
 int h24_quantize(const float *x, int64_t n, int rule, int32_t *out_idx, void *stream) {
   H24_TABLES_OR_FAIL(T);
   if (n < 0) return fail(H24_ERR_INVALID, "quantize: negative atom count");

@@ -1,0 +1,1147 @@
+// h24_ce.cu -- softmax cross entropy of a head's product without its logits.
+//
+//   z[t][v] = sum_k x[t][k] W[v][k],  lse[t] = log sum_v exp(z[t][v])
+//   loss[t] = lse[t] - z[t][y_t]
+//   d[t][v] = softmax(z[t])[v] - [v = y_t]
+//   dx[t]   = g_t sum_v d[t][v] W[v],   dW[v] = sum_t g_t d[t][v] x[t]
+//
+// x and W are fp16 or bf16, products exact, sums fp32.  Tokens whose target is
+// ignored are left out: the others' rows are copied together first (a pass of
+// 4 bytes an element, which also gives rows that TMA can read), so a masked
+// token costs nothing and what stands in its row does not matter.
+//
+// All four products run in one kernel, ce_gemm_kernel: persistent pairs of CTAs
+// on 256 x 256 tiles (tcgen05.mma.cta_group::2, operands by TMA into a ring of
+// six stages, two accumulators in TMEM, eight epilogue warps a CTA), each
+// operand K-major or MN-major as it lies in memory, so nothing is transposed.
+//   forward: the logits' tiles end in a running maximum and a sum of
+//     exponentials a row (a TMEM lane, so a thread, holds a row);
+//   backward: the vocabulary goes by in pieces.  A piece's logits are computed
+//     again and end as d in 16 bits; its part of dx (added up in fp32) and its
+//     rows of dW are products with d.  One launch holds a piece's gradients and
+//     the logits of the next piece, the long tiles first, so that few SMs wait
+//     at a launch's end.
+// d is rounded to the operands' type (half a step, 2^-8 relative in bf16), as
+// the tensor cores want it; in fp16 it is held times 2^15, so that probabilities
+// down to 2^-39 keep their place.
+#include "h24_tile.cuh"
+
+namespace h24 {
+namespace {
+
+constexpr int kTileM = 256;      // rows of a pair's tile, 128 a CTA
+constexpr int kTileN = 256;      // its columns at most
+constexpr int kTileK = 64;       // k of a stage: one 128-byte swizzle row of 16-bit elements
+constexpr int kOperand = 128 * 128;  // bytes of a CTA's share of an operand's stage
+constexpr int kStage = 2 * kOperand;
+constexpr int kStages = 6;
+constexpr int kHead = 1024;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 320;    // warp 0 loads, warp 1 issues MMAs, warps 2-9 read TMEM
+constexpr int kStagePitch = 33;  // fp32 of a row of an epilogue warp's 32 x 32 block
+constexpr int kBlockBytes = 32 * kStagePitch * 4;
+constexpr int kSmem = 1024 + kHead + kStages * kStage + kEpiWarps * kBlockBytes;
+static_assert(kSmem <= 227 * 1024, "shared memory");
+constexpr int kChunk = 64;       // columns of an MN-major box
+constexpr int kMaxJobs = 3;
+constexpr int kGroupM = 32;      // row tiles that run through the vocabulary together
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNegInf = -INFINITY;
+
+enum Kind { kLoss, kProb, kStates, kHeadRows };
+
+// One product of a launch.  Rows and sums over tokens go by the number of kept
+// tokens, which only the device knows.
+struct Job {
+  int kind;
+  int n_total, bn;   // columns, of which a tile takes bn
+  int m_total;       // rows (kHeadRows); the other kinds' rows are the tokens
+  int k_total;       // length of the sum (kHeadRows: the tokens)
+  int split;         // slices of the sum, each with its own output (kStates)
+  int v0;            // first vocabulary row of the piece
+  bool add;          // kStates: onto what is there
+  void *out;
+  int64_t pitch;     // elements between the output's rows
+  int64_t plane;     // elements between the slices' outputs
+};
+
+struct GemmArgs {
+  CUtensorMap map[2 * kMaxJobs];  // A and B of each job
+  Job job[kMaxJobs];
+  int jobs;
+  int vocab;
+  const int *kept;     // number of tokens with a loss
+  const int *target;   // of each kept token
+  const float *lse;    // of each kept token
+  float *z_target;
+  float2 *parts;       // kLoss: maximum and sum of half a tile's columns
+  int64_t part_pitch;
+  const float *scale;  // kHeadRows: factor of the sum
+  float prob_scale;
+  bool wide_rows;      // kHeadRows: rows of the output lie on 32 bytes
+  int *err;
+};
+
+struct PairHead {
+  uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], drain;
+  uint32_t tmem;
+  int abort;
+};
+static_assert(sizeof(PairHead) <= kHead, "head");
+
+// Shared-memory descriptor of an MN-major operand with the 128-byte swizzle:
+// boxes of 64 columns (128 bytes) x 64 k, 8 KB apart; groups of 8 k 1,024
+// bytes apart.
+__device__ __forceinline__ uint64_t mn_desc(uint32_t addr) {
+  return tile_desc(addr) | (uint64_t((kChunk * 128) >> 4) << 16);
+}
+
+// Instruction descriptor: kind::f16, D fp32, A and B of one 16-bit type, each
+// K-major (0) or MN-major (1), M = 256.
+__device__ __forceinline__ uint32_t f16_idesc(bool bf16, int a_mn, int b_mn, int n) {
+  const uint32_t type = bf16 ? 1u : 0u;
+  return (1u << 4) | (type << 7) | (type << 10) | (static_cast<uint32_t>(a_mn) << 15) |
+         (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (static_cast<uint32_t>(kTileM >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_f16_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+struct Tile {
+  int job, m, n, cols;  // first row, first column, columns (a multiple of 32)
+  int kb, nkb, slice;   // k blocks
+};
+
+__device__ __forceinline__ int tiles_of(const Job &j, int kept) {
+  const int rows = j.kind == kHeadRows ? j.m_total : kept;
+  return (rows + kTileM - 1) / kTileM * ((j.n_total + j.bn - 1) / j.bn) * j.split;
+}
+
+__device__ __forceinline__ Tile tile_at(const GemmArgs &a, int kept, int idx) {
+  Tile t;
+  t.job = 0;
+  for (; t.job + 1 < a.jobs; ++t.job) {
+    const int c = tiles_of(a.job[t.job], kept);
+    if (idx < c) break;
+    idx -= c;
+  }
+  const Job &j = a.job[t.job];
+  const int nt = (j.n_total + j.bn - 1) / j.bn;
+  const int mt = ((j.kind == kHeadRows ? j.m_total : kept) + kTileM - 1) / kTileM;
+  int m, n;
+  t.slice = 0;
+  if (j.kind == kLoss || j.kind == kProb) {
+    // Up to 32 row tiles side by side, so that these rows stay in L2 while the
+    // vocabulary passes once.
+    const int group = idx / (kGroupM * nt), g = min(kGroupM, mt - group * kGroupM);
+    const int at = idx - group * kGroupM * nt;
+    n = at / g;
+    m = group * kGroupM + at - n * g;
+  } else {
+    // All columns of a row tile side by side: d, the larger operand, passes once.
+    n = idx % nt;
+    const int rest = idx / nt;
+    t.slice = rest / mt;
+    m = rest - t.slice * mt;
+  }
+  t.m = m * kTileM;
+  t.n = n * j.bn;
+  t.cols = min(j.bn, (j.n_total - t.n + 31) / 32 * 32);
+  const int kblocks = ((j.kind == kHeadRows ? kept : j.k_total) + kTileK - 1) / kTileK;
+  t.kb = static_cast<int>(static_cast<int64_t>(kblocks) * t.slice / j.split);
+  t.nkb = static_cast<int>(static_cast<int64_t>(kblocks) * (t.slice + 1) / j.split) - t.kb;
+  return t;
+}
+
+__device__ __forceinline__ void store32B(void *p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+__device__ __forceinline__ void load32B(const void *p, uint32_t (&w)[8]) {
+  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(p)
+               : "memory");
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (kBf16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  } else {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  }
+}
+template <bool kBf16>
+__device__ __forceinline__ uint16_t pack1(float a) {
+  if constexpr (kBf16) return __bfloat16_as_ushort(__float2bfloat16_rn(a));
+  return __half_as_ushort(__float2half_rn(a));
+}
+
+// What an epilogue thread does with 32 columns of its row.  `c` is the column
+// within the tile; r the sums.
+struct RowState {
+  int64_t row;   // of the job's output
+  bool live;
+  float lse2;    // kProb: log2e * lse
+  int target;    // kLoss, kProb: the target's column of the tile (any number where it is elsewhere)
+  int limit;     // kLoss, kProb: columns of the tile that the vocabulary has
+  float m, s, z; // kLoss: running maximum, sum of exponentials, the target's logit
+  bool found;
+};
+
+__device__ __forceinline__ void loss_chunk(RowState &st, int c, const float (&z)[32]) {
+  float top = kNegInf;
+  if (c + 32 <= st.limit) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) top = fmaxf(top, z[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (c + j < st.limit) top = fmaxf(top, z[j]);
+  }
+  const float m = fmaxf(st.m, top);
+  const float base = m == kNegInf ? 0.f : m * kLog2e;
+  float s0 = st.s * exp2_fast(fmaf(st.m, kLog2e, -base)), s1 = 0.f;  // (2^-inf is 0)
+  if (c + 32 <= st.limit) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      s0 += exp2_fast(fmaf(z[j], kLog2e, -base));
+      s1 += exp2_fast(fmaf(z[j + 1], kLog2e, -base));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (c + j < st.limit) s0 += exp2_fast(fmaf(z[j], kLog2e, -base));
+  }
+  st.s = s0 + s1;
+  st.m = m;
+  const int at = st.target - c;
+  if (static_cast<unsigned>(at) < 32u) {
+    st.found = true;
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j == at) st.z = z[j];
+  }
+}
+
+template <bool kBf16>
+__device__ __forceinline__ void prob_chunk(const GemmArgs &a, const RowState &st, uint16_t *out, int c,
+                                           const float (&z)[32]) {
+  float d[32];
+#pragma unroll
+  for (int j = 0; j < 32; ++j) d[j] = exp2_fast(fmaf(z[j], kLog2e, -st.lse2)) * a.prob_scale;
+  const int at = st.target - c;
+  if (static_cast<unsigned>(at) < 32u) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (j == at) d[j] -= a.prob_scale;
+  }
+  if (!st.live || c + 32 > st.limit) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (!st.live || c + j >= st.limit) d[j] = 0.f;
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = pack2<kBf16>(d[16 * h + 2 * j], d[16 * h + 2 * j + 1]);
+    store32B(out + c + 16 * h, w);
+  }
+}
+
+__device__ __forceinline__ void states_chunk(bool add, float *out, const float (&z)[32]) {
+  uint32_t w[4][8];
+  if (add) {
+#pragma unroll
+    for (int h = 0; h < 4; ++h) load32B(out + 8 * h, w[h]);
+  }
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      w[h][j] = __float_as_uint(add ? __uint_as_float(w[h][j]) + z[8 * h + j] : z[8 * h + j]);
+    store32B(out + 8 * h, w[h]);
+  }
+}
+
+template <bool kBf16>
+__global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_constant__ GemmArgs a) {
+  extern __shared__ uint8_t ce_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(ce_raw) + 1023) & ~uintptr_t(1023));
+  PairHead &H = *reinterpret_cast<PairHead *>(smem);
+  uint8_t *stages = smem + kHead;
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+  const int rank = static_cast<int>(blockIdx.x) & 1;
+  const int first = static_cast<int>(blockIdx.x) >> 1, step = static_cast<int>(gridDim.x) >> 1;
+  volatile int *abort = &H.abort;
+
+  if (t == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      bar_init(&H.full[s], 1);
+      bar_init(&H.empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      bar_init(&H.acc_full[s], 1);
+      bar_init(&H.acc_empty[s], 2 * kEpiWarps);
+    }
+    bar_init(&H.drain, 1);
+    H.abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    for (int i = 0; i < 2 * a.jobs; ++i) asm volatile("prefetch.tensormap [%0];" ::"l"(&a.map[i]) : "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(&H.tmem)), "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers stand
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = H.tmem;
+  pdl_enter();
+  const int kept = *a.kept;
+  int tiles = 0;
+  for (int j = 0; j < a.jobs; ++j) tiles += tiles_of(a.job[j], kept);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      asm volatile("fence.proxy.async;" ::: "memory");  // the rows were written by ordinary stores
+      int s = 0;
+      uint32_t ph = 0;
+      for (int idx = first; idx < tiles; idx += step) {
+        const Tile tl = tile_at(a, kept, idx);
+        const Job &j = a.job[tl.job];
+        const CUtensorMap *ma = &a.map[2 * tl.job], *mb = ma + 1;
+        const int half = tl.cols / 2, chunks = (half + kChunk - 1) / kChunk;
+        const bool a_mn = j.kind == kHeadRows, b_mn = j.kind == kStates || j.kind == kHeadRows;
+        const uint32_t bytes = kOperand + (b_mn ? chunks * (kOperand / 2) : j.bn / 2 * 128);
+        const int am = tl.m + rank * (kTileM / 2), bn = tl.n + rank * half;
+        for (int i = 0; i < tl.nkb; ++i) {
+          if (!bar_wait(&H.empty[s], ph ^ 1, abort, a.err)) goto loaded;
+          uint8_t *sa = stages + static_cast<size_t>(s) * kStage, *sb = sa + kOperand;
+          const int k = (tl.kb + i) * kTileK;
+          // The first CTA's barrier counts the bytes of both; its phase cannot
+          // end before its own arrival here.
+          const uint32_t bar = cluster_addr(&H.full[s], 0);
+          if (rank == 0) bar_expect(&H.full[s], 2 * bytes);
+          if (a_mn) {
+            tma_load_pair(ma, sa, bar, am, k);
+            tma_load_pair(ma, sa + kOperand / 2, bar, am + kChunk, k);
+          } else {
+            tma_load_pair(ma, sa, bar, k, am);
+          }
+          if (b_mn) {
+            const int kr = j.kind == kStates ? j.v0 + k : k;
+            for (int c = 0; c < chunks; ++c) tma_load_pair(mb, sb + c * (kOperand / 2), bar, bn + c * kChunk, kr);
+          } else {
+            tma_load_pair(mb, sb, bar, k, j.v0 + bn);
+          }
+          if (++s == kStages) s = 0, ph ^= 1;
+        }
+      }
+    loaded:
+      if (*abort) {  // copies in flight land long before this
+        const unsigned long long t1 = now_ns();
+        while (now_ns() - t1 < 20000000ull) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      int s = 0, acc = 0;
+      uint32_t ph = 0, acc_ph = 0;
+      bool ok = true;
+      for (int idx = first; ok && idx < tiles; idx += step) {
+        const Tile tl = tile_at(a, kept, idx);
+        const Job &j = a.job[tl.job];
+        const bool a_mn = j.kind == kHeadRows, b_mn = j.kind == kStates || j.kind == kHeadRows;
+        const uint32_t idesc = f16_idesc(kBf16, a_mn, b_mn, tl.cols);
+        // 16 k are 32 bytes of a K-major row, 16 rows of 128 bytes of an MN-major box.
+        const uint64_t step_a = a_mn ? 2048 >> 4 : 32 >> 4, step_b = b_mn ? 2048 >> 4 : 32 >> 4;
+        ok = __all_sync(0xffffffffu, bar_wait(&H.acc_empty[acc], acc_ph ^ 1, abort, a.err));
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        for (int i = 0; i < tl.nkb; ++i) {
+          ok = __all_sync(0xffffffffu, bar_wait(&H.full[s], ph, abort, a.err));
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t st = su32(stages) + static_cast<uint32_t>(s * kStage);
+          const uint64_t ad = a_mn ? mn_desc(st) : tile_desc(st);
+          const uint64_t bd = b_mn ? mn_desc(st + kOperand) : tile_desc(st + kOperand);
+#pragma unroll
+          for (int k = 0; k < kTileK / 16; ++k)
+            mma_f16_pair(tmem + acc * kTileN, ad + k * step_a, bd + k * step_b, idesc, i > 0 || k > 0);
+          mma_commit_pair(&H.empty[s]);
+          if (++s == kStages) s = 0, ph ^= 1;
+        }
+        if (!ok) break;
+        mma_commit_pair(&H.acc_full[acc]);
+        if (++acc == 2) acc = 0, acc_ph ^= 1;
+      }
+      // No MMA of the pair is left when this arrives (the last sync below holds
+      // the other CTA until then).
+      asm volatile(
+          "{\n\t.reg .pred e;\n\t"
+          "elect.sync _|e, 0xffffffff;\n\t"
+          "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(su32(&H.drain))
+          : "memory");
+      bar_wait(&H.drain, 0, abort, a.err, false);
+    }
+  } else {
+    // The warp's number from lane 0: the compiler then keeps what follows from
+    // it, the column addresses above all, in uniform registers.
+    const int uwarp = __shfl_sync(0xffffffffu, warp, 0);
+    const int quarter = uwarp & 3, part = (uwarp - 2) >> 2;  // TMEM lanes, and first or second part of the columns
+    const uint32_t ta = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+    float *block = reinterpret_cast<float *>(stages + kStages * kStage) + (uwarp - 2) * 32 * kStagePitch;
+    int acc = 0;
+    uint32_t ph = 0;
+    for (int idx = first; idx < tiles; idx += step) {
+      const Tile tl = tile_at(a, kept, idx);
+      const Job &j = a.job[tl.job];
+      const int mid = (tl.cols / 2 + 31) / 32 * 32, c0 = part ? mid : 0, c1 = part ? tl.cols : mid;
+      const int row0 = tl.m + rank * (kTileM / 2) + quarter * 32, row = row0 + lane;
+      RowState st;
+      st.live = row < (j.kind == kHeadRows ? j.m_total : kept);
+      st.target = 0x7fffffff;
+      st.lse2 = 0.f;
+      st.limit = a.vocab - (j.v0 + tl.n);
+      st.m = kNegInf;
+      st.s = st.z = 0.f;
+      st.found = false;
+      if ((j.kind == kLoss || j.kind == kProb) && st.live) {
+        st.target = a.target[row] - (j.v0 + tl.n);
+        if (j.kind == kProb) st.lse2 = a.lse[row] * kLog2e;
+      }
+      const float scale = j.kind == kHeadRows ? *a.scale : 1.f;
+      if (!__all_sync(0xffffffffu, bar_wait(&H.acc_full[acc], ph, abort, a.err))) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t d = ta + acc * kTileN;
+      for (int c = c0; c < c1; c += 32) {
+        int r[32];
+        float z[32];
+        __syncwarp();
+        tmem_ask32(d + c, r);
+        tmem_wait32(r);
+        if (tl.nkb == 0) {  // an empty sum has no MMA
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) z[i] = __int_as_float(r[i]);
+        if (j.kind == kLoss) {
+          loss_chunk(st, c, z);
+        } else if (j.kind == kProb) {
+          prob_chunk<kBf16>(a, st, static_cast<uint16_t *>(j.out) + row * j.pitch + tl.n, c, z);
+        } else if (j.kind == kStates) {
+          if (st.live)
+            states_chunk(j.add, static_cast<float *>(j.out) + tl.slice * j.plane + row * j.pitch + tl.n + c, z);
+        } else {
+          uint16_t *out = static_cast<uint16_t *>(j.out) + (j.v0 + static_cast<int64_t>(row0)) * j.pitch + tl.n + c;
+          const int left = j.n_total - (tl.n + c);
+          if (a.wide_rows) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t w[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) w[i] = pack2<kBf16>(z[16 * h + 2 * i] * scale, z[16 * h + 2 * i + 1] * scale);
+              if (st.live && 16 * h < left) store32B(out + lane * j.pitch + 16 * h, w);
+            }
+          } else {
+            // Rows off 32 bytes: a warp writes a row's 32 elements at a time.
+#pragma unroll
+            for (int i = 0; i < 32; ++i) block[lane * kStagePitch + i] = z[i] * scale;
+            __syncwarp();
+            const int rows = min(32, j.m_total - row0);
+            if (lane < left)
+              for (int i = 0; i < rows; ++i) out[i * j.pitch + lane] = pack1<kBf16>(block[i * kStagePitch + lane]);
+          }
+        }
+      }
+      // The accumulator is free once both CTAs' warps have read it.
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                         cluster_addr(&H.acc_empty[acc], 0))
+                     : "memory");
+      if (j.kind == kLoss && st.live) {
+        a.parts[(static_cast<int64_t>(tl.n / j.bn) * 2 + part) * a.part_pitch + row] = make_float2(st.m, st.s);
+        if (st.found) a.z_target[row] = st.z;
+      }
+      if (++acc == 2) acc = 0, ph ^= 1;
+    }
+  }
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync_all();  // no CTA leaves while the other may signal it
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+// ---------------------------------------------------------------------------
+// Rows: which tokens have a loss, and their states side by side
+// ---------------------------------------------------------------------------
+constexpr int kRowThreads = 256;
+
+// What the forward pass leaves for the backward pass: the number of kept
+// tokens, each token's place among them (-1: ignored), and by place the target
+// (-1: not in the vocabulary) and the log of the sum of exponentials.
+struct State {
+  int *kept, *place, *target;
+  float *lse;
+};
+State state_at(const int32_t *state, int64_t tokens) {
+  int32_t *p = const_cast<int32_t *>(state);  // (only the forward pass writes it)
+  return {p, p + 1, p + 1 + tokens, reinterpret_cast<float *>(p + 1 + 2 * tokens)};
+}
+
+struct RowsArgs {
+  const void *x;
+  int64_t x_stride;
+  int tokens, in;
+  const int64_t *labels;
+  int64_t ignore;
+  int vocab;
+  State st;
+  int *token;      // of each place
+  uint16_t *rows;  // copied states, `pitch` elements a row
+  int64_t pitch;
+  float *loss;     // of each token, or null
+  unsigned *ticket;
+  int per_block;
+  bool vec;        // rows of x lie on 16 bytes
+};
+
+// One row, by a warp.
+__device__ __forceinline__ void copy_row(const uint16_t *src, uint16_t *dst, int n, bool vec, int lane) {
+  if (vec) {
+    for (int c = lane; c < n / 8; c += 32) reinterpret_cast<uint4 *>(dst)[c] = reinterpret_cast<const uint4 *>(src)[c];
+  } else {
+    for (int c = lane; c < n; c += 32) dst[c] = src[c];
+  }
+}
+
+__device__ __forceinline__ int block_sum(int v, int *red) {
+  v = __reduce_add_sync(0xffffffffu, v);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  int sum = 0;
+  for (int w = 0; w < kRowThreads / 32; ++w) sum += red[w];
+  __syncthreads();
+  return sum;
+}
+
+// Block b takes tokens b * per_block on.  It counts the kept tokens before its
+// own, so the places are those of the tokens' order whatever the blocks' order
+// is (the targets, 8 bytes a token, lie in L2).
+__global__ void __launch_bounds__(kRowThreads) ce_rows_kernel(const RowsArgs a) {
+  __shared__ int red[kRowThreads / 32], warp_base[kRowThreads / 32], from[kRowThreads];
+  pdl_enter();
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * a.per_block;
+  int before = 0;
+  for (int64_t i = t; i < r0; i += kRowThreads) before += __ldg(a.labels + i) != a.ignore;
+  before = block_sum(before, red);
+  // per_block is at most the number of threads.
+  const int64_t r = r0 + t;
+  const bool mine = t < a.per_block && r < a.tokens;
+  const int64_t label = mine ? __ldg(a.labels + r) : a.ignore;
+  const bool keep = mine && label != a.ignore;
+  const unsigned votes = __ballot_sync(0xffffffffu, keep);
+  if (lane == 0) warp_base[warp] = __popc(votes);
+  __syncthreads();
+  int at = __popc(votes & ((1u << lane) - 1)), count = 0;
+  for (int w = 0; w < kRowThreads / 32; ++w) {
+    if (w < warp) at += warp_base[w];
+    count += warp_base[w];
+  }
+  if (mine) {
+    a.st.place[r] = keep ? before + at : -1;
+    if (!keep && a.loss) a.loss[r] = 0.f;
+  }
+  if (keep) {
+    from[at] = t;
+    a.st.target[before + at] = label >= 0 && label < a.vocab ? static_cast<int>(label) : -1;
+    if (a.token) a.token[before + at] = static_cast<int>(r);
+  }
+  __syncthreads();
+  const uint16_t *x = static_cast<const uint16_t *>(a.x);
+  for (int i = warp; i < count; i += kRowThreads / 32)
+    copy_row(x + (r0 + from[i]) * a.x_stride, a.rows + (before + static_cast<int64_t>(i)) * a.pitch, a.in, a.vec, lane);
+  if (blockIdx.x + 1 == gridDim.x && t == 0) {
+    *a.st.kept = before + count;
+    *a.ticket = 0;
+  }
+}
+
+struct BackRowsArgs {
+  const void *x;
+  int64_t x_stride;
+  int tokens, in;
+  State st;
+  uint16_t *rows;    // copied states
+  uint16_t *scaled;  // the same times g / max |g|, or null (g the same for all)
+  int64_t pitch;
+  const float *dloss;
+  int64_t dloss_stride;
+  bool mean, vec;
+  float inv_prob_scale;
+  float *scale;      // [0] factor of dW, [1] factor of dx where g is the same for all
+  int per_block;
+};
+
+// The copies of the backward pass.  A token's own factor g goes into its states
+// for dW, relative to the largest one (so that it neither passes the type's
+// range nor falls below it: what a much smaller factor loses is small beside
+// dW), and into dx exactly, at the end.
+template <bool kBf16>
+__global__ void __launch_bounds__(kRowThreads) ce_back_rows_kernel(const BackRowsArgs a) {
+  __shared__ float red[kRowThreads / 32];
+  pdl_enter();
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int kept = *a.st.kept;
+  float top = 0.f;
+  if (a.scaled) {
+    for (int64_t i = t; i < a.tokens; i += kRowThreads)
+      if (__ldg(a.st.place + i) >= 0) {
+        const float g = fabsf(__ldg(a.dloss + i * a.dloss_stride));
+        top = g != g ? g : fmaxf(g, top);  // (a NaN that is overtaken here is in the states all the same)
+      }
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) red[warp] = top;
+    __syncthreads();
+    top = 0.f;
+    for (int w = 0; w < kRowThreads / 32; ++w) top = fmaxf(top, red[w]);
+  }
+  const uint16_t *x = static_cast<const uint16_t *>(a.x);
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * a.per_block;
+  for (int64_t r = r0 + warp; r < r0 + a.per_block && r < a.tokens; r += kRowThreads / 32) {
+    const int place = a.st.place[r];
+    if (place < 0) continue;
+    const uint16_t *src = x + r * a.x_stride;
+    copy_row(src, a.rows + place * a.pitch, a.in, a.vec, lane);
+    if (a.scaled) {
+      const float g = top > 0.f ? a.dloss[r * a.dloss_stride] / top : a.dloss[r * a.dloss_stride];
+      for (int c = lane; c < a.in; c += 32) {
+        const float v = kBf16 ? __bfloat162float(__ushort_as_bfloat16(src[c])) : __half2float(__ushort_as_half(src[c]));
+        a.scaled[place * a.pitch + c] = pack1<kBf16>(v * g);
+      }
+    }
+  }
+  if (blockIdx.x + 1 == gridDim.x) {
+    // The sums over tokens run in steps of 64: zeros up to there.
+    const int end = (kept + kTileK - 1) / kTileK * kTileK;
+    uint16_t *rows = a.scaled ? a.scaled : a.rows;
+    for (int r = kept + warp; r < end; r += kRowThreads / 32)
+      for (int c = lane; c < a.in; c += 32) rows[r * a.pitch + c] = 0;
+    if (t == 0) {
+      const float g = a.scaled ? (top > 0.f ? top : 1.f) : a.mean ? a.dloss[0] / static_cast<float>(kept) : a.dloss[0];
+      a.scale[0] = kept ? g * a.inv_prob_scale : 0.f;
+      a.scale[1] = g * a.inv_prob_scale;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The loss from the tiles' maxima and sums
+// ---------------------------------------------------------------------------
+struct CombineArgs {
+  State st;
+  const float2 *parts;
+  int64_t part_pitch;
+  int n_parts;
+  const float *z_target;
+  const int *token;
+  float *row_loss;   // by place (sum, mean)
+  float *loss;       // of each token, or the one value
+  int reduction;     // H24_REDUCE_*
+  unsigned *ticket;
+};
+constexpr int kCombineRows = 4;  // 32 bytes of neighbouring parts
+
+__global__ void __launch_bounds__(kRowThreads) ce_combine_kernel(const CombineArgs a) {
+  __shared__ float2 red[kRowThreads / 32][kCombineRows];
+  __shared__ double sums[kRowThreads / 32];
+  __shared__ bool last;
+  pdl_enter();
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, kept = *a.st.kept;
+  const int r = t % kCombineRows;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kCombineRows + r;
+  auto join = [](float2 &p, float2 q) {
+    const float m = fmaxf(p.x, q.x), base = m == kNegInf ? 0.f : m * kLog2e;
+    p.y = p.y * exp2_fast(fmaf(p.x, kLog2e, -base)) + q.y * exp2_fast(fmaf(q.x, kLog2e, -base));
+    p.x = m;
+  };
+  float2 p = make_float2(kNegInf, 0.f);
+  if (row < kept) {
+#pragma unroll 4
+    for (int i = t / kCombineRows; i < a.n_parts; i += kRowThreads / kCombineRows)
+      join(p, __ldg(a.parts + i * a.part_pitch + row));
+  }
+  for (int o = 16; o >= kCombineRows; o >>= 1)
+    join(p, make_float2(__shfl_xor_sync(0xffffffffu, p.x, o), __shfl_xor_sync(0xffffffffu, p.y, o)));
+  if (lane < kCombineRows) red[warp][lane] = p;
+  __syncthreads();
+  if (t < kCombineRows && row < kept) {
+    for (int w = 1; w < kRowThreads / 32; ++w) join(p, red[w][t]);
+    // A target outside the vocabulary has no loss: NaN, here and in the gradients.
+    const bool known = a.st.target[row] >= 0;
+    const float lse = known ? p.x + logf(p.y) : __int_as_float(0x7fffffff);
+    const float loss = known ? lse - a.z_target[row] : lse;
+    a.st.lse[row] = lse;
+    if (a.reduction == H24_REDUCE_NONE)
+      a.loss[a.token[row]] = loss;
+    else
+      a.row_loss[row] = loss;
+  }
+  if (a.reduction == H24_REDUCE_NONE) return;
+  // The block that is last to finish adds up all rows, in an order of its own
+  // threads: the same for every call.
+  __threadfence();
+  __syncthreads();
+  if (t == 0) last = atomicAdd(a.ticket, 1u) + 1 == gridDim.x;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double sum = 0.0;
+  for (int i = t; i < kept; i += kRowThreads) sum += static_cast<double>(__ldcg(a.row_loss + i));
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) sums[warp] = sum;
+  __syncthreads();
+  if (t == 0) {
+    sum = 0.0;
+    for (int w = 0; w < kRowThreads / 32; ++w) sum += sums[w];
+    *a.loss = static_cast<float>(a.reduction == H24_REDUCE_MEAN ? sum / kept : sum);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// dx from the slices' sums
+// ---------------------------------------------------------------------------
+struct StatesArgs {
+  State st;
+  const float *acc;
+  int64_t pitch, plane;
+  int slices;
+  int64_t tokens;
+  int in;
+  const float *scale;
+  const float *dloss;  // a factor for each token, or null
+  int64_t dloss_stride;
+  float inv_prob_scale;
+  uint16_t *out;
+  bool vec;            // out's rows lie on 16 bytes
+};
+
+template <bool kBf16>
+__global__ void __launch_bounds__(kRowThreads) ce_states_kernel(const StatesArgs a) {
+  pdl_enter();
+  const int groups = (a.in + 7) / 8;
+  const int64_t total = a.tokens * groups;
+  for (int64_t i = blockIdx.x * static_cast<int64_t>(kRowThreads) + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * kRowThreads) {
+    const int64_t r = i / groups;
+    const int c = static_cast<int>(i - r * groups) * 8;
+    const int place = __ldg(a.st.place + r);
+    float v[8] = {};
+    if (place >= 0) {
+      // (The rows of acc are padded to 32 columns.)
+      const float *p = a.acc + place * a.pitch + c;
+      for (int s = 0; s < a.slices; ++s, p += a.plane) {
+        const float4 x = __ldcs(reinterpret_cast<const float4 *>(p)), y = __ldcs(reinterpret_cast<const float4 *>(p) + 1);
+        v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+        v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+      }
+      const float g = a.dloss ? a.dloss[r * a.dloss_stride] * a.inv_prob_scale : a.scale[1];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= g;
+    }
+    uint16_t *out = a.out + r * a.in + c;
+    if (a.vec) {
+      *reinterpret_cast<uint4 *>(out) = make_uint4(pack2<kBf16>(v[0], v[1]), pack2<kBf16>(v[2], v[3]),
+                                                   pack2<kBf16>(v[4], v[5]), pack2<kBf16>(v[6], v[7]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < a.in) out[j] = pack1<kBf16>(v[j]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+constexpr int64_t kPieceBytes = int64_t(96) << 20;  // of d, for one piece of the vocabulary
+
+// Map of a matrix of 16-bit elements [rows][cols], row pitch `pitch` elements,
+// in boxes of 64 columns x box_rows with the 128-byte swizzle.
+bool map16(CUtensorMap *map, const void *base, int64_t rows, int64_t cols, int64_t pitch, int box_rows) {
+  const EncodeTiled fn = encode_tiled();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch) * 2};
+  const cuuint32_t box[2] = {kTileK, static_cast<cuuint32_t>(box_rows)}, es[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void *>(base), dims, strides, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+int64_t cdiv(int64_t n, int64_t by) { return (n + by - 1) / by; }
+
+// Pool scratch that is freed on the stream when the call is through with it.
+struct Scratch {
+  cudaStream_t s;
+  uint8_t *base = nullptr;
+  int64_t used = 0;
+  explicit Scratch(cudaStream_t stream) : s(stream) {}
+  ~Scratch() {
+    if (base) cudaFreeAsync(base, s);
+  }
+  // Offsets are given out first, then one block is allocated.
+  int64_t take(int64_t bytes) {
+    const int64_t at = used;
+    used += up(bytes, 256);
+    return at;
+  }
+  int allocate(const Tables *T) {
+    H24_CUDA_TRY(cudaMallocFromPoolAsync(reinterpret_cast<void **>(&base), static_cast<size_t>(used > 0 ? used : 256),
+                                         T->pool, s));
+    return H24_OK;
+  }
+  template <typename P>
+  P *at(int64_t offset) const {
+    return reinterpret_cast<P *>(base + offset);
+  }
+};
+
+int launch_gemm(const GemmArgs &a, bool bf16, int64_t tiles, cudaStream_t s) {
+  H24_CUDA_TRY(bf16 ? allow_smem<ce_gemm_kernel<true>>(kSmem) : allow_smem<ce_gemm_kernel<false>>(kSmem));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * (tiles < 1 ? 1 : tiles < kPairs ? tiles : kPairs)));
+  cfg.blockDim = dim3(kThreads);
+  // All of the SM's shared memory: the pair takes all TMEM columns, so nothing
+  // that waits for columns may be resident beside it.
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  H24_CUDA_TRY(cudaLaunchKernelEx(&cfg, bf16 ? ce_gemm_kernel<true> : ce_gemm_kernel<false>, a));
+  count_launches(1);
+  return H24_OK;
+}
+
+// Columns of the logits' tiles: 256, fewer where that leaves pairs of SMs without one.
+int logits_bn(int64_t tokens, int64_t vocab) {
+  int bn = kTileN;
+  while (bn > 64 && cdiv(tokens, kTileM) * cdiv(vocab, bn) < kPairs) bn /= 2;
+  return bn;
+}
+
+// Rows of a block of the row kernels: the blocks fill the GPU four times at most.
+int rows_per_block(int64_t tokens) {
+  const int64_t per = cdiv(tokens, 592);
+  return static_cast<int>(per > kRowThreads ? kRowThreads : per);
+}
+
+bool rows_on_16(const void *p, int64_t pitch, int64_t cols) { return aligned16(p) && pitch % 8 == 0 && cols % 8 == 0; }
+
+// W as TMA can read it: itself, or a copy with rows on 16 bytes.
+int readable_head(const CeArgs &c, const Scratch &sc, int64_t copy_at, const void **w, int64_t *pitch) {
+  *w = c.w;
+  *pitch = c.w_stride;
+  if (copy_at < 0) return H24_OK;
+  *w = sc.at<void>(copy_at);
+  *pitch = up(c.in, 8);
+  const RepackArgs rw{static_cast<const int8_t *>(c.w), 2 * c.w_stride, sc.at<int8_t>(copy_at), c.vocab}, none{};
+  const int chunks = static_cast<int>(*pitch / 8);
+  H24_CUDA_TRY(launch_pdl(repack_rows_kernel, dim3(wave_grid(cdiv(c.vocab * chunks, kRepackThreads), 8)),
+                          dim3(kRepackThreads), sc.s, rw, none, static_cast<int>(2 * c.in), chunks));
+  count_launches(1);
+  return H24_OK;
+}
+bool head_readable(const CeArgs &c) { return aligned16(c.w) && c.w_stride % 8 == 0 && c.w_stride >= c.in; }
+
+}  // namespace
+
+int launch_ce_forward(const Tables *T, const CeArgs &c, const int64_t *labels, int64_t ignore, float *loss,
+                      int32_t *state, cudaStream_t s) {
+  const bool bf16 = c.dtype == H24_DTYPE_BF16;
+  const int bn = logits_bn(c.tokens, c.vocab);
+  const int64_t n_tiles = cdiv(c.vocab, bn), pitch = up(c.in, 8), part_pitch = up(c.tokens, kCombineRows);
+  Scratch sc(s);
+  const int64_t rows_at = sc.take((c.tokens + kTileK) * pitch * 2), token_at = sc.take(c.tokens * 4);
+  const int64_t zt_at = sc.take(c.tokens * 4), loss_at = sc.take(c.tokens * 4), ticket_at = sc.take(4);
+  const int64_t parts_at = sc.take(2 * n_tiles * part_pitch * 8);
+  const int64_t w_at = head_readable(c) ? -1 : sc.take(c.vocab * pitch * 2);
+  int rc = sc.allocate(T);
+  if (rc != H24_OK) return rc;
+  const State st = state_at(state, c.tokens);
+  RowsArgs r{};
+  r.x = c.x;
+  r.x_stride = c.x_stride;
+  r.tokens = static_cast<int>(c.tokens);
+  r.in = static_cast<int>(c.in);
+  r.labels = labels;
+  r.ignore = ignore;
+  r.vocab = static_cast<int>(c.vocab);
+  r.st = st;
+  r.token = sc.at<int>(token_at);
+  r.rows = sc.at<uint16_t>(rows_at);
+  r.pitch = pitch;
+  r.loss = c.reduction == H24_REDUCE_NONE ? loss : nullptr;
+  r.ticket = sc.at<unsigned>(ticket_at);
+  r.per_block = rows_per_block(c.tokens);
+  r.vec = rows_on_16(c.x, c.x_stride, c.in);
+  H24_CUDA_TRY(launch_pdl(ce_rows_kernel, dim3(static_cast<unsigned>(cdiv(c.tokens, r.per_block))), dim3(kRowThreads),
+                          s, r));
+  count_launches(1);
+  const void *w;
+  int64_t w_pitch;
+  if ((rc = readable_head(c, sc, w_at, &w, &w_pitch)) != H24_OK) return rc;
+
+  GemmArgs g{};
+  if (!map16(&g.map[0], r.rows, c.tokens, c.in, pitch, kTileM / 2) || !map16(&g.map[1], w, c.vocab, c.in, w_pitch, bn / 2))
+    return fail(H24_ERR_CUDA, "linear_ce_forward: cuTensorMapEncodeTiled failed");
+  g.jobs = 1;
+  g.job[0].kind = kLoss;
+  g.job[0].n_total = static_cast<int>(c.vocab);
+  g.job[0].bn = bn;
+  g.job[0].k_total = static_cast<int>(c.in);
+  g.job[0].split = 1;
+  g.vocab = static_cast<int>(c.vocab);
+  g.kept = st.kept;
+  g.target = st.target;
+  g.lse = st.lse;
+  g.z_target = sc.at<float>(zt_at);
+  g.parts = sc.at<float2>(parts_at);
+  g.part_pitch = part_pitch;
+  g.err = T->err;
+  if ((rc = launch_gemm(g, bf16, cdiv(c.tokens, kTileM) * n_tiles, s)) != H24_OK) return rc;
+
+  CombineArgs cb{};
+  cb.st = st;
+  cb.parts = g.parts;
+  cb.part_pitch = part_pitch;
+  cb.n_parts = static_cast<int>(2 * n_tiles);
+  cb.z_target = g.z_target;
+  cb.token = r.token;
+  cb.row_loss = sc.at<float>(loss_at);
+  cb.loss = loss;
+  cb.reduction = c.reduction;
+  cb.ticket = r.ticket;
+  H24_CUDA_TRY(launch_pdl(ce_combine_kernel, dim3(static_cast<unsigned>(cdiv(c.tokens, kCombineRows))),
+                          dim3(kRowThreads), s, cb));
+  count_launches(1);
+  return H24_OK;
+}
+
+namespace {
+
+// How the backward pass cuts its work.
+struct BackPlan {
+  int64_t piece;   // vocabulary rows of a piece, a multiple of 256
+  int64_t pieces;
+  int split;       // slices of a dx tile's sum
+};
+BackPlan back_plan(const CeArgs &c, bool want_states, bool want_head) {
+  BackPlan p;
+  const int64_t rows = up(c.tokens, kTileM);
+  const int64_t most = kPieceBytes / (rows * 2) / kTileN * kTileN;
+  p.pieces = cdiv(c.vocab, most < kTileN ? kTileN : most);
+  p.piece = up(cdiv(c.vocab, p.pieces), kTileN);
+  p.pieces = cdiv(c.vocab, p.piece);
+  // A dx tile sums over a whole piece.  Slices of it where that is more than a
+  // third of what a pair of SMs does in a launch.
+  const int64_t kb = cdiv(p.piece, kTileK), m_tiles = rows / kTileM, n_tiles = cdiv(c.in, kTileN);
+  int64_t work = m_tiles * n_tiles * kb;
+  if (want_head) work += cdiv(p.piece, kTileM) * n_tiles * cdiv(c.tokens, kTileK);
+  if (p.pieces > 1) work += m_tiles * cdiv(p.piece, kTileN) * cdiv(c.in, kTileK);
+  int64_t split = want_states ? cdiv(3 * kb * kPairs, work) : 1;
+  if (split > kb) split = kb;
+  if (split > 32) split = 32;
+  p.split = static_cast<int>(split);
+  return p;
+}
+
+}  // namespace
+
+int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int64_t dloss_stride, const int32_t *state,
+                       void *dx, void *dw, cudaStream_t s) {
+  const bool bf16 = c.dtype == H24_DTYPE_BF16, each = c.reduction == H24_REDUCE_NONE;
+  const BackPlan plan = back_plan(c, dx != nullptr, dw != nullptr);
+  const int64_t pitch = up(c.in, 8), rows = up(c.tokens, kTileM), acc_pitch = up(c.in, 32);
+  Scratch sc(s);
+  const int64_t rows_at = sc.take((c.tokens + kTileK) * pitch * 2);
+  const int64_t scaled_at = each && dw ? sc.take((c.tokens + kTileK) * pitch * 2) : -1;
+  const int64_t scale_at = sc.take(8);
+  const int64_t w_at = head_readable(c) ? -1 : sc.take(c.vocab * pitch * 2);
+  const int64_t acc_at = dx ? sc.take(plan.split * c.tokens * acc_pitch * 4) : -1;
+  const int64_t d_bytes = rows * plan.piece * 2;
+  const int64_t d_at = sc.take(d_bytes), d2_at = plan.pieces > 1 ? sc.take(d_bytes) : d_at;
+  int rc = sc.allocate(T);
+  if (rc != H24_OK) return rc;
+  const State st = state_at(state, c.tokens);
+  const float prob_scale = bf16 ? 1.f : 32768.f;
+
+  BackRowsArgs r{};
+  r.x = c.x;
+  r.x_stride = c.x_stride;
+  r.tokens = static_cast<int>(c.tokens);
+  r.in = static_cast<int>(c.in);
+  r.st = st;
+  r.rows = sc.at<uint16_t>(rows_at);
+  r.scaled = scaled_at < 0 ? nullptr : sc.at<uint16_t>(scaled_at);
+  r.pitch = pitch;
+  r.dloss = dloss;
+  r.dloss_stride = dloss_stride;
+  r.mean = c.reduction == H24_REDUCE_MEAN;
+  r.vec = rows_on_16(c.x, c.x_stride, c.in);
+  r.inv_prob_scale = 1.f / prob_scale;
+  r.scale = sc.at<float>(scale_at);
+  r.per_block = rows_per_block(c.tokens);
+  H24_CUDA_TRY(launch_pdl(bf16 ? ce_back_rows_kernel<true> : ce_back_rows_kernel<false>,
+                          dim3(static_cast<unsigned>(cdiv(c.tokens, r.per_block))), dim3(kRowThreads), s, r));
+  count_launches(1);
+  const void *w;
+  int64_t w_pitch;
+  if ((rc = readable_head(c, sc, w_at, &w, &w_pitch)) != H24_OK) return rc;
+
+  GemmArgs base{};
+  base.vocab = static_cast<int>(c.vocab);
+  base.kept = st.kept;
+  base.target = st.target;
+  base.lse = st.lse;
+  base.scale = r.scale;
+  base.prob_scale = prob_scale;
+  base.wide_rows = dw && c.in % 16 == 0 && (reinterpret_cast<uintptr_t>(dw) & 31) == 0;
+  base.err = T->err;
+  const int64_t rows_alloc = c.tokens + kTileK;
+  const uint16_t *head_rows = r.scaled ? r.scaled : r.rows;
+  const int bn_in = static_cast<int>(c.in >= kTileN ? kTileN : up(c.in, 32));
+  for (int64_t i = 0; i <= plan.pieces; ++i) {
+    // The gradients of piece i - 1 beside the logits of piece i.
+    GemmArgs g = base;
+    bool ok = true;
+    int64_t tiles = 0;
+    int64_t longest = 0;
+    if (i > 0) {
+      const int64_t v0 = (i - 1) * plan.piece, v = c.vocab - v0 < plan.piece ? c.vocab - v0 : plan.piece;
+      uint16_t *d = sc.at<uint16_t>(i & 1 ? d_at : d2_at);
+      auto add_states = [&] {
+        if (!dx) return;
+        Job &j = g.job[g.jobs];
+        j.kind = kStates;
+        j.n_total = static_cast<int>(c.in);
+        j.bn = bn_in;
+        j.k_total = static_cast<int>(v);
+        j.split = plan.split;
+        j.v0 = static_cast<int>(v0);
+        j.add = i > 1;
+        j.out = sc.at<float>(acc_at);
+        j.pitch = acc_pitch;
+        j.plane = c.tokens * acc_pitch;
+        ok = ok && map16(&g.map[2 * g.jobs], d, rows, plan.piece, plan.piece, kTileM / 2) &&
+             map16(&g.map[2 * g.jobs + 1], w, c.vocab, c.in, w_pitch, kTileK);
+        tiles += rows / kTileM * cdiv(c.in, bn_in) * plan.split;
+        ++g.jobs;
+      };
+      auto add_head = [&] {
+        if (!dw) return;
+        Job &j = g.job[g.jobs];
+        j.kind = kHeadRows;
+        j.n_total = static_cast<int>(c.in);
+        j.bn = bn_in;
+        j.m_total = static_cast<int>(v);
+        j.split = 1;
+        j.v0 = static_cast<int>(v0);
+        j.out = dw;
+        j.pitch = c.in;
+        ok = ok && map16(&g.map[2 * g.jobs], d, rows, plan.piece, plan.piece, kTileK) &&
+             map16(&g.map[2 * g.jobs + 1], head_rows, rows_alloc, c.in, pitch, kTileK);
+        tiles += cdiv(v, kTileM) * cdiv(c.in, bn_in);
+        ++g.jobs;
+      };
+      longest = cdiv(c.tokens, kTileK);
+      if (longest > cdiv(v, kTileK) / plan.split) {
+        add_head();
+        add_states();
+      } else {
+        add_states();
+        add_head();
+      }
+    }
+    if (i < plan.pieces) {
+      const int64_t v0 = i * plan.piece, v = c.vocab - v0 < plan.piece ? c.vocab - v0 : plan.piece;
+      Job &j = g.job[g.jobs];
+      j.kind = kProb;
+      j.n_total = static_cast<int>(up(v, kTileK));
+      j.bn = plan.pieces > 1 ? kTileN : logits_bn(c.tokens, c.vocab);
+      j.k_total = static_cast<int>(c.in);
+      j.split = 1;
+      j.v0 = static_cast<int>(v0);
+      j.out = sc.at<uint16_t>(i & 1 ? d2_at : d_at);
+      j.pitch = plan.piece;
+      ok = ok && map16(&g.map[2 * g.jobs], r.rows, c.tokens, c.in, pitch, kTileM / 2) &&
+           map16(&g.map[2 * g.jobs + 1], w, c.vocab, c.in, w_pitch, j.bn / 2);
+      tiles += rows / kTileM * cdiv(j.n_total, j.bn);
+      ++g.jobs;
+    }
+    if (!ok) return fail(H24_ERR_CUDA, "linear_ce_backward: cuTensorMapEncodeTiled failed");
+    if ((rc = launch_gemm(g, bf16, tiles, s)) != H24_OK) return rc;
+  }
+  if (dx) {
+    StatesArgs o{};
+    o.st = st;
+    o.acc = sc.at<float>(acc_at);
+    o.pitch = acc_pitch;
+    o.plane = c.tokens * acc_pitch;
+    o.slices = plan.split;
+    o.tokens = c.tokens;
+    o.in = static_cast<int>(c.in);
+    o.scale = r.scale;
+    o.dloss = each ? dloss : nullptr;
+    o.dloss_stride = dloss_stride;
+    o.inv_prob_scale = r.inv_prob_scale;
+    o.out = static_cast<uint16_t *>(dx);
+    o.vec = rows_on_16(dx, c.in, c.in);
+    const int64_t blocks = cdiv(c.tokens * cdiv(c.in, 8), kRowThreads);
+    H24_CUDA_TRY(launch_pdl(bf16 ? ce_states_kernel<true> : ce_states_kernel<false>, dim3(wave_grid(blocks, 8)),
+                            dim3(kRowThreads), s, o));
+    count_launches(1);
+  }
+  return H24_OK;
+}
+
+}  // namespace h24

@@ -248,6 +248,19 @@ void int8_linear_plan(int64_t tokens, int64_t out, int64_t in, int out_dtype, in
 int launch_int8_linear(const Tables *t, const int8_t *q, const float *scale, int64_t tokens, int64_t q_stride,
                        const int8_t *w, const uint16_t *mu16, int64_t out, int64_t in, const float *bias,
                        int out_dtype, void *y, cudaStream_t s);
+// Cross entropy of a head's product (h24_ce.cu): x [tokens][in] and w
+// [vocab][in] of one 16-bit type, row strides in elements.
+struct CeArgs {
+  const void *x;
+  int64_t tokens, x_stride;
+  const void *w;
+  int64_t vocab, w_stride, in;
+  int dtype, reduction;
+};
+int launch_ce_forward(const Tables *t, const CeArgs &c, const int64_t *labels, int64_t ignore, float *loss,
+                      int32_t *state, cudaStream_t s);
+int launch_ce_backward(const Tables *t, const CeArgs &c, const float *dloss, int64_t dloss_stride, const int32_t *state,
+                       void *dx, void *dw, cudaStream_t s);
 int launch_sample(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t stride, const float *u,
                   const float *temperature, float temperature1, const int32_t *top_k, int32_t top_k1,
                   const float *top_p, float top_p1, const float *min_p, float min_p1, int64_t *tokens,

@@ -1,0 +1,142 @@
+"""Cross entropy of a head's product (loss.linear_cross_entropy) against its formula in 64 bits.
+
+Bounds.  h is half a step of the operands' type relative to the value (eps / 2: 2^-8 in bf16, 2^-11 in fp16), u = 2^-23 (a tensor core may truncate where it adds).
+  z       products are exact; sums run over in/16 groups of 16: |dz| <= ez = (in/16 + 16) u max sum|x w|
+  loss    log-sum-exp and logit carry ez each, exponentials and their sum 2^-20, the last roundings
+          of lse, logit and loss 4 * 2^-24 of the largest magnitude
+  d       |dd| <= h |d| + p (2 ez + 2^-20) + 2^-40 (fp16 holds d in steps of 2^-24 * 2^-15)
+  dx, dW  the sum of |dd| times the other factor's magnitude, (length/16 + 16) u of the sum of magnitudes
+          for the additions, h of the value at the end and half the type's smallest step;
+          with a factor for each token, dW's states are rounded once more: h of the sum of magnitudes,
+          and half a smallest step of the largest factor."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -23
+HALF = {t: torch.finfo(t).eps / 2 for t in (torch.bfloat16, torch.float16)}  # 8 bits: 2^-8; 11 bits: 2^-11
+TINY = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25}
+DTYPES = [torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(scope="module")
+def ce(lib):
+    from pollux_b200 import loss
+    return loss.linear_cross_entropy
+
+
+def _inputs(tokens, vocab, k, dtype, seed=0, masked=0.0, lean=0.6):
+    g = torch.Generator(device="cuda").manual_seed(seed * 7919 + tokens * 31 + vocab * 17 + k)
+    w = torch.randn(vocab, k, generator=g, device="cuda") * (2.2 / k ** 0.5)
+    target = torch.randint(0, vocab, (tokens,), generator=g, device="cuda")
+    on = (torch.rand(tokens, generator=g, device="cuda") < lean).float()
+    x = torch.randn(tokens, k, generator=g, device="cuda") + 1.6 * on[:, None] * w[target]
+    if masked:
+        target[torch.rand(tokens, generator=g, device="cuda") < masked] = -100
+    return x.to(dtype), w.to(dtype), target
+
+
+def _reference(x, w, target, factor):
+    """loss of each token and the gradients of sum(factor * loss), with their bounds.  (In steps of rows.)"""
+    dtype, half = x.dtype, HALF[x.dtype]
+    x, w = x.double(), w.double()
+    t, k = x.shape
+    v = w.shape[0]
+    keep = target != -100
+    loss = torch.zeros(t, dtype=torch.float64, device=x.device)
+    eloss = torch.zeros_like(loss)
+    dx, edx = torch.zeros_like(x), torch.zeros_like(x)
+    dw, edw, mag = torch.zeros_like(w), torch.zeros_like(w), torch.zeros_like(w)
+    top = factor[keep].abs().max() if bool(keep.any()) else factor.new_zeros(())
+    step = max(1, (1 << 25) // v)
+    for a in range(0, t, step):
+        r = torch.arange(a, min(t, a + step), device=x.device)
+        r = r[keep[r]]
+        if r.numel() == 0:
+            continue
+        z = x[r] @ w.t()
+        ez = (k / 16 + 16) * U * (x[r].abs() @ w.abs().t()).amax(1)
+        lse = torch.logsumexp(z, 1)
+        zt = z.gather(1, target[r][:, None])[:, 0]
+        loss[r] = lse - zt
+        eloss[r] = 2 * ez + 2.0 ** -20 + 4 * 2.0 ** -24 * torch.maximum(lse.abs(), zt.abs())
+        p = torch.exp(z - lse[:, None])
+        d = p.scatter_add(1, target[r][:, None], torch.full_like(zt, -1.0)[:, None])
+        ed = half * d.abs() + p * (2 * ez + 2.0 ** -20)[:, None] + 2.0 ** -40
+        f = factor[r][:, None]
+        dx[r] = f * (d @ w)
+        edx[r] = f.abs() * (ed @ w.abs() + (v / 16 + 16) * U * (d.abs() @ w.abs()))
+        dw += d.t() @ (f * x[r])
+        edw += ed.t() @ (f * x[r]).abs()
+        mag += d.abs().t() @ (f * x[r]).abs()
+        edw += d.abs().t() @ torch.full_like(x[r], float(top) * TINY[dtype])
+    edw += (t / 16 + 16) * U * mag
+    edx += half * (dx.abs() + edx) + TINY[dtype]
+    edw2 = edw + half * mag  # states rounded with their factors
+    edw2 += half * (dw.abs() + edw2) + TINY[dtype]
+    edw += half * (dw.abs() + edw) + TINY[dtype]
+    return loss, eloss, dx, edx, dw, edw, edw2
+
+
+def _close(got, want, bound, what):
+    bad = ~((got.double() - want).abs() <= bound)
+    assert not bool(bad.any()), (what, int(bad.sum()), float((got.double() - want).abs().max()), float(bound.max()))
+
+
+def _factor(target, reduction, scale=1.0):
+    keep = target != -100
+    n = int(keep.sum())
+    return torch.full(target.shape, scale / (n if reduction == "mean" and n else 1), dtype=torch.float64,
+                      device=target.device)
+
+
+def _check(ce, x, w, target, reduction, dloss=None):
+    xs, ws = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    value = ce(xs, ws, target, reduction=reduction)
+    assert value.dtype == torch.float32
+    dx, dw = torch.autograd.grad(value, (xs, ws), dloss)
+    assert dx.dtype == x.dtype and dw.dtype == w.dtype and dx.shape == x.shape and dw.shape == w.shape
+    factor = dloss.double() if reduction == "none" else _factor(target, reduction, 1.0 if dloss is None else float(dloss))
+    loss, eloss, rdx, edx, rdw, edw, edw2 = _reference(x, w, target, factor)
+    n = max(1, int((target != -100).sum()))
+    if reduction == "none":
+        _close(value, loss, eloss, "loss")
+    elif reduction == "sum":
+        _close(value, loss.sum(), eloss.sum() + 2.0 ** -23 * loss.sum().abs(), "loss")
+    else:
+        _close(value, loss.sum() / n, eloss.sum() / n + 2.0 ** -23 * loss.sum().abs() / n, "loss")
+    _close(dx, rdx, edx, "dx")
+    _close(dw, rdw, edw2 if reduction == "none" else edw, "dw")
+    assert bool((dx[target == -100] == 0).all())
+    with torch.no_grad():
+        assert torch.equal(ce(x, w, target, reduction=reduction), value.detach())
+
+
+SIZES = [(1, 1, 1), (1, 2, 8), (3, 200, 24), (9, 1009, 240), (33, 257, 1153), (130, 300, 65), (257, 1000, 96),
+         (64, 64, 64), (65, 511, 7), (520, 131, 1920), (300, 50257, 40), (1, 50688, 128), (256, 256, 256)]
+
+
+@pytest.mark.parametrize("tokens,vocab,k", SIZES)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_loss_and_gradients(ce, tokens, vocab, k, dtype):
+    x, w, target = _inputs(tokens, vocab, k, dtype)
+    _check(ce, x, w, target, "mean", torch.tensor(64.0, device="cuda"))
+
+
+@pytest.mark.parametrize("reduction", ["sum", "none", "mean"])
+@pytest.mark.parametrize("masked", [0.1, 0.6])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_masks_and_reductions(ce, reduction, masked, dtype):
+    for tokens, vocab, k in ((70, 515, 120), (700, 300, 33), (1500, 77, 200)):
+        x, w, target = _inputs(tokens, vocab, k, dtype, seed=3, masked=masked)
+        dloss = torch.rand(tokens, device="cuda") if reduction == "none" else None
+        _check(ce, x, w, target, reduction, dloss)
+
+
+@pytest.mark.parametrize("tokens,vocab,k", [(1000, 50257, 48), (4100, 30001, 40)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_several_pieces(ce, tokens, vocab, k, dtype):
+    x, w, target = _inputs(tokens, vocab, k, dtype, seed=5, masked=0.2)
+    _check(ce, x, w, target, "mean")
