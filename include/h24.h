@@ -240,9 +240,39 @@ int h24_sample_tokens(const void *logits, int dtype, int64_t rows, int64_t vocab
                       void *stream);
 
 /* ---- the training head path ------------------------------------------------
- * Loss of a model's head and its gradients, with the logits never in memory
- * (F.linear + F.cross_entropy of a [vocab, d] head in torch; no counterpart in
- * the reference's code). */
+ * From the residual stream to the loss and back: norms with their gradients,
+ * and the loss of a model's head and its gradients, with the logits never in
+ * memory (F.linear + F.cross_entropy of a [vocab, d] head in torch; no
+ * counterpart in the reference's code, which calls torch). */
+
+/* Residual addition and RMS (layer 0) or layer norm (1) of each row:
+ *   s = x + residual rounded to x's type, m = mean(s) or 0 (RMS),
+ *   i = 1/sqrt(mean((s - m)^2) + eps), y = (s - m) * i * gain + bias,
+ * sums and statistics fp32, y rounded once.  summed receives s (NULL without
+ * a residual).  x, residual, y and summed have element type `dtype`; row r of x
+ * starts at r * x_stride elements, of residual at r * residual_stride; y and
+ * summed are contiguous and overlap no input.  gain and bias (layer norm; may
+ * be NULL): cols elements of param_dtype, which is `dtype` or H24_DTYPE_F32.
+ * stats: 2 * rows fp32 for the backward pass.  A finite row whose squares pass
+ * fp32's range is normed as any other. */
+int h24_add_norm(const void *x, const void *residual, const void *gain, const void *bias,
+                 int param_dtype, int layer, int64_t rows, int64_t cols, int64_t x_stride,
+                 int64_t residual_stride, int dtype, float eps, void *y, void *summed, float *stats,
+                 void *stream);
+
+/* With n = (s - m) * i and v = dy * gain:
+ *   dx = i * (v - [layer] mean(v) - n * mean(v * n)) + dsummed
+ * (the gradient of x and of the residual alike), dgain = sum over rows of
+ * dy * n, dbias = sum over rows of dy; sums fp32 in a fixed order, each result
+ * rounded once.  summed: what h24_add_norm wrote, or its x where there was no
+ * residual.  dsummed (may be NULL): the gradient of summed.  dx (contiguous,
+ * `dtype`), dgain and dbias (param_dtype) may each be NULL.  The sums of blocks
+ * lie in the library's pool, freed on the stream. */
+int h24_add_norm_backward(const void *summed, const void *gain, int param_dtype, int layer,
+                          int64_t rows, int64_t cols, int64_t summed_stride, int dtype,
+                          const float *stats, const void *dy, int64_t dy_stride, const void *dsummed,
+                          int64_t dsummed_stride, void *dx, void *dgain, void *dbias, void *stream);
+
 #define H24_REDUCE_NONE 0
 #define H24_REDUCE_MEAN 1
 #define H24_REDUCE_SUM 2

@@ -58,6 +58,8 @@ SIGNATURES = {
     "h24_int8_linear": (_I, [_P, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _I, _P, _P]),
     "h24_int8_linear_plan": (_I, [_I64, _I64, _I64, _I, _P]),
     "h24_sample_tokens": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _F, _P, _I, _P, _F, _P, _F, _P, _P, _P]),
+    "h24_add_norm": (_I, [_P, _P, _P, _P, _I, _I, _I64, _I64, _I64, _I64, _I, _F, _P, _P, _P, _P]),
+    "h24_add_norm_backward": (_I, [_P, _P, _I, _I, _I64, _I64, _I64, _I, _P, _P, _I64, _P, _I64, _P, _P, _P, _P]),
     "h24_linear_ce_forward": (_I, [_P, _I64, _I64, _P, _I64, _I64, _I64, _I, _P, _I64, _I, _P, _P, _P]),
     "h24_linear_ce_backward": (_I, [_P, _I64, _I64, _P, _I64, _I64, _I64, _I, _I, _P, _I64, _P, _P, _P, _P]),
     "h24_quantize": (_I, [_P, _I64, _I, _P, _P]),

@@ -605,6 +605,54 @@ int h24_sample_tokens(const void *logits, int dtype, int64_t rows, int64_t vocab
                        top_p_all, min_p, min_p_all, tokens, logprobs, as_stream(stream));
 }
 
+static int check_norm(const char *what, const void *gain, int param_dtype, int64_t rows, int64_t cols, int dtype) {
+  const std::string name = what;
+  if (rows < 0 || cols < 1) return fail(H24_ERR_INVALID, name + ": negative size or empty rows");
+  if (!known_dtype(dtype)) return fail(H24_ERR_INVALID, name + ": unknown dtype");
+  if (param_dtype != dtype && param_dtype != H24_DTYPE_F32)
+    return fail(H24_ERR_INVALID, name + ": gain and bias must have x's dtype or fp32");
+  if (rows > INT32_MAX || cols > INT32_MAX) return fail(H24_ERR_INVALID, name + ": size above 2^31 - 1");
+  if (!gain) return fail(H24_ERR_INVALID, name + ": null pointer");
+  return H24_OK;
+}
+
+int h24_add_norm(const void *x, const void *residual, const void *gain, const void *bias, int param_dtype, int layer,
+                 int64_t rows, int64_t cols, int64_t x_stride, int64_t residual_stride, int dtype, float eps, void *y,
+                 void *summed, float *stats, void *stream) {
+  const int rc = check_norm("add_norm", gain, param_dtype, rows, cols, dtype);
+  if (rc != H24_OK) return rc;
+  if (!(eps >= 0.f)) return fail(H24_ERR_INVALID, "add_norm: eps must not be negative");
+  if (x_stride < 0 || (residual && residual_stride < 0)) return fail(H24_ERR_INVALID, "add_norm: negative stride");
+  if (bias && !layer) return fail(H24_ERR_INVALID, "add_norm: the RMS norm has no bias");
+  if ((residual != nullptr) != (summed != nullptr)) return fail(H24_ERR_INVALID, "add_norm: summed goes with a residual");
+  if (rows == 0) return H24_OK;
+  if (!x || !y || !stats) return fail(H24_ERR_INVALID, "add_norm: null pointer");
+  return launch_add_norm({gain, param_dtype, layer != 0, rows, cols, dtype}, x, x_stride, residual, residual_stride, bias,
+                         eps, y, summed, stats, as_stream(stream));
+}
+
+int h24_add_norm_backward(const void *summed, const void *gain, int param_dtype, int layer, int64_t rows, int64_t cols,
+                          int64_t summed_stride, int dtype, const float *stats, const void *dy, int64_t dy_stride,
+                          const void *dsummed, int64_t dsummed_stride, void *dx, void *dgain, void *dbias,
+                          void *stream) {
+  const int rc = check_norm("add_norm_backward", gain, param_dtype, rows, cols, dtype);
+  if (rc != H24_OK) return rc;
+  if (summed_stride < 0 || dy_stride < 0 || (dsummed && dsummed_stride < 0))
+    return fail(H24_ERR_INVALID, "add_norm_backward: negative stride");
+  if (dbias && !layer) return fail(H24_ERR_INVALID, "add_norm_backward: the RMS norm has no bias");
+  if (!dx && !dgain && !dbias) return H24_OK;
+  if (rows == 0) {
+    const size_t bytes = static_cast<size_t>(cols) * (param_dtype == H24_DTYPE_F32 ? 4 : 2);
+    if (dgain) H24_CUDA_TRY(cudaMemsetAsync(dgain, 0, bytes, as_stream(stream)));
+    if (dbias) H24_CUDA_TRY(cudaMemsetAsync(dbias, 0, bytes, as_stream(stream)));
+    return H24_OK;
+  }
+  if (!summed || !dy || !stats) return fail(H24_ERR_INVALID, "add_norm_backward: null pointer");
+  H24_TABLES_OR_FAIL(T);
+  return launch_add_norm_backward(T, {gain, param_dtype, layer != 0, rows, cols, dtype}, summed, summed_stride, stats, dy,
+                                  dy_stride, dsummed, dsummed_stride, dx, dgain, dbias, as_stream(stream));
+}
+
 static int check_ce(const char *what, const void *x, int64_t tokens, int64_t x_stride, const void *w, int64_t vocab,
                     int64_t w_stride, int64_t in_features, int dtype, int reduction) {
   const std::string name = what;

@@ -248,6 +248,19 @@ void int8_linear_plan(int64_t tokens, int64_t out, int64_t in, int out_dtype, in
 int launch_int8_linear(const Tables *t, const int8_t *q, const float *scale, int64_t tokens, int64_t q_stride,
                        const int8_t *w, const uint16_t *mu16, int64_t out, int64_t in, const float *bias,
                        int out_dtype, void *y, cudaStream_t s);
+// RMS and layer norm with their gradients (h24_norm.cu).  stats: 2 * rows.
+struct AddNormArgs {
+  const void *gain;
+  int param_dtype;  // of gain, bias and their gradients: `dtype` or fp32
+  bool layer;
+  int64_t rows, cols;
+  int dtype;
+};
+int launch_add_norm(const AddNormArgs &c, const void *x, int64_t x_stride, const void *residual, int64_t residual_stride,
+                    const void *bias, float eps, void *y, void *summed, float *stats, cudaStream_t s);
+int launch_add_norm_backward(const Tables *t, const AddNormArgs &c, const void *summed, int64_t summed_stride,
+                             const float *stats, const void *dy, int64_t dy_stride, const void *dsummed,
+                             int64_t dsummed_stride, void *dx, void *dgain, void *dbias, cudaStream_t s);
 // Cross entropy of a head's product (h24_ce.cu): x [tokens][in] and w
 // [vocab][in] of one 16-bit type, row strides in elements.
 struct CeArgs {

@@ -1,0 +1,644 @@
+// h24_norm.cu -- RMS and layer norm of a residual stream, and their gradients.
+//
+//   s_c = x_c + r_c, rounded to x's type (what is handed on)
+//   m   = mean(s) under the layer norm, 0 under the RMS norm
+//   i   = 1 / sqrt(mean((s - m)^2) + eps),  n_c = (s_c - m) i
+//   y_c = n_c w_c + b_c
+// and back, with v_c = dy_c w_c:
+//   ds_c = i (v_c - [layer] mean(v) - n_c mean(v n)) + dsummed_c
+//   dw_c = sum over rows of dy_c n_c,  db_c = sum over rows of dy_c
+// The norm is taken of the rounded sum, so that the gradients, which are taken
+// of it too (the unrounded one is nowhere in memory), are those of what was
+// computed.  Sums and statistics are fp32; deviations are squared, not squares
+// subtracted.  Where the squares of a row of finite numbers pass fp32's range,
+// its statistics are those of s * 2^-80, and i is stored negative to say so.
+//
+// A thread holds 16 columns of a row, so a row is read once; rows of up to 512
+// columns take a warp, of up to 16,384 a block.  In the backward pass a thread
+// keeps its columns for all of its rows and adds dw and db up in registers; the
+// blocks' sums meet in a second kernel, in a fixed order.
+#include "h24_internal.cuh"
+
+namespace h24 {
+namespace {
+
+constexpr float kSmall = 8.271806125530277e-25f;  // 2^-80
+constexpr int kHold = 16;                         // columns a thread holds
+constexpr int kWarpCols = 32 * kHold;
+constexpr int kBlockCols = 1024 * kHold;
+constexpr int kWarpRows = 8;                      // warps of a block where a warp has a row
+constexpr int kLongThreads = 512;
+constexpr int kSumCols = 32, kSumGroups = 32;     // of a block of the last sum
+
+template <int DT>
+struct Elem;
+template <>
+struct Elem<H24_DTYPE_F32> {
+  using T = float;
+  static constexpr int kVec = 4;
+  static __device__ __forceinline__ float up(float v) { return v; }
+  static __device__ __forceinline__ float down(float v) { return v; }
+};
+template <>
+struct Elem<H24_DTYPE_F16> {
+  using T = __half;
+  static constexpr int kVec = 8;
+  static __device__ __forceinline__ float up(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ __half down(float v) { return __float2half_rn(v); }
+};
+template <>
+struct Elem<H24_DTYPE_BF16> {
+  using T = __nv_bfloat16;
+  static constexpr int kVec = 8;
+  static __device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
+};
+
+struct NormArgs {
+  const void *x, *residual, *gain, *bias;
+  int64_t rows, cols, x_stride, residual_stride;
+  float eps;
+  bool gain_f32;
+  void *y, *summed;
+  float *inv, *mean;  // of each row; mean: layer norm only
+};
+
+struct BackArgs {
+  const void *s, *dy, *dsummed, *gain;
+  int64_t rows, cols, s_stride, dy_stride, dsummed_stride;
+  bool gain_f32;
+  const float *inv, *mean;
+  void *dx;
+  float *dgain, *dbias;  // sums of each block, `cols` apart; either may be null
+};
+
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
+
+// Thread t of a row's threads holds the columns of the vectors t, t + nt, ...
+template <int DT>
+struct Held {
+  static constexpr int VEC = Elem<DT>::kVec, NV = kHold / VEC;
+  uint4 raw[NV];
+
+  template <bool kAligned>
+  __device__ __forceinline__ void load(const void *base, int64_t offset, int t, int nt, int cols) {
+    using T = typename Elem<DT>::T;
+    const T *p = static_cast<const T *>(base) + offset;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int at = (t + i * nt) * VEC;
+      raw[i] = make_uint4(0, 0, 0, 0);
+      if (kAligned) {
+        if (at < cols) raw[i] = __ldg(reinterpret_cast<const uint4 *>(p + at));
+      } else {
+        T *e = reinterpret_cast<T *>(&raw[i]);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (at + j < cols) e[j] = p[at + j];
+      }
+    }
+  }
+  __device__ __forceinline__ float get(int k) const {
+    return Elem<DT>::up(reinterpret_cast<const typename Elem<DT>::T *>(&raw[k / VEC])[k % VEC]);
+  }
+};
+
+// The held columns of a row to memory.
+template <int DT, bool kAligned>
+__device__ __forceinline__ void store_held(void *base, int64_t offset, const float (&v)[kHold], int t, int nt, int cols) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  constexpr int VEC = E::kVec;
+  T *p = static_cast<T *>(base) + offset;
+#pragma unroll
+  for (int i = 0; i < kHold / VEC; ++i) {
+    const int at = (t + i * nt) * VEC;
+    alignas(16) T o[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) o[j] = E::down(v[i * VEC + j]);
+    if (kAligned) {
+      if (at < cols) *reinterpret_cast<uint4 *>(p + at) = *reinterpret_cast<const uint4 *>(o);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (at + j < cols) p[at + j] = o[j];
+    }
+  }
+}
+
+// The held columns of a parameter vector as fp32 (0 past the end).
+template <int DT, bool kAligned>
+__device__ __forceinline__ void load_param(const void *param, bool f32, float (&v)[kHold], int t, int nt, int cols) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  constexpr int VEC = E::kVec;
+  if (!f32 || DT == H24_DTYPE_F32) {
+    Held<DT> h;
+    h.template load<kAligned>(param, 0, t, nt, cols);
+#pragma unroll
+    for (int k = 0; k < kHold; ++k) v[k] = h.get(k);
+    return;
+  }
+  const float *p = static_cast<const float *>(param);
+#pragma unroll
+  for (int i = 0; i < kHold / VEC; ++i) {
+    const int at = (t + i * nt) * VEC;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[i * VEC + j] = at + j < cols ? __ldg(p + at + j) : 0.f;
+  }
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Sums over a row's threads: a warp, or the block (`red` is not used again
+// before a barrier that all of its threads pass).
+template <bool kWarp>
+__device__ __forceinline__ float row_sum(float v, float *red) {
+  v = warp_sum(v);
+  if (kWarp) return v;
+  const int warps = blockDim.x >> 5;
+  if (warps == 1) return v;
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.f;
+  for (int w = 0; w < warps; ++w) v += red[w];
+  return v;
+}
+
+// The finite rows among those whose statistics passed fp32's range, again and
+// by the element, from s * 2^-80.
+template <int DT, bool kLayer, bool kWarp>
+__device__ __noinline__ void wide_rows(const NormArgs &a, float (*red)[32]) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  const int t = kWarp ? threadIdx.x & 31 : threadIdx.x, nt = kWarp ? 32 : blockDim.x;
+  const int64_t first = kWarp ? blockIdx.x * static_cast<int64_t>(kWarpRows) + (threadIdx.x >> 5) : blockIdx.x;
+  const int64_t step = kWarp ? static_cast<int64_t>(gridDim.x) * kWarpRows : gridDim.x;
+  auto param = [&](const void *p, int64_t c) {
+    return a.gain_f32 ? static_cast<const float *>(p)[c] : E::up(static_cast<const T *>(p)[c]);
+  };
+  for (int64_t r = first; r < a.rows; r += step) {
+    const float marked = a.inv[r];
+    if (marked > 0.f && finite(marked)) continue;
+    const T *s = a.summed ? static_cast<const T *>(a.summed) + r * a.cols : static_cast<const T *>(a.x) + r * a.x_stride;
+    float sum = 0.f, bad = 0.f;
+    for (int64_t c = t; c < a.cols; c += nt) {
+      const float v = E::up(s[c]);
+      sum = fmaf(v, kSmall, sum);
+      bad += finite(v) ? 0.f : 1.f;
+    }
+    sum = row_sum<kWarp>(sum, red[0]);
+    bad = row_sum<kWarp>(bad, red[1]);
+    if (bad == 0.f) {  // (the same for all threads of the row)
+      const float mean = kLayer ? sum / static_cast<float>(a.cols) : 0.f;
+      float ss = 0.f;
+      for (int64_t c = t; c < a.cols; c += nt) {
+        const float v = fmaf(E::up(s[c]), kSmall, -mean);
+        ss = fmaf(v, v, ss);
+      }
+      ss = row_sum<kWarp>(ss, red[2]);
+      const double var = static_cast<double>(ss) / static_cast<double>(a.cols);
+      const float inv = static_cast<float>(1.0 / sqrt(var + static_cast<double>(a.eps) * kSmall * kSmall));
+      for (int64_t c = t; c < a.cols; c += nt) {
+        const float n = fmaf(E::up(s[c]), kSmall, -mean) * inv;
+        static_cast<T *>(a.y)[r * a.cols + c] = E::down(fmaf(n, param(a.gain, c), a.bias ? param(a.bias, c) : 0.f));
+      }
+      if (!kWarp) __syncthreads();  // all have read the mark
+      __syncwarp();
+      if (t == 0) {
+        a.inv[r] = -inv;
+        if (kLayer) a.mean[r] = mean;
+      }
+    }
+    if (!kWarp) __syncthreads();
+  }
+}
+
+template <int DT, bool kAligned, bool kLayer, bool kWarp, int kMax>
+__global__ void __launch_bounds__(kMax) norm_kernel(const __grid_constant__ NormArgs a) {
+  __shared__ float red[2][3][32];
+  pdl_enter();
+  const int t = kWarp ? threadIdx.x & 31 : threadIdx.x, nt = kWarp ? 32 : blockDim.x;
+  const int cols = static_cast<int>(a.cols);
+  const int64_t first = kWarp ? blockIdx.x * static_cast<int64_t>(kWarpRows) + (threadIdx.x >> 5) : blockIdx.x;
+  const int64_t step = kWarp ? static_cast<int64_t>(gridDim.x) * kWarpRows : gridDim.x;
+  const float n_cols = static_cast<float>(cols);
+  constexpr int VEC = Elem<DT>::kVec;
+  Held<DT> x, res;
+  auto ask = [&](int64_t r) {
+    if (r >= a.rows) return;
+    x.template load<kAligned>(a.x, r * a.x_stride, t, nt, cols);
+    if (a.residual) res.template load<kAligned>(a.residual, r * a.residual_stride, t, nt, cols);
+  };
+  ask(first);
+  int turn = 0;
+  for (int64_t r = first; r < a.rows; r += step, turn ^= 1) {
+    float v[kHold];
+#pragma unroll
+    for (int k = 0; k < kHold; ++k) v[k] = x.get(k);
+    if (a.residual) {
+#pragma unroll
+      for (int k = 0; k < kHold; ++k) v[k] = Elem<DT>::up(Elem<DT>::down(v[k] + res.get(k)));
+    }
+    ask(r + step);
+    if (a.summed) store_held<DT, kAligned>(a.summed, r * a.cols, v, t, nt, cols);
+    float mean = 0.f, ss = 0.f;
+    if (kLayer) {
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < kHold; ++k) sum += v[k];
+      mean = row_sum<kWarp>(sum, red[turn][0]) / n_cols;
+    }
+#pragma unroll
+    for (int k = 0; k < kHold; ++k) {
+      if (kLayer) {
+        const int at = (t + k / VEC * nt) * VEC + k % VEC;
+        v[k] = at < cols ? v[k] - mean : 0.f;
+      }
+      ss = fmaf(v[k], v[k], ss);
+    }
+    ss = row_sum<kWarp>(ss, red[turn][1]);
+    const float inv = 1.0f / sqrtf(ss / n_cols + a.eps);
+    float w[kHold];
+    load_param<DT, kAligned>(a.gain, a.gain_f32, w, t, nt, cols);
+#pragma unroll
+    for (int k = 0; k < kHold; ++k) v[k] = v[k] * inv * w[k];
+    if (kLayer && a.bias) {
+      load_param<DT, kAligned>(a.bias, a.gain_f32, w, t, nt, cols);
+#pragma unroll
+      for (int k = 0; k < kHold; ++k) v[k] += w[k];
+    }
+    store_held<DT, kAligned>(a.y, r * a.cols, v, t, nt, cols);
+    if (t == 0) {
+      a.inv[r] = inv;
+      if (kLayer) a.mean[r] = mean;
+    }
+  }
+  // Rows that passed fp32's range are looked for here, outside the loop.  (The
+  // squares of fp16 cannot.)
+  if (DT != H24_DTYPE_F16) {
+    bool marked = false;
+    __syncthreads();
+    for (int64_t r = first + t * step; r < a.rows; r += nt * step) marked |= !(a.inv[r] > 0.f && finite(a.inv[r]));
+    if (__syncthreads_or(marked)) wide_rows<DT, kLayer, kWarp>(a, red[0]);
+  }
+}
+
+// Rows too long for the registers of a block: three passes over the row.
+template <int DT, bool kLayer>
+__global__ void __launch_bounds__(kLongThreads) norm_long_kernel(const __grid_constant__ NormArgs a) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  __shared__ float red[3][32];
+  pdl_enter();
+  const int t = threadIdx.x;
+  const int64_t r = blockIdx.x;
+  const T *x = static_cast<const T *>(a.x) + r * a.x_stride;
+  const T *res = a.residual ? static_cast<const T *>(a.residual) + r * a.residual_stride : nullptr;
+  T *out = a.summed ? static_cast<T *>(a.summed) + r * a.cols : nullptr;
+  auto param = [&](const void *p, int64_t c) {
+    return a.gain_f32 ? static_cast<const float *>(p)[c] : E::up(static_cast<const T *>(p)[c]);
+  };
+  // (Each thread reads back only what it wrote itself.)
+  auto at = [&](int64_t c) { return E::up(res ? E::down(E::up(x[c]) + E::up(res[c])) : x[c]); };
+  float sum = 0.f, ss = 0.f, mean = 0.f;
+  if (kLayer) {
+    for (int64_t c = t; c < a.cols; c += kLongThreads) sum += at(c);
+    mean = row_sum<false>(sum, red[0]) / static_cast<float>(a.cols);
+  }
+  for (int64_t c = t; c < a.cols; c += kLongThreads) {
+    const float s = at(c);
+    if (out) out[c] = E::down(s);
+    ss = fmaf(s - mean, s - mean, ss);
+  }
+  ss = row_sum<false>(ss, red[1]);
+  const float inv = 1.0f / sqrtf(ss / static_cast<float>(a.cols) + a.eps);
+  for (int64_t c = t; c < a.cols; c += kLongThreads)
+    static_cast<T *>(a.y)[r * a.cols + c] =
+        E::down((at(c) - mean) * inv * param(a.gain, c) + (kLayer && a.bias ? param(a.bias, c) : 0.f));
+  if (t == 0) {
+    a.inv[r] = inv;
+    if (kLayer) a.mean[r] = mean;
+  }
+  if (DT != H24_DTYPE_F16) {
+    const bool marked = !(inv > 0.f && finite(inv));  // (the same for the whole block)
+    __syncthreads();
+    if (marked) wide_rows<DT, kLayer, false>(a, red);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Back
+// ---------------------------------------------------------------------------
+
+// A row's factors: n = fmaf(s, k, -shift) * inv.
+struct RowScale {
+  float inv, k, shift;
+};
+template <bool kLayer>
+__device__ __forceinline__ RowScale row_scale(const BackArgs &a, int64_t r) {
+  const float i = __ldg(a.inv + r);
+  return {fabsf(i), i < 0.f ? kSmall : 1.f, kLayer ? __ldg(a.mean + r) : 0.f};
+}
+
+template <int DT, bool kAligned, bool kLayer, bool kWarp, int kMax>
+__global__ void __launch_bounds__(kMax) norm_back_kernel(const __grid_constant__ BackArgs a) {
+  __shared__ float red[2][2][32];
+  __shared__ float held[kWarp ? kWarpRows * kWarpCols : 1];
+  pdl_enter();
+  const int t = kWarp ? threadIdx.x & 31 : threadIdx.x, nt = kWarp ? 32 : blockDim.x;
+  const int cols = static_cast<int>(a.cols);
+  const int64_t first = kWarp ? blockIdx.x * static_cast<int64_t>(kWarpRows) + (threadIdx.x >> 5) : blockIdx.x;
+  const int64_t step = kWarp ? static_cast<int64_t>(gridDim.x) * kWarpRows : gridDim.x;
+  const float one_over = 1.0f / static_cast<float>(cols);
+  constexpr int VEC = Elem<DT>::kVec;
+  float dw[kHold] = {}, db[kHold] = {};
+  int turn = 0;
+  for (int64_t r = first; r < a.rows; r += step, turn ^= 1) {
+    Held<DT> s, dy, ds;
+    s.template load<kAligned>(a.s, r * a.s_stride, t, nt, cols);
+    dy.template load<kAligned>(a.dy, r * a.dy_stride, t, nt, cols);
+    if (a.dsummed) ds.template load<kAligned>(a.dsummed, r * a.dsummed_stride, t, nt, cols);
+    const RowScale sc = row_scale<kLayer>(a, r);
+    float n[kHold], v[kHold];
+    load_param<DT, kAligned>(a.gain, a.gain_f32, v, t, nt, cols);
+    float c1 = 0.f, c2 = 0.f;
+#pragma unroll
+    for (int k = 0; k < kHold; ++k) {
+      const float g = dy.get(k);
+      n[k] = fmaf(s.get(k), sc.k, -sc.shift) * sc.inv;
+      dw[k] = fmaf(g, n[k], dw[k]);
+      if (kLayer) db[k] += g;
+      v[k] *= g;  // (0 past the row's end)
+      c1 = fmaf(v[k], n[k], c1);
+      if (kLayer) c2 += v[k];
+    }
+    if (a.dx) {
+      c1 = row_sum<kWarp>(c1, red[turn][0]) * one_over;
+      if (kLayer) c2 = row_sum<kWarp>(c2, red[turn][1]) * one_over;
+#pragma unroll
+      for (int k = 0; k < kHold; ++k) {
+        v[k] = (fmaf(-n[k], c1, v[k]) - c2) * sc.inv * sc.k;
+        if (a.dsummed) v[k] += ds.get(k);
+      }
+      store_held<DT, kAligned>(a.dx, r * a.cols, v, t, nt, cols);
+    }
+  }
+  // The sums of this block.
+  auto put = [&](float *out, float (&sum)[kHold]) {
+    if (!out) return;
+    float *o = out + static_cast<int64_t>(blockIdx.x) * a.cols;
+    if (!kWarp) {
+#pragma unroll
+      for (int k = 0; k < kHold; ++k) {
+        const int at = (t + k / VEC * nt) * VEC + k % VEC;
+        if (at < cols) o[at] = sum[k];
+      }
+      return;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kHold; ++k)
+      held[(threadIdx.x >> 5) * kWarpCols + (t + k / VEC * 32) * VEC + k % VEC] = sum[k];
+    __syncthreads();
+    for (int c = threadIdx.x; c < cols; c += 32 * kWarpRows) {
+      float total = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarpRows; ++w) total += held[w * kWarpCols + c];
+      o[c] = total;
+    }
+  };
+  put(a.dgain, dw);
+  if (kLayer) put(a.dbias, db);
+}
+
+// dx of rows too long for the registers of a block.
+template <int DT, bool kLayer>
+__global__ void __launch_bounds__(kLongThreads) norm_back_long_kernel(const __grid_constant__ BackArgs a) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  __shared__ float red[2][32];
+  pdl_enter();
+  const int64_t r = blockIdx.x;
+  const T *s = static_cast<const T *>(a.s) + r * a.s_stride, *dy = static_cast<const T *>(a.dy) + r * a.dy_stride;
+  const T *ds = a.dsummed ? static_cast<const T *>(a.dsummed) + r * a.dsummed_stride : nullptr;
+  const RowScale sc = row_scale<kLayer>(a, r);
+  const float one_over = 1.0f / static_cast<float>(a.cols);
+  auto gain = [&](int64_t c) {
+    return a.gain_f32 ? static_cast<const float *>(a.gain)[c] : E::up(static_cast<const T *>(a.gain)[c]);
+  };
+  float c1 = 0.f, c2 = 0.f;
+  for (int64_t c = threadIdx.x; c < a.cols; c += kLongThreads) {
+    const float v = E::up(dy[c]) * gain(c);
+    c1 = fmaf(v, fmaf(E::up(s[c]), sc.k, -sc.shift) * sc.inv, c1);
+    if (kLayer) c2 += v;
+  }
+  c1 = row_sum<false>(c1, red[0]) * one_over;
+  if (kLayer) c2 = row_sum<false>(c2, red[1]) * one_over;
+  for (int64_t c = threadIdx.x; c < a.cols; c += kLongThreads) {
+    const float n = fmaf(E::up(s[c]), sc.k, -sc.shift) * sc.inv;
+    float d = (fmaf(-n, c1, E::up(dy[c]) * gain(c)) - c2) * sc.inv * sc.k;
+    if (ds) d += E::up(ds[c]);
+    static_cast<T *>(a.dx)[r * a.cols + c] = E::down(d);
+  }
+}
+
+// Sums of dw and db of such rows: a thread a column, blockIdx.y a part of the rows.
+template <int DT, bool kLayer>
+__global__ void __launch_bounds__(256) norm_back_columns_kernel(const __grid_constant__ BackArgs a) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  pdl_enter();
+  const int64_t c = blockIdx.x * static_cast<int64_t>(256) + threadIdx.x;
+  if (c >= a.cols) return;
+  float dw = 0.f, db = 0.f;
+  for (int64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
+    const RowScale sc = row_scale<kLayer>(a, r);
+    const float g = E::up(static_cast<const T *>(a.dy)[r * a.dy_stride + c]);
+    dw = fmaf(g, fmaf(E::up(static_cast<const T *>(a.s)[r * a.s_stride + c]), sc.k, -sc.shift) * sc.inv, dw);
+    db += g;
+  }
+  if (a.dgain) a.dgain[blockIdx.y * a.cols + c] = dw;
+  if (a.dbias) a.dbias[blockIdx.y * a.cols + c] = db;
+}
+
+// The blocks' sums, in the blocks' order: blockIdx.y 0 is dw, 1 db.
+template <typename Out>
+__global__ void __launch_bounds__(kSumCols * kSumGroups) norm_sums_kernel(const float *dgain, const float *dbias,
+                                                                          int parts, int64_t cols, Out *gain_out,
+                                                                          Out *bias_out) {
+  __shared__ float red[kSumGroups][kSumCols + 1];
+  pdl_enter();
+  const float *in = blockIdx.y ? dbias : dgain;
+  Out *out = blockIdx.y ? bias_out : gain_out;
+  const int x = threadIdx.x % kSumCols, g = threadIdx.x / kSumCols;
+  const int64_t c = blockIdx.x * static_cast<int64_t>(kSumCols) + x;
+  float sum = 0.f;
+  if (in && c < cols) {
+#pragma unroll 4
+    for (int p = g; p < parts; p += kSumGroups) sum += __ldcs(in + p * cols + c);
+  }
+  red[g][x] = sum;
+  __syncthreads();
+  // Warp w adds up column w.
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float total = warp_sum(red[lane][w]);
+  const int64_t cw = blockIdx.x * static_cast<int64_t>(kSumCols) + w;
+  if (lane == 0 && in && cw < cols) {
+    if constexpr (sizeof(Out) == 4)
+      out[cw] = total;
+    else
+      out[cw] = Out(total);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+// Threads of a block.  (A kernel that is compiled for 1,024 has too few
+// registers for what a thread holds in the backward pass.)
+int row_threads(int64_t cols) {
+  return cols <= kWarpCols ? 32 * kWarpRows : static_cast<int>(((cols + kHold - 1) / kHold + 31) / 32 * 32);
+}
+template <auto kernel>
+int norm_grid(int64_t rows, int64_t cols, int threads) {
+  return wave_grid(cols <= kWarpCols ? (rows + kWarpRows - 1) / kWarpRows : rows, blocks_per_sm_once<kernel>(threads));
+}
+template <auto kernel>
+int launch_norm_rows(const NormArgs &a, int threads, cudaStream_t s) {
+  H24_CUDA_TRY(launch_pdl(kernel, dim3(norm_grid<kernel>(a.rows, a.cols, threads)), dim3(threads), s, a));
+  count_launches(1);
+  return H24_OK;
+}
+template <int DT, bool kAligned, bool kLayer>
+int launch_norm_width(const NormArgs &a, cudaStream_t s) {
+  const int threads = row_threads(a.cols);
+  if (a.cols <= kWarpCols) return launch_norm_rows<norm_kernel<DT, kAligned, kLayer, true, 32 * kWarpRows>>(a, threads, s);
+  if (threads <= 512) return launch_norm_rows<norm_kernel<DT, kAligned, kLayer, false, 512>>(a, threads, s);
+  return launch_norm_rows<norm_kernel<DT, kAligned, kLayer, false, 1024>>(a, threads, s);
+}
+
+template <int DT, bool kLayer>
+int launch_norm_typed(const NormArgs &a, cudaStream_t s) {
+  constexpr int kVec = Elem<DT>::kVec;
+  if (a.cols > kBlockCols) {
+    H24_CUDA_TRY(launch_pdl(norm_long_kernel<DT, kLayer>, dim3(static_cast<unsigned>(a.rows)), dim3(kLongThreads), s, a));
+    count_launches(1);
+    return H24_OK;
+  }
+  const bool aligned = a.cols % kVec == 0 && a.x_stride % kVec == 0 && a.residual_stride % kVec == 0 && aligned16(a.x) &&
+                       aligned16(a.residual) && aligned16(a.summed) && aligned16(a.y) && aligned16(a.gain) && aligned16(a.bias);
+  return aligned ? launch_norm_width<DT, true, kLayer>(a, s) : launch_norm_width<DT, false, kLayer>(a, s);
+}
+
+// The backward kernel of rows that a block holds: its grid (one wave; asked for
+// first, since each block has its sums), or its launch.
+template <auto kernel>
+int back_rows(const BackArgs &a, int grid, int threads, int *ask, cudaStream_t s) {
+  if (ask) {
+    *ask = norm_grid<kernel>(a.rows, a.cols, threads);
+    return H24_OK;
+  }
+  H24_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(threads), s, a));
+  count_launches(1);
+  return H24_OK;
+}
+template <int DT, bool kAligned, bool kLayer>
+int back_width(const BackArgs &a, int grid, int *ask, cudaStream_t s) {
+  const int threads = row_threads(a.cols);
+  if (a.cols <= kWarpCols)
+    return back_rows<norm_back_kernel<DT, kAligned, kLayer, true, 32 * kWarpRows>>(a, grid, threads, ask, s);
+  if (threads <= 512) return back_rows<norm_back_kernel<DT, kAligned, kLayer, false, 512>>(a, grid, threads, ask, s);
+  return back_rows<norm_back_kernel<DT, kAligned, kLayer, false, 1024>>(a, grid, threads, ask, s);
+}
+
+template <int DT, bool kLayer>
+int launch_back_typed(const Tables *T, BackArgs a, void *dgain, void *dbias, cudaStream_t s) {
+  constexpr int kVec = Elem<DT>::kVec;
+  const bool sums = dgain || dbias;
+  const bool is_long = a.cols > kBlockCols;
+  const bool aligned = a.cols % kVec == 0 && a.s_stride % kVec == 0 && a.dy_stride % kVec == 0 &&
+                       a.dsummed_stride % kVec == 0 && aligned16(a.s) && aligned16(a.dy) && aligned16(a.dsummed) &&
+                       aligned16(a.dx) && aligned16(a.gain);
+  const int64_t col_blocks = (a.cols + 255) / 256;
+  auto rows = [&](int grid, int *ask) {
+    return aligned ? back_width<DT, true, kLayer>(a, grid, ask, s) : back_width<DT, false, kLayer>(a, grid, ask, s);
+  };
+  int grid = static_cast<int>(wave_grid(a.rows, 8) / col_blocks + 1);
+  if (!is_long) rows(0, &grid);
+  float *parts = nullptr;
+  if (sums) {
+    const size_t one = static_cast<size_t>(grid) * static_cast<size_t>(a.cols);
+    H24_CUDA_TRY(cudaMallocFromPoolAsync(reinterpret_cast<void **>(&parts), one * 8, T->pool, s));
+    a.dgain = dgain ? parts : nullptr;
+    a.dbias = dbias ? parts + one : nullptr;
+  }
+  auto run = [&]() -> int {
+    if (is_long) {
+      if (a.dx) {
+        H24_CUDA_TRY(launch_pdl(norm_back_long_kernel<DT, kLayer>, dim3(static_cast<unsigned>(a.rows)),
+                                dim3(kLongThreads), s, a));
+        count_launches(1);
+      }
+      if (sums) {
+        H24_CUDA_TRY(launch_pdl(norm_back_columns_kernel<DT, kLayer>,
+                                dim3(static_cast<unsigned>(col_blocks), static_cast<unsigned>(grid)), dim3(256), s, a));
+        count_launches(1);
+      }
+    } else {
+      const int rc = rows(grid, nullptr);
+      if (rc != H24_OK) return rc;
+    }
+    if (sums) {
+      const dim3 blocks(static_cast<unsigned>((a.cols + kSumCols - 1) / kSumCols), dbias ? 2 : 1);
+      const dim3 threads(kSumCols * kSumGroups);
+      if (a.gain_f32 || DT == H24_DTYPE_F32)
+        H24_CUDA_TRY(launch_pdl(norm_sums_kernel<float>, blocks, threads, s, static_cast<const float *>(a.dgain),
+                                static_cast<const float *>(a.dbias), grid, a.cols, static_cast<float *>(dgain),
+                                static_cast<float *>(dbias)));
+      else
+        H24_CUDA_TRY(launch_pdl(norm_sums_kernel<typename Elem<DT>::T>, blocks, threads, s,
+                                static_cast<const float *>(a.dgain), static_cast<const float *>(a.dbias), grid, a.cols,
+                                static_cast<typename Elem<DT>::T *>(dgain), static_cast<typename Elem<DT>::T *>(dbias)));
+      count_launches(1);
+    }
+    return H24_OK;
+  };
+  int rc = run();
+  if (parts) {
+    const cudaError_t e = cudaFreeAsync(parts, s);
+    if (rc == H24_OK && e != cudaSuccess) rc = cuda_fail(e, "cudaFreeAsync");
+  }
+  return rc;
+}
+
+}  // namespace
+
+int launch_add_norm(const AddNormArgs &c, const void *x, int64_t x_stride, const void *residual, int64_t residual_stride,
+                    const void *bias, float eps, void *y, void *summed, float *stats, cudaStream_t s) {
+  const NormArgs a{x, residual, c.gain, bias, c.rows, c.cols, x_stride, residual ? residual_stride : 0, eps,
+                   c.param_dtype == H24_DTYPE_F32, y, summed, stats, stats + c.rows};
+  switch (c.dtype) {
+    case H24_DTYPE_F32: return c.layer ? launch_norm_typed<H24_DTYPE_F32, true>(a, s) : launch_norm_typed<H24_DTYPE_F32, false>(a, s);
+    case H24_DTYPE_F16: return c.layer ? launch_norm_typed<H24_DTYPE_F16, true>(a, s) : launch_norm_typed<H24_DTYPE_F16, false>(a, s);
+    default: return c.layer ? launch_norm_typed<H24_DTYPE_BF16, true>(a, s) : launch_norm_typed<H24_DTYPE_BF16, false>(a, s);
+  }
+}
+
+int launch_add_norm_backward(const Tables *T, const AddNormArgs &c, const void *summed, int64_t summed_stride,
+                             const float *stats, const void *dy, int64_t dy_stride, const void *dsummed,
+                             int64_t dsummed_stride, void *dx, void *dgain, void *dbias, cudaStream_t s) {
+  const BackArgs a{summed, dy, dsummed, c.gain, c.rows, c.cols, summed_stride, dy_stride, dsummed ? dsummed_stride : 0,
+                   c.param_dtype == H24_DTYPE_F32, stats, stats + c.rows, dx, nullptr, nullptr};
+  switch (c.dtype) {
+    case H24_DTYPE_F32: return c.layer ? launch_back_typed<H24_DTYPE_F32, true>(T, a, dgain, dbias, s) : launch_back_typed<H24_DTYPE_F32, false>(T, a, dgain, dbias, s);
+    case H24_DTYPE_F16: return c.layer ? launch_back_typed<H24_DTYPE_F16, true>(T, a, dgain, dbias, s) : launch_back_typed<H24_DTYPE_F16, false>(T, a, dgain, dbias, s);
+    default: return c.layer ? launch_back_typed<H24_DTYPE_BF16, true>(T, a, dgain, dbias, s) : launch_back_typed<H24_DTYPE_BF16, false>(T, a, dgain, dbias, s);
+  }
+}
+
+}  // namespace h24
