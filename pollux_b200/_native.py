@@ -136,7 +136,8 @@ def load() -> ctypes.CDLL:
 
 _torch_calls = None
 _TORCH_ENTRIES = ("h24_add_rms_norm_int8", "h24_rows_int8_quantize", "h24_rows_int8_dequant", "h24_int8_linear",
-                  "h24_sample_tokens")
+                  "h24_sample_tokens", "h24_add_norm", "h24_add_norm_backward", "h24_linear_ce_forward",
+                  "h24_linear_ce_backward", "h24_last_error")
 
 
 def torch_module_path() -> str:
@@ -154,8 +155,8 @@ class _GeneralPath:
 
 
 def torch_calls():
-    """The module _h24_torch, which makes the decoding-step calls of libh24
-    straight from torch tensors.  Without it they take the general path, which
+    """The module _h24_torch, which makes the calls of a decoding step and of a
+    training step's norms and loss straight from torch tensors.  Without it they take the general path, which
     makes the same calls of libh24 at some ten microseconds more."""
     global _torch_calls
     if _torch_calls is None:

@@ -1,23 +1,32 @@
 // h24_torch.cpp -- the short way from a torch tensor to libh24 for the calls of
-// a decoding step, where a few microseconds of Python for each call would cost
-// more than the kernel.  Each function takes the Python call's arguments; are
+// a decoding step and of a training step's norms and loss, where the
+// microseconds of Python for each call would cost more than the kernel.  Each function takes the Python call's arguments; are
 // they contiguous CUDA tensors of the current device in types that the kernel
 // reads, it allocates the outputs, launches on the current stream and returns
 // them.  For anything else, errors included, it returns None and the caller
-// (int8.py, sampling.py) takes the general path, which checks, copies and
-// raises.
+// (int8.py, sampling.py, norm.py, loss.py) takes the general path, which checks,
+// copies and raises.  The nodes of the autograd graph that norms and loss leave
+// are here too.
 //
 // The module is not linked against libh24: bind() receives the entry points'
 // addresses from the library that Python has loaded.
 #include <Python.h>
 
+#include <ATen/autocast_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
 #include <limits>
+#include <memory>
+#include <mutex>
 
 #include "../../include/h24.h"
 
@@ -29,17 +38,26 @@ struct {
   decltype(&h24_rows_int8_dequant) dequant;
   decltype(&h24_int8_linear) linear;
   decltype(&h24_sample_tokens) sample;
+  decltype(&h24_add_norm) add_norm;
+  decltype(&h24_add_norm_backward) add_norm_backward;
+  decltype(&h24_linear_ce_forward) ce_forward;
+  decltype(&h24_linear_ce_backward) ce_backward;
+  decltype(&h24_last_error) last_error;
 } g_h24;
 
-// The tensor behind `o` if it is a contiguous CUDA tensor of device `dev` of
-// which no gradient is asked.
-const at::Tensor *plain(PyObject *o, int dev) {
+// The tensor (or parameter, but no other subclass) behind `o` if it is a
+// contiguous CUDA tensor of device `dev`.
+const at::Tensor *dense(PyObject *o, int dev) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor &t = THPVariable_Unpack(o);
-  return t.is_cuda() && t.get_device() == dev && t.layout() == at::kStrided && t.is_contiguous() &&
-                 !(t.requires_grad() && c10::GradMode::is_enabled())
-             ? &t
-             : nullptr;
+  return t.is_cuda() && t.get_device() == dev && t.layout() == at::kStrided && t.is_contiguous() ? &t : nullptr;
+}
+bool tracked(const at::Tensor *t) { return t && t->requires_grad() && c10::GradMode::is_enabled(); }
+
+// The same, and no gradient is asked of it.
+const at::Tensor *plain(PyObject *o, int dev) {
+  const at::Tensor *t = dense(o, dev);
+  return tracked(t) ? nullptr : t;
 }
 
 // Whether `t` has a value for each row of `x`, in their order: x's leading
@@ -258,19 +276,212 @@ PyObject *sample_tokens(PyObject *, PyObject *const *a, Py_ssize_t n) {
   });
 }
 
+// ---------------------------------------------------------------------------
+// Norms and loss, with their nodes in the autograd graph
+// ---------------------------------------------------------------------------
+using torch::autograd::SavedVariable;
+using torch::autograd::variable_list;
+
+void check(int rc, const char *what) {
+  if (rc != H24_OK) throw std::runtime_error(std::string(what) + ": " + g_h24.last_error());
+}
+
+// Gradients that are themselves tracked (create_graph) say so when they are
+// differentiated, as torch's once_differentiable does.
+variable_list once(variable_list grads, const char *what) {
+  if (!c10::GradMode::is_enabled()) return grads;
+  for (at::Tensor &g : grads)
+    if (g.defined()) g = g.detach().requires_grad_(true);
+  const auto error = std::make_shared<torch::autograd::DelayedError>(
+      std::string("trying to differentiate twice: ") + what + " has one derivative", static_cast<int64_t>(grads.size()));
+  return (*error)(std::move(grads));
+}
+
+struct NormNode : torch::autograd::Node {
+  SavedVariable s, weight;
+  at::Tensor stats;
+  bool layer = false, saved_output = false;
+
+  std::string name() const override { return layer ? "AddLayerNormBackward" : "AddRmsNormBackward"; }
+  void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    s.reset_data();
+    weight.reset_data();
+    stats.reset();
+  }
+
+  // (dy, dsummed) -> (x, residual, weight, bias)
+  variable_list apply(variable_list &&grads) override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    const at::Tensor sum = s.unpack(saved_output ? shared_from_this() : nullptr), w = weight.unpack();
+    const int dev = static_cast<int>(sum.get_device());
+    const c10::cuda::OptionalCUDAGuard guard(sum.device());
+    const bool need_x = should_compute_output(0), need_r = should_compute_output(1);
+    const bool need_w = should_compute_output(2), need_b = should_compute_output(3);
+    variable_list out(4);
+    if (!grads[0].defined()) {  // nothing reached y
+      if (need_x) out[0] = grads[1];
+      if (need_r) out[1] = grads[1];
+      if (need_w) out[2] = at::zeros_like(w);
+      if (need_b) out[3] = at::zeros_like(w);
+      return once(std::move(out), "the norm");
+    }
+    const at::Tensor dy = grads[0].contiguous();
+    const at::Tensor dsum = grads.size() > 1 && grads[1].defined() ? grads[1].contiguous() : at::Tensor();
+    const int64_t cols = sum.size(-1), rows = sum.numel() / cols;
+    const at::Tensor dx = need_x || need_r ? fresh(sum.sizes(), sum.scalar_type(), dev) : at::Tensor();
+    const at::Tensor dw = need_w ? fresh(w.sizes(), w.scalar_type(), dev) : at::Tensor();
+    const at::Tensor db = need_b ? fresh(w.sizes(), w.scalar_type(), dev) : at::Tensor();
+    check(g_h24.add_norm_backward(sum.const_data_ptr(), w.const_data_ptr(), code_of(w.scalar_type()), layer, rows, cols,
+                                  cols, code_of(sum.scalar_type()), static_cast<const float *>(stats.const_data_ptr()),
+                                  dy.const_data_ptr(), cols, dsum.defined() ? dsum.const_data_ptr() : nullptr, cols,
+                                  dx.defined() ? dx.data_ptr() : nullptr, dw.defined() ? dw.data_ptr() : nullptr,
+                                  db.defined() ? db.data_ptr() : nullptr, stream_of(dev)),
+          "h24_add_norm_backward");
+    if (need_x) out[0] = dx;
+    if (need_r) out[1] = dx;
+    out[2] = dw;
+    out[3] = db;
+    return once(std::move(out), "the norm");
+  }
+};
+
+// (x, weight, bias or None, residual or None, eps, layer) -> (y, summed or None)
+PyObject *add_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject * {
+    const int dev = c10::cuda::current_device();
+    const at::Tensor *x = n == 6 ? dense(a[0], dev) : nullptr;
+    const at::Tensor *w = x ? dense(a[1], dev) : nullptr;
+    const bool has_bias = w && a[2] != Py_None, has_residual = w && a[3] != Py_None;
+    const at::Tensor *b = has_bias ? dense(a[2], dev) : nullptr, *r = has_residual ? dense(a[3], dev) : nullptr;
+    double eps;
+    if (!w || (has_bias && !b) || (has_residual && !r) || x->dim() < 1 || x->numel() == 0 || !number(a[4], &eps) ||
+        !(eps >= 0))
+      Py_RETURN_NONE;
+    const int64_t cols = x->size(-1), rows = x->numel() / cols;
+    const int code = code_of(x->scalar_type());
+    const auto param = [&](const at::Tensor *p) {
+      return p->dim() == 1 && p->numel() == cols && p->scalar_type() == w->scalar_type();
+    };
+    if (code < 0 || !param(w) || (w->scalar_type() != x->scalar_type() && w->scalar_type() != at::kFloat) ||
+        (b && !param(b)) || (r && (r->scalar_type() != x->scalar_type() || !r->sizes().equals(x->sizes()))))
+      Py_RETURN_NONE;
+    const bool layer = a[5] == Py_True;
+    const at::Tensor y = fresh(x->sizes(), x->scalar_type(), dev);
+    const at::Tensor sum = r ? fresh(x->sizes(), x->scalar_type(), dev) : at::Tensor();
+    const at::Tensor stats = fresh({2 * rows}, at::kFloat, dev);
+    if (g_h24.add_norm(x->const_data_ptr(), r ? r->const_data_ptr() : nullptr, w->const_data_ptr(),
+                       b ? b->const_data_ptr() : nullptr, code_of(w->scalar_type()), layer, rows, cols, cols, cols, code,
+                       static_cast<float>(eps), y.data_ptr(), r ? sum.data_ptr() : nullptr,
+                       static_cast<float *>(stats.data_ptr()), stream_of(dev)) != H24_OK)
+      Py_RETURN_NONE;
+    if (tracked(x) || tracked(w) || tracked(b) || tracked(r)) {
+      const at::Tensor none;
+      const std::shared_ptr<NormNode> node(new NormNode(), torch::autograd::deleteNode);
+      node->set_next_edges(torch::autograd::collect_next_edges(*x, r ? *r : none, *w, b ? *b : none));
+      torch::autograd::set_history(y, node);
+      if (r) torch::autograd::set_history(sum, node);
+      node->s = SavedVariable(r ? sum : *x, r != nullptr);
+      node->weight = SavedVariable(*w, false);
+      node->stats = stats;
+      node->layer = layer;
+      node->saved_output = r != nullptr;
+    }
+    return wrap({&y, r ? &sum : nullptr});
+  });
+}
+
+struct LossNode : torch::autograd::Node {
+  SavedVariable x, weight;
+  at::Tensor state;
+  int reduction = 0;
+
+  std::string name() const override { return "LinearCrossEntropyBackward"; }
+  void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    x.reset_data();
+    weight.reset_data();
+    state.reset();
+  }
+
+  variable_list apply(variable_list &&grads) override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    const at::Tensor rows = x.unpack(), w = weight.unpack();
+    variable_list out(2);
+    if (!grads[0].defined()) return out;
+    const int dev = static_cast<int>(rows.get_device());
+    const c10::cuda::OptionalCUDAGuard guard(rows.device());
+    const at::Tensor g = grads[0].dim() <= 1 ? grads[0] : grads[0].contiguous();
+    const int64_t step = g.dim() == 1 ? g.stride(0) : g.dim() ? 1 : 0, in = w.size(1);
+    if (should_compute_output(0)) out[0] = fresh(rows.sizes(), rows.scalar_type(), dev);
+    if (should_compute_output(1)) out[1] = fresh(w.sizes(), w.scalar_type(), dev);
+    check(g_h24.ce_backward(rows.const_data_ptr(), rows.numel() / in, in, w.const_data_ptr(), w.size(0), in, in,
+                            code_of(w.scalar_type()), reduction, static_cast<const float *>(g.const_data_ptr()), step,
+                            static_cast<const int32_t *>(state.const_data_ptr()),
+                            out[0].defined() ? out[0].data_ptr() : nullptr,
+                            out[1].defined() ? out[1].data_ptr() : nullptr, stream_of(dev)),
+          "h24_linear_ce_backward");
+    return once(std::move(out), "linear_cross_entropy");
+  }
+};
+
+// (x, weight, target, ignore_index, reduction) -> loss
+PyObject *linear_ce(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject * {
+    const int dev = c10::cuda::current_device();
+    const at::Tensor *x = n == 5 ? dense(a[0], dev) : nullptr;
+    const at::Tensor *w = x ? dense(a[1], dev) : nullptr;
+    const at::Tensor *t = w ? dense(a[2], dev) : nullptr;
+    if (!t || x->dim() < 1 || x->numel() == 0 || w->dim() != 2 || w->numel() == 0 || x->size(-1) != w->size(1) ||
+        (x->scalar_type() != at::kHalf && x->scalar_type() != at::kBFloat16) || w->scalar_type() != x->scalar_type() ||
+        t->scalar_type() != at::kLong || !holds_rows(*t, *x) || at::autocast::is_autocast_enabled(at::kCUDA) ||
+        !PyLong_CheckExact(a[3]) || !PyLong_CheckExact(a[4]))
+      Py_RETURN_NONE;
+    int overflow = 0;
+    const long long ignore = PyLong_AsLongLongAndOverflow(a[3], &overflow);
+    const long reduction = PyLong_AsLong(a[4]);
+    if (overflow) Py_RETURN_NONE;
+    const int64_t in = w->size(1), tokens = x->numel() / in;
+    const at::Tensor loss = reduction == H24_REDUCE_NONE ? fresh(x->sizes().slice(0, x->dim() - 1), at::kFloat, dev)
+                                                         : fresh({}, at::kFloat, dev);
+    const at::Tensor state = fresh({3 * tokens + 1}, at::kInt, dev);
+    if (g_h24.ce_forward(x->const_data_ptr(), tokens, in, w->const_data_ptr(), w->size(0), in, in,
+                         code_of(x->scalar_type()), static_cast<const int64_t *>(t->const_data_ptr()), ignore,
+                         static_cast<int>(reduction), static_cast<float *>(loss.data_ptr()),
+                         static_cast<int32_t *>(state.data_ptr()), stream_of(dev)) != H24_OK)
+      Py_RETURN_NONE;
+    if (tracked(x) || tracked(w)) {
+      const std::shared_ptr<LossNode> node(new LossNode(), torch::autograd::deleteNode);
+      node->set_next_edges(torch::autograd::collect_next_edges(*x, *w));
+      torch::autograd::set_history(loss, node);
+      node->x = SavedVariable(*x, false);
+      node->weight = SavedVariable(*w, false);
+      node->state = state;
+      node->reduction = static_cast<int>(reduction);
+    }
+    return THPVariable_Wrap(loss);
+  });
+}
+
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
-  void *p[5];
-  if (n != 5) {
-    PyErr_SetString(PyExc_TypeError, "bind takes the addresses of five entry points");
+  constexpr int kEntries = 10;
+  void *p[kEntries];
+  if (n != kEntries) {
+    PyErr_SetString(PyExc_TypeError, "bind takes the addresses of ten entry points");
     return nullptr;
   }
-  for (int i = 0; i < 5; ++i) p[i] = PyLong_AsVoidPtr(a[i]);
+  for (int i = 0; i < kEntries; ++i) p[i] = PyLong_AsVoidPtr(a[i]);
   if (PyErr_Occurred()) return nullptr;
   g_h24.norm = reinterpret_cast<decltype(g_h24.norm)>(p[0]);
   g_h24.quantize = reinterpret_cast<decltype(g_h24.quantize)>(p[1]);
   g_h24.dequant = reinterpret_cast<decltype(g_h24.dequant)>(p[2]);
   g_h24.linear = reinterpret_cast<decltype(g_h24.linear)>(p[3]);
   g_h24.sample = reinterpret_cast<decltype(g_h24.sample)>(p[4]);
+  g_h24.add_norm = reinterpret_cast<decltype(g_h24.add_norm)>(p[5]);
+  g_h24.add_norm_backward = reinterpret_cast<decltype(g_h24.add_norm_backward)>(p[6]);
+  g_h24.ce_forward = reinterpret_cast<decltype(g_h24.ce_forward)>(p[7]);
+  g_h24.ce_backward = reinterpret_cast<decltype(g_h24.ce_backward)>(p[8]);
+  g_h24.last_error = reinterpret_cast<decltype(g_h24.last_error)>(p[9]);
   Py_RETURN_NONE;
 }
 
@@ -279,6 +490,7 @@ PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
 PyMethodDef g_methods[] = {H24_METHOD(bind),        H24_METHOD(add_rms_norm_int8),
                            H24_METHOD(quantize_rows_int8), H24_METHOD(dequantize_rows_int8),
                            H24_METHOD(int8_linear), H24_METHOD(sample_tokens),
+                           H24_METHOD(add_norm), H24_METHOD(linear_ce),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_h24_torch", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -75,6 +75,9 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     red = _REDUCTIONS.get(reduction)
     if red is None:
         raise ValueError(f"reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
+    got = (N._torch_calls or N.torch_calls()).linear_ce(x, weight, target, ignore_index, red)
+    if got is not None:
+        return got
     if x.dim() < 1 or weight.dim() != 2:
         raise ValueError(f"x must have at least one dimension and weight two, got {tuple(x.shape)} and "
                          f"{tuple(weight.shape)}")

@@ -112,7 +112,8 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor |
     ``summed = x + residual``, the next layer's residual (None without
     ``residual``), and its norm; sums and statistics are fp32.  Both outputs have
     gradients, which go to x, residual and weight."""
-    return _add_norm(x, weight, None, residual, eps, False)
+    got = (N._torch_calls or N.torch_calls()).add_norm(x, weight, None, residual, eps, False)
+    return _add_norm(x, weight, None, residual, eps, False) if got is None else got
 
 
 def add_layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
@@ -120,4 +121,5 @@ def add_layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
                    eps: float = 1e-5) -> tuple[torch.Tensor, torch.Tensor | None]:
     """Layer norm of ``x + residual`` over the last dimension, times ``weight``
     plus ``bias``; otherwise as ``add_rms_norm``."""
-    return _add_norm(x, weight, bias, residual, eps, True)
+    got = (N._torch_calls or N.torch_calls()).add_norm(x, weight, bias, residual, eps, True)
+    return _add_norm(x, weight, bias, residual, eps, True) if got is None else got
