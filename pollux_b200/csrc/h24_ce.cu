@@ -12,7 +12,7 @@
 //
 // All four products run in one kernel, ce_gemm_kernel: persistent pairs of CTAs
 // on 256 x 256 tiles (tcgen05.mma.cta_group::2, operands by TMA into a ring of
-// six stages, two accumulators in TMEM, eight epilogue warps a CTA), each
+// three stages of 128 k, two accumulators in TMEM, eight epilogue warps a CTA), each
 // operand K-major or MN-major as it lies in memory, so nothing is transposed.
 //   forward: the logits' tiles end in a running maximum and a sum of
 //     exponentials a row (a TMEM lane, so a thread, holds a row);
@@ -31,10 +31,12 @@ namespace {
 
 constexpr int kTileM = 256;      // rows of a pair's tile, 128 a CTA
 constexpr int kTileN = 256;      // its columns at most
-constexpr int kTileK = 64;       // k of a stage: one 128-byte swizzle row of 16-bit elements
-constexpr int kOperand = 128 * 128;  // bytes of a CTA's share of an operand's stage
+constexpr int kTileK = 128;      // k of a stage
+constexpr int kChunk = 64;       // a 128-byte swizzle row of 16-bit elements
+constexpr int kOperand = 128 * kTileK * 2;  // bytes of a CTA's share of an operand's stage
+constexpr int kBox = kOperand / 2;  // one load: 128 rows x 64 k (K-major) or 128 k x 64 columns (MN-major)
 constexpr int kStage = 2 * kOperand;
-constexpr int kStages = 6;
+constexpr int kStages = 3;
 constexpr int kHead = 1024;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 320;    // warp 0 loads, warp 1 issues MMAs, warps 2-9 read TMEM
@@ -42,7 +44,6 @@ constexpr int kStagePitch = 33;  // fp32 of a row of an epilogue warp's 32 x 32 
 constexpr int kBlockBytes = 32 * kStagePitch * 4;
 constexpr int kSmem = 1024 + kHead + kStages * kStage + kEpiWarps * kBlockBytes;
 static_assert(kSmem <= 227 * 1024, "shared memory");
-constexpr int kChunk = 64;       // columns of an MN-major box
 constexpr int kMaxJobs = 3;
 constexpr int kGroupM = 32;      // row tiles that run through the vocabulary together
 constexpr float kLog2e = 1.4426950408889634f;
@@ -90,10 +91,10 @@ struct PairHead {
 static_assert(sizeof(PairHead) <= kHead, "head");
 
 // Shared-memory descriptor of an MN-major operand with the 128-byte swizzle:
-// boxes of 64 columns (128 bytes) x 64 k, 8 KB apart; groups of 8 k 1,024
+// boxes of 64 columns (128 bytes) x 128 k, 16 KB apart; groups of 8 k 1,024
 // bytes apart.
 __device__ __forceinline__ uint64_t mn_desc(uint32_t addr) {
-  return tile_desc(addr) | (uint64_t((kChunk * 128) >> 4) << 16);
+  return tile_desc(addr) | (uint64_t(kBox >> 4) << 16);
 }
 
 // Instruction descriptor: kind::f16, D fp32, A and B of one 16-bit type, each
@@ -335,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
         const CUtensorMap *ma = &a.map[2 * tl.job], *mb = ma + 1;
         const int half = tl.cols / 2, chunks = (half + kChunk - 1) / kChunk;
         const bool a_mn = j.kind == kHeadRows, b_mn = j.kind == kStates || j.kind == kHeadRows;
-        const uint32_t bytes = kOperand + (b_mn ? chunks * (kOperand / 2) : j.bn / 2 * 128);
+        const uint32_t bytes = kOperand + (b_mn ? chunks * kBox : j.bn / 2 * 2 * kTileK);
         const int am = tl.m + rank * (kTileM / 2), bn = tl.n + rank * half;
         for (int i = 0; i < tl.nkb; ++i) {
           if (!bar_wait(&H.empty[s], ph ^ 1, abort, a.err)) goto loaded;
@@ -347,15 +348,17 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
           if (rank == 0) bar_expect(&H.full[s], 2 * bytes);
           if (a_mn) {
             tma_load_pair(ma, sa, bar, am, k);
-            tma_load_pair(ma, sa + kOperand / 2, bar, am + kChunk, k);
+            tma_load_pair(ma, sa + kBox, bar, am + kChunk, k);
           } else {
             tma_load_pair(ma, sa, bar, k, am);
+            tma_load_pair(ma, sa + kBox, bar, k + kChunk, am);
           }
           if (b_mn) {
             const int kr = j.kind == kStates ? j.v0 + k : k;
-            for (int c = 0; c < chunks; ++c) tma_load_pair(mb, sb + c * (kOperand / 2), bar, bn + c * kChunk, kr);
+            for (int c = 0; c < chunks; ++c) tma_load_pair(mb, sb + c * kBox, bar, bn + c * kChunk, kr);
           } else {
             tma_load_pair(mb, sb, bar, k, j.v0 + bn);
+            tma_load_pair(mb, sb + kBox, bar, k + kChunk, j.v0 + bn);
           }
           if (++s == kStages) s = 0, ph ^= 1;
         }
@@ -377,8 +380,10 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
         const Job &j = a.job[tl.job];
         const bool a_mn = j.kind == kHeadRows, b_mn = j.kind == kStates || j.kind == kHeadRows;
         const uint32_t idesc = f16_idesc(kBf16, a_mn, b_mn, tl.cols);
-        // 16 k are 32 bytes of a K-major row, 16 rows of 128 bytes of an MN-major box.
-        const uint64_t step_a = a_mn ? 2048 >> 4 : 32 >> 4, step_b = b_mn ? 2048 >> 4 : 32 >> 4;
+        // 16 k are 32 bytes of a K-major row, 16 rows of 128 bytes of an MN-major
+        // box; 64 k are a box of the one, half a box of the other.
+        const uint64_t step_a = a_mn ? 2048 >> 4 : 32 >> 4, half_a = a_mn ? 8192 >> 4 : kBox >> 4;
+        const uint64_t step_b = b_mn ? 2048 >> 4 : 32 >> 4, half_b = b_mn ? 8192 >> 4 : kBox >> 4;
         ok = __all_sync(0xffffffffu, bar_wait(&H.acc_empty[acc], acc_ph ^ 1, abort, a.err));
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -391,7 +396,8 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
           const uint64_t bd = b_mn ? mn_desc(st + kOperand) : tile_desc(st + kOperand);
 #pragma unroll
           for (int k = 0; k < kTileK / 16; ++k)
-            mma_f16_pair(tmem + acc * kTileN, ad + k * step_a, bd + k * step_b, idesc, i > 0 || k > 0);
+            mma_f16_pair(tmem + acc * kTileN, ad + k / 4 * half_a + k % 4 * step_a, bd + k / 4 * half_b + k % 4 * step_b,
+                         idesc, i > 0 || k > 0);
           mma_commit_pair(&H.empty[s]);
           if (++s == kStages) s = 0, ph ^= 1;
         }
@@ -653,7 +659,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_back_rows_kernel(const BackRow
     }
   }
   if (blockIdx.x + 1 == gridDim.x) {
-    // The sums over tokens run in steps of 64: zeros up to there.
+    // The sums over tokens run in steps of 128: zeros up to there.
     const int end = (kept + kTileK - 1) / kTileK * kTileK;
     uint16_t *rows = a.scaled ? a.scaled : a.rows;
     for (int r = kept + warp; r < end; r += kRowThreads / 32)
@@ -804,7 +810,7 @@ bool map16(CUtensorMap *map, const void *base, int64_t rows, int64_t cols, int64
   if (!fn) return false;
   const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch) * 2};
-  const cuuint32_t box[2] = {kTileK, static_cast<cuuint32_t>(box_rows)}, es[2] = {1, 1};
+  const cuuint32_t box[2] = {kChunk, static_cast<cuuint32_t>(box_rows)}, es[2] = {1, 1};
   return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void *>(base), dims, strides, box, es,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -1008,7 +1014,7 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   const int64_t scale_at = sc.take(8);
   const int64_t w_at = head_readable(c) ? -1 : sc.take(c.vocab * pitch * 2);
   const int64_t acc_at = dx ? sc.take(plan.split * c.tokens * acc_pitch * 4) : -1;
-  const int64_t d_bytes = rows * plan.piece * 2;
+  const int64_t d_pitch = plan.piece, d_bytes = rows * d_pitch * 2;
   const int64_t d_at = sc.take(d_bytes), d2_at = plan.pieces > 1 ? sc.take(d_bytes) : d_at;
   int rc = sc.allocate(T);
   if (rc != H24_OK) return rc;
@@ -1072,7 +1078,7 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
         j.out = sc.at<float>(acc_at);
         j.pitch = acc_pitch;
         j.plane = c.tokens * acc_pitch;
-        ok = ok && map16(&g.map[2 * g.jobs], d, rows, plan.piece, plan.piece, kTileM / 2) &&
+        ok = ok && map16(&g.map[2 * g.jobs], d, rows, plan.piece, d_pitch, kTileM / 2) &&
              map16(&g.map[2 * g.jobs + 1], w, c.vocab, c.in, w_pitch, kTileK);
         tiles += rows / kTileM * cdiv(c.in, bn_in) * plan.split;
         ++g.jobs;
@@ -1088,7 +1094,7 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
         j.v0 = static_cast<int>(v0);
         j.out = dw;
         j.pitch = c.in;
-        ok = ok && map16(&g.map[2 * g.jobs], d, rows, plan.piece, plan.piece, kTileK) &&
+        ok = ok && map16(&g.map[2 * g.jobs], d, rows, plan.piece, d_pitch, kTileK) &&
              map16(&g.map[2 * g.jobs + 1], head_rows, rows_alloc, c.in, pitch, kTileK);
         tiles += cdiv(v, kTileM) * cdiv(c.in, bn_in);
         ++g.jobs;
@@ -1112,7 +1118,7 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
       j.split = 1;
       j.v0 = static_cast<int>(v0);
       j.out = sc.at<uint16_t>(i & 1 ? d2_at : d_at);
-      j.pitch = plan.piece;
+      j.pitch = d_pitch;
       ok = ok && map16(&g.map[2 * g.jobs], r.rows, c.tokens, c.in, pitch, kTileM / 2) &&
            map16(&g.map[2 * g.jobs + 1], w, c.vocab, c.in, w_pitch, j.bn / 2);
       tiles += rows / kTileM * cdiv(j.n_total, j.bn);
