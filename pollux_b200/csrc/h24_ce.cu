@@ -40,8 +40,8 @@ constexpr int kStages = 3;
 constexpr int kHead = 1024;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 320;    // warp 0 loads, warp 1 issues MMAs, warps 2-9 read TMEM
-constexpr int kStagePitch = 33;  // fp32 of a row of an epilogue warp's 32 x 32 block
-constexpr int kBlockBytes = 32 * kStagePitch * 4;
+constexpr int kBlockPitch = 66;  // elements of a row of an epilogue warp's 32 x 64 block
+constexpr int kBlockBytes = 32 * kBlockPitch * 2;
 constexpr int kSmem = 1024 + kHead + kStages * kStage + kEpiWarps * kBlockBytes;
 static_assert(kSmem <= 227 * 1024, "shared memory");
 constexpr int kMaxJobs = 3;
@@ -71,6 +71,7 @@ struct GemmArgs {
   Job job[kMaxJobs];
   int jobs;
   int vocab;
+  int a_rows;          // rows of a CTA's share of the tokens' tiles that are loaded
   const int *kept;     // number of tokens with a loss
   const int *target;   // of each kept token
   const float *lse;    // of each kept token
@@ -336,7 +337,10 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
         const CUtensorMap *ma = &a.map[2 * tl.job], *mb = ma + 1;
         const int half = tl.cols / 2, chunks = (half + kChunk - 1) / kChunk;
         const bool a_mn = j.kind == kHeadRows, b_mn = j.kind == kStates || j.kind == kHeadRows;
-        const uint32_t bytes = kOperand + (b_mn ? chunks * kBox : j.bn / 2 * 2 * kTileK);
+        // (The second CTA of a pair loads no tokens' rows where the first has room for all.)
+        const bool load_a = a_mn || a.a_rows == kTileM / 2 || rank == 0;
+        const uint32_t bytes_a = a_mn || a.a_rows == kTileM / 2 ? 2 * kOperand : a.a_rows * kTileK * 2;
+        const uint32_t bytes = bytes_a + 2 * (b_mn ? chunks * kBox : j.bn / 2 * 2 * kTileK);
         const int am = tl.m + rank * (kTileM / 2), bn = tl.n + rank * half;
         for (int i = 0; i < tl.nkb; ++i) {
           if (!bar_wait(&H.empty[s], ph ^ 1, abort, a.err)) goto loaded;
@@ -345,11 +349,11 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
           // The first CTA's barrier counts the bytes of both; its phase cannot
           // end before its own arrival here.
           const uint32_t bar = cluster_addr(&H.full[s], 0);
-          if (rank == 0) bar_expect(&H.full[s], 2 * bytes);
+          if (rank == 0) bar_expect(&H.full[s], bytes);
           if (a_mn) {
             tma_load_pair(ma, sa, bar, am, k);
             tma_load_pair(ma, sa + kBox, bar, am + kChunk, k);
-          } else {
+          } else if (load_a) {
             tma_load_pair(ma, sa, bar, k, am);
             tma_load_pair(ma, sa + kBox, bar, k + kChunk, am);
           }
@@ -420,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
     const int uwarp = __shfl_sync(0xffffffffu, warp, 0);
     const int quarter = uwarp & 3, part = (uwarp - 2) >> 2;  // TMEM lanes, and first or second part of the columns
     const uint32_t ta = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    float *block = reinterpret_cast<float *>(stages + kStages * kStage) + (uwarp - 2) * 32 * kStagePitch;
+    uint16_t *block = reinterpret_cast<uint16_t *>(stages + kStages * kStage) + (uwarp - 2) * 32 * kBlockPitch;
     int acc = 0;
     uint32_t ph = 0;
     for (int idx = first; idx < tiles; idx += step) {
@@ -475,13 +479,26 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
               if (st.live && 16 * h < left) store32B(out + lane * j.pitch + 16 * h, w);
             }
           } else {
-            // Rows off 32 bytes: a warp writes a row's 32 elements at a time.
+            // Rows off 32 bytes: 64 columns of 32 rows in shared memory, from
+            // which a warp writes a row's 128 bytes at a time, in words of two
+            // elements from the first whole word on.
+            const int at = (c - c0) & 32;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) block[lane * kStagePitch + i] = z[i] * scale;
+            for (int i = 0; i < 32; ++i) block[lane * kBlockPitch + at + i] = pack1<kBf16>(z[i] * scale);
+            if (at == 0 && c + 32 < c1) continue;
             __syncwarp();
-            const int rows = min(32, j.m_total - row0);
-            if (lane < left)
-              for (int i = 0; i < rows; ++i) out[i * j.pitch + lane] = pack1<kBf16>(block[i * kStagePitch + lane]);
+            const int rows = min(32, j.m_total - row0), have = min(at + 32, left + at);
+            out -= at;
+            for (int i = 0; i < rows; ++i, out += j.pitch) {
+              const uint16_t *from = block + i * kBlockPitch;
+              const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(out) >> 1 & 1), e = 2 * lane + odd;
+              if (e + 1 < have)
+                *reinterpret_cast<uint32_t *>(out + e) = from[e] | static_cast<uint32_t>(from[e + 1]) << 16;
+              else if (e < have)
+                out[e] = from[e];
+              if (odd && lane == 0 && have > 0) out[0] = from[0];
+            }
+            __syncwarp();
           }
         }
       }
@@ -525,10 +542,23 @@ State state_at(const int32_t *state, int64_t tokens) {
   return {p, p + 1, p + 1 + tokens, reinterpret_cast<float *>(p + 1 + 2 * tokens)};
 }
 
-struct RowsArgs {
-  const void *x;
-  int64_t x_stride;
+// 8 elements at a row's element c (a multiple of 8) of x, from any alignment;
+// zeros past the row's end.
+struct RowSource {
+  const uint16_t *x;
+  int64_t stride;
   int tokens, in;
+  bool vec;  // rows lie on 16 bytes
+  __device__ __forceinline__ uint4 load(int64_t r, int c) const {
+    const uint16_t *p = x + r * stride + c;
+    if (vec) return __ldg(reinterpret_cast<const uint4 *>(p));
+    return load16_any(reinterpret_cast<const int8_t *>(p), 2 * (in - c), reinterpret_cast<const int8_t *>(x),
+                      reinterpret_cast<const int8_t *>(x + (tokens - 1) * stride + in));
+  }
+};
+
+struct RowsArgs {
+  RowSource x;
   const int64_t *labels;
   int64_t ignore;
   int vocab;
@@ -539,17 +569,7 @@ struct RowsArgs {
   float *loss;     // of each token, or null
   unsigned *ticket;
   int per_block;
-  bool vec;        // rows of x lie on 16 bytes
 };
-
-// One row, by a warp.
-__device__ __forceinline__ void copy_row(const uint16_t *src, uint16_t *dst, int n, bool vec, int lane) {
-  if (vec) {
-    for (int c = lane; c < n / 8; c += 32) reinterpret_cast<uint4 *>(dst)[c] = reinterpret_cast<const uint4 *>(src)[c];
-  } else {
-    for (int c = lane; c < n; c += 32) dst[c] = src[c];
-  }
-}
 
 __device__ __forceinline__ int block_sum(int v, int *red) {
   v = __reduce_add_sync(0xffffffffu, v);
@@ -574,7 +594,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_rows_kernel(const RowsArgs a) 
   before = block_sum(before, red);
   // per_block is at most the number of threads.
   const int64_t r = r0 + t;
-  const bool mine = t < a.per_block && r < a.tokens;
+  const bool mine = t < a.per_block && r < a.x.tokens;
   const int64_t label = mine ? __ldg(a.labels + r) : a.ignore;
   const bool keep = mine && label != a.ignore;
   const unsigned votes = __ballot_sync(0xffffffffu, keep);
@@ -595,9 +615,13 @@ __global__ void __launch_bounds__(kRowThreads) ce_rows_kernel(const RowsArgs a) 
     if (a.token) a.token[before + at] = static_cast<int>(r);
   }
   __syncthreads();
-  const uint16_t *x = static_cast<const uint16_t *>(a.x);
-  for (int i = warp; i < count; i += kRowThreads / 32)
-    copy_row(x + (r0 + from[i]) * a.x_stride, a.rows + (before + static_cast<int64_t>(i)) * a.pitch, a.in, a.vec, lane);
+  const int vecs = (a.x.in + 7) / 8;
+  uint4 *out = reinterpret_cast<uint4 *>(a.rows + before * a.pitch);
+#pragma unroll 4
+  for (int i = t; i < count * vecs; i += kRowThreads) {
+    const int row = i / vecs, c = i - row * vecs;
+    out[row * (a.pitch / 8) + c] = a.x.load(r0 + from[row], 8 * c);
+  }
   if (blockIdx.x + 1 == gridDim.x && t == 0) {
     *a.st.kept = before + count;
     *a.ticket = 0;
@@ -605,16 +629,14 @@ __global__ void __launch_bounds__(kRowThreads) ce_rows_kernel(const RowsArgs a) 
 }
 
 struct BackRowsArgs {
-  const void *x;
-  int64_t x_stride;
-  int tokens, in;
+  RowSource x;
   State st;
   uint16_t *rows;    // copied states
   uint16_t *scaled;  // the same times g / max |g|, or null (g the same for all)
   int64_t pitch;
   const float *dloss;
   int64_t dloss_stride;
-  bool mean, vec;
+  bool mean;
   float inv_prob_scale;
   float *scale;      // [0] factor of dW, [1] factor of dx where g is the same for all
   int per_block;
@@ -632,7 +654,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_back_rows_kernel(const BackRow
   const int kept = *a.st.kept;
   float top = 0.f;
   if (a.scaled) {
-    for (int64_t i = t; i < a.tokens; i += kRowThreads)
+    for (int64_t i = t; i < a.x.tokens; i += kRowThreads)
       if (__ldg(a.st.place + i) >= 0) {
         const float g = fabsf(__ldg(a.dloss + i * a.dloss_stride));
         top = g != g ? g : fmaxf(g, top);  // (a NaN that is overtaken here is in the states all the same)
@@ -643,27 +665,35 @@ __global__ void __launch_bounds__(kRowThreads) ce_back_rows_kernel(const BackRow
     top = 0.f;
     for (int w = 0; w < kRowThreads / 32; ++w) top = fmaxf(top, red[w]);
   }
-  const uint16_t *x = static_cast<const uint16_t *>(a.x);
   const int64_t r0 = static_cast<int64_t>(blockIdx.x) * a.per_block;
-  for (int64_t r = r0 + warp; r < r0 + a.per_block && r < a.tokens; r += kRowThreads / 32) {
-    const int place = a.st.place[r];
+  const int rows = static_cast<int>(min(static_cast<int64_t>(a.per_block), a.x.tokens - r0)), vecs = (a.x.in + 7) / 8;
+#pragma unroll 2
+  for (int i = t; i < rows * vecs; i += kRowThreads) {
+    const int row = i / vecs, c = i - row * vecs;
+    const int place = __ldg(a.st.place + r0 + row);
     if (place < 0) continue;
-    const uint16_t *src = x + r * a.x_stride;
-    copy_row(src, a.rows + place * a.pitch, a.in, a.vec, lane);
-    if (a.scaled) {
-      const float g = top > 0.f ? a.dloss[r * a.dloss_stride] / top : a.dloss[r * a.dloss_stride];
-      for (int c = lane; c < a.in; c += 32) {
-        const float v = kBf16 ? __bfloat162float(__ushort_as_bfloat16(src[c])) : __half2float(__ushort_as_half(src[c]));
-        a.scaled[place * a.pitch + c] = pack1<kBf16>(v * g);
-      }
+    const uint4 v = a.x.load(r0 + row, 8 * c);
+    reinterpret_cast<uint4 *>(a.rows + place * a.pitch)[c] = v;
+    if (!a.scaled) continue;
+    float g = __ldg(a.dloss + (r0 + row) * a.dloss_stride);
+    if (top > 0.f) g /= top;
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t o[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint16_t lo = static_cast<uint16_t>(w[k]), hi = static_cast<uint16_t>(w[k] >> 16);
+      const float x0 = kBf16 ? __bfloat162float(__ushort_as_bfloat16(lo)) : __half2float(__ushort_as_half(lo));
+      const float x1 = kBf16 ? __bfloat162float(__ushort_as_bfloat16(hi)) : __half2float(__ushort_as_half(hi));
+      o[k] = pack2<kBf16>(x0 * g, x1 * g);
     }
+    reinterpret_cast<uint4 *>(a.scaled + place * a.pitch)[c] = make_uint4(o[0], o[1], o[2], o[3]);
   }
   if (blockIdx.x + 1 == gridDim.x) {
     // The sums over tokens run in steps of 128: zeros up to there.
     const int end = (kept + kTileK - 1) / kTileK * kTileK;
     uint16_t *rows = a.scaled ? a.scaled : a.rows;
     for (int r = kept + warp; r < end; r += kRowThreads / 32)
-      for (int c = lane; c < a.in; c += 32) rows[r * a.pitch + c] = 0;
+      for (int c = lane; c < a.x.in; c += 32) rows[r * a.pitch + c] = 0;
     if (t == 0) {
       const float g = a.scaled ? (top > 0.f ? top : 1.f) : a.mean ? a.dloss[0] / static_cast<float>(kept) : a.dloss[0];
       a.scale[0] = kept ? g * a.inv_prob_scale : 0.f;
@@ -875,6 +905,10 @@ int logits_bn(int64_t tokens, int64_t vocab) {
   return bn;
 }
 
+// Rows that a CTA loads of the tokens' tiles: all 128, or of the one tile of up
+// to 128 tokens those that are there, since no output takes the others.
+int token_rows(int64_t tokens) { return tokens > 128 ? 128 : static_cast<int>(up(tokens, 8)); }
+
 // Rows of a block of the row kernels: the blocks fill the GPU four times at most.
 int rows_per_block(int64_t tokens) {
   const int64_t per = cdiv(tokens, 592);
@@ -915,10 +949,8 @@ int launch_ce_forward(const Tables *T, const CeArgs &c, const int64_t *labels, i
   if (rc != H24_OK) return rc;
   const State st = state_at(state, c.tokens);
   RowsArgs r{};
-  r.x = c.x;
-  r.x_stride = c.x_stride;
-  r.tokens = static_cast<int>(c.tokens);
-  r.in = static_cast<int>(c.in);
+  r.x = {static_cast<const uint16_t *>(c.x), c.x_stride, static_cast<int>(c.tokens), static_cast<int>(c.in),
+         rows_on_16(c.x, c.x_stride, c.in)};
   r.labels = labels;
   r.ignore = ignore;
   r.vocab = static_cast<int>(c.vocab);
@@ -929,7 +961,6 @@ int launch_ce_forward(const Tables *T, const CeArgs &c, const int64_t *labels, i
   r.loss = c.reduction == H24_REDUCE_NONE ? loss : nullptr;
   r.ticket = sc.at<unsigned>(ticket_at);
   r.per_block = rows_per_block(c.tokens);
-  r.vec = rows_on_16(c.x, c.x_stride, c.in);
   H24_CUDA_TRY(launch_pdl(ce_rows_kernel, dim3(static_cast<unsigned>(cdiv(c.tokens, r.per_block))), dim3(kRowThreads),
                           s, r));
   count_launches(1);
@@ -938,9 +969,10 @@ int launch_ce_forward(const Tables *T, const CeArgs &c, const int64_t *labels, i
   if ((rc = readable_head(c, sc, w_at, &w, &w_pitch)) != H24_OK) return rc;
 
   GemmArgs g{};
-  if (!map16(&g.map[0], r.rows, c.tokens, c.in, pitch, kTileM / 2) || !map16(&g.map[1], w, c.vocab, c.in, w_pitch, bn / 2))
+  if (!map16(&g.map[0], r.rows, c.tokens, c.in, pitch, token_rows(c.tokens)) || !map16(&g.map[1], w, c.vocab, c.in, w_pitch, bn / 2))
     return fail(H24_ERR_CUDA, "linear_ce_forward: cuTensorMapEncodeTiled failed");
   g.jobs = 1;
+  g.a_rows = token_rows(c.tokens);
   g.job[0].kind = kLoss;
   g.job[0].n_total = static_cast<int>(c.vocab);
   g.job[0].bn = bn;
@@ -1022,10 +1054,8 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   const float prob_scale = bf16 ? 1.f : 32768.f;
 
   BackRowsArgs r{};
-  r.x = c.x;
-  r.x_stride = c.x_stride;
-  r.tokens = static_cast<int>(c.tokens);
-  r.in = static_cast<int>(c.in);
+  r.x = {static_cast<const uint16_t *>(c.x), c.x_stride, static_cast<int>(c.tokens), static_cast<int>(c.in),
+         rows_on_16(c.x, c.x_stride, c.in)};
   r.st = st;
   r.rows = sc.at<uint16_t>(rows_at);
   r.scaled = scaled_at < 0 ? nullptr : sc.at<uint16_t>(scaled_at);
@@ -1033,7 +1063,6 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   r.dloss = dloss;
   r.dloss_stride = dloss_stride;
   r.mean = c.reduction == H24_REDUCE_MEAN;
-  r.vec = rows_on_16(c.x, c.x_stride, c.in);
   r.inv_prob_scale = 1.f / prob_scale;
   r.scale = sc.at<float>(scale_at);
   r.per_block = rows_per_block(c.tokens);
@@ -1046,6 +1075,7 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
 
   GemmArgs base{};
   base.vocab = static_cast<int>(c.vocab);
+  base.a_rows = token_rows(c.tokens);
   base.kept = st.kept;
   base.target = st.target;
   base.lse = st.lse;
@@ -1078,7 +1108,7 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
         j.out = sc.at<float>(acc_at);
         j.pitch = acc_pitch;
         j.plane = c.tokens * acc_pitch;
-        ok = ok && map16(&g.map[2 * g.jobs], d, rows, plan.piece, d_pitch, kTileM / 2) &&
+        ok = ok && map16(&g.map[2 * g.jobs], d, rows, plan.piece, d_pitch, token_rows(c.tokens)) &&
              map16(&g.map[2 * g.jobs + 1], w, c.vocab, c.in, w_pitch, kTileK);
         tiles += rows / kTileM * cdiv(c.in, bn_in) * plan.split;
         ++g.jobs;
@@ -1119,7 +1149,7 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
       j.v0 = static_cast<int>(v0);
       j.out = sc.at<uint16_t>(i & 1 ? d2_at : d_at);
       j.pitch = d_pitch;
-      ok = ok && map16(&g.map[2 * g.jobs], r.rows, c.tokens, c.in, pitch, kTileM / 2) &&
+      ok = ok && map16(&g.map[2 * g.jobs], r.rows, c.tokens, c.in, pitch, token_rows(c.tokens)) &&
            map16(&g.map[2 * g.jobs + 1], w, c.vocab, c.in, w_pitch, j.bn / 2);
       tiles += rows / kTileM * cdiv(j.n_total, j.bn);
       ++g.jobs;
