@@ -35,14 +35,14 @@ constexpr int kTileK = 128;      // k of a stage
 constexpr int kChunk = 64;       // a 128-byte swizzle row of 16-bit elements
 constexpr int kOperand = 128 * kTileK * 2;  // bytes of a CTA's share of an operand's stage
 constexpr int kBox = kOperand / 2;  // one load: 128 rows x 64 k (K-major) or 128 k x 64 columns (MN-major)
-constexpr int kStage = 2 * kOperand;
-constexpr int kStages = 3;
+constexpr int kRing = 6 * kOperand;  // bytes of the ring of stages
+constexpr int kMaxStages = 5;
 constexpr int kHead = 1024;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 320;    // warp 0 loads, warp 1 issues MMAs, warps 2-9 read TMEM
 constexpr int kBlockPitch = 66;  // elements of a row of an epilogue warp's 32 x 64 block
 constexpr int kBlockBytes = 32 * kBlockPitch * 2;
-constexpr int kSmem = 1024 + kHead + kStages * kStage + kEpiWarps * kBlockBytes;
+constexpr int kSmem = 1024 + kHead + kRing + kEpiWarps * kBlockBytes;
 static_assert(kSmem <= 227 * 1024, "shared memory");
 constexpr int kMaxJobs = 3;
 constexpr int kGroupM = 32;      // row tiles that run through the vocabulary together
@@ -72,6 +72,7 @@ struct GemmArgs {
   int jobs;
   int vocab;
   int a_rows;          // rows of a CTA's share of the tokens' tiles that are loaded
+  int stages, stage_a; // of the ring; bytes of A in a stage
   const int *kept;     // number of tokens with a loss
   const int *target;   // of each kept token
   const float *lse;    // of each kept token
@@ -80,12 +81,12 @@ struct GemmArgs {
   int64_t part_pitch;
   const float *scale;  // kHeadRows: factor of the sum
   float prob_scale;
-  bool wide_rows;      // kHeadRows: rows of the output lie on 32 bytes
+  int row_bytes;       // kHeadRows: rows of the output lie on 32, 16 or 2 bytes
   int *err;
 };
 
 struct PairHead {
-  uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], drain;
+  uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2], drain;
   uint32_t tmem;
   int abort;
 };
@@ -197,6 +198,9 @@ __device__ __forceinline__ uint16_t pack1(float a) {
   return __half_as_ushort(__float2half_rn(a));
 }
 
+// 1 where an element lies in a word's second half.
+__device__ __forceinline__ int odd16(const uint16_t *p) { return static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 1 & 1); }
+
 // What an epilogue thread does with 32 columns of its row.  `c` is the column
 // within the tile; r the sums.
 struct RowState {
@@ -294,10 +298,11 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const int rank = static_cast<int>(blockIdx.x) & 1;
   const int first = static_cast<int>(blockIdx.x) >> 1, step = static_cast<int>(gridDim.x) >> 1;
+  const int stage_bytes = a.stage_a + kOperand;
   volatile int *abort = &H.abort;
 
   if (t == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < a.stages; ++s) {
       bar_init(&H.full[s], 1);
       bar_init(&H.empty[s], 1);
     }
@@ -344,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
         const int am = tl.m + rank * (kTileM / 2), bn = tl.n + rank * half;
         for (int i = 0; i < tl.nkb; ++i) {
           if (!bar_wait(&H.empty[s], ph ^ 1, abort, a.err)) goto loaded;
-          uint8_t *sa = stages + static_cast<size_t>(s) * kStage, *sb = sa + kOperand;
+          uint8_t *sa = stages + s * stage_bytes, *sb = sa + a.stage_a;
           const int k = (tl.kb + i) * kTileK;
           // The first CTA's barrier counts the bytes of both; its phase cannot
           // end before its own arrival here.
@@ -355,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
             tma_load_pair(ma, sa + kBox, bar, am + kChunk, k);
           } else if (load_a) {
             tma_load_pair(ma, sa, bar, k, am);
-            tma_load_pair(ma, sa + kBox, bar, k + kChunk, am);
+            tma_load_pair(ma, sa + a.stage_a / 2, bar, k + kChunk, am);
           }
           if (b_mn) {
             const int kr = j.kind == kStates ? j.v0 + k : k;
@@ -364,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
             tma_load_pair(mb, sb, bar, k, j.v0 + bn);
             tma_load_pair(mb, sb + kBox, bar, k + kChunk, j.v0 + bn);
           }
-          if (++s == kStages) s = 0, ph ^= 1;
+          if (++s == a.stages) s = 0, ph ^= 1;
         }
       }
     loaded:
@@ -386,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
         const uint32_t idesc = f16_idesc(kBf16, a_mn, b_mn, tl.cols);
         // 16 k are 32 bytes of a K-major row, 16 rows of 128 bytes of an MN-major
         // box; 64 k are a box of the one, half a box of the other.
-        const uint64_t step_a = a_mn ? 2048 >> 4 : 32 >> 4, half_a = a_mn ? 8192 >> 4 : kBox >> 4;
+        const uint64_t step_a = a_mn ? 2048 >> 4 : 32 >> 4, half_a = a_mn ? 8192 >> 4 : a.stage_a >> 5;
         const uint64_t step_b = b_mn ? 2048 >> 4 : 32 >> 4, half_b = b_mn ? 8192 >> 4 : kBox >> 4;
         ok = __all_sync(0xffffffffu, bar_wait(&H.acc_empty[acc], acc_ph ^ 1, abort, a.err));
         if (!ok) break;
@@ -395,15 +400,15 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
           ok = __all_sync(0xffffffffu, bar_wait(&H.full[s], ph, abort, a.err));
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t st = su32(stages) + static_cast<uint32_t>(s * kStage);
+          const uint32_t st = su32(stages) + static_cast<uint32_t>(s * stage_bytes);
           const uint64_t ad = a_mn ? mn_desc(st) : tile_desc(st);
-          const uint64_t bd = b_mn ? mn_desc(st + kOperand) : tile_desc(st + kOperand);
+          const uint64_t bd = b_mn ? mn_desc(st + a.stage_a) : tile_desc(st + a.stage_a);
 #pragma unroll
           for (int k = 0; k < kTileK / 16; ++k)
             mma_f16_pair(tmem + acc * kTileN, ad + k / 4 * half_a + k % 4 * step_a, bd + k / 4 * half_b + k % 4 * step_b,
                          idesc, i > 0 || k > 0);
           mma_commit_pair(&H.empty[s]);
-          if (++s == kStages) s = 0, ph ^= 1;
+          if (++s == a.stages) s = 0, ph ^= 1;
         }
         if (!ok) break;
         mma_commit_pair(&H.acc_full[acc]);
@@ -424,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
     const int uwarp = __shfl_sync(0xffffffffu, warp, 0);
     const int quarter = uwarp & 3, part = (uwarp - 2) >> 2;  // TMEM lanes, and first or second part of the columns
     const uint32_t ta = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    uint16_t *block = reinterpret_cast<uint16_t *>(stages + kStages * kStage) + (uwarp - 2) * 32 * kBlockPitch;
+    uint16_t *block = reinterpret_cast<uint16_t *>(stages + kRing) + (uwarp - 2) * 32 * kBlockPitch;
     int acc = 0;
     uint32_t ph = 0;
     for (int idx = first; idx < tiles; idx += step) {
@@ -470,33 +475,53 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
         } else {
           uint16_t *out = static_cast<uint16_t *>(j.out) + (j.v0 + static_cast<int64_t>(row0)) * j.pitch + tl.n + c;
           const int left = j.n_total - (tl.n + c);
-          if (a.wide_rows) {
+          if (a.row_bytes >= 16) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               uint32_t w[8];
 #pragma unroll
               for (int i = 0; i < 8; ++i) w[i] = pack2<kBf16>(z[16 * h + 2 * i] * scale, z[16 * h + 2 * i + 1] * scale);
-              if (st.live && 16 * h < left) store32B(out + lane * j.pitch + 16 * h, w);
+              uint16_t *to = out + lane * j.pitch + 16 * h;
+              if (a.row_bytes == 32) {
+                if (st.live && 16 * h < left) store32B(to, w);
+              } else {
+                if (st.live && 16 * h < left) *reinterpret_cast<uint4 *>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+                if (st.live && 16 * h + 8 < left) *reinterpret_cast<uint4 *>(to + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+              }
             }
           } else {
-            // Rows off 32 bytes: 64 columns of 32 rows in shared memory, from
-            // which a warp writes a row's 128 bytes at a time, in words of two
-            // elements from the first whole word on.
+            // Rows on single elements: 64 columns of 32 rows in shared memory,
+            // each row shifted so that its words there are words of memory; a
+            // warp then writes a row's 128 bytes at a time.  (The loop is bound by
+            // its instructions, two warps a scheduler.)
             const int at = (c - c0) & 32;
+            out -= at;
+            const int first_odd = odd16(out), turn = static_cast<int>(j.pitch & 1);
+            uint16_t *mine = block + lane * kBlockPitch + ((first_odd + lane * turn) & 1) + at;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) block[lane * kBlockPitch + at + i] = pack1<kBf16>(z[i] * scale);
+            for (int i = 0; i < 32; ++i) mine[i] = pack1<kBf16>(z[i] * scale);
             if (at == 0 && c + 32 < c1) continue;
             __syncwarp();
             const int rows = min(32, j.m_total - row0), have = min(at + 32, left + at);
-            out -= at;
-            for (int i = 0; i < rows; ++i, out += j.pitch) {
-              const uint16_t *from = block + i * kBlockPitch;
-              const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(out) >> 1 & 1), e = 2 * lane + odd;
-              if (e + 1 < have)
-                *reinterpret_cast<uint32_t *>(out + e) = from[e] | static_cast<uint32_t>(from[e + 1]) << 16;
-              else if (e < have)
-                out[e] = from[e];
-              if (odd && lane == 0 && have > 0) out[0] = from[0];
+            const uint32_t *words = reinterpret_cast<const uint32_t *>(block) + lane;
+            auto put = [&](uint16_t *to, uint32_t v, int i, int odd) {
+              const int e = 2 * lane - odd;  // the word's first element
+              if (e >= 0 && e + 1 < have) {
+                *reinterpret_cast<uint32_t *>(to + e) = v;
+              } else if (e < 0) {
+                if (have > 0) to[0] = static_cast<uint16_t>(v >> 16);
+                if (have == 64) to[63] = block[i * kBlockPitch + 64];
+              } else if (e < have) {
+                to[e] = static_cast<uint16_t>(v);
+              }
+            };
+            for (int i0 = 0; i0 < rows; i0 += 8) {
+              uint32_t v[8];
+#pragma unroll
+              for (int u = 0; u < 8; ++u) v[u] = words[(i0 + u) * (kBlockPitch / 2)];
+#pragma unroll
+              for (int u = 0; u < 8; ++u, out += j.pitch)
+                if (i0 + u < rows) put(out, v[u], i0 + u, (first_odd + u * turn) & 1);  // (i0 is even)
             }
             __syncwarp();
           }
@@ -702,6 +727,64 @@ __global__ void __launch_bounds__(kRowThreads) ce_back_rows_kernel(const BackRow
   }
 }
 
+// 8 elements from S words and H halves into two neighbouring 16-byte blocks.
+template <int S, bool H>
+__device__ __forceinline__ uint4 shifted(uint4 x, uint4 y) {
+  const uint32_t v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = H ? __funnelshift_r(v[S + i], v[S + i + 1], 16) : v[S + i];
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// The head's rows at any pitch and alignment, copied to rows of `pitch`
+// elements on 16 bytes, a warp a row: [50257,1153] 41 us for 232 MB, where the
+// general copy by vectors (repack_rows_kernel), whose shifts differ from thread
+// to thread, took 59.  What stands past a row's end is not read.
+__global__ void __launch_bounds__(kRowThreads) ce_copy_head_kernel(const uint16_t *w, int64_t stride, int64_t rows,
+                                                                   int in, uint16_t *out, int64_t pitch) {
+  pdl_enter();
+  const int lane = threadIdx.x & 31, vecs = (in + 7) / 8;
+  const int8_t *lo = reinterpret_cast<const int8_t *>(w);
+  const int8_t *hi = reinterpret_cast<const int8_t *>(w + (rows - 1) * stride + in);
+  for (int64_t r = blockIdx.x * static_cast<int64_t>(kRowThreads / 32) + (threadIdx.x >> 5); r < rows;
+       r += static_cast<int64_t>(gridDim.x) * (kRowThreads / 32)) {
+    const int8_t *p = reinterpret_cast<const int8_t *>(w + r * stride);
+    const uint32_t off = offset16(p);
+    uint4 *to = reinterpret_cast<uint4 *>(out + r * pitch);
+    if (p - off < lo || p - off + (vecs + 1) * 16 > hi) {  // blocks that reach past the matrix
+      for (int c = lane; c < vecs; c += 32) to[c] = load16_any(p + 16 * c, 2 * in - 16 * c, lo, hi);
+      continue;
+    }
+    const uint4 *from = reinterpret_cast<const uint4 *>(p - off);
+    constexpr int U = 4;
+    for (int c0 = lane; c0 < vecs; c0 += 32 * U) {
+      uint4 x[U], y[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int c = min(c0 + 32 * u, vecs - 1);
+        x[u] = __ldg(from + c);
+        y[u] = __ldg(from + c + 1);
+      }
+      auto put = [&](auto f) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (c0 + 32 * u < vecs) to[c0 + 32 * u] = f(x[u], y[u]);
+      };
+      switch (off >> 1) {  // (the same for the warp)
+        case 0: put([](uint4 a, uint4 b) { return shifted<0, false>(a, b); }); break;
+        case 1: put([](uint4 a, uint4 b) { return shifted<0, true>(a, b); }); break;
+        case 2: put([](uint4 a, uint4 b) { return shifted<1, false>(a, b); }); break;
+        case 3: put([](uint4 a, uint4 b) { return shifted<1, true>(a, b); }); break;
+        case 4: put([](uint4 a, uint4 b) { return shifted<2, false>(a, b); }); break;
+        case 5: put([](uint4 a, uint4 b) { return shifted<2, true>(a, b); }); break;
+        case 6: put([](uint4 a, uint4 b) { return shifted<3, false>(a, b); }); break;
+        default: put([](uint4 a, uint4 b) { return shifted<3, true>(a, b); }); break;
+      }
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
 // The loss from the tiles' maxima and sums
 // ---------------------------------------------------------------------------
@@ -734,7 +817,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_combine_kernel(const CombineAr
   };
   float2 p = make_float2(kNegInf, 0.f);
   if (row < kept) {
-#pragma unroll 4
+#pragma unroll 8
     for (int i = t / kCombineRows; i < a.n_parts; i += kRowThreads / kCombineRows)
       join(p, __ldg(a.parts + i * a.part_pitch + row));
   }
@@ -807,6 +890,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_states_kernel(const StatesArgs
     if (place >= 0) {
       // (The rows of acc are padded to 32 columns.)
       const float *p = a.acc + place * a.pitch + c;
+#pragma unroll 4
       for (int s = 0; s < a.slices; ++s, p += a.plane) {
         const float4 x = __ldcs(reinterpret_cast<const float4 *>(p)), y = __ldcs(reinterpret_cast<const float4 *>(p) + 1);
         v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
@@ -875,7 +959,14 @@ struct Scratch {
   }
 };
 
-int launch_gemm(const GemmArgs &a, bool bf16, int64_t tiles, cudaStream_t s) {
+int launch_gemm(GemmArgs a, bool bf16, int64_t tiles, cudaStream_t s) {
+  // Where a tile has few tokens, A is small and the ring has more stages, so that
+  // more of the other operand is on its way (one token: 46 -> 36 us).
+  bool full = a.a_rows == kTileM / 2;
+  for (int i = 0; i < a.jobs; ++i) full = full || a.job[i].kind == kHeadRows;
+  a.stage_a = full ? kOperand : a.a_rows * kTileK * 2;
+  a.stages = kRing / (a.stage_a + kOperand);
+  if (a.stages > kMaxStages) a.stages = kMaxStages;
   H24_CUDA_TRY(bf16 ? allow_smem<ce_gemm_kernel<true>>(kSmem) : allow_smem<ce_gemm_kernel<false>>(kSmem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * (tiles < 1 ? 1 : tiles < kPairs ? tiles : kPairs)));
@@ -924,10 +1015,9 @@ int readable_head(const CeArgs &c, const Scratch &sc, int64_t copy_at, const voi
   if (copy_at < 0) return H24_OK;
   *w = sc.at<void>(copy_at);
   *pitch = up(c.in, 8);
-  const RepackArgs rw{static_cast<const int8_t *>(c.w), 2 * c.w_stride, sc.at<int8_t>(copy_at), c.vocab}, none{};
-  const int chunks = static_cast<int>(*pitch / 8);
-  H24_CUDA_TRY(launch_pdl(repack_rows_kernel, dim3(wave_grid(cdiv(c.vocab * chunks, kRepackThreads), 8)),
-                          dim3(kRepackThreads), sc.s, rw, none, static_cast<int>(2 * c.in), chunks));
+  H24_CUDA_TRY(launch_pdl(ce_copy_head_kernel, dim3(wave_grid(cdiv(c.vocab, kRowThreads / 32), 8)), dim3(kRowThreads),
+                          sc.s, static_cast<const uint16_t *>(c.w), c.w_stride, c.vocab, static_cast<int>(c.in),
+                          sc.at<uint16_t>(copy_at), *pitch));
   count_launches(1);
   return H24_OK;
 }
@@ -1081,7 +1171,9 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   base.lse = st.lse;
   base.scale = r.scale;
   base.prob_scale = prob_scale;
-  base.wide_rows = dw && c.in % 16 == 0 && (reinterpret_cast<uintptr_t>(dw) & 31) == 0;
+  base.row_bytes = c.in % 16 == 0 && (reinterpret_cast<uintptr_t>(dw) & 31) == 0 ? 32
+                   : c.in % 8 == 0 && aligned16(dw)                              ? 16
+                                                                                 : 2;
   base.err = T->err;
   const int64_t rows_alloc = c.tokens + kTileK;
   const uint16_t *head_rows = r.scaled ? r.scaled : r.rows;

@@ -147,26 +147,14 @@ static __global__ void __launch_bounds__(kRepackThreads) repack_rows_kernel(cons
                                                                      int chunks) {
   pdl_enter();
   const int64_t total0 = a0.rows * chunks, total = total0 + a1.rows * chunks;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kRepackThreads;
-  // Two vectors' blocks in flight a thread.  [50257,1153] of 16 bits: 59 us one by one.
-  constexpr int U = 2;
-  for (int64_t i = blockIdx.x * static_cast<int64_t>(kRepackThreads) + threadIdx.x; i < total; i += U * step) {
-    uint4 v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t g = min(i + u * step, total - 1);
-      const RepackArgs &a = g < total0 ? a0 : a1;
-      const int64_t at = g < total0 ? g : g - total0;
-      const int64_t r = at <= 0xFFFFFFFFll ? static_cast<uint32_t>(at) / static_cast<uint32_t>(chunks) : at / chunks;
-      const int c = static_cast<int>(at - r * chunks) * 16;
-      const int8_t *hi = a.src + (a.rows - 1) * a.stride + cols;
-      v[u] = load16_any(a.src + r * a.stride + c, cols - c, a.src, hi);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t g = i + u * step;
-      if (g < total) reinterpret_cast<uint4 *>(g < total0 ? a0.dst : a1.dst)[g < total0 ? g : g - total0] = v[u];
-    }
+  for (int64_t i = blockIdx.x * static_cast<int64_t>(kRepackThreads) + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * kRepackThreads) {
+    const RepackArgs &a = i < total0 ? a0 : a1;
+    const int64_t at = i < total0 ? i : i - total0;
+    const int64_t r = at <= 0xFFFFFFFFll ? static_cast<uint32_t>(at) / static_cast<uint32_t>(chunks) : at / chunks;
+    const int c = static_cast<int>(at - r * chunks) * 16;
+    const int8_t *hi = a.src + (a.rows - 1) * a.stride + cols;
+    reinterpret_cast<uint4 *>(a.dst)[at] = load16_any(a.src + r * a.stride + c, cols - c, a.src, hi);
   }
 }
 
