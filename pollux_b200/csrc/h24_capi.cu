@@ -627,7 +627,8 @@ int h24_add_norm(const void *x, const void *residual, const void *gain, const vo
   if ((residual != nullptr) != (summed != nullptr)) return fail(H24_ERR_INVALID, "add_norm: summed goes with a residual");
   if (rows == 0) return H24_OK;
   if (!x || !y || !stats) return fail(H24_ERR_INVALID, "add_norm: null pointer");
-  return launch_add_norm({gain, param_dtype, layer != 0, rows, cols, dtype}, x, x_stride, residual, residual_stride, bias,
+  H24_TABLES_OR_FAIL(T);
+  return launch_add_norm(T, {gain, param_dtype, layer != 0, rows, cols, dtype}, x, x_stride, residual, residual_stride, bias,
                          eps, y, summed, stats, as_stream(stream));
 }
 

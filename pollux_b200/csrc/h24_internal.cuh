@@ -256,7 +256,7 @@ struct AddNormArgs {
   int64_t rows, cols;
   int dtype;
 };
-int launch_add_norm(const AddNormArgs &c, const void *x, int64_t x_stride, const void *residual, int64_t residual_stride,
+int launch_add_norm(const Tables *t, const AddNormArgs &c, const void *x, int64_t x_stride, const void *residual, int64_t residual_stride,
                     const void *bias, float eps, void *y, void *summed, float *stats, cudaStream_t s);
 int launch_add_norm_backward(const Tables *t, const AddNormArgs &c, const void *summed, int64_t summed_stride,
                              const float *stats, const void *dy, int64_t dy_stride, const void *dsummed,

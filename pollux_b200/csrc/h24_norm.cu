@@ -17,7 +17,7 @@
 // columns take a warp, of up to 16,384 a block.  In the backward pass a thread
 // keeps its columns for all of its rows and adds dw and db up in registers; the
 // blocks' sums meet in a second kernel, in a fixed order.
-#include "h24_internal.cuh"
+#include "h24_tile.cuh"
 
 namespace h24 {
 namespace {
@@ -75,9 +75,9 @@ struct BackArgs {
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
 
 // Thread t of a row's threads holds the columns of the vectors t, t + nt, ...
-template <int DT>
+template <int DT, int HOLD = kHold>
 struct Held {
-  static constexpr int VEC = Elem<DT>::kVec, NV = kHold / VEC;
+  static constexpr int VEC = Elem<DT>::kVec, NV = HOLD / VEC;
   uint4 raw[NV];
 
   template <bool kAligned>
@@ -98,20 +98,27 @@ struct Held {
       }
     }
   }
+  // The same columns of a row in shared memory.
+  __device__ __forceinline__ void take(const uint8_t *row, int t, int nt, int cols) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      raw[i] = (t + i * nt) * VEC < cols ? *reinterpret_cast<const uint4 *>(row + (t + i * nt) * 16)
+                                         : make_uint4(0, 0, 0, 0);
+  }
   __device__ __forceinline__ float get(int k) const {
     return Elem<DT>::up(reinterpret_cast<const typename Elem<DT>::T *>(&raw[k / VEC])[k % VEC]);
   }
 };
 
 // The held columns of a row to memory.
-template <int DT, bool kAligned>
-__device__ __forceinline__ void store_held(void *base, int64_t offset, const float (&v)[kHold], int t, int nt, int cols) {
+template <int DT, bool kAligned, int HOLD>
+__device__ __forceinline__ void store_held(void *base, int64_t offset, const float (&v)[HOLD], int t, int nt, int cols) {
   using E = Elem<DT>;
   using T = typename E::T;
   constexpr int VEC = E::kVec;
   T *p = static_cast<T *>(base) + offset;
 #pragma unroll
-  for (int i = 0; i < kHold / VEC; ++i) {
+  for (int i = 0; i < HOLD / VEC; ++i) {
     const int at = (t + i * nt) * VEC;
     alignas(16) T o[VEC];
 #pragma unroll
@@ -127,21 +134,21 @@ __device__ __forceinline__ void store_held(void *base, int64_t offset, const flo
 }
 
 // The held columns of a parameter vector as fp32 (0 past the end).
-template <int DT, bool kAligned>
-__device__ __forceinline__ void load_param(const void *param, bool f32, float (&v)[kHold], int t, int nt, int cols) {
+template <int DT, bool kAligned, int HOLD>
+__device__ __forceinline__ void load_param(const void *param, bool f32, float (&v)[HOLD], int t, int nt, int cols) {
   using E = Elem<DT>;
   using T = typename E::T;
   constexpr int VEC = E::kVec;
   if (!f32 || DT == H24_DTYPE_F32) {
-    Held<DT> h;
+    Held<DT, HOLD> h;
     h.template load<kAligned>(param, 0, t, nt, cols);
 #pragma unroll
-    for (int k = 0; k < kHold; ++k) v[k] = h.get(k);
+    for (int k = 0; k < HOLD; ++k) v[k] = h.get(k);
     return;
   }
   const float *p = static_cast<const float *>(param);
 #pragma unroll
-  for (int i = 0; i < kHold / VEC; ++i) {
+  for (int i = 0; i < HOLD / VEC; ++i) {
     const int at = (t + i * nt) * VEC;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) v[i * VEC + j] = at + j < cols ? __ldg(p + at + j) : 0.f;
@@ -155,18 +162,29 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 // Sums over a row's threads: a warp, or the block (`red` is not used again
-// before a barrier that all of its threads pass).
+// before a barrier that all of its threads pass).  Each warp adds up the warps'
+// sums across its lanes: one after the other they cost 30 reads of shared memory.
 template <bool kWarp>
 __device__ __forceinline__ float row_sum(float v, float *red) {
   v = warp_sum(v);
   if (kWarp) return v;
-  const int warps = blockDim.x >> 5;
-  if (warps == 1) return v;
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = 0.f;
-  for (int w = 0; w < warps; ++w) v += red[w];
-  return v;
+  return warp_sum(lane < (blockDim.x >> 5) ? red[lane] : 0.f);
+}
+// Two sums behind one barrier.
+template <bool kWarp>
+__device__ __forceinline__ void row_sums(float &v, float &w, float (*red)[32]) {
+  v = warp_sum(v);
+  w = warp_sum(w);
+  if (kWarp) return;
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) red[0][threadIdx.x >> 5] = v, red[1][threadIdx.x >> 5] = w;
+  __syncthreads();
+  const bool live = lane < (blockDim.x >> 5);
+  v = warp_sum(live ? red[0][lane] : 0.f);
+  w = warp_sum(live ? red[1][lane] : 0.f);
 }
 
 // The finite rows among those whose statistics passed fp32's range, again and
@@ -218,7 +236,7 @@ __device__ __noinline__ void wide_rows(const NormArgs &a, float (*red)[32]) {
   }
 }
 
-template <int DT, bool kAligned, bool kLayer, bool kWarp, int kMax>
+template <int DT, bool kAligned, bool kLayer, bool kWarp, int kMax, int HOLD>
 __global__ void __launch_bounds__(kMax) norm_kernel(const __grid_constant__ NormArgs a) {
   __shared__ float red[2][3][32];
   pdl_enter();
@@ -228,7 +246,7 @@ __global__ void __launch_bounds__(kMax) norm_kernel(const __grid_constant__ Norm
   const int64_t step = kWarp ? static_cast<int64_t>(gridDim.x) * kWarpRows : gridDim.x;
   const float n_cols = static_cast<float>(cols);
   constexpr int VEC = Elem<DT>::kVec;
-  Held<DT> x, res;
+  Held<DT, HOLD> x, res;
   auto ask = [&](int64_t r) {
     if (r >= a.rows) return;
     x.template load<kAligned>(a.x, r * a.x_stride, t, nt, cols);
@@ -237,24 +255,24 @@ __global__ void __launch_bounds__(kMax) norm_kernel(const __grid_constant__ Norm
   ask(first);
   int turn = 0;
   for (int64_t r = first; r < a.rows; r += step, turn ^= 1) {
-    float v[kHold];
+    float v[HOLD];
 #pragma unroll
-    for (int k = 0; k < kHold; ++k) v[k] = x.get(k);
+    for (int k = 0; k < HOLD; ++k) v[k] = x.get(k);
     if (a.residual) {
 #pragma unroll
-      for (int k = 0; k < kHold; ++k) v[k] = Elem<DT>::up(Elem<DT>::down(v[k] + res.get(k)));
+      for (int k = 0; k < HOLD; ++k) v[k] = Elem<DT>::up(Elem<DT>::down(v[k] + res.get(k)));
     }
     ask(r + step);
-    if (a.summed) store_held<DT, kAligned>(a.summed, r * a.cols, v, t, nt, cols);
+    if (a.summed) store_held<DT, kAligned, HOLD>(a.summed, r * a.cols, v, t, nt, cols);
     float mean = 0.f, ss = 0.f;
     if (kLayer) {
       float sum = 0.f;
 #pragma unroll
-      for (int k = 0; k < kHold; ++k) sum += v[k];
+      for (int k = 0; k < HOLD; ++k) sum += v[k];
       mean = row_sum<kWarp>(sum, red[turn][0]) / n_cols;
     }
 #pragma unroll
-    for (int k = 0; k < kHold; ++k) {
+    for (int k = 0; k < HOLD; ++k) {
       if (kLayer) {
         const int at = (t + k / VEC * nt) * VEC + k % VEC;
         v[k] = at < cols ? v[k] - mean : 0.f;
@@ -263,16 +281,16 @@ __global__ void __launch_bounds__(kMax) norm_kernel(const __grid_constant__ Norm
     }
     ss = row_sum<kWarp>(ss, red[turn][1]);
     const float inv = 1.0f / sqrtf(ss / n_cols + a.eps);
-    float w[kHold];
-    load_param<DT, kAligned>(a.gain, a.gain_f32, w, t, nt, cols);
+    float w[HOLD];
+    load_param<DT, kAligned, HOLD>(a.gain, a.gain_f32, w, t, nt, cols);
 #pragma unroll
-    for (int k = 0; k < kHold; ++k) v[k] = v[k] * inv * w[k];
+    for (int k = 0; k < HOLD; ++k) v[k] = v[k] * inv * w[k];
     if (kLayer && a.bias) {
-      load_param<DT, kAligned>(a.bias, a.gain_f32, w, t, nt, cols);
+      load_param<DT, kAligned, HOLD>(a.bias, a.gain_f32, w, t, nt, cols);
 #pragma unroll
-      for (int k = 0; k < kHold; ++k) v[k] += w[k];
+      for (int k = 0; k < HOLD; ++k) v[k] += w[k];
     }
-    store_held<DT, kAligned>(a.y, r * a.cols, v, t, nt, cols);
+    store_held<DT, kAligned, HOLD>(a.y, r * a.cols, v, t, nt, cols);
     if (t == 0) {
       a.inv[r] = inv;
       if (kLayer) a.mean[r] = mean;
@@ -285,6 +303,134 @@ __global__ void __launch_bounds__(kMax) norm_kernel(const __grid_constant__ Norm
     __syncthreads();
     for (int64_t r = first + t * step; r < a.rows; r += nt * step) marked |= !(a.inv[r] > 0.f && finite(a.inv[r]));
     if (__syncthreads_or(marked)) wide_rows<DT, kLayer, kWarp>(a, red[0]);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Rows through a ring in shared memory
+// ---------------------------------------------------------------------------
+// Rows of 513 to 8,192 columns on 16 bytes: one thread keeps the next rows on
+// their way (bulk copies into a ring of stages, each with a row of every input),
+// so that the loads of a block do not wait for its sums; a thread holds 8
+// columns.  RING1, RING2
+constexpr int kRingHold = 8, kRingCols = 1024 * kRingHold, kMaxRing = 8;
+constexpr int kRingHead = 128;  // barriers
+constexpr int kRingSmem = 220 * 1024;  // of an SM, for the rings of its blocks
+
+struct Ring {
+  uint8_t *rows;    // stage s, input i: rows + (s * inputs + i) * pitch
+  uint64_t *full;
+  int stages, inputs, pitch;
+  uint32_t bytes;   // of a row
+};
+
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(su32(dst)),
+               "l"(src), "r"(bytes), "r"(su32(bar))
+               : "memory");
+}
+
+struct RingInput {
+  const uint8_t *base;
+  int64_t stride;  // bytes
+};
+// Row r of every input on its way to stage s, by one thread.
+template <int N>
+__device__ __forceinline__ void ring_ask(const Ring &g, const RingInput (&in)[N], int s, int64_t r) {
+  bar_expect(&g.full[s], g.inputs * g.bytes);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < g.inputs) bulk_load(g.rows + (s * g.inputs + i) * g.pitch, in[i].base + r * in[i].stride, g.bytes, &g.full[s]);
+}
+
+template <int N>
+__device__ __forceinline__ Ring ring_start(uint8_t *smem, int stages, int inputs, int64_t cols, int size,
+                                           const RingInput (&in)[N], int64_t rows) {
+  Ring g;
+  g.full = reinterpret_cast<uint64_t *>(smem);
+  g.rows = smem + kRingHead;
+  g.stages = stages;
+  g.inputs = inputs;
+  g.bytes = static_cast<uint32_t>(cols * size);
+  g.pitch = static_cast<int>((g.bytes + 127) / 128 * 128);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) bar_init(&g.full[s], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  __syncthreads();
+  pdl_enter();
+  if (threadIdx.x == 0) {
+    asm volatile("fence.proxy.async;" ::: "memory");  // the rows were written by ordinary stores
+    for (int s = 0; s < stages && blockIdx.x + static_cast<int64_t>(s) * gridDim.x < rows; ++s)
+      ring_ask(g, in, s, blockIdx.x + static_cast<int64_t>(s) * gridDim.x);
+  }
+  return g;
+}
+
+template <int DT, bool kLayer, int kMax>
+__global__ void __launch_bounds__(kMax) norm_ring_kernel(const __grid_constant__ NormArgs a, int stages, int *err) {
+  extern __shared__ __align__(128) uint8_t norm_smem[];
+  __shared__ float red[2][3][32];
+  __shared__ int abort;
+  constexpr int VEC = Elem<DT>::kVec, SIZE = 16 / VEC;
+  const int t = threadIdx.x, nt = blockDim.x;
+  const int cols = static_cast<int>(a.cols);
+  const int64_t step = gridDim.x;
+  const float n_cols = static_cast<float>(cols);
+  if (t == 0) abort = 0;
+  const RingInput in[2] = {{static_cast<const uint8_t *>(a.x), a.x_stride * SIZE},
+                           {static_cast<const uint8_t *>(a.residual), a.residual_stride * SIZE}};
+  const Ring g = ring_start(norm_smem, stages, a.residual ? 2 : 1, a.cols, SIZE, in, a.rows);
+  float w[kRingHold], b[kRingHold] = {};
+  load_param<DT, true, kRingHold>(a.gain, a.gain_f32, w, t, nt, cols);
+  if (kLayer && a.bias) load_param<DT, true, kRingHold>(a.bias, a.gain_f32, b, t, nt, cols);
+  int turn = 0, s = 0;
+  uint32_t ph = 0;
+  for (int64_t r = blockIdx.x; r < a.rows; r += step, turn ^= 1) {
+    if (!bar_wait(&g.full[s], ph, &abort, err, false)) break;
+    Held<DT, kRingHold> x, res;
+    const uint8_t *row = g.rows + s * g.inputs * g.pitch;
+    x.take(row, t, nt, cols);
+    float v[kRingHold];
+#pragma unroll
+    for (int k = 0; k < kRingHold; ++k) v[k] = x.get(k);
+    if (a.residual) {
+      res.take(row + g.pitch, t, nt, cols);
+#pragma unroll
+      for (int k = 0; k < kRingHold; ++k) v[k] = Elem<DT>::up(Elem<DT>::down(v[k] + res.get(k)));
+      store_held<DT, true, kRingHold>(a.summed, r * a.cols, v, t, nt, cols);
+    }
+    float mean = 0.f, ss = 0.f;
+    if (kLayer) {
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < kRingHold; ++k) sum += v[k];
+      mean = row_sum<false>(sum, red[turn][0]) / n_cols;
+    }
+#pragma unroll
+    for (int k = 0; k < kRingHold; ++k) {
+      if (kLayer) v[k] = (t + k / VEC * nt) * VEC < cols ? v[k] - mean : 0.f;
+      ss = fmaf(v[k], v[k], ss);
+    }
+    ss = row_sum<false>(ss, red[turn][1]);
+    // All threads have taken their columns: the stage is free.
+    if (t == 0 && r + stages * step < a.rows) ring_ask(g, in, s, r + stages * step);
+    if (++s == stages) s = 0, ph ^= 1;
+    const float inv = 1.0f / sqrtf(ss / n_cols + a.eps);
+#pragma unroll
+    for (int k = 0; k < kRingHold; ++k) v[k] = kLayer ? v[k] * inv * w[k] + b[k] : v[k] * inv * w[k];
+    store_held<DT, true, kRingHold>(a.y, r * a.cols, v, t, nt, cols);
+    if (t == 0) {
+      a.inv[r] = inv;
+      if (kLayer) a.mean[r] = mean;
+    }
+  }
+  if (DT != H24_DTYPE_F16) {
+    bool marked = false;
+    __syncthreads();
+    for (int64_t r = blockIdx.x + t * step; r < a.rows; r += nt * step) marked |= !(a.inv[r] > 0.f && finite(a.inv[r]));
+    if (__syncthreads_or(marked)) wide_rows<DT, kLayer, false>(a, red[0]);
   }
 }
 
@@ -345,7 +491,7 @@ __device__ __forceinline__ RowScale row_scale(const BackArgs &a, int64_t r) {
   return {fabsf(i), i < 0.f ? kSmall : 1.f, kLayer ? __ldg(a.mean + r) : 0.f};
 }
 
-template <int DT, bool kAligned, bool kLayer, bool kWarp, int kMax>
+template <int DT, bool kAligned, bool kLayer, bool kWarp, int kMax, int HOLD>
 __global__ void __launch_bounds__(kMax) norm_back_kernel(const __grid_constant__ BackArgs a) {
   __shared__ float red[2][2][32];
   __shared__ float held[kWarp ? kWarpRows * kWarpCols : 1];
@@ -356,19 +502,19 @@ __global__ void __launch_bounds__(kMax) norm_back_kernel(const __grid_constant__
   const int64_t step = kWarp ? static_cast<int64_t>(gridDim.x) * kWarpRows : gridDim.x;
   const float one_over = 1.0f / static_cast<float>(cols);
   constexpr int VEC = Elem<DT>::kVec;
-  float dw[kHold] = {}, db[kHold] = {};
+  float dw[HOLD] = {}, db[HOLD] = {};
   int turn = 0;
   for (int64_t r = first; r < a.rows; r += step, turn ^= 1) {
-    Held<DT> s, dy, ds;
+    Held<DT, HOLD> s, dy, ds;
     s.template load<kAligned>(a.s, r * a.s_stride, t, nt, cols);
     dy.template load<kAligned>(a.dy, r * a.dy_stride, t, nt, cols);
     if (a.dsummed) ds.template load<kAligned>(a.dsummed, r * a.dsummed_stride, t, nt, cols);
     const RowScale sc = row_scale<kLayer>(a, r);
-    float n[kHold], v[kHold];
-    load_param<DT, kAligned>(a.gain, a.gain_f32, v, t, nt, cols);
+    float n[HOLD], v[HOLD];
+    load_param<DT, kAligned, HOLD>(a.gain, a.gain_f32, v, t, nt, cols);
     float c1 = 0.f, c2 = 0.f;
 #pragma unroll
-    for (int k = 0; k < kHold; ++k) {
+    for (int k = 0; k < HOLD; ++k) {
       const float g = dy.get(k);
       n[k] = fmaf(s.get(k), sc.k, -sc.shift) * sc.inv;
       dw[k] = fmaf(g, n[k], dw[k]);
@@ -378,23 +524,24 @@ __global__ void __launch_bounds__(kMax) norm_back_kernel(const __grid_constant__
       if (kLayer) c2 += v[k];
     }
     if (a.dx) {
-      c1 = row_sum<kWarp>(c1, red[turn][0]) * one_over;
-      if (kLayer) c2 = row_sum<kWarp>(c2, red[turn][1]) * one_over;
+      if (kLayer) row_sums<kWarp>(c1, c2, red[turn]);
+      else c1 = row_sum<kWarp>(c1, red[turn][0]);
+      c1 *= one_over, c2 *= one_over;
 #pragma unroll
-      for (int k = 0; k < kHold; ++k) {
+      for (int k = 0; k < HOLD; ++k) {
         v[k] = (fmaf(-n[k], c1, v[k]) - c2) * sc.inv * sc.k;
         if (a.dsummed) v[k] += ds.get(k);
       }
-      store_held<DT, kAligned>(a.dx, r * a.cols, v, t, nt, cols);
+      store_held<DT, kAligned, HOLD>(a.dx, r * a.cols, v, t, nt, cols);
     }
   }
   // The sums of this block.
-  auto put = [&](float *out, float (&sum)[kHold]) {
+  auto put = [&](float *out, float (&sum)[HOLD]) {
     if (!out) return;
     float *o = out + static_cast<int64_t>(blockIdx.x) * a.cols;
     if (!kWarp) {
 #pragma unroll
-      for (int k = 0; k < kHold; ++k) {
+      for (int k = 0; k < HOLD; ++k) {
         const int at = (t + k / VEC * nt) * VEC + k % VEC;
         if (at < cols) o[at] = sum[k];
       }
@@ -402,7 +549,7 @@ __global__ void __launch_bounds__(kMax) norm_back_kernel(const __grid_constant__
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kHold; ++k)
+    for (int k = 0; k < HOLD; ++k)
       held[(threadIdx.x >> 5) * kWarpCols + (t + k / VEC * 32) * VEC + k % VEC] = sum[k];
     __syncthreads();
     for (int c = threadIdx.x; c < cols; c += 32 * kWarpRows) {
@@ -410,6 +557,75 @@ __global__ void __launch_bounds__(kMax) norm_back_kernel(const __grid_constant__
 #pragma unroll
       for (int w = 0; w < kWarpRows; ++w) total += held[w * kWarpCols + c];
       o[c] = total;
+    }
+  };
+  put(a.dgain, dw);
+  if (kLayer) put(a.dbias, db);
+}
+
+template <int DT, bool kLayer, int kMax>
+__global__ void __launch_bounds__(kMax) norm_back_ring_kernel(const __grid_constant__ BackArgs a, int stages, int *err) {
+  extern __shared__ __align__(128) uint8_t norm_smem[];
+  __shared__ float red[2][2][32];
+  __shared__ int abort;
+  constexpr int VEC = Elem<DT>::kVec, SIZE = 16 / VEC;
+  const int t = threadIdx.x, nt = blockDim.x;
+  const int cols = static_cast<int>(a.cols);
+  const int64_t step = gridDim.x;
+  const float one_over = 1.0f / static_cast<float>(cols);
+  if (t == 0) abort = 0;
+  const RingInput in[3] = {{static_cast<const uint8_t *>(a.s), a.s_stride * SIZE},
+                           {static_cast<const uint8_t *>(a.dy), a.dy_stride * SIZE},
+                           {static_cast<const uint8_t *>(a.dsummed), a.dsummed_stride * SIZE}};
+  const Ring g = ring_start(norm_smem, stages, a.dsummed ? 3 : 2, a.cols, SIZE, in, a.rows);
+  float w[kRingHold], dw[kRingHold] = {}, db[kRingHold] = {};
+  load_param<DT, true, kRingHold>(a.gain, a.gain_f32, w, t, nt, cols);
+  int turn = 0, st = 0;
+  uint32_t ph = 0;
+  RowScale next = {};
+  if (blockIdx.x < a.rows) next = row_scale<kLayer>(a, blockIdx.x);
+  for (int64_t r = blockIdx.x; r < a.rows; r += step, turn ^= 1) {
+    const RowScale sc = next;
+    if (r + step < a.rows) next = row_scale<kLayer>(a, r + step);
+    if (!bar_wait(&g.full[st], ph, &abort, err, false)) break;
+    Held<DT, kRingHold> s, dy, ds;
+    const uint8_t *row = g.rows + st * g.inputs * g.pitch;
+    s.take(row, t, nt, cols);
+    dy.take(row + g.pitch, t, nt, cols);
+    if (a.dsummed) ds.take(row + 2 * g.pitch, t, nt, cols);
+    float n[kRingHold], v[kRingHold], c1 = 0.f, c2 = 0.f;
+#pragma unroll
+    for (int k = 0; k < kRingHold; ++k) {
+      const float d = dy.get(k);
+      n[k] = fmaf(s.get(k), sc.k, -sc.shift) * sc.inv;
+      dw[k] = fmaf(d, n[k], dw[k]);
+      if (kLayer) db[k] += d;
+      v[k] = w[k] * d;  // (0 past the row's end)
+      c1 = fmaf(v[k], n[k], c1);
+      if (kLayer) c2 += v[k];
+    }
+    // (The sums' barrier also says that the stage is free.)
+    if (kLayer) row_sums<false>(c1, c2, red[turn]);
+    else c1 = row_sum<false>(c1, red[turn][0]);
+    c1 *= one_over, c2 *= one_over;
+    if (t == 0 && r + stages * step < a.rows) ring_ask(g, in, st, r + stages * step);
+    if (++st == stages) st = 0, ph ^= 1;
+    if (a.dx) {
+#pragma unroll
+      for (int k = 0; k < kRingHold; ++k) {
+        v[k] = (fmaf(-n[k], c1, v[k]) - c2) * sc.inv * sc.k;
+        if (a.dsummed) v[k] += ds.get(k);
+      }
+      store_held<DT, true, kRingHold>(a.dx, r * a.cols, v, t, nt, cols);
+    }
+  }
+  auto put = [&](float *out, const float (&sum)[kRingHold]) {
+    if (!out) return;
+    float *o = out + static_cast<int64_t>(blockIdx.x) * a.cols;
+#pragma unroll
+    for (int k = 0; k < kRingHold; k += 4) {
+      const int at = (t + k / VEC * nt) * VEC + k % VEC;
+      if (at < cols) *reinterpret_cast<float4 *>(o + at) = make_float4(sum[k], sum[k + 1], sum[k + 2], sum[k + 3]);
     }
   };
   put(a.dgain, dw);
@@ -437,8 +653,8 @@ __global__ void __launch_bounds__(kLongThreads) norm_back_long_kernel(const __gr
     c1 = fmaf(v, fmaf(E::up(s[c]), sc.k, -sc.shift) * sc.inv, c1);
     if (kLayer) c2 += v;
   }
-  c1 = row_sum<false>(c1, red[0]) * one_over;
-  if (kLayer) c2 = row_sum<false>(c2, red[1]) * one_over;
+  row_sums<false>(c1, c2, red);
+  c1 *= one_over, c2 *= one_over;
   for (int64_t c = threadIdx.x; c < a.cols; c += kLongThreads) {
     const float n = fmaf(E::up(s[c]), sc.k, -sc.shift) * sc.inv;
     float d = (fmaf(-n, c1, E::up(dy[c]) * gain(c)) - c2) * sc.inv * sc.k;
@@ -479,7 +695,7 @@ __global__ void __launch_bounds__(kSumCols * kSumGroups) norm_sums_kernel(const 
   const int64_t c = blockIdx.x * static_cast<int64_t>(kSumCols) + x;
   float sum = 0.f;
   if (in && c < cols) {
-#pragma unroll 4
+#pragma unroll 8
     for (int p = g; p < parts; p += kSumGroups) sum += __ldcs(in + p * cols + c);
   }
   red[g][x] = sum;
@@ -499,10 +715,13 @@ __global__ void __launch_bounds__(kSumCols * kSumGroups) norm_sums_kernel(const 
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
-// Threads of a block.  (A kernel that is compiled for 1,024 has too few
-// registers for what a thread holds in the backward pass.)
+// Columns of a thread and threads of a block.  They go by the columns alone, and
+// whether a row comes through the ring or not, its sums have the same order: a
+// row's result does not depend on where it lies.
 int row_threads(int64_t cols) {
-  return cols <= kWarpCols ? 32 * kWarpRows : static_cast<int>(((cols + kHold - 1) / kHold + 31) / 32 * 32);
+  if (cols <= kWarpCols) return 32 * kWarpRows;
+  const int hold = cols <= kRingCols ? kRingHold : kHold;
+  return static_cast<int>(((cols + hold - 1) / hold + 31) / 32 * 32);
 }
 template <auto kernel>
 int norm_grid(int64_t rows, int64_t cols, int threads) {
@@ -514,16 +733,50 @@ int launch_norm_rows(const NormArgs &a, int threads, cudaStream_t s) {
   count_launches(1);
   return H24_OK;
 }
-template <int DT, bool kAligned, bool kLayer>
-int launch_norm_width(const NormArgs &a, cudaStream_t s) {
-  const int threads = row_threads(a.cols);
-  if (a.cols <= kWarpCols) return launch_norm_rows<norm_kernel<DT, kAligned, kLayer, true, 32 * kWarpRows>>(a, threads, s);
-  if (threads <= 512) return launch_norm_rows<norm_kernel<DT, kAligned, kLayer, false, 512>>(a, threads, s);
-  return launch_norm_rows<norm_kernel<DT, kAligned, kLayer, false, 1024>>(a, threads, s);
+
+// Stages of a ring and blocks an SM: about 200 KB of rows on their way, in
+// blocks of what the registers of an SM hold, two stages at least.
+struct RingPlan {
+  int threads, stages, smem, grid;
+};
+template <auto kernel>
+int ring_plan(int64_t rows, int64_t cols, int size, int inputs, RingPlan *p) {
+  H24_CUDA_TRY(allow_smem<kernel>(kRingSmem));
+  p->threads = row_threads(cols);
+  const int one = static_cast<int>((cols * size + 127) / 128 * 128) * inputs;
+  int per_sm = blocks_per_sm_once<kernel>(p->threads);
+  while (per_sm > 1 && kRingSmem / per_sm < kRingHead + 2 * one) --per_sm;
+  p->stages = (kRingSmem / per_sm - kRingHead - 1024) / one;
+  p->stages = p->stages < 1 ? 1 : p->stages > kMaxRing ? kMaxRing : p->stages;
+  p->smem = kRingHead + p->stages * one;
+  p->grid = wave_grid(rows, per_sm);
+  return H24_OK;
+}
+template <typename K, typename Args>
+int launch_ring(K kernel, const Args &a, const RingPlan &p, int *err, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.grid);
+  cfg.blockDim = dim3(p.threads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(p.smem);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  H24_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, p.stages, err));
+  count_launches(1);
+  return H24_OK;
+}
+template <auto kernel, int DT>
+int run_norm_ring(const Tables *T, const NormArgs &a, cudaStream_t s) {
+  RingPlan p;
+  const int rc = ring_plan<kernel>(a.rows, a.cols, 16 / Elem<DT>::kVec, a.residual ? 2 : 1, &p);
+  return rc != H24_OK ? rc : launch_ring(kernel, a, p, T->err, s);
 }
 
 template <int DT, bool kLayer>
-int launch_norm_typed(const NormArgs &a, cudaStream_t s) {
+int launch_norm_typed(const Tables *T, const NormArgs &a, cudaStream_t s) {
   constexpr int kVec = Elem<DT>::kVec;
   if (a.cols > kBlockCols) {
     H24_CUDA_TRY(launch_pdl(norm_long_kernel<DT, kLayer>, dim3(static_cast<unsigned>(a.rows)), dim3(kLongThreads), s, a));
@@ -532,7 +785,18 @@ int launch_norm_typed(const NormArgs &a, cudaStream_t s) {
   }
   const bool aligned = a.cols % kVec == 0 && a.x_stride % kVec == 0 && a.residual_stride % kVec == 0 && aligned16(a.x) &&
                        aligned16(a.residual) && aligned16(a.summed) && aligned16(a.y) && aligned16(a.gain) && aligned16(a.bias);
-  return aligned ? launch_norm_width<DT, true, kLayer>(a, s) : launch_norm_width<DT, false, kLayer>(a, s);
+  const int threads = row_threads(a.cols);
+  if (a.cols <= kWarpCols)
+    return aligned ? launch_norm_rows<norm_kernel<DT, true, kLayer, true, 32 * kWarpRows, kHold>>(a, threads, s)
+                   : launch_norm_rows<norm_kernel<DT, false, kLayer, true, 32 * kWarpRows, kHold>>(a, threads, s);
+  if (a.cols > kRingCols)
+    return aligned ? launch_norm_rows<norm_kernel<DT, true, kLayer, false, 1024, kHold>>(a, threads, s)
+                   : launch_norm_rows<norm_kernel<DT, false, kLayer, false, 1024, kHold>>(a, threads, s);
+  if (threads <= 512)
+    return aligned ? run_norm_ring<norm_ring_kernel<DT, kLayer, 512>, DT>(T, a, s)
+                   : launch_norm_rows<norm_kernel<DT, false, kLayer, false, 512, kRingHold>>(a, threads, s);
+  return aligned ? run_norm_ring<norm_ring_kernel<DT, kLayer, 1024>, DT>(T, a, s)
+                 : launch_norm_rows<norm_kernel<DT, false, kLayer, false, 1024, kRingHold>>(a, threads, s);
 }
 
 // The backward kernel of rows that a block holds: its grid (one wave; asked for
@@ -547,13 +811,27 @@ int back_rows(const BackArgs &a, int grid, int threads, int *ask, cudaStream_t s
   count_launches(1);
   return H24_OK;
 }
-template <int DT, bool kAligned, bool kLayer>
-int back_width(const BackArgs &a, int grid, int *ask, cudaStream_t s) {
+template <auto kernel, int DT>
+int back_ring(const Tables *T, const BackArgs &a, int *ask, cudaStream_t s) {
+  RingPlan p;
+  const int rc = ring_plan<kernel>(a.rows, a.cols, 16 / Elem<DT>::kVec, a.dsummed ? 3 : 2, &p);
+  if (rc == H24_OK && ask) *ask = p.grid;
+  return rc != H24_OK || ask ? rc : launch_ring(kernel, a, p, T->err, s);
+}
+template <int DT, bool kLayer>
+int back_width(const Tables *T, const BackArgs &a, bool aligned, int grid, int *ask, cudaStream_t s) {
   const int threads = row_threads(a.cols);
   if (a.cols <= kWarpCols)
-    return back_rows<norm_back_kernel<DT, kAligned, kLayer, true, 32 * kWarpRows>>(a, grid, threads, ask, s);
-  if (threads <= 512) return back_rows<norm_back_kernel<DT, kAligned, kLayer, false, 512>>(a, grid, threads, ask, s);
-  return back_rows<norm_back_kernel<DT, kAligned, kLayer, false, 1024>>(a, grid, threads, ask, s);
+    return aligned ? back_rows<norm_back_kernel<DT, true, kLayer, true, 32 * kWarpRows, kHold>>(a, grid, threads, ask, s)
+                   : back_rows<norm_back_kernel<DT, false, kLayer, true, 32 * kWarpRows, kHold>>(a, grid, threads, ask, s);
+  if (a.cols > kRingCols)
+    return aligned ? back_rows<norm_back_kernel<DT, true, kLayer, false, 1024, kHold>>(a, grid, threads, ask, s)
+                   : back_rows<norm_back_kernel<DT, false, kLayer, false, 1024, kHold>>(a, grid, threads, ask, s);
+  if (threads <= 512)
+    return aligned ? back_ring<norm_back_ring_kernel<DT, kLayer, 512>, DT>(T, a, ask, s)
+                   : back_rows<norm_back_kernel<DT, false, kLayer, false, 512, kRingHold>>(a, grid, threads, ask, s);
+  return aligned ? back_ring<norm_back_ring_kernel<DT, kLayer, 1024>, DT>(T, a, ask, s)
+                 : back_rows<norm_back_kernel<DT, false, kLayer, false, 1024, kRingHold>>(a, grid, threads, ask, s);
 }
 
 template <int DT, bool kLayer>
@@ -566,10 +844,13 @@ int launch_back_typed(const Tables *T, BackArgs a, void *dgain, void *dbias, cud
                        aligned16(a.dx) && aligned16(a.gain);
   const int64_t col_blocks = (a.cols + 255) / 256;
   auto rows = [&](int grid, int *ask) {
-    return aligned ? back_width<DT, true, kLayer>(a, grid, ask, s) : back_width<DT, false, kLayer>(a, grid, ask, s);
+    return back_width<DT, kLayer>(T, a, aligned, grid, ask, s);
   };
   int grid = static_cast<int>(wave_grid(a.rows, 8) / col_blocks + 1);
-  if (!is_long) rows(0, &grid);
+  if (!is_long) {
+    const int rc = rows(0, &grid);
+    if (rc != H24_OK) return rc;
+  }
   float *parts = nullptr;
   if (sums) {
     const size_t one = static_cast<size_t>(grid) * static_cast<size_t>(a.cols);
@@ -618,14 +899,14 @@ int launch_back_typed(const Tables *T, BackArgs a, void *dgain, void *dbias, cud
 
 }  // namespace
 
-int launch_add_norm(const AddNormArgs &c, const void *x, int64_t x_stride, const void *residual, int64_t residual_stride,
+int launch_add_norm(const Tables *T, const AddNormArgs &c, const void *x, int64_t x_stride, const void *residual, int64_t residual_stride,
                     const void *bias, float eps, void *y, void *summed, float *stats, cudaStream_t s) {
   const NormArgs a{x, residual, c.gain, bias, c.rows, c.cols, x_stride, residual ? residual_stride : 0, eps,
                    c.param_dtype == H24_DTYPE_F32, y, summed, stats, stats + c.rows};
   switch (c.dtype) {
-    case H24_DTYPE_F32: return c.layer ? launch_norm_typed<H24_DTYPE_F32, true>(a, s) : launch_norm_typed<H24_DTYPE_F32, false>(a, s);
-    case H24_DTYPE_F16: return c.layer ? launch_norm_typed<H24_DTYPE_F16, true>(a, s) : launch_norm_typed<H24_DTYPE_F16, false>(a, s);
-    default: return c.layer ? launch_norm_typed<H24_DTYPE_BF16, true>(a, s) : launch_norm_typed<H24_DTYPE_BF16, false>(a, s);
+    case H24_DTYPE_F32: return c.layer ? launch_norm_typed<H24_DTYPE_F32, true>(T, a, s) : launch_norm_typed<H24_DTYPE_F32, false>(T, a, s);
+    case H24_DTYPE_F16: return c.layer ? launch_norm_typed<H24_DTYPE_F16, true>(T, a, s) : launch_norm_typed<H24_DTYPE_F16, false>(T, a, s);
+    default: return c.layer ? launch_norm_typed<H24_DTYPE_BF16, true>(T, a, s) : launch_norm_typed<H24_DTYPE_BF16, false>(T, a, s);
   }
 }
 
