@@ -55,8 +55,9 @@ enum Kind { kLoss, kProb, kStates, kHeadRows };
 // tokens, which only the device knows.
 struct Job {
   int kind;
+  bool swap;         // the weights' rows (kStates: columns) are the tile's rows, the tokens, at most 128, its columns
   int n_total, bn;   // columns, of which a tile takes bn
-  int m_total;       // rows (kHeadRows); the other kinds' rows are the tokens
+  int m_total;       // rows (kHeadRows, swap); the other kinds' rows are the tokens
   int k_total;       // length of the sum (kHeadRows: the tokens)
   int split;         // slices of the sum, each with its own output (kStates)
   int v0;            // first vocabulary row of the piece
@@ -71,8 +72,7 @@ struct GemmArgs {
   Job job[kMaxJobs];
   int jobs;
   int vocab;
-  int a_rows;          // rows of a CTA's share of the tokens' tiles that are loaded
-  int stages, stage_a; // of the ring; bytes of A in a stage
+  int stages, stage_a, stage_b;  // of the ring; bytes of A and of B in a stage
   const int *kept;     // number of tokens with a loss
   const int *target;   // of each kept token
   const float *lse;    // of each kept token
@@ -123,8 +123,13 @@ struct Tile {
   int kb, nkb, slice;   // k blocks
 };
 
+__device__ __forceinline__ bool rows_known(const Job &j) { return j.kind == kHeadRows || j.swap; }
+__device__ __forceinline__ bool a_is_mn(const Job &j) { return j.kind == kHeadRows || (j.swap && j.kind == kStates); }
+__device__ __forceinline__ bool b_is_mn(const Job &j) { return j.kind == kHeadRows || (!j.swap && j.kind == kStates); }
+
 __device__ __forceinline__ int tiles_of(const Job &j, int kept) {
-  const int rows = j.kind == kHeadRows ? j.m_total : kept;
+  if (j.swap && kept == 0) return 0;
+  const int rows = rows_known(j) ? j.m_total : kept;
   return (rows + kTileM - 1) / kTileM * ((j.n_total + j.bn - 1) / j.bn) * j.split;
 }
 
@@ -138,7 +143,7 @@ __device__ __forceinline__ Tile tile_at(const GemmArgs &a, int kept, int idx) {
   }
   const Job &j = a.job[t.job];
   const int nt = (j.n_total + j.bn - 1) / j.bn;
-  const int mt = ((j.kind == kHeadRows ? j.m_total : kept) + kTileM - 1) / kTileM;
+  const int mt = ((rows_known(j) ? j.m_total : kept) + kTileM - 1) / kTileM;
   int m, n;
   t.slice = 0;
   if (j.kind == kLoss || j.kind == kProb) {
@@ -298,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
   const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
   const int rank = static_cast<int>(blockIdx.x) & 1;
   const int first = static_cast<int>(blockIdx.x) >> 1, step = static_cast<int>(gridDim.x) >> 1;
-  const int stage_bytes = a.stage_a + kOperand;
+  const int stage_bytes = a.stage_a + a.stage_b;
   volatile int *abort = &H.abort;
 
   if (t == 0) {
@@ -341,11 +346,11 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
         const Job &j = a.job[tl.job];
         const CUtensorMap *ma = &a.map[2 * tl.job], *mb = ma + 1;
         const int half = tl.cols / 2, chunks = (half + kChunk - 1) / kChunk;
-        const bool a_mn = j.kind == kHeadRows, b_mn = j.kind == kStates || j.kind == kHeadRows;
-        // (The second CTA of a pair loads no tokens' rows where the first has room for all.)
-        const bool load_a = a_mn || a.a_rows == kTileM / 2 || rank == 0;
-        const uint32_t bytes_a = a_mn || a.a_rows == kTileM / 2 ? 2 * kOperand : a.a_rows * kTileK * 2;
-        const uint32_t bytes = bytes_a + 2 * (b_mn ? chunks * kBox : j.bn / 2 * 2 * kTileK);
+        const bool a_mn = a_is_mn(j), b_mn = b_is_mn(j);
+        const uint32_t bytes = kOperand + (b_mn ? chunks * kBox : j.bn / 2 * 2 * kTileK);
+        // Where the rows of the weights start: with the tile's rows, with the sum, or with its columns.
+        const int a_row = j.swap && j.kind != kStates ? j.v0 : 0, a_k = j.swap && j.kind == kStates ? j.v0 : 0;
+        const int b_row = !j.swap && !b_mn ? j.v0 : 0, b_k = !j.swap && j.kind == kStates ? j.v0 : 0;
         const int am = tl.m + rank * (kTileM / 2), bn = tl.n + rank * half;
         for (int i = 0; i < tl.nkb; ++i) {
           if (!bar_wait(&H.empty[s], ph ^ 1, abort, a.err)) goto loaded;
@@ -354,20 +359,19 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
           // The first CTA's barrier counts the bytes of both; its phase cannot
           // end before its own arrival here.
           const uint32_t bar = cluster_addr(&H.full[s], 0);
-          if (rank == 0) bar_expect(&H.full[s], bytes);
+          if (rank == 0) bar_expect(&H.full[s], 2 * bytes);
           if (a_mn) {
-            tma_load_pair(ma, sa, bar, am, k);
-            tma_load_pair(ma, sa + kBox, bar, am + kChunk, k);
-          } else if (load_a) {
-            tma_load_pair(ma, sa, bar, k, am);
-            tma_load_pair(ma, sa + a.stage_a / 2, bar, k + kChunk, am);
+            tma_load_pair(ma, sa, bar, am, a_k + k);
+            tma_load_pair(ma, sa + kBox, bar, am + kChunk, a_k + k);
+          } else {
+            tma_load_pair(ma, sa, bar, k, a_row + am);
+            tma_load_pair(ma, sa + kBox, bar, k + kChunk, a_row + am);
           }
           if (b_mn) {
-            const int kr = j.kind == kStates ? j.v0 + k : k;
-            for (int c = 0; c < chunks; ++c) tma_load_pair(mb, sb + c * kBox, bar, bn + c * kChunk, kr);
+            for (int c = 0; c < chunks; ++c) tma_load_pair(mb, sb + c * kBox, bar, bn + c * kChunk, b_k + k);
           } else {
-            tma_load_pair(mb, sb, bar, k, j.v0 + bn);
-            tma_load_pair(mb, sb + kBox, bar, k + kChunk, j.v0 + bn);
+            tma_load_pair(mb, sb, bar, k, b_row + bn);
+            tma_load_pair(mb, sb + a.stage_b / 2, bar, k + kChunk, b_row + bn);
           }
           if (++s == a.stages) s = 0, ph ^= 1;
         }
@@ -387,12 +391,12 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
       for (int idx = first; ok && idx < tiles; idx += step) {
         const Tile tl = tile_at(a, kept, idx);
         const Job &j = a.job[tl.job];
-        const bool a_mn = j.kind == kHeadRows, b_mn = j.kind == kStates || j.kind == kHeadRows;
+        const bool a_mn = a_is_mn(j), b_mn = b_is_mn(j);
         const uint32_t idesc = f16_idesc(kBf16, a_mn, b_mn, tl.cols);
         // 16 k are 32 bytes of a K-major row, 16 rows of 128 bytes of an MN-major
         // box; 64 k are a box of the one, half a box of the other.
-        const uint64_t step_a = a_mn ? 2048 >> 4 : 32 >> 4, half_a = a_mn ? 8192 >> 4 : a.stage_a >> 5;
-        const uint64_t step_b = b_mn ? 2048 >> 4 : 32 >> 4, half_b = b_mn ? 8192 >> 4 : kBox >> 4;
+        const uint64_t step_a = a_mn ? 2048 >> 4 : 32 >> 4, half_a = a_mn ? 8192 >> 4 : kBox >> 4;
+        const uint64_t step_b = b_mn ? 2048 >> 4 : 32 >> 4, half_b = b_mn ? 8192 >> 4 : a.stage_b >> 5;
         ok = __all_sync(0xffffffffu, bar_wait(&H.acc_empty[acc], acc_ph ^ 1, abort, a.err));
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -430,12 +434,71 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
     const int quarter = uwarp & 3, part = (uwarp - 2) >> 2;  // TMEM lanes, and first or second part of the columns
     const uint32_t ta = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     uint16_t *block = reinterpret_cast<uint16_t *>(stages + kRing) + (uwarp - 2) * 32 * kBlockPitch;
+    float *turned = reinterpret_cast<float *>(block);
     int acc = 0;
     uint32_t ph = 0;
+    RowState few[2];  // of this lane's tokens where they are the tiles' columns: kept from tile to tile
+    int few_target[2];
+    const bool swapped = a.job[a.jobs - 1].swap || a.job[0].swap;
+    if (swapped) {
+      const Job &j = a.job[a.job[0].swap ? 0 : a.jobs - 1];
+      const int mid = (j.bn / 2 + 31) / 32 * 32;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int token = (part ? mid : 0) + 32 * q + lane;
+        RowState &st = few[q];
+        st.live = token < kept && token < (part ? j.bn : mid);
+        st.lse2 = st.live && a.lse ? a.lse[token] * kLog2e : 0.f;
+        few_target[q] = st.live ? a.target[token] : -1;
+        st.m = kNegInf;
+        st.s = st.z = 0.f;
+        st.found = false;
+      }
+    }
     for (int idx = first; idx < tiles; idx += step) {
       const Tile tl = tile_at(a, kept, idx);
       const Job &j = a.job[tl.job];
       const int mid = (tl.cols / 2 + 31) / 32 * 32, c0 = part ? mid : 0, c1 = part ? tl.cols : mid;
+      if (j.swap) {
+        // A lane holds a row of the weights and the columns are tokens: 32 x 32 of
+        // them turn in shared memory, and each lane goes on with a token's row.
+        const int row0 = tl.m + rank * (kTileM / 2) + quarter * 32;
+        if (!__all_sync(0xffffffffu, bar_wait(&H.acc_full[acc], ph, abort, a.err))) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int c = c0 + 32 * q, token = c + lane;
+          if (c >= c1) break;
+          int r[32];
+          float z[32];
+          __syncwarp();
+          tmem_ask32(ta + acc * kTileN + c, r);
+          tmem_wait32(r);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) turned[lane * 33 + i] = tl.nkb ? __int_as_float(r[i]) : 0.f;
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) z[i] = turned[i * 33 + lane];
+          RowState &st = few[q];
+          st.target = st.live ? few_target[q] - (j.v0 + row0) : 0x7fffffff;
+          st.limit = a.vocab - (j.v0 + row0);
+          if (j.kind == kLoss) {
+            loss_chunk(st, 0, z);
+          } else if (j.kind == kProb) {
+            prob_chunk<kBf16>(a, st, static_cast<uint16_t *>(j.out) + token * j.pitch + row0, 0, z);
+          } else if (st.live && row0 < j.pitch) {
+            states_chunk(j.add, static_cast<float *>(j.out) + tl.slice * j.plane + token * j.pitch + row0, z);
+          }
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0)
+          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                           cluster_addr(&H.acc_empty[acc], 0))
+                       : "memory");
+        if (++acc == 2) acc = 0, ph ^= 1;
+        continue;
+      }
       const int row0 = tl.m + rank * (kTileM / 2) + quarter * 32, row = row0 + lane;
       RowState st;
       st.live = row < (j.kind == kHeadRows ? j.m_total : kept);
@@ -539,6 +602,15 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
         if (st.found) a.z_target[row] = st.z;
       }
       if (++acc == 2) acc = 0, ph ^= 1;
+    }
+    if (a.job[0].swap && a.job[0].kind == kLoss) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int token = (part ? (a.job[0].bn / 2 + 31) / 32 * 32 : 0) + 32 * q + lane;
+        if (!few[q].live) continue;
+        a.parts[(static_cast<int64_t>(blockIdx.x) * 4 + quarter) * a.part_pitch + token] = make_float2(few[q].m, few[q].s);
+        if (few[q].found) a.z_target[token] = few[q].z;
+      }
     }
   }
   __syncwarp();
@@ -960,12 +1032,14 @@ struct Scratch {
 };
 
 int launch_gemm(GemmArgs a, bool bf16, int64_t tiles, cudaStream_t s) {
-  // Where a tile has few tokens, A is small and the ring has more stages, so that
-  // more of the other operand is on its way (one token: 46 -> 36 us).
-  bool full = a.a_rows == kTileM / 2;
-  for (int i = 0; i < a.jobs; ++i) full = full || a.job[i].kind == kHeadRows;
-  a.stage_a = full ? kOperand : a.a_rows * kTileK * 2;
-  a.stages = kRing / (a.stage_a + kOperand);
+  // Where all tiles have few tokens, B is small and the ring has more stages.
+  a.stage_a = kOperand;
+  a.stage_b = 0;
+  for (int i = 0; i < a.jobs; ++i) {
+    const int need = a.job[i].swap ? a.job[i].bn / 2 * 2 * kTileK : kOperand;
+    a.stage_b = need > a.stage_b ? need : a.stage_b;
+  }
+  a.stages = kRing / (a.stage_a + a.stage_b);
   if (a.stages > kMaxStages) a.stages = kMaxStages;
   H24_CUDA_TRY(bf16 ? allow_smem<ce_gemm_kernel<true>>(kSmem) : allow_smem<ce_gemm_kernel<false>>(kSmem));
   cudaLaunchConfig_t cfg = {};
@@ -996,9 +1070,10 @@ int logits_bn(int64_t tokens, int64_t vocab) {
   return bn;
 }
 
-// Rows that a CTA loads of the tokens' tiles: all 128, or of the one tile of up
-// to 128 tokens those that are there, since no output takes the others.
-int token_rows(int64_t tokens) { return tokens > 128 ? 128 : static_cast<int>(up(tokens, 8)); }
+// Up to 128 tokens are the columns of the tiles of logits and of dx, not their
+// rows: 256 rows of which few are there would cost more of the tensor cores than
+// the weights' bytes cost of HBM (one token and [50688,1920]: 44 us, TURNED).
+bool few_tokens(int64_t tokens) { return tokens <= 128; }
 
 // Rows of a block of the row kernels: the blocks fill the GPU four times at most.
 int rows_per_block(int64_t tokens) {
@@ -1028,12 +1103,17 @@ bool head_readable(const CeArgs &c) { return aligned16(c.w) && c.w_stride % 8 ==
 int launch_ce_forward(const Tables *T, const CeArgs &c, const int64_t *labels, int64_t ignore, float *loss,
                       int32_t *state, cudaStream_t s) {
   const bool bf16 = c.dtype == H24_DTYPE_BF16;
-  const int bn = logits_bn(c.tokens, c.vocab);
-  const int64_t n_tiles = cdiv(c.vocab, bn), pitch = up(c.in, 8), part_pitch = up(c.tokens, kCombineRows);
+  const bool swap = few_tokens(c.tokens);
+  const int bn = swap ? static_cast<int>(up(c.tokens, 32)) : logits_bn(c.tokens, c.vocab);
+  // Tiles, and the parts of a token's sum that they leave: one for each half of a
+  // tile's columns, or for each warp of the grid that has its tokens.
+  const int64_t n_tiles = cdiv(c.vocab, swap ? kTileM : bn), m_tiles = swap ? 1 : cdiv(c.tokens, kTileM);
+  const int64_t n_parts = swap ? 8 * (n_tiles < kPairs ? n_tiles : kPairs) : 2 * n_tiles;
+  const int64_t pitch = up(c.in, 8), part_pitch = up(c.tokens, kCombineRows);
   Scratch sc(s);
   const int64_t rows_at = sc.take((c.tokens + kTileK) * pitch * 2), token_at = sc.take(c.tokens * 4);
   const int64_t zt_at = sc.take(c.tokens * 4), loss_at = sc.take(c.tokens * 4), ticket_at = sc.take(4);
-  const int64_t parts_at = sc.take(2 * n_tiles * part_pitch * 8);
+  const int64_t parts_at = sc.take(n_parts * part_pitch * 8);
   const int64_t w_at = head_readable(c) ? -1 : sc.take(c.vocab * pitch * 2);
   int rc = sc.allocate(T);
   if (rc != H24_OK) return rc;
@@ -1059,30 +1139,32 @@ int launch_ce_forward(const Tables *T, const CeArgs &c, const int64_t *labels, i
   if ((rc = readable_head(c, sc, w_at, &w, &w_pitch)) != H24_OK) return rc;
 
   GemmArgs g{};
-  if (!map16(&g.map[0], r.rows, c.tokens, c.in, pitch, token_rows(c.tokens)) || !map16(&g.map[1], w, c.vocab, c.in, w_pitch, bn / 2))
+  // A and B: the tokens' states and the head, or the other way round.
+  if (!map16(&g.map[swap], r.rows, c.tokens, c.in, pitch, swap ? bn / 2 : kTileM / 2) ||
+      !map16(&g.map[!swap], w, c.vocab, c.in, w_pitch, swap ? kTileM / 2 : bn / 2))
     return fail(H24_ERR_CUDA, "linear_ce_forward: cuTensorMapEncodeTiled failed");
   g.jobs = 1;
-  g.a_rows = token_rows(c.tokens);
   g.job[0].kind = kLoss;
-  g.job[0].n_total = static_cast<int>(c.vocab);
+  g.job[0].swap = swap;
+  g.job[0].n_total = swap ? bn : static_cast<int>(c.vocab);
+  g.job[0].m_total = static_cast<int>(c.vocab);
   g.job[0].bn = bn;
   g.job[0].k_total = static_cast<int>(c.in);
   g.job[0].split = 1;
   g.vocab = static_cast<int>(c.vocab);
   g.kept = st.kept;
   g.target = st.target;
-  g.lse = st.lse;
   g.z_target = sc.at<float>(zt_at);
   g.parts = sc.at<float2>(parts_at);
   g.part_pitch = part_pitch;
   g.err = T->err;
-  if ((rc = launch_gemm(g, bf16, cdiv(c.tokens, kTileM) * n_tiles, s)) != H24_OK) return rc;
+  if ((rc = launch_gemm(g, bf16, m_tiles * n_tiles, s)) != H24_OK) return rc;
 
   CombineArgs cb{};
   cb.st = st;
   cb.parts = g.parts;
   cb.part_pitch = part_pitch;
-  cb.n_parts = static_cast<int>(2 * n_tiles);
+  cb.n_parts = static_cast<int>(n_parts);
   cb.z_target = g.z_target;
   cb.token = r.token;
   cb.row_loss = sc.at<float>(loss_at);
@@ -1112,7 +1194,7 @@ BackPlan back_plan(const CeArgs &c, bool want_states, bool want_head) {
   p.pieces = cdiv(c.vocab, p.piece);
   // A dx tile sums over a whole piece.  Slices of it where that is more than a
   // third of what a pair of SMs does in a launch.
-  const int64_t kb = cdiv(p.piece, kTileK), m_tiles = rows / kTileM, n_tiles = cdiv(c.in, kTileN);
+  const int64_t kb = cdiv(p.piece, kTileK), m_tiles = rows / kTileM, n_tiles = cdiv(c.in, kTileN);  // (few tokens: the same count)
   int64_t work = m_tiles * n_tiles * kb;
   if (want_head) work += cdiv(p.piece, kTileM) * n_tiles * cdiv(c.tokens, kTileK);
   if (p.pieces > 1) work += m_tiles * cdiv(p.piece, kTileN) * cdiv(c.in, kTileK);
@@ -1165,7 +1247,6 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
 
   GemmArgs base{};
   base.vocab = static_cast<int>(c.vocab);
-  base.a_rows = token_rows(c.tokens);
   base.kept = st.kept;
   base.target = st.target;
   base.lse = st.lse;
@@ -1178,6 +1259,9 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   const int64_t rows_alloc = c.tokens + kTileK;
   const uint16_t *head_rows = r.scaled ? r.scaled : r.rows;
   const int bn_in = static_cast<int>(c.in >= kTileN ? kTileN : up(c.in, 32));
+  const bool swap = few_tokens(c.tokens);
+  const int bn_few = static_cast<int>(up(c.tokens, 32));
+  const int64_t d_rows = swap ? bn_few : rows;  // rows of d that are written
   for (int64_t i = 0; i <= plan.pieces; ++i) {
     // The gradients of piece i - 1 beside the logits of piece i.
     GemmArgs g = base;
@@ -1191,8 +1275,10 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
         if (!dx) return;
         Job &j = g.job[g.jobs];
         j.kind = kStates;
-        j.n_total = static_cast<int>(c.in);
-        j.bn = bn_in;
+        j.swap = swap;
+        j.n_total = swap ? bn_few : static_cast<int>(c.in);
+        j.m_total = static_cast<int>(c.in);
+        j.bn = swap ? bn_few : bn_in;
         j.k_total = static_cast<int>(v);
         j.split = plan.split;
         j.v0 = static_cast<int>(v0);
@@ -1200,8 +1286,8 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
         j.out = sc.at<float>(acc_at);
         j.pitch = acc_pitch;
         j.plane = c.tokens * acc_pitch;
-        ok = ok && map16(&g.map[2 * g.jobs], d, rows, plan.piece, d_pitch, token_rows(c.tokens)) &&
-             map16(&g.map[2 * g.jobs + 1], w, c.vocab, c.in, w_pitch, kTileK);
+        ok = ok && map16(&g.map[2 * g.jobs + swap], d, d_rows, plan.piece, d_pitch, swap ? bn_few / 2 : kTileM / 2) &&
+             map16(&g.map[2 * g.jobs + !swap], w, c.vocab, c.in, w_pitch, kTileK);
         tiles += rows / kTileM * cdiv(c.in, bn_in) * plan.split;
         ++g.jobs;
       };
@@ -1216,7 +1302,7 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
         j.v0 = static_cast<int>(v0);
         j.out = dw;
         j.pitch = c.in;
-        ok = ok && map16(&g.map[2 * g.jobs], d, rows, plan.piece, d_pitch, kTileK) &&
+        ok = ok && map16(&g.map[2 * g.jobs], d, d_rows, plan.piece, d_pitch, kTileK) &&
              map16(&g.map[2 * g.jobs + 1], head_rows, rows_alloc, c.in, pitch, kTileK);
         tiles += cdiv(v, kTileM) * cdiv(c.in, bn_in);
         ++g.jobs;
@@ -1234,16 +1320,18 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
       const int64_t v0 = i * plan.piece, v = c.vocab - v0 < plan.piece ? c.vocab - v0 : plan.piece;
       Job &j = g.job[g.jobs];
       j.kind = kProb;
-      j.n_total = static_cast<int>(up(v, kTileK));
-      j.bn = plan.pieces > 1 ? kTileN : logits_bn(c.tokens, c.vocab);
+      j.swap = swap;
+      j.n_total = swap ? bn_few : static_cast<int>(up(v, kTileK));
+      j.m_total = static_cast<int>(v);
+      j.bn = swap ? bn_few : plan.pieces > 1 ? kTileN : logits_bn(c.tokens, c.vocab);
       j.k_total = static_cast<int>(c.in);
       j.split = 1;
       j.v0 = static_cast<int>(v0);
       j.out = sc.at<uint16_t>(i & 1 ? d2_at : d_at);
       j.pitch = d_pitch;
-      ok = ok && map16(&g.map[2 * g.jobs], r.rows, c.tokens, c.in, pitch, token_rows(c.tokens)) &&
-           map16(&g.map[2 * g.jobs + 1], w, c.vocab, c.in, w_pitch, j.bn / 2);
-      tiles += rows / kTileM * cdiv(j.n_total, j.bn);
+      ok = ok && map16(&g.map[2 * g.jobs + swap], r.rows, c.tokens, c.in, pitch, swap ? bn_few / 2 : kTileM / 2) &&
+           map16(&g.map[2 * g.jobs + !swap], w, c.vocab, c.in, w_pitch, swap ? kTileM / 2 : j.bn / 2);
+      tiles += swap ? cdiv(v, kTileM) : rows / kTileM * cdiv(j.n_total, j.bn);
       ++g.jobs;
     }
     if (!ok) return fail(H24_ERR_CUDA, "linear_ce_backward: cuTensorMapEncodeTiled failed");

@@ -135,7 +135,17 @@ def test_masks_and_reductions(ce, reduction, masked, dtype):
         _check(ce, x, w, target, reduction, dloss)
 
 
-@pytest.mark.parametrize("tokens,vocab,k", [(1000, 50257, 48), (4100, 30001, 40)])
+@pytest.mark.parametrize("tokens,vocab,k", [(96, 1025, 1160), (97, 2049, 520), (128, 3001, 264), (129, 3001, 264),
+                                            (20, 20011, 1920)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_few_tokens(ce, tokens, vocab, k, dtype):
+    """Around the 128 tokens up to which they are the tiles' columns."""
+    for masked, reduction in ((0.0, "mean"), (0.3, "sum")):
+        x, w, target = _inputs(tokens, vocab, k, dtype, seed=7, masked=masked)
+        _check(ce, x, w, target, reduction, torch.tensor(8.0, device="cuda"))
+
+
+@pytest.mark.parametrize("tokens,vocab,k", [(1000, 50257, 48), (4100, 30001, 40), (40, 400003, 24)])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_several_pieces(ce, tokens, vocab, k, dtype):
     x, w, target = _inputs(tokens, vocab, k, dtype, seed=5, masked=0.2)
