@@ -40,8 +40,8 @@ constexpr int kMaxStages = 5;
 constexpr int kHead = 1024;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 320;    // warp 0 loads, warp 1 issues MMAs, warps 2-9 read TMEM
-constexpr int kBlockPitch = 66;  // elements of a row of an epilogue warp's 32 x 64 block
-constexpr int kBlockBytes = 32 * kBlockPitch * 2;
+constexpr int kBlockPitch = 33;  // fp32 of a row of an epilogue warp's 32 x 32 block
+constexpr int kBlockBytes = 32 * kBlockPitch * 4;
 constexpr int kSmem = 1024 + kHead + kRing + kEpiWarps * kBlockBytes;
 static_assert(kSmem <= 227 * 1024, "shared memory");
 constexpr int kMaxJobs = 3;
@@ -73,6 +73,7 @@ struct GemmArgs {
   int jobs;
   int vocab;
   int stages, stage_a, stage_b;  // of the ring; bytes of A and of B in a stage
+  int *next_tile;      // counts the tiles that pairs have taken beyond their first; null: each takes its turn
   const int *kept;     // number of tokens with a loss
   const int *target;   // of each kept token
   const float *lse;    // of each kept token
@@ -81,12 +82,19 @@ struct GemmArgs {
   int64_t part_pitch;
   const float *scale;  // kHeadRows: factor of the sum
   float prob_scale;
-  int row_bytes;       // kHeadRows: rows of the output lie on 32, 16 or 2 bytes
+  int row_bytes;       // kHeadRows: rows of the output lie on 32 or on 16 bytes
   int *err;
 };
 
+// Numbers of tiles handed on within a pair.  No slot is waited for: the loading
+// thread is at most a ring (5 k blocks, a tile has one at least) and two
+// accumulators ahead of the warp that is last to read, 8 tiles.
+constexpr int kSlots = 16;
+
 struct PairHead {
   uint64_t full[kMaxStages], empty[kMaxStages], acc_full[2], acc_empty[2], drain;
+  uint64_t slot_full[kSlots];
+  int slot[kSlots];
   uint32_t tmem;
   int abort;
 };
@@ -203,9 +211,6 @@ __device__ __forceinline__ uint16_t pack1(float a) {
   return __half_as_ushort(__float2half_rn(a));
 }
 
-// 1 where an element lies in a word's second half.
-__device__ __forceinline__ int odd16(const uint16_t *p) { return static_cast<int>(reinterpret_cast<uintptr_t>(p) >> 1 & 1); }
-
 // What an epilogue thread does with 32 columns of its row.  `c` is the column
 // within the tile; r the sums.
 struct RowState {
@@ -294,6 +299,51 @@ __device__ __forceinline__ void states_chunk(bool add, float *out, const float (
   }
 }
 
+// The order in which a pair of CTAs takes tiles.  Where tiles differ in length,
+// a pair takes the next one when it is ready for it: the first CTA's loading
+// thread counts it off in global memory and hands its number to the other warps
+// of both CTAs.  The list has the long tiles first.  (Each pair in its turn: the
+// gradients of [1024,1152] x [50688,1152] 455 us, DYN.)
+struct Turn {
+  const GemmArgs &a;
+  PairHead &H;
+  bool counting;
+  int tiles, n;
+  volatile int *abort;
+
+  // The next tile's number, or -1: for a warp, or (kThread) for one thread of it.
+  template <bool kThread>
+  __device__ __forceinline__ int take(int before, int first, int step) {
+    if (!counting) {
+      const int idx = before < 0 ? first : before + step;
+      return idx < tiles ? idx : -1;
+    }
+    const int s = n % kSlots;
+    const bool ok = bar_wait(&H.slot_full[s], n / kSlots & 1, abort, a.err);
+    if (kThread ? !ok : !__all_sync(0xffffffffu, ok)) return -1;
+    ++n;
+    return *const_cast<volatile int *>(&H.slot[s]);
+  }
+  // The same for the thread that counts.
+  __device__ __forceinline__ int give(int before, int counted, int first, int step) {
+    int idx = before < 0 ? first : counting ? step + counted : before + step;
+    if (idx >= tiles) idx = -1;
+    if (!counting) return idx;
+    const int s = n++ % kSlots;
+    // The other CTA's slot is written and its barrier told of the bytes by one
+    // asynchronous store, so that its readers need no more than for a load's bytes.
+    const uint32_t bar = cluster_addr(&H.slot_full[s], 1);
+    asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], 4;" ::"r"(bar) : "memory");
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.u32 [%0], %1, [%2];" ::"r"(
+                     cluster_addr(&H.slot[s], 1)),
+                 "r"(idx), "r"(bar)
+                 : "memory");
+    *const_cast<volatile int *>(&H.slot[s]) = idx;
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(su32(&H.slot_full[s])) : "memory");
+    return idx;
+  }
+};
+
 template <bool kBf16>
 __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_constant__ GemmArgs a) {
   extern __shared__ uint8_t ce_raw[];
@@ -315,6 +365,9 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
       bar_init(&H.acc_full[s], 1);
       bar_init(&H.acc_empty[s], 2 * kEpiWarps);
     }
+    for (int s = 0; s < kSlots; ++s) {
+      bar_init(&H.slot_full[s], 1);
+    }
     bar_init(&H.drain, 1);
     H.abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -335,13 +388,22 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
   const int kept = *a.kept;
   int tiles = 0;
   for (int j = 0; j < a.jobs; ++j) tiles += tiles_of(a.job[j], kept);
+  Turn turn{a, H, a.next_tile != nullptr && kept > 0, tiles, 0, abort};  // (without a token no tile has a k block)
 
   if (warp == 0) {
     if (lane == 0) {
       asm volatile("fence.proxy.async;" ::: "memory");  // the rows were written by ordinary stores
-      int s = 0;
+      int s = 0, counted = 0;
       uint32_t ph = 0;
-      for (int idx = first; idx < tiles; idx += step) {
+      for (int idx = -1;;) {
+        if (rank == 0) {
+          idx = turn.give(idx, counted, first, step);
+          if (idx < 0) break;
+          if (turn.counting) counted = atomicAdd(a.next_tile, 1);  // (its result is wanted after this tile's loads)
+        } else {
+          idx = turn.take<true>(idx, first, step);
+          if (idx < 0) break;
+        }
         const Tile tl = tile_at(a, kept, idx);
         const Job &j = a.job[tl.job];
         const CUtensorMap *ma = &a.map[2 * tl.job], *mb = ma + 1;
@@ -388,7 +450,9 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
       int s = 0, acc = 0;
       uint32_t ph = 0, acc_ph = 0;
       bool ok = true;
-      for (int idx = first; ok && idx < tiles; idx += step) {
+      for (int idx = -1; ok;) {
+        idx = turn.take<false>(idx, first, step);
+        if (idx < 0) break;
         const Tile tl = tile_at(a, kept, idx);
         const Job &j = a.job[tl.job];
         const bool a_mn = a_is_mn(j), b_mn = b_is_mn(j);
@@ -433,8 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
     const int uwarp = __shfl_sync(0xffffffffu, warp, 0);
     const int quarter = uwarp & 3, part = (uwarp - 2) >> 2;  // TMEM lanes, and first or second part of the columns
     const uint32_t ta = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    uint16_t *block = reinterpret_cast<uint16_t *>(stages + kRing) + (uwarp - 2) * 32 * kBlockPitch;
-    float *turned = reinterpret_cast<float *>(block);
+    float *turned = reinterpret_cast<float *>(stages + kRing) + (uwarp - 2) * 32 * kBlockPitch;
     int acc = 0;
     uint32_t ph = 0;
     RowState few[2];  // of this lane's tokens where they are the tiles' columns: kept from tile to tile
@@ -455,7 +518,9 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
         st.found = false;
       }
     }
-    for (int idx = first; idx < tiles; idx += step) {
+    for (int idx = -1;;) {
+      idx = turn.take<false>(idx, first, step);
+      if (idx < 0) break;
       const Tile tl = tile_at(a, kept, idx);
       const Job &j = a.job[tl.job];
       const int mid = (tl.cols / 2 + 31) / 32 * 32, c0 = part ? mid : 0, c1 = part ? tl.cols : mid;
@@ -475,10 +540,10 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
           tmem_ask32(ta + acc * kTileN + c, r);
           tmem_wait32(r);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) turned[lane * 33 + i] = tl.nkb ? __int_as_float(r[i]) : 0.f;
+          for (int i = 0; i < 32; ++i) turned[lane * kBlockPitch + i] = tl.nkb ? __int_as_float(r[i]) : 0.f;
           __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) z[i] = turned[i * 33 + lane];
+          for (int i = 0; i < 32; ++i) z[i] = turned[i * kBlockPitch + lane];
           RowState &st = few[q];
           st.target = st.live ? few_target[q] - (j.v0 + row0) : 0x7fffffff;
           st.limit = a.vocab - (j.v0 + row0);
@@ -538,55 +603,18 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
         } else {
           uint16_t *out = static_cast<uint16_t *>(j.out) + (j.v0 + static_cast<int64_t>(row0)) * j.pitch + tl.n + c;
           const int left = j.n_total - (tl.n + c);
-          if (a.row_bytes >= 16) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t w[8];
+          for (int h = 0; h < 2; ++h) {
+            uint32_t w[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) w[i] = pack2<kBf16>(z[16 * h + 2 * i] * scale, z[16 * h + 2 * i + 1] * scale);
-              uint16_t *to = out + lane * j.pitch + 16 * h;
-              if (a.row_bytes == 32) {
-                if (st.live && 16 * h < left) store32B(to, w);
-              } else {
-                if (st.live && 16 * h < left) *reinterpret_cast<uint4 *>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-                if (st.live && 16 * h + 8 < left) *reinterpret_cast<uint4 *>(to + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-              }
+            for (int i = 0; i < 8; ++i) w[i] = pack2<kBf16>(z[16 * h + 2 * i] * scale, z[16 * h + 2 * i + 1] * scale);
+            uint16_t *to = out + lane * j.pitch + 16 * h;
+            if (a.row_bytes == 32) {
+              if (st.live && 16 * h < left) store32B(to, w);
+            } else {
+              if (st.live && 16 * h < left) *reinterpret_cast<uint4 *>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+              if (st.live && 16 * h + 8 < left) *reinterpret_cast<uint4 *>(to + 8) = make_uint4(w[4], w[5], w[6], w[7]);
             }
-          } else {
-            // Rows on single elements: 64 columns of 32 rows in shared memory,
-            // each row shifted so that its words there are words of memory; a
-            // warp then writes a row's 128 bytes at a time.  (The loop is bound by
-            // its instructions, two warps a scheduler.)
-            const int at = (c - c0) & 32;
-            out -= at;
-            const int first_odd = odd16(out), turn = static_cast<int>(j.pitch & 1);
-            uint16_t *mine = block + lane * kBlockPitch + ((first_odd + lane * turn) & 1) + at;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) mine[i] = pack1<kBf16>(z[i] * scale);
-            if (at == 0 && c + 32 < c1) continue;
-            __syncwarp();
-            const int rows = min(32, j.m_total - row0), have = min(at + 32, left + at);
-            const uint32_t *words = reinterpret_cast<const uint32_t *>(block) + lane;
-            auto put = [&](uint16_t *to, uint32_t v, int i, int odd) {
-              const int e = 2 * lane - odd;  // the word's first element
-              if (e >= 0 && e + 1 < have) {
-                *reinterpret_cast<uint32_t *>(to + e) = v;
-              } else if (e < 0) {
-                if (have > 0) to[0] = static_cast<uint16_t>(v >> 16);
-                if (have == 64) to[63] = block[i * kBlockPitch + 64];
-              } else if (e < have) {
-                to[e] = static_cast<uint16_t>(v);
-              }
-            };
-            for (int i0 = 0; i0 < rows; i0 += 8) {
-              uint32_t v[8];
-#pragma unroll
-              for (int u = 0; u < 8; ++u) v[u] = words[(i0 + u) * (kBlockPitch / 2)];
-#pragma unroll
-              for (int u = 0; u < 8; ++u, out += j.pitch)
-                if (i0 + u < rows) put(out, v[u], i0 + u, (first_odd + u * turn) & 1);  // (i0 is even)
-            }
-            __syncwarp();
           }
         }
       }
@@ -736,6 +764,8 @@ struct BackRowsArgs {
   bool mean;
   float inv_prob_scale;
   float *scale;      // [0] factor of dW, [1] factor of dx where g is the same for all
+  int *counters;     // of the launches that follow, set to 0
+  int n_counters;
   int per_block;
 };
 
@@ -786,6 +816,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_back_rows_kernel(const BackRow
     reinterpret_cast<uint4 *>(a.scaled + place * a.pitch)[c] = make_uint4(o[0], o[1], o[2], o[3]);
   }
   if (blockIdx.x + 1 == gridDim.x) {
+    for (int i = t; i < a.n_counters; i += kRowThreads) a.counters[i] = 0;
     // The sums over tokens run in steps of 128: zeros up to there.
     const int end = (kept + kTileK - 1) / kTileK * kTileK;
     uint16_t *rows = a.scaled ? a.scaled : a.rows;
@@ -857,6 +888,54 @@ __global__ void __launch_bounds__(kRowThreads) ce_copy_head_kernel(const uint16_
   }
 }
 
+// The way back: rows of `pitch` elements on 16 bytes to rows of `in` side by
+// side at any alignment, a warp a row, whole vectors of the destination.  Where
+// dW's rows are off 16 bytes its tiles go to scratch first and then through this
+// copy: written by the element or word from the tiles they cost more (dW of
+// [333,1153] x [50257,1153] DENSE).
+__global__ void __launch_bounds__(kRowThreads) ce_dense_rows_kernel(const uint16_t *src, int64_t pitch, int64_t rows,
+                                                                    int in, uint16_t *out) {
+  pdl_enter();
+  const int lane = threadIdx.x & 31;
+  for (int64_t r = blockIdx.x * static_cast<int64_t>(kRowThreads / 32) + (threadIdx.x >> 5); r < rows;
+       r += static_cast<int64_t>(gridDim.x) * (kRowThreads / 32)) {
+    const uint16_t *from = src + r * pitch;
+    uint16_t *to = out + r * in;
+    // Elements before the first whole vector, vectors, elements after the last.
+    const int head = min(in, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(to) & 15)) / 2 & 7));
+    const int vecs = (in - head) / 8, tail = head + 8 * vecs;
+    if (lane < head) to[lane] = from[lane];
+    if (tail + lane < in && lane < 8) to[tail + lane] = from[tail + lane];
+    uint4 *o = reinterpret_cast<uint4 *>(to + head);
+    const uint4 *f = reinterpret_cast<const uint4 *>(from);
+    constexpr int U = 4;
+    for (int c0 = lane; c0 < vecs; c0 += 32 * U) {
+      uint4 x[U], y[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int c = min(c0 + 32 * u, vecs - 1);
+        x[u] = __ldcs(f + c);
+        y[u] = __ldcs(f + min(c + 1, static_cast<int>(pitch / 8) - 1));
+      }
+      auto put = [&](auto g) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (c0 + 32 * u < vecs) o[c0 + 32 * u] = g(x[u], y[u]);
+      };
+      switch (head) {  // (the same for the warp)
+        case 0: put([](uint4 a, uint4 b) { return shifted<0, false>(a, b); }); break;
+        case 1: put([](uint4 a, uint4 b) { return shifted<0, true>(a, b); }); break;
+        case 2: put([](uint4 a, uint4 b) { return shifted<1, false>(a, b); }); break;
+        case 3: put([](uint4 a, uint4 b) { return shifted<1, true>(a, b); }); break;
+        case 4: put([](uint4 a, uint4 b) { return shifted<2, false>(a, b); }); break;
+        case 5: put([](uint4 a, uint4 b) { return shifted<2, true>(a, b); }); break;
+        case 6: put([](uint4 a, uint4 b) { return shifted<3, false>(a, b); }); break;
+        default: put([](uint4 a, uint4 b) { return shifted<3, true>(a, b); }); break;
+      }
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
 // The loss from the tiles' maxima and sums
 // ---------------------------------------------------------------------------
@@ -872,16 +951,17 @@ struct CombineArgs {
   int reduction;     // H24_REDUCE_*
   unsigned *ticket;
 };
-constexpr int kCombineRows = 4;  // 32 bytes of neighbouring parts
+constexpr int kCombineRows = 4;  // 32 bytes of neighbouring parts; one row a block where tokens are few
 
+template <int ROWS>
 __global__ void __launch_bounds__(kRowThreads) ce_combine_kernel(const CombineArgs a) {
-  __shared__ float2 red[kRowThreads / 32][kCombineRows];
+  __shared__ float2 red[kRowThreads / 32][ROWS];
   __shared__ double sums[kRowThreads / 32];
   __shared__ bool last;
   pdl_enter();
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5, kept = *a.st.kept;
-  const int r = t % kCombineRows;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kCombineRows + r;
+  const int r = t % ROWS;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + r;
   auto join = [](float2 &p, float2 q) {
     const float m = fmaxf(p.x, q.x), base = m == kNegInf ? 0.f : m * kLog2e;
     p.y = p.y * exp2_fast(fmaf(p.x, kLog2e, -base)) + q.y * exp2_fast(fmaf(q.x, kLog2e, -base));
@@ -890,14 +970,14 @@ __global__ void __launch_bounds__(kRowThreads) ce_combine_kernel(const CombineAr
   float2 p = make_float2(kNegInf, 0.f);
   if (row < kept) {
 #pragma unroll 8
-    for (int i = t / kCombineRows; i < a.n_parts; i += kRowThreads / kCombineRows)
+    for (int i = t / ROWS; i < a.n_parts; i += kRowThreads / ROWS)
       join(p, __ldg(a.parts + i * a.part_pitch + row));
   }
-  for (int o = 16; o >= kCombineRows; o >>= 1)
+  for (int o = 16; o >= ROWS; o >>= 1)
     join(p, make_float2(__shfl_xor_sync(0xffffffffu, p.x, o), __shfl_xor_sync(0xffffffffu, p.y, o)));
-  if (lane < kCombineRows) red[warp][lane] = p;
+  if (lane < ROWS) red[warp][lane] = p;
   __syncthreads();
-  if (t < kCombineRows && row < kept) {
+  if (t < ROWS && row < kept) {
     for (int w = 1; w < kRowThreads / 32; ++w) join(p, red[w][t]);
     // A target outside the vocabulary has no loss: NaN, here and in the gradients.
     const bool known = a.st.target[row] >= 0;
@@ -1171,8 +1251,11 @@ int launch_ce_forward(const Tables *T, const CeArgs &c, const int64_t *labels, i
   cb.loss = loss;
   cb.reduction = c.reduction;
   cb.ticket = r.ticket;
-  H24_CUDA_TRY(launch_pdl(ce_combine_kernel, dim3(static_cast<unsigned>(cdiv(c.tokens, kCombineRows))),
-                          dim3(kRowThreads), s, cb));
+  if (swap)
+    H24_CUDA_TRY(launch_pdl(ce_combine_kernel<1>, dim3(static_cast<unsigned>(c.tokens)), dim3(kRowThreads), s, cb));
+  else
+    H24_CUDA_TRY(launch_pdl(ce_combine_kernel<kCombineRows>, dim3(static_cast<unsigned>(cdiv(c.tokens, kCombineRows))),
+                            dim3(kRowThreads), s, cb));
   count_launches(1);
   return H24_OK;
 }
@@ -1215,8 +1298,9 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   Scratch sc(s);
   const int64_t rows_at = sc.take((c.tokens + kTileK) * pitch * 2);
   const int64_t scaled_at = each && dw ? sc.take((c.tokens + kTileK) * pitch * 2) : -1;
-  const int64_t scale_at = sc.take(8);
+  const int64_t scale_at = sc.take(8), counters_at = sc.take((plan.pieces + 1) * 4);
   const int64_t w_at = head_readable(c) ? -1 : sc.take(c.vocab * pitch * 2);
+  const int64_t dw_at = dw && !(c.in % 8 == 0 && aligned16(dw)) ? sc.take(c.vocab * up(c.in, 16) * 2) : -1;
   const int64_t acc_at = dx ? sc.take(plan.split * c.tokens * acc_pitch * 4) : -1;
   const int64_t d_pitch = plan.piece, d_bytes = rows * d_pitch * 2;
   const int64_t d_at = sc.take(d_bytes), d2_at = plan.pieces > 1 ? sc.take(d_bytes) : d_at;
@@ -1237,6 +1321,8 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   r.mean = c.reduction == H24_REDUCE_MEAN;
   r.inv_prob_scale = 1.f / prob_scale;
   r.scale = sc.at<float>(scale_at);
+  r.counters = sc.at<int>(counters_at);
+  r.n_counters = static_cast<int>(plan.pieces + 1);
   r.per_block = rows_per_block(c.tokens);
   H24_CUDA_TRY(launch_pdl(bf16 ? ce_back_rows_kernel<true> : ce_back_rows_kernel<false>,
                           dim3(static_cast<unsigned>(cdiv(c.tokens, r.per_block))), dim3(kRowThreads), s, r));
@@ -1252,9 +1338,10 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   base.lse = st.lse;
   base.scale = r.scale;
   base.prob_scale = prob_scale;
-  base.row_bytes = c.in % 16 == 0 && (reinterpret_cast<uintptr_t>(dw) & 31) == 0 ? 32
-                   : c.in % 8 == 0 && aligned16(dw)                              ? 16
-                                                                                 : 2;
+  const bool dense = dw_at >= 0;
+  void *head_out = dense ? sc.at<void>(dw_at) : dw;
+  const int64_t head_pitch = dense ? up(c.in, 16) : c.in;
+  base.row_bytes = head_pitch % 16 == 0 && (reinterpret_cast<uintptr_t>(head_out) & 31) == 0 ? 32 : 16;
   base.err = T->err;
   const int64_t rows_alloc = c.tokens + kTileK;
   const uint16_t *head_rows = r.scaled ? r.scaled : r.rows;
@@ -1265,6 +1352,7 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   for (int64_t i = 0; i <= plan.pieces; ++i) {
     // The gradients of piece i - 1 beside the logits of piece i.
     GemmArgs g = base;
+    g.next_tile = r.counters + i;
     bool ok = true;
     int64_t tiles = 0;
     int64_t longest = 0;
@@ -1300,8 +1388,8 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
         j.m_total = static_cast<int>(v);
         j.split = 1;
         j.v0 = static_cast<int>(v0);
-        j.out = dw;
-        j.pitch = c.in;
+        j.out = head_out;
+        j.pitch = head_pitch;
         ok = ok && map16(&g.map[2 * g.jobs], d, d_rows, plan.piece, d_pitch, kTileK) &&
              map16(&g.map[2 * g.jobs + 1], head_rows, rows_alloc, c.in, pitch, kTileK);
         tiles += cdiv(v, kTileM) * cdiv(c.in, bn_in);
@@ -1336,6 +1424,12 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
     }
     if (!ok) return fail(H24_ERR_CUDA, "linear_ce_backward: cuTensorMapEncodeTiled failed");
     if ((rc = launch_gemm(g, bf16, tiles, s)) != H24_OK) return rc;
+  }
+  if (dense) {
+    H24_CUDA_TRY(launch_pdl(ce_dense_rows_kernel, dim3(wave_grid(cdiv(c.vocab, kRowThreads / 32), 8)), dim3(kRowThreads),
+                            s, static_cast<const uint16_t *>(head_out), head_pitch, c.vocab, static_cast<int>(c.in),
+                            static_cast<uint16_t *>(dw)));
+    count_launches(1);
   }
   if (dx) {
     StatesArgs o{};
