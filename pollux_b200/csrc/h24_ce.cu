@@ -44,6 +44,13 @@ constexpr int kBlockPitch = 33;  // fp32 of a row of an epilogue warp's 32 x 32 
 constexpr int kBlockBytes = 32 * kBlockPitch * 4;
 constexpr int kSmem = 1024 + kHead + kRing + kEpiWarps * kBlockBytes;
 static_assert(kSmem <= 227 * 1024, "shared memory");
+// k blocks at most of a sum in the tensor cores (the loss's tiles), in slices of one length.
+template <bool kBf16>
+__device__ __forceinline__ int slice_blocks(int nkb) {
+  constexpr int kMost = kBf16 ? 8 : 4;
+  const int n = (nkb + kMost - 1) / kMost;
+  return (nkb + n - 1) / n;
+}
 constexpr int kMaxJobs = 3;
 constexpr int kGroupM = 32;      // row tiles that run through the vocabulary together
 constexpr float kLog2e = 1.4426950408889634f;
@@ -81,7 +88,7 @@ struct GemmArgs {
   float2 *parts;       // kLoss: maximum and sum of half a tile's columns
   int64_t part_pitch;
   const float *scale;  // kHeadRows: factor of the sum
-  float prob_scale;
+  float prob_scale, prob_log2;  // what d is held times, and its logarithm
   int row_bytes;       // kHeadRows: rows of the output lie on 32 or on 16 bytes
   int *err;
 };
@@ -216,7 +223,7 @@ __device__ __forceinline__ uint16_t pack1(float a) {
 struct RowState {
   int64_t row;   // of the job's output
   bool live;
-  float lse2;    // kProb: log2e * lse
+  float lse2;    // kProb: log2e * lse - log2(prob_scale)
   int target;    // kLoss, kProb: the target's column of the tile (any number where it is elsewhere)
   int limit;     // kLoss, kProb: columns of the tile that the vocabulary has
   float m, s, z; // kLoss: running maximum, sum of exponentials, the target's logit
@@ -263,7 +270,7 @@ __device__ __forceinline__ void prob_chunk(const GemmArgs &a, const RowState &st
                                            const float (&z)[32]) {
   float d[32];
 #pragma unroll
-  for (int j = 0; j < 32; ++j) d[j] = exp2_fast(fmaf(z[j], kLog2e, -st.lse2)) * a.prob_scale;
+  for (int j = 0; j < 32; ++j) d[j] = exp2_fast(fmaf(z[j], kLog2e, -st.lse2));  // (times prob_scale: in lse2)
   const int at = st.target - c;
   if (static_cast<unsigned>(at) < 32u) {
 #pragma unroll
@@ -344,8 +351,19 @@ struct Turn {
   }
 };
 
-template <bool kBf16>
+// Forward: the loss's tiles alone, of many tokens or of few.  The tensor cores
+// cut off what falls below a sum's last place where they add to it, so a long sum
+// shrinks: z of 7,680 k by 8e-6 of itself in bf16, 1.4e-5 in fp16 (measured:
+// 1.7e-8 and 3e-8 to 5e-8 for each 16 k), which shows in an fp32 loss.  The
+// forward pass therefore sums 1,024 k at most there, in fp16 512, and these sums
+// rounded to nearest in registers: about 1e-6 whatever the length.  Shorter
+// slices cost time, since reading a tile's TMEM takes 1,400 cycles (256 k: 2e-7,
+// and [8192,1920] x [50688,1920] 1,405 us where 1,024 k take 1,037).
+// Probabilities rounded to 16 bits have no use for it.
+enum Mode { kBackward, kForwardRows, kForwardFew };
+template <bool kBf16, Mode kMode>
 __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_constant__ GemmArgs a) {
+  constexpr bool kForward = kMode != kBackward;
   extern __shared__ uint8_t ce_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(ce_raw) + 1023) & ~uintptr_t(1023));
   PairHead &H = *reinterpret_cast<PairHead *>(smem);
@@ -461,10 +479,14 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
         // box; 64 k are a box of the one, half a box of the other.
         const uint64_t step_a = a_mn ? 2048 >> 4 : 32 >> 4, half_a = a_mn ? 8192 >> 4 : kBox >> 4;
         const uint64_t step_b = b_mn ? 2048 >> 4 : 32 >> 4, half_b = b_mn ? 8192 >> 4 : a.stage_b >> 5;
-        ok = __all_sync(0xffffffffu, bar_wait(&H.acc_empty[acc], acc_ph ^ 1, abort, a.err));
-        if (!ok) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        for (int i = 0; i < tl.nkb; ++i) {
+        const int slice = kForward ? slice_blocks<kBf16>(tl.nkb) : 0x7fffffff;
+        for (int i = 0, at = 0; i < max(tl.nkb, 1); ++i) {  // (at: within a slice)
+          if (at == 0) {
+            ok = __all_sync(0xffffffffu, bar_wait(&H.acc_empty[acc], acc_ph ^ 1, abort, a.err));
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          }
+          if (tl.nkb == 0) break;
           ok = __all_sync(0xffffffffu, bar_wait(&H.full[s], ph, abort, a.err));
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -474,9 +496,14 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
 #pragma unroll
           for (int k = 0; k < kTileK / 16; ++k)
             mma_f16_pair(tmem + acc * kTileN, ad + k / 4 * half_a + k % 4 * step_a, bd + k / 4 * half_b + k % 4 * step_b,
-                         idesc, i > 0 || k > 0);
+                         idesc, at > 0 || k > 0);
           mma_commit_pair(&H.empty[s]);
           if (++s == a.stages) s = 0, ph ^= 1;
+          if (++at == slice && i + 1 < tl.nkb) {
+            mma_commit_pair(&H.acc_full[acc]);
+            if (++acc == 2) acc = 0, acc_ph ^= 1;
+            at = 0;
+          }
         }
         if (!ok) break;
         mma_commit_pair(&H.acc_full[acc]);
@@ -500,9 +527,51 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
     float *turned = reinterpret_cast<float *>(stages + kRing) + (uwarp - 2) * 32 * kBlockPitch;
     int acc = 0;
     uint32_t ph = 0;
+    // An accumulator is free once both CTAs' warps have read it.
+    auto release = [&] {
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                         cluster_addr(&H.acc_empty[acc], 0))
+                     : "memory");
+      if (++acc == 2) acc = 0, ph ^= 1;
+    };
+    // The bits of the sums of a tile's columns c0 + 32 q, for the loss: a slice of
+    // k after the other.  The first slice's loads are in flight together.
+    auto gather = [&](auto &sum, int nkb, int c0, int c1) {
+      constexpr int Q = sizeof(sum) / sizeof(sum[0]);
+      const int slice = slice_blocks<kBf16>(nkb);
+      for (int i = 0; i < nkb; i += slice) {
+        if (!__all_sync(0xffffffffu, bar_wait(&H.acc_full[acc], ph, abort, a.err))) return false;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t d = ta + acc * kTileN + c0;
+        __syncwarp();
+        if (i == 0) {
+#pragma unroll
+          for (int q = 0; q < Q; ++q)
+            if (c0 + 32 * q < c1) tmem_ask32(d + 32 * q, sum[q]);
+#pragma unroll
+          for (int q = 0; q < Q; ++q) tmem_wait32(sum[q]);
+        } else {
+#pragma unroll
+          for (int q = 0; q < Q; ++q) {
+            if (c0 + 32 * q >= c1) break;
+            int r[32];
+            tmem_ask32(d + 32 * q, r);
+            tmem_wait32(r);
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              sum[q][k] = __float_as_int(__int_as_float(sum[q][k]) + __int_as_float(r[k]));
+          }
+        }
+        release();
+      }
+      return true;
+    };
     RowState few[2];  // of this lane's tokens where they are the tiles' columns: kept from tile to tile
     int few_target[2];
-    const bool swapped = a.job[a.jobs - 1].swap || a.job[0].swap;
+    const bool swapped = kMode == kForwardFew || (kMode == kBackward && (a.job[a.jobs - 1].swap || a.job[0].swap));
     if (swapped) {
       const Job &j = a.job[a.job[0].swap ? 0 : a.jobs - 1];
       const int mid = (j.bn / 2 + 31) / 32 * 32;
@@ -511,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
         const int token = (part ? mid : 0) + 32 * q + lane;
         RowState &st = few[q];
         st.live = token < kept && token < (part ? j.bn : mid);
-        st.lse2 = st.live && a.lse ? a.lse[token] * kLog2e : 0.f;
+        st.lse2 = st.live && kMode == kBackward ? fmaf(a.lse[token], kLog2e, -a.prob_log2) : 0.f;
         few_target[q] = st.live ? a.target[token] : -1;
         st.m = kNegInf;
         st.s = st.z = 0.f;
@@ -524,30 +593,44 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
       const Tile tl = tile_at(a, kept, idx);
       const Job &j = a.job[tl.job];
       const int mid = (tl.cols / 2 + 31) / 32 * 32, c0 = part ? mid : 0, c1 = part ? tl.cols : mid;
-      if (j.swap) {
+      if (kMode == kForwardRows) {  // (asked for ahead of the wait)
+        const int row = tl.m + rank * (kTileM / 2) + quarter * 32 + lane;
+        few_target[0] = row < kept ? a.target[row] : -1;
+      }
+      if (kMode == kForwardFew || (kMode == kBackward && j.swap)) {
         // A lane holds a row of the weights and the columns are tokens: 32 x 32 of
         // them turn in shared memory, and each lane goes on with a token's row.
         const int row0 = tl.m + rank * (kTileM / 2) + quarter * 32;
-        if (!__all_sync(0xffffffffu, bar_wait(&H.acc_full[acc], ph, abort, a.err))) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        int sum[kForward ? 2 : 1][32];
+        if (kForward) {
+          if (!gather(sum, tl.nkb, c0, c1)) break;
+        } else {
+          if (!__all_sync(0xffffffffu, bar_wait(&H.acc_full[acc], ph, abort, a.err))) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        }
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           const int c = c0 + 32 * q, token = c + lane;
           if (c >= c1) break;
-          int r[32];
           float z[32];
           __syncwarp();
-          tmem_ask32(ta + acc * kTileN + c, r);
-          tmem_wait32(r);
+          if (kForward) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) turned[lane * kBlockPitch + i] = tl.nkb ? __int_as_float(r[i]) : 0.f;
+            for (int i = 0; i < 32; ++i) turned[lane * kBlockPitch + i] = __int_as_float(sum[kForward ? q : 0][i]);
+          } else {
+            int r[32];
+            tmem_ask32(ta + acc * kTileN + c, r);
+            tmem_wait32(r);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) turned[lane * kBlockPitch + i] = __int_as_float(r[i]);
+          }
           __syncwarp();
 #pragma unroll
           for (int i = 0; i < 32; ++i) z[i] = turned[i * kBlockPitch + lane];
           RowState &st = few[q];
           st.target = st.live ? few_target[q] - (j.v0 + row0) : 0x7fffffff;
           st.limit = a.vocab - (j.v0 + row0);
-          if (j.kind == kLoss) {
+          if (kForward) {
             loss_chunk(st, 0, z);
           } else if (j.kind == kProb) {
             prob_chunk<kBf16>(a, st, static_cast<uint16_t *>(j.out) + token * j.pitch + row0, 0, z);
@@ -555,13 +638,50 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
             states_chunk(j.add, static_cast<float *>(j.out) + tl.slice * j.plane + token * j.pitch + row0, z);
           }
         }
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncwarp();
-        if (lane == 0)
-          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
-                           cluster_addr(&H.acc_empty[acc], 0))
-                       : "memory");
-        if (++acc == 2) acc = 0, ph ^= 1;
+        if (!kForward) release();
+        continue;
+      }
+      if constexpr (kMode == kForwardRows) {
+        int sum[4][32];
+        if (!gather(sum, tl.nkb, c0, c1)) break;
+        auto z = [&](int q, int k) -> float { return __int_as_float(sum[q][k]); };
+        const int limit = a.vocab - tl.n;
+        if (c1 > limit || c0 + 128 > c1) {  // columns that are not there
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (c0 + 32 * q + k >= min(c1, limit)) sum[q][k] = __float_as_int(kNegInf);
+        }
+        // Four chains each, of the 128 columns' maximum and sum.
+        float top[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          top[q] = z(q, 0);
+#pragma unroll
+          for (int k = 1; k < 32; ++k) top[q] = fmaxf(top[q], z(q, k));
+        }
+        const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), base = m == kNegInf ? 0.f : m * kLog2e;
+        float part_sum[4] = {};
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) part_sum[q] += exp2_fast(fmaf(z(q, k), kLog2e, -base));
+        const int row = tl.m + rank * (kTileM / 2) + quarter * 32 + lane;
+        if (row < kept) {
+          a.parts[(static_cast<int64_t>(tl.n / j.bn) * 2 + part) * a.part_pitch + row] =
+              make_float2(m, (part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3]));
+          const int at = few_target[0] - tl.n - c0;
+          if (at >= 0 && at < c1 - c0) {
+            float own = 0.f;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                if (at == 32 * q + k) own = z(q, k);
+            a.z_target[row] = own;
+          }
+        }
         continue;
       }
       const int row0 = tl.m + rank * (kTileM / 2) + quarter * 32, row = row0 + lane;
@@ -573,42 +693,35 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
       st.m = kNegInf;
       st.s = st.z = 0.f;
       st.found = false;
-      if ((j.kind == kLoss || j.kind == kProb) && st.live) {
+      if (j.kind == kProb && st.live) {
         st.target = a.target[row] - (j.v0 + tl.n);
-        if (j.kind == kProb) st.lse2 = a.lse[row] * kLog2e;
+        st.lse2 = fmaf(a.lse[row], kLog2e, -a.prob_log2);
       }
       const float scale = j.kind == kHeadRows ? *a.scale : 1.f;
       if (!__all_sync(0xffffffffu, bar_wait(&H.acc_full[acc], ph, abort, a.err))) break;
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const uint32_t d = ta + acc * kTileN;
-      for (int c = c0; c < c1; c += 32) {
-        int r[32];
+      const int kind = j.kind, left0 = j.n_total - tl.n;
+      const int64_t pitch = j.pitch;
+      const bool add = j.add;
+      uint16_t *out16 = static_cast<uint16_t *>(j.out) + (kind == kProb ? row : j.v0 + static_cast<int64_t>(row)) * pitch + tl.n;
+      float *out32 = static_cast<float *>(j.out) + tl.slice * j.plane + row * pitch + tl.n;
+      auto chunk = [&](int c, const int (&r)[32]) {
         float z[32];
-        __syncwarp();
-        tmem_ask32(d + c, r);
-        tmem_wait32(r);
-        if (tl.nkb == 0) {  // an empty sum has no MMA
-#pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = 0;
-        }
 #pragma unroll
         for (int i = 0; i < 32; ++i) z[i] = __int_as_float(r[i]);
-        if (j.kind == kLoss) {
-          loss_chunk(st, c, z);
-        } else if (j.kind == kProb) {
-          prob_chunk<kBf16>(a, st, static_cast<uint16_t *>(j.out) + row * j.pitch + tl.n, c, z);
-        } else if (j.kind == kStates) {
-          if (st.live)
-            states_chunk(j.add, static_cast<float *>(j.out) + tl.slice * j.plane + row * j.pitch + tl.n + c, z);
+        if (kind == kProb) {
+          prob_chunk<kBf16>(a, st, out16, c, z);
+        } else if (kind == kStates) {
+          if (st.live) states_chunk(add, out32 + c, z);
         } else {
-          uint16_t *out = static_cast<uint16_t *>(j.out) + (j.v0 + static_cast<int64_t>(row0)) * j.pitch + tl.n + c;
-          const int left = j.n_total - (tl.n + c);
+          const int left = left0 - c;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t w[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) w[i] = pack2<kBf16>(z[16 * h + 2 * i] * scale, z[16 * h + 2 * i + 1] * scale);
-            uint16_t *to = out + lane * j.pitch + 16 * h;
+            uint16_t *to = out16 + c + 16 * h;
             if (a.row_bytes == 32) {
               if (st.live && 16 * h < left) store32B(to, w);
             } else {
@@ -617,21 +730,21 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
             }
           }
         }
+      };
+      for (int c = c0; c < c1; c += 32) {
+        int r[32];
+        __syncwarp();
+        tmem_ask32(d + c, r);
+        tmem_wait32(r);
+        if (tl.nkb == 0) {  // an empty sum has no MMA
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = 0;
+        }
+        chunk(c, r);
       }
-      // The accumulator is free once both CTAs' warps have read it.
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0)
-        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
-                         cluster_addr(&H.acc_empty[acc], 0))
-                     : "memory");
-      if (j.kind == kLoss && st.live) {
-        a.parts[(static_cast<int64_t>(tl.n / j.bn) * 2 + part) * a.part_pitch + row] = make_float2(st.m, st.s);
-        if (st.found) a.z_target[row] = st.z;
-      }
-      if (++acc == 2) acc = 0, ph ^= 1;
+      release();
     }
-    if (a.job[0].swap && a.job[0].kind == kLoss) {
+    if (kMode == kForwardFew) {
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         const int token = (part ? (a.job[0].bn / 2 + 31) / 32 * 32 : 0) + 32 * q + lane;
@@ -1111,7 +1224,9 @@ struct Scratch {
   }
 };
 
-int launch_gemm(GemmArgs a, bool bf16, int64_t tiles, cudaStream_t s) {
+template <auto kernel>
+int launch_gemm(GemmArgs a, int64_t tiles, cudaStream_t s) {
+  H24_CUDA_TRY(allow_smem<kernel>(kSmem));
   // Where all tiles have few tokens, B is small and the ring has more stages.
   a.stage_a = kOperand;
   a.stage_b = 0;
@@ -1121,7 +1236,6 @@ int launch_gemm(GemmArgs a, bool bf16, int64_t tiles, cudaStream_t s) {
   }
   a.stages = kRing / (a.stage_a + a.stage_b);
   if (a.stages > kMaxStages) a.stages = kMaxStages;
-  H24_CUDA_TRY(bf16 ? allow_smem<ce_gemm_kernel<true>>(kSmem) : allow_smem<ce_gemm_kernel<false>>(kSmem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * (tiles < 1 ? 1 : tiles < kPairs ? tiles : kPairs)));
   cfg.blockDim = dim3(kThreads);
@@ -1138,7 +1252,7 @@ int launch_gemm(GemmArgs a, bool bf16, int64_t tiles, cudaStream_t s) {
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  H24_CUDA_TRY(cudaLaunchKernelEx(&cfg, bf16 ? ce_gemm_kernel<true> : ce_gemm_kernel<false>, a));
+  H24_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a));
   count_launches(1);
   return H24_OK;
 }
@@ -1238,7 +1352,14 @@ int launch_ce_forward(const Tables *T, const CeArgs &c, const int64_t *labels, i
   g.parts = sc.at<float2>(parts_at);
   g.part_pitch = part_pitch;
   g.err = T->err;
-  if ((rc = launch_gemm(g, bf16, m_tiles * n_tiles, s)) != H24_OK) return rc;
+  const int64_t tiles = m_tiles * n_tiles;
+  if (swap)
+    rc = bf16 ? launch_gemm<ce_gemm_kernel<true, kForwardFew>>(g, tiles, s)
+              : launch_gemm<ce_gemm_kernel<false, kForwardFew>>(g, tiles, s);
+  else
+    rc = bf16 ? launch_gemm<ce_gemm_kernel<true, kForwardRows>>(g, tiles, s)
+              : launch_gemm<ce_gemm_kernel<false, kForwardRows>>(g, tiles, s);
+  if (rc != H24_OK) return rc;
 
   CombineArgs cb{};
   cb.st = st;
@@ -1277,7 +1398,7 @@ BackPlan back_plan(const CeArgs &c, bool want_states, bool want_head) {
   p.pieces = cdiv(c.vocab, p.piece);
   // A dx tile sums over a whole piece.  Slices of it where that is more than a
   // third of what a pair of SMs does in a launch.
-  const int64_t kb = cdiv(p.piece, kTileK), m_tiles = rows / kTileM, n_tiles = cdiv(c.in, kTileN);  // (few tokens: the same count)
+  const int64_t kb = cdiv(p.pieces > 1 ? p.piece : c.vocab, kTileK), m_tiles = rows / kTileM, n_tiles = cdiv(c.in, kTileN);  // (few tokens: the same count)
   int64_t work = m_tiles * n_tiles * kb;
   if (want_head) work += cdiv(p.piece, kTileM) * n_tiles * cdiv(c.tokens, kTileK);
   if (p.pieces > 1) work += m_tiles * cdiv(p.piece, kTileN) * cdiv(c.in, kTileK);
@@ -1338,6 +1459,7 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   base.lse = st.lse;
   base.scale = r.scale;
   base.prob_scale = prob_scale;
+  base.prob_log2 = bf16 ? 0.f : 15.f;
   const bool dense = dw_at >= 0;
   void *head_out = dense ? sc.at<void>(dw_at) : dw;
   const int64_t head_pitch = dense ? up(c.in, 16) : c.in;
@@ -1368,7 +1490,8 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
         j.m_total = static_cast<int>(c.in);
         j.bn = swap ? bn_few : bn_in;
         j.k_total = static_cast<int>(v);
-        j.split = plan.split;
+        // (Each slice has a k block; a shorter last piece adds to fewer of them.)
+        j.split = static_cast<int>(cdiv(v, kTileK) < plan.split ? cdiv(v, kTileK) : plan.split);
         j.v0 = static_cast<int>(v0);
         j.add = i > 1;
         j.out = sc.at<float>(acc_at);
@@ -1423,7 +1546,9 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
       ++g.jobs;
     }
     if (!ok) return fail(H24_ERR_CUDA, "linear_ce_backward: cuTensorMapEncodeTiled failed");
-    if ((rc = launch_gemm(g, bf16, tiles, s)) != H24_OK) return rc;
+    rc = bf16 ? launch_gemm<ce_gemm_kernel<true, kBackward>>(g, tiles, s)
+              : launch_gemm<ce_gemm_kernel<false, kBackward>>(g, tiles, s);
+    if (rc != H24_OK) return rc;
   }
   if (dense) {
     H24_CUDA_TRY(launch_pdl(ce_dense_rows_kernel, dim3(wave_grid(cdiv(c.vocab, kRowThreads / 32), 8)), dim3(kRowThreads),
