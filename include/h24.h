@@ -301,7 +301,7 @@ int h24_linear_ce_forward(const void *x, int64_t tokens, int64_t x_stride, const
  * multiplied with g_t / max|g| and rounded) or one.  dx (tokens x in_features)
  * and dw (vocab x in_features) are contiguous and of `dtype`; either may be
  * NULL.  The logits are computed again, for a piece of the vocabulary at a
- * time; scratch as above, and 2 * 96 MiB at most for the pieces (more where 256
+ * time; scratch as above, and 2 * 192 MiB at most for the pieces (more where 256
  * columns of all tokens are more) and 4 bytes for each element of dx and slice
  * of its sum. */
 int h24_linear_ce_backward(const void *x, int64_t tokens, int64_t x_stride, const void *w, int64_t vocab,

@@ -527,13 +527,14 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
     float *turned = reinterpret_cast<float *>(stages + kRing) + (uwarp - 2) * 32 * kBlockPitch;
     int acc = 0;
     uint32_t ph = 0;
-    // An accumulator is free once both CTAs' warps have read it.
+    // An accumulator is free once both CTAs' warps have read it.  (The arrival
+    // tells of reads of TMEM and of nothing in memory: its release at the scope of
+    // the cluster would wait for the tile's stores to arrive in L2.)
     auto release = [&] {
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0)
-        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
-                         cluster_addr(&H.acc_empty[acc], 0))
+        asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr(&H.acc_empty[acc], 0))
                      : "memory");
       if (++acc == 2) acc = 0, ph ^= 1;
     };
@@ -1180,7 +1181,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_states_kernel(const StatesArgs
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
-constexpr int64_t kPieceBytes = int64_t(96) << 20;  // of d, for one piece of the vocabulary
+constexpr int64_t kPieceBytes = int64_t(192) << 20;  // of d, for one piece of the vocabulary
 
 // Map of a matrix of 16-bit elements [rows][cols], row pitch `pitch` elements,
 // in boxes of 64 columns x box_rows with the 128-byte swizzle.
