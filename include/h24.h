@@ -452,8 +452,8 @@ int64_t h24_launch_count(void);
 
 /* Synchronise `stream` and report a device-side failure of earlier quantize
  * calls on the current device: H24_ERR_TIMEOUT if a bounded wait inside the
- * screening kernel, the LUT GEMV or the int8 product ran out (the word is then
- * cleared), else H24_OK. */
+ * screening kernel, the LUT GEMV, the int8 product, the norms or the cross
+ * entropy ran out (the word is then cleared), else H24_OK. */
 int h24_check(void *stream);
 
 

@@ -12,6 +12,8 @@ Modules:
   plx            -- .plx container reader / writer
   int8           -- INT8 head path: residual + RMS norm to int8 rows, int8 product
   sampling       -- temperature, top-k, top-p and min-p from given numbers
+  norm           -- residual + RMS or layer norm, with gradients
+  loss           -- cross entropy of a head's product without its logits, with gradients
   shard          -- row sharding across ranks, optional all-gather of packed bytes
   build          -- build recipe of libh24.so and of its torch module
 """
