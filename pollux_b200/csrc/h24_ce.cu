@@ -81,7 +81,10 @@ struct GemmArgs {
   int vocab;
   int stages, stage_a, stage_b;  // of the ring; bytes of A and of B in a stage
   int *next_tile;      // counts the tiles that pairs have taken beyond their first; null: each takes its turn
-  const int *kept;     // number of tokens with a loss
+  const int *kept;     // number of tokens with a loss; null: the tokens' own rows are read, `tokens` of them
+  int tokens;
+  const int64_t *labels;  // of the tokens, where kept is null
+  unsigned *ticket;       // set to 0, where kept is null
   const int *target;   // of each kept token
   const float *lse;    // of each kept token
   float *z_target;
@@ -403,7 +406,8 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = H.tmem;
   pdl_enter();
-  const int kept = *a.kept;
+  const int kept = a.kept ? *a.kept : a.tokens;
+  if (kMode == kForwardFew && a.ticket && blockIdx.x == 0 && t == 0) *a.ticket = 0;
   int tiles = 0;
   for (int j = 0; j < a.jobs; ++j) tiles += tiles_of(a.job[j], kept);
   Turn turn{a, H, a.next_tile != nullptr && kept > 0, tiles, 0, abort};  // (without a token no tile has a k block)
@@ -582,7 +586,11 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
         RowState &st = few[q];
         st.live = token < kept && token < (part ? j.bn : mid);
         st.lse2 = st.live && kMode == kBackward ? fmaf(a.lse[token], kLog2e, -a.prob_log2) : 0.f;
-        few_target[q] = st.live ? a.target[token] : -1;
+        few_target[q] = -1;
+        if (st.live) {
+          const int64_t label = a.labels ? a.labels[token] : a.target[token];
+          few_target[q] = label >= 0 && label < a.vocab ? static_cast<int>(label) : -1;
+        }
         st.m = kNegInf;
         st.s = st.z = 0.f;
         st.found = false;
@@ -1064,6 +1072,10 @@ struct CombineArgs {
   float *loss;       // of each token, or the one value
   int reduction;     // H24_REDUCE_*
   unsigned *ticket;
+  // Where the tokens' own rows were multiplied (few tokens): the state is made here.
+  const int64_t *labels;
+  int64_t ignore;
+  int tokens, vocab;
 };
 constexpr int kCombineRows = 4;  // 32 bytes of neighbouring parts; one row a block where tokens are few
 
@@ -1073,7 +1085,30 @@ __global__ void __launch_bounds__(kRowThreads) ce_combine_kernel(const CombineAr
   __shared__ double sums[kRowThreads / 32];
   __shared__ bool last;
   pdl_enter();
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, kept = *a.st.kept;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const bool own = ROWS == 1 && a.labels;  // rows by token, not by place
+  int kept, place = 0, n_mean = 0;
+  bool known = true, keep = true;
+  if (own) {
+    const bool counts = t < a.tokens && a.labels[t] != a.ignore;  // (at most 128 tokens)
+    const int64_t label = a.labels[blockIdx.x];
+    keep = label != a.ignore;
+    known = label >= 0 && label < a.vocab;
+    place = __syncthreads_count(counts && t < static_cast<int>(blockIdx.x));
+    const int total = __syncthreads_count(counts);
+    kept = a.tokens;
+    if (t == 0) {
+      a.st.place[blockIdx.x] = keep ? place : -1;
+      if (keep) a.st.target[place] = known ? static_cast<int>(label) : -1;
+      if (blockIdx.x == 0) *a.st.kept = total;
+      if (!keep && a.reduction == H24_REDUCE_NONE) a.loss[blockIdx.x] = 0.f;
+      if (!keep && a.reduction != H24_REDUCE_NONE) a.row_loss[blockIdx.x] = 0.f;
+    }
+    n_mean = total;
+  } else {
+    kept = *a.st.kept;
+    n_mean = kept;
+  }
   const int r = t % ROWS;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + r;
   auto join = [](float2 &p, float2 q) {
@@ -1091,15 +1126,15 @@ __global__ void __launch_bounds__(kRowThreads) ce_combine_kernel(const CombineAr
     join(p, make_float2(__shfl_xor_sync(0xffffffffu, p.x, o), __shfl_xor_sync(0xffffffffu, p.y, o)));
   if (lane < ROWS) red[warp][lane] = p;
   __syncthreads();
-  if (t < ROWS && row < kept) {
+  if (t < ROWS && row < kept && keep) {
     for (int w = 1; w < kRowThreads / 32; ++w) join(p, red[w][t]);
     // A target outside the vocabulary has no loss: NaN, here and in the gradients.
-    const bool known = a.st.target[row] >= 0;
+    if (!own) known = a.st.target[row] >= 0;
     const float lse = known ? p.x + logf(p.y) : __int_as_float(0x7fffffff);
     const float loss = known ? lse - a.z_target[row] : lse;
-    a.st.lse[row] = lse;
+    a.st.lse[own ? place : row] = lse;
     if (a.reduction == H24_REDUCE_NONE)
-      a.loss[a.token[row]] = loss;
+      a.loss[own ? row : a.token[row]] = loss;
     else
       a.row_loss[row] = loss;
   }
@@ -1120,7 +1155,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_combine_kernel(const CombineAr
   if (t == 0) {
     sum = 0.0;
     for (int w = 0; w < kRowThreads / 32; ++w) sum += sums[w];
-    *a.loss = static_cast<float>(a.reduction == H24_REDUCE_MEAN ? sum / kept : sum);
+    *a.loss = static_cast<float>(a.reduction == H24_REDUCE_MEAN ? sum / n_mean : sum);
   }
 }
 
@@ -1313,6 +1348,10 @@ int launch_ce_forward(const Tables *T, const CeArgs &c, const int64_t *labels, i
   int rc = sc.allocate(T);
   if (rc != H24_OK) return rc;
   const State st = state_at(state, c.tokens);
+  // Few tokens whose rows TMA can read are multiplied as they lie, the ignored
+  // ones among them (they cost nothing more, and a column is a token's own); their
+  // places are counted with the loss.  That spares a kernel of three.
+  const bool own = swap && aligned16(c.x) && c.x_stride % 8 == 0 && c.x_stride >= c.in;
   RowsArgs r{};
   r.x = {static_cast<const uint16_t *>(c.x), c.x_stride, static_cast<int>(c.tokens), static_cast<int>(c.in),
          rows_on_16(c.x, c.x_stride, c.in)};
@@ -1326,16 +1365,18 @@ int launch_ce_forward(const Tables *T, const CeArgs &c, const int64_t *labels, i
   r.loss = c.reduction == H24_REDUCE_NONE ? loss : nullptr;
   r.ticket = sc.at<unsigned>(ticket_at);
   r.per_block = rows_per_block(c.tokens);
-  H24_CUDA_TRY(launch_pdl(ce_rows_kernel, dim3(static_cast<unsigned>(cdiv(c.tokens, r.per_block))), dim3(kRowThreads),
-                          s, r));
-  count_launches(1);
+  if (!own) {
+    H24_CUDA_TRY(launch_pdl(ce_rows_kernel, dim3(static_cast<unsigned>(cdiv(c.tokens, r.per_block))), dim3(kRowThreads),
+                            s, r));
+    count_launches(1);
+  }
   const void *w;
   int64_t w_pitch;
   if ((rc = readable_head(c, sc, w_at, &w, &w_pitch)) != H24_OK) return rc;
 
   GemmArgs g{};
   // A and B: the tokens' states and the head, or the other way round.
-  if (!map16(&g.map[swap], r.rows, c.tokens, c.in, pitch, swap ? bn / 2 : kTileM / 2) ||
+  if (!map16(&g.map[swap], own ? c.x : r.rows, c.tokens, c.in, own ? c.x_stride : pitch, swap ? bn / 2 : kTileM / 2) ||
       !map16(&g.map[!swap], w, c.vocab, c.in, w_pitch, swap ? kTileM / 2 : bn / 2))
     return fail(H24_ERR_CUDA, "linear_ce_forward: cuTensorMapEncodeTiled failed");
   g.jobs = 1;
@@ -1347,7 +1388,10 @@ int launch_ce_forward(const Tables *T, const CeArgs &c, const int64_t *labels, i
   g.job[0].k_total = static_cast<int>(c.in);
   g.job[0].split = 1;
   g.vocab = static_cast<int>(c.vocab);
-  g.kept = st.kept;
+  g.kept = own ? nullptr : st.kept;
+  g.tokens = static_cast<int>(c.tokens);
+  g.labels = own ? labels : nullptr;
+  g.ticket = own ? r.ticket : nullptr;
   g.target = st.target;
   g.z_target = sc.at<float>(zt_at);
   g.parts = sc.at<float2>(parts_at);
@@ -1373,6 +1417,10 @@ int launch_ce_forward(const Tables *T, const CeArgs &c, const int64_t *labels, i
   cb.loss = loss;
   cb.reduction = c.reduction;
   cb.ticket = r.ticket;
+  cb.labels = own ? labels : nullptr;
+  cb.ignore = ignore;
+  cb.tokens = static_cast<int>(c.tokens);
+  cb.vocab = static_cast<int>(c.vocab);
   if (swap)
     H24_CUDA_TRY(launch_pdl(ce_combine_kernel<1>, dim3(static_cast<unsigned>(c.tokens)), dim3(kRowThreads), s, cb));
   else
