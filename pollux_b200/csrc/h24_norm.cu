@@ -20,8 +20,9 @@
 //
 // Bound by HBM where there are rows: forward and backward move 8 bytes an element
 // each in bf16 (x, r, y, s; s, dy, dsummed, dx).  On a B200 [16384,1920] bf16
-// with the RMS norm takes 42 us forward (5.9 TB/s, 0.91 of the measured copy rate)
-// and 49 + 6 back (5.1); [8192,7680] with the layer norm 93 (5.4) and 105 + 6 (4.8).
+// with the RMS norm takes 40 us forward (6.4 TB/s, 0.97 of the measured copy rate)
+// and 43 + 6 back (5.8); [8192,7680] with the layer norm 90 (5.6) and 95 + 6 (5.3).
+// Rows off 16 bytes are read and written by the element, several times slower.
 #include "h24_tile.cuh"
 
 #include <type_traits>
@@ -81,9 +82,64 @@ struct BackArgs {
 
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
 
-// Thread t of a row's threads holds the columns of the vectors t, t + nt, ...
+// Two columns at a time: one instruction for both, where the kernels were bound by
+// their instructions ([16384,1920] bf16 42 and 49 us one by one, 40 and 43 in
+// pairs; [8192,7680] with the layer norm 93 and 105, 90 and 95).
+__device__ __forceinline__ float2 as_pair(uint64_t v) { return make_float2(__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32))); }
+__device__ __forceinline__ uint64_t bits(float2 v) {
+  return static_cast<uint64_t>(__float_as_uint(v.x)) | static_cast<uint64_t>(__float_as_uint(v.y)) << 32;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+  return as_pair(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+  return as_pair(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+  return as_pair(r);
+}
+
+// Two neighbouring elements, as words of memory.
+template <int DT>
+struct Pair;
+template <>
+struct Pair<H24_DTYPE_F32> {
+  using W = uint64_t;
+  static __device__ __forceinline__ float2 up(W w) { return as_pair(w); }
+  static __device__ __forceinline__ W down(float2 v) { return bits(v); }
+};
+template <>
+struct Pair<H24_DTYPE_F16> {
+  using W = uint32_t;
+  static __device__ __forceinline__ float2 up(W w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+  static __device__ __forceinline__ W down(float2 v) {
+    const __half2 h = __float22half2_rn(v);
+    return *reinterpret_cast<const W *>(&h);
+  }
+};
+template <>
+struct Pair<H24_DTYPE_BF16> {
+  using W = uint32_t;
+  static __device__ __forceinline__ float2 up(W w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  static __device__ __forceinline__ W down(float2 v) {
+    const __nv_bfloat162 h = __float22bfloat162_rn(v);
+    return *reinterpret_cast<const W *>(&h);
+  }
+};
+
+// Thread t of a row's threads holds the columns of the vectors t, t + nt, ..., in pairs.
 template <int DT, int HOLD = kHold>
 struct Held {
+  using W = typename Pair<DT>::W;
   static constexpr int VEC = Elem<DT>::kVec, NV = HOLD / VEC;
   uint4 raw[NV];
 
@@ -112,53 +168,68 @@ struct Held {
       raw[i] = (t + i * nt) * VEC < cols ? *reinterpret_cast<const uint4 *>(row + (t + i * nt) * 16)
                                          : make_uint4(0, 0, 0, 0);
   }
-  __device__ __forceinline__ float get(int k) const {
-    return Elem<DT>::up(reinterpret_cast<const typename Elem<DT>::T *>(&raw[k / VEC])[k % VEC]);
-  }
+  __device__ __forceinline__ float2 get(int k) const { return Pair<DT>::up(reinterpret_cast<const W *>(raw)[k]); }
 };
 
 // The held columns of a row to memory.
-template <int DT, bool kAligned, int HOLD>
-__device__ __forceinline__ void store_held(void *base, int64_t offset, const float (&v)[HOLD], int t, int nt, int cols) {
-  using E = Elem<DT>;
-  using T = typename E::T;
-  constexpr int VEC = E::kVec;
+template <int DT, bool kAligned, int P>
+__device__ __forceinline__ void store_held(void *base, int64_t offset, const float2 (&v)[P], int t, int nt, int cols) {
+  using T = typename Elem<DT>::T;
+  using W = typename Pair<DT>::W;
+  constexpr int VEC = Elem<DT>::kVec;
   T *p = static_cast<T *>(base) + offset;
 #pragma unroll
-  for (int i = 0; i < HOLD / VEC; ++i) {
+  for (int i = 0; i < 2 * P / VEC; ++i) {
     const int at = (t + i * nt) * VEC;
-    alignas(16) T o[VEC];
+    alignas(16) W o[VEC / 2];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) o[j] = E::down(v[i * VEC + j]);
+    for (int j = 0; j < VEC / 2; ++j) o[j] = Pair<DT>::down(v[i * VEC / 2 + j]);
     if (kAligned) {
       if (at < cols) *reinterpret_cast<uint4 *>(p + at) = *reinterpret_cast<const uint4 *>(o);
     } else {
 #pragma unroll
       for (int j = 0; j < VEC; ++j)
-        if (at + j < cols) p[at + j] = o[j];
+        if (at + j < cols) p[at + j] = reinterpret_cast<const T *>(o)[j];
     }
   }
 }
 
 // The held columns of a parameter vector as fp32 (0 past the end).
-template <int DT, bool kAligned, int HOLD>
-__device__ __forceinline__ void load_param(const void *param, bool f32, float (&v)[HOLD], int t, int nt, int cols) {
-  using E = Elem<DT>;
-  using T = typename E::T;
-  constexpr int VEC = E::kVec;
+template <int DT, bool kAligned, int P>
+__device__ __forceinline__ void load_param(const void *param, bool f32, float2 (&v)[P], int t, int nt, int cols) {
+  constexpr int VEC = Elem<DT>::kVec;
   if (!f32 || DT == H24_DTYPE_F32) {
-    Held<DT, HOLD> h;
+    Held<DT, 2 * P> h;
     h.template load<kAligned>(param, 0, t, nt, cols);
 #pragma unroll
-    for (int k = 0; k < HOLD; ++k) v[k] = h.get(k);
+    for (int k = 0; k < P; ++k) v[k] = h.get(k);
     return;
   }
   const float *p = static_cast<const float *>(param);
 #pragma unroll
-  for (int i = 0; i < HOLD / VEC; ++i) {
-    const int at = (t + i * nt) * VEC;
+  for (int k = 0; k < P; ++k) {
+    const int at = (t + 2 * k / VEC * nt) * VEC + 2 * k % VEC;
+    v[k] = make_float2(at < cols ? __ldg(p + at) : 0.f, at + 1 < cols ? __ldg(p + at + 1) : 0.f);
+  }
+}
+
+// The mean off the held columns; past the row's end they stay 0.
+template <int DT, int P>
+__device__ __forceinline__ void center(float2 (&v)[P], float mean, int t, int nt, int cols) {
+  constexpr int VEC = Elem<DT>::kVec;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) v[i * VEC + j] = at + j < cols ? __ldg(p + at + j) : 0.f;
+  for (int i = 0; i < 2 * P / VEC; ++i) {
+    const int left = cols - (t + i * nt) * VEC;  // columns of the vector that are there
+    const float2 m = both(left > 0 ? -mean : 0.f);
+#pragma unroll
+    for (int j = 0; j < VEC / 2; ++j) {
+      float2 &x = v[i * VEC / 2 + j];
+      x = add2(x, m);
+      if (left < VEC) {  // (rows that end inside a vector)
+        if (2 * j >= left) x.x = 0.f;
+        if (2 * j + 1 >= left) x.y = 0.f;
+      }
+    }
   }
 }
 
@@ -252,7 +323,6 @@ __global__ void __launch_bounds__(kMax) norm_kernel(const __grid_constant__ Norm
   const int64_t first = kWarp ? blockIdx.x * static_cast<int64_t>(kWarpRows) + (threadIdx.x >> 5) : blockIdx.x;
   const int64_t step = kWarp ? static_cast<int64_t>(gridDim.x) * kWarpRows : gridDim.x;
   const float n_cols = static_cast<float>(cols);
-  constexpr int VEC = Elem<DT>::kVec;
   Held<DT, HOLD> x, res;
   auto ask = [&](int64_t r) {
     if (r >= a.rows) return;
@@ -262,42 +332,42 @@ __global__ void __launch_bounds__(kMax) norm_kernel(const __grid_constant__ Norm
   ask(first);
   int turn = 0;
   for (int64_t r = first; r < a.rows; r += step, turn ^= 1) {
-    float v[HOLD];
+    constexpr int P = HOLD / 2;
+    float2 v[P];
 #pragma unroll
-    for (int k = 0; k < HOLD; ++k) v[k] = x.get(k);
+    for (int k = 0; k < P; ++k) v[k] = x.get(k);
     if (a.residual) {
 #pragma unroll
-      for (int k = 0; k < HOLD; ++k) v[k] = Elem<DT>::up(Elem<DT>::down(v[k] + res.get(k)));
+      for (int k = 0; k < P; ++k) v[k] = Pair<DT>::up(Pair<DT>::down(add2(v[k], res.get(k))));
     }
     ask(r + step);
-    if (a.summed) store_held<DT, kAligned, HOLD>(a.summed, r * a.cols, v, t, nt, cols);
-    float mean = 0.f, ss = 0.f;
+    if (a.summed) store_held<DT, kAligned>(a.summed, r * a.cols, v, t, nt, cols);
+    float mean = 0.f;
+    float2 sum = both(0.f), ss = both(0.f);
     if (kLayer) {
-      float sum = 0.f;
 #pragma unroll
-      for (int k = 0; k < HOLD; ++k) sum += v[k];
-      mean = row_sum<kWarp>(sum, red[turn][0]) / n_cols;
+      for (int k = 0; k < P; ++k) sum = add2(sum, v[k]);
+      mean = row_sum<kWarp>(sum.x + sum.y, red[turn][0]) / n_cols;
+      center<DT>(v, mean, t, nt, cols);
     }
 #pragma unroll
-    for (int k = 0; k < HOLD; ++k) {
-      if (kLayer) {
-        const int at = (t + k / VEC * nt) * VEC + k % VEC;
-        v[k] = at < cols ? v[k] - mean : 0.f;
-      }
-      ss = fmaf(v[k], v[k], ss);
-    }
-    ss = row_sum<kWarp>(ss, red[turn][1]);
-    const float inv = 1.0f / sqrtf(ss / n_cols + a.eps);
-    float w[HOLD];
-    load_param<DT, kAligned, HOLD>(a.gain, a.gain_f32, w, t, nt, cols);
+    for (int k = 0; k < P; ++k) ss = fma2(v[k], v[k], ss);
+    const float var = row_sum<kWarp>(ss.x + ss.y, red[turn][1]) / n_cols;
+    const float inv = 1.0f / sqrtf(var + a.eps);
+    float2 w[P];
+    load_param<DT, kAligned>(a.gain, a.gain_f32, w, t, nt, cols);
 #pragma unroll
-    for (int k = 0; k < HOLD; ++k) v[k] = v[k] * inv * w[k];
+    for (int k = 0; k < P; ++k) v[k] = mul2(v[k], both(inv));
     if (kLayer && a.bias) {
-      load_param<DT, kAligned, HOLD>(a.bias, a.gain_f32, w, t, nt, cols);
+      float2 b[P];
+      load_param<DT, kAligned>(a.bias, a.gain_f32, b, t, nt, cols);
 #pragma unroll
-      for (int k = 0; k < HOLD; ++k) v[k] += w[k];
+      for (int k = 0; k < P; ++k) v[k] = fma2(v[k], w[k], b[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < P; ++k) v[k] = mul2(v[k], w[k]);
     }
-    store_held<DT, kAligned, HOLD>(a.y, r * a.cols, v, t, nt, cols);
+    store_held<DT, kAligned>(a.y, r * a.cols, v, t, nt, cols);
     if (t == 0) {
       a.inv[r] = inv;
       if (kLayer) a.mean[r] = mean;
@@ -324,7 +394,7 @@ __global__ void __launch_bounds__(kMax) norm_kernel(const __grid_constant__ Norm
 // layer norm 104 and 117 us, 93 and 105 with 15 warps of 16).  Two rows at a
 // time behind one barrier cost more registers than they save waits: 130 and 146.
 // Before the ring, rows asked for one ahead in registers: 129 and 153, and
-// [16384,1920] with the RMS norm 42 and 60, now 42 and 49.
+// [16384,1920] with the RMS norm 42 and 60, 42 and 49 with it.
 constexpr int kFew = 8, kFewCols = 512 * kFew, kMaxRing = 8;
 constexpr int kRingHead = 128;  // barriers
 constexpr int kRingSmem = 220 * 1024;  // of an SM, for the rings of its blocks
@@ -394,9 +464,10 @@ __global__ void __launch_bounds__(kMax, 1024 / kMax) norm_ring_kernel(const __gr
   const RingInput in[2] = {{static_cast<const uint8_t *>(a.x), a.x_stride * SIZE},
                            {static_cast<const uint8_t *>(a.residual), a.residual_stride * SIZE}};
   const Ring g = ring_start(norm_smem, stages, a.residual ? 2 : 1, a.cols, SIZE, in, a.rows);
-  float w[HOLD], b[HOLD] = {};
-  load_param<DT, true, HOLD>(a.gain, a.gain_f32, w, t, nt, cols);
-  if (kLayer && a.bias) load_param<DT, true, HOLD>(a.bias, a.gain_f32, b, t, nt, cols);
+  constexpr int P = HOLD / 2;
+  float2 w[P], b[P] = {};
+  load_param<DT, true>(a.gain, a.gain_f32, w, t, nt, cols);
+  if (kLayer && a.bias) load_param<DT, true>(a.bias, a.gain_f32, b, t, nt, cols);
   int turn = 0, s = 0;
   uint32_t ph = 0;
   for (int64_t r = blockIdx.x; r < a.rows; r += step, turn ^= 1) {
@@ -404,35 +475,36 @@ __global__ void __launch_bounds__(kMax, 1024 / kMax) norm_ring_kernel(const __gr
     Held<DT, HOLD> x, res;
     const uint8_t *row = g.rows + s * g.inputs * g.pitch;
     x.take(row, t, nt, cols);
-    float v[HOLD];
+    float2 v[P];
 #pragma unroll
-    for (int k = 0; k < HOLD; ++k) v[k] = x.get(k);
+    for (int k = 0; k < P; ++k) v[k] = x.get(k);
     if (a.residual) {
       res.take(row + g.pitch, t, nt, cols);
 #pragma unroll
-      for (int k = 0; k < HOLD; ++k) v[k] = Elem<DT>::up(Elem<DT>::down(v[k] + res.get(k)));
-      store_held<DT, true, HOLD>(a.summed, r * a.cols, v, t, nt, cols);
+      for (int k = 0; k < P; ++k) v[k] = Pair<DT>::up(Pair<DT>::down(add2(v[k], res.get(k))));
+      store_held<DT, true>(a.summed, r * a.cols, v, t, nt, cols);
     }
-    float mean = 0.f, ss = 0.f;
+    float mean = 0.f;
+    float2 sum = both(0.f), ss = both(0.f);
     if (kLayer) {
-      float sum = 0.f;
 #pragma unroll
-      for (int k = 0; k < HOLD; ++k) sum += v[k];
-      mean = row_sum<false>(sum, red[turn][0]) / n_cols;
+      for (int k = 0; k < P; ++k) sum = add2(sum, v[k]);
+      mean = row_sum<false>(sum.x + sum.y, red[turn][0]) / n_cols;
+      center<DT>(v, mean, t, nt, cols);
     }
 #pragma unroll
-    for (int k = 0; k < HOLD; ++k) {
-      if (kLayer) v[k] = (t + k / VEC * nt) * VEC < cols ? v[k] - mean : 0.f;
-      ss = fmaf(v[k], v[k], ss);
-    }
-    ss = row_sum<false>(ss, red[turn][1]);
+    for (int k = 0; k < P; ++k) ss = fma2(v[k], v[k], ss);
+    const float var = row_sum<false>(ss.x + ss.y, red[turn][1]) / n_cols;
     // All threads have taken their columns: the stage is free.
     if (t == 0 && r + stages * step < a.rows) ring_ask(g, in, s, r + stages * step);
     if (++s == stages) s = 0, ph ^= 1;
-    const float inv = 1.0f / sqrtf(ss / n_cols + a.eps);
+    const float inv = 1.0f / sqrtf(var + a.eps);
 #pragma unroll
-    for (int k = 0; k < HOLD; ++k) v[k] = kLayer ? v[k] * inv * w[k] + b[k] : v[k] * inv * w[k];
-    store_held<DT, true, HOLD>(a.y, r * a.cols, v, t, nt, cols);
+    for (int k = 0; k < P; ++k) {
+      v[k] = mul2(v[k], both(inv));
+      v[k] = kLayer ? fma2(v[k], w[k], b[k]) : mul2(v[k], w[k]);
+    }
+    store_held<DT, true>(a.y, r * a.cols, v, t, nt, cols);
     if (t == 0) {
       a.inv[r] = inv;
       if (kLayer) a.mean[r] = mean;
@@ -503,18 +575,51 @@ __device__ __forceinline__ RowScale row_scale(const BackArgs &a, int64_t r) {
   return {fabsf(i), i < 0.f ? kSmall : 1.f, kLayer ? __ldg(a.mean + r) : 0.f};
 }
 
+// A row's n and v = w dy (v holds w before), what it adds to dw and db, and the
+// thread's part of the sums of v n and v.
+template <int DT, bool kLayer, int HOLD, int P>
+__device__ __forceinline__ void back_sums(const Held<DT, HOLD> &s, const Held<DT, HOLD> &dy, const RowScale &sc,
+                                          float2 (&n)[P], float2 (&v)[P], float2 (&dw)[P], float2 (&db)[P], float &c1,
+                                          float &c2) {
+  const float2 k2 = both(sc.k), shift = both(-sc.shift), inv = both(sc.inv), direct = both(sc.k * sc.inv);
+  float2 a1 = both(0.f), a2 = both(0.f);
+#pragma unroll
+  for (int k = 0; k < P; ++k) {
+    const float2 g = dy.get(k);
+    n[k] = kLayer ? mul2(fma2(s.get(k), k2, shift), inv) : mul2(s.get(k), direct);
+    dw[k] = fma2(g, n[k], dw[k]);
+    if (kLayer) db[k] = add2(db[k], g);
+    v[k] = mul2(v[k], g);  // (0 past the row's end)
+    a1 = fma2(v[k], n[k], a1);
+    if (kLayer) a2 = add2(a2, v[k]);
+  }
+  c1 = a1.x + a1.y;
+  c2 = a2.x + a2.y;
+}
+// dx from them, in v.
+template <int DT, int HOLD, int P>
+__device__ __forceinline__ void back_row(const float2 (&n)[P], float2 (&v)[P], const Held<DT, HOLD> &ds, bool has_ds,
+                                         const RowScale &sc, float c1, float c2) {
+  const float2 m1 = both(-c1), m2 = both(-c2), scale = both(sc.inv * sc.k);
+#pragma unroll
+  for (int k = 0; k < P; ++k) {
+    const float2 d = add2(fma2(n[k], m1, v[k]), m2);
+    v[k] = has_ds ? fma2(d, scale, ds.get(k)) : mul2(d, scale);
+  }
+}
+
 template <int DT, bool kAligned, bool kLayer, bool kWarp, int kMax, int HOLD>
 __global__ void __launch_bounds__(kMax) norm_back_kernel(const __grid_constant__ BackArgs a) {
   __shared__ float red[2][2][32];
-  __shared__ float held[kWarp ? kWarpRows * kWarpCols : 1];
+  __shared__ __align__(8) float held[kWarp ? kWarpRows * kWarpCols : 2];
   pdl_enter();
   const int t = kWarp ? threadIdx.x & 31 : threadIdx.x, nt = kWarp ? 32 : blockDim.x;
   const int cols = static_cast<int>(a.cols);
   const int64_t first = kWarp ? blockIdx.x * static_cast<int64_t>(kWarpRows) + (threadIdx.x >> 5) : blockIdx.x;
   const int64_t step = kWarp ? static_cast<int64_t>(gridDim.x) * kWarpRows : gridDim.x;
   const float one_over = 1.0f / static_cast<float>(cols);
-  constexpr int VEC = Elem<DT>::kVec;
-  float dw[HOLD] = {}, db[HOLD] = {};
+  constexpr int VEC = Elem<DT>::kVec, P = HOLD / 2;
+  float2 dw[P] = {}, db[P] = {};
   int turn = 0;
   for (int64_t r = first; r < a.rows; r += step, turn ^= 1) {
     Held<DT, HOLD> s, dy, ds;
@@ -522,47 +627,34 @@ __global__ void __launch_bounds__(kMax) norm_back_kernel(const __grid_constant__
     dy.template load<kAligned>(a.dy, r * a.dy_stride, t, nt, cols);
     if (a.dsummed) ds.template load<kAligned>(a.dsummed, r * a.dsummed_stride, t, nt, cols);
     const RowScale sc = row_scale<kLayer>(a, r);
-    float n[HOLD], v[HOLD];
-    load_param<DT, kAligned, HOLD>(a.gain, a.gain_f32, v, t, nt, cols);
-    float c1 = 0.f, c2 = 0.f;
-#pragma unroll
-    for (int k = 0; k < HOLD; ++k) {
-      const float g = dy.get(k);
-      n[k] = fmaf(s.get(k), sc.k, -sc.shift) * sc.inv;
-      dw[k] = fmaf(g, n[k], dw[k]);
-      if (kLayer) db[k] += g;
-      v[k] *= g;  // (0 past the row's end)
-      c1 = fmaf(v[k], n[k], c1);
-      if (kLayer) c2 += v[k];
-    }
+    float2 n[P], v[P];
+    load_param<DT, kAligned>(a.gain, a.gain_f32, v, t, nt, cols);
+    float c1, c2;
+    back_sums<DT, kLayer>(s, dy, sc, n, v, dw, db, c1, c2);
     if (a.dx) {
       if (kLayer) row_sums<kWarp>(c1, c2, red[turn]);
       else c1 = row_sum<kWarp>(c1, red[turn][0]);
-      c1 *= one_over, c2 *= one_over;
-#pragma unroll
-      for (int k = 0; k < HOLD; ++k) {
-        v[k] = (fmaf(-n[k], c1, v[k]) - c2) * sc.inv * sc.k;
-        if (a.dsummed) v[k] += ds.get(k);
-      }
-      store_held<DT, kAligned, HOLD>(a.dx, r * a.cols, v, t, nt, cols);
+      back_row<DT>(n, v, ds, a.dsummed != nullptr, sc, c1 * one_over, c2 * one_over);
+      store_held<DT, kAligned>(a.dx, r * a.cols, v, t, nt, cols);
     }
   }
   // The sums of this block.
-  auto put = [&](float *out, float (&sum)[HOLD]) {
+  auto put = [&](float *out, const float2 (&sum)[P]) {
     if (!out) return;
     float *o = out + static_cast<int64_t>(blockIdx.x) * a.cols;
     if (!kWarp) {
 #pragma unroll
-      for (int k = 0; k < HOLD; ++k) {
-        const int at = (t + k / VEC * nt) * VEC + k % VEC;
-        if (at < cols) o[at] = sum[k];
+      for (int k = 0; k < P; ++k) {
+        const int at = (t + 2 * k / VEC * nt) * VEC + 2 * k % VEC;
+        if (at < cols) o[at] = sum[k].x;
+        if (at + 1 < cols) o[at + 1] = sum[k].y;
       }
       return;
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < HOLD; ++k)
-      held[(threadIdx.x >> 5) * kWarpCols + (t + k / VEC * 32) * VEC + k % VEC] = sum[k];
+    for (int k = 0; k < P; ++k)
+      *reinterpret_cast<float2 *>(held + (threadIdx.x >> 5) * kWarpCols + (t + 2 * k / VEC * 32) * VEC + 2 * k % VEC) = sum[k];
     __syncthreads();
     for (int c = threadIdx.x; c < cols; c += 32 * kWarpRows) {
       float total = 0.f;
@@ -590,8 +682,9 @@ __global__ void __launch_bounds__(kMax) norm_back_ring_kernel(const __grid_const
                            {static_cast<const uint8_t *>(a.dy), a.dy_stride * SIZE},
                            {static_cast<const uint8_t *>(a.dsummed), a.dsummed_stride * SIZE}};
   const Ring g = ring_start(norm_smem, stages, a.dsummed ? 3 : 2, a.cols, SIZE, in, a.rows);
-  float w[HOLD], dw[HOLD] = {}, db[HOLD] = {};
-  load_param<DT, true, HOLD>(a.gain, a.gain_f32, w, t, nt, cols);
+  constexpr int P = HOLD / 2;
+  float2 w[P], dw[P] = {}, db[P] = {};
+  load_param<DT, true>(a.gain, a.gain_f32, w, t, nt, cols);
   int turn = 0, st = 0;
   uint32_t ph = 0;
   RowScale next = {};
@@ -605,39 +698,28 @@ __global__ void __launch_bounds__(kMax) norm_back_ring_kernel(const __grid_const
     s.take(row, t, nt, cols);
     dy.take(row + g.pitch, t, nt, cols);
     if (a.dsummed) ds.take(row + 2 * g.pitch, t, nt, cols);
-    float n[HOLD], v[HOLD], c1 = 0.f, c2 = 0.f;
+    float2 n[P], v[P];
 #pragma unroll
-    for (int k = 0; k < HOLD; ++k) {
-      const float d = dy.get(k);
-      n[k] = fmaf(s.get(k), sc.k, -sc.shift) * sc.inv;
-      dw[k] = fmaf(d, n[k], dw[k]);
-      if (kLayer) db[k] += d;
-      v[k] = w[k] * d;  // (0 past the row's end)
-      c1 = fmaf(v[k], n[k], c1);
-      if (kLayer) c2 += v[k];
-    }
+    for (int k = 0; k < P; ++k) v[k] = w[k];
+    float c1, c2;
+    back_sums<DT, kLayer>(s, dy, sc, n, v, dw, db, c1, c2);
     // (The sums' barrier also says that the stage is free.)
     if (kLayer) row_sums<false>(c1, c2, red[turn]);
     else c1 = row_sum<false>(c1, red[turn][0]);
-    c1 *= one_over, c2 *= one_over;
     if (t == 0 && r + stages * step < a.rows) ring_ask(g, in, st, r + stages * step);
     if (++st == stages) st = 0, ph ^= 1;
     if (a.dx) {
-#pragma unroll
-      for (int k = 0; k < HOLD; ++k) {
-        v[k] = (fmaf(-n[k], c1, v[k]) - c2) * sc.inv * sc.k;
-        if (a.dsummed) v[k] += ds.get(k);
-      }
-      store_held<DT, true, HOLD>(a.dx, r * a.cols, v, t, nt, cols);
+      back_row<DT>(n, v, ds, a.dsummed != nullptr, sc, c1 * one_over, c2 * one_over);
+      store_held<DT, true>(a.dx, r * a.cols, v, t, nt, cols);
     }
   }
-  auto put = [&](float *out, const float (&sum)[HOLD]) {
+  auto put = [&](float *out, const float2 (&sum)[P]) {
     if (!out) return;
     float *o = out + static_cast<int64_t>(blockIdx.x) * a.cols;
 #pragma unroll
-    for (int k = 0; k < HOLD; k += 4) {
-      const int at = (t + k / VEC * nt) * VEC + k % VEC;
-      if (at < cols) *reinterpret_cast<float4 *>(o + at) = make_float4(sum[k], sum[k + 1], sum[k + 2], sum[k + 3]);
+    for (int k = 0; k < P; k += 2) {
+      const int at = (t + 2 * k / VEC * nt) * VEC + 2 * k % VEC;
+      if (at < cols) *reinterpret_cast<float4 *>(o + at) = make_float4(sum[k].x, sum[k].y, sum[k + 1].x, sum[k + 1].y);
     }
   };
   put(a.dgain, dw);
@@ -890,7 +972,8 @@ int launch_back_typed(const Tables *T, BackArgs a, void *dgain, void *dbias, cud
     }
     if (sums) {
       // 32 groups of rows a block where that leaves the GPU in one wave, 8 where
-      // the columns alone fill it ([8192,7680], dw and db: 9.4 us with 32).
+      // the columns alone fill it ([8192,7680], dw and db: 6.4 us, 9.4 with 32).
+      // Blocks of 16 columns took 8 us instead of 6 for [16384,1920].
       using P = typename Elem<DT>::T;
       const int64_t blocks = (a.cols + kSumCols - 1) / kSumCols * (dbias ? 2 : 1);
       auto sum = [&](auto out_type, auto groups) -> int {
