@@ -12,18 +12,28 @@
 //
 // All four products run in one kernel, ce_gemm_kernel: persistent pairs of CTAs
 // on 256 x 256 tiles (tcgen05.mma.cta_group::2, operands by TMA into a ring of
-// three stages of 128 k, two accumulators in TMEM, eight epilogue warps a CTA), each
+// stages of 128 k, two accumulators in TMEM, eight epilogue warps a CTA), each
 // operand K-major or MN-major as it lies in memory, so nothing is transposed.
-//   forward: the logits' tiles end in a running maximum and a sum of
-//     exponentials a row (a TMEM lane, so a thread, holds a row);
+//   forward: the logits' tiles end in a maximum and a sum of exponentials a row
+//     (a TMEM lane, so a thread, holds a row);
 //   backward: the vocabulary goes by in pieces.  A piece's logits are computed
 //     again and end as d in 16 bits; its part of dx (added up in fp32) and its
 //     rows of dW are products with d.  One launch holds a piece's gradients and
-//     the logits of the next piece, the long tiles first, so that few SMs wait
-//     at a launch's end.
+//     the logits of the next piece, the long tiles first and each pair of SMs
+//     taking the next one as it is ready.
+// Up to 128 tokens are the tiles' columns instead, so that a tile holds 256 rows
+// of the weights whatever the tokens.
+//
 // d is rounded to the operands' type (half a step, 2^-8 relative in bf16), as
 // the tensor cores want it; in fp16 it is held times 2^15, so that probabilities
 // down to 2^-39 keep their place.
+//
+// Many tokens are bound by what an SM takes from L2: 64 KB a stage and CTA, for
+// 1,024 cycles of the tensor cores, at some 54 of 64 bytes a cycle.  [8192,1920] x
+// [50688,1920] bf16: the loss 1,037 us (1.54 PFLOP/s, 0.92 of the measured burst),
+// its gradients 3.4 ms (three products, 1.41 PFLOP/s; 1.2 to 1.3 under the power
+// cap, with the loss 5.2 ms a step).  Few are bound by the head's bytes: one token
+// and [50688,1920] 38 us of tiles (5.1 TB/s).
 #include "h24_tile.cuh"
 
 namespace h24 {
@@ -224,12 +234,11 @@ __device__ __forceinline__ uint16_t pack1(float a) {
 // What an epilogue thread does with 32 columns of its row.  `c` is the column
 // within the tile; r the sums.
 struct RowState {
-  int64_t row;   // of the job's output
   bool live;
   float lse2;    // kProb: log2e * lse - log2(prob_scale)
-  int target;    // kLoss, kProb: the target's column of the tile (any number where it is elsewhere)
-  int limit;     // kLoss, kProb: columns of the tile that the vocabulary has
-  float m, s, z; // kLoss: running maximum, sum of exponentials, the target's logit
+  int target;    // the target's column of the tile (any number where it is elsewhere)
+  int limit;     // columns of the tile that the vocabulary has
+  float m, s, z; // kLoss, few tokens: running maximum, sum of exponentials, the target's logit
   bool found;
 };
 
@@ -312,8 +321,8 @@ __device__ __forceinline__ void states_chunk(bool add, float *out, const float (
 // The order in which a pair of CTAs takes tiles.  Where tiles differ in length,
 // a pair takes the next one when it is ready for it: the first CTA's loading
 // thread counts it off in global memory and hands its number to the other warps
-// of both CTAs.  The list has the long tiles first.  (Each pair in its turn: the
-// gradients of [1024,1152] x [50688,1152] 455 us, DYN.)
+// of both CTAs.  The list has the long tiles first.  (The gradients of [1024,1152]
+// x [50688,1152] take 323 us so, 393 with each pair in its turn.)
 struct Turn {
   const GemmArgs &a;
   PairHead &H;
@@ -1013,8 +1022,8 @@ __global__ void __launch_bounds__(kRowThreads) ce_copy_head_kernel(const uint16_
 // The way back: rows of `pitch` elements on 16 bytes to rows of `in` side by
 // side at any alignment, a warp a row, whole vectors of the destination.  Where
 // dW's rows are off 16 bytes its tiles go to scratch first and then through this
-// copy: written by the element or word from the tiles they cost more (dW of
-// [333,1153] x [50257,1153] DENSE).
+// copy: written from the tiles in words of two elements they cost more (the
+// gradients of [333,1153] x [50257,1153]: 203 us, 125 and 40 of copy so).
 __global__ void __launch_bounds__(kRowThreads) ce_dense_rows_kernel(const uint16_t *src, int64_t pitch, int64_t rows,
                                                                     int in, uint16_t *out) {
   pdl_enter();
@@ -1302,7 +1311,7 @@ int logits_bn(int64_t tokens, int64_t vocab) {
 
 // Up to 128 tokens are the columns of the tiles of logits and of dx, not their
 // rows: 256 rows of which few are there would cost more of the tensor cores than
-// the weights' bytes cost of HBM (one token and [50688,1920]: 44 us, TURNED).
+// the weights' bytes cost of HBM (one token and [50688,1920]: 44 us, 38 so).
 bool few_tokens(int64_t tokens) { return tokens <= 128; }
 
 // Rows of a block of the row kernels: the blocks fill the GPU four times at most.

@@ -75,6 +75,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     red = _REDUCTIONS.get(reduction)
     if red is None:
         raise ValueError(f"reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
+    if not -2 ** 63 <= ignore_index < 2 ** 63:
+        raise ValueError(f"ignore_index must be a token number of 64 bits, got {ignore_index}")
     got = (N._torch_calls or N.torch_calls()).linear_ce(x, weight, target, ignore_index, red)
     if got is not None:
         return got
