@@ -22,7 +22,10 @@
 // each in bf16 (x, r, y, s; s, dy, dsummed, dx).  On a B200 [16384,1920] bf16
 // with the RMS norm takes 40 us forward (6.4 TB/s, 0.97 of the measured copy rate)
 // and 43 + 6 back (5.8); [8192,7680] with the layer norm 90 (5.6) and 95 + 6 (5.3).
-// Rows off 16 bytes are read and written by the element, several times slower.
+// Rows off 16 bytes cost more instructions: [8838,6946] bf16 211 us forward and
+// 165 + 6 back, where [8838,6944] takes 88 and 108 + 6 (read and written by the
+// element, as up to 1,023 rows and those of more than 16,384 columns are, 740 us
+// for both).
 #include "h24_tile.cuh"
 
 #include <type_traits>
@@ -168,6 +171,19 @@ struct Held {
       raw[i] = (t + i * nt) * VEC < cols ? *reinterpret_cast<const uint4 *>(row + (t + i * nt) * 16)
                                          : make_uint4(0, 0, 0, 0);
   }
+  // The same of a row that lies `off` bytes into its place there.
+  __device__ __forceinline__ void take_off(const uint8_t *row, uint32_t off, int t, int nt, int cols) {
+    const uint4 *p = reinterpret_cast<const uint4 *>(row);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int at = t + i * nt, left = cols - at * VEC;
+      raw[i] = make_uint4(0, 0, 0, 0);
+      if (left >= VEC)
+        raw[i] = join16(p[at], p[at + 1], off, 16);
+      else if (left > 0)
+        raw[i] = join16(p[at], p[at + 1], off, left * (16 / VEC));
+    }
+  }
   __device__ __forceinline__ float2 get(int k) const { return Pair<DT>::up(reinterpret_cast<const W *>(raw)[k]); }
 };
 
@@ -191,6 +207,41 @@ __device__ __forceinline__ void store_held(void *base, int64_t offset, const flo
       for (int j = 0; j < VEC; ++j)
         if (at + j < cols) p[at + j] = reinterpret_cast<const T *>(o)[j];
     }
+  }
+}
+
+// The same to a row anywhere: a lane puts the end of its neighbour's vector and
+// the start of its own into one block of 16 bytes; what is left at the ends of a
+// warp and of the row goes by the element.  For whole warps.
+template <int DT, int P>
+__device__ __forceinline__ void store_off(void *base, int64_t offset, const float2 (&v)[P], int t, int nt, int cols) {
+  using T = typename Elem<DT>::T;
+  using W = typename Pair<DT>::W;
+  constexpr int VEC = Elem<DT>::kVec, SIZE = 16 / VEC;
+  T *p = static_cast<T *>(base) + offset;
+  const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 15u);  // the same for all
+  const int over = static_cast<int>(off) / SIZE, first = VEC - over;  // a vector's elements in the next block, in its own
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 2 * P / VEC; ++i) {
+    const int at = t + i * nt, left = cols - at * VEC;
+    alignas(16) W o[VEC / 2];
+#pragma unroll
+    for (int j = 0; j < VEC / 2; ++j) o[j] = Pair<DT>::down(v[i * VEC / 2 + j]);
+    const uint4 mine = *reinterpret_cast<const uint4 *>(o);
+    T *to = p + at * VEC;
+    uint4 before;
+    before.x = __shfl_up_sync(0xffffffffu, mine.x, 1);
+    before.y = __shfl_up_sync(0xffffffffu, mine.y, 1);
+    before.z = __shfl_up_sync(0xffffffffu, mine.z, 1);
+    before.w = __shfl_up_sync(0xffffffffu, mine.w, 1);
+    const bool whole = left >= first && (lane > 0 || over == 0);
+    if (whole) *reinterpret_cast<uint4 *>(to - over) = over ? join16(before, mine, 16 - off, 16) : mine;
+    const T *e = reinterpret_cast<const T *>(&mine);
+    const bool tail = lane == 31 || left - VEC < first;  // the next block has no lane that writes it whole
+#pragma unroll
+    for (int j = 0; j < VEC; ++j)
+      if (j < left && (j < first ? !whole : tail)) to[j] = e[j];
   }
 }
 
@@ -416,16 +467,52 @@ struct RingInput {
   const uint8_t *base;
   int64_t stride;  // bytes
 };
+// Rows off 16 bytes (kOff) are copied with what stands around them in their first
+// and last 16 bytes, the first row and the last one, around which nothing of the
+// tensor may stand, not at all: the threads read these themselves.
+__device__ __forceinline__ bool row_at_edge(int64_t r, int64_t rows) { return r == 0 || r + 1 == rows; }
+
 // Row r of every input on its way to stage s, by one thread.
-template <int N>
-__device__ __forceinline__ void ring_ask(const Ring &g, const RingInput (&in)[N], int s, int64_t r) {
-  bar_expect(&g.full[s], g.inputs * g.bytes);
+template <bool kOff, int N>
+__device__ __forceinline__ void ring_ask(const Ring &g, const RingInput (&in)[N], int s, int64_t r, int64_t rows) {
+  uint32_t total = g.inputs * g.bytes, size[N], off[N];
+  if (kOff) {
+    total = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      off[i] = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(in[i].base + r * in[i].stride) & 15u);
+      size[i] = (off[i] + g.bytes + 15u) & ~15u;
+      if (i < g.inputs && !row_at_edge(r, rows)) total += size[i];
+    }
+  }
+  bar_expect(&g.full[s], total);
+  if (kOff && row_at_edge(r, rows)) return;
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    if (i < g.inputs) bulk_load(g.rows + (s * g.inputs + i) * g.pitch, in[i].base + r * in[i].stride, g.bytes, &g.full[s]);
+    if (i < g.inputs)
+      bulk_load(g.rows + (s * g.inputs + i) * g.pitch, in[i].base + r * in[i].stride - (kOff ? off[i] : 0u),
+                kOff ? size[i] : g.bytes, &g.full[s]);
 }
 
-template <int N>
+// The columns of input i of the row that stage s holds.
+template <bool kOff, int DT, int HOLD>
+__device__ __forceinline__ void ring_take(Held<DT, HOLD> &h, const Ring &g, const RingInput &in, int s, int i, int64_t r,
+                                          int64_t rows, int t, int nt, int cols) {
+  const uint8_t *row = g.rows + (s * g.inputs + i) * g.pitch;
+  if (!kOff)
+    h.take(row, t, nt, cols);
+  else if (row_at_edge(r, rows))
+    h.template load<false>(in.base, r * in.stride / (16 / Elem<DT>::kVec), t, nt, cols);
+  else
+    h.take_off(row, static_cast<uint32_t>(reinterpret_cast<uintptr_t>(in.base + r * in.stride) & 15u), t, nt, cols);
+}
+
+// Bytes between a stage's rows.
+__host__ __device__ __forceinline__ int ring_pitch(int64_t bytes, bool off) {
+  return static_cast<int>((bytes + (off ? 48 : 0) + 127) / 128 * 128);
+}
+
+template <bool kOff, int N>
 __device__ __forceinline__ Ring ring_start(uint8_t *smem, int stages, int inputs, int64_t cols, int size,
                                            const RingInput (&in)[N], int64_t rows) {
   Ring g;
@@ -434,7 +521,7 @@ __device__ __forceinline__ Ring ring_start(uint8_t *smem, int stages, int inputs
   g.stages = stages;
   g.inputs = inputs;
   g.bytes = static_cast<uint32_t>(cols * size);
-  g.pitch = static_cast<int>((g.bytes + 127) / 128 * 128);
+  g.pitch = ring_pitch(g.bytes, kOff);
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) bar_init(&g.full[s], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -445,12 +532,12 @@ __device__ __forceinline__ Ring ring_start(uint8_t *smem, int stages, int inputs
   if (threadIdx.x == 0) {
     asm volatile("fence.proxy.async;" ::: "memory");  // the rows were written by ordinary stores
     for (int s = 0; s < stages && blockIdx.x + static_cast<int64_t>(s) * gridDim.x < rows; ++s)
-      ring_ask(g, in, s, blockIdx.x + static_cast<int64_t>(s) * gridDim.x);
+      ring_ask<kOff>(g, in, s, blockIdx.x + static_cast<int64_t>(s) * gridDim.x, rows);
   }
   return g;
 }
 
-template <int DT, bool kLayer, int HOLD, int kMax>
+template <int DT, bool kLayer, int HOLD, int kMax, bool kOff>
 __global__ void __launch_bounds__(kMax, 1024 / kMax) norm_ring_kernel(const __grid_constant__ NormArgs a, int stages, int *err) {
   extern __shared__ __align__(128) uint8_t norm_smem[];
   __shared__ float red[2][3][32];
@@ -463,26 +550,26 @@ __global__ void __launch_bounds__(kMax, 1024 / kMax) norm_ring_kernel(const __gr
   if (t == 0) abort = 0;
   const RingInput in[2] = {{static_cast<const uint8_t *>(a.x), a.x_stride * SIZE},
                            {static_cast<const uint8_t *>(a.residual), a.residual_stride * SIZE}};
-  const Ring g = ring_start(norm_smem, stages, a.residual ? 2 : 1, a.cols, SIZE, in, a.rows);
+  const Ring g = ring_start<kOff>(norm_smem, stages, a.residual ? 2 : 1, a.cols, SIZE, in, a.rows);
   constexpr int P = HOLD / 2;
   float2 w[P], b[P] = {};
-  load_param<DT, true>(a.gain, a.gain_f32, w, t, nt, cols);
-  if (kLayer && a.bias) load_param<DT, true>(a.bias, a.gain_f32, b, t, nt, cols);
+  load_param<DT, !kOff>(a.gain, a.gain_f32, w, t, nt, cols);
+  if (kLayer && a.bias) load_param<DT, !kOff>(a.bias, a.gain_f32, b, t, nt, cols);
   int turn = 0, s = 0;
   uint32_t ph = 0;
   for (int64_t r = blockIdx.x; r < a.rows; r += step, turn ^= 1) {
     if (!bar_wait(&g.full[s], ph, &abort, err, false)) break;
     Held<DT, HOLD> x, res;
-    const uint8_t *row = g.rows + s * g.inputs * g.pitch;
-    x.take(row, t, nt, cols);
+    ring_take<kOff>(x, g, in[0], s, 0, r, a.rows, t, nt, cols);
     float2 v[P];
 #pragma unroll
     for (int k = 0; k < P; ++k) v[k] = x.get(k);
     if (a.residual) {
-      res.take(row + g.pitch, t, nt, cols);
+      ring_take<kOff>(res, g, in[1], s, 1, r, a.rows, t, nt, cols);
 #pragma unroll
       for (int k = 0; k < P; ++k) v[k] = Pair<DT>::up(Pair<DT>::down(add2(v[k], res.get(k))));
-      store_held<DT, true>(a.summed, r * a.cols, v, t, nt, cols);
+      if constexpr (kOff) store_off<DT>(a.summed, r * a.cols, v, t, nt, cols);
+      else store_held<DT, true>(a.summed, r * a.cols, v, t, nt, cols);
     }
     float mean = 0.f;
     float2 sum = both(0.f), ss = both(0.f);
@@ -496,7 +583,7 @@ __global__ void __launch_bounds__(kMax, 1024 / kMax) norm_ring_kernel(const __gr
     for (int k = 0; k < P; ++k) ss = fma2(v[k], v[k], ss);
     const float var = row_sum<false>(ss.x + ss.y, red[turn][1]) / n_cols;
     // All threads have taken their columns: the stage is free.
-    if (t == 0 && r + stages * step < a.rows) ring_ask(g, in, s, r + stages * step);
+    if (t == 0 && r + stages * step < a.rows) ring_ask<kOff>(g, in, s, r + stages * step, a.rows);
     if (++s == stages) s = 0, ph ^= 1;
     const float inv = 1.0f / sqrtf(var + a.eps);
 #pragma unroll
@@ -504,7 +591,8 @@ __global__ void __launch_bounds__(kMax, 1024 / kMax) norm_ring_kernel(const __gr
       v[k] = mul2(v[k], both(inv));
       v[k] = kLayer ? fma2(v[k], w[k], b[k]) : mul2(v[k], w[k]);
     }
-    store_held<DT, true>(a.y, r * a.cols, v, t, nt, cols);
+    if constexpr (kOff) store_off<DT>(a.y, r * a.cols, v, t, nt, cols);
+    else store_held<DT, true>(a.y, r * a.cols, v, t, nt, cols);
     if (t == 0) {
       a.inv[r] = inv;
       if (kLayer) a.mean[r] = mean;
@@ -667,7 +755,7 @@ __global__ void __launch_bounds__(kMax) norm_back_kernel(const __grid_constant__
   if (kLayer) put(a.dbias, db);
 }
 
-template <int DT, bool kLayer, int HOLD, int kMax>
+template <int DT, bool kLayer, int HOLD, int kMax, bool kOff>
 __global__ void __launch_bounds__(kMax) norm_back_ring_kernel(const __grid_constant__ BackArgs a, int stages, int *err) {
   extern __shared__ __align__(128) uint8_t norm_smem[];
   __shared__ float red[2][2][32];
@@ -681,10 +769,10 @@ __global__ void __launch_bounds__(kMax) norm_back_ring_kernel(const __grid_const
   const RingInput in[3] = {{static_cast<const uint8_t *>(a.s), a.s_stride * SIZE},
                            {static_cast<const uint8_t *>(a.dy), a.dy_stride * SIZE},
                            {static_cast<const uint8_t *>(a.dsummed), a.dsummed_stride * SIZE}};
-  const Ring g = ring_start(norm_smem, stages, a.dsummed ? 3 : 2, a.cols, SIZE, in, a.rows);
+  const Ring g = ring_start<kOff>(norm_smem, stages, a.dsummed ? 3 : 2, a.cols, SIZE, in, a.rows);
   constexpr int P = HOLD / 2;
   float2 w[P], dw[P] = {}, db[P] = {};
-  load_param<DT, true>(a.gain, a.gain_f32, w, t, nt, cols);
+  load_param<DT, !kOff>(a.gain, a.gain_f32, w, t, nt, cols);
   int turn = 0, st = 0;
   uint32_t ph = 0;
   RowScale next = {};
@@ -694,10 +782,9 @@ __global__ void __launch_bounds__(kMax) norm_back_ring_kernel(const __grid_const
     if (r + step < a.rows) next = row_scale<kLayer>(a, r + step);
     if (!bar_wait(&g.full[st], ph, &abort, err, false)) break;
     Held<DT, HOLD> s, dy, ds;
-    const uint8_t *row = g.rows + st * g.inputs * g.pitch;
-    s.take(row, t, nt, cols);
-    dy.take(row + g.pitch, t, nt, cols);
-    if (a.dsummed) ds.take(row + 2 * g.pitch, t, nt, cols);
+    ring_take<kOff>(s, g, in[0], st, 0, r, a.rows, t, nt, cols);
+    ring_take<kOff>(dy, g, in[1], st, 1, r, a.rows, t, nt, cols);
+    if (a.dsummed) ring_take<kOff>(ds, g, in[2], st, 2, r, a.rows, t, nt, cols);
     float2 n[P], v[P];
 #pragma unroll
     for (int k = 0; k < P; ++k) v[k] = w[k];
@@ -706,11 +793,12 @@ __global__ void __launch_bounds__(kMax) norm_back_ring_kernel(const __grid_const
     // (The sums' barrier also says that the stage is free.)
     if (kLayer) row_sums<false>(c1, c2, red[turn]);
     else c1 = row_sum<false>(c1, red[turn][0]);
-    if (t == 0 && r + stages * step < a.rows) ring_ask(g, in, st, r + stages * step);
+    if (t == 0 && r + stages * step < a.rows) ring_ask<kOff>(g, in, st, r + stages * step, a.rows);
     if (++st == stages) st = 0, ph ^= 1;
     if (a.dx) {
       back_row<DT>(n, v, ds, a.dsummed != nullptr, sc, c1 * one_over, c2 * one_over);
-      store_held<DT, true>(a.dx, r * a.cols, v, t, nt, cols);
+      if constexpr (kOff) store_off<DT>(a.dx, r * a.cols, v, t, nt, cols);
+      else store_held<DT, true>(a.dx, r * a.cols, v, t, nt, cols);
     }
   }
   auto put = [&](float *out, const float2 (&sum)[P]) {
@@ -719,7 +807,14 @@ __global__ void __launch_bounds__(kMax) norm_back_ring_kernel(const __grid_const
 #pragma unroll
     for (int k = 0; k < P; k += 2) {
       const int at = (t + 2 * k / VEC * nt) * VEC + 2 * k % VEC;
-      if (at < cols) *reinterpret_cast<float4 *>(o + at) = make_float4(sum[k].x, sum[k].y, sum[k + 1].x, sum[k + 1].y);
+      const float f[4] = {sum[k].x, sum[k].y, sum[k + 1].x, sum[k + 1].y};
+      if (kOff) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (at + i < cols) o[at + i] = f[i];
+      } else if (at < cols) {
+        *reinterpret_cast<float4 *>(o + at) = make_float4(f[0], f[1], f[2], f[3]);
+      }
     }
   };
   put(a.dgain, dw);
@@ -830,16 +925,22 @@ int launch_norm_rows(const NormArgs &a, int threads, cudaStream_t s) {
   return H24_OK;
 }
 
+// Whether rows off 16 bytes come through the ring: where a block has several rows,
+// so that the first and the last of all, which it reads itself, are few among
+// them.  (Inputs whose rows lie over one another, a row stride below their
+// length, do not: what stands around such a row may be outside the tensor.)
+bool ring_of_any_rows(int64_t rows, int64_t cols) { return rows >= 1024 && cols > kWarpCols; }
+
 // Stages of a ring and blocks an SM: about 200 KB of rows on their way, in
 // blocks of what the registers of an SM hold, two stages at least.
 struct RingPlan {
   int threads, stages, smem, grid;
 };
 template <auto kernel>
-int ring_plan(int64_t rows, int64_t cols, int size, int inputs, RingPlan *p) {
+int ring_plan(int64_t rows, int64_t cols, int size, int inputs, bool off, RingPlan *p) {
   H24_CUDA_TRY(allow_smem<kernel>(kRingSmem));
   p->threads = row_threads(cols);
-  const int one = static_cast<int>((cols * size + 127) / 128 * 128) * inputs;
+  const int one = ring_pitch(cols * size, off) * inputs;
   int per_sm = blocks_per_sm_once<kernel>(p->threads);
   while (per_sm > 1 && kRingSmem / per_sm < kRingHead + 2 * one) --per_sm;
   p->stages = (kRingSmem / per_sm - kRingHead - 1024) / one;
@@ -864,10 +965,10 @@ int launch_ring(K kernel, const Args &a, const RingPlan &p, int *err, cudaStream
   count_launches(1);
   return H24_OK;
 }
-template <auto kernel, int DT>
+template <auto kernel, int DT, bool kOff>
 int run_norm_ring(const Tables *T, const NormArgs &a, cudaStream_t s) {
   RingPlan p;
-  const int rc = ring_plan<kernel>(a.rows, a.cols, 16 / Elem<DT>::kVec, a.residual ? 2 : 1, &p);
+  const int rc = ring_plan<kernel>(a.rows, a.cols, 16 / Elem<DT>::kVec, a.residual ? 2 : 1, kOff, &p);
   return rc != H24_OK ? rc : launch_ring(kernel, a, p, T->err, s);
 }
 
@@ -882,16 +983,20 @@ int launch_norm_typed(const Tables *T, const NormArgs &a, cudaStream_t s) {
   const bool aligned = a.cols % kVec == 0 && a.x_stride % kVec == 0 && a.residual_stride % kVec == 0 && aligned16(a.x) &&
                        aligned16(a.residual) && aligned16(a.summed) && aligned16(a.y) && aligned16(a.gain) && aligned16(a.bias);
   const int threads = row_threads(a.cols);
+  const bool off = !aligned && ring_of_any_rows(a.rows, a.cols) && a.x_stride >= a.cols && (!a.residual || a.residual_stride >= a.cols);
   if (a.cols <= kWarpCols)
     return aligned ? launch_norm_rows<norm_kernel<DT, true, kLayer, true, 32 * kWarpRows, kHold>>(a, threads, s)
                    : launch_norm_rows<norm_kernel<DT, false, kLayer, true, 32 * kWarpRows, kHold>>(a, threads, s);
   if (a.cols <= kFewCols)
-    return aligned ? run_norm_ring<norm_ring_kernel<DT, kLayer, kFew, 512>, DT>(T, a, s)
+    return aligned ? run_norm_ring<norm_ring_kernel<DT, kLayer, kFew, 512, false>, DT, false>(T, a, s)
+           : off   ? run_norm_ring<norm_ring_kernel<DT, kLayer, kFew, 512, true>, DT, true>(T, a, s)
                    : launch_norm_rows<norm_kernel<DT, false, kLayer, false, 512, kFew>>(a, threads, s);
   if (threads <= 512)
-    return aligned ? run_norm_ring<norm_ring_kernel<DT, kLayer, kHold, 512>, DT>(T, a, s)
+    return aligned ? run_norm_ring<norm_ring_kernel<DT, kLayer, kHold, 512, false>, DT, false>(T, a, s)
+           : off   ? run_norm_ring<norm_ring_kernel<DT, kLayer, kHold, 512, true>, DT, true>(T, a, s)
                    : launch_norm_rows<norm_kernel<DT, false, kLayer, false, 512, kHold>>(a, threads, s);
-  return aligned ? run_norm_ring<norm_ring_kernel<DT, kLayer, kHold, 1024>, DT>(T, a, s)
+  return aligned ? run_norm_ring<norm_ring_kernel<DT, kLayer, kHold, 1024, false>, DT, false>(T, a, s)
+         : off   ? run_norm_ring<norm_ring_kernel<DT, kLayer, kHold, 1024, true>, DT, true>(T, a, s)
                  : launch_norm_rows<norm_kernel<DT, false, kLayer, false, 1024, kHold>>(a, threads, s);
 }
 
@@ -907,10 +1012,10 @@ int back_rows(const BackArgs &a, int grid, int threads, int *ask, cudaStream_t s
   count_launches(1);
   return H24_OK;
 }
-template <auto kernel, int DT>
+template <auto kernel, int DT, bool kOff>
 int back_ring(const Tables *T, const BackArgs &a, int *ask, cudaStream_t s) {
   RingPlan p;
-  const int rc = ring_plan<kernel>(a.rows, a.cols, 16 / Elem<DT>::kVec, a.dsummed ? 3 : 2, &p);
+  const int rc = ring_plan<kernel>(a.rows, a.cols, 16 / Elem<DT>::kVec, a.dsummed ? 3 : 2, kOff, &p);
   if (rc == H24_OK && ask) *ask = p.grid;
   return rc != H24_OK || ask ? rc : launch_ring(kernel, a, p, T->err, s);
 }
@@ -920,13 +1025,18 @@ int back_width(const Tables *T, const BackArgs &a, bool aligned, int grid, int *
   if (a.cols <= kWarpCols)
     return aligned ? back_rows<norm_back_kernel<DT, true, kLayer, true, 32 * kWarpRows, kHold>>(a, grid, threads, ask, s)
                    : back_rows<norm_back_kernel<DT, false, kLayer, true, 32 * kWarpRows, kHold>>(a, grid, threads, ask, s);
+  const bool off = !aligned && ring_of_any_rows(a.rows, a.cols) && a.s_stride >= a.cols && a.dy_stride >= a.cols &&
+                   (!a.dsummed || a.dsummed_stride >= a.cols);
   if (a.cols <= kFewCols)
-    return aligned ? back_ring<norm_back_ring_kernel<DT, kLayer, kFew, 512>, DT>(T, a, ask, s)
+    return aligned ? back_ring<norm_back_ring_kernel<DT, kLayer, kFew, 512, false>, DT, false>(T, a, ask, s)
+           : off   ? back_ring<norm_back_ring_kernel<DT, kLayer, kFew, 512, true>, DT, true>(T, a, ask, s)
                    : back_rows<norm_back_kernel<DT, false, kLayer, false, 512, kFew>>(a, grid, threads, ask, s);
   if (threads <= 512)
-    return aligned ? back_ring<norm_back_ring_kernel<DT, kLayer, kHold, 512>, DT>(T, a, ask, s)
+    return aligned ? back_ring<norm_back_ring_kernel<DT, kLayer, kHold, 512, false>, DT, false>(T, a, ask, s)
+           : off   ? back_ring<norm_back_ring_kernel<DT, kLayer, kHold, 512, true>, DT, true>(T, a, ask, s)
                    : back_rows<norm_back_kernel<DT, false, kLayer, false, 512, kHold>>(a, grid, threads, ask, s);
-  return aligned ? back_ring<norm_back_ring_kernel<DT, kLayer, kHold, 1024>, DT>(T, a, ask, s)
+  return aligned ? back_ring<norm_back_ring_kernel<DT, kLayer, kHold, 1024, false>, DT, false>(T, a, ask, s)
+         : off   ? back_ring<norm_back_ring_kernel<DT, kLayer, kHold, 1024, true>, DT, true>(T, a, ask, s)
                  : back_rows<norm_back_kernel<DT, false, kLayer, false, 1024, kHold>>(a, grid, threads, ask, s);
 }
 

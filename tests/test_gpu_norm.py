@@ -123,6 +123,52 @@ def test_norm_and_gradients(m, dtype, rows, cols, layer, residual):
     _check(m, _inputs(rows, cols, dtype, residual, layer), layer)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(1024, 513), (1025, 1153), (1500, 1930), (1111, 4100), (1060, 6947), (1030, 8198),
+                                       (1026, 16383)])
+@pytest.mark.parametrize("layer", [False, True])
+def test_many_rows_off_16_bytes(m, dtype, rows, cols, layer):
+    """Rows at every offset come through the ring, the first and the last by themselves; what lies around the outputs stays."""
+    i = _inputs(rows, cols, dtype, cols % 2 == 1, layer)
+    _check(m, i, layer)
+    for off in (1, 3):
+        for pitch in (cols, cols + 5):
+            j = dict(i)
+            for k in ("x", "residual", "dy", "dsummed"):
+                if i[k] is None:
+                    continue
+                flat = torch.full((rows * pitch + 8,), float("nan"), device="cuda", dtype=dtype)
+                j[k] = flat[off:off + rows * pitch].view(rows, pitch)[:, :cols]
+                j[k].copy_(i[k])
+            a, b = _run(m, i, layer), _run(m, j, layer)
+            assert torch.equal(a[0], b[0]) and all(torch.equal(a[2][k], b[2][k]) for k in ("x",))
+            for k in a[2]:
+                assert bool(torch.isfinite(b[2][k]).all())
+
+
+def test_outputs_off_16_bytes_leave_their_surroundings(m, lib):
+    """Through the C entry, where outputs may lie anywhere."""
+    from pollux_b200 import _native as N
+    rows, cols = 1300, 1153
+    i = _inputs(rows, cols, torch.bfloat16, True, True)
+    want = _run(m, i, True)
+    stream = torch.cuda.current_stream().cuda_stream
+    for off in range(1, 9):
+        y, s, dx = (torch.full((rows * cols + 16,), 7.0, device="cuda", dtype=torch.bfloat16) for _ in range(3))
+        stats = torch.empty(2 * rows, device="cuda")
+        at = 2 * off
+        N.check(lib.h24_add_norm(i["x"].data_ptr(), i["residual"].data_ptr(), i["weight"].data_ptr(), i["bias"].data_ptr(),
+                                 N.DTYPE_BF16, 1, rows, cols, cols, cols, N.DTYPE_BF16, 1e-5, y.data_ptr() + at,
+                                 s.data_ptr() + at, stats.data_ptr(), stream), "norm")
+        N.check(lib.h24_add_norm_backward(s.data_ptr() + at, i["weight"].data_ptr(), N.DTYPE_BF16, 1, rows, cols, cols,
+                                          N.DTYPE_BF16, stats.data_ptr(), i["dy"].data_ptr(), cols, i["dsummed"].data_ptr(),
+                                          cols, dx.data_ptr() + at, None, None, stream), "back")
+        for t, w in ((y, want[0]), (s, want[1]), (dx, want[2]["x"])):
+            assert torch.equal(t[off:off + rows * cols].view(rows, cols), w)
+            assert bool((t[:off] == 7).all()) and bool((t[off + rows * cols:] == 7).all())
+    N.check(lib.h24_check(stream), "check")
+
+
 @pytest.mark.parametrize("layer", [False, True])
 def test_parameter_types(m, layer):
     for dtype in (torch.bfloat16, torch.float16):

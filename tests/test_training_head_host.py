@@ -46,6 +46,8 @@ def test_loss_refusals(lib):
     for bad in ("avg", None, 1):
         with pytest.raises(ValueError, match="reduction"):
             ce(x, w, t, reduction=bad)
+    with pytest.raises(ValueError, match="ignore_index"):
+        ce(x, w, t, ignore_index=2 ** 63)
     with pytest.raises(TypeError, match="float16"):
         ce(x.float(), w.float(), t)
     with pytest.raises(TypeError, match="float16"):
