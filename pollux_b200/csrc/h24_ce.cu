@@ -102,6 +102,7 @@ struct GemmArgs {
   int64_t part_pitch;
   const float *scale;  // kHeadRows: factor of the sum
   float prob_scale, prob_log2;  // what d is held times, and its logarithm
+  const float *factor; // the first for each kept token; null: prob_scale for all
   int row_bytes;       // kHeadRows: rows of the output lie on 32 or on 16 bytes
   int *err;
 };
@@ -235,7 +236,8 @@ __device__ __forceinline__ uint16_t pack1(float a) {
 // within the tile; r the sums.
 struct RowState {
   bool live;
-  float lse2;    // kProb: log2e * lse - log2(prob_scale)
+  float lse2;    // kProb: log2e * lse - log2(factor)
+  float factor;  // kProb: what the row of d is held times
   int target;    // the target's column of the tile (any number where it is elsewhere)
   int limit;     // columns of the tile that the vocabulary has
   float m, s, z; // kLoss, few tokens: running maximum, sum of exponentials, the target's logit
@@ -277,17 +279,23 @@ __device__ __forceinline__ void loss_chunk(RowState &st, int c, const float (&z)
   }
 }
 
+// The row's factor; z's log-sum-exp takes its logarithm along.
+__device__ __forceinline__ void row_factor(const GemmArgs &a, int row, RowState &st) {
+  st.factor = a.factor ? a.factor[row] : a.prob_scale;
+  st.lse2 = fmaf(a.lse[row], kLog2e, -(a.factor ? log2f(st.factor) : a.prob_log2));
+}
+
 template <bool kBf16>
 __device__ __forceinline__ void prob_chunk(const GemmArgs &a, const RowState &st, uint16_t *out, int c,
                                            const float (&z)[32]) {
   float d[32];
 #pragma unroll
-  for (int j = 0; j < 32; ++j) d[j] = exp2_fast(fmaf(z[j], kLog2e, -st.lse2));  // (times prob_scale: in lse2)
+  for (int j = 0; j < 32; ++j) d[j] = exp2_fast(fmaf(z[j], kLog2e, -st.lse2));  // (times factor: in lse2)
   const int at = st.target - c;
   if (static_cast<unsigned>(at) < 32u) {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
-      if (j == at) d[j] -= a.prob_scale;
+      if (j == at) d[j] -= st.factor;
   }
   if (!st.live || c + 32 > st.limit) {
 #pragma unroll
@@ -594,7 +602,8 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
         const int token = (part ? mid : 0) + 32 * q + lane;
         RowState &st = few[q];
         st.live = token < kept && token < (part ? j.bn : mid);
-        st.lse2 = st.live && kMode == kBackward ? fmaf(a.lse[token], kLog2e, -a.prob_log2) : 0.f;
+        st.lse2 = 0.f;
+        if (kMode == kBackward && st.live) row_factor(a, token, st);
         few_target[q] = -1;
         if (st.live) {
           const int64_t label = a.labels ? a.labels[token] : a.target[token];
@@ -713,7 +722,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
       st.found = false;
       if (j.kind == kProb && st.live) {
         st.target = a.target[row] - (j.v0 + tl.n);
-        st.lse2 = fmaf(a.lse[row], kLog2e, -a.prob_log2);
+        row_factor(a, row, st);
       }
       const float scale = j.kind == kHeadRows ? *a.scale : 1.f;
       if (!__all_sync(0xffffffffu, bar_wait(&H.acc_full[acc], ph, abort, a.err))) break;
@@ -888,22 +897,45 @@ struct BackRowsArgs {
   RowSource x;
   State st;
   uint16_t *rows;    // copied states
-  uint16_t *scaled;  // the same times g / max |g|, or null (g the same for all)
+  uint16_t *scaled;  // the same times their factor's power of two (for dW), or null
+  float *factor;     // the rest of each kept token's factor times prob_scale; null: g is the same for all
+  float *power;      // each token's power of two / prob_scale
   int64_t pitch;
   const float *dloss;
   int64_t dloss_stride;
   bool mean;
-  float inv_prob_scale;
+  float prob_scale;
   float *scale;      // [0] factor of dW, [1] factor of dx where g is the same for all
   int *counters;     // of the launches that follow, set to 0
   int n_counters;
   int per_block;
 };
 
-// The copies of the backward pass.  A token's own factor g goes into its states
-// for dW, relative to the largest one (so that it neither passes the type's
-// range nor falls below it: what a much smaller factor loses is small beside
-// dW), and into dx exactly, at the end.
+// A token's factor as m * power: |power| a power of two, m in [1, 2) and held in
+// d before its rounding.  In fp16 m ends at 1.999, and then starts at half of that:
+// 2^15 * m stays below 65,504.  Zeros, infinities and NaN are all in m.
+struct Factor {
+  float m, power;
+  __device__ Factor(float g, bool half_open) {
+    m = fabsf(g);
+    power = copysignf(1.f, g);
+    if (!(m > 0.f && m < INFINITY)) return;
+    int e;
+    m = 2.f * frexpf(m, &e);
+    --e;
+    if (!half_open && m > 1.999f) {
+      m *= 0.5f;
+      ++e;
+    }
+    power = ldexpf(power, e);
+  }
+};
+
+// The copies of the backward pass.  A token's own factor is cut in two.  m goes
+// into its row of d, and is rounded with it: no rounding more, and d's relative
+// error is the one it has without.  The power of two goes into the token's states
+// for dW, relative to the largest one (exactly, but where it takes them below the
+// type's range: that is small beside dW), and into dx at the end.
 template <bool kBf16>
 __global__ void __launch_bounds__(kRowThreads) ce_back_rows_kernel(const BackRowsArgs a) {
   __shared__ float red[kRowThreads / 32];
@@ -911,7 +943,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_back_rows_kernel(const BackRow
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int kept = *a.st.kept;
   float top = 0.f;
-  if (a.scaled) {
+  if (a.factor) {
     for (int64_t i = t; i < a.x.tokens; i += kRowThreads)
       if (__ldg(a.st.place + i) >= 0) {
         const float g = fabsf(__ldg(a.dloss + i * a.dloss_stride));
@@ -923,6 +955,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_back_rows_kernel(const BackRow
     top = 0.f;
     for (int w = 0; w < kRowThreads / 32; ++w) top = fmaxf(top, red[w]);
   }
+  const float unit = Factor(top, kBf16).power;  // (1 where no factor is above 0)
   const int64_t r0 = static_cast<int64_t>(blockIdx.x) * a.per_block;
   const int rows = static_cast<int>(min(static_cast<int64_t>(a.per_block), a.x.tokens - r0)), vecs = (a.x.in + 7) / 8;
 #pragma unroll 2
@@ -932,9 +965,14 @@ __global__ void __launch_bounds__(kRowThreads) ce_back_rows_kernel(const BackRow
     if (place < 0) continue;
     const uint4 v = a.x.load(r0 + row, 8 * c);
     reinterpret_cast<uint4 *>(a.rows + place * a.pitch)[c] = v;
+    if (!a.factor) continue;
+    const Factor f(__ldg(a.dloss + (r0 + row) * a.dloss_stride), kBf16);
+    if (c == 0) {
+      a.factor[place] = f.m * a.prob_scale;
+      a.power[r0 + row] = f.power / a.prob_scale;
+    }
     if (!a.scaled) continue;
-    float g = __ldg(a.dloss + (r0 + row) * a.dloss_stride);
-    if (top > 0.f) g /= top;
+    const float g = f.m > 0.f && f.m < INFINITY ? f.power / unit : f.power;
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     uint32_t o[4];
 #pragma unroll
@@ -954,9 +992,9 @@ __global__ void __launch_bounds__(kRowThreads) ce_back_rows_kernel(const BackRow
     for (int r = kept + warp; r < end; r += kRowThreads / 32)
       for (int c = lane; c < a.x.in; c += 32) rows[r * a.pitch + c] = 0;
     if (t == 0) {
-      const float g = a.scaled ? (top > 0.f ? top : 1.f) : a.mean ? a.dloss[0] / static_cast<float>(kept) : a.dloss[0];
-      a.scale[0] = kept ? g * a.inv_prob_scale : 0.f;
-      a.scale[1] = g * a.inv_prob_scale;
+      const float g = a.factor ? unit : a.mean ? a.dloss[0] / static_cast<float>(kept) : a.dloss[0];
+      a.scale[0] = kept ? g / a.prob_scale : 0.f;
+      a.scale[1] = g / a.prob_scale;
     }
   }
 }
@@ -1179,9 +1217,7 @@ struct StatesArgs {
   int64_t tokens;
   int in;
   const float *scale;
-  const float *dloss;  // a factor for each token, or null
-  int64_t dloss_stride;
-  float inv_prob_scale;
+  const float *power;  // a factor for each token, or null: scale[1]
   uint16_t *out;
   bool vec;            // out's rows lie on 16 bytes
 };
@@ -1206,7 +1242,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_states_kernel(const StatesArgs
         v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
         v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
       }
-      const float g = a.dloss ? a.dloss[r * a.dloss_stride] * a.inv_prob_scale : a.scale[1];
+      const float g = a.power ? a.power[r] : a.scale[1];
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] *= g;
     }
@@ -1477,6 +1513,7 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   Scratch sc(s);
   const int64_t rows_at = sc.take((c.tokens + kTileK) * pitch * 2);
   const int64_t scaled_at = each && dw ? sc.take((c.tokens + kTileK) * pitch * 2) : -1;
+  const int64_t factor_at = each ? sc.take(2 * c.tokens * 4) : -1;
   const int64_t scale_at = sc.take(8), counters_at = sc.take((plan.pieces + 1) * 4);
   const int64_t w_at = head_readable(c) ? -1 : sc.take(c.vocab * pitch * 2);
   const int64_t dw_at = dw && !(c.in % 8 == 0 && aligned16(dw)) ? sc.take(c.vocab * up(c.in, 16) * 2) : -1;
@@ -1494,11 +1531,13 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   r.st = st;
   r.rows = sc.at<uint16_t>(rows_at);
   r.scaled = scaled_at < 0 ? nullptr : sc.at<uint16_t>(scaled_at);
+  r.factor = each ? sc.at<float>(factor_at) : nullptr;
+  r.power = each ? r.factor + c.tokens : nullptr;
   r.pitch = pitch;
   r.dloss = dloss;
   r.dloss_stride = dloss_stride;
   r.mean = c.reduction == H24_REDUCE_MEAN;
-  r.inv_prob_scale = 1.f / prob_scale;
+  r.prob_scale = prob_scale;
   r.scale = sc.at<float>(scale_at);
   r.counters = sc.at<int>(counters_at);
   r.n_counters = static_cast<int>(plan.pieces + 1);
@@ -1518,6 +1557,7 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   base.scale = r.scale;
   base.prob_scale = prob_scale;
   base.prob_log2 = bf16 ? 0.f : 15.f;
+  base.factor = r.factor;
   const bool dense = dw_at >= 0;
   void *head_out = dense ? sc.at<void>(dw_at) : dw;
   const int64_t head_pitch = dense ? up(c.in, 16) : c.in;
@@ -1624,9 +1664,7 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
     o.tokens = c.tokens;
     o.in = static_cast<int>(c.in);
     o.scale = r.scale;
-    o.dloss = each ? dloss : nullptr;
-    o.dloss_stride = dloss_stride;
-    o.inv_prob_scale = r.inv_prob_scale;
+    o.power = r.power;
     o.out = static_cast<uint16_t *>(dx);
     o.vec = rows_on_16(dx, c.in, c.in);
     const int64_t blocks = cdiv(c.tokens * cdiv(c.in, 8), kRowThreads);
