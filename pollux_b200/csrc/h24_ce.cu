@@ -55,9 +55,9 @@ constexpr int kBlockBytes = 32 * kBlockPitch * 4;
 constexpr int kSmem = 1024 + kHead + kRing + kEpiWarps * kBlockBytes;
 static_assert(kSmem <= 227 * 1024, "shared memory");
 // k blocks at most of a sum in the tensor cores (the loss's tiles), in slices of one length.
-template <bool kBf16>
+template <bool kBf16, bool kFew>
 __device__ __forceinline__ int slice_blocks(int nkb) {
-  constexpr int kMost = kBf16 ? 8 : 4;
+  constexpr int kMost = kFew ? (kBf16 ? 2 : 1) : kBf16 ? 8 : 4;
   const int n = (nkb + kMost - 1) / kMost;
   return (nkb + n - 1) / n;
 }
@@ -378,7 +378,8 @@ struct Turn {
 // forward pass therefore sums 1,024 k at most there, in fp16 512, and these sums
 // rounded to nearest in registers: about 1e-6 whatever the length.  Shorter
 // slices cost time, since reading a tile's TMEM takes 1,400 cycles (256 k: 2e-7,
-// and [8192,1920] x [50688,1920] 1,405 us where 1,024 k take 1,037).
+// and [8192,1920] x [50688,1920] 1,405 us where 1,024 k take 1,037).  The narrower
+// tiles of few tokens wait for HBM, and 256 and 128 k cost nothing there.
 // Probabilities rounded to 16 bits have no use for it.
 enum Mode { kBackward, kForwardRows, kForwardFew };
 template <bool kBf16, Mode kMode>
@@ -500,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
         // box; 64 k are a box of the one, half a box of the other.
         const uint64_t step_a = a_mn ? 2048 >> 4 : 32 >> 4, half_a = a_mn ? 8192 >> 4 : kBox >> 4;
         const uint64_t step_b = b_mn ? 2048 >> 4 : 32 >> 4, half_b = b_mn ? 8192 >> 4 : a.stage_b >> 5;
-        const int slice = kForward ? slice_blocks<kBf16>(tl.nkb) : 0x7fffffff;
+        const int slice = kForward ? slice_blocks<kBf16, kMode == kForwardFew>(tl.nkb) : 0x7fffffff;
         for (int i = 0, at = 0; i < max(tl.nkb, 1); ++i) {  // (at: within a slice)
           if (at == 0) {
             ok = __all_sync(0xffffffffu, bar_wait(&H.acc_empty[acc], acc_ph ^ 1, abort, a.err));
@@ -563,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
     // k after the other.  The first slice's loads are in flight together.
     auto gather = [&](auto &sum, int nkb, int c0, int c1) {
       constexpr int Q = sizeof(sum) / sizeof(sum[0]);
-      const int slice = slice_blocks<kBf16>(nkb);
+      const int slice = slice_blocks<kBf16, kMode == kForwardFew>(nkb);
       for (int i = 0; i < nkb; i += slice) {
         if (!__all_sync(0xffffffffu, bar_wait(&H.acc_full[acc], ph, abort, a.err))) return false;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
