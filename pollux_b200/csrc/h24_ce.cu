@@ -103,7 +103,7 @@ struct GemmArgs {
   const float *scale;  // kHeadRows: factor of the sum
   float prob_scale, prob_log2;  // what d is held times, and its logarithm
   const float *factor; // the first for each kept token; null: prob_scale for all
-  int row_bytes;       // kHeadRows: rows of the output lie on 32 or on 16 bytes
+  int row_bytes;       // kHeadRows: rows of the output lie on 32, 16 or 2 bytes
   int *err;
 };
 
@@ -547,6 +547,8 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
     const int quarter = uwarp & 3, part = (uwarp - 2) >> 2;  // TMEM lanes, and first or second part of the columns
     const uint32_t ta = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     float *turned = reinterpret_cast<float *>(stages + kRing) + (uwarp - 2) * 32 * kBlockPitch;
+    constexpr int kWordPitch = 17;  // the same of 16-bit elements
+    uint32_t *words = reinterpret_cast<uint32_t *>(turned);
     int acc = 0;
     uint32_t ph = 0;
     // An accumulator is free once both CTAs' warps have read it.  (The arrival
@@ -744,6 +746,26 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
           if (st.live) states_chunk(add, out32 + c, z);
         } else {
           const int left = left0 - c;
+          if (a.row_bytes == 2) {
+            // A lane holds a row.  Turned, a warp writes 32 columns of a row at a
+            // time (the gradients of [333,1153] x [50257,1153] in 133 us; with padded
+            // rows in scratch and a copy of them behind it 111 + 40, in words of two
+            // elements shifted by one in odd rows 172, from the row's lane 203).
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) words[lane * kWordPitch + i] = pack2<kBf16>(z[2 * i] * scale, z[2 * i + 1] * scale);
+            __syncwarp();
+            const int rows = min(32, j.m_total - row0);
+            const uint16_t *from = reinterpret_cast<const uint16_t *>(words) + lane;
+            uint16_t *to = out16 + c + lane - lane * pitch;
+            if (lane < left && rows == 32) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i, to += pitch) *to = from[2 * kWordPitch * i];
+            } else if (lane < left) {
+              for (int i = 0; i < rows; ++i, to += pitch) *to = from[2 * kWordPitch * i];
+            }
+            return;
+          }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t w[8];
@@ -1045,54 +1067,6 @@ __global__ void __launch_bounds__(kRowThreads) ce_copy_head_kernel(const uint16_
           if (c0 + 32 * u < vecs) to[c0 + 32 * u] = f(x[u], y[u]);
       };
       switch (off >> 1) {  // (the same for the warp)
-        case 0: put([](uint4 a, uint4 b) { return shifted<0, false>(a, b); }); break;
-        case 1: put([](uint4 a, uint4 b) { return shifted<0, true>(a, b); }); break;
-        case 2: put([](uint4 a, uint4 b) { return shifted<1, false>(a, b); }); break;
-        case 3: put([](uint4 a, uint4 b) { return shifted<1, true>(a, b); }); break;
-        case 4: put([](uint4 a, uint4 b) { return shifted<2, false>(a, b); }); break;
-        case 5: put([](uint4 a, uint4 b) { return shifted<2, true>(a, b); }); break;
-        case 6: put([](uint4 a, uint4 b) { return shifted<3, false>(a, b); }); break;
-        default: put([](uint4 a, uint4 b) { return shifted<3, true>(a, b); }); break;
-      }
-    }
-  }
-}
-
-// The way back: rows of `pitch` elements on 16 bytes to rows of `in` side by
-// side at any alignment, a warp a row, whole vectors of the destination.  Where
-// dW's rows are off 16 bytes its tiles go to scratch first and then through this
-// copy: written from the tiles in words of two elements they cost more (the
-// gradients of [333,1153] x [50257,1153]: 203 us, 125 and 40 of copy so).
-__global__ void __launch_bounds__(kRowThreads) ce_dense_rows_kernel(const uint16_t *src, int64_t pitch, int64_t rows,
-                                                                    int in, uint16_t *out) {
-  pdl_enter();
-  const int lane = threadIdx.x & 31;
-  for (int64_t r = blockIdx.x * static_cast<int64_t>(kRowThreads / 32) + (threadIdx.x >> 5); r < rows;
-       r += static_cast<int64_t>(gridDim.x) * (kRowThreads / 32)) {
-    const uint16_t *from = src + r * pitch;
-    uint16_t *to = out + r * in;
-    // Elements before the first whole vector, vectors, elements after the last.
-    const int head = min(in, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(to) & 15)) / 2 & 7));
-    const int vecs = (in - head) / 8, tail = head + 8 * vecs;
-    if (lane < head) to[lane] = from[lane];
-    if (tail + lane < in && lane < 8) to[tail + lane] = from[tail + lane];
-    uint4 *o = reinterpret_cast<uint4 *>(to + head);
-    const uint4 *f = reinterpret_cast<const uint4 *>(from);
-    constexpr int U = 4;
-    for (int c0 = lane; c0 < vecs; c0 += 32 * U) {
-      uint4 x[U], y[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int c = min(c0 + 32 * u, vecs - 1);
-        x[u] = __ldcs(f + c);
-        y[u] = __ldcs(f + min(c + 1, static_cast<int>(pitch / 8) - 1));
-      }
-      auto put = [&](auto g) {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (c0 + 32 * u < vecs) o[c0 + 32 * u] = g(x[u], y[u]);
-      };
-      switch (head) {  // (the same for the warp)
         case 0: put([](uint4 a, uint4 b) { return shifted<0, false>(a, b); }); break;
         case 1: put([](uint4 a, uint4 b) { return shifted<0, true>(a, b); }); break;
         case 2: put([](uint4 a, uint4 b) { return shifted<1, false>(a, b); }); break;
@@ -1517,7 +1491,6 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   const int64_t factor_at = each ? sc.take(2 * c.tokens * 4) : -1;
   const int64_t scale_at = sc.take(8), counters_at = sc.take((plan.pieces + 1) * 4);
   const int64_t w_at = head_readable(c) ? -1 : sc.take(c.vocab * pitch * 2);
-  const int64_t dw_at = dw && !(c.in % 8 == 0 && aligned16(dw)) ? sc.take(c.vocab * up(c.in, 16) * 2) : -1;
   const int64_t acc_at = dx ? sc.take(plan.split * c.tokens * acc_pitch * 4) : -1;
   const int64_t d_pitch = plan.piece, d_bytes = rows * d_pitch * 2;
   const int64_t d_at = sc.take(d_bytes), d2_at = plan.pieces > 1 ? sc.take(d_bytes) : d_at;
@@ -1559,10 +1532,7 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   base.prob_scale = prob_scale;
   base.prob_log2 = bf16 ? 0.f : 15.f;
   base.factor = r.factor;
-  const bool dense = dw_at >= 0;
-  void *head_out = dense ? sc.at<void>(dw_at) : dw;
-  const int64_t head_pitch = dense ? up(c.in, 16) : c.in;
-  base.row_bytes = head_pitch % 16 == 0 && (reinterpret_cast<uintptr_t>(head_out) & 31) == 0 ? 32 : 16;
+  base.row_bytes = c.in % 16 == 0 && (reinterpret_cast<uintptr_t>(dw) & 31) == 0 ? 32 : c.in % 8 == 0 && aligned16(dw) ? 16 : 2;
   base.err = T->err;
   const int64_t rows_alloc = c.tokens + kTileK;
   const uint16_t *head_rows = r.scaled ? r.scaled : r.rows;
@@ -1610,8 +1580,8 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
         j.m_total = static_cast<int>(v);
         j.split = 1;
         j.v0 = static_cast<int>(v0);
-        j.out = head_out;
-        j.pitch = head_pitch;
+        j.out = dw;
+        j.pitch = c.in;
         ok = ok && map16(&g.map[2 * g.jobs], d, d_rows, plan.piece, d_pitch, kTileK) &&
              map16(&g.map[2 * g.jobs + 1], head_rows, rows_alloc, c.in, pitch, kTileK);
         tiles += cdiv(v, kTileM) * cdiv(c.in, bn_in);
@@ -1648,12 +1618,6 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
     rc = bf16 ? launch_gemm<ce_gemm_kernel<true, kBackward>>(g, tiles, s)
               : launch_gemm<ce_gemm_kernel<false, kBackward>>(g, tiles, s);
     if (rc != H24_OK) return rc;
-  }
-  if (dense) {
-    H24_CUDA_TRY(launch_pdl(ce_dense_rows_kernel, dim3(wave_grid(cdiv(c.vocab, kRowThreads / 32), 8)), dim3(kRowThreads),
-                            s, static_cast<const uint16_t *>(head_out), head_pitch, c.vocab, static_cast<int>(c.in),
-                            static_cast<uint16_t *>(dw)));
-    count_launches(1);
   }
   if (dx) {
     StatesArgs o{};
