@@ -848,6 +848,7 @@ struct RowSource {
 struct RowsArgs {
   RowSource x;
   const int64_t *labels;
+  const int *counts;  // kept tokens of each block, or null
   int64_t ignore;
   int vocab;
   State st;
@@ -869,16 +870,64 @@ __device__ __forceinline__ int block_sum(int v, int *red) {
   return sum;
 }
 
+// What each block of a row kernel needs of all tokens, by the tokens of a block:
+// how many are kept, or the largest |g| of the kept ones.  Up to 16,384 tokens the
+// row kernels' blocks look at all tokens themselves, which costs less than one
+// launch more; with 2^20 it made 0.5 ms of [1048576,64] x [256,64]'s loss (1.8 ms)
+// and 9 ms of its gradients with a factor for each token (14.8).
+constexpr int64_t kGroupedTokens = 16384;
+struct GroupArgs {
+  const int64_t *labels;  // counts
+  int64_t ignore;
+  const int *place;       // tops
+  const float *dloss;
+  int64_t dloss_stride;
+  int64_t tokens;
+  int per_block;
+  int *counts;
+  float *tops;
+};
+__device__ __forceinline__ float larger(float top, float g) {
+  return g != g ? g : fmaxf(g, top);  // (a NaN that is overtaken here is in its row of d all the same)
+}
+// Largest of the threads' values, to all of them.
+__device__ __forceinline__ float block_top(float top, float *red) {
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+  __syncthreads();
+  top = 0.f;
+  for (int w = 0; w < kRowThreads / 32; ++w) top = fmaxf(top, red[w]);
+  return top;
+}
+__global__ void __launch_bounds__(kRowThreads) ce_groups_kernel(const GroupArgs a) {
+  __shared__ int red[kRowThreads / 32];
+  __shared__ float red_top[kRowThreads / 32];
+  pdl_enter();
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * a.per_block + threadIdx.x;
+  const bool mine = static_cast<int>(threadIdx.x) < a.per_block && r < a.tokens;
+  if (a.counts) {
+    const int count = block_sum(mine && __ldg(a.labels + r) != a.ignore, red);
+    if (threadIdx.x == 0) a.counts[blockIdx.x] = count;
+  } else {
+    const bool kept = mine && __ldg(a.place + r) >= 0;
+    const float top = block_top(kept ? larger(0.f, fabsf(__ldg(a.dloss + r * a.dloss_stride))) : 0.f, red_top);
+    if (threadIdx.x == 0) a.tops[blockIdx.x] = top;
+  }
+}
+
 // Block b takes tokens b * per_block on.  It counts the kept tokens before its
 // own, so the places are those of the tokens' order whatever the blocks' order
-// is (the targets, 8 bytes a token, lie in L2).
+// is (the targets, 8 bytes a token, lie in L2; of many tokens it adds the blocks' counts).
 __global__ void __launch_bounds__(kRowThreads) ce_rows_kernel(const RowsArgs a) {
   __shared__ int red[kRowThreads / 32], warp_base[kRowThreads / 32], from[kRowThreads];
   pdl_enter();
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int64_t r0 = static_cast<int64_t>(blockIdx.x) * a.per_block;
   int before = 0;
-  for (int64_t i = t; i < r0; i += kRowThreads) before += __ldg(a.labels + i) != a.ignore;
+  if (a.counts)
+    for (int i = t; i < static_cast<int>(blockIdx.x); i += kRowThreads) before += __ldg(a.counts + i);
+  else
+    for (int64_t i = t; i < r0; i += kRowThreads) before += __ldg(a.labels + i) != a.ignore;
   before = block_sum(before, red);
   // per_block is at most the number of threads.
   const int64_t r = r0 + t;
@@ -926,6 +975,7 @@ struct BackRowsArgs {
   int64_t pitch;
   const float *dloss;
   int64_t dloss_stride;
+  const float *tops; // largest |g| of each block's tokens, or null
   bool mean;
   float prob_scale;
   float *scale;      // [0] factor of dW, [1] factor of dx where g is the same for all
@@ -967,16 +1017,12 @@ __global__ void __launch_bounds__(kRowThreads) ce_back_rows_kernel(const BackRow
   const int kept = *a.st.kept;
   float top = 0.f;
   if (a.factor) {
-    for (int64_t i = t; i < a.x.tokens; i += kRowThreads)
-      if (__ldg(a.st.place + i) >= 0) {
-        const float g = fabsf(__ldg(a.dloss + i * a.dloss_stride));
-        top = g != g ? g : fmaxf(g, top);  // (a NaN that is overtaken here is in the states all the same)
-      }
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (lane == 0) red[warp] = top;
-    __syncthreads();
-    top = 0.f;
-    for (int w = 0; w < kRowThreads / 32; ++w) top = fmaxf(top, red[w]);
+    if (a.tops)
+      for (int i = t; i < static_cast<int>(gridDim.x); i += kRowThreads) top = larger(top, __ldg(a.tops + i));
+    else
+      for (int64_t i = t; i < a.x.tokens; i += kRowThreads)
+        if (__ldg(a.st.place + i) >= 0) top = larger(top, fabsf(__ldg(a.dloss + i * a.dloss_stride)));
+    top = block_top(top, red);
   }
   const float unit = Factor(top, kBf16).power;  // (1 where no factor is above 0)
   const int64_t r0 = static_cast<int64_t>(blockIdx.x) * a.per_block;
@@ -1170,6 +1216,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_combine_kernel(const CombineAr
   if (!last) return;
   __threadfence();
   double sum = 0.0;
+#pragma unroll 8
   for (int i = t; i < kept; i += kRowThreads) sum += static_cast<double>(__ldcg(a.row_loss + i));
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) sums[warp] = sum;
@@ -1365,6 +1412,9 @@ int launch_ce_forward(const Tables *T, const CeArgs &c, const int64_t *labels, i
   const int64_t zt_at = sc.take(c.tokens * 4), loss_at = sc.take(c.tokens * 4), ticket_at = sc.take(4);
   const int64_t parts_at = sc.take(n_parts * part_pitch * 8);
   const int64_t w_at = head_readable(c) ? -1 : sc.take(c.vocab * pitch * 2);
+  const int per_block = rows_per_block(c.tokens);
+  const int64_t row_blocks = cdiv(c.tokens, per_block);
+  const int64_t counts_at = c.tokens > kGroupedTokens ? sc.take(row_blocks * 4) : -1;
   int rc = sc.allocate(T);
   if (rc != H24_OK) return rc;
   const State st = state_at(state, c.tokens);
@@ -1384,10 +1434,20 @@ int launch_ce_forward(const Tables *T, const CeArgs &c, const int64_t *labels, i
   r.pitch = pitch;
   r.loss = c.reduction == H24_REDUCE_NONE ? loss : nullptr;
   r.ticket = sc.at<unsigned>(ticket_at);
-  r.per_block = rows_per_block(c.tokens);
+  r.per_block = per_block;
+  if (counts_at >= 0) {
+    GroupArgs q{};
+    q.labels = labels;
+    q.ignore = ignore;
+    q.tokens = c.tokens;
+    q.per_block = per_block;
+    q.counts = sc.at<int>(counts_at);
+    r.counts = q.counts;
+    H24_CUDA_TRY(launch_pdl(ce_groups_kernel, dim3(static_cast<unsigned>(row_blocks)), dim3(kRowThreads), s, q));
+    count_launches(1);
+  }
   if (!own) {
-    H24_CUDA_TRY(launch_pdl(ce_rows_kernel, dim3(static_cast<unsigned>(cdiv(c.tokens, r.per_block))), dim3(kRowThreads),
-                            s, r));
+    H24_CUDA_TRY(launch_pdl(ce_rows_kernel, dim3(static_cast<unsigned>(row_blocks)), dim3(kRowThreads), s, r));
     count_launches(1);
   }
   const void *w;
@@ -1489,6 +1549,9 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   const int64_t rows_at = sc.take((c.tokens + kTileK) * pitch * 2);
   const int64_t scaled_at = each && dw ? sc.take((c.tokens + kTileK) * pitch * 2) : -1;
   const int64_t factor_at = each ? sc.take(2 * c.tokens * 4) : -1;
+  const int per_block = rows_per_block(c.tokens);
+  const int64_t row_blocks = cdiv(c.tokens, per_block);
+  const int64_t tops_at = each && c.tokens > kGroupedTokens ? sc.take(row_blocks * 4) : -1;
   const int64_t scale_at = sc.take(8), counters_at = sc.take((plan.pieces + 1) * 4);
   const int64_t w_at = head_readable(c) ? -1 : sc.take(c.vocab * pitch * 2);
   const int64_t acc_at = dx ? sc.take(plan.split * c.tokens * acc_pitch * 4) : -1;
@@ -1515,9 +1578,21 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   r.scale = sc.at<float>(scale_at);
   r.counters = sc.at<int>(counters_at);
   r.n_counters = static_cast<int>(plan.pieces + 1);
-  r.per_block = rows_per_block(c.tokens);
+  r.per_block = per_block;
+  if (tops_at >= 0) {
+    GroupArgs q{};
+    q.place = st.place;
+    q.dloss = dloss;
+    q.dloss_stride = dloss_stride;
+    q.tokens = c.tokens;
+    q.per_block = per_block;
+    q.tops = sc.at<float>(tops_at);
+    r.tops = q.tops;
+    H24_CUDA_TRY(launch_pdl(ce_groups_kernel, dim3(static_cast<unsigned>(row_blocks)), dim3(kRowThreads), s, q));
+    count_launches(1);
+  }
   H24_CUDA_TRY(launch_pdl(bf16 ? ce_back_rows_kernel<true> : ce_back_rows_kernel<false>,
-                          dim3(static_cast<unsigned>(cdiv(c.tokens, r.per_block))), dim3(kRowThreads), s, r));
+                          dim3(static_cast<unsigned>(row_blocks)), dim3(kRowThreads), s, r));
   count_launches(1);
   const void *w;
   int64_t w_pitch;

@@ -133,6 +133,19 @@ def test_masks_and_reductions(ce, reduction, masked, dtype):
         _check(ce, x, w, target, reduction, dloss)
 
 
+@pytest.mark.parametrize("tokens,vocab,k", [(16385, 33, 40), (200001, 17, 24)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_many_tokens(ce, reduction, tokens, vocab, k):
+    """Tokens counted by blocks; the largest factor is the last kept token's."""
+    x, w, target = _inputs(tokens, vocab, k, torch.bfloat16, seed=23, masked=0.3)
+    target[-1] = 1
+    dloss = None
+    if reduction == "none":
+        dloss = torch.rand(tokens, device="cuda")
+        dloss[-1] = -37.0
+    _check(ce, x, w, target, reduction, dloss)
+
+
 @pytest.mark.parametrize("tokens", [40, 300])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_factors_of_all_sizes(ce, tokens, dtype):
