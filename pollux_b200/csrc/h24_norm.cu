@@ -13,8 +13,8 @@
 // subtracted.  Where the squares of a row of finite numbers pass fp32's range,
 // its statistics are those of s * 2^-80, and i is stored negative to say so.
 //
-// A thread holds 16 columns of a row, so a row is read once; rows of up to 512
-// columns take a warp, of up to 16,384 a block.  In the backward pass a thread
+// A thread holds 8 or 16 columns of a row, so a row is read once; rows of up to
+// 512 columns take a warp or a part of one, of up to 16,384 a block.  In the backward pass a thread
 // keeps its columns for all of its rows and adds dw and db up in registers; the
 // blocks' sums meet in a second kernel, in a fixed order.
 //
@@ -35,9 +35,9 @@ namespace {
 
 constexpr float kSmall = 8.271806125530277e-25f;  // 2^-80
 constexpr int kHold = 16;                         // columns a thread holds
-constexpr int kWarpCols = 32 * kHold;
+constexpr int kWarpCols = 32 * kHold;              // of a row that lanes of a warp hold
 constexpr int kBlockCols = 1024 * kHold;
-constexpr int kWarpRows = 8;                      // warps of a block where a warp has a row
+constexpr int kNarrowThreads = 256, kWarpRows = kNarrowThreads / 32;  // of a block with such rows
 constexpr int kLongThreads = 512;
 constexpr int kSumCols = 32;                      // of a block of the last sum
 
@@ -184,6 +184,10 @@ struct Held {
         raw[i] = join16(p[at], p[at + 1], off, left * (16 / VEC));
     }
   }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) raw[i] = make_uint4(0, 0, 0, 0);
+  }
   __device__ __forceinline__ float2 get(int k) const { return Pair<DT>::up(reinterpret_cast<const W *>(raw)[k]); }
 };
 
@@ -290,6 +294,14 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// Over each `lanes` neighbouring lanes, a power of two.
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1)
+    if (o < lanes) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
 // Sums over a row's threads: a warp, or the block (`red` is not used again
 // before a barrier that all of its threads pass).  Each warp adds up the warps'
 // sums across its lanes: one after the other they cost 30 reads of shared memory.
@@ -302,12 +314,10 @@ __device__ __forceinline__ float row_sum(float v, float *red) {
   __syncthreads();
   return warp_sum(lane < (blockDim.x >> 5) ? red[lane] : 0.f);
 }
-// Two sums behind one barrier.
-template <bool kWarp>
+// Two sums over the block behind one barrier.
 __device__ __forceinline__ void row_sums(float &v, float &w, float (*red)[32]) {
   v = warp_sum(v);
   w = warp_sum(w);
-  if (kWarp) return;
   const int lane = threadIdx.x & 31;
   if (lane == 0) red[0][threadIdx.x >> 5] = v, red[1][threadIdx.x >> 5] = w;
   __syncthreads();
@@ -317,20 +327,18 @@ __device__ __forceinline__ void row_sums(float &v, float &w, float (*red)[32]) {
 }
 
 // The finite rows among those whose statistics passed fp32's range, again and
-// by the element, from s * 2^-80.
+// by the element, from s * 2^-80.  The block had `per_block` neighbours at a time.
 template <int DT, bool kLayer, bool kWarp>
-__device__ __noinline__ void wide_rows(const NormArgs &a, float (*red)[32]) {
+__device__ __noinline__ void wide_rows(const NormArgs &a, int per_block, float (*red)[32]) {
   using E = Elem<DT>;
   using T = typename E::T;
   const int t = kWarp ? threadIdx.x & 31 : threadIdx.x, nt = kWarp ? 32 : blockDim.x;
-  const int64_t first = kWarp ? blockIdx.x * static_cast<int64_t>(kWarpRows) + (threadIdx.x >> 5) : blockIdx.x;
-  const int64_t step = kWarp ? static_cast<int64_t>(gridDim.x) * kWarpRows : gridDim.x;
   auto param = [&](const void *p, int64_t c) {
     return a.gain_f32 ? static_cast<const float *>(p)[c] : E::up(static_cast<const T *>(p)[c]);
   };
-  for (int64_t r = first; r < a.rows; r += step) {
+  auto again = [&](int64_t r) {
     const float marked = a.inv[r];
-    if (marked > 0.f && finite(marked)) continue;
+    if (marked > 0.f && finite(marked)) return;
     const T *s = a.summed ? static_cast<const T *>(a.summed) + r * a.cols : static_cast<const T *>(a.x) + r * a.x_stride;
     float sum = 0.f, bad = 0.f;
     for (int64_t c = t; c < a.cols; c += nt) {
@@ -362,17 +370,18 @@ __device__ __noinline__ void wide_rows(const NormArgs &a, float (*red)[32]) {
       }
     }
     if (!kWarp) __syncthreads();
-  }
+  };
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * per_block; r0 < a.rows; r0 += static_cast<int64_t>(gridDim.x) * per_block)
+    for (int i = kWarp ? threadIdx.x >> 5 : 0; i < per_block && r0 + i < a.rows; i += kWarp ? kWarpRows : 1) again(r0 + i);
 }
 
-template <int DT, bool kAligned, bool kLayer, bool kWarp, int kMax, int HOLD>
+template <int DT, bool kAligned, bool kLayer, int kMax, int HOLD>
 __global__ void __launch_bounds__(kMax) norm_kernel(const __grid_constant__ NormArgs a) {
   __shared__ float red[2][3][32];
   pdl_enter();
-  const int t = kWarp ? threadIdx.x & 31 : threadIdx.x, nt = kWarp ? 32 : blockDim.x;
+  const int t = threadIdx.x, nt = blockDim.x;
   const int cols = static_cast<int>(a.cols);
-  const int64_t first = kWarp ? blockIdx.x * static_cast<int64_t>(kWarpRows) + (threadIdx.x >> 5) : blockIdx.x;
-  const int64_t step = kWarp ? static_cast<int64_t>(gridDim.x) * kWarpRows : gridDim.x;
+  const int64_t first = blockIdx.x, step = gridDim.x;
   const float n_cols = static_cast<float>(cols);
   Held<DT, HOLD> x, res;
   auto ask = [&](int64_t r) {
@@ -398,12 +407,12 @@ __global__ void __launch_bounds__(kMax) norm_kernel(const __grid_constant__ Norm
     if (kLayer) {
 #pragma unroll
       for (int k = 0; k < P; ++k) sum = add2(sum, v[k]);
-      mean = row_sum<kWarp>(sum.x + sum.y, red[turn][0]) / n_cols;
+      mean = row_sum<false>(sum.x + sum.y, red[turn][0]) / n_cols;
       center<DT>(v, mean, t, nt, cols);
     }
 #pragma unroll
     for (int k = 0; k < P; ++k) ss = fma2(v[k], v[k], ss);
-    const float var = row_sum<kWarp>(ss.x + ss.y, red[turn][1]) / n_cols;
+    const float var = row_sum<false>(ss.x + ss.y, red[turn][1]) / n_cols;
     const float inv = 1.0f / sqrtf(var + a.eps);
     float2 w[P];
     load_param<DT, kAligned>(a.gain, a.gain_f32, w, t, nt, cols);
@@ -430,7 +439,76 @@ __global__ void __launch_bounds__(kMax) norm_kernel(const __grid_constant__ Norm
     bool marked = false;
     __syncthreads();
     for (int64_t r = first + t * step; r < a.rows; r += nt * step) marked |= !(a.inv[r] > 0.f && finite(a.inv[r]));
-    if (__syncthreads_or(marked)) wide_rows<DT, kLayer, kWarp>(a, red[0]);
+    if (__syncthreads_or(marked)) wide_rows<DT, kLayer, false>(a, 1, red[0]);
+  }
+}
+
+// Rows of up to 512 columns: `lanes` lanes have a row and a warp 32 / lanes of
+// them, so that no lane is left without columns ([1048576,64] bf16 55 us forward,
+// 214 with a warp a row; both directions of a training step 150 and 628).  A lane
+// holds 8, of rows of more than 256 columns 16.  The parameters stay in registers.
+template <int DT, bool kAligned, bool kLayer, int HOLD>
+__global__ void __launch_bounds__(kNarrowThreads) norm_narrow_kernel(const __grid_constant__ NormArgs a, int lanes) {
+  __shared__ float red[3][32];
+  pdl_enter();
+  constexpr int P = HOLD / 2;
+  const int t = threadIdx.x & (lanes - 1), cols = static_cast<int>(a.cols), per_block = kNarrowThreads / lanes;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * per_block;
+  const int mine = threadIdx.x / lanes;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * per_block + mine;
+  const int ahead = mine - (threadIdx.x & ~31) / lanes;  // of the warp's first row
+  const float n_cols = static_cast<float>(cols);
+  float2 w[P], b[P] = {};
+  load_param<DT, kAligned>(a.gain, a.gain_f32, w, t, lanes, cols);
+  if (kLayer && a.bias) load_param<DT, kAligned>(a.bias, a.gain_f32, b, t, lanes, cols);
+  Held<DT, HOLD> x, res;
+  auto ask = [&](int64_t r) {
+    if (r >= a.rows) return;
+    x.template load<kAligned>(a.x, r * a.x_stride, t, lanes, cols);
+    if (a.residual) res.template load<kAligned>(a.residual, r * a.residual_stride, t, lanes, cols);
+  };
+  x.clear();
+  res.clear();
+  ask(first);
+  for (int64_t r = first; r - ahead < a.rows; r += step) {  // (as often for the whole warp)
+    float2 v[P];
+#pragma unroll
+    for (int k = 0; k < P; ++k) v[k] = x.get(k);
+    if (a.residual) {
+#pragma unroll
+      for (int k = 0; k < P; ++k) v[k] = Pair<DT>::up(Pair<DT>::down(add2(v[k], res.get(k))));
+    }
+    ask(r + step);
+    const bool live = r < a.rows;
+    if (a.summed && live) store_held<DT, kAligned>(a.summed, r * a.cols, v, t, lanes, cols);
+    float mean = 0.f;
+    float2 sum = both(0.f), ss = both(0.f);
+    if (kLayer) {
+#pragma unroll
+      for (int k = 0; k < P; ++k) sum = add2(sum, v[k]);
+      mean = lanes_sum(sum.x + sum.y, lanes) / n_cols;
+      center<DT>(v, mean, t, lanes, cols);
+    }
+#pragma unroll
+    for (int k = 0; k < P; ++k) ss = fma2(v[k], v[k], ss);
+    const float var = lanes_sum(ss.x + ss.y, lanes) / n_cols;
+    const float inv = 1.0f / sqrtf(var + a.eps);
+#pragma unroll
+    for (int k = 0; k < P; ++k) v[k] = mul2(v[k], both(inv));
+#pragma unroll
+    for (int k = 0; k < P; ++k) v[k] = kLayer && a.bias ? fma2(v[k], w[k], b[k]) : mul2(v[k], w[k]);
+    if (!live) continue;
+    store_held<DT, kAligned>(a.y, r * a.cols, v, t, lanes, cols);
+    if (t == 0) {
+      a.inv[r] = inv;
+      if (kLayer) a.mean[r] = mean;
+    }
+  }
+  if (DT != H24_DTYPE_F16) {  // as above
+    bool marked = false;
+    __syncthreads();
+    for (int64_t r = first + t * step; r < a.rows; r += lanes * step) marked |= !(a.inv[r] > 0.f && finite(a.inv[r]));
+    if (__syncthreads_or(marked)) wide_rows<DT, kLayer, true>(a, per_block, red);
   }
 }
 
@@ -602,7 +680,7 @@ __global__ void __launch_bounds__(kMax, 1024 / kMax) norm_ring_kernel(const __gr
     bool marked = false;
     __syncthreads();
     for (int64_t r = blockIdx.x + t * step; r < a.rows; r += nt * step) marked |= !(a.inv[r] > 0.f && finite(a.inv[r]));
-    if (__syncthreads_or(marked)) wide_rows<DT, kLayer, false>(a, red[0]);
+    if (__syncthreads_or(marked)) wide_rows<DT, kLayer, false>(a, 1, red[0]);
   }
 }
 
@@ -645,7 +723,7 @@ __global__ void __launch_bounds__(kLongThreads) norm_long_kernel(const __grid_co
   if (DT != H24_DTYPE_F16) {
     const bool marked = !(inv > 0.f && finite(inv));  // (the same for the whole block)
     __syncthreads();
-    if (marked) wide_rows<DT, kLayer, false>(a, red);
+    if (marked) wide_rows<DT, kLayer, false>(a, 1, red);
   }
 }
 
@@ -696,15 +774,13 @@ __device__ __forceinline__ void back_row(const float2 (&n)[P], float2 (&v)[P], c
   }
 }
 
-template <int DT, bool kAligned, bool kLayer, bool kWarp, int kMax, int HOLD>
+template <int DT, bool kAligned, bool kLayer, int kMax, int HOLD>
 __global__ void __launch_bounds__(kMax) norm_back_kernel(const __grid_constant__ BackArgs a) {
   __shared__ float red[2][2][32];
-  __shared__ __align__(8) float held[kWarp ? kWarpRows * kWarpCols : 2];
   pdl_enter();
-  const int t = kWarp ? threadIdx.x & 31 : threadIdx.x, nt = kWarp ? 32 : blockDim.x;
+  const int t = threadIdx.x, nt = blockDim.x;
   const int cols = static_cast<int>(a.cols);
-  const int64_t first = kWarp ? blockIdx.x * static_cast<int64_t>(kWarpRows) + (threadIdx.x >> 5) : blockIdx.x;
-  const int64_t step = kWarp ? static_cast<int64_t>(gridDim.x) * kWarpRows : gridDim.x;
+  const int64_t first = blockIdx.x, step = gridDim.x;
   const float one_over = 1.0f / static_cast<float>(cols);
   constexpr int VEC = Elem<DT>::kVec, P = HOLD / 2;
   float2 dw[P] = {}, db[P] = {};
@@ -720,8 +796,8 @@ __global__ void __launch_bounds__(kMax) norm_back_kernel(const __grid_constant__
     float c1, c2;
     back_sums<DT, kLayer>(s, dy, sc, n, v, dw, db, c1, c2);
     if (a.dx) {
-      if (kLayer) row_sums<kWarp>(c1, c2, red[turn]);
-      else c1 = row_sum<kWarp>(c1, red[turn][0]);
+      if (kLayer) row_sums(c1, c2, red[turn]);
+      else c1 = row_sum<false>(c1, red[turn][0]);
       back_row<DT>(n, v, ds, a.dsummed != nullptr, sc, c1 * one_over, c2 * one_over);
       store_held<DT, kAligned>(a.dx, r * a.cols, v, t, nt, cols);
     }
@@ -730,24 +806,85 @@ __global__ void __launch_bounds__(kMax) norm_back_kernel(const __grid_constant__
   auto put = [&](float *out, const float2 (&sum)[P]) {
     if (!out) return;
     float *o = out + static_cast<int64_t>(blockIdx.x) * a.cols;
-    if (!kWarp) {
 #pragma unroll
-      for (int k = 0; k < P; ++k) {
-        const int at = (t + 2 * k / VEC * nt) * VEC + 2 * k % VEC;
-        if (at < cols) o[at] = sum[k].x;
-        if (at + 1 < cols) o[at + 1] = sum[k].y;
-      }
-      return;
+    for (int k = 0; k < P; ++k) {
+      const int at = (t + 2 * k / VEC * nt) * VEC + 2 * k % VEC;
+      if (at < cols) o[at] = sum[k].x;
+      if (at + 1 < cols) o[at + 1] = sum[k].y;
+    }
+  };
+  put(a.dgain, dw);
+  if (kLayer) put(a.dbias, db);
+}
+
+// Rows of up to 512 columns, as in the forward pass; each lane adds dw and db up
+// over its rows, and the block over its lanes with the same columns.
+template <int DT, bool kAligned, bool kLayer, int HOLD>
+__global__ void __launch_bounds__(kNarrowThreads) norm_back_narrow_kernel(const __grid_constant__ BackArgs a, int lanes) {
+  __shared__ __align__(8) float held[kNarrowThreads * HOLD];
+  pdl_enter();
+  constexpr int VEC = Elem<DT>::kVec, P = HOLD / 2;
+  const int t = threadIdx.x & (lanes - 1), cols = static_cast<int>(a.cols), per_block = kNarrowThreads / lanes;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * per_block;
+  const int mine = threadIdx.x / lanes;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * per_block + mine;
+  const int ahead = mine - (threadIdx.x & ~31) / lanes;
+  const float one_over = 1.0f / static_cast<float>(cols);
+  float2 w[P], dw[P] = {}, db[P] = {};
+  load_param<DT, kAligned>(a.gain, a.gain_f32, w, t, lanes, cols);
+  Held<DT, HOLD> s, dy, ds;
+  RowScale sc;
+  auto ask = [&](int64_t r) {
+    s.clear();
+    dy.clear();
+    ds.clear();
+    sc = {0.f, 1.f, 0.f};
+    if (r >= a.rows) return;
+    s.template load<kAligned>(a.s, r * a.s_stride, t, lanes, cols);
+    dy.template load<kAligned>(a.dy, r * a.dy_stride, t, lanes, cols);
+    if (a.dsummed) ds.template load<kAligned>(a.dsummed, r * a.dsummed_stride, t, lanes, cols);
+    sc = row_scale<kLayer>(a, r);
+  };
+  ask(first);
+  for (int64_t r = first; r - ahead < a.rows; r += step) {
+    float2 n[P], v[P];
+    float c1, c2;
+#pragma unroll
+    for (int k = 0; k < P; ++k) v[k] = w[k];
+    back_sums<DT, kLayer>(s, dy, sc, n, v, dw, db, c1, c2);
+    const Held<DT, HOLD> own = ds;
+    const RowScale scale = sc;
+    ask(r + step);
+    if (a.dx) {
+      c1 = lanes_sum(c1, lanes);
+      if (kLayer) c2 = lanes_sum(c2, lanes);
+      back_row<DT>(n, v, own, a.dsummed != nullptr, scale, c1 * one_over, c2 * one_over);
+      if (r < a.rows) store_held<DT, kAligned>(a.dx, r * a.cols, v, t, lanes, cols);
+    }
+  }
+  // The sums of this block: of a warp's rows across its lanes, then of the warps.
+  const int row_cols = lanes * HOLD;
+  auto put = [&](float *out, const float2 (&sum)[P]) {
+    if (!out) return;
+    float *o = out + static_cast<int64_t>(blockIdx.x) * a.cols;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      float2 v = sum[k];
+#pragma unroll
+      for (int o = 16; o; o >>= 1)
+        if (o >= lanes) {
+          v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+          v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+        }
+      if ((threadIdx.x & 31) < lanes)
+        *reinterpret_cast<float2 *>(held + (threadIdx.x >> 5) * row_cols + (t + 2 * k / VEC * lanes) * VEC + 2 * k % VEC) = v;
     }
     __syncthreads();
-#pragma unroll
-    for (int k = 0; k < P; ++k)
-      *reinterpret_cast<float2 *>(held + (threadIdx.x >> 5) * kWarpCols + (t + 2 * k / VEC * 32) * VEC + 2 * k % VEC) = sum[k];
-    __syncthreads();
-    for (int c = threadIdx.x; c < cols; c += 32 * kWarpRows) {
+    for (int c = threadIdx.x; c < cols; c += kNarrowThreads) {
       float total = 0.f;
 #pragma unroll
-      for (int w = 0; w < kWarpRows; ++w) total += held[w * kWarpCols + c];
+      for (int g = 0; g < kWarpRows; ++g) total += held[g * row_cols + c];
       o[c] = total;
     }
   };
@@ -791,7 +928,7 @@ __global__ void __launch_bounds__(kMax) norm_back_ring_kernel(const __grid_const
     float c1, c2;
     back_sums<DT, kLayer>(s, dy, sc, n, v, dw, db, c1, c2);
     // (The sums' barrier also says that the stage is free.)
-    if (kLayer) row_sums<false>(c1, c2, red[turn]);
+    if (kLayer) row_sums(c1, c2, red[turn]);
     else c1 = row_sum<false>(c1, red[turn][0]);
     if (t == 0 && r + stages * step < a.rows) ring_ask<kOff>(g, in, st, r + stages * step, a.rows);
     if (++st == stages) st = 0, ph ^= 1;
@@ -842,7 +979,7 @@ __global__ void __launch_bounds__(kLongThreads) norm_back_long_kernel(const __gr
     c1 = fmaf(v, fmaf(E::up(s[c]), sc.k, -sc.shift) * sc.inv, c1);
     if (kLayer) c2 += v;
   }
-  row_sums<false>(c1, c2, red);
+  row_sums(c1, c2, red);
   c1 *= one_over, c2 *= one_over;
   for (int64_t c = threadIdx.x; c < a.cols; c += kLongThreads) {
     const float n = fmaf(E::up(s[c]), sc.k, -sc.shift) * sc.inv;
@@ -910,17 +1047,30 @@ __global__ void __launch_bounds__(kSumCols * kSumGroups) norm_sums_kernel(const 
 // whether a row comes through the ring or not, its sums have the same order: a
 // row's result does not depend on where it lies.
 int row_threads(int64_t cols) {
-  if (cols <= kWarpCols) return 32 * kWarpRows;
   const int hold = cols <= kFewCols ? kFew : kHold;
   return static_cast<int>(((cols + hold - 1) / hold + 31) / 32 * 32);
 }
+// Lanes of a row of up to kWarpCols columns.
+int narrow_lanes(int64_t cols) {
+  const int hold = cols > 32 * kFew ? kHold : kFew;
+  int lanes = 1;
+  while (lanes * hold < cols) lanes *= 2;
+  return lanes;
+}
 template <auto kernel>
-int norm_grid(int64_t rows, int64_t cols, int threads) {
-  return wave_grid(cols <= kWarpCols ? (rows + kWarpRows - 1) / kWarpRows : rows, blocks_per_sm_once<kernel>(threads));
+int narrow_grid(int64_t rows, int64_t cols) {
+  const int per_block = kNarrowThreads / narrow_lanes(cols);
+  return wave_grid((rows + per_block - 1) / per_block, blocks_per_sm_once<kernel>(kNarrowThreads));
+}
+template <auto kernel>
+int launch_norm_narrow(const NormArgs &a, cudaStream_t s) {
+  H24_CUDA_TRY(launch_pdl(kernel, dim3(narrow_grid<kernel>(a.rows, a.cols)), dim3(kNarrowThreads), s, a, narrow_lanes(a.cols)));
+  count_launches(1);
+  return H24_OK;
 }
 template <auto kernel>
 int launch_norm_rows(const NormArgs &a, int threads, cudaStream_t s) {
-  H24_CUDA_TRY(launch_pdl(kernel, dim3(norm_grid<kernel>(a.rows, a.cols, threads)), dim3(threads), s, a));
+  H24_CUDA_TRY(launch_pdl(kernel, dim3(wave_grid(a.rows, blocks_per_sm_once<kernel>(threads))), dim3(threads), s, a));
   count_launches(1);
   return H24_OK;
 }
@@ -982,22 +1132,25 @@ int launch_norm_typed(const Tables *T, const NormArgs &a, cudaStream_t s) {
   }
   const bool aligned = a.cols % kVec == 0 && a.x_stride % kVec == 0 && a.residual_stride % kVec == 0 && aligned16(a.x) &&
                        aligned16(a.residual) && aligned16(a.summed) && aligned16(a.y) && aligned16(a.gain) && aligned16(a.bias);
+  if (a.cols <= 32 * kFew)
+    return aligned ? launch_norm_narrow<norm_narrow_kernel<DT, true, kLayer, kFew>>(a, s)
+                   : launch_norm_narrow<norm_narrow_kernel<DT, false, kLayer, kFew>>(a, s);
+  if (a.cols <= kWarpCols)
+    return aligned ? launch_norm_narrow<norm_narrow_kernel<DT, true, kLayer, kHold>>(a, s)
+                   : launch_norm_narrow<norm_narrow_kernel<DT, false, kLayer, kHold>>(a, s);
   const int threads = row_threads(a.cols);
   const bool off = !aligned && ring_of_any_rows(a.rows, a.cols) && a.x_stride >= a.cols && (!a.residual || a.residual_stride >= a.cols);
-  if (a.cols <= kWarpCols)
-    return aligned ? launch_norm_rows<norm_kernel<DT, true, kLayer, true, 32 * kWarpRows, kHold>>(a, threads, s)
-                   : launch_norm_rows<norm_kernel<DT, false, kLayer, true, 32 * kWarpRows, kHold>>(a, threads, s);
   if (a.cols <= kFewCols)
     return aligned ? run_norm_ring<norm_ring_kernel<DT, kLayer, kFew, 512, false>, DT, false>(T, a, s)
            : off   ? run_norm_ring<norm_ring_kernel<DT, kLayer, kFew, 512, true>, DT, true>(T, a, s)
-                   : launch_norm_rows<norm_kernel<DT, false, kLayer, false, 512, kFew>>(a, threads, s);
+                   : launch_norm_rows<norm_kernel<DT, false, kLayer, 512, kFew>>(a, threads, s);
   if (threads <= 512)
     return aligned ? run_norm_ring<norm_ring_kernel<DT, kLayer, kHold, 512, false>, DT, false>(T, a, s)
            : off   ? run_norm_ring<norm_ring_kernel<DT, kLayer, kHold, 512, true>, DT, true>(T, a, s)
-                   : launch_norm_rows<norm_kernel<DT, false, kLayer, false, 512, kHold>>(a, threads, s);
+                   : launch_norm_rows<norm_kernel<DT, false, kLayer, 512, kHold>>(a, threads, s);
   return aligned ? run_norm_ring<norm_ring_kernel<DT, kLayer, kHold, 1024, false>, DT, false>(T, a, s)
          : off   ? run_norm_ring<norm_ring_kernel<DT, kLayer, kHold, 1024, true>, DT, true>(T, a, s)
-                 : launch_norm_rows<norm_kernel<DT, false, kLayer, false, 1024, kHold>>(a, threads, s);
+                 : launch_norm_rows<norm_kernel<DT, false, kLayer, 1024, kHold>>(a, threads, s);
 }
 
 // The backward kernel of rows that a block holds: its grid (one wave; asked for
@@ -1005,10 +1158,20 @@ int launch_norm_typed(const Tables *T, const NormArgs &a, cudaStream_t s) {
 template <auto kernel>
 int back_rows(const BackArgs &a, int grid, int threads, int *ask, cudaStream_t s) {
   if (ask) {
-    *ask = norm_grid<kernel>(a.rows, a.cols, threads);
+    *ask = wave_grid(a.rows, blocks_per_sm_once<kernel>(threads));
     return H24_OK;
   }
   H24_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(threads), s, a));
+  count_launches(1);
+  return H24_OK;
+}
+template <auto kernel>
+int back_narrow(const BackArgs &a, int grid, int *ask, cudaStream_t s) {
+  if (ask) {
+    *ask = narrow_grid<kernel>(a.rows, a.cols);
+    return H24_OK;
+  }
+  H24_CUDA_TRY(launch_pdl(kernel, dim3(grid), dim3(kNarrowThreads), s, a, narrow_lanes(a.cols)));
   count_launches(1);
   return H24_OK;
 }
@@ -1021,23 +1184,26 @@ int back_ring(const Tables *T, const BackArgs &a, int *ask, cudaStream_t s) {
 }
 template <int DT, bool kLayer>
 int back_width(const Tables *T, const BackArgs &a, bool aligned, int grid, int *ask, cudaStream_t s) {
-  const int threads = row_threads(a.cols);
+  if (a.cols <= 32 * kFew)
+    return aligned ? back_narrow<norm_back_narrow_kernel<DT, true, kLayer, kFew>>(a, grid, ask, s)
+                   : back_narrow<norm_back_narrow_kernel<DT, false, kLayer, kFew>>(a, grid, ask, s);
   if (a.cols <= kWarpCols)
-    return aligned ? back_rows<norm_back_kernel<DT, true, kLayer, true, 32 * kWarpRows, kHold>>(a, grid, threads, ask, s)
-                   : back_rows<norm_back_kernel<DT, false, kLayer, true, 32 * kWarpRows, kHold>>(a, grid, threads, ask, s);
+    return aligned ? back_narrow<norm_back_narrow_kernel<DT, true, kLayer, kHold>>(a, grid, ask, s)
+                   : back_narrow<norm_back_narrow_kernel<DT, false, kLayer, kHold>>(a, grid, ask, s);
+  const int threads = row_threads(a.cols);
   const bool off = !aligned && ring_of_any_rows(a.rows, a.cols) && a.s_stride >= a.cols && a.dy_stride >= a.cols &&
                    (!a.dsummed || a.dsummed_stride >= a.cols);
   if (a.cols <= kFewCols)
     return aligned ? back_ring<norm_back_ring_kernel<DT, kLayer, kFew, 512, false>, DT, false>(T, a, ask, s)
            : off   ? back_ring<norm_back_ring_kernel<DT, kLayer, kFew, 512, true>, DT, true>(T, a, ask, s)
-                   : back_rows<norm_back_kernel<DT, false, kLayer, false, 512, kFew>>(a, grid, threads, ask, s);
+                   : back_rows<norm_back_kernel<DT, false, kLayer, 512, kFew>>(a, grid, threads, ask, s);
   if (threads <= 512)
     return aligned ? back_ring<norm_back_ring_kernel<DT, kLayer, kHold, 512, false>, DT, false>(T, a, ask, s)
            : off   ? back_ring<norm_back_ring_kernel<DT, kLayer, kHold, 512, true>, DT, true>(T, a, ask, s)
-                   : back_rows<norm_back_kernel<DT, false, kLayer, false, 512, kHold>>(a, grid, threads, ask, s);
+                   : back_rows<norm_back_kernel<DT, false, kLayer, 512, kHold>>(a, grid, threads, ask, s);
   return aligned ? back_ring<norm_back_ring_kernel<DT, kLayer, kHold, 1024, false>, DT, false>(T, a, ask, s)
          : off   ? back_ring<norm_back_ring_kernel<DT, kLayer, kHold, 1024, true>, DT, true>(T, a, ask, s)
-                 : back_rows<norm_back_kernel<DT, false, kLayer, false, 1024, kHold>>(a, grid, threads, ask, s);
+                 : back_rows<norm_back_kernel<DT, false, kLayer, 1024, kHold>>(a, grid, threads, ask, s);
 }
 
 template <int DT, bool kLayer>

@@ -124,6 +124,15 @@ def test_norm_and_gradients(m, dtype, rows, cols, layer, residual):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(1000, 1), (5001, 2), (700, 5), (70003, 8), (333, 9), (2050, 16), (30, 17), (50001, 64),
+                                       (777, 65), (1001, 127), (20000, 128), (900, 129), (901, 256), (500, 257), (601, 500)])
+@pytest.mark.parametrize("layer", [False, True])
+def test_narrow_rows(m, dtype, rows, cols, layer):
+    """Several rows a warp, as the norms of a model's heads have them."""
+    _check(m, _inputs(rows, cols, dtype, cols % 2 == 0, layer), layer)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,cols", [(1024, 513), (1025, 1153), (1500, 1930), (1111, 4100), (1060, 6947), (1030, 8198),
                                        (1026, 16383)])
 @pytest.mark.parametrize("layer", [False, True])
@@ -216,7 +225,7 @@ def test_strides_and_shapes(m, cols, layer):
     assert torch.equal(a[0], b[0]) and torch.equal(a[2]["x"], b[2]["x"]) and torch.equal(a[2]["weight"], b[2]["weight"])
 
 
-@pytest.mark.parametrize("cols", [48, 1920, 20001])
+@pytest.mark.parametrize("cols", [5, 48, 64, 200, 300, 1920, 20001])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("layer", [False, True])
 def test_rows_beyond_the_range_of_squares(m, cols, dtype, layer):
