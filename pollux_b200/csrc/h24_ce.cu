@@ -32,7 +32,7 @@
 // 1,024 cycles of the tensor cores, at some 54 of 64 bytes a cycle.  [8192,1920] x
 // [50688,1920] bf16: the loss 1,037 us (1.54 PFLOP/s, 0.92 of the measured burst),
 // its gradients 3.4 ms (three products, 1.41 PFLOP/s; 1.2 to 1.3 under the power
-// cap, with the loss 5.2 ms a step).  Few are bound by the head's bytes: one token
+// cap, with the loss 5.1 ms a step).  Few are bound by the head's bytes: one token
 // and [50688,1920] 38 us of tiles (5.1 TB/s).
 #include "h24_tile.cuh"
 
