@@ -301,8 +301,8 @@ int h24_linear_ce_forward(const void *x, int64_t tokens, int64_t x_stride, const
  * d before its rounding, its power of two in x for dw) or one.  dx (tokens x in_features)
  * and dw (vocab x in_features) are contiguous and of `dtype`; either may be
  * NULL.  The logits are computed again, for a piece of the vocabulary at a
- * time; scratch as above, and 2 * 192 MiB at most for the pieces (more where 256
- * columns of all tokens are more) and 4 bytes for each element of dx and slice
+ * time; scratch as above, and 2 * 192 MiB at most for the pieces (or 2 * 4,096
+ * columns of all tokens, where that is more) and 4 bytes for each element of dx and slice
  * of its sum. */
 int h24_linear_ce_backward(const void *x, int64_t tokens, int64_t x_stride, const void *w, int64_t vocab,
                            int64_t w_stride, int64_t in_features, int dtype, int reduction,

@@ -1283,7 +1283,12 @@ __global__ void __launch_bounds__(kRowThreads) ce_states_kernel(const StatesArgs
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
-constexpr int64_t kPieceBytes = int64_t(192) << 20;  // of d, for one piece of the vocabulary
+// Bytes of d for one piece of the vocabulary, and the columns that it has at
+// least: with many tokens narrow pieces cost more in dx's fp32 sums, which are
+// read and written for each, and leave too few tiles of dW (with 192 MiB alone
+// [131072,1920] x [50688,1920] 108 ms a step, 87 so; [262144,1024] x [4096,1024] 29
+// and 9).
+constexpr int64_t kPieceBytes = int64_t(192) << 20, kPieceCols = 4096;
 
 // Map of a matrix of 16-bit elements [rows][cols], row pitch `pitch` elements,
 // in boxes of 64 columns x box_rows with the 128-byte swizzle.
@@ -1522,7 +1527,7 @@ BackPlan back_plan(const CeArgs &c, bool want_states, bool want_head) {
   BackPlan p;
   const int64_t rows = up(c.tokens, kTileM);
   const int64_t most = kPieceBytes / (rows * 2) / kTileN * kTileN;
-  p.pieces = cdiv(c.vocab, most < kTileN ? kTileN : most);
+  p.pieces = cdiv(c.vocab, most < kPieceCols ? kPieceCols : most);
   p.piece = up(cdiv(c.vocab, p.pieces), kTileN);
   p.pieces = cdiv(c.vocab, p.piece);
   // A dx tile sums over a whole piece.  Slices of it where that is more than a
