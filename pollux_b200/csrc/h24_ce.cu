@@ -244,6 +244,12 @@ struct RowState {
   bool found;
 };
 
+// The maximum that exponents are taken from.  2^((z - m) log2 e) is 1 where z is the
+// maximum, with no rounding that would grow from join to join (z log2 e less a
+// rounded m log2 e is off by as much as that rounding: 2^-24 of the logit each
+// time, and a certain token's loss got below 0), so a sum is never below 1.
+__device__ __forceinline__ float exp_base(float m) { return m == kNegInf ? 0.f : m; }
+
 __device__ __forceinline__ void loss_chunk(RowState &st, int c, const float (&z)[32]) {
   float top = kNegInf;
   if (c + 32 <= st.limit) {
@@ -255,18 +261,18 @@ __device__ __forceinline__ void loss_chunk(RowState &st, int c, const float (&z)
       if (c + j < st.limit) top = fmaxf(top, z[j]);
   }
   const float m = fmaxf(st.m, top);
-  const float base = m == kNegInf ? 0.f : m * kLog2e;
-  float s0 = st.s * exp2_fast(fmaf(st.m, kLog2e, -base)), s1 = 0.f;  // (2^-inf is 0)
+  const float base = exp_base(m);
+  float s0 = st.s * exp2_fast((st.m - base) * kLog2e), s1 = 0.f;  // (2^-inf is 0)
   if (c + 32 <= st.limit) {
 #pragma unroll
     for (int j = 0; j < 32; j += 2) {
-      s0 += exp2_fast(fmaf(z[j], kLog2e, -base));
-      s1 += exp2_fast(fmaf(z[j + 1], kLog2e, -base));
+      s0 += exp2_fast((z[j] - base) * kLog2e);
+      s1 += exp2_fast((z[j + 1] - base) * kLog2e);
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
-      if (c + j < st.limit) s0 += exp2_fast(fmaf(z[j], kLog2e, -base));
+      if (c + j < st.limit) s0 += exp2_fast((z[j] - base) * kLog2e);
   }
   st.s = s0 + s1;
   st.m = m;
@@ -691,12 +697,12 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
 #pragma unroll
           for (int k = 1; k < 32; ++k) top[q] = fmaxf(top[q], z(q, k));
         }
-        const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), base = m == kNegInf ? 0.f : m * kLog2e;
+        const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), base = exp_base(m);
         float part_sum[4] = {};
 #pragma unroll
         for (int k = 0; k < 32; ++k)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) part_sum[q] += exp2_fast(fmaf(z(q, k), kLog2e, -base));
+          for (int q = 0; q < 4; ++q) part_sum[q] += exp2_fast((z(q, k) - base) * kLog2e);
         const int row = tl.m + rank * (kTileM / 2) + quarter * 32 + lane;
         if (row < kept) {
           a.parts[(static_cast<int64_t>(tl.n / j.bn) * 2 + part) * a.part_pitch + row] =
@@ -1180,8 +1186,8 @@ __global__ void __launch_bounds__(kRowThreads) ce_combine_kernel(const CombineAr
   const int r = t % ROWS;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * ROWS + r;
   auto join = [](float2 &p, float2 q) {
-    const float m = fmaxf(p.x, q.x), base = m == kNegInf ? 0.f : m * kLog2e;
-    p.y = p.y * exp2_fast(fmaf(p.x, kLog2e, -base)) + q.y * exp2_fast(fmaf(q.x, kLog2e, -base));
+    const float m = fmaxf(p.x, q.x), base = exp_base(m);
+    p.y = p.y * exp2_fast((p.x - base) * kLog2e) + q.y * exp2_fast((q.x - base) * kLog2e);
     p.x = m;
   };
   float2 p = make_float2(kNegInf, 0.f);
@@ -1198,8 +1204,8 @@ __global__ void __launch_bounds__(kRowThreads) ce_combine_kernel(const CombineAr
     for (int w = 1; w < kRowThreads / 32; ++w) join(p, red[w][t]);
     // A target outside the vocabulary has no loss: NaN, here and in the gradients.
     if (!own) known = a.st.target[row] >= 0;
-    const float lse = known ? p.x + logf(p.y) : __int_as_float(0x7fffffff);
-    const float loss = known ? lse - a.z_target[row] : lse;
+    const float rest = known ? logf(p.y) : __int_as_float(0x7fffffff), lse = p.x + rest;
+    const float loss = known ? (p.x - a.z_target[row]) + rest : rest;  // (both parts are 0 or more)
     a.st.lse[own ? place : row] = lse;
     if (a.reduction == H24_REDUCE_NONE)
       a.loss[own ? row : a.token[row]] = loss;
