@@ -36,6 +36,8 @@
 // and [50688,1920] 38 us of tiles (5.1 TB/s).
 #include "h24_tile.cuh"
 
+#include <type_traits>
+
 namespace h24 {
 namespace {
 
@@ -54,10 +56,11 @@ constexpr int kBlockPitch = 33;  // fp32 of a row of an epilogue warp's 32 x 32 
 constexpr int kBlockBytes = 32 * kBlockPitch * 4;
 constexpr int kSmem = 1024 + kHead + kRing + kEpiWarps * kBlockBytes;
 static_assert(kSmem <= 227 * 1024, "shared memory");
-// k blocks at most of a sum in the tensor cores (the loss's tiles), in slices of one length.
-template <bool kBf16, bool kFew>
+constexpr int kBackBf16 = 32, kBackHalf = 11;  // (bf16, fp16)
+// k blocks at most of a logit's sum in the tensor cores, in slices of one length.
+template <bool kBf16, bool kForward, bool kFew>
 __device__ __forceinline__ int slice_blocks(int nkb) {
-  constexpr int kMost = kFew ? (kBf16 ? 2 : 1) : kBf16 ? 8 : 4;
+  constexpr int kMost = !kForward ? (kBf16 ? kBackBf16 : kBackHalf) : kFew ? (kBf16 ? 2 : 1) : kBf16 ? 8 : 4;
   const int n = (nkb + kMost - 1) / kMost;
   return (nkb + n - 1) / n;
 }
@@ -97,12 +100,13 @@ struct GemmArgs {
   unsigned *ticket;       // set to 0, where kept is null
   const int *target;   // of each kept token
   const float *lse;    // of each kept token
+  const float *own;    // d at each kept token's target, times what its row of d is held times
   float *z_target;
   float2 *parts;       // kLoss: maximum and sum of half a tile's columns
   int64_t part_pitch;
   const float *scale;  // kHeadRows: factor of the sum
-  float prob_scale, prob_log2;  // what d is held times, and its logarithm
-  const float *factor; // the first for each kept token; null: prob_scale for all
+  const float *log_factor; // log2 of what each kept token's row of d is held times; null: prob_log2 for all
+  float prob_log2;
   int row_bytes;       // kHeadRows: rows of the output lie on 32, 16 or 2 bytes
   int *err;
 };
@@ -236,8 +240,9 @@ __device__ __forceinline__ uint16_t pack1(float a) {
 // within the tile; r the sums.
 struct RowState {
   bool live;
-  float lse2;    // kProb: log2e * lse - log2(factor)
-  float factor;  // kProb: what the row of d is held times
+  float lse;     // kProb
+  float log2f;   // kProb: log2 of what the row of d is held times
+  float own;     // kProb: the target's d, times that
   int target;    // the target's column of the tile (any number where it is elsewhere)
   int limit;     // columns of the tile that the vocabulary has
   float m, s, z; // kLoss, few tokens: running maximum, sum of exponentials, the target's logit
@@ -285,23 +290,24 @@ __device__ __forceinline__ void loss_chunk(RowState &st, int c, const float (&z)
   }
 }
 
-// The row's factor; z's log-sum-exp takes its logarithm along.
-__device__ __forceinline__ void row_factor(const GemmArgs &a, int row, RowState &st) {
-  st.factor = a.factor ? a.factor[row] : a.prob_scale;
-  st.lse2 = fmaf(a.lse[row], kLog2e, -(a.factor ? log2f(st.factor) : a.prob_log2));
+__device__ __forceinline__ void prob_row(const GemmArgs &a, int row, RowState &st) {
+  st.lse = a.lse[row];
+  st.log2f = a.log_factor ? a.log_factor[row] : a.prob_log2;
+  st.own = a.own[row];
 }
 
+// The target's d is p - 1, which of a certain token's p would keep nothing but
+// roundings; it comes from the loss instead, as expm1(-loss).
 template <bool kBf16>
-__device__ __forceinline__ void prob_chunk(const GemmArgs &a, const RowState &st, uint16_t *out, int c,
-                                           const float (&z)[32]) {
+__device__ __forceinline__ void prob_chunk(const RowState &st, uint16_t *out, int c, const float (&z)[32]) {
   float d[32];
 #pragma unroll
-  for (int j = 0; j < 32; ++j) d[j] = exp2_fast(fmaf(z[j], kLog2e, -st.lse2));  // (times factor: in lse2)
+  for (int j = 0; j < 32; ++j) d[j] = exp2_fast(fmaf(z[j] - st.lse, kLog2e, st.log2f));
   const int at = st.target - c;
   if (static_cast<unsigned>(at) < 32u) {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
-      if (j == at) d[j] -= st.factor;
+      if (j == at) d[j] = st.own;
   }
   if (!st.live || c + 32 > st.limit) {
 #pragma unroll
@@ -386,11 +392,19 @@ struct Turn {
 // slices cost time, since reading a tile's TMEM takes 1,400 cycles (256 k: 2e-7,
 // and [8192,1920] x [50688,1920] 1,405 us where 1,024 k take 1,037).  The narrower
 // tiles of few tokens wait for HBM, and 256 and 128 k cost nothing there.
-// Probabilities rounded to 16 bits have no use for it.
-enum Mode { kBackward, kForwardRows, kForwardFew };
-template <bool kBf16, Mode kMode>
+// The backward pass's probabilities are rounded to 16 bits, and the one entry that
+// is a difference comes from the loss: slices of 4,096 k, in fp16 1,408, keep z
+// to 4.4e-6 of itself, so a probability of a logit of 30 to 2^-13, where half a
+// step is 2^-9 and 2^-12.
+//
+// kFew: up to 128 tokens, the columns of the tiles of logits and of dx.  kLong: a
+// sum in several slices, for which an epilogue thread holds 128 of them: always in
+// the forward pass, in the backward pass where k is longer than a slice.  (Within
+// one kernel for both the gradients of [1024,1152] x [50688,1152] took 567 us, 479
+// without; the long kernel's spills cost a step of [8192,1920] x [50688,1920] in
+// fp16 5.1 ms instead of 4.8, and of [1024,7680] x [50688,7680] in bf16 nothing.)
+template <bool kBf16, bool kForward, bool kFew, bool kLong>
 __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_constant__ GemmArgs a) {
-  constexpr bool kForward = kMode != kBackward;
   extern __shared__ uint8_t ce_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(ce_raw) + 1023) & ~uintptr_t(1023));
   PairHead &H = *reinterpret_cast<PairHead *>(smem);
@@ -431,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
   const uint32_t tmem = H.tmem;
   pdl_enter();
   const int kept = a.kept ? *a.kept : a.tokens;
-  if (kMode == kForwardFew && a.ticket && blockIdx.x == 0 && t == 0) *a.ticket = 0;
+  if (kForward && kFew && a.ticket && blockIdx.x == 0 && t == 0) *a.ticket = 0;
   int tiles = 0;
   for (int j = 0; j < a.jobs; ++j) tiles += tiles_of(a.job[j], kept);
   Turn turn{a, H, a.next_tile != nullptr && kept > 0, tiles, 0, abort};  // (without a token no tile has a k block)
@@ -507,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
         // box; 64 k are a box of the one, half a box of the other.
         const uint64_t step_a = a_mn ? 2048 >> 4 : 32 >> 4, half_a = a_mn ? 8192 >> 4 : kBox >> 4;
         const uint64_t step_b = b_mn ? 2048 >> 4 : 32 >> 4, half_b = b_mn ? 8192 >> 4 : a.stage_b >> 5;
-        const int slice = kForward ? slice_blocks<kBf16, kMode == kForwardFew>(tl.nkb) : 0x7fffffff;
+        const int slice = kForward || (kLong && j.kind == kProb) ? slice_blocks<kBf16, kForward, kFew>(tl.nkb) : 0x7fffffff;
         for (int i = 0, at = 0; i < max(tl.nkb, 1); ++i) {  // (at: within a slice)
           if (at == 0) {
             ok = __all_sync(0xffffffffu, bar_wait(&H.acc_empty[acc], acc_ph ^ 1, abort, a.err));
@@ -568,11 +582,10 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
                      : "memory");
       if (++acc == 2) acc = 0, ph ^= 1;
     };
-    // The bits of the sums of a tile's columns c0 + 32 q, for the loss: a slice of
-    // k after the other.  The first slice's loads are in flight together.
-    auto gather = [&](auto &sum, int nkb, int c0, int c1) {
+    // The bits of the logits of a tile's columns c0 + 32 q: a slice of k after the
+    // other.  The first slice's loads are in flight together.
+    auto gather = [&](auto &sum, int nkb, int slice, int c0, int c1) {
       constexpr int Q = sizeof(sum) / sizeof(sum[0]);
-      const int slice = slice_blocks<kBf16, kMode == kForwardFew>(nkb);
       for (int i = 0; i < nkb; i += slice) {
         if (!__all_sync(0xffffffffu, bar_wait(&H.acc_full[acc], ph, abort, a.err))) return false;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -602,8 +615,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
     };
     RowState few[2];  // of this lane's tokens where they are the tiles' columns: kept from tile to tile
     int few_target[2];
-    const bool swapped = kMode == kForwardFew || (kMode == kBackward && (a.job[a.jobs - 1].swap || a.job[0].swap));
-    if (swapped) {
+    if (kFew) {
       const Job &j = a.job[a.job[0].swap ? 0 : a.jobs - 1];
       const int mid = (j.bn / 2 + 31) / 32 * 32;
 #pragma unroll
@@ -611,8 +623,8 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
         const int token = (part ? mid : 0) + 32 * q + lane;
         RowState &st = few[q];
         st.live = token < kept && token < (part ? j.bn : mid);
-        st.lse2 = 0.f;
-        if (kMode == kBackward && st.live) row_factor(a, token, st);
+        st.lse = st.log2f = st.own = 0.f;
+        if (!kForward && st.live) prob_row(a, token, st);
         few_target[q] = -1;
         if (st.live) {
           const int64_t label = a.labels ? a.labels[token] : a.target[token];
@@ -629,17 +641,18 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
       const Tile tl = tile_at(a, kept, idx);
       const Job &j = a.job[tl.job];
       const int mid = (tl.cols / 2 + 31) / 32 * 32, c0 = part ? mid : 0, c1 = part ? tl.cols : mid;
-      if (kMode == kForwardRows) {  // (asked for ahead of the wait)
+      if (kForward && !kFew) {  // (asked for ahead of the wait)
         const int row = tl.m + rank * (kTileM / 2) + quarter * 32 + lane;
         few_target[0] = row < kept ? a.target[row] : -1;
       }
-      if (kMode == kForwardFew || (kMode == kBackward && j.swap)) {
+      if (kFew && (kForward || j.swap)) {
         // A lane holds a row of the weights and the columns are tokens: 32 x 32 of
         // them turn in shared memory, and each lane goes on with a token's row.
         const int row0 = tl.m + rank * (kTileM / 2) + quarter * 32;
-        int sum[kForward ? 2 : 1][32];
-        if (kForward) {
-          if (!gather(sum, tl.nkb, c0, c1)) break;
+        int sum[kLong ? 2 : 1][32];
+        const bool logits = kForward || (kLong && j.kind == kProb);
+        if (logits) {
+          if (!gather(sum, tl.nkb, slice_blocks<kBf16, kForward, kFew>(tl.nkb), c0, c1)) break;
         } else {
           if (!__all_sync(0xffffffffu, bar_wait(&H.acc_full[acc], ph, abort, a.err))) break;
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -650,9 +663,9 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
           if (c >= c1) break;
           float z[32];
           __syncwarp();
-          if (kForward) {
+          if (logits) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) turned[lane * kBlockPitch + i] = __int_as_float(sum[kForward ? q : 0][i]);
+            for (int i = 0; i < 32; ++i) turned[lane * kBlockPitch + i] = __int_as_float(sum[kLong ? q : 0][i]);
           } else {
             int r[32];
             tmem_ask32(ta + acc * kTileN + c, r);
@@ -669,17 +682,17 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
           if (kForward) {
             loss_chunk(st, 0, z);
           } else if (j.kind == kProb) {
-            prob_chunk<kBf16>(a, st, static_cast<uint16_t *>(j.out) + token * j.pitch + row0, 0, z);
+            prob_chunk<kBf16>(st, static_cast<uint16_t *>(j.out) + token * j.pitch + row0, 0, z);
           } else if (st.live && row0 < j.pitch) {
             states_chunk(j.add, static_cast<float *>(j.out) + tl.slice * j.plane + token * j.pitch + row0, z);
           }
         }
-        if (!kForward) release();
+        if (!logits) release();
         continue;
       }
-      if constexpr (kMode == kForwardRows) {
+      if constexpr (kForward && !kFew) {
         int sum[4][32];
-        if (!gather(sum, tl.nkb, c0, c1)) break;
+        if (!gather(sum, tl.nkb, slice_blocks<kBf16, kForward, kFew>(tl.nkb), c0, c1)) break;
         auto z = [&](int q, int k) -> float { return __int_as_float(sum[q][k]); };
         const int limit = a.vocab - tl.n;
         if (c1 > limit || c0 + 128 > c1) {  // columns that are not there
@@ -724,19 +737,16 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
       RowState st;
       st.live = row < (j.kind == kHeadRows ? j.m_total : kept);
       st.target = 0x7fffffff;
-      st.lse2 = 0.f;
+      st.lse = st.log2f = st.own = 0.f;
       st.limit = a.vocab - (j.v0 + tl.n);
       st.m = kNegInf;
       st.s = st.z = 0.f;
       st.found = false;
-      if (j.kind == kProb && st.live) {
+      if (!kFew && j.kind == kProb && st.live) {
         st.target = a.target[row] - (j.v0 + tl.n);
-        row_factor(a, row, st);
+        prob_row(a, row, st);
       }
       const float scale = j.kind == kHeadRows ? *a.scale : 1.f;
-      if (!__all_sync(0xffffffffu, bar_wait(&H.acc_full[acc], ph, abort, a.err))) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t d = ta + acc * kTileN;
       const int kind = j.kind, left0 = j.n_total - tl.n;
       const int64_t pitch = j.pitch;
       const bool add = j.add;
@@ -746,8 +756,8 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
         float z[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) z[i] = __int_as_float(r[i]);
-        if (kind == kProb) {
-          prob_chunk<kBf16>(a, st, out16, c, z);
+        if (!kFew && kind == kProb) {
+          prob_chunk<kBf16>(st, out16, c, z);
         } else if (kind == kStates) {
           if (st.live) states_chunk(add, out32 + c, z);
         } else {
@@ -787,10 +797,25 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
           }
         }
       };
+      if (!kFew && kLong && kind == kProb) {
+        int sum[4][32];
+        if (!gather(sum, tl.nkb, slice_blocks<kBf16, kForward, kFew>(tl.nkb), c0, c1)) break;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (c0 + 32 * q >= c1) break;
+          float z[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) z[i] = __int_as_float(sum[q][i]);
+          prob_chunk<kBf16>(st, out16, c0 + 32 * q, z);
+        }
+        continue;
+      }
+      if (!__all_sync(0xffffffffu, bar_wait(&H.acc_full[acc], ph, abort, a.err))) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       for (int c = c0; c < c1; c += 32) {
         int r[32];
         __syncwarp();
-        tmem_ask32(d + c, r);
+        tmem_ask32(ta + acc * kTileN + c, r);
         tmem_wait32(r);
         if (tl.nkb == 0) {  // an empty sum has no MMA
 #pragma unroll
@@ -800,7 +825,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
       }
       release();
     }
-    if (kMode == kForwardFew) {
+    if (kForward && kFew) {
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         const int token = (part ? (a.job[0].bn / 2 + 31) / 32 * 32 : 0) + 32 * q + lane;
@@ -825,15 +850,16 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
 constexpr int kRowThreads = 256;
 
 // What the forward pass leaves for the backward pass: the number of kept
-// tokens, each token's place among them (-1: ignored), and by place the target
-// (-1: not in the vocabulary) and the log of the sum of exponentials.
+// tokens, each token's target (kNoTarget: not in the vocabulary, kIgnored), and
+// by the kept tokens' places the log of the sum of exponentials and the loss.
+constexpr int kNoTarget = -1, kIgnored = -2;
 struct State {
-  int *kept, *place, *target;
-  float *lse;
+  int *kept, *target;
+  float *lse, *loss;
 };
 State state_at(const int32_t *state, int64_t tokens) {
   int32_t *p = const_cast<int32_t *>(state);  // (only the forward pass writes it)
-  return {p, p + 1, p + 1 + tokens, reinterpret_cast<float *>(p + 1 + 2 * tokens)};
+  return {p, p + 1, reinterpret_cast<float *>(p + 1 + tokens), reinterpret_cast<float *>(p + 1 + 2 * tokens)};
 }
 
 // 8 elements at a row's element c (a multiple of 8) of x, from any alignment;
@@ -858,7 +884,7 @@ struct RowsArgs {
   int64_t ignore;
   int vocab;
   State st;
-  int *token;      // of each place
+  int *token, *target;  // of each place
   uint16_t *rows;  // copied states, `pitch` elements a row
   int64_t pitch;
   float *loss;     // of each token, or null
@@ -876,17 +902,32 @@ __device__ __forceinline__ int block_sum(int v, int *red) {
   return sum;
 }
 
+// The place of the thread's token among the block's kept ones, and their number.
+__device__ __forceinline__ int block_place(bool keep, int *count, int *warp_base) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const unsigned votes = __ballot_sync(0xffffffffu, keep);
+  if (lane == 0) warp_base[warp] = __popc(votes);
+  __syncthreads();
+  int at = __popc(votes & ((1u << lane) - 1));
+  *count = 0;
+  for (int w = 0; w < kRowThreads / 32; ++w) {
+    if (w < warp) at += warp_base[w];
+    *count += warp_base[w];
+  }
+  return at;
+}
+
 // What each block of a row kernel needs of all tokens, by the tokens of a block:
-// how many are kept, or the largest |g| of the kept ones.  Up to 16,384 tokens the
+// how many are kept, and the largest |g| of the kept ones.  Up to 16,384 tokens the
 // row kernels' blocks look at all tokens themselves, which costs less than one
 // launch more; with 2^20 it made 0.5 ms of [1048576,64] x [256,64]'s loss (1.8 ms)
 // and 9 ms of its gradients with a factor for each token (14.8).
 constexpr int64_t kGroupedTokens = 16384;
 struct GroupArgs {
-  const int64_t *labels;  // counts
+  const int64_t *labels;  // forward: the targets as they are given
   int64_t ignore;
-  const int *place;       // tops
-  const float *dloss;
+  const int *target;      // backward: the state's
+  const float *dloss;     // null: no tops
   int64_t dloss_stride;
   int64_t tokens;
   int per_block;
@@ -911,14 +952,12 @@ __global__ void __launch_bounds__(kRowThreads) ce_groups_kernel(const GroupArgs 
   pdl_enter();
   const int64_t r = static_cast<int64_t>(blockIdx.x) * a.per_block + threadIdx.x;
   const bool mine = static_cast<int>(threadIdx.x) < a.per_block && r < a.tokens;
-  if (a.counts) {
-    const int count = block_sum(mine && __ldg(a.labels + r) != a.ignore, red);
-    if (threadIdx.x == 0) a.counts[blockIdx.x] = count;
-  } else {
-    const bool kept = mine && __ldg(a.place + r) >= 0;
-    const float top = block_top(kept ? larger(0.f, fabsf(__ldg(a.dloss + r * a.dloss_stride))) : 0.f, red_top);
-    if (threadIdx.x == 0) a.tops[blockIdx.x] = top;
-  }
+  const bool kept = mine && (a.labels ? __ldg(a.labels + r) != a.ignore : __ldg(a.target + r) != kIgnored);
+  const int count = block_sum(kept, red);
+  if (threadIdx.x == 0) a.counts[blockIdx.x] = count;
+  if (!a.dloss) return;
+  const float top = block_top(kept ? larger(0.f, fabsf(__ldg(a.dloss + r * a.dloss_stride))) : 0.f, red_top);
+  if (threadIdx.x == 0) a.tops[blockIdx.x] = top;
 }
 
 // Block b takes tokens b * per_block on.  It counts the kept tokens before its
@@ -927,9 +966,9 @@ __global__ void __launch_bounds__(kRowThreads) ce_groups_kernel(const GroupArgs 
 __global__ void __launch_bounds__(kRowThreads) ce_rows_kernel(const RowsArgs a) {
   __shared__ int red[kRowThreads / 32], warp_base[kRowThreads / 32], from[kRowThreads];
   pdl_enter();
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int t = threadIdx.x;
   const int64_t r0 = static_cast<int64_t>(blockIdx.x) * a.per_block;
-  int before = 0;
+  int before = 0, count;
   if (a.counts)
     for (int i = t; i < static_cast<int>(blockIdx.x); i += kRowThreads) before += __ldg(a.counts + i);
   else
@@ -940,22 +979,16 @@ __global__ void __launch_bounds__(kRowThreads) ce_rows_kernel(const RowsArgs a) 
   const bool mine = t < a.per_block && r < a.x.tokens;
   const int64_t label = mine ? __ldg(a.labels + r) : a.ignore;
   const bool keep = mine && label != a.ignore;
-  const unsigned votes = __ballot_sync(0xffffffffu, keep);
-  if (lane == 0) warp_base[warp] = __popc(votes);
-  __syncthreads();
-  int at = __popc(votes & ((1u << lane) - 1)), count = 0;
-  for (int w = 0; w < kRowThreads / 32; ++w) {
-    if (w < warp) at += warp_base[w];
-    count += warp_base[w];
-  }
+  const int at = block_place(keep, &count, warp_base);
+  const int target = !keep ? kIgnored : label >= 0 && label < a.vocab ? static_cast<int>(label) : kNoTarget;
   if (mine) {
-    a.st.place[r] = keep ? before + at : -1;
+    a.st.target[r] = target;
     if (!keep && a.loss) a.loss[r] = 0.f;
   }
   if (keep) {
     from[at] = t;
-    a.st.target[before + at] = label >= 0 && label < a.vocab ? static_cast<int>(label) : -1;
-    if (a.token) a.token[before + at] = static_cast<int>(r);
+    a.target[before + at] = target;
+    a.token[before + at] = static_cast<int>(r);
   }
   __syncthreads();
   const int vecs = (a.x.in + 7) / 8;
@@ -976,12 +1009,16 @@ struct BackRowsArgs {
   State st;
   uint16_t *rows;    // copied states
   uint16_t *scaled;  // the same times their factor's power of two (for dW), or null
-  float *factor;     // the rest of each kept token's factor times prob_scale; null: g is the same for all
+  int *place;        // of each token among the kept ones (-1: ignored)
+  int *target;       // of each kept token
+  float *own;        // and d there, times what its row of d is held times
+  float *log_factor; // log2 of the rest of each kept token's factor times prob_scale; null: g is the same for all
   float *power;      // each token's power of two / prob_scale
   int64_t pitch;
   const float *dloss;
   int64_t dloss_stride;
-  const float *tops; // largest |g| of each block's tokens, or null
+  const int *counts; // kept tokens and largest |g| of each block's tokens, or null
+  const float *tops;
   bool mean;
   float prob_scale;
   float *scale;      // [0] factor of dW, [1] factor of dx where g is the same for all
@@ -1017,37 +1054,62 @@ struct Factor {
 // type's range: that is small beside dW), and into dx at the end.
 template <bool kBf16>
 __global__ void __launch_bounds__(kRowThreads) ce_back_rows_kernel(const BackRowsArgs a) {
-  __shared__ float red[kRowThreads / 32];
+  __shared__ float red[kRowThreads / 32], powers[kRowThreads];
+  __shared__ int sums[kRowThreads / 32], warp_base[kRowThreads / 32], places[kRowThreads];
   pdl_enter();
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int kept = *a.st.kept;
-  float top = 0.f;
-  if (a.factor) {
-    if (a.tops)
-      for (int i = t; i < static_cast<int>(gridDim.x); i += kRowThreads) top = larger(top, __ldg(a.tops + i));
-    else
-      for (int64_t i = t; i < a.x.tokens; i += kRowThreads)
-        if (__ldg(a.st.place + i) >= 0) top = larger(top, fabsf(__ldg(a.dloss + i * a.dloss_stride)));
-    top = block_top(top, red);
-  }
-  const float unit = Factor(top, kBf16).power;  // (1 where no factor is above 0)
   const int64_t r0 = static_cast<int64_t>(blockIdx.x) * a.per_block;
+  const bool each = a.log_factor != nullptr;
+  float top = 0.f;
+  int before = 0, count;
+  if (a.counts) {
+    for (int i = t; i < static_cast<int>(gridDim.x); i += kRowThreads) {
+      if (i < static_cast<int>(blockIdx.x)) before += __ldg(a.counts + i);
+      if (each) top = larger(top, __ldg(a.tops + i));
+    }
+  } else {
+    for (int64_t i = t; i < (each ? a.x.tokens : r0); i += kRowThreads) {
+      if (__ldg(a.st.target + i) == kIgnored) continue;
+      if (i < r0) ++before;
+      if (each) top = larger(top, fabsf(__ldg(a.dloss + i * a.dloss_stride)));
+    }
+  }
+  before = block_sum(before, sums);
+  if (each) top = block_top(top, red);
+  const float unit = Factor(top, kBf16).power;  // (1 where no factor is above 0)
+  // The thread's token: its place, its target's d (see prob_chunk), its factor.
+  const int64_t r = r0 + t;
+  const bool mine = t < a.per_block && r < a.x.tokens;
+  const int target = mine ? __ldg(a.st.target + r) : kIgnored;
+  const bool keep = target != kIgnored;
+  const int place = before + block_place(keep, &count, warp_base);
+  places[t] = keep ? place : -1;
+  if (mine) a.place[r] = places[t];
+  if (keep) {
+    float held = a.prob_scale;
+    if (each) {
+      const Factor f(__ldg(a.dloss + r * a.dloss_stride), kBf16);
+      held *= f.m;
+      a.log_factor[place] = log2f(held);
+      a.power[r] = f.power / a.prob_scale;
+      powers[t] = f.m > 0.f && f.m < INFINITY ? f.power / unit : f.power;
+    }
+    a.target[place] = target;
+    // (With an infinite factor the row is no number: NaN at the target, so that dW is loud.)
+    a.own[place] = held < INFINITY ? held * expm1f(-__ldg(a.st.loss + place)) : NAN;
+  }
+  __syncthreads();
   const int rows = static_cast<int>(min(static_cast<int64_t>(a.per_block), a.x.tokens - r0)), vecs = (a.x.in + 7) / 8;
 #pragma unroll 2
   for (int i = t; i < rows * vecs; i += kRowThreads) {
     const int row = i / vecs, c = i - row * vecs;
-    const int place = __ldg(a.st.place + r0 + row);
-    if (place < 0) continue;
+    const int at = places[row];
+    if (at < 0) continue;
     const uint4 v = a.x.load(r0 + row, 8 * c);
-    reinterpret_cast<uint4 *>(a.rows + place * a.pitch)[c] = v;
-    if (!a.factor) continue;
-    const Factor f(__ldg(a.dloss + (r0 + row) * a.dloss_stride), kBf16);
-    if (c == 0) {
-      a.factor[place] = f.m * a.prob_scale;
-      a.power[r0 + row] = f.power / a.prob_scale;
-    }
+    reinterpret_cast<uint4 *>(a.rows + at * a.pitch)[c] = v;
     if (!a.scaled) continue;
-    const float g = f.m > 0.f && f.m < INFINITY ? f.power / unit : f.power;
+    const float g = powers[row];
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     uint32_t o[4];
 #pragma unroll
@@ -1057,7 +1119,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_back_rows_kernel(const BackRow
       const float x1 = kBf16 ? __bfloat162float(__ushort_as_bfloat16(hi)) : __half2float(__ushort_as_half(hi));
       o[k] = pack2<kBf16>(x0 * g, x1 * g);
     }
-    reinterpret_cast<uint4 *>(a.scaled + place * a.pitch)[c] = make_uint4(o[0], o[1], o[2], o[3]);
+    reinterpret_cast<uint4 *>(a.scaled + at * a.pitch)[c] = make_uint4(o[0], o[1], o[2], o[3]);
   }
   if (blockIdx.x + 1 == gridDim.x) {
     for (int i = t; i < a.n_counters; i += kRowThreads) a.counters[i] = 0;
@@ -1067,7 +1129,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_back_rows_kernel(const BackRow
     for (int r = kept + warp; r < end; r += kRowThreads / 32)
       for (int c = lane; c < a.x.in; c += 32) rows[r * a.pitch + c] = 0;
     if (t == 0) {
-      const float g = a.factor ? unit : a.mean ? a.dloss[0] / static_cast<float>(kept) : a.dloss[0];
+      const float g = each ? unit : a.mean ? a.dloss[0] / static_cast<float>(kept) : a.dloss[0];
       a.scale[0] = kept ? g / a.prob_scale : 0.f;
       a.scale[1] = g / a.prob_scale;
     }
@@ -1141,7 +1203,7 @@ struct CombineArgs {
   int64_t part_pitch;
   int n_parts;
   const float *z_target;
-  const int *token;
+  const int *token, *target;
   float *row_loss;   // by place (sum, mean)
   float *loss;       // of each token, or the one value
   int reduction;     // H24_REDUCE_*
@@ -1172,8 +1234,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_combine_kernel(const CombineAr
     const int total = __syncthreads_count(counts);
     kept = a.tokens;
     if (t == 0) {
-      a.st.place[blockIdx.x] = keep ? place : -1;
-      if (keep) a.st.target[place] = known ? static_cast<int>(label) : -1;
+      a.st.target[blockIdx.x] = !keep ? kIgnored : known ? static_cast<int>(label) : kNoTarget;
       if (blockIdx.x == 0) *a.st.kept = total;
       if (!keep && a.reduction == H24_REDUCE_NONE) a.loss[blockIdx.x] = 0.f;
       if (!keep && a.reduction != H24_REDUCE_NONE) a.row_loss[blockIdx.x] = 0.f;
@@ -1203,10 +1264,11 @@ __global__ void __launch_bounds__(kRowThreads) ce_combine_kernel(const CombineAr
   if (t < ROWS && row < kept && keep) {
     for (int w = 1; w < kRowThreads / 32; ++w) join(p, red[w][t]);
     // A target outside the vocabulary has no loss: NaN, here and in the gradients.
-    if (!own) known = a.st.target[row] >= 0;
+    if (!own) known = a.target[row] >= 0;
     const float rest = known ? logf(p.y) : __int_as_float(0x7fffffff), lse = p.x + rest;
     const float loss = known ? (p.x - a.z_target[row]) + rest : rest;  // (both parts are 0 or more)
     a.st.lse[own ? place : row] = lse;
+    a.st.loss[own ? place : row] = loss;
     if (a.reduction == H24_REDUCE_NONE)
       a.loss[own ? row : a.token[row]] = loss;
     else
@@ -1238,7 +1300,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_combine_kernel(const CombineAr
 // dx from the slices' sums
 // ---------------------------------------------------------------------------
 struct StatesArgs {
-  State st;
+  const int *place;
   const float *acc;
   int64_t pitch, plane;
   int slices;
@@ -1259,7 +1321,7 @@ __global__ void __launch_bounds__(kRowThreads) ce_states_kernel(const StatesArgs
        i += static_cast<int64_t>(gridDim.x) * kRowThreads) {
     const int64_t r = i / groups;
     const int c = static_cast<int>(i - r * groups) * 8;
-    const int place = __ldg(a.st.place + r);
+    const int place = __ldg(a.place + r);
     float v[8] = {};
     if (place >= 0) {
       // (The rows of acc are padded to 32 columns.)
@@ -1420,6 +1482,7 @@ int launch_ce_forward(const Tables *T, const CeArgs &c, const int64_t *labels, i
   const int64_t pitch = up(c.in, 8), part_pitch = up(c.tokens, kCombineRows);
   Scratch sc(s);
   const int64_t rows_at = sc.take((c.tokens + kTileK) * pitch * 2), token_at = sc.take(c.tokens * 4);
+  const int64_t target_at = sc.take(c.tokens * 4);
   const int64_t zt_at = sc.take(c.tokens * 4), loss_at = sc.take(c.tokens * 4), ticket_at = sc.take(4);
   const int64_t parts_at = sc.take(n_parts * part_pitch * 8);
   const int64_t w_at = head_readable(c) ? -1 : sc.take(c.vocab * pitch * 2);
@@ -1441,6 +1504,7 @@ int launch_ce_forward(const Tables *T, const CeArgs &c, const int64_t *labels, i
   r.vocab = static_cast<int>(c.vocab);
   r.st = st;
   r.token = sc.at<int>(token_at);
+  r.target = sc.at<int>(target_at);
   r.rows = sc.at<uint16_t>(rows_at);
   r.pitch = pitch;
   r.loss = c.reduction == H24_REDUCE_NONE ? loss : nullptr;
@@ -1483,18 +1547,18 @@ int launch_ce_forward(const Tables *T, const CeArgs &c, const int64_t *labels, i
   g.tokens = static_cast<int>(c.tokens);
   g.labels = own ? labels : nullptr;
   g.ticket = own ? r.ticket : nullptr;
-  g.target = st.target;
+  g.target = r.target;
   g.z_target = sc.at<float>(zt_at);
   g.parts = sc.at<float2>(parts_at);
   g.part_pitch = part_pitch;
   g.err = T->err;
   const int64_t tiles = m_tiles * n_tiles;
   if (swap)
-    rc = bf16 ? launch_gemm<ce_gemm_kernel<true, kForwardFew>>(g, tiles, s)
-              : launch_gemm<ce_gemm_kernel<false, kForwardFew>>(g, tiles, s);
+    rc = bf16 ? launch_gemm<ce_gemm_kernel<true, true, true, true>>(g, tiles, s)
+              : launch_gemm<ce_gemm_kernel<false, true, true, true>>(g, tiles, s);
   else
-    rc = bf16 ? launch_gemm<ce_gemm_kernel<true, kForwardRows>>(g, tiles, s)
-              : launch_gemm<ce_gemm_kernel<false, kForwardRows>>(g, tiles, s);
+    rc = bf16 ? launch_gemm<ce_gemm_kernel<true, true, false, true>>(g, tiles, s)
+              : launch_gemm<ce_gemm_kernel<false, true, false, true>>(g, tiles, s);
   if (rc != H24_OK) return rc;
 
   CombineArgs cb{};
@@ -1504,6 +1568,7 @@ int launch_ce_forward(const Tables *T, const CeArgs &c, const int64_t *labels, i
   cb.n_parts = static_cast<int>(n_parts);
   cb.z_target = g.z_target;
   cb.token = r.token;
+  cb.target = r.target;
   cb.row_loss = sc.at<float>(loss_at);
   cb.loss = loss;
   cb.reduction = c.reduction;
@@ -1559,10 +1624,10 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   Scratch sc(s);
   const int64_t rows_at = sc.take((c.tokens + kTileK) * pitch * 2);
   const int64_t scaled_at = each && dw ? sc.take((c.tokens + kTileK) * pitch * 2) : -1;
-  const int64_t factor_at = each ? sc.take(2 * c.tokens * 4) : -1;
+  const int64_t token_at = sc.take((each ? 5 : 3) * c.tokens * 4);  // words of each token
   const int per_block = rows_per_block(c.tokens);
   const int64_t row_blocks = cdiv(c.tokens, per_block);
-  const int64_t tops_at = each && c.tokens > kGroupedTokens ? sc.take(row_blocks * 4) : -1;
+  const int64_t groups_at = c.tokens > kGroupedTokens ? sc.take(2 * row_blocks * 4) : -1;
   const int64_t scale_at = sc.take(8), counters_at = sc.take((plan.pieces + 1) * 4);
   const int64_t w_at = head_readable(c) ? -1 : sc.take(c.vocab * pitch * 2);
   const int64_t acc_at = dx ? sc.take(plan.split * c.tokens * acc_pitch * 4) : -1;
@@ -1579,8 +1644,11 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   r.st = st;
   r.rows = sc.at<uint16_t>(rows_at);
   r.scaled = scaled_at < 0 ? nullptr : sc.at<uint16_t>(scaled_at);
-  r.factor = each ? sc.at<float>(factor_at) : nullptr;
-  r.power = each ? r.factor + c.tokens : nullptr;
+  r.place = sc.at<int>(token_at);
+  r.target = r.place + c.tokens;
+  r.own = sc.at<float>(token_at) + 2 * c.tokens;
+  r.log_factor = each ? r.own + c.tokens : nullptr;
+  r.power = each ? r.own + 2 * c.tokens : nullptr;
   r.pitch = pitch;
   r.dloss = dloss;
   r.dloss_stride = dloss_stride;
@@ -1590,14 +1658,16 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   r.counters = sc.at<int>(counters_at);
   r.n_counters = static_cast<int>(plan.pieces + 1);
   r.per_block = per_block;
-  if (tops_at >= 0) {
+  if (groups_at >= 0) {
     GroupArgs q{};
-    q.place = st.place;
-    q.dloss = dloss;
+    q.target = st.target;
+    q.dloss = each ? dloss : nullptr;
     q.dloss_stride = dloss_stride;
     q.tokens = c.tokens;
     q.per_block = per_block;
-    q.tops = sc.at<float>(tops_at);
+    q.counts = sc.at<int>(groups_at);
+    q.tops = sc.at<float>(groups_at) + row_blocks;
+    r.counts = q.counts;
     r.tops = q.tops;
     H24_CUDA_TRY(launch_pdl(ce_groups_kernel, dim3(static_cast<unsigned>(row_blocks)), dim3(kRowThreads), s, q));
     count_launches(1);
@@ -1612,18 +1682,18 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   GemmArgs base{};
   base.vocab = static_cast<int>(c.vocab);
   base.kept = st.kept;
-  base.target = st.target;
+  base.target = r.target;
   base.lse = st.lse;
+  base.own = r.own;
   base.scale = r.scale;
-  base.prob_scale = prob_scale;
   base.prob_log2 = bf16 ? 0.f : 15.f;
-  base.factor = r.factor;
+  base.log_factor = r.log_factor;
   base.row_bytes = c.in % 16 == 0 && (reinterpret_cast<uintptr_t>(dw) & 31) == 0 ? 32 : c.in % 8 == 0 && aligned16(dw) ? 16 : 2;
   base.err = T->err;
   const int64_t rows_alloc = c.tokens + kTileK;
   const uint16_t *head_rows = r.scaled ? r.scaled : r.rows;
   const int bn_in = static_cast<int>(c.in >= kTileN ? kTileN : up(c.in, 32));
-  const bool swap = few_tokens(c.tokens);
+  const bool swap = few_tokens(c.tokens), is_long = cdiv(c.in, kTileK) > (bf16 ? kBackBf16 : kBackHalf);
   const int bn_few = static_cast<int>(up(c.tokens, 32));
   const int64_t d_rows = swap ? bn_few : rows;  // rows of d that are written
   for (int64_t i = 0; i <= plan.pieces; ++i) {
@@ -1701,13 +1771,18 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
       ++g.jobs;
     }
     if (!ok) return fail(H24_ERR_CUDA, "linear_ce_backward: cuTensorMapEncodeTiled failed");
-    rc = bf16 ? launch_gemm<ce_gemm_kernel<true, kBackward>>(g, tiles, s)
-              : launch_gemm<ce_gemm_kernel<false, kBackward>>(g, tiles, s);
+    auto launch = [&](auto few, auto several) {
+      return bf16 ? launch_gemm<ce_gemm_kernel<true, false, decltype(few)::value, decltype(several)::value>>(g, tiles, s)
+                  : launch_gemm<ce_gemm_kernel<false, false, decltype(few)::value, decltype(several)::value>>(g, tiles, s);
+    };
+    constexpr std::true_type yes;
+    constexpr std::false_type no;
+    rc = swap ? (is_long ? launch(yes, yes) : launch(yes, no)) : is_long ? launch(no, yes) : launch(no, no);
     if (rc != H24_OK) return rc;
   }
   if (dx) {
     StatesArgs o{};
-    o.st = st;
+    o.place = r.place;
     o.acc = sc.at<float>(acc_at);
     o.pitch = acc_pitch;
     o.plane = c.tokens * acc_pitch;

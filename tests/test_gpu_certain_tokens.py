@@ -61,3 +61,83 @@ def test_certain_tokens(ce, tokens, vocab, top, dtype):
             value = ce(x, w, target, reduction=reduction)
             assert float(value) >= 0
             assert abs(float(value) - float(want.sum()) / n) <= float(bound.sum()) / n + U * float(want.sum()) / n
+
+
+# Gradients.  Where k is long, the forward pass's z may be off by ez and the backward pass's by eb: d of another token v is
+# p (1 + ez + eb), rounded to 16 bits; the target's is -(1 - e^-loss), whose error is that of the loss.
+def _long(tokens, vocab, k, dtype, top, seed=0):
+    """Near-certain tokens whose logit is a sum of one sign over all of k."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    kinds = min(tokens, 32)
+    places = torch.arange(kinds, device="cuda") * (vocab // kinds) + 3
+    sign = torch.where(torch.rand(kinds, k, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    w = torch.randn(vocab, k, generator=g, device="cuda") * (0.3 / k ** 0.5)
+    size = (0.5 + torch.rand(kinds, k, generator=g, device="cuda")) * (top / k) ** 0.5
+    w[places] = sign * size
+    which = torch.arange(tokens, device="cuda") % kinds
+    x = (sign * size)[which] * (0.8 + 0.25 * torch.rand(tokens, 1, generator=g, device="cuda"))
+    return x.to(dtype), w.to(dtype), places[which]
+
+
+@pytest.mark.parametrize("tokens,vocab,k,top", [(20, 5003, 7680, 18), (200, 5003, 7680, 18), (200, 9001, 1920, 22),
+                                                (64, 9001, 1153, 16), (300, 1009, 4097, 14), (40, 1009, 12000, 14)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradients_of_certain_tokens(ce, tokens, vocab, k, top, dtype):
+    """The target's entry of d is right relative to 1 - p, and the others to p."""
+    x, w, target = _long(tokens, vocab, k, dtype, top)
+    half, tiny = torch.finfo(dtype).eps / 2, (2.0 ** -134 if dtype == torch.bfloat16 else 2.0 ** -25)
+    z = x.double() @ w.double().t()
+    lse = torch.logsumexp(z, 1)
+    rest = z.scatter(1, target[:, None], float("-inf"))
+    loss = torch.nn.functional.softplus(torch.logsumexp(rest, 1) - z.gather(1, target[:, None])[:, 0])
+    assert 1e-7 < float(loss.min()) and float(loss.max()) < 0.5
+    # Truncated sums: 2^-23 of the sum of magnitudes for each 16 k of a slice (1,024 k, in fp16 512), and its additions.
+    mags = x.double().abs() @ w.double().abs().t()
+    ez = ((1024 / 16 + k / 512 + 8) * 2.0 ** -23 * mags.amax(1))
+    # ... and of what the backward pass sums at once (4,096 and 1,408).
+    eb = ((min(k, 4096) / 16 + k / 1408 + 8) * 2.0 ** -23 * mags.amax(1))
+    eloss = (1 - torch.exp(-loss)) * (torch.expm1(2 * ez) + 2.0 ** -18) + 100 * U
+    xs, ws = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    scale = 256.0
+    value = ce(xs, ws, target, reduction="none")
+    assert bool(((value.detach().double() - loss).abs() <= eloss).all())
+    dx, dw = torch.autograd.grad(value, (xs, ws), torch.full((tokens,), scale, device="cuda"))
+    own = torch.expm1(-loss)
+    ed_own = own.abs() * half + eloss * (1 + half)
+    p = torch.exp(rest - lse[:, None])
+    ed = (p * (half + torch.expm1(ez + eb) + 2.0 ** -18)[:, None] + 2.0 ** -40).scatter(1, target[:, None], ed_own[:, None])
+    d = p.scatter(1, target[:, None], own[:, None])
+    for got, want, err in ((dx, d @ w.double(), ed @ w.double().abs() + (vocab / 16 + 16) * 2.0 ** -23 * (d.abs() @ w.double().abs())),
+                           (dw, d.t() @ x.double(), ed.t() @ x.double().abs() + (tokens / 16 + 16) * 2.0 ** -23 * (d.abs().t() @ x.double().abs()))):
+        want, err = scale * want, scale * err
+        err = err + half * (want.abs() + err) + tiny
+        assert bool(((got.double() - want).abs() <= err).all()), float(((got.double() - want).abs() / err).max())
+
+
+@pytest.mark.parametrize("top", [30, 100, 1000])
+@pytest.mark.parametrize("tokens", [33, 300])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_entry_of_d_at_the_target(ce, tokens, top, dtype):
+    """Exact logits, one other token 9 below the largest: 1 - p = 1.2e-4.  One state is there in one token alone, so that
+    an element of the target's row of dW is that token's d times powers of two: half a step of d, half a step of dW, and
+    100 u of the loss's sum."""
+    k, vocab = 64, 515
+    x = torch.zeros(tokens, k, device="cuda")
+    w = torch.zeros(vocab, k, device="cuda")
+    t = torch.arange(tokens, device="cuda")
+    x[:, 0] = float(top)
+    x[:, 1] = 1
+    x[:, 2] = (t == 5).float() * 0.5  # one token alone
+    w[7, 0], w[9, 0], w[9, 1] = 1, 1, -9
+    target = torch.full((tokens,), 7, device="cuda")
+    z = torch.zeros(tokens, vocab, dtype=torch.float64, device="cuda")
+    z[:, 7], z[:, 9] = top, top - 9
+    loss = torch.log1p(torch.exp(z.scatter(1, target[:, None], float("-inf")) - top).sum(1))
+    xs, ws = x.to(dtype).requires_grad_(True), w.to(dtype).requires_grad_(True)
+    value = ce(xs, ws, target, reduction="none")
+    dx, dw = torch.autograd.grad(value, (xs, ws), torch.full((tokens,), 1024.0, device="cuda"))
+    half = torch.finfo(dtype).eps / 2
+    assert bool(((value.detach().double() - loss).abs() <= 100 * U).all())
+    want = 1024.0 * 0.5 * torch.expm1(-loss[5])
+    bound = abs(float(want)) * 2.01 * half + 1024 * 0.5 * 100 * U
+    assert abs(float(dw[7, 2]) - float(want)) <= bound, (float(dw[7, 2]), float(want))
