@@ -297,7 +297,7 @@ int h24_linear_ce_forward(const void *x, int64_t tokens, int64_t x_stride, const
  * d = softmax(z) - onehot(target) rounded to `dtype` (in fp16 held times 2^15),
  * sums in fp32, each result rounded once.  x, w and the sizes are those of the
  * forward call that wrote `state`, and unchanged.  dloss: the loss's gradient,
- * one a token at t * dloss_stride (H24_REDUCE_NONE: g_t's part in [1, 2) is in
+ * one a token at t * dloss_stride (H24_REDUCE_NONE: g_t's part in [1, 2), in fp16 in [1/2, 1), is in
  * d before its rounding, its power of two in x for dw) or one.  dx (tokens x in_features)
  * and dw (vocab x in_features) are contiguous and of `dtype`; either may be
  * NULL.  The logits are computed again, for a piece of the vocabulary at a

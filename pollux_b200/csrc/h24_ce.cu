@@ -1028,20 +1028,21 @@ struct BackRowsArgs {
 };
 
 // A token's factor as m * power: |power| a power of two, m in [1, 2) and held in
-// d before its rounding.  In fp16 m ends at 1.999, and then starts at half of that:
-// 2^15 * m stays below 65,504.  Zeros, infinities and NaN are all in m.
+// d before its rounding, in fp16 in [1/2, 1): there d is held times 2^15, and p may
+// come out above 1 by what its logit's sum was cut off (4e-4 of a logit of -100),
+// so that a factor up to 2 would leave fp16's range.  Zeros, infinities and NaN are
+// all in m.
 struct Factor {
   float m, power;
-  __device__ Factor(float g, bool half_open) {
+  __device__ Factor(float g, bool bf16) {
     m = fabsf(g);
     power = copysignf(1.f, g);
     if (!(m > 0.f && m < INFINITY)) return;
     int e;
-    m = 2.f * frexpf(m, &e);
-    --e;
-    if (!half_open && m > 1.999f) {
-      m *= 0.5f;
-      ++e;
+    m = frexpf(m, &e);
+    if (bf16) {
+      m *= 2.f;
+      --e;
     }
     power = ldexpf(power, e);
   }

@@ -141,3 +141,33 @@ def test_entry_of_d_at_the_target(ce, tokens, top, dtype):
     want = 1024.0 * 0.5 * torch.expm1(-loss[5])
     bound = abs(float(want)) * 2.01 * half + 1024 * 0.5 * 100 * U
     assert abs(float(dw[7, 2]) - float(want)) <= bound, (float(dw[7, 2]), float(want))
+
+
+@pytest.mark.parametrize("tokens", [20, 200])
+@pytest.mark.parametrize("factor", [1.9989, -1.9985, 1.0, 0.99951, 3.9978])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_certain_wrong_token(ce, tokens, factor, dtype):
+    """All logits far below 0 and one of them certain: its sum loses magnitude in the tensor cores, so p comes out above 1,
+    and times a factor just below 2 it stays finite.  dx = g (W[7] - W[target]) up to e^-140: half a step of each entry of
+    d, with what z[7] was cut off in p (an addition in a tensor core may truncate, by up to 2^-23 of the sum: that for each
+    16 k, of |z[7]| since all products have one sign), and half a step of the result."""
+    k, vocab = 1400, 300
+    g = torch.Generator(device="cuda").manual_seed(5)
+    size = (0.5 + torch.rand(k, generator=g, device="cuda")) * (150.0 / k) ** 0.5
+    w = -2 * size.expand(vocab, k) * (1 + 0.01 * torch.rand(vocab, k, generator=g, device="cuda"))
+    w[7] = -size
+    x = size.expand(tokens, k) * (0.95 + 0.05 * torch.rand(tokens, 1, generator=g, device="cuda"))
+    target = torch.arange(tokens, device="cuda") % 5 + 20
+    xs, ws = x.to(dtype).requires_grad_(True), w.to(dtype).requires_grad_(True)
+    value = ce(xs, ws, target, reduction="none")
+    z = xs.detach().double() @ ws.detach().double().t()
+    assert bool(((value.detach().double() - (z[:, 7] - z.gather(1, target[:, None])[:, 0])).abs() <= 1e-2).all())
+    dx, dw = torch.autograd.grad(value, (xs, ws), torch.full((tokens,), factor, device="cuda"))
+    half = torch.finfo(dtype).eps / 2
+    wd = ws.detach().double()
+    want = factor * (wd[7] - wd[target])
+    cut = torch.expm1(z[:, 7:8].abs() * (k / 16 + 8) * 2.0 ** -23)
+    err = abs(factor) * (wd[7].abs() * (half + cut + 2.0 ** -18) + wd[target].abs() * half)
+    err = err + half * (want.abs() + err) + 2.0 ** -25
+    assert bool(((dx.double() - want).abs() <= err).all())
+    assert bool(torch.isfinite(dw).all())
