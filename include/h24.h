@@ -297,8 +297,10 @@ int h24_linear_ce_forward(const void *x, int64_t tokens, int64_t x_stride, const
  * d = softmax(z) - onehot(target) rounded to `dtype` (in fp16 held times 2^15),
  * sums in fp32, each result rounded once.  x, w and the sizes are those of the
  * forward call that wrote `state`, and unchanged.  dloss: the loss's gradient,
- * one a token at t * dloss_stride (H24_REDUCE_NONE: g_t's part in [1, 2), in fp16 in [1/2, 1), is in
- * d before its rounding, its power of two in x for dw) or one.  dx (tokens x in_features)
+ * one a token at t * dloss_stride (H24_REDUCE_NONE) or one.  A token's own g_t is cut
+ * in two: a part in [1, 2), in fp16 [1/2, 1), goes into d before its rounding, its
+ * power of two into dx and, for dw, into x; in fp16 such states are held in steps of
+ * 2^-39 of the largest |g_t x| at most.  dx (tokens x in_features)
  * and dw (vocab x in_features) are contiguous and of `dtype`; either may be
  * NULL.  The logits are computed again, for a piece of the vocabulary at a
  * time; scratch as above, and 2 * 192 MiB at most for the pieces (or 2 * 4,096

@@ -36,6 +36,8 @@
 // and [50688,1920] 38 us of tiles (5.1 TB/s).
 #include "h24_tile.cuh"
 
+#include <limits.h>
+
 #include <type_traits>
 
 namespace h24 {
@@ -929,35 +931,88 @@ struct GroupArgs {
   const int *target;      // backward: the state's
   const float *dloss;     // null: no tops
   int64_t dloss_stride;
+  RowSource x;            // of tops with the states' sizes; x null: without
   int64_t tokens;
   int per_block;
-  int *counts;
-  float *tops;
+  int *counts, *tops;
 };
-__device__ __forceinline__ float larger(float top, float g) {
-  return g != g ? g : fmaxf(g, top);  // (a NaN that is overtaken here is in its row of d all the same)
-}
-// Largest of the threads' values, to all of them.
-__device__ __forceinline__ float block_top(float top, float *red) {
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+
+// A token's factor as m * 2^power: m, never below 0, in [1, 2) and held in d
+// before its rounding, in fp16 in [1/2, 1): there d is held times 2^15, and p may
+// come out above 1 by what its logit's sum was cut off (4e-4 of a logit of -100),
+// so that a factor up to 2 would leave fp16's range.  Zeros, infinities and NaN are
+// all in m, and have no say in what the others are relative to.
+struct Factor {
+  float m, sign;
+  int power;
+  bool real;
+  __device__ Factor(float g, bool bf16) {
+    m = fabsf(g);
+    sign = copysignf(1.f, g);
+    power = 0;
+    real = m > 0.f && m < INFINITY;
+    if (!real) return;
+    m = frexpf(m, &power);
+    if (bf16) {
+      m *= 2.f;
+      --power;
+    }
+  }
+};
+constexpr int kNoTop = INT_MIN;
+
+__device__ __forceinline__ int block_max(int v, int *red) {
+  v = __reduce_max_sync(0xffffffffu, v);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
-  top = 0.f;
-  for (int w = 0; w < kRowThreads / 32; ++w) top = fmaxf(top, red[w]);
-  return top;
+  for (int w = 0; w < kRowThreads / 32; ++w) v = max(v, red[w]);
+  __syncthreads();
+  return v;
 }
+
+// (tops: of bf16 where there are no sizes, of fp16 with them)
 __global__ void __launch_bounds__(kRowThreads) ce_groups_kernel(const GroupArgs a) {
   __shared__ int red[kRowThreads / 32];
-  __shared__ float red_top[kRowThreads / 32];
+  __shared__ unsigned size[kRowThreads];
   pdl_enter();
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * a.per_block + threadIdx.x;
-  const bool mine = static_cast<int>(threadIdx.x) < a.per_block && r < a.tokens;
+  const int t = threadIdx.x;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * a.per_block, r = r0 + t;
+  const bool mine = t < a.per_block && r < a.tokens;
   const bool kept = mine && (a.labels ? __ldg(a.labels + r) != a.ignore : __ldg(a.target + r) != kIgnored);
   const int count = block_sum(kept, red);
-  if (threadIdx.x == 0) a.counts[blockIdx.x] = count;
+  if (t == 0) a.counts[blockIdx.x] = count;
   if (!a.dloss) return;
-  const float top = block_top(kept ? larger(0.f, fabsf(__ldg(a.dloss + r * a.dloss_stride))) : 0.f, red_top);
-  if (threadIdx.x == 0) a.tops[blockIdx.x] = top;
+  const bool sizes = a.x.x != nullptr;
+  const Factor f(kept ? __ldg(a.dloss + r * a.dloss_stride) : 0.f, !sizes);
+  int top = f.real ? f.power : kNoTop;
+  if (sizes) {
+    // The largest finite magnitude of each row, as bits.
+    size[t] = f.real ? 0 : ~0u;
+    __syncthreads();
+    const int rows = static_cast<int>(min(static_cast<int64_t>(a.per_block), a.tokens - r0)), vecs = (a.x.in + 7) / 8;
+    for (int i = t; i < rows * vecs; i += kRowThreads) {
+      const int row = i / vecs;
+      if (size[row] == ~0u) continue;
+      const uint4 v = a.x.load(r0 + row, 8 * (i - row * vecs));
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      unsigned most = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const unsigned h = w[k / 2] >> (16 * (k & 1)) & 0x7fffu;
+        if (h < 0x7c00u) most = max(most, h);
+      }
+      if (most > *const_cast<volatile unsigned *>(&size[row])) atomicMax(&size[row], most);
+    }
+    __syncthreads();
+    if (f.real) {
+      int e;
+      const float most = __half2float(__ushort_as_half(static_cast<uint16_t>(size[t])));
+      frexpf(most, &e);
+      top = most > 0.f ? f.power + e : kNoTop;
+    }
+  }
+  top = block_max(top, red);
+  if (t == 0) a.tops[blockIdx.x] = top;
 }
 
 // Block b takes tokens b * per_block on.  It counts the kept tokens before its
@@ -1012,73 +1067,60 @@ struct BackRowsArgs {
   int *place;        // of each token among the kept ones (-1: ignored)
   int *target;       // of each kept token
   float *own;        // and d there, times what its row of d is held times
-  float *log_factor; // log2 of the rest of each kept token's factor times prob_scale; null: g is the same for all
-  float *power;      // each token's power of two / prob_scale
+  float *log_factor; // log2 of the rest of each kept token's factor, in fp16 times 2^15; null: g is the same for all
+  float *power;      // each token's power of two, signed, in fp16 over 2^15
   int64_t pitch;
   const float *dloss;
   int64_t dloss_stride;
-  const int *counts; // kept tokens and largest |g| of each block's tokens, or null
-  const float *tops;
+  const int *counts; // kept tokens of each block's tokens, or null
+  const int *tops;   // and the power that their scaled states are relative to
   bool mean;
-  float prob_scale;
   float *scale;      // [0] factor of dW, [1] factor of dx where g is the same for all
   int *counters;     // of the launches that follow, set to 0
   int n_counters;
   int per_block;
 };
 
-// A token's factor as m * power: |power| a power of two, m in [1, 2) and held in
-// d before its rounding, in fp16 in [1/2, 1): there d is held times 2^15, and p may
-// come out above 1 by what its logit's sum was cut off (4e-4 of a logit of -100),
-// so that a factor up to 2 would leave fp16's range.  Zeros, infinities and NaN are
-// all in m.
-struct Factor {
-  float m, power;
-  __device__ Factor(float g, bool bf16) {
-    m = fabsf(g);
-    power = copysignf(1.f, g);
-    if (!(m > 0.f && m < INFINITY)) return;
-    int e;
-    m = frexpf(m, &e);
-    if (bf16) {
-      m *= 2.f;
-      --e;
-    }
-    power = ldexpf(power, e);
-  }
-};
-
 // The copies of the backward pass.  A token's own factor is cut in two.  m goes
 // into its row of d, and is rounded with it: no rounding more, and d's relative
-// error is the one it has without.  The power of two goes into the token's states
-// for dW, relative to the largest one (exactly, but where it takes them below the
-// type's range: that is small beside dW), and into dx at the end.
+// error is the one it has without.  The power of two goes into dx at the end, and
+// for dW into the token's states.  bf16 has fp32's range for that: the powers are
+// relative to the largest, and the states exact.  fp16 has not: relative to the
+// largest factor, a state of 1 keeps 8 bits at a ratio of 2^-16 and none from 2^-25
+// on, and a row of dW that only such tokens feed is off by as much.  There the
+// powers are such that the largest state times its factor comes to lie below 2^15,
+// and what is cut off is 2^-40 of that: less than half of dW's own smallest step
+// wherever that product, times a d of one, is in fp16's range itself.  (A launch
+// more and a pass over x for its sizes: 3 us of the step of [16,512] x [5000,512].)
 template <bool kBf16>
 __global__ void __launch_bounds__(kRowThreads) ce_back_rows_kernel(const BackRowsArgs a) {
-  __shared__ float red[kRowThreads / 32], powers[kRowThreads];
-  __shared__ int sums[kRowThreads / 32], warp_base[kRowThreads / 32], places[kRowThreads];
+  __shared__ float powers[kRowThreads];
+  __shared__ int red[kRowThreads / 32], warp_base[kRowThreads / 32], places[kRowThreads];
   pdl_enter();
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int kept = *a.st.kept;
   const int64_t r0 = static_cast<int64_t>(blockIdx.x) * a.per_block;
   const bool each = a.log_factor != nullptr;
-  float top = 0.f;
-  int before = 0, count;
+  int before = 0, count, top = kNoTop;
   if (a.counts) {
     for (int i = t; i < static_cast<int>(gridDim.x); i += kRowThreads) {
       if (i < static_cast<int>(blockIdx.x)) before += __ldg(a.counts + i);
-      if (each) top = larger(top, __ldg(a.tops + i));
+      if (a.scaled) top = max(top, __ldg(a.tops + i));
     }
   } else {
-    for (int64_t i = t; i < (each ? a.x.tokens : r0); i += kRowThreads) {
+    for (int64_t i = t; i < (a.scaled ? a.x.tokens : r0); i += kRowThreads) {
       if (__ldg(a.st.target + i) == kIgnored) continue;
       if (i < r0) ++before;
-      if (each) top = larger(top, fabsf(__ldg(a.dloss + i * a.dloss_stride)));
+      if (a.scaled) {
+        const Factor f(__ldg(a.dloss + i * a.dloss_stride), kBf16);
+        if (f.real) top = max(top, f.power);
+      }
     }
   }
-  before = block_sum(before, sums);
-  if (each) top = block_top(top, red);
-  const float unit = Factor(top, kBf16).power;  // (1 where no factor is above 0)
+  before = block_sum(before, red);
+  if (a.scaled) top = block_max(top, red);
+  // The scaled states are those of a factor of 2^unit.
+  const int prob_power = kBf16 ? 0 : 15, unit = top == kNoTop ? 0 : top - prob_power;
   // The thread's token: its place, its target's d (see prob_chunk), its factor.
   const int64_t r = r0 + t;
   const bool mine = t < a.per_block && r < a.x.tokens;
@@ -1088,13 +1130,13 @@ __global__ void __launch_bounds__(kRowThreads) ce_back_rows_kernel(const BackRow
   places[t] = keep ? place : -1;
   if (mine) a.place[r] = places[t];
   if (keep) {
-    float held = a.prob_scale;
+    float held = static_cast<float>(1 << prob_power);
     if (each) {
       const Factor f(__ldg(a.dloss + r * a.dloss_stride), kBf16);
       held *= f.m;
       a.log_factor[place] = log2f(held);
-      a.power[r] = f.power / a.prob_scale;
-      powers[t] = f.m > 0.f && f.m < INFINITY ? f.power / unit : f.power;
+      a.power[r] = ldexpf(f.sign, f.power - prob_power);
+      powers[t] = f.real ? ldexpf(f.sign, f.power - unit) : f.sign;
     }
     a.target[place] = target;
     // (With an infinite factor the row is no number: NaN at the target, so that dW is loud.)
@@ -1130,9 +1172,10 @@ __global__ void __launch_bounds__(kRowThreads) ce_back_rows_kernel(const BackRow
     for (int r = kept + warp; r < end; r += kRowThreads / 32)
       for (int c = lane; c < a.x.in; c += 32) rows[r * a.pitch + c] = 0;
     if (t == 0) {
-      const float g = each ? unit : a.mean ? a.dloss[0] / static_cast<float>(kept) : a.dloss[0];
-      a.scale[0] = kept ? g / a.prob_scale : 0.f;
-      a.scale[1] = g / a.prob_scale;
+      const float g = each ? ldexpf(1.f, unit - prob_power)
+                           : (a.mean ? a.dloss[0] / static_cast<float>(kept) : a.dloss[0]) / static_cast<float>(1 << prob_power);
+      a.scale[0] = kept ? g : 0.f;
+      a.scale[1] = g;
     }
   }
 }
@@ -1628,7 +1671,8 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   const int64_t token_at = sc.take((each ? 5 : 3) * c.tokens * 4);  // words of each token
   const int per_block = rows_per_block(c.tokens);
   const int64_t row_blocks = cdiv(c.tokens, per_block);
-  const int64_t groups_at = c.tokens > kGroupedTokens ? sc.take(2 * row_blocks * 4) : -1;
+  const bool sizes = scaled_at >= 0 && !bf16;
+  const int64_t groups_at = c.tokens > kGroupedTokens || sizes ? sc.take(2 * row_blocks * 4) : -1;
   const int64_t scale_at = sc.take(8), counters_at = sc.take((plan.pieces + 1) * 4);
   const int64_t w_at = head_readable(c) ? -1 : sc.take(c.vocab * pitch * 2);
   const int64_t acc_at = dx ? sc.take(plan.split * c.tokens * acc_pitch * 4) : -1;
@@ -1637,7 +1681,6 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   int rc = sc.allocate(T);
   if (rc != H24_OK) return rc;
   const State st = state_at(state, c.tokens);
-  const float prob_scale = bf16 ? 1.f : 32768.f;
 
   BackRowsArgs r{};
   r.x = {static_cast<const uint16_t *>(c.x), c.x_stride, static_cast<int>(c.tokens), static_cast<int>(c.in),
@@ -1654,7 +1697,6 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   r.dloss = dloss;
   r.dloss_stride = dloss_stride;
   r.mean = c.reduction == H24_REDUCE_MEAN;
-  r.prob_scale = prob_scale;
   r.scale = sc.at<float>(scale_at);
   r.counters = sc.at<int>(counters_at);
   r.n_counters = static_cast<int>(plan.pieces + 1);
@@ -1662,12 +1704,13 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   if (groups_at >= 0) {
     GroupArgs q{};
     q.target = st.target;
-    q.dloss = each ? dloss : nullptr;
+    q.dloss = scaled_at >= 0 ? dloss : nullptr;
+    if (sizes) q.x = r.x;
     q.dloss_stride = dloss_stride;
     q.tokens = c.tokens;
     q.per_block = per_block;
     q.counts = sc.at<int>(groups_at);
-    q.tops = sc.at<float>(groups_at) + row_blocks;
+    q.tops = q.counts + row_blocks;
     r.counts = q.counts;
     r.tops = q.tops;
     H24_CUDA_TRY(launch_pdl(ce_groups_kernel, dim3(static_cast<unsigned>(row_blocks)), dim3(kRowThreads), s, q));
