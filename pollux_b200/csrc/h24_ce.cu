@@ -66,6 +66,15 @@ __device__ __forceinline__ int slice_blocks(int nkb) {
   const int n = (nkb + kMost - 1) / kMost;
   return (nkb + n - 1) / n;
 }
+// The same of a gradient's sum, over the vocabulary (dx: each of its slices has an
+// output of its own) or over the tokens (dW).
+constexpr int kSumBf16 = 1024, kSumHalf = 256;
+template <bool kBf16>
+__device__ __forceinline__ int sum_blocks(int nkb) {
+  constexpr int kMost = kBf16 ? kSumBf16 : kSumHalf;
+  const int n = max(1, (nkb + kMost - 1) / kMost);
+  return (nkb + n - 1) / n;
+}
 constexpr int kMaxJobs = 3;
 constexpr int kGroupM = 32;      // row tiles that run through the vocabulary together
 constexpr float kLog2e = 1.4426950408889634f;
@@ -397,15 +406,20 @@ struct Turn {
 // The backward pass's probabilities are rounded to 16 bits, and the one entry that
 // is a difference comes from the loss: slices of 4,096 k, in fp16 1,408, keep z
 // to 4.4e-6 of itself, so a probability of a logit of 30 to 2^-13, where half a
-// step is 2^-9 and 2^-12.
+// step is 2^-9 and 2^-12.  The gradients' own sums are cut at 131,072 terms, in
+// fp16 at 32,768: terms of one sign lose 1.4e-4 and 1e-4 of their sum, where half a
+// step of the result is 2e-3 and 2.4e-4 at least.
 //
-// kFew: up to 128 tokens, the columns of the tiles of logits and of dx.  kLong: a
-// sum in several slices, for which an epilogue thread holds 128 of them: always in
-// the forward pass, in the backward pass where k is longer than a slice.  (Within
-// one kernel for both the gradients of [1024,1152] x [50688,1152] took 567 us, 479
-// without; the long kernel's spills cost a step of [8192,1920] x [50688,1920] in
-// fp16 5.1 ms instead of 4.8, and of [1024,7680] x [50688,7680] in bf16 nothing.)
-template <bool kBf16, bool kForward, bool kFew, bool kLong>
+// kFew: up to 128 tokens, the columns of the tiles of logits and of dx.  kLong: what
+// is summed in several slices, for which an epilogue thread holds 128 of them: in
+// the forward pass the logits, in the backward pass those where k is longer than a
+// slice, or they and dW where the tokens are (a step of [140000,1024] x
+// [20000,1024] in bf16: 22.1 ms, 19.4 without).  (Within one kernel for all the
+// gradients of [1024,1152] x [50688,1152] took 567 us, 479 so; the spills of the
+// long kernels cost a step of [8192,1920] x [50688,1920] in fp16 5.1 ms instead of
+// 4.8, and of [1024,7680] x [50688,7680] in bf16 nothing.)
+enum Long { kNone, kLogits, kTokens };
+template <bool kBf16, bool kForward, bool kFew, Long kLong>
 __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_constant__ GemmArgs a) {
   extern __shared__ uint8_t ce_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(ce_raw) + 1023) & ~uintptr_t(1023));
@@ -523,7 +537,9 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
         // box; 64 k are a box of the one, half a box of the other.
         const uint64_t step_a = a_mn ? 2048 >> 4 : 32 >> 4, half_a = a_mn ? 8192 >> 4 : kBox >> 4;
         const uint64_t step_b = b_mn ? 2048 >> 4 : 32 >> 4, half_b = b_mn ? 8192 >> 4 : a.stage_b >> 5;
-        const int slice = kForward || (kLong && j.kind == kProb) ? slice_blocks<kBf16, kForward, kFew>(tl.nkb) : 0x7fffffff;
+        const int slice = kForward || (kLong != kNone && j.kind == kProb) ? slice_blocks<kBf16, kForward, kFew>(tl.nkb)
+                          : kLong == kTokens && j.kind == kHeadRows       ? sum_blocks<kBf16>(tl.nkb)
+                                                                          : 0x7fffffff;
         for (int i = 0, at = 0; i < max(tl.nkb, 1); ++i) {  // (at: within a slice)
           if (at == 0) {
             ok = __all_sync(0xffffffffu, bar_wait(&H.acc_empty[acc], acc_ph ^ 1, abort, a.err));
@@ -651,8 +667,8 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
         // A lane holds a row of the weights and the columns are tokens: 32 x 32 of
         // them turn in shared memory, and each lane goes on with a token's row.
         const int row0 = tl.m + rank * (kTileM / 2) + quarter * 32;
-        int sum[kLong ? 2 : 1][32];
-        const bool logits = kForward || (kLong && j.kind == kProb);
+        const bool logits = kForward || (kLong != kNone && j.kind == kProb);
+        int sum[kLong != kNone ? 2 : 1][32];
         if (logits) {
           if (!gather(sum, tl.nkb, slice_blocks<kBf16, kForward, kFew>(tl.nkb), c0, c1)) break;
         } else {
@@ -667,7 +683,7 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
           __syncwarp();
           if (logits) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) turned[lane * kBlockPitch + i] = __int_as_float(sum[kLong ? q : 0][i]);
+            for (int i = 0; i < 32; ++i) turned[lane * kBlockPitch + i] = __int_as_float(sum[kLong != kNone ? q : 0][i]);
           } else {
             int r[32];
             tmem_ask32(ta + acc * kTileN + c, r);
@@ -754,61 +770,71 @@ __global__ void __launch_bounds__(kThreads, 1) ce_gemm_kernel(const __grid_const
       const bool add = j.add;
       uint16_t *out16 = static_cast<uint16_t *>(j.out) + (kind == kProb ? row : j.v0 + static_cast<int64_t>(row)) * pitch + tl.n;
       float *out32 = static_cast<float *>(j.out) + tl.slice * j.plane + row * pitch + tl.n;
+      auto head_chunk = [&](int c, const int (&r)[32]) {
+        float z[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) z[i] = __int_as_float(r[i]) * scale;
+        const int left = left0 - c;
+        if (a.row_bytes == 2) {
+          // A lane holds a row.  Turned, a warp writes 32 columns of a row at a
+          // time (the gradients of [333,1153] x [50257,1153] in 133 us; with padded
+          // rows in scratch and a copy of them behind it 111 + 40, in words of two
+          // elements shifted by one in odd rows 172, from the row's lane 203).
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) words[lane * kWordPitch + i] = pack2<kBf16>(z[2 * i], z[2 * i + 1]);
+          __syncwarp();
+          const int rows = min(32, j.m_total - row0);
+          const uint16_t *from = reinterpret_cast<const uint16_t *>(words) + lane;
+          uint16_t *to = out16 + c + lane - lane * pitch;
+          if (lane < left && rows == 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i, to += pitch) *to = from[2 * kWordPitch * i];
+          } else if (lane < left) {
+            for (int i = 0; i < rows; ++i, to += pitch) *to = from[2 * kWordPitch * i];
+          }
+          return;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t w[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = pack2<kBf16>(z[16 * h + 2 * i], z[16 * h + 2 * i + 1]);
+          uint16_t *to = out16 + c + 16 * h;
+          if (a.row_bytes == 32) {
+            if (st.live && 16 * h < left) store32B(to, w);
+          } else {
+            if (st.live && 16 * h < left) *reinterpret_cast<uint4 *>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+            if (st.live && 16 * h + 8 < left) *reinterpret_cast<uint4 *>(to + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+          }
+        }
+      };
       auto chunk = [&](int c, const int (&r)[32]) {
+        if (kind == kHeadRows) return head_chunk(c, r);
         float z[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) z[i] = __int_as_float(r[i]);
         if (!kFew && kind == kProb) {
           prob_chunk<kBf16>(st, out16, c, z);
-        } else if (kind == kStates) {
-          if (st.live) states_chunk(add, out32 + c, z);
-        } else {
-          const int left = left0 - c;
-          if (a.row_bytes == 2) {
-            // A lane holds a row.  Turned, a warp writes 32 columns of a row at a
-            // time (the gradients of [333,1153] x [50257,1153] in 133 us; with padded
-            // rows in scratch and a copy of them behind it 111 + 40, in words of two
-            // elements shifted by one in odd rows 172, from the row's lane 203).
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) words[lane * kWordPitch + i] = pack2<kBf16>(z[2 * i] * scale, z[2 * i + 1] * scale);
-            __syncwarp();
-            const int rows = min(32, j.m_total - row0);
-            const uint16_t *from = reinterpret_cast<const uint16_t *>(words) + lane;
-            uint16_t *to = out16 + c + lane - lane * pitch;
-            if (lane < left && rows == 32) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i, to += pitch) *to = from[2 * kWordPitch * i];
-            } else if (lane < left) {
-              for (int i = 0; i < rows; ++i, to += pitch) *to = from[2 * kWordPitch * i];
-            }
-            return;
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t w[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = pack2<kBf16>(z[16 * h + 2 * i] * scale, z[16 * h + 2 * i + 1] * scale);
-            uint16_t *to = out16 + c + 16 * h;
-            if (a.row_bytes == 32) {
-              if (st.live && 16 * h < left) store32B(to, w);
-            } else {
-              if (st.live && 16 * h < left) *reinterpret_cast<uint4 *>(to) = make_uint4(w[0], w[1], w[2], w[3]);
-              if (st.live && 16 * h + 8 < left) *reinterpret_cast<uint4 *>(to + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-            }
-          }
+        } else if (st.live) {
+          states_chunk(add, out32 + c, z);
         }
       };
-      if (!kFew && kLong && kind == kProb) {
+      if (!kFew && ((kLong != kNone && kind == kProb) || (kLong == kTokens && kind == kHeadRows && kept > 0))) {
         int sum[4][32];
-        if (!gather(sum, tl.nkb, slice_blocks<kBf16, kForward, kFew>(tl.nkb), c0, c1)) break;
+        const int slice = kind == kProb ? slice_blocks<kBf16, kForward, kFew>(tl.nkb) : sum_blocks<kBf16>(tl.nkb);
+        if (!gather(sum, tl.nkb, slice, c0, c1)) break;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           if (c0 + 32 * q >= c1) break;
-          float z[32];
+          if (kLong == kTokens && kind == kHeadRows) {
+            head_chunk(c0 + 32 * q, sum[q]);
+          } else {
+            float z[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) z[i] = __int_as_float(sum[q][i]);
-          prob_chunk<kBf16>(st, out16, c0 + 32 * q, z);
+            for (int i = 0; i < 32; ++i) z[i] = __int_as_float(sum[q][i]);
+            prob_chunk<kBf16>(st, out16, c0 + 32 * q, z);
+          }
         }
         continue;
       }
@@ -1598,11 +1624,11 @@ int launch_ce_forward(const Tables *T, const CeArgs &c, const int64_t *labels, i
   g.err = T->err;
   const int64_t tiles = m_tiles * n_tiles;
   if (swap)
-    rc = bf16 ? launch_gemm<ce_gemm_kernel<true, true, true, true>>(g, tiles, s)
-              : launch_gemm<ce_gemm_kernel<false, true, true, true>>(g, tiles, s);
+    rc = bf16 ? launch_gemm<ce_gemm_kernel<true, true, true, kLogits>>(g, tiles, s)
+              : launch_gemm<ce_gemm_kernel<false, true, true, kLogits>>(g, tiles, s);
   else
-    rc = bf16 ? launch_gemm<ce_gemm_kernel<true, true, false, true>>(g, tiles, s)
-              : launch_gemm<ce_gemm_kernel<false, true, false, true>>(g, tiles, s);
+    rc = bf16 ? launch_gemm<ce_gemm_kernel<true, true, false, kLogits>>(g, tiles, s)
+              : launch_gemm<ce_gemm_kernel<false, true, false, kLogits>>(g, tiles, s);
   if (rc != H24_OK) return rc;
 
   CombineArgs cb{};
@@ -1652,6 +1678,8 @@ BackPlan back_plan(const CeArgs &c, bool want_states, bool want_head) {
   if (want_head) work += cdiv(p.piece, kTileM) * n_tiles * cdiv(c.tokens, kTileK);
   if (p.pieces > 1) work += m_tiles * cdiv(p.piece, kTileN) * cdiv(c.in, kTileK);
   int64_t split = want_states ? cdiv(3 * kb * kPairs, work) : 1;
+  const int64_t least = want_states ? cdiv(kb, c.dtype == H24_DTYPE_BF16 ? kSumBf16 : kSumHalf) : 1;  // (12 at most)
+  if (split < least) split = least;
   if (split > kb) split = kb;
   if (split > 32) split = 32;
   p.split = static_cast<int>(split);
@@ -1737,7 +1765,8 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
   const int64_t rows_alloc = c.tokens + kTileK;
   const uint16_t *head_rows = r.scaled ? r.scaled : r.rows;
   const int bn_in = static_cast<int>(c.in >= kTileN ? kTileN : up(c.in, 32));
-  const bool swap = few_tokens(c.tokens), is_long = cdiv(c.in, kTileK) > (bf16 ? kBackBf16 : kBackHalf);
+  const bool swap = few_tokens(c.tokens), long_k = cdiv(c.in, kTileK) > (bf16 ? kBackBf16 : kBackHalf);
+  const bool long_tokens = dw && cdiv(c.tokens, kTileK) > (bf16 ? kSumBf16 : kSumHalf);
   const int bn_few = static_cast<int>(up(c.tokens, 32));
   const int64_t d_rows = swap ? bn_few : rows;  // rows of d that are written
   for (int64_t i = 0; i <= plan.pieces; ++i) {
@@ -1816,12 +1845,18 @@ int launch_ce_backward(const Tables *T, const CeArgs &c, const float *dloss, int
     }
     if (!ok) return fail(H24_ERR_CUDA, "linear_ce_backward: cuTensorMapEncodeTiled failed");
     auto launch = [&](auto few, auto several) {
-      return bf16 ? launch_gemm<ce_gemm_kernel<true, false, decltype(few)::value, decltype(several)::value>>(g, tiles, s)
-                  : launch_gemm<ce_gemm_kernel<false, false, decltype(few)::value, decltype(several)::value>>(g, tiles, s);
+      constexpr bool kFew = decltype(few)::value;
+      constexpr Long kLong = decltype(several)::value;
+      return bf16 ? launch_gemm<ce_gemm_kernel<true, false, kFew, kLong>>(g, tiles, s)
+                  : launch_gemm<ce_gemm_kernel<false, false, kFew, kLong>>(g, tiles, s);
     };
-    constexpr std::true_type yes;
-    constexpr std::false_type no;
-    rc = swap ? (is_long ? launch(yes, yes) : launch(yes, no)) : is_long ? launch(no, yes) : launch(no, no);
+    constexpr std::integral_constant<Long, kNone> none;
+    constexpr std::integral_constant<Long, kLogits> logits;
+    constexpr std::integral_constant<Long, kTokens> both;
+    rc = swap          ? (long_k ? launch(std::true_type(), logits) : launch(std::true_type(), none))
+         : long_tokens ? launch(std::false_type(), both)
+         : long_k      ? launch(std::false_type(), logits)
+                       : launch(std::false_type(), none);
     if (rc != H24_OK) return rc;
   }
   if (dx) {
