@@ -11,6 +11,8 @@ from __future__ import annotations
 import pytest
 import torch
 
+from test_gpu_linear_ce import _check, _inputs
+
 pytestmark = pytest.mark.gpu
 SLICE = {torch.bfloat16: 131072, torch.float16: 32768}
 DTYPES = [torch.bfloat16, torch.float16]
@@ -63,3 +65,14 @@ def test_dx_over_a_large_vocabulary(ce, tokens, vocab, k, dtype):
     (dx,) = torch.autograd.grad(ce(x, w, target, reduction="sum"), x)
     bound = mean * _bound(dtype, vocab) + (2.0 ** -134 if dtype == torch.bfloat16 else 2.0 ** -25)
     assert bool(((dx.double() - mean).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("tokens,vocab,k", [(24577, 8200, 40), (25000, 9001, 24), (40000, 4097, 33)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_several_pieces_of_many_tokens(ce, tokens, vocab, k, reduction, dtype):
+    """From 24,577 tokens on a piece of the vocabulary is 4,096 columns at least, whatever its bytes: two and three of them,
+    the last one short, against the formulas."""
+    x, w, target = _inputs(tokens, vocab, k, dtype, seed=37, masked=0.2)
+    dloss = torch.rand(tokens, device="cuda") * 0.05 if reduction == "none" else None
+    _check(ce, x, w, target, reduction, dloss)
