@@ -18,6 +18,7 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -121,13 +122,18 @@ PyObject *wrap(std::initializer_list<const at::Tensor *> ts) {
   return r;
 }
 
-// A C++ exception (an allocation that fails, say) leaves the call to the general path.
+// A C++ exception (an allocation that fails, say) leaves the call to the general
+// path.  What Python code raised goes on to the caller: a hook on saved tensors may
+// end the call that way (a checkpoint's recomputation does, once it has all it needs).
 template <typename F>
 PyObject *guarded(F f) {
   try {
     return f();
+  } catch (python_error &e) {
+    e.restore();
   } catch (const std::exception &) {
   }
+  if (PyErr_Occurred()) return nullptr;
   Py_RETURN_NONE;
 }
 
