@@ -47,11 +47,14 @@ struct {
 } g_h24;
 
 // The tensor (or parameter, but no other subclass) behind `o` if it is a
-// contiguous CUDA tensor of device `dev`.
+// contiguous CUDA tensor of device `dev` without a tangent of forward-mode
+// derivatives (which nothing here has: the general path says so).
 const at::Tensor *dense(PyObject *o, int dev) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor &t = THPVariable_Unpack(o);
-  return t.is_cuda() && t.get_device() == dev && t.layout() == at::kStrided && t.is_contiguous() ? &t : nullptr;
+  const bool ok = t.is_cuda() && t.get_device() == dev && t.layout() == at::kStrided && t.is_contiguous() &&
+                  !t._fw_grad(0).defined();
+  return ok ? &t : nullptr;
 }
 bool tracked(const at::Tensor *t) { return t && t->requires_grad() && c10::GradMode::is_enabled(); }
 

@@ -22,6 +22,7 @@ import math
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _native as N
 from .castor import _aligned, _call, _stream, _work_device
@@ -64,7 +65,11 @@ class _NoGradient(torch.autograd.Function):
 
 
 def _tracked(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether a derivative is asked of a call with these: a gradient on the way back, or the tangent of a dual tensor
+    (forward mode).  Nothing here has the latter, and an autograd Function says so where a plain call would lose it."""
+    tensors = [t for t in tensors if t is not None]
+    return (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)) or any(
+        unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _vector(t: torch.Tensor, n: int, dtype: torch.dtype | None, dev: torch.device, what: str) -> torch.Tensor:
