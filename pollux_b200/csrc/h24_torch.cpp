@@ -306,16 +306,39 @@ variable_list once(variable_list grads, const char *what) {
   return (*error)(std::move(grads));
 }
 
+// A saved tensor, as the kernels read it.  Hooks may give back another than they
+// were given: its strides are put right, anything else is refused.
+struct Saved {
+  SavedVariable variable;
+  at::ScalarType type = at::kFloat;
+  at::DimVector sizes;
+  at::Device device{at::kCPU};
+
+  void keep(const at::Tensor &t, bool is_output) {
+    variable = SavedVariable(t, is_output);
+    type = t.scalar_type();
+    sizes = t.sizes();
+    device = t.device();
+  }
+  at::Tensor unpack(std::shared_ptr<torch::autograd::Node> owner = nullptr) const {
+    const at::Tensor t = variable.unpack(std::move(owner));
+    if (t.scalar_type() != type || !t.sizes().equals(sizes) || t.device() != device || t.layout() != at::kStrided)
+      throw std::runtime_error("a hook on saved tensors gave back another type, shape or device than it was given");
+    const at::NoGradGuard none;
+    return t.contiguous();
+  }
+};
+
 struct NormNode : torch::autograd::Node {
-  SavedVariable s, weight;
+  Saved s, weight;
   at::Tensor stats;
   bool layer = false, saved_output = false;
 
   std::string name() const override { return layer ? "AddLayerNormBackward" : "AddRmsNormBackward"; }
   void release_variables() override {
     const std::lock_guard<std::mutex> lock(mutex_);
-    s.reset_data();
-    weight.reset_data();
+    s.variable.reset_data();
+    weight.variable.reset_data();
     stats.reset();
   }
 
@@ -390,8 +413,8 @@ PyObject *add_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
       node->set_next_edges(torch::autograd::collect_next_edges(*x, r ? *r : none, *w, b ? *b : none));
       torch::autograd::set_history(y, node);
       if (r) torch::autograd::set_history(sum, node);
-      node->s = SavedVariable(r ? sum : *x, r != nullptr);
-      node->weight = SavedVariable(*w, false);
+      node->s.keep(r ? sum : *x, r != nullptr);
+      node->weight.keep(*w, false);
       node->stats = stats;
       node->layer = layer;
       node->saved_output = r != nullptr;
@@ -401,15 +424,15 @@ PyObject *add_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
 }
 
 struct LossNode : torch::autograd::Node {
-  SavedVariable x, weight;
+  Saved x, weight;
   at::Tensor state;
   int reduction = 0;
 
   std::string name() const override { return "LinearCrossEntropyBackward"; }
   void release_variables() override {
     const std::lock_guard<std::mutex> lock(mutex_);
-    x.reset_data();
-    weight.reset_data();
+    x.variable.reset_data();
+    weight.variable.reset_data();
     state.reset();
   }
 
@@ -463,8 +486,8 @@ PyObject *linear_ce(PyObject *, PyObject *const *a, Py_ssize_t n) {
       const std::shared_ptr<LossNode> node(new LossNode(), torch::autograd::deleteNode);
       node->set_next_edges(torch::autograd::collect_next_edges(*x, *w));
       torch::autograd::set_history(loss, node);
-      node->x = SavedVariable(*x, false);
-      node->weight = SavedVariable(*w, false);
+      node->x.keep(*x, false);
+      node->weight.keep(*w, false);
       node->state = state;
       node->reduction = static_cast<int>(reduction);
     }

@@ -72,6 +72,22 @@ def _tracked(*tensors) -> bool:
         unpack_dual(t).tangent is not None for t in tensors)
 
 
+def _save(ctx, *tensors) -> None:
+    ctx.save_for_backward(*tensors)
+    ctx.kept = [(t.shape, t.dtype, t.device) for t in tensors]
+
+
+def _saved(ctx) -> list:
+    """The tensors of ``_save`` as the kernels read them: rows of matrices and vectors contiguous.  A hook on saved tensors
+    that gives back another type, shape or device than it was given is refused."""
+    out = []
+    for t, kept in zip(ctx.saved_tensors, ctx.kept):
+        if (t.shape, t.dtype, t.device) != kept:
+            raise RuntimeError("a hook on saved tensors gave back another type, shape or device than it was given")
+        out.append(_rows(t, t.device) if t.dim() == 2 else t.contiguous())
+    return out
+
+
 def _vector(t: torch.Tensor, n: int, dtype: torch.dtype | None, dev: torch.device, what: str) -> torch.Tensor:
     if t.numel() != n:
         raise ValueError(f"{what} must hold {n} values, got {tuple(t.shape)}")

@@ -15,7 +15,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _native as N
 from .castor import _call, _stream, _work_device
-from .int8 import _holds_rows, _rows, _tracked
+from .int8 import _holds_rows, _rows, _save, _saved, _tracked
 
 _DTYPES = {torch.float16: N.DTYPE_F16, torch.bfloat16: N.DTYPE_BF16}
 _REDUCTIONS = {"none": N.REDUCE_NONE, "mean": N.REDUCE_MEAN, "sum": N.REDUCE_SUM}
@@ -40,14 +40,14 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, target, ignore_index, reduction):
         loss, state = _forward(x, weight, target, ignore_index, reduction)
-        ctx.save_for_backward(x, weight, state)
+        _save(ctx, x, weight, state)
         ctx.reduction = reduction
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
-        x, weight, state = ctx.saved_tensors
+        x, weight, state = _saved(ctx)
         dev = x.device
         dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if ctx.needs_input_grad[0] else None
         dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if ctx.needs_input_grad[1] else None

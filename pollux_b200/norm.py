@@ -14,7 +14,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _native as N
 from .castor import _call, _stream, _work_device
-from .int8 import _DTYPES, _code, _rows, _tracked
+from .int8 import _DTYPES, _code, _rows, _save, _saved, _tracked
 
 
 def _forward(x, residual, weight, bias, eps: float, layer: bool):
@@ -35,7 +35,7 @@ class _AddNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, bias, eps, layer):
         y, summed, stats = _forward(x, residual, weight, bias, eps, layer)
-        ctx.save_for_backward(x if summed is None else summed, weight, stats)
+        _save(ctx, x if summed is None else summed, weight, stats)
         ctx.layer = layer
         ctx.set_materialize_grads(False)
         return y, summed
@@ -43,7 +43,7 @@ class _AddNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dsummed):
-        s, weight, stats = ctx.saved_tensors
+        s, weight, stats = _saved(ctx)
         need_x, need_r, need_w, need_b = ctx.needs_input_grad[:4]
         rows, cols = s.shape
         dev = s.device

@@ -95,3 +95,42 @@ def test_kept_on_the_host(calls, path, name):
     with torch.autograd.graph.save_on_cpu():
         value = fn(*leaves).float().square().sum()
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(value, leaves), want))
+
+
+def _other_strides(t):
+    """The same values: a matrix by columns, a vector by every second element, another view of the same rows."""
+    if t.dim() == 2:
+        return t.t().contiguous().t()
+    if t.dim() == 1:
+        wide = t.new_zeros(2 * t.numel())
+        wide[::2] = t
+        return wide[::2]
+    return t
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_a_hook_that_gives_other_strides(calls, path, name):
+    fn, leaves = calls[name]
+    want = _grads(fn, leaves)
+    with saved_tensors_hooks(lambda t: t, _other_strides):
+        value = fn(*leaves).float().square().sum()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(value, leaves), want))
+
+
+@pytest.mark.parametrize("name", ["rms", "residual", "layer", "loss"])
+@pytest.mark.parametrize("change", [lambda t: t.float() if t.dtype == BF else t.double(), lambda t: t[..., :-1], lambda t: t.cpu(),
+                                    lambda t: t[None]], ids=["type", "shorter", "device", "shape"])
+def test_a_hook_that_gives_something_else(calls, path, name, change):
+    """What is saved by the call itself comes back changed, and is refused before a kernel sees it."""
+    fn, leaves = calls[name]
+    want = _grads(fn, leaves)
+    inside = []
+
+    def unpack(t):
+        return change(t) if inside else t
+    with saved_tensors_hooks(lambda t: t, unpack):
+        out = fn(*leaves)
+    inside.append(1)
+    with pytest.raises(RuntimeError, match="hook on saved tensors"):
+        torch.autograd.grad(out, leaves, torch.ones_like(out))
+    assert all(torch.equal(a, b) for a, b in zip(_grads(fn, leaves), want))
