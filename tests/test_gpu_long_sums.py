@@ -76,3 +76,38 @@ def test_several_pieces_of_many_tokens(ce, tokens, vocab, k, reduction, dtype):
     x, w, target = _inputs(tokens, vocab, k, dtype, seed=37, masked=0.2)
     dloss = torch.rand(tokens, device="cuda") * 0.05 if reduction == "none" else None
     _check(ce, x, w, target, reduction, dloss)
+
+
+@pytest.mark.parametrize("tokens,vocab,k,dtype", [(33000, 300, 1500, torch.float16), (132000, 260, 4200, torch.bfloat16)])
+def test_long_in_both(ce, tokens, vocab, k, dtype):
+    """Tokens and k longer than a slice, in one kernel."""
+    x, w, target = _inputs(tokens, vocab, k, dtype, seed=41, masked=0.1)
+    _check(ce, x, w, target, "mean", torch.tensor(512.0, device="cuda"))
+
+
+def test_captured_with_factors_in_fp16(ce):
+    """Scratch of the sizes and counts by blocks, new values at each replay."""
+    for tokens, vocab, k in ((60, 300, 72), (700, 900, 113), (17000, 40, 24)):
+        x, w, target = _inputs(tokens, vocab, k, torch.float16, seed=43, masked=0.2)
+        x, w = x.requires_grad_(True), w.requires_grad_(True)
+        dloss = torch.rand(tokens, device="cuda")
+
+        def step():
+            value = ce(x, w, target, reduction="none")
+            return (value, *torch.autograd.grad(value, (x, w), dloss))
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        for seed in range(3):
+            with torch.no_grad():
+                x.normal_()
+                dloss.copy_(2.0 ** (torch.rand(tokens, device="cuda") * 20 - 18 + seed))
+                target.random_(0, vocab)
+                target[seed::4] = -100
+            graph.replay()
+            assert all(torch.equal(a, b) for a, b in zip(out, step()))
