@@ -1218,7 +1218,7 @@ __device__ __forceinline__ uint4 shifted(uint4 x, uint4 y) {
 
 // The head's rows at any pitch and alignment, copied to rows of `pitch`
 // elements on 16 bytes, a warp a row: [50257,1153] 41 us for 232 MB, where the
-// general copy by vectors (repack_rows_kernel), whose shifts differ from thread
+// general copy by vectors of the int8 product, whose shifts differ from thread
 // to thread, took 59.  What stands past a row's end is not read.
 __global__ void __launch_bounds__(kRowThreads) ce_copy_head_kernel(const uint16_t *w, int64_t stride, int64_t rows,
                                                                    int in, uint16_t *out, int64_t pitch) {
@@ -1424,8 +1424,8 @@ __global__ void __launch_bounds__(kRowThreads) ce_states_kernel(const StatesArgs
 // Bytes of d for one piece of the vocabulary, and the columns that it has at
 // least: with many tokens narrow pieces cost more in dx's fp32 sums, which are
 // read and written for each, and leave too few tiles of dW (with 192 MiB alone
-// [131072,1920] x [50688,1920] 108 ms a step, 87 so; [262144,1024] x [4096,1024] 29
-// and 9).
+// [131072,1920] x [50688,1920] took 108 ms a step, 86 so; [262144,1024] x
+// [4096,1024] 29 and 9.0).
 constexpr int64_t kPieceBytes = int64_t(192) << 20, kPieceCols = 4096;
 
 // Map of a matrix of 16-bit elements [rows][cols], row pitch `pitch` elements,

@@ -375,7 +375,8 @@ __device__ __noinline__ void wide_rows(const NormArgs &a, int per_block, float (
     for (int i = kWarp ? threadIdx.x >> 5 : 0; i < per_block && r0 + i < a.rows; i += kWarp ? kWarpRows : 1) again(r0 + i);
 }
 
-template <int DT, bool kAligned, bool kLayer, int kMax, int HOLD>
+// Rows off 16 bytes that do not come through the ring (ring_of_any_rows), by the element.
+template <int DT, bool kLayer, int kMax, int HOLD>
 __global__ void __launch_bounds__(kMax) norm_kernel(const __grid_constant__ NormArgs a) {
   __shared__ float red[2][3][32];
   pdl_enter();
@@ -386,8 +387,8 @@ __global__ void __launch_bounds__(kMax) norm_kernel(const __grid_constant__ Norm
   Held<DT, HOLD> x, res;
   auto ask = [&](int64_t r) {
     if (r >= a.rows) return;
-    x.template load<kAligned>(a.x, r * a.x_stride, t, nt, cols);
-    if (a.residual) res.template load<kAligned>(a.residual, r * a.residual_stride, t, nt, cols);
+    x.template load<false>(a.x, r * a.x_stride, t, nt, cols);
+    if (a.residual) res.template load<false>(a.residual, r * a.residual_stride, t, nt, cols);
   };
   ask(first);
   int turn = 0;
@@ -401,7 +402,7 @@ __global__ void __launch_bounds__(kMax) norm_kernel(const __grid_constant__ Norm
       for (int k = 0; k < P; ++k) v[k] = Pair<DT>::up(Pair<DT>::down(add2(v[k], res.get(k))));
     }
     ask(r + step);
-    if (a.summed) store_held<DT, kAligned>(a.summed, r * a.cols, v, t, nt, cols);
+    if (a.summed) store_held<DT, false>(a.summed, r * a.cols, v, t, nt, cols);
     float mean = 0.f;
     float2 sum = both(0.f), ss = both(0.f);
     if (kLayer) {
@@ -415,19 +416,19 @@ __global__ void __launch_bounds__(kMax) norm_kernel(const __grid_constant__ Norm
     const float var = row_sum<false>(ss.x + ss.y, red[turn][1]) / n_cols;
     const float inv = 1.0f / sqrtf(var + a.eps);
     float2 w[P];
-    load_param<DT, kAligned>(a.gain, a.gain_f32, w, t, nt, cols);
+    load_param<DT, false>(a.gain, a.gain_f32, w, t, nt, cols);
 #pragma unroll
     for (int k = 0; k < P; ++k) v[k] = mul2(v[k], both(inv));
     if (kLayer && a.bias) {
       float2 b[P];
-      load_param<DT, kAligned>(a.bias, a.gain_f32, b, t, nt, cols);
+      load_param<DT, false>(a.bias, a.gain_f32, b, t, nt, cols);
 #pragma unroll
       for (int k = 0; k < P; ++k) v[k] = fma2(v[k], w[k], b[k]);
     } else {
 #pragma unroll
       for (int k = 0; k < P; ++k) v[k] = mul2(v[k], w[k]);
     }
-    store_held<DT, kAligned>(a.y, r * a.cols, v, t, nt, cols);
+    store_held<DT, false>(a.y, r * a.cols, v, t, nt, cols);
     if (t == 0) {
       a.inv[r] = inv;
       if (kLayer) a.mean[r] = mean;
@@ -774,7 +775,7 @@ __device__ __forceinline__ void back_row(const float2 (&n)[P], float2 (&v)[P], c
   }
 }
 
-template <int DT, bool kAligned, bool kLayer, int kMax, int HOLD>
+template <int DT, bool kLayer, int kMax, int HOLD>
 __global__ void __launch_bounds__(kMax) norm_back_kernel(const __grid_constant__ BackArgs a) {
   __shared__ float red[2][2][32];
   pdl_enter();
@@ -787,19 +788,19 @@ __global__ void __launch_bounds__(kMax) norm_back_kernel(const __grid_constant__
   int turn = 0;
   for (int64_t r = first; r < a.rows; r += step, turn ^= 1) {
     Held<DT, HOLD> s, dy, ds;
-    s.template load<kAligned>(a.s, r * a.s_stride, t, nt, cols);
-    dy.template load<kAligned>(a.dy, r * a.dy_stride, t, nt, cols);
-    if (a.dsummed) ds.template load<kAligned>(a.dsummed, r * a.dsummed_stride, t, nt, cols);
+    s.template load<false>(a.s, r * a.s_stride, t, nt, cols);
+    dy.template load<false>(a.dy, r * a.dy_stride, t, nt, cols);
+    if (a.dsummed) ds.template load<false>(a.dsummed, r * a.dsummed_stride, t, nt, cols);
     const RowScale sc = row_scale<kLayer>(a, r);
     float2 n[P], v[P];
-    load_param<DT, kAligned>(a.gain, a.gain_f32, v, t, nt, cols);
+    load_param<DT, false>(a.gain, a.gain_f32, v, t, nt, cols);
     float c1, c2;
     back_sums<DT, kLayer>(s, dy, sc, n, v, dw, db, c1, c2);
     if (a.dx) {
       if (kLayer) row_sums(c1, c2, red[turn]);
       else c1 = row_sum<false>(c1, red[turn][0]);
       back_row<DT>(n, v, ds, a.dsummed != nullptr, sc, c1 * one_over, c2 * one_over);
-      store_held<DT, kAligned>(a.dx, r * a.cols, v, t, nt, cols);
+      store_held<DT, false>(a.dx, r * a.cols, v, t, nt, cols);
     }
   }
   // The sums of this block.
@@ -1082,7 +1083,10 @@ int launch_norm_rows(const NormArgs &a, int threads, cudaStream_t s) {
 bool ring_of_any_rows(int64_t rows, int64_t cols) { return rows >= 1024 && cols > kWarpCols; }
 
 // Stages of a ring and blocks an SM: about 200 KB of rows on their way, in
-// blocks of what the registers of an SM hold, two stages at least.
+// blocks of what the registers of an SM hold, and fewer of them where a block's
+// ring would have less than two stages.  Of the longest rows one SM holds one stage
+// alone (fp32 with three inputs from some 9,300 columns on, with two from some
+// 14,000): the next row is then asked for once this one's sums are there.
 struct RingPlan {
   int threads, stages, smem, grid;
 };
@@ -1143,14 +1147,14 @@ int launch_norm_typed(const Tables *T, const NormArgs &a, cudaStream_t s) {
   if (a.cols <= kFewCols)
     return aligned ? run_norm_ring<norm_ring_kernel<DT, kLayer, kFew, 512, false>, DT, false>(T, a, s)
            : off   ? run_norm_ring<norm_ring_kernel<DT, kLayer, kFew, 512, true>, DT, true>(T, a, s)
-                   : launch_norm_rows<norm_kernel<DT, false, kLayer, 512, kFew>>(a, threads, s);
+                   : launch_norm_rows<norm_kernel<DT, kLayer, 512, kFew>>(a, threads, s);
   if (threads <= 512)
     return aligned ? run_norm_ring<norm_ring_kernel<DT, kLayer, kHold, 512, false>, DT, false>(T, a, s)
            : off   ? run_norm_ring<norm_ring_kernel<DT, kLayer, kHold, 512, true>, DT, true>(T, a, s)
-                   : launch_norm_rows<norm_kernel<DT, false, kLayer, 512, kHold>>(a, threads, s);
+                   : launch_norm_rows<norm_kernel<DT, kLayer, 512, kHold>>(a, threads, s);
   return aligned ? run_norm_ring<norm_ring_kernel<DT, kLayer, kHold, 1024, false>, DT, false>(T, a, s)
          : off   ? run_norm_ring<norm_ring_kernel<DT, kLayer, kHold, 1024, true>, DT, true>(T, a, s)
-                 : launch_norm_rows<norm_kernel<DT, false, kLayer, 1024, kHold>>(a, threads, s);
+                 : launch_norm_rows<norm_kernel<DT, kLayer, 1024, kHold>>(a, threads, s);
 }
 
 // The backward kernel of rows that a block holds: its grid (one wave; asked for
@@ -1196,14 +1200,14 @@ int back_width(const Tables *T, const BackArgs &a, bool aligned, int grid, int *
   if (a.cols <= kFewCols)
     return aligned ? back_ring<norm_back_ring_kernel<DT, kLayer, kFew, 512, false>, DT, false>(T, a, ask, s)
            : off   ? back_ring<norm_back_ring_kernel<DT, kLayer, kFew, 512, true>, DT, true>(T, a, ask, s)
-                   : back_rows<norm_back_kernel<DT, false, kLayer, 512, kFew>>(a, grid, threads, ask, s);
+                   : back_rows<norm_back_kernel<DT, kLayer, 512, kFew>>(a, grid, threads, ask, s);
   if (threads <= 512)
     return aligned ? back_ring<norm_back_ring_kernel<DT, kLayer, kHold, 512, false>, DT, false>(T, a, ask, s)
            : off   ? back_ring<norm_back_ring_kernel<DT, kLayer, kHold, 512, true>, DT, true>(T, a, ask, s)
-                   : back_rows<norm_back_kernel<DT, false, kLayer, 512, kHold>>(a, grid, threads, ask, s);
+                   : back_rows<norm_back_kernel<DT, kLayer, 512, kHold>>(a, grid, threads, ask, s);
   return aligned ? back_ring<norm_back_ring_kernel<DT, kLayer, kHold, 1024, false>, DT, false>(T, a, ask, s)
          : off   ? back_ring<norm_back_ring_kernel<DT, kLayer, kHold, 1024, true>, DT, true>(T, a, ask, s)
-                 : back_rows<norm_back_kernel<DT, false, kLayer, 1024, kHold>>(a, grid, threads, ask, s);
+                 : back_rows<norm_back_kernel<DT, kLayer, 1024, kHold>>(a, grid, threads, ask, s);
 }
 
 template <int DT, bool kLayer>

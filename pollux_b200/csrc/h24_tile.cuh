@@ -1,6 +1,6 @@
 // h24_tile.cuh -- what the tcgen05 kernels over TMA-filled tiles share: bounded
-// barrier waits, tile loads, commits, TMEM reads, tensor maps and the copy of
-// rows that TMA cannot read as they lie.
+// barrier waits, tile loads, commits, TMEM reads, tensor maps and loads of 16
+// bytes from any alignment.
 #pragma once
 
 #include <cuda.h>  // CUtensorMap and its enums; the entry point is looked up at run time
@@ -129,33 +129,6 @@ __device__ __forceinline__ uint4 load16_any(const int8_t *p, int valid, const in
   const uint32_t off = offset16(p);
   return join16(load16_within(p - off, lo, hi), off ? load16_within(p - off + 16, lo, hi) : make_uint4(0, 0, 0, 0), off,
                 valid);
-}
-
-// Rows of a byte matrix at any pitch and alignment, copied to rows of `pitch`
-// bytes (a multiple of 16), zeros past their end: what TMA can read.  Where a
-// layer or its input is not 16-byte aligned, the copy and the tiles over it
-// (2 more bytes of traffic a byte) take [4096,1919] x [7680,1919] from 1,106 us
-// with tiles filled by hand to 57, and [20,1921] x [7680,1921] from 61 to 14.
-struct RepackArgs {
-  const int8_t *src;
-  int64_t stride;
-  int8_t *dst;
-  int64_t rows;
-};
-constexpr int kRepackThreads = 256;
-static __global__ void __launch_bounds__(kRepackThreads) repack_rows_kernel(const RepackArgs a0, const RepackArgs a1, int cols,
-                                                                     int chunks) {
-  pdl_enter();
-  const int64_t total0 = a0.rows * chunks, total = total0 + a1.rows * chunks;
-  for (int64_t i = blockIdx.x * static_cast<int64_t>(kRepackThreads) + threadIdx.x; i < total;
-       i += static_cast<int64_t>(gridDim.x) * kRepackThreads) {
-    const RepackArgs &a = i < total0 ? a0 : a1;
-    const int64_t at = i < total0 ? i : i - total0;
-    const int64_t r = at <= 0xFFFFFFFFll ? static_cast<uint32_t>(at) / static_cast<uint32_t>(chunks) : at / chunks;
-    const int c = static_cast<int>(at - r * chunks) * 16;
-    const int8_t *hi = a.src + (a.rows - 1) * a.stride + cols;
-    reinterpret_cast<uint4 *>(a.dst)[at] = load16_any(a.src + r * a.stride + c, cols - c, a.src, hi);
-  }
 }
 
 // 16 TMEM columns of this warp's 32 lanes.
