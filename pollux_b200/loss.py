@@ -85,8 +85,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
                          f"{tuple(weight.shape)}")
     if torch.is_autocast_enabled("cuda"):
         low = torch.get_autocast_dtype("cuda")
-        if x.is_floating_point() and weight.is_floating_point():
-            x, weight = x.to(low), weight.to(low)
+        # (float64 is not cast by autocast: it is refused below, as without.)
+        x, weight = (a.to(low) if a.is_floating_point() and a.dtype != torch.float64 else a for a in (x, weight))
     if x.dtype not in _DTYPES or weight.dtype != x.dtype:
         raise TypeError(f"x and weight must both be float16 or both bfloat16, got {x.dtype} and {weight.dtype}")
     vocab, in_f = weight.shape
