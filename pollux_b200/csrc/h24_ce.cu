@@ -1162,7 +1162,8 @@ __global__ void __launch_bounds__(kRowThreads) ce_back_rows_kernel(const BackRow
       held *= f.m;
       a.log_factor[place] = log2f(held);
       a.power[r] = ldexpf(f.sign, f.power - prob_power);
-      powers[t] = f.real ? ldexpf(f.sign, f.power - unit) : f.sign;
+      // (At most 2^39 where a state is not 0; one of zeros stays 0.)
+      powers[t] = f.real ? ldexpf(f.sign, min(f.power - unit, 64)) : f.sign;
     }
     a.target[place] = target;
     // (With an infinite factor the row is no number: NaN at the target, so that dW is loud.)

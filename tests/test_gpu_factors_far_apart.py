@@ -95,3 +95,18 @@ def test_sizes_at_the_ends_of_the_types(ce, tokens):
         else:
             assert not bool(dx.isnan().any()) and not bool(dw.isnan().any())
             assert bool((dw[bw.abs() > 2.0 ** -13].isinf()).all())
+
+
+@pytest.mark.parametrize("tokens", [40, 300])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_a_state_of_zeros_with_a_large_factor(ce, tokens, dtype):
+    """It adds nothing to dW, however far its factor lies above the others'."""
+    x, w, target = _inputs(tokens, 90, 48, dtype, seed=47)
+    x[3] = 0
+    dloss = torch.full((tokens,), 2.0 ** -70, device="cuda")
+    dloss[3] = 2.0 ** 120
+    xs, ws = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    dw = torch.autograd.grad(ce(xs, ws, target, reduction="none"), ws, dloss)[0]
+    assert bool(torch.isfinite(dw).all())
+    if dtype == torch.float16:
+        assert not bool(dw.any())
